@@ -33,6 +33,18 @@ ts_tensor *ts_tensor_zeros(const size_t *dims, size_t rank);
 ts_tensor *ts_tensor_ones(const size_t *dims, size_t rank);
 /* Tensor::from_slice (init/data.rs:227-247) */
 ts_tensor *ts_tensor_from_slice(const float *data, size_t len, const size_t *dims, size_t rank);
+/* A tensor over the caller's device memory (row-major f32, not copied; no
+ * counterpart in the reference).  `release` (may be NULL) is called with ctx,
+ * from whichever thread lets the last user go, once every handle, saved
+ * operand and step graph that uses the memory is gone and the work queued by
+ * then has run; also at once when this call fails or the tensor is empty.
+ * Work on other streams that writes the memory must have finished before the
+ * library reads it, and the library's work before others read what it wrote
+ * (ts_synchronize, or an event on ts_stream).  Memory that is not device
+ * memory of one allocation is refused. */
+ts_tensor *ts_tensor_from_device(float *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx);
+/* The process is ending: from here on no release call is made. */
+void ts_external_detach(void);
 /* Tensor::randn(dims, seed) / fill_randn (init/random.rs:231-299): values of
  * the reference's XorShiftRng + Box-Muller, generated on the device.  With
  * has_seed == 0 the seed comes from the clock, as XorShiftRng::new_from_time
@@ -84,6 +96,43 @@ ts_tensor *ts_tensor_softmax(const ts_tensor *a, size_t dim);
 ts_tensor *ts_tensor_sum_dims(const ts_tensor *a, const size_t *dims, size_t ndims, int keepdim);
 ts_tensor *ts_tensor_mean_dims(const ts_tensor *a, const size_t *dims, size_t ndims, int keepdim);
 
+/* ---- a feed-forward block's operators (no counterpart in the reference) --------
+ * Root-mean-square norm over the last axis, h / sqrt(mean(h^2) + eps) * weight:
+ * of x, or of h = x + residual (same shape), which *h_out receives (recorded as
+ * add_tensor's sum).  Gradients go to x, residual and weight. */
+ts_tensor *ts_tensor_rms_norm(const ts_tensor *x, const ts_tensor *weight, float eps);
+ts_tensor *ts_tensor_add_rms_norm(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight, float eps,
+                                  ts_tensor **h_out);
+/* The layer act(x weight + bias) + residual as one op: x [..., fan_in], weight
+ * [fan_in, fan_out], bias [fan_out] and residual [..., fan_out] may be NULL;
+ * activation one of TS_HIP_ACT_* (ts_hip.h).  For the backward pass it keeps
+ * its input, and with an activation the values before it (checkpoint 0), or the
+ * input's values in 8 bits alone (checkpoint 1): the backward pass then computes
+ * the layer again from them where it needs the activation's slope, and the
+ * weight's gradient from them. */
+ts_tensor *ts_tensor_linear(const ts_tensor *x, const ts_tensor *weight, const ts_tensor *bias, int activation,
+                            const ts_tensor *residual, int checkpoint);
+/* Matrices in 8 bits (layout and rounding: ts_hip_pack8).  No gradient passes
+ * through them.  residual of the norm: NULL, or h goes to *h_out. */
+typedef struct ts_packed8 ts_packed8;
+ts_packed8 *ts_tensor_pack8(const ts_tensor *x);
+ts_packed8 *ts_tensor_rms_norm_packed(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight, float eps,
+                                      ts_tensor **h_out);
+/* the caller's codes [rows, pitch] (16-byte aligned) and scales [pitch / 128,
+ * rows, 4] on the device, as ts_tensor_from_device */
+ts_packed8 *ts_packed8_from_device(uint8_t *codes, uint8_t *scales, size_t rows, size_t cols, void (*release)(void *),
+                                   void *ctx);
+void ts_packed8_free(ts_packed8 *p);
+size_t ts_packed8_rows(const ts_packed8 *p);
+size_t ts_packed8_cols(const ts_packed8 *p);
+size_t ts_packed8_pitch(const ts_packed8 *p);
+const uint8_t *ts_packed8_codes_ptr(const ts_packed8 *p);
+const uint8_t *ts_packed8_scales_ptr(const ts_packed8 *p);
+ts_tensor *ts_packed8_unpack(const ts_packed8 *p);
+/* act(x weight^T + bias) + residual, x [batch, fan_in] and weight [fan_out, fan_in] */
+ts_tensor *ts_packed8_linear(const ts_packed8 *x, const ts_packed8 *weight, const ts_tensor *bias, int activation,
+                             const ts_tensor *residual);
+
 /* transpose(dim0, dim1) / t() (transform/transpose.rs:156-208, :283-291): a
  * transposed view, recorded (Transpose GradFn, grad_fn/mod.rs:243-249, :575)
  * whenever the input requires grad.  The view's values are copied only when
@@ -110,6 +159,9 @@ int ts_tensor_backward(ts_tensor *t, const ts_tensor *grad_output);
  * with ts_last_error() "" when there is none -- also when only the graph's
  * gradient map holds one, as in the reference. */
 ts_tensor *ts_tensor_grad(const ts_tensor *t);
+/* The gradient that grad_by_value copies, as a handle on its buffer (free the
+ * handle, the gradient stays); NULL as there.  No counterpart in the reference. */
+ts_tensor *ts_tensor_grad_view(const ts_tensor *t);
 /* grad_by_value (utils.rs:525-534): a copy, or NULL with ts_last_error() ""
  * when there is no gradient */
 ts_tensor *ts_tensor_grad_by_value(const ts_tensor *t);

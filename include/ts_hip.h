@@ -112,6 +112,8 @@ int ts_hip_graph_launch(void *graph_exec, void *stream);
 int ts_hip_graph_destroy(void *graph_exec);
 /* message for a status returned by any ts_hip_* call */
 const char *ts_hip_error_string(int status);
+/* TS_HIP_OK when [ptr, ptr + bytes) is device memory of one allocation, else TS_HIP_EINVAL */
+int ts_hip_check_device_range(const void *ptr, size_t bytes);
 /* free / total device memory in bytes */
 int ts_hip_mem_info(size_t *free_bytes, size_t *total_bytes);
 
@@ -582,6 +584,79 @@ int ts_hip_dot(const float *a, const float *b, size_t n, float *out, float *work
                void *stream);
 /* out[i][j] = a[i] * b[j] (grad_fn/ops/matmul.rs compute_outer_product, fp32) */
 int ts_hip_outer(const float *a, size_t m, const float *b, size_t n, float *out, void *stream);
+
+/* ---- a feed-forward block's operators (no counterpart in the reference) ----------
+ *
+ * Values in 8 bits.  A matrix [rows, cols] is held as e4m3 codes with one
+ * power-of-two scale per 32 columns of a row.  A row is padded with zeros to
+ * pitch = ts_hip_packed_pitch(cols) columns (a multiple of 128):
+ *   codes  [rows][pitch] bytes
+ *   scales [pitch / 128][rows][4] bytes: the scale of columns 128 g + 32 b ..
+ *          of row r is 2^(byte - 127), byte at (g * rows + r) * 4 + b
+ * A block's exponent is the smallest in -117 .. 119 that keeps its largest
+ * magnitude within 448 times its scale; each value is rounded to the nearest
+ * code (ties to even), so it is off by at most 2^-4 of itself or 2^-10 of the
+ * scale, whichever is more.  A NaN gets a NaN code (of either sign) and is left out
+ * of its block's largest; magnitudes past 448 2^119 (infinities) become 448 2^119.
+ * Every value that codes stand for is a normal fp32 (and bf16) number or zero.
+ * codes are 16-byte aligned, scales 4-byte aligned. */
+size_t ts_hip_packed_pitch(size_t cols);
+int ts_hip_pack8(const float *x, size_t rows, size_t cols, uint8_t *codes, uint8_t *scales, void *stream);
+/* out [rows, cols]: the values that the codes stand for */
+int ts_hip_unpack8(const uint8_t *codes, const uint8_t *scales, size_t rows, size_t cols, float *out, void *stream);
+
+/* Root-mean-square norm over the rows of [rows, cols], with the residual's
+ * addition: h = x + residual (fp32; residual NULL: h = x and the argument h is
+ * NULL too), y = h / sqrt(mean(h^2) + eps) * weight.  The mean is taken in f64.
+ * h may be x or residual. */
+int ts_hip_rms_norm(const float *x, const float *residual, const float *weight, size_t rows, size_t cols, float eps,
+                    float *h, float *y, void *stream);
+/* The same with y in 8 bits (as ts_hip_pack8 of y, y taken before its rounding to fp32). */
+int ts_hip_rms_norm_packed(const float *x, const float *residual, const float *weight, size_t rows, size_t cols,
+                           float eps, float *h, uint8_t *codes, uint8_t *scales, void *stream);
+/* The gradients of y = h r weight, r = 1 / sqrt(mean(h^2) + eps), from go = dy:
+ *   dh = r (go weight) - h r^3 mean(go weight h),  dweight = sum over rows of go h r
+ * Either may be NULL.  The workspace is needed for dweight.  A pass adds in a
+ * fixed order, so equal calls give equal bits. */
+size_t ts_hip_rms_norm_backward_workspace_floats(size_t rows, size_t cols);
+int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
+                             float *dh, float *dweight, float *workspace, size_t workspace_floats, void *stream);
+
+/* Activations of a layer: none, max(z, 0), z s(z) with s(v) = 1 / (1 + e^-v), and
+ * z s(2 sqrt(2 / pi) (z + 0.044715 z^3)) (the tanh form of gelu). */
+enum { TS_HIP_ACT_NONE = 0, TS_HIP_ACT_RELU = 1, TS_HIP_ACT_SILU = 2, TS_HIP_ACT_GELU_TANH = 3 };
+
+/* y [batch, fan_out] = act(x W^T + bias) + residual with x [batch, fan_in] and
+ * W [fan_out, fan_in] in 8 bits; bias (fan_out) and residual (laid out as y)
+ * may be NULL.  The products of the codes are exact and summed in fp32. */
+size_t ts_hip_linear_packed_workspace_floats(size_t batch, size_t fan_in, size_t fan_out);
+int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const uint8_t *w_codes,
+                         const uint8_t *w_scales, size_t batch, size_t fan_in, size_t fan_out, const float *bias,
+                         int act, const float *residual, float *y, float *workspace, size_t workspace_floats,
+                         void *stream);
+
+/* A layer's forward: z = x W + bias, y = act(z) + residual, x [batch, fan_in],
+ * W [fan_in, fan_out]; bias and residual may be NULL.  z != NULL: z is stored
+ * there as well (what the backward pass reads).  codes != NULL: x is also
+ * packed into codes / scales (ts_hip_pack8). */
+typedef struct ts_hip_linear_shape {
+    size_t batch, fan_in, fan_out;
+} ts_hip_linear_shape;
+size_t ts_hip_linear_workspace_floats(const ts_hip_linear_shape *shape);
+int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float *weight, const float *bias, int act,
+                  const float *residual, float *y, float *z, uint8_t *codes, uint8_t *scales, float *workspace,
+                  size_t workspace_floats, void *stream);
+/* The layer's gradients from go = dy:
+ *   dz = go act'(z),  dx = dz W^T,  dweight = X^T dz,  dbias = dz's column sums
+ * each of dx, dweight and dbias NULL where it is not wanted.  X is x, or what
+ * codes / scales hold where codes != NULL (x is then not read); z is the
+ * forward's (needed with x and an activation), or NULL: with codes it is
+ * computed again from what they hold, z = X W + bias.  relu's slope at 0 is 0. */
+size_t ts_hip_linear_backward_workspace_floats(const ts_hip_linear_shape *shape);
+int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, const uint8_t *codes,
+                           const uint8_t *scales, const float *weight, const float *bias, int act, const float *z,
+                           const float *go, float *dx, float *dweight, float *dbias, float *workspace,
+                           size_t workspace_floats, void *stream);
 
 /* ---- optimizer ------------------------------------------------------------------ */
 

@@ -1,0 +1,507 @@
+"""A feed-forward block's operators on the device against their plain forms in
+64 bits (feedforward_ref.py, which derives the tolerances)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import feedforward_ref as R
+from conftest import normal
+from gpu_util import Dev, T, hip, hip_check, sync
+
+pytestmark = pytest.mark.gpu
+
+
+class DeviceArray:
+    """A device buffer as other libraries expose theirs."""
+
+    def __init__(self, a):
+        self.host = np.ascontiguousarray(a)
+        words = np.zeros(max((self.host.nbytes + 3) // 4, 1), np.float32)
+        words.view(np.uint8)[: self.host.nbytes] = self.host.reshape(-1).view(np.uint8)
+        self.dev = Dev.of(words)
+        kind = "<f4" if self.host.dtype == np.float32 else "|u1"
+        self.__cuda_array_interface__ = dict(shape=self.host.shape, typestr=kind, data=(self.dev.ptr, False), version=2)
+
+    def get(self):
+        return self.dev.get().view(np.uint8)[: self.host.nbytes].view(self.host.dtype).reshape(self.host.shape)
+
+
+def tensor(a):
+    return T.Tensor.from_slice(np.ascontiguousarray(a, np.float32), a.shape)
+
+
+def packed(a):
+    """A Packed8 of the plain form's codes."""
+    codes, scales = R.pack8(a)
+    return T.Packed8.from_device(DeviceArray(codes), DeviceArray(scales), a.shape[1])
+
+
+def parts(p):
+    """codes and scales of a Packed8, on the host."""
+    T.synchronize()
+    rows, pitch = p.shape[0], p.pitch
+    codes, scales = np.empty((rows, pitch), np.uint8), np.empty((pitch // 128, rows, 4), np.uint8)
+    hip_check(hip.ts_hip_memcpy_bytes(codes.ctypes.data, p.codes_ptr(), codes.nbytes, 1, None), "codes")
+    hip_check(hip.ts_hip_memcpy_bytes(scales.ctypes.data, p.scales_ptr(), scales.nbytes, 1, None), "scales")
+    sync()
+    return codes, scales
+
+
+def assert_within(got, want, bound, what):
+    got = np.asarray(got, np.float64)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    off = np.abs(got - want) / bound
+    assert np.all(off <= 1), f"{what}: {np.nanmax(off):.3g} of its bound at {np.unravel_index(np.nanargmax(off), off.shape)}"
+
+
+# ---- values in 8 bits ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 31), (3, 32), (2, 33), (5, 127), (4, 128), (3, 129), (70, 1003), (1, 5000)])
+def test_pack8(rows, cols):
+    rng = np.random.default_rng(rows * cols)
+    x = (rng.standard_normal((rows, cols)) * 10.0 ** rng.integers(-38, 37, (rows, 1))).astype(np.float32)
+    x[rng.random((rows, cols)) < 0.1] = 0.0
+    p = tensor(x).pack8()
+    assert p.shape == (rows, cols) and p.pitch == R.pitch_of(cols)
+    codes, scales = parts(p)
+    want = R.pack8(x)
+    assert np.array_equal(codes, want[0]) and np.array_equal(scales, want[1])
+    assert np.array_equal(p.unpack().data(), R.unpack8(*want, cols).astype(np.float32))
+
+
+def test_pack8_borders():
+    """Every code, every border between two, their neighbours, at the smallest, middle and largest scales."""
+    v = R.e4m3_values()[:127]
+    mid = (v[1:] + v[:-1]) / 2
+    base = np.r_[v, mid, -v, -mid].astype(np.float32)
+    line = np.r_[base, np.nextafter(base, np.float32(np.inf)), np.nextafter(base, np.float32(-np.inf))]
+    line = np.clip(line, -448, 448)
+    line = np.resize(line, -(-line.size // 31) * 31).reshape(-1, 31)
+    blocks = np.concatenate([line, np.full((line.shape[0], 1), 448.0)], 1).reshape(1, -1)
+    x = np.concatenate([blocks * 2.0 ** k for k in (-117, -60, 0, 60, 119)]).astype(np.float32)
+    codes, scales = parts(tensor(x).pack8())
+    want = R.pack8(x)
+    assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
+
+
+def test_pack8_what_no_code_holds():
+    x = np.zeros((4, 64), np.float32)
+    x[0, :3] = [np.inf, -np.inf, 1.0]
+    x[1, :3] = [np.nan, 2.0, -np.nan]
+    x[2, :2] = np.finfo(np.float32).max, -np.finfo(np.float32).max
+    x[3, :3] = [1e-45, 2.0 ** -127, 2.0 ** -126]
+    codes, scales = parts(tensor(x).pack8())
+    want = R.pack8(x)
+    assert np.array_equal(scales, want[1])
+    nan = (want[0] & 127) == 127  # either of the two NaN codes
+    assert nan.sum() == 2 and np.all((codes[nan] & 127) == 127) and np.array_equal(codes[~nan], want[0][~nan])
+    assert scales[0, 0, 0] == 246 and codes[0, 0] == 0x7e and codes[0, 1] == 0xfe
+
+
+# ---- norm -----------------------------------------------------------------------------
+
+NORMS = [(1, 1), (1, 4096), (3, 7), (5, 256), (6, 257), (9, 512), (4, 1003), (130, 784), (7, 1025), (3, 2048), (2, 4095),
+         (5, 4097), (2, 8192), (3, 8193), (2, 16384), (3, 16385), (2, 40001), (700, 64)]
+
+
+def norm_case(rows, cols, residual, eps=1e-6):
+    x, r = normal((rows, cols), 1), normal((rows, cols), 2) * 3 if residual else None
+    w = (1 + 0.2 * normal((cols,), 3)).astype(np.float32)
+    h = x if r is None else (x + r).astype(np.float32)
+    return x, r, w, h
+
+
+@pytest.mark.parametrize("rows,cols", NORMS)
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm(rows, cols, residual):
+    x, r, w, h = norm_case(rows, cols, residual)
+    go = normal((rows, cols), 4)
+    X, W = tensor(x).with_requires_grad(), tensor(w).with_requires_grad()
+    Rs = tensor(r).with_requires_grad() if residual else None
+    if residual:
+        y, stream = X.add_rms_norm(Rs, W, 1e-6)
+        assert np.array_equal(stream.data(), h)
+    else:
+        y = X.rms_norm(W, 1e-6)
+    want = R.rms_norm(h, w, 1e-6)
+    assert_within(y.data(), want, 4 * R.U * np.abs(want) + 1e-40, "y")
+    y.backward(tensor(go))
+    dh, dw = R.rms_norm_grads(h, w, go, 1e-6)
+    s = 1 / np.sqrt((h.astype(np.float64) ** 2).mean(1, keepdims=True) + 1e-6)
+    g = np.abs(go.astype(np.float64) * w)
+    back = np.abs(h) * s ** 3 * np.abs((go.astype(np.float64) * w * h).mean(1, keepdims=True))
+    assert_within(X.grad_by_value().data(), dh, 4 * R.U * (s * g + back) + 1e-40, "dx")
+    if residual:
+        assert np.array_equal(Rs.grad_by_value().data(), X.grad_by_value().data())
+    # a rounding each of r and h r, one of each part (the long rows': one a row) and one at the end
+    steps = 5 + (rows if cols > 16384 else 0)
+    assert_within(W.grad_by_value().data(), dw, steps * R.U * np.abs(go * h * s).sum(0) + 1e-40, "dweight")
+    T.clear_gradients()
+
+
+@pytest.mark.parametrize("rows,cols", NORMS)
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm_packed(rows, cols, residual):
+    x, r, w, h = norm_case(rows, cols, residual)
+    if residual:
+        p, stream = tensor(x).add_rms_norm_packed(tensor(r), tensor(w), 1e-6)
+        assert np.array_equal(stream.data(), h)
+    else:
+        p = tensor(x).rms_norm_packed(tensor(w), 1e-6)
+    codes, scales = parts(p)
+    want = R.pack8(R.rms_norm(h, w, 1e-6))
+    assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
+
+
+def test_norm_of_zero_and_tiny_and_huge_rows():
+    x = np.zeros((4, 40), np.float32)
+    x[1], x[2], x[3, 5] = 1e-30, 1e30, np.nan
+    w = np.ones(40, np.float32)
+    y = tensor(x).rms_norm(tensor(w), 1e-6).data()
+    assert not y[0].any() and np.isnan(y[3]).all()
+    assert_within(y[1:3], R.rms_norm(x[1:3].astype(np.float64), w, 1e-6), np.abs(y[1:3]) * 4 * R.U + 1e-44, "y")
+    z = tensor(x[:1]).rms_norm(tensor(w), 0.0).data()  # 0 / 0
+    assert np.isnan(z).all()
+
+
+def test_norm_gradients_accumulate_and_pass_through_the_sum():
+    x, r, w, h = norm_case(6, 96, True)
+    X, Rs, W = (tensor(a).with_requires_grad() for a in (x, r, w))
+    y, stream = X.add_rms_norm(Rs, W, 1e-6)
+    loss = y.mul_tensor(y).add_tensor(stream).sum()
+    loss.backward()
+    yv = R.rms_norm(h, w, 1e-6)
+    dh, dw = R.rms_norm_grads(h, w, 2 * yv, 1e-6)
+    assert np.allclose(X.grad_by_value().data(), dh + 1, rtol=1e-5, atol=1e-5)
+    assert np.allclose(Rs.grad_by_value().data(), dh + 1, rtol=1e-5, atol=1e-5)
+    assert np.allclose(W.grad_by_value().data(), dw, rtol=1e-5, atol=1e-4)
+    T.clear_gradients()
+
+
+def test_norm_of_more_axes_and_of_nothing():
+    x, w = normal((2, 3, 5), 1), normal((5,), 2)
+    X = tensor(x).with_requires_grad()
+    y = X.rms_norm(tensor(w))
+    assert y.shape == (2, 3, 5)
+    want = R.rms_norm(x.reshape(6, 5), w, 1e-6).reshape(2, 3, 5)
+    assert_within(y.data(), want, 4 * R.U * np.abs(want) + 1e-40, "y")
+    y.backward(tensor(np.ones((2, 3, 5), np.float32)))
+    assert X.grad_by_value().shape == (2, 3, 5)
+    E, W = T.Tensor.zeros((0, 5)).with_requires_grad(), tensor(w).with_requires_grad()
+    y = E.rms_norm(W)
+    assert y.shape == (0, 5)
+    y.backward(T.Tensor.zeros((0, 5)))
+    assert not W.grad_by_value().data().any()
+    T.clear_gradients()
+
+
+# ---- layers ---------------------------------------------------------------------------
+
+LAYERS = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (16, 32, 128), (33, 65, 31), (64, 784, 10), (128, 129, 130), (2, 1000, 3),
+          (257, 40, 300), (1, 513, 65), (300, 17, 33)]
+
+
+def layer_case(m, k, n, bias, residual, seed=0):
+    x, w = normal((m, k), seed + 1), normal((k, n), seed + 2, k ** -0.5)
+    b = normal((n,), seed + 3, 0.1) if bias else None
+    r = normal((m, n), seed + 4) if residual else None
+    return x, w, b, r, normal((m, n), seed + 5, 1 / m)
+
+
+def check_layer(m, k, n, name, bias, residual, checkpoint, seed=0):
+    x, w, b, r, go = layer_case(m, k, n, bias, residual, seed)
+    X, W = tensor(x).with_requires_grad(), tensor(w).with_requires_grad()
+    B = tensor(b).with_requires_grad() if bias else None
+    Rs = tensor(r).with_requires_grad() if residual else None
+    y = X.linear(W, bias=B, activation=name, residual=Rs, checkpoint=checkpoint)
+    want, z = R.linear(x, w, b, name, r)
+    assert_within(y.data(), want, R.linear_bound(x, w, b, name, r, z), "y")
+    y.backward(tensor(go))
+    kept = x if checkpoint == "full" else R.unpack8(*R.pack8(x), k)
+    z = R.linear(kept, w, b, "none", None)[0]
+    dx, dw, db = R.linear_grads(kept, w, z, name, go)
+    ex, ew, eb = R.linear_grads_bound(kept, w, b, z, name, go)
+    if name == "relu":  # an input within rounding of zero takes either slope: its whole gradient
+        turn = np.abs(go) * ~R.relu_safe(x, w, b, kept)
+        ex, ew, eb = ex + turn @ np.abs(w).T, ew + np.abs(kept).T @ turn, eb + turn.sum(0)
+    assert_within(X.grad_by_value().data(), dx, ex, "dx")
+    assert_within(W.grad_by_value().data(), dw, ew, "dweight")
+    if bias:
+        assert_within(B.grad_by_value().data(), db, eb, "dbias")
+    if residual:
+        assert np.array_equal(Rs.grad_by_value().data(), go)
+    T.clear_gradients()
+
+
+@pytest.mark.parametrize("m,k,n", LAYERS)
+@pytest.mark.parametrize("checkpoint", ["full", "8bit"])
+@pytest.mark.parametrize("name,bias,residual", [("none", False, False), ("relu", True, False), ("silu", True, True),
+                                                ("gelu_tanh", False, True)])
+def test_linear(m, k, n, name, bias, residual, checkpoint):
+    check_layer(m, k, n, name, bias, residual, checkpoint)
+
+
+@pytest.mark.parametrize("checkpoint", ["full", "8bit"])
+def test_linear_gradient_is_the_difference(checkpoint):
+    """Along a random direction of every input, by the device's own forward values."""
+    m, k, n, t = 24, 40, 33, 2.0 ** -7
+    x, w, b, r, _ = layer_case(m, k, n, True, True)
+    x = R.unpack8(*R.pack8(x), k).astype(np.float32)  # its checkpoint is itself
+    go = normal((m, n), 9)
+    leaves = [tensor(a).with_requires_grad() for a in (x, w, b, r)]
+    X, W, B, Rs = leaves
+    X.linear(W, bias=B, activation="gelu_tanh", residual=Rs, checkpoint=checkpoint).backward(tensor(go))
+    for at, (a, leaf) in enumerate(zip((x, w, b, r), leaves)):
+        d = normal(a.shape, 20 + at)
+        ends = []
+        for s in (-t, t):
+            args = [x, w, b, r]
+            args[at] = (a + np.float32(s) * d).astype(np.float32)
+            A = [tensor(v) for v in args]
+            ends.append(A[0].linear(A[1], bias=A[2], activation="gelu_tanh", residual=A[3]).data().astype(np.float64))
+        diff = ((ends[1] - ends[0]) * go).sum() / (2 * t)
+        slope = (leaf.grad_by_value().data().astype(np.float64) * d).sum()
+        # rounding of the values over the step, and t^2 of a third derivative of order 1 of each output
+        scale = np.abs(go).sum()
+        assert abs(diff - slope) <= scale * (16 * R.U * 8 / t) + np.abs(go).sum() * t * t * 2 * np.abs(d).max() ** 3, at
+    T.clear_gradients()
+
+
+def test_linear_grads_for_some_inputs_only():
+    x, w, b, r, go = layer_case(12, 20, 9, True, True)
+    for need in range(16):
+        ts = [tensor(a) for a in (x, w, b, r)]
+        for i, t in enumerate(ts):
+            if need >> i & 1:
+                t.with_requires_grad()
+        y = ts[0].linear(ts[1], bias=ts[2], activation="silu", residual=ts[3], checkpoint="8bit" if need & 2 else "full")
+        assert y.requires_grad() == bool(need)
+        if need:
+            y.backward(tensor(go))
+        for i, t in enumerate(ts):
+            g = t.grad_by_value()
+            assert (g is not None) == bool(need >> i & 1), (need, i)
+        T.clear_gradients()
+    with T.NoGradTrack():
+        assert not tensor(x).with_requires_grad().linear(tensor(w)).requires_grad()
+
+
+@pytest.mark.parametrize("shape", [(0, 5, 3), (4, 0, 3), (4, 5, 0)])
+@pytest.mark.parametrize("checkpoint", ["full", "8bit"])
+def test_linear_of_nothing(shape, checkpoint):
+    m, k, n = shape
+    X, W = T.Tensor.zeros((m, k)).with_requires_grad(), T.Tensor.zeros((k, n)).with_requires_grad()
+    b = normal((n,), 1)
+    B = tensor(b).with_requires_grad()
+    y = X.linear(W, bias=B, activation="silu", checkpoint=checkpoint)
+    assert y.shape == (m, n)
+    want = np.tile(R.act(b.astype(np.float64), "silu"), (m, 1))
+    assert_within(y.data(), want, 20 * R.U * np.abs(want) + 1e-40, "y")
+    y.backward(T.Tensor.ones((m, n)))
+    assert W.grad_by_value().shape == (k, n) and not W.grad_by_value().data().any()
+    want = m * R.act_slope(b.astype(np.float64), "silu")
+    assert_within(B.grad_by_value().data(), want, 40 * R.U * np.abs(want) + 1e-40, "dbias")
+    if m * k:
+        assert not X.grad_by_value().data().any()
+    T.clear_gradients()
+
+
+def test_linear_of_more_axes():
+    x, w = normal((2, 3, 5), 1), normal((5, 4), 2)
+    X = tensor(x).with_requires_grad()
+    y = X.linear(tensor(w), activation="relu")
+    assert y.shape == (2, 3, 4)
+    y.backward(T.Tensor.ones((2, 3, 4)))
+    assert X.grad_by_value().shape == (2, 3, 5)
+    T.clear_gradients()
+
+
+def far_values():
+    return np.r_[np.linspace(-100, 100, 801), [-1e20, 1e20, -1e38, 1e38, -88.7, 88.7, -104, -0.0, 1e-30, -1e-42]]
+
+
+@pytest.mark.parametrize("name", ["relu", "silu", "gelu_tanh"])
+def test_activations_and_slopes_far_out(name):
+    z = far_values().astype(np.float32)
+    X, W = tensor(z.reshape(-1, 1)).with_requires_grad(), tensor(np.ones((1, 1), np.float32))
+    y = X.linear(W, activation=name)
+    zz = z.astype(np.float64).reshape(-1, 1)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want, slope = R.act(zz, name), np.nan_to_num(R.act_slope(zz, name))
+    # an exponential, a reciprocal and the cubic, each relative: the cubic's error enters times |v|, which is below 110
+    # wherever the result is not the limit
+    assert_within(y.data(), want, 16 * R.U * np.abs(want) * (1 + np.minimum(np.abs(zz) ** 3, 110)) + 1e-43, "y")
+    y.backward(T.Tensor.ones((z.size, 1)))
+    g = X.grad_by_value().data()
+    near = (np.abs(zz) < 20).reshape(-1)
+    assert np.all(np.isfinite(g))
+    assert_within(g[near], slope[near], 64 * R.U * np.maximum(np.abs(slope[near]), 1), "slope")
+    far = ~near
+    assert np.allclose(g[far], (zz[far] > 0).astype(float), atol=1e-6)
+    T.clear_gradients()
+
+
+def test_linear_with_values_that_are_not_finite():
+    x, w, b, r, go = layer_case(40, 70, 50, True, False)
+    x[3, 5], x[7, 1], x[8, 2] = np.nan, np.inf, -np.inf
+    y = tensor(x).linear(tensor(w), bias=tensor(b)).data()
+    with np.errstate(invalid="ignore"):
+        want = x.astype(np.float64) @ w + b
+    assert np.array_equal(np.isnan(y), np.isnan(want)) and np.array_equal(np.isinf(y), np.isinf(want))
+    assert np.array_equal(y[np.isinf(y)] > 0, want[np.isinf(want)] > 0)
+    rest = np.isfinite(want).all(1)
+    assert_within(y[rest], want[rest], R.linear_bound(x[rest], w, b, "none", None, want[rest]), "y")
+
+
+# ---- layers in 8 bits -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 8, 8), (1, 4096, 512), (2, 33, 5), (5, 127, 19), (16, 128, 64), (17, 129, 65),
+                                   (33, 1531, 31), (70, 300, 77), (200, 640, 130)])
+@pytest.mark.parametrize("name,bias,residual", [("none", False, False), ("relu", True, False), ("silu", True, True),
+                                                ("gelu_tanh", False, True)])
+def test_linear_packed(m, k, n, name, bias, residual):
+    x, w, b, r, _ = layer_case(m, k, n, bias, residual)
+    w = np.ascontiguousarray(w.T)
+    xq, wq = (R.unpack8(*R.pack8(a), k) for a in (x, w))
+    y = packed(x).linear(packed(w), bias=tensor(b) if bias else None, activation=name,
+                         residual=tensor(r) if residual else None)
+    want, z = R.linear(xq, wq.T, b, name, r)
+    assert_within(y.data(), want, R.linear_bound(xq, wq.T, b, name, r, z), "y")
+
+
+def test_linear_packed_scales_of_every_size():
+    """Blocks from the smallest scale to the largest, the products' exponents in range."""
+    m, n, k = 9, 20, 32 * 40
+    rng = np.random.default_rng(3)
+    e = rng.integers(-110, 111, (40,))
+    x = (rng.standard_normal((m, k)) * 2.0 ** np.repeat(e, 32)).astype(np.float32)
+    w = (rng.standard_normal((n, k)) * 2.0 ** np.repeat(-e, 32)).astype(np.float32)
+    xq, wq = (R.unpack8(*R.pack8(a), k) for a in (x, w))
+    y = packed(x).linear(packed(w))
+    want = xq @ wq.T
+    assert_within(y.data(), want, R.product_bound(xq, wq.T), "y")
+
+
+def test_linear_packed_nan_codes_and_nothing():
+    x, w = normal((4, 50), 1), normal((6, 50), 2)
+    x[2, 7] = np.nan
+    y = tensor(x).pack8().linear(tensor(w).pack8()).data()
+    assert np.isnan(y[2]).all() and np.isfinite(np.delete(y, 2, 0)).all()
+    b = normal((6,), 3)
+    y = T.Tensor.zeros((4, 0)).pack8().linear(T.Tensor.zeros((6, 0)).pack8(), bias=tensor(b)).data()
+    assert np.array_equal(y, np.tile(b, (4, 1)))
+    assert T.Tensor.zeros((0, 5)).pack8().linear(tensor(w[:, :5]).pack8()).shape == (0, 6)
+
+
+# ---- the rest ---------------------------------------------------------------------------
+
+
+def test_refusals():
+    x, w = tensor(normal((4, 6), 1)), tensor(normal((6, 5), 2))
+    v5, v6 = tensor(normal((5,), 3)), tensor(normal((6,), 4))
+    r = tensor(normal((4, 5), 5))
+    for call, what in ((lambda: x.linear(x), "Inner dimensions must match"), (lambda: x.linear(v6), "weight matrix"),
+                       (lambda: x.linear(w, bias=v6), "bias"), (lambda: x.linear(w, residual=x), "residual"),
+                       (lambda: x.rms_norm(v5), "weight"), (lambda: x.add_rms_norm(r, v6), "residual"),
+                       (lambda: x.rms_norm(v6, -1.0), "eps"), (lambda: x.rms_norm(v6, float("nan")), "eps"),
+                       (lambda: v6.pack8(), "matrix"), (lambda: v6.rms_norm_packed(v6), "matrix"),
+                       (lambda: x.pack8().linear(r.pack8()), "Inner dimensions must match"),
+                       (lambda: x.pack8().linear(x.pack8(), bias=v5), "bias")):
+        with pytest.raises(T.TsError, match=what):
+            call()
+
+
+def test_device_memory_is_used_in_place_and_given_back():
+    import gc
+
+    a = DeviceArray(normal((8, 16), 1))
+    t = T.Tensor.from_device(a)
+    assert t.device_ptr() == a.dev.ptr and np.array_equal(t.data(), a.host)
+    t.fill(2.0)
+    T.synchronize()
+    assert np.array_equal(a.get(), np.full((8, 16), 2.0, np.float32))
+    from train_station_amd import tensor as module
+
+    held = len(module._lent)
+    w = tensor(normal((16, 4), 2)).with_requires_grad()
+    y = t.linear(w)
+    del t
+    gc.collect()
+    assert len(module._lent) == held  # the recorded layer reads it in its backward pass
+    y.backward(T.Tensor.ones((8, 4)))
+    assert np.allclose(w.grad_by_value().data(), 16.0)
+    T.clear_gradients()
+    del y
+    gc.collect()
+    assert len(module._lent) == held - 1
+    host = np.zeros((2, 3), np.float32)
+
+    class Host:
+        __cuda_array_interface__ = dict(shape=(2, 3), typestr="<f4", data=(host.ctypes.data, False), version=2)
+
+    class Past(Host):  # more than the allocation holds
+        __cuda_array_interface__ = dict(shape=(1 << 40,), typestr="<f4", data=(a.dev.ptr, False), version=2)
+
+    for bad in (Host(), Past()):
+        with pytest.raises(T.TsError, match="device memory"):
+            T.Tensor.from_device(bad)
+    assert len(module._lent) == held - 1
+
+
+def block_parameters(seed=0):
+    d, f = 48, 80
+    return [tensor(a).with_requires_grad() for a in (np.ones(d, np.float32), normal((d, f), seed + 1, d ** -0.5),
+                                                     np.zeros(f, np.float32), normal((f, d), seed + 2, f ** -0.5),
+                                                     np.zeros(d, np.float32))]
+
+
+def block_step(ps, opt, x, r, t):
+    norm, w1, b1, w2, b2 = ps
+    h, stream = x.add_rms_norm(r, norm)
+    y = h.linear(w1, bias=b1, activation="silu", checkpoint="8bit").linear(w2, bias=b2, residual=stream, checkpoint="8bit")
+    d = y.sub_tensor(t)
+    loss = d.mul_tensor(d).mean()
+    loss.backward()
+    opt.step(ps)
+    opt.zero_grad(ps)
+    T.clear_gradients()
+    return loss
+
+
+def test_block_trains_and_replays_as_it_runs():
+    """A block's step recorded and replayed, with eager work between the replays, has the eager steps' bits."""
+    x, r, t = (tensor(normal((32, 48), s)) for s in (5, 6, 7))
+    eager, opt = block_parameters(), T.Adam.with_learning_rate(1e-2)
+    opt.add_parameters(eager)
+    losses = [block_step(eager, opt, x, r, t).value() for _ in range(7)]
+    assert losses[-1] < 0.7 * losses[0]
+    ps, opt2 = block_parameters(), T.Adam.with_learning_rate(1e-2)
+    opt2.add_parameters(ps)
+    block_step(ps, opt2, x, r, t)
+    with T.StepGraph.record() as g:
+        block_step(ps, opt2, x, r, t)
+    for n in (1, 2, 1):
+        g.replay(n)
+        T.synchronize()
+        tensor(normal((16, 48), 9)).linear(ps[1]).sum().value()
+    block_step(ps, opt2, x, r, t)
+    block_step(ps, opt2, x, r, t)
+    for a, b in zip(eager, ps):
+        assert np.array_equal(a.data(), b.data())
+    g.free()
+
+
+def test_equal_calls_give_equal_bits():
+    outs = []
+    for _ in range(2):
+        x, w, b, r, go = layer_case(150, 260, 190, True, True)
+        X, W, B = (tensor(a).with_requires_grad() for a in (x, w, b))
+        y = X.linear(W, bias=B, activation="gelu_tanh", residual=tensor(r), checkpoint="8bit")
+        y.backward(tensor(go))
+        outs.append([y.data()] + [t.grad_by_value().data() for t in (X, W, B)])
+        T.clear_gradients()
+    for a, b in zip(*outs):
+        assert np.array_equal(a, b)

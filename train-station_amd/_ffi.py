@@ -53,6 +53,15 @@ class OperandXf(ctypes.Structure):
     _fields_ = [("n_ops", _c.c_uint32), ("code", _c.c_uint8 * XF_MAX_OPS), ("imm", _c.c_float * XF_MAX_OPS)]
 
 
+class LinearShape(ctypes.Structure):
+    """struct ts_hip_linear_shape of include/ts_hip.h"""
+    _fields_ = [("batch", SZ), ("fan_in", SZ), ("fan_out", SZ)]
+
+
+# TS_HIP_ACT_* of include/ts_hip.h
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
+
+
 class MapOp(ctypes.Structure):
     """struct ts_hip_map_op of include/ts_hip.h"""
     _fields_ = [("code", _c.c_uint8), ("a", _c.c_uint8), ("b", _c.c_uint8), ("flags", _c.c_uint8),
@@ -174,6 +183,20 @@ HIP_SIGNATURES = {
     "ts_hip_gemv": (_c.c_int, [_c.c_int, SZ, SZ, VP, SZ, VP, VP, VP, SZ, VP]),
     "ts_hip_dot": (_c.c_int, [VP, VP, SZ, VP, VP, SZ, VP]),
     "ts_hip_outer": (_c.c_int, [VP, SZ, VP, SZ, VP, VP]),
+    "ts_hip_check_device_range": (_c.c_int, [VP, SZ]),
+    "ts_hip_packed_pitch": (SZ, [SZ]),
+    "ts_hip_pack8": (_c.c_int, [VP, SZ, SZ, VP, VP, VP]),
+    "ts_hip_unpack8": (_c.c_int, [VP, VP, SZ, SZ, VP, VP]),
+    "ts_hip_rms_norm": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP]),
+    "ts_hip_rms_norm_packed": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, VP]),
+    "ts_hip_rms_norm_backward_workspace_floats": (SZ, [SZ, SZ]),
+    "ts_hip_rms_norm_backward": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, SZ, VP]),
+    "ts_hip_linear_packed_workspace_floats": (SZ, [SZ, SZ, SZ]),
+    "ts_hip_linear_packed": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, SZ, VP, _c.c_int, VP, VP, VP, SZ, VP]),
+    "ts_hip_linear_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),
+    "ts_hip_linear": (_c.c_int, [_c.POINTER(LinearShape), VP, VP, VP, _c.c_int, VP, VP, VP, VP, VP, VP, SZ, VP]),
+    "ts_hip_linear_backward_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),
+    "ts_hip_linear_backward": (_c.c_int, [_c.POINTER(LinearShape), VP, VP, VP, VP, VP, _c.c_int, VP, VP, VP, VP, VP, VP, SZ, VP]),
     "ts_hip_adam_step": (_c.c_int, [VP, VP, VP, VP, VP, SZ, _c.c_float, _c.c_float, _c.c_float,
                                     _c.c_float, _c.c_float, _c.c_uint64, SZ, _c.c_int, VP]),
     "ts_hip_adam_step_multi": (_c.c_int, [VP, SZ, _c.c_float, _c.c_float, _c.c_float, _c.c_float,
@@ -224,6 +247,23 @@ GRADTRACK_SIGNATURES = {
     "ts_tensor_with_requires_grad": (_c.c_int, [TP]),
     "ts_tensor_set_requires_grad": (_c.c_int, [TP, _c.c_int]),
     "ts_tensor_requires_grad": (_c.c_int, [TP]),
+    "ts_tensor_from_device": (TP, [VP, _c.POINTER(SZ), SZ, VP, VP]),
+    "ts_external_detach": (None, []),
+    "ts_tensor_grad_view": (TP, [TP]),
+    "ts_tensor_rms_norm": (TP, [TP, TP, _c.c_float]),
+    "ts_tensor_add_rms_norm": (TP, [TP, TP, TP, _c.c_float, _c.POINTER(TP)]),
+    "ts_tensor_linear": (TP, [TP, TP, TP, _c.c_int, TP, _c.c_int]),
+    "ts_tensor_pack8": (TP, [TP]),
+    "ts_tensor_rms_norm_packed": (TP, [TP, TP, TP, _c.c_float, _c.POINTER(TP)]),
+    "ts_packed8_from_device": (TP, [VP, VP, SZ, SZ, VP, VP]),
+    "ts_packed8_free": (None, [TP]),
+    "ts_packed8_rows": (SZ, [TP]),
+    "ts_packed8_cols": (SZ, [TP]),
+    "ts_packed8_pitch": (SZ, [TP]),
+    "ts_packed8_codes_ptr": (VP, [TP]),
+    "ts_packed8_scales_ptr": (VP, [TP]),
+    "ts_packed8_unpack": (TP, [TP]),
+    "ts_packed8_linear": (TP, [TP, TP, TP, _c.c_int, TP]),
     "ts_tensor_add_tensor": (TP, [TP, TP]),
     "ts_tensor_sub_tensor": (TP, [TP, TP]),
     "ts_tensor_mul_tensor": (TP, [TP, TP]),

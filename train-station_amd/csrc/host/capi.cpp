@@ -15,6 +15,10 @@ struct ts_adam {
     ts::Adam a;
 };
 
+struct ts_packed8 {
+    ts::Packed8 p;
+};
+
 struct ts_step_graph {
     std::unique_ptr<ts::StepGraph> g;
 };
@@ -62,6 +66,26 @@ const ts::Tensor &T(const ts_tensor *h) {
     return h->t;
 }
 
+const ts::Packed8 &P(const ts_packed8 *h) {
+    if (!h) throw ts::Error("packed handle is NULL");
+    return h->p;
+}
+
+const ts::Tensor *optional_tensor(const ts_tensor *h) { return h ? &h->t : nullptr; }
+
+ts::Activation activation_of(int act) {
+    if (act < 0 || act > 3) throw ts::Error("unknown activation " + std::to_string(act));
+    return static_cast<ts::Activation>(act);
+}
+
+// A caller's release call, for the memory's last user (when the tensor is not
+// made, the entry itself makes it).
+std::function<void()> release_call(void (*release)(void *), void *ctx) {
+    if (!release) return {};
+    return [release, ctx] {
+        if (!ts::external_detached()) release(ctx);
+    };
+}
 std::vector<ts::Tensor *> param_list(ts_tensor *const *params, size_t count) {
     if (count && !params) throw ts::Error("parameter list is NULL");
     std::vector<ts::Tensor *> v;
@@ -103,6 +127,77 @@ int ts_tensor_fill_randn(ts_tensor *t, uint64_t seed, int has_seed) {
         t->t.fill_randn(has_seed ? &seed : nullptr);
     });
 }
+ts_tensor *ts_tensor_from_device(float *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx) {
+    ts_tensor *t =
+        guard_ptr([&] { return wrap(ts::Tensor::from_device(data, dims_of(dims, rank), release_call(release, ctx))); });
+    if (!t && release) release(ctx);
+    return t;
+}
+void ts_external_detach(void) { ts::detach_external(); }
+
+ts_tensor *ts_tensor_rms_norm(const ts_tensor *x, const ts_tensor *weight, float eps) {
+    return guard_ptr([&] { return wrap(T(x).rms_norm(T(weight), eps)); });
+}
+ts_tensor *ts_tensor_add_rms_norm(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight, float eps,
+                                  ts_tensor **h_out) {
+    return guard_ptr([&] {
+        if (!h_out) throw ts::Error("h_out is NULL");
+        auto r = T(x).add_rms_norm(T(residual), T(weight), eps);
+        std::unique_ptr<ts_tensor> y(wrap(std::move(r.first)));
+        *h_out = wrap(std::move(r.second));
+        return y.release();
+    });
+}
+ts_tensor *ts_tensor_linear(const ts_tensor *x, const ts_tensor *weight, const ts_tensor *bias, int activation,
+                            const ts_tensor *residual, int checkpoint) {
+    return guard_ptr([&] {
+        if (checkpoint != 0 && checkpoint != 1) throw ts::Error("unknown checkpoint " + std::to_string(checkpoint));
+        return wrap(T(x).linear(T(weight), optional_tensor(bias), activation_of(activation), optional_tensor(residual),
+                                static_cast<ts::Checkpoint>(checkpoint)));
+    });
+}
+ts_packed8 *ts_tensor_pack8(const ts_tensor *x) {
+    return guard_ptr([&] { return new ts_packed8{T(x).pack8()}; });
+}
+ts_packed8 *ts_tensor_rms_norm_packed(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight, float eps,
+                                      ts_tensor **h_out) {
+    return guard_ptr([&] {
+        if (!residual) return new ts_packed8{T(x).rms_norm_packed(T(weight), eps)};
+        if (!h_out) throw ts::Error("h_out is NULL");
+        auto r = T(x).add_rms_norm_packed(T(residual), T(weight), eps);
+        std::unique_ptr<ts_packed8> p(new ts_packed8{std::move(r.first)});
+        *h_out = wrap(std::move(r.second));
+        return p.release();
+    });
+}
+ts_packed8 *ts_packed8_from_device(uint8_t *codes, uint8_t *scales, size_t rows, size_t cols, void (*release)(void *),
+                                   void *ctx) {
+    ts_packed8 *p = guard_ptr([&] {
+        return new ts_packed8{ts::Packed8::from_device(codes, scales, rows, cols, release_call(release, ctx))};
+    });
+    if (!p && release) release(ctx);
+    return p;
+}
+void ts_packed8_free(ts_packed8 *p) { delete p; }
+size_t ts_packed8_rows(const ts_packed8 *p) { return p ? p->p.rows() : 0; }
+size_t ts_packed8_cols(const ts_packed8 *p) { return p ? p->p.cols() : 0; }
+size_t ts_packed8_pitch(const ts_packed8 *p) { return p ? p->p.pitch() : 0; }
+const uint8_t *ts_packed8_codes_ptr(const ts_packed8 *p) {
+    return guard_ptr([&] { return static_cast<const uint8_t *>(P(p).codes()); });
+}
+const uint8_t *ts_packed8_scales_ptr(const ts_packed8 *p) {
+    return guard_ptr([&] { return static_cast<const uint8_t *>(P(p).scales()); });
+}
+ts_tensor *ts_packed8_unpack(const ts_packed8 *p) {
+    return guard_ptr([&] { return wrap(P(p).unpack()); });
+}
+ts_tensor *ts_packed8_linear(const ts_packed8 *x, const ts_packed8 *weight, const ts_tensor *bias, int activation,
+                             const ts_tensor *residual) {
+    return guard_ptr([&] {
+        return wrap(P(x).linear(P(weight), optional_tensor(bias), activation_of(activation), optional_tensor(residual)));
+    });
+}
+
 ts_tensor *ts_tensor_clone(const ts_tensor *t) {
     return guard_ptr([&] { return wrap(T(t).clone()); });
 }
@@ -205,6 +300,13 @@ int ts_tensor_backward(ts_tensor *t, const ts_tensor *grad_output) {
     });
 }
 
+ts_tensor *ts_tensor_grad_view(const ts_tensor *t) {
+    return guard_ptr([&]() -> ts_tensor * {
+        const ts::Tensor *g = T(t).grad_ref();
+        if (!g) return nullptr;
+        return wrap(g->view());
+    });
+}
 ts_tensor *ts_tensor_grad(const ts_tensor *t) {
     return guard_ptr([&]() -> ts_tensor * {
         const ts::Tensor *g = T(t).grad_direct();

@@ -67,6 +67,17 @@ void StepRecorder::adam_param(size_t use, size_t param_id) {
     graph_->adams[use].params.push_back(param_id);
 }
 
+void StepRecorder::keep(std::shared_ptr<Allocation> external) {
+    if (!graph_) return;
+    for (const auto &a : graph_->external)
+        if (a == external) return;
+    graph_->external.push_back(std::move(external));
+}
+
+void StepRecorder::put_off(std::function<void()> release) {
+    if (graph_) graph_->releases.push_back(std::move(release));
+}
+
 void StepRecorder::take_back(StepGraph &g) {
     for (StepGraph::AdamUse &u : g.adams) {
         u.ledger->step_count -= 1;
@@ -112,6 +123,7 @@ StepGraph::~StepGraph() {
         (void)ts_hip_graph_destroy(exec);
     }
     DevicePool::get().unpin(pins);
+    for (auto &release : releases) release();
 }
 
 void StepGraph::replay(size_t times) {

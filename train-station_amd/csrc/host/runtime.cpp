@@ -164,7 +164,30 @@ Allocation::Allocation(size_t n_floats) : n(n_floats) {
     ptr_ = DevicePool::get().acquire(n_floats, &rounded);
 }
 
-Allocation::~Allocation() { DevicePool::get().release(ptr_, rounded); }
+Allocation::Allocation(float *external, size_t n_floats, std::function<void()> release)
+    : n(n_floats), ptr_(external), release_(std::move(release)) {
+    if (!release_) release_ = [] {};
+}
+
+static std::atomic<bool> g_detached{false};
+void detach_external() { g_detached = true; }
+bool external_detached() { return g_detached; }
+
+Allocation::~Allocation() {
+    if (!release_) {
+        DevicePool::get().release(ptr_, rounded);
+        return;
+    }
+    // a caller may reuse the memory at once: queued work runs first
+    if (g_detached) return;
+    StepRecorder &rec = StepRecorder::get();
+    if (rec.open()) {
+        rec.put_off(std::move(release_));
+        return;
+    }
+    (void)ts_hip_stream_synchronize(Runtime::get().stream());
+    release_();
+}
 
 float *Allocation::get() {
     if (pending) materialize(*this);
@@ -173,7 +196,12 @@ float *Allocation::get() {
     else if (transpose) materialize_transpose(*this);
     else if (reduce) materialize_reduce(*this);
     else if (sibling) run_sibling(*this);
-    DevicePool::get().note_use(ptr_);
+    if (release_) {
+        StepRecorder &rec = StepRecorder::get();
+        if (rec.open()) rec.keep(shared_from_this());
+    } else {
+        DevicePool::get().note_use(ptr_);
+    }
     return ptr_;
 }
 

@@ -1141,6 +1141,23 @@ Tensor Tensor::from_slice(const float *data, size_t len, std::vector<size_t> dim
     return t;
 }
 
+Tensor Tensor::from_device(float *data, std::vector<size_t> dims, std::function<void()> release) {
+    Tensor t;
+    t.size_ = product(dims);
+    t.dims_ = std::move(dims);
+    t.id_ = next_tensor_id();
+    if (t.size_ == 0) {
+        if (release) release();
+        return t;
+    }
+    Runtime::get();  // a stream to wait for when it is let go
+    if (!data || reinterpret_cast<uintptr_t>(data) % sizeof(float) != 0 ||
+        ts_hip_check_device_range(data, t.size_ * sizeof(float)) != TS_HIP_OK)
+        throw Error("from_device: " + dims_str(t.dims_) + " floats are not in one allocation of device memory");
+    t.alloc_ = std::make_shared<Allocation>(data, t.size_, std::move(release));
+    return t;
+}
+
 Tensor Tensor::clone() const {
     Tensor t = new_uninit(dims_);
     if (size_)
@@ -2197,6 +2214,10 @@ std::vector<std::optional<Tensor>> GradFn::apply(const Tensor &go) const {
             r.emplace_back(std::move(gr));
             break;
         }
+        case K::RmsNorm:
+            return rms_norm_backward(*this, go);
+        case K::Linear:
+            return linear_backward(*this, go);
         case K::Transpose:  // grad_fn/transforms/transpose.rs: the same two axes swapped back
             r.emplace_back(transposed_value(go, dim0, dim1, false));
             break;

@@ -239,6 +239,9 @@ struct PendingReduce {
 // buffer; shared (Arc-like) by tensors, saved graph operands and gradients.
 struct Allocation : std::enable_shared_from_this<Allocation> {
     explicit Allocation(size_t n_floats);
+    // A caller's device memory, not the pool's: `release` is called once the
+    // last user is gone and the work queued by then has run.
+    Allocation(float *external, size_t n_floats, std::function<void()> release);
     ~Allocation();
     Allocation(const Allocation &) = delete;
     Allocation &operator=(const Allocation &) = delete;
@@ -265,7 +268,12 @@ struct Allocation : std::enable_shared_from_this<Allocation> {
 
   private:
     float *ptr_ = nullptr;
+    std::function<void()> release_;  // a caller's memory
 };
+
+// The process is ending: callers' memory is let go without their release calls.
+void detach_external();
+bool external_detached();
 
 // Runs a's pending producer (tensor.cpp).
 void materialize(Allocation &a);
@@ -401,6 +409,14 @@ void launch(KernelClass k, double work, const char *what, F &&f) {
 // ---- tensors --------------------------------------------------------------------
 
 class Tensor;
+class Packed8;
+
+// Activations of Tensor::linear (TS_HIP_ACT_*)
+enum class Activation : int { None = 0, Relu = 1, Silu = 2, GeluTanh = 3 };
+// What a layer keeps of its input for the backward pass: the tensor itself
+// (and, with an activation, the values before it), or its values in 8 bits,
+// from which the backward pass computes the layer again.
+enum class Checkpoint : int { Full = 0, EightBit = 1 };
 
 struct SavedTensor {
     std::shared_ptr<Allocation> alloc;
@@ -414,7 +430,7 @@ struct GradFn {
         Add, Sub, Mul, Div, AddScalar, SubScalar, MulScalar, DivScalar,
         Relu, PowScalar, MatMul, ReduceSum, ReduceMean,
         Exp, Log, Sqrt, Tanh, Sigmoid, LeakyRelu, Softmax, ReduceSumDims, ReduceMeanDims,
-        Transpose, Contiguous
+        Transpose, Contiguous, RmsNorm, Linear
     };
     explicit GradFn(Kind k) : kind(k) {}
     Kind kind;
@@ -429,6 +445,11 @@ struct GradFn {
     bool keepdim = false;
     size_t axis = 0;                   // softmax
     size_t dim0 = 0, dim1 = 0;         // transpose: the axes swapped
+    // a layer: saved = {x, weight, bias, z}, without a buffer where there is
+    // none; its input's values in 8 bits instead of x
+    Activation activation = Activation::None;
+    std::shared_ptr<Packed8> checkpoint;
+    bool has_bias = false, has_residual = false, req_bias = false, req_residual = false;
 
     // GradFn::apply (grad_fn/mod.rs:490-789): gradients by operand position.
     std::vector<std::optional<Tensor>> apply(const Tensor &grad_output) const;
@@ -452,6 +473,8 @@ class Tensor {
     // backward(None)), and is written only if something else reads it.
     static Tensor constant(std::vector<size_t> dims, float v);
     static Tensor from_slice(const float *data, size_t len, std::vector<size_t> dims);
+    // A tensor over a caller's device memory (row-major, not copied).
+    static Tensor from_device(float *data, std::vector<size_t> dims, std::function<void()> release);
     // Tensor::randn (init/random.rs:231-235): XorShiftRng values generated on
     // the device; without a seed, one derived from the clock (random.rs:492-497)
     static Tensor randn(std::vector<size_t> dims, const uint64_t *seed);
@@ -526,6 +549,17 @@ class Tensor {
     // reductions/sum.rs:225-306, reductions/mean.rs:186-230
     Tensor sum_dims(const std::vector<size_t> &dims, bool keepdim) const;
     Tensor mean_dims(const std::vector<size_t> &dims, bool keepdim) const;
+    // A feed-forward block's operators (feedforward.cpp; no counterpart in the
+    // reference), over the last axis: h / sqrt(mean(h^2) + eps) * weight, h this
+    // tensor or its sum with residual; act(self weight + bias) + residual.
+    Tensor rms_norm(const Tensor &weight, float eps) const;
+    std::pair<Tensor, Tensor> add_rms_norm(const Tensor &residual, const Tensor &weight, float eps) const;  // y, h
+    // y in 8 bits (no gradient passes through it)
+    Packed8 rms_norm_packed(const Tensor &weight, float eps) const;
+    std::pair<Packed8, Tensor> add_rms_norm_packed(const Tensor &residual, const Tensor &weight, float eps) const;
+    Tensor linear(const Tensor &weight, const Tensor *bias, Activation act, const Tensor *residual,
+                  Checkpoint checkpoint) const;
+    Packed8 pack8() const;
     // transform/transpose.rs:156-291, contiguous.rs:123-157: a transposed
     // view (deferred copy, see PendingTranspose), t() = the last two axes;
     // contiguous() of a view is its copy, of anything else a clone; both
@@ -561,6 +595,32 @@ class Tensor {
     bool strided_ = false;
     std::shared_ptr<Tensor> grad_;
 };
+
+// A matrix in 8 bits (the layout: ts_hip.h, ts_hip_pack8).
+class Packed8 {
+  public:
+    static Packed8 new_uninit(size_t rows, size_t cols);
+    // a caller's codes [rows, pitch] and scales [pitch / 128, rows, 4] on the device
+    static Packed8 from_device(uint8_t *codes, uint8_t *scales, size_t rows, size_t cols,
+                               std::function<void()> release);
+    size_t rows() const { return rows_; }
+    size_t cols() const { return cols_; }
+    size_t pitch() const;
+    uint8_t *codes() const { return codes_ ? reinterpret_cast<uint8_t *>(codes_->get()) : nullptr; }
+    uint8_t *scales() const { return scales_ ? reinterpret_cast<uint8_t *>(scales_->get()) : nullptr; }
+    // the values that the codes stand for
+    Tensor unpack() const;
+    // act(self weight^T + bias) + residual, weight [fan_out, fan_in] in 8 bits too
+    Tensor linear(const Packed8 &weight, const Tensor *bias, Activation act, const Tensor *residual) const;
+
+  private:
+    std::shared_ptr<Allocation> codes_, scales_;
+    size_t rows_ = 0, cols_ = 0;
+};
+
+// The gradients of Kind::RmsNorm and Kind::Linear (feedforward.cpp).
+std::vector<std::optional<Tensor>> rms_norm_backward(const GradFn &fn, const Tensor &go);
+std::vector<std::optional<Tensor>> linear_backward(const GradFn &fn, const Tensor &go);
 
 // x with axes d0 != d1 swapped, deferred (no recording): a deferred bare
 // matrix product becomes the product of its swapped operands; a pending view
@@ -703,6 +763,10 @@ struct StepGraph {
     };
     std::vector<AdamUse> adams;
     uint64_t executed = 0;  // replays run so far
+    // callers' memory that the recorded work touches, and release calls that
+    // came up while recording (nothing may wait for the device then)
+    std::vector<std::shared_ptr<Allocation>> external;
+    std::vector<std::function<void()>> releases;
 };
 
 class StepRecorder {
@@ -727,6 +791,10 @@ class StepRecorder {
     // before each run of replays).
     unsigned *adam_tickets(size_t waves);
     void adam_param(size_t use, size_t param_id);
+    // Called while recording: keeps a caller's memory for the graph's life;
+    // puts a release call off until the graph is freed.
+    void keep(std::shared_ptr<Allocation> external);
+    void put_off(std::function<void()> release);
 
   private:
     // The counts the recorded Adam steps added while recording, taken back.

@@ -1,0 +1,431 @@
+// Root-mean-square norm with the residual's addition (ts_hip.h, ts_hip_rms_norm
+// and the entries after it), its packed form, its backward, and the packing of
+// plain rows.
+//
+//   h = x + residual,  r = 1 / sqrt(mean(h^2) + eps),  y = h r w
+//   g = go w:  dh = r g - h r^3 mean(g h),  dw = sum over rows of go h r
+//
+// A row is held in registers by W waves, four neighbouring columns a lane and
+// NV such quads, so memory is passed over once; sums are f64.  Backward needs
+// h^2's and g h's row sums only, and takes both in the same pass: nothing but h
+// is kept from the forward.
+#include "ts_hip_pack8.h"
+
+namespace tship {
+
+namespace {
+
+constexpr size_t kMaxHeldCols = 16384;  // 16 waves of 64 lanes of four quads
+
+__device__ __forceinline__ void load4(const float *p, size_t c, size_t cols, float (&v)[4]) {
+    if (c + 4 <= cols) {
+        const pk4u_t q = *reinterpret_cast<const pk4u_t *>(p + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? p[c + e] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void store4(float *p, size_t c, size_t cols, const float (&v)[4]) {
+    if (c + 4 <= cols) {
+        *reinterpret_cast<pk4u_t *>(p + c) = pk4u_t{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < cols) p[c + e] = v[e];
+    }
+}
+
+// The sum over the W waves of a row, in every lane; lds: N * W doubles of this row.
+template <int W, int N>
+__device__ __forceinline__ void row_sum(double (&s)[N], double *lds) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] = wave_sum(s[n]);
+    if (W == 1) return;
+    const int wave = (threadIdx.x >> 6) % W;
+    __syncthreads();  // the last row's reads
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) lds[n * W + wave] = s[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[n] = 0.0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s[n] += lds[n * W + w];
+    }
+}
+
+template <int W>
+constexpr int kNormThreads = W < 4 ? 256 : 64 * W;
+template <int W>
+constexpr int kNormRows = kNormThreads<W> / (64 * W);  // rows of a workgroup
+
+struct NormArgs {
+    const float *x, *residual, *weight;
+    float *h, *y;             // h: with a residual
+    uint8_t *codes, *scales;  // packed
+    size_t rows, cols, pitch;
+    double eps;
+};
+
+// One row per W waves; LONG: more columns than the waves hold, passed over twice.
+template <int W, int NV, bool RES, bool PACK, bool LONG>
+__global__ __launch_bounds__(kNormThreads<W>) void rms_norm_rows(NormArgs a) {
+    constexpr int RPB = kNormRows<W>;
+    __shared__ double lds[RPB * W];
+    const int slot = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W);
+    const size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot;
+    const bool live = row < a.rows;  // uniform per wave; the others reach the barriers
+    const size_t base = live ? row * a.cols : 0;
+    const float *x = a.x + base, *res = RES ? a.residual + base : nullptr;
+    const size_t span = static_cast<size_t>(256) * W * NV, end = PACK ? a.pitch : a.cols;
+
+    float v[NV][4];
+    auto fetch = [&](size_t c0) {  // h of the columns from c0 on (past the row: zeros)
+        float r[NV][4];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load4(x, c0 + 4 * (t + 64 * W * i), live ? a.cols : 0, v[i]);
+        if (RES) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load4(res, c0 + 4 * (t + 64 * W * i), live ? a.cols : 0, r[i]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
+        }
+    };
+    double s[1] = {0.0};
+    size_t c0 = 0;
+    do {
+        fetch(c0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0] += static_cast<double>(v[i][e]) * v[i][e];
+        c0 += span;
+    } while (LONG && c0 < a.cols);
+    // the weights are on their way while the row's sum is taken
+    float w[NV][4];
+    auto weights = [&](size_t from) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load4(a.weight, from + 4 * (t + 64 * W * i), a.cols, w[i]);
+    };
+    if (!LONG) weights(0);
+    row_sum<W, 1>(s, lds + slot * W);
+    if (!live) return;  // (no barrier follows)
+    const double r = 1.0 / sqrt(s[0] / static_cast<double>(a.cols) + a.eps);
+    const float rf = static_cast<float>(r);
+    c0 = 0;
+    do {
+        if (LONG) {
+            fetch(c0);
+            weights(c0);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const size_t c = c0 + 4 * (t + 64 * W * i);
+            if (c >= end) continue;
+            if (RES) store4(a.h + base, c, a.cols, v[i]);
+            float o[4];
+            if (PACK) {  // in f64: a code takes the side of its border that y itself is on
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = round_odd(static_cast<double>(v[i][e]) * r * w[i][e]);
+                pack_store(o, c, a.codes + row * a.pitch, a.scales + 4 * row, 4 * a.rows);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = v[i][e] * rf * w[i][e];
+                store4(a.y + base, c, a.cols, o);
+            }
+        }
+        c0 += span;
+    } while (LONG && c0 < end);
+}
+
+struct NormBackArgs {
+    const float *h, *weight, *go;
+    float *dh, *dw_part;  // dw_part: [gridDim.x][cols]
+    size_t rows, cols;
+    double eps;
+};
+
+// Rows blockIdx.x * RPB + slot, and on by the grid's; a thread keeps dw's sums
+// of its columns (f64), the workgroup's go to dw_part.
+template <int W, int NV, bool DH, bool DW, bool LONG>
+__global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a) {
+    constexpr int RPB = kNormRows<W>;
+    __shared__ double lds[RPB * 2 * W];
+    const int slot = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W);
+    const size_t span = static_cast<size_t>(256) * W * NV;
+    double dw[NV][4] = {};
+    float w[NV][4];
+    auto weights = [&](size_t c0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load4(a.weight, c0 + 4 * (t + 64 * W * i), a.cols, w[i]);
+    };
+    if (!LONG) weights(0);
+    float *part = DW ? a.dw_part + static_cast<size_t>(blockIdx.x) * a.cols : nullptr;
+    bool first = true;
+    const size_t step = static_cast<size_t>(gridDim.x) * RPB;
+    // every wave of the workgroup takes every round (the barriers)
+    for (size_t r0 = static_cast<size_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += step) {
+        const size_t row = r0 + slot;
+        const bool live = row < a.rows;
+        const size_t base = live ? row * a.cols : 0, n = live ? a.cols : 0;
+        float h[NV][4], g[NV][4];
+        auto fetch = [&](size_t c0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load4(a.h + base, c0 + 4 * (t + 64 * W * i), n, h[i]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load4(a.go + base, c0 + 4 * (t + 64 * W * i), n, g[i]);
+        };
+        double s[2] = {0.0, 0.0};
+        size_t c0 = 0;
+        do {
+            fetch(c0);
+            if (LONG) weights(c0);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double hv = h[i][e];
+                    s[0] += hv * hv;
+                    s[1] += hv * (static_cast<double>(g[i][e]) * w[i][e]);
+                }
+            c0 += span;
+        } while (LONG && c0 < a.cols);
+        row_sum<W, 2>(s, lds + slot * 2 * W);
+        const double cols = static_cast<double>(a.cols);
+        const double r = 1.0 / sqrt(s[0] / cols + a.eps);
+        const float rf = static_cast<float>(r), back = static_cast<float>(r * r * r * (s[1] / cols));
+        c0 = 0;
+        do {
+            if (LONG) {
+                fetch(c0);
+                weights(c0);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const size_t c = c0 + 4 * (t + 64 * W * i);
+                if (DH && c < n) {
+                    float o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = rf * (g[i][e] * w[i][e]) - h[i][e] * back;
+                    store4(a.dh + base, c, a.cols, o);
+                }
+                if (DW && !LONG && live) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dw[i][e] += static_cast<double>(g[i][e]) * (h[i][e] * rf);
+                }
+                if (DW && LONG && c < n) {  // (one row at a time: the workgroup's own line)
+                    float o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = 0.0f;
+                    if (!first) load4(part, c, a.cols, o);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] += g[i][e] * (h[i][e] * rf);
+                    store4(part, c, a.cols, o);
+                }
+            }
+            c0 += span;
+        } while (LONG && c0 < a.cols);
+        first = false;
+    }
+    if (DW && !LONG) {
+        if constexpr (RPB > 1) {  // the workgroup's rows together, in their order
+            __shared__ double sum[(RPB - 1) * 64 * W * NV * 4];
+            __syncthreads();
+            if (slot > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = dw[i][e];
+            }
+            __syncthreads();
+            if (slot > 0) return;
+#pragma unroll
+            for (int k = 0; k < RPB - 1; ++k)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dw[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const size_t c = 4 * (t + 64 * W * i);
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw[i][e]);
+            if (c < a.cols) store4(part, c, a.cols, o);
+        }
+    }
+}
+
+// out[c] = the parts' sum over g, f64: 16 columns a workgroup, 16 groups of parts
+__global__ __launch_bounds__(kBlock) void sum_parts(const float *__restrict__ part, size_t parts, size_t cols,
+                                                    float *__restrict__ out) {
+    __shared__ double lds[16][17];
+    const int j = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const size_t c = static_cast<size_t>(blockIdx.x) * 16 + j;
+    double s = 0.0;
+    if (c < cols) {
+#pragma unroll 8
+        for (size_t g = q; g < parts; g += 16) s += part[g * cols + c];
+    }
+    lds[q][j] = s;
+    __syncthreads();
+    if (q == 0 && c < cols) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += lds[k][j];
+        out[c] = static_cast<float>(s);
+    }
+}
+
+// Rows of plain values to 8 bits: a thread packs a quad, a grid stride over all quads.
+__global__ __launch_bounds__(kBlock) void pack_rows(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
+                                                    uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+    const size_t quads = pitch / 4, total = rows * quads;  // a multiple of 32: blocks of eight lanes stay together
+    const size_t stride = static_cast<size_t>(gridDim.x) * kBlock;
+    for (size_t q = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; q < total; q += stride) {
+        const size_t row = q / quads, c = 4 * (q % quads);
+        float v[4];
+        load4(x + row * cols, c, cols, v);
+        pack_store(v, c, codes + row * pitch, scales + 4 * row, 4 * rows);
+    }
+}
+
+__global__ __launch_bounds__(kBlock) void unpack_rows(const uint8_t *__restrict__ codes,
+                                                      const uint8_t *__restrict__ scales, size_t rows, size_t cols,
+                                                      size_t pitch, float *__restrict__ out) {
+    const size_t quads = (cols + 3) / 4, total = rows * quads;
+    const size_t stride = static_cast<size_t>(gridDim.x) * kBlock;
+    for (size_t q = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; q < total; q += stride) {
+        const size_t row = q / quads, c = 4 * (q % quads);
+        const unsigned code = *reinterpret_cast<const unsigned *>(codes + row * pitch + c);
+        const uint8_t k = scales[(c / kPackGroup * rows + row) * 4 + c / kPackBlock % 4];
+        float v[4];
+        unpack4(code, k, v);
+        store4(out + row * cols, c, cols, v);
+    }
+}
+
+template <int W, int NV, bool LONG>
+void launch_norm(const NormArgs &a, bool pack, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>((a.rows + kNormRows<W> - 1) / kNormRows<W>)), block(kNormThreads<W>);
+    if (a.residual && pack) launch((rms_norm_rows<W, NV, true, true, LONG>), grid, block, 0, s, a);
+    else if (a.residual) launch((rms_norm_rows<W, NV, true, false, LONG>), grid, block, 0, s, a);
+    else if (pack) launch((rms_norm_rows<W, NV, false, true, LONG>), grid, block, 0, s, a);
+    else launch((rms_norm_rows<W, NV, false, false, LONG>), grid, block, 0, s, a);
+}
+
+template <int W, int NV, bool LONG>
+void launch_back(const NormBackArgs &a, unsigned grid, hipStream_t s) {
+    const dim3 block(kNormThreads<W>);
+    if (a.dh && a.dw_part) launch((rms_norm_back<W, NV, true, true, LONG>), dim3(grid), block, 0, s, a);
+    else if (a.dh) launch((rms_norm_back<W, NV, true, false, LONG>), dim3(grid), block, 0, s, a);
+    else launch((rms_norm_back<W, NV, false, true, LONG>), dim3(grid), block, 0, s, a);
+}
+
+// Calls f(W, NV, LONG as constants) for a row of n columns: the fewest waves
+// that hold it with at most four quads a lane.
+template <class F>
+void for_cols(size_t n, F &&f) {
+    using std::integral_constant;
+    if (n <= 256) f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<bool, false>{});
+    else if (n <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 2>{}, integral_constant<bool, false>{});
+    else if (n <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
+    else if (n <= 2048) f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<bool, false>{});
+    else if (n <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
+    else if (n <= 8192) f(integral_constant<int, 16>{}, integral_constant<int, 2>{}, integral_constant<bool, false>{});
+    else if (n <= kMaxHeldCols)
+        f(integral_constant<int, 16>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
+    else f(integral_constant<int, 16>{}, integral_constant<int, 4>{}, integral_constant<bool, true>{});
+}
+
+size_t rows_per_block(size_t cols) { return cols <= 1024 ? 4 : 1; }
+
+// Workgroups of the backward pass: as many as run at once (2048 threads a CU, at
+// most 4 workgroups), so that each sums many rows before it writes dw.
+size_t back_blocks(size_t rows, size_t cols) {
+    const size_t need = (rows + rows_per_block(cols) - 1) / rows_per_block(cols);
+    const size_t cap = static_cast<size_t>(device_cu_count()) * (cols > 4096 ? 1 : 2);
+    return need < cap ? need : cap;
+}
+
+constexpr size_t kMaxRows = size_t(1) << 31;
+
+}  // namespace
+
+}  // namespace tship
+
+using namespace tship;
+
+extern "C" {
+
+size_t ts_hip_packed_pitch(size_t cols) { return packed_pitch(cols); }
+
+int ts_hip_pack8(const float *x, size_t rows, size_t cols, uint8_t *codes, uint8_t *scales, void *stream) {
+    if (rows == 0 || cols == 0) return TS_HIP_OK;
+    if (!x || !codes || !scales) return TS_HIP_EINVAL;
+    const size_t pitch = packed_pitch(cols);
+    launch(pack_rows, dim3(grid_for(rows * pitch / 4)), dim3(kBlock), 0, as_stream(stream), x, rows, cols, pitch, codes,
+           scales);
+    return launch_status();
+}
+
+int ts_hip_unpack8(const uint8_t *codes, const uint8_t *scales, size_t rows, size_t cols, float *out, void *stream) {
+    if (rows == 0 || cols == 0) return TS_HIP_OK;
+    if (!codes || !scales || !out) return TS_HIP_EINVAL;
+    launch(unpack_rows, dim3(grid_for(rows * ((cols + 3) / 4))), dim3(kBlock), 0, as_stream(stream), codes, scales, rows,
+           cols, packed_pitch(cols), out);
+    return launch_status();
+}
+
+static int norm_forward(const float *x, const float *residual, const float *weight, size_t rows, size_t cols, float eps,
+                        float *h, float *y, uint8_t *codes, uint8_t *scales, void *stream) {
+    if (rows == 0 || cols == 0) return TS_HIP_OK;
+    if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
+    const NormArgs a = {x, residual, weight, h, y, codes, scales, rows, cols, packed_pitch(cols), eps};
+    for_cols(codes ? a.pitch : cols, [&](auto w, auto nv, auto long_rows) {
+        launch_norm<w.value, nv.value, long_rows.value>(a, codes != nullptr, as_stream(stream));
+    });
+    return launch_status();
+}
+
+int ts_hip_rms_norm(const float *x, const float *residual, const float *weight, size_t rows, size_t cols, float eps,
+                    float *h, float *y, void *stream) {
+    if (rows && cols && !y) return TS_HIP_EINVAL;
+    return norm_forward(x, residual, weight, rows, cols, eps, h, y, nullptr, nullptr, stream);
+}
+
+int ts_hip_rms_norm_packed(const float *x, const float *residual, const float *weight, size_t rows, size_t cols,
+                           float eps, float *h, uint8_t *codes, uint8_t *scales, void *stream) {
+    if (rows && cols && (!codes || !scales)) return TS_HIP_EINVAL;
+    return norm_forward(x, residual, weight, rows, cols, eps, h, nullptr, codes, scales, stream);
+}
+
+size_t ts_hip_rms_norm_backward_workspace_floats(size_t rows, size_t cols) { return back_blocks(rows, cols) * cols; }
+
+int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
+                             float *dh, float *dweight, float *workspace, size_t workspace_floats, void *stream) {
+    if (cols == 0 || (!dh && !dweight)) return TS_HIP_OK;
+    if (rows == 0) return dweight ? ts_hip_fill(dweight, 0.0f, cols, stream) : TS_HIP_OK;
+    if (!h || !weight || !go || rows >= kMaxRows) return TS_HIP_EINVAL;
+    if (dweight && (!workspace || workspace_floats < ts_hip_rms_norm_backward_workspace_floats(rows, cols)))
+        return TS_HIP_EWORKSPACE;
+    const unsigned grid = static_cast<unsigned>(back_blocks(rows, cols));
+    const NormBackArgs a = {h, weight, go, dh, dweight ? workspace : nullptr, rows, cols, eps};
+    const hipStream_t s = as_stream(stream);
+    for_cols(cols, [&](auto w, auto nv, auto long_rows) {
+        launch_back<w.value, nv.value, long_rows.value>(a, grid, s);
+    });
+    if (dweight)
+        launch(sum_parts, dim3(static_cast<unsigned>((cols + 15) / 16)), dim3(kBlock), 0, s,
+               static_cast<const float *>(workspace), static_cast<size_t>(grid), cols, dweight);
+    return launch_status();
+}
+
+}  // extern "C"

@@ -301,6 +301,23 @@ const char *ts_hip_error_string(int status) {
     }
 }
 
+int ts_hip_check_device_range(const void *ptr, size_t bytes) {
+    if (!ptr) return TS_HIP_EINVAL;
+    hipPointerAttribute_t at{};
+    if (hipPointerGetAttributes(&at, ptr) != hipSuccess || at.type != hipMemoryTypeDevice) {
+        (void)hipGetLastError();  // a host pointer is not an error of a later call
+        return TS_HIP_EINVAL;
+    }
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipMemGetAddressRange(&base, &size, const_cast<void *>(ptr)) != hipSuccess) {
+        (void)hipGetLastError();
+        return TS_HIP_EINVAL;
+    }
+    const size_t before = static_cast<size_t>(static_cast<const char *>(ptr) - static_cast<const char *>(base));
+    return before <= size && bytes <= size - before ? TS_HIP_OK : TS_HIP_EINVAL;
+}
+
 int ts_hip_mem_info(size_t *free_bytes, size_t *total_bytes) {
     if (!free_bytes || !total_bytes) return TS_HIP_EINVAL;
     return tship::status_of(hipMemGetInfo(free_bytes, total_bytes));

@@ -8,13 +8,15 @@ panics surface as ``TsError``.
 """
 from __future__ import annotations
 
+import atexit
 import contextlib
 import ctypes
+import itertools
 from typing import Iterable, Optional, Sequence
 
 import numpy as np
 
-from ._ffi import F, SZ, TsError, gradtrack as _G, last_error
+from ._ffi import ACTIVATIONS, F, SZ, TsError, gradtrack as _G, last_error
 
 
 def _dims(shape: Sequence[int]):
@@ -46,6 +48,57 @@ def _take_bytes(call) -> bytes:
 
 def _path(path) -> bytes:
     return str(path).encode()
+
+
+# Objects whose device memory the native library uses, by token: held until its
+# last user there is gone (the library's release call).
+_lent: dict = {}
+_tokens = itertools.count(1)
+
+
+@ctypes.CFUNCTYPE(None, ctypes.c_void_p)
+def _give_back(token):
+    _lent.pop(token, None)
+
+
+atexit.register(_G.ts_external_detach)  # handles that outlive the interpreter make no call into it
+
+
+def _lend(owners) -> int:
+    token = next(_tokens)
+    _lent[token] = owners
+    return token
+
+
+def _device_array(obj, typestr: str):
+    """(address, shape) of an object that exposes contiguous device memory."""
+    try:
+        a = obj.__cuda_array_interface__
+    except (AttributeError, TypeError) as e:
+        raise TsError(f"from_device: {type(obj).__name__} exposes no device memory") from e
+    shape = tuple(int(d) for d in a["shape"])
+    if a["typestr"] != typestr:
+        raise TsError(f"from_device: values of type {a['typestr']}, not {typestr}")
+    strides, step = a.get("strides"), int(typestr[2:])
+    if strides is not None and 0 not in shape:
+        for d, s in zip(reversed(shape), reversed(strides)):
+            if d != 1 and s != step:
+                raise TsError("from_device: the array is not contiguous")
+            step *= d
+    return int(a["data"][0] or 0), shape
+
+
+def _optional(t: Optional["Tensor"]):
+    return t._h if t is not None else None
+
+
+def _activation(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise TsError(f"unknown activation {name!r}: one of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
+
+
+_CHECKPOINTS = {"full": 0, "8bit": 1}
 
 
 class Tensor:
@@ -83,6 +136,17 @@ class Tensor:
         a = np.ascontiguousarray(np.asarray(data, dtype=np.float32).reshape(-1))
         d, r = _dims(shape)
         return _wrap(_G.ts_tensor_from_slice(a.ctypes.data_as(F), a.size, d, r))
+
+    @staticmethod
+    def from_device(array) -> "Tensor":
+        """A tensor over the memory of a contiguous float32 device array (any
+        object with ``__cuda_array_interface__``), not copied; the array is held
+        until the library's last use of it.  What wrote it must have finished,
+        and others may read what the library writes to it only after
+        ``synchronize()`` (or an event on ``stream()``)."""
+        ptr, shape = _device_array(array, "<f4")
+        d, r = _dims(shape)
+        return _wrap(_G.ts_tensor_from_device(ptr, d, r, _give_back, _lend(array)))
 
     @staticmethod
     def randn(shape: Sequence[int], seed: Optional[int] = None) -> "Tensor":
@@ -158,6 +222,42 @@ class Tensor:
 
     def matmul(self, other: "Tensor") -> "Tensor":
         return _wrap(_G.ts_tensor_matmul(self._h, other._h))
+
+    # -- a feed-forward block's operators (include/ts_gradtrack.h) ------------------
+    def rms_norm(self, weight: "Tensor", eps: float = 1e-6) -> "Tensor":
+        """self / sqrt(mean(self^2) + eps) * weight over the last axis."""
+        return _wrap(_G.ts_tensor_rms_norm(self._h, weight._h, eps))
+
+    def add_rms_norm(self, residual: "Tensor", weight: "Tensor", eps: float = 1e-6):
+        """(rms_norm(h), h) of h = self + residual, in one pass."""
+        h = ctypes.c_void_p()
+        y = _wrap(_G.ts_tensor_add_rms_norm(self._h, residual._h, weight._h, eps, ctypes.byref(h)))
+        return y, Tensor(h.value)
+
+    def rms_norm_packed(self, weight: "Tensor", eps: float = 1e-6) -> "Packed8":
+        """rms_norm of a matrix, in 8 bits."""
+        return _wrap_packed(_G.ts_tensor_rms_norm_packed(self._h, None, weight._h, eps, None))
+
+    def add_rms_norm_packed(self, residual: "Tensor", weight: "Tensor", eps: float = 1e-6):
+        """(rms_norm(h) in 8 bits, h) of the matrix h = self + residual, in one pass."""
+        h = ctypes.c_void_p()
+        p = _wrap_packed(_G.ts_tensor_rms_norm_packed(self._h, residual._h, weight._h, eps, ctypes.byref(h)))
+        return p, Tensor(h.value)
+
+    def linear(self, weight: "Tensor", bias: Optional["Tensor"] = None, activation: str = "none",
+               residual: Optional["Tensor"] = None, checkpoint: str = "full") -> "Tensor":
+        """The layer act(self weight + bias) + residual as one op; activation one
+        of none, relu, silu and gelu_tanh.  checkpoint "8bit" keeps the input's
+        values in 8 bits for the backward pass (and nothing else), "full" the
+        input itself and the values before the activation."""
+        if checkpoint not in _CHECKPOINTS:
+            raise TsError(f"unknown checkpoint {checkpoint!r}: one of {', '.join(_CHECKPOINTS)}")
+        return _wrap(_G.ts_tensor_linear(self._h, weight._h, _optional(bias), _activation(activation),
+                                         _optional(residual), _CHECKPOINTS[checkpoint]))
+
+    def pack8(self) -> "Packed8":
+        """The matrix in 8 bits."""
+        return _wrap_packed(_G.ts_tensor_pack8(self._h))
 
     # -- tensor/ops/{exp,log,sqrt,tanh,sigmoid,leaky_relu,softmax}.rs -------------
     def exp(self) -> "Tensor":
@@ -237,6 +337,16 @@ class Tensor:
             return None
         return Tensor(h)
 
+    def grad_view(self) -> Optional["Tensor"]:
+        """What grad_by_value copies, on the gradient's own buffer."""
+        h = _G.ts_tensor_grad_view(self._h)
+        if not h:
+            err = last_error()
+            if err:
+                raise TsError(err)
+            return None
+        return Tensor(h)
+
     def set_grad(self, grad: "Tensor") -> None:
         _ok(_G.ts_tensor_set_grad(self._h, grad._h))
 
@@ -287,6 +397,66 @@ class Tensor:
     @staticmethod
     def load_json(path) -> "Tensor":
         return _wrap(_G.ts_tensor_load_json(_path(path)))
+
+
+def _wrap_packed(handle) -> "Packed8":
+    if not handle:
+        raise TsError(last_error() or "native call returned no packed matrix")
+    return Packed8(handle)
+
+
+class Packed8:
+    """Handle on a matrix in 8 bits: e4m3 codes [rows, pitch] and one
+    power-of-two scale per 32 columns, [pitch / 128, rows, 4] bytes (include/
+    ts_hip.h, ts_hip_pack8)."""
+
+    __slots__ = ("_h",)
+
+    def __init__(self, handle):
+        self._h = ctypes.c_void_p(handle)
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            _G.ts_packed8_free(h)
+            self._h = None
+
+    @staticmethod
+    def from_device(codes, scales, cols: int) -> "Packed8":
+        """Over a caller's uint8 device arrays, codes [rows, pitch] and scales
+        [pitch / 128, rows, 4], as Tensor.from_device."""
+        (cp, cshape), (sp, sshape) = _device_array(codes, "|u1"), _device_array(scales, "|u1")
+        pitch = -(-int(cols) // 128) * 128
+        if cols < 0 or len(cshape) != 2 or cshape[1] != pitch or sshape != (pitch // 128, cshape[0], 4):
+            raise TsError(f"Packed8: codes {list(cshape)} and scales {list(sshape)} for {cols} columns")
+        return _wrap_packed(_G.ts_packed8_from_device(cp, sp, cshape[0], int(cols), _give_back, _lend((codes, scales))))
+
+    @property
+    def shape(self) -> tuple:
+        return int(_G.ts_packed8_rows(self._h)), int(_G.ts_packed8_cols(self._h))
+
+    @property
+    def pitch(self) -> int:
+        return int(_G.ts_packed8_pitch(self._h))
+
+    def codes_ptr(self) -> int:
+        return int(_G.ts_packed8_codes_ptr(self._h) or 0)
+
+    def scales_ptr(self) -> int:
+        return int(_G.ts_packed8_scales_ptr(self._h) or 0)
+
+    def unpack(self) -> Tensor:
+        """The values that the codes stand for."""
+        return _wrap(_G.ts_packed8_unpack(self._h))
+
+    def linear(self, weight: "Packed8", bias: Optional[Tensor] = None, activation: str = "none",
+               residual: Optional[Tensor] = None) -> Tensor:
+        """act(self weight^T + bias) + residual, weight [fan_out, fan_in]."""
+        return _wrap(_G.ts_packed8_linear(self._h, weight._h, _optional(bias), _activation(activation),
+                                          _optional(residual)))
+
+    def __repr__(self) -> str:
+        return f"Packed8(shape={list(self.shape)})"
 
 
 def _handles(params: Iterable[Tensor]):
