@@ -243,6 +243,47 @@ def test_linear(m, k, n, name, bias, residual, checkpoint):
     check_layer(m, k, n, name, bias, residual, checkpoint)
 
 
+# products large enough for the bf16 cores: every one of the three, some of them, odd sizes, k past a block's end
+LARGE = [(1024, 1024, 1024), (1000, 777, 1531), (129, 8000, 1000), (1003, 129, 8191), (5000, 640, 260), (257, 4100, 1025)]
+
+
+@pytest.mark.parametrize("m,k,n", LARGE)
+@pytest.mark.parametrize("name,bias,residual,checkpoint", [("none", False, True, "full"), ("silu", True, False, "8bit"),
+                                                           ("gelu_tanh", True, True, "full"), ("relu", True, False, "8bit")])
+def test_linear_large(m, k, n, name, bias, residual, checkpoint):
+    check_layer(m, k, n, name, bias, residual, checkpoint)
+
+
+def test_linear_large_keeps_small_values_beside_large_ones():
+    """Pieces are exact whatever else a row holds: magnitudes over sixty binades, and the smallest of fp32."""
+    m, k, n = 600, 1100, 1200
+    x, w, b, r, go = layer_case(m, k, n, False, False)
+    rng = np.random.default_rng(1)
+    x = (x * 2.0 ** rng.integers(-30, 31, x.shape)).astype(np.float32)
+    w = (w * 2.0 ** rng.integers(-30, 31, w.shape)).astype(np.float32)
+    x[5] *= np.float32(2.0 ** -100)
+    got = tensor(x).linear(tensor(w)).data()
+    want = R.linear(x, w, None, "none", None)[0]
+    assert_within(got, want, R.product_bound(x, w) + 1e-37, "y")
+
+
+def test_linear_large_with_values_that_are_not_finite():
+    m, k, n = 900, 1030, 1000
+    x, w, b, r, go = layer_case(m, k, n, True, False)
+    x[3, 5], x[300, 1], x[301, 2], x[899, 1029] = np.nan, np.inf, -np.inf, 3e38
+    w[1029] = np.abs(w[1029]) + 2.0  # a sum past fp32's range
+    w[7, 999] = np.inf
+    with np.errstate(invalid="ignore", over="ignore"):
+        want = x.astype(np.float64) @ w.astype(np.float64) + b
+        limit = np.where(np.abs(want) > np.finfo(np.float32).max, np.sign(want) * np.inf, want)
+    got = tensor(x).linear(tensor(w), bias=tensor(b)).data()
+    assert np.array_equal(np.isnan(got), np.isnan(limit))
+    assert np.array_equal(np.isinf(got), np.isinf(limit)) and np.array_equal(got[np.isinf(got)], limit[np.isinf(limit)])
+    fine = np.isfinite(limit)
+    bound = R.product_bound(np.nan_to_num(x, posinf=0, neginf=0), np.nan_to_num(w, posinf=0)) + R.U * np.abs(np.nan_to_num(want))
+    assert np.all(np.abs(got[fine] - want[fine]) <= bound[fine])
+
+
 @pytest.mark.parametrize("checkpoint", ["full", "8bit"])
 def test_linear_gradient_is_the_difference(checkpoint):
     """Along a random direction of every input, by the device's own forward values."""
@@ -359,7 +400,8 @@ def test_linear_with_values_that_are_not_finite():
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 8, 8), (1, 4096, 512), (2, 33, 5), (5, 127, 19), (16, 128, 64), (17, 129, 65),
-                                   (33, 1531, 31), (70, 300, 77), (200, 640, 130)])
+                                   (33, 1531, 31), (70, 300, 77), (200, 640, 130), (1024, 1024, 1024), (1999, 1531, 777),
+                                   (129, 8000, 1000), (5000, 100, 2050)])
 @pytest.mark.parametrize("name,bias,residual", [("none", False, False), ("relu", True, False), ("silu", True, True),
                                                 ("gelu_tanh", False, True)])
 def test_linear_packed(m, k, n, name, bias, residual):
@@ -496,12 +538,13 @@ def test_block_trains_and_replays_as_it_runs():
 
 def test_equal_calls_give_equal_bits():
     outs = []
-    for _ in range(2):
-        x, w, b, r, go = layer_case(150, 260, 190, True, True)
+    for m, k, n in 2 * [(150, 260, 190)] + 2 * [(1100, 1030, 900)]:
+        x, w, b, r, go = layer_case(m, k, n, True, True)
         X, W, B = (tensor(a).with_requires_grad() for a in (x, w, b))
         y = X.linear(W, bias=B, activation="gelu_tanh", residual=tensor(r), checkpoint="8bit")
         y.backward(tensor(go))
         outs.append([y.data()] + [t.grad_by_value().data() for t in (X, W, B)])
         T.clear_gradients()
-    for a, b in zip(*outs):
-        assert np.array_equal(a, b)
+    for first, second in (outs[:2], outs[2:]):
+        for a, b in zip(first, second):
+            assert np.array_equal(a, b)

@@ -1,5 +1,6 @@
-// What a layer's kernels share: activations, the epilogues and the operands as
-// their elements are read one by one.
+// What a layer's kernels share (ts_hip_linear.hip: the entries and the small
+// products; ts_hip_linear_planes.hip: the large ones): activations, the
+// epilogues and the operands as their elements are read one by one.
 #pragma once
 
 #include "ts_hip_pack8.h"
@@ -131,5 +132,22 @@ struct LinearProduct {
     float *C;
     LinearEpi epi;
 };
+
+// ---- the large products (ts_hip_linear_planes.hip) ---------------------------------
+
+// What the pass over an operand does beside its planes.
+struct PlanesExtra {
+    // A along k: its values in 8 bits as well
+    uint8_t *codes = nullptr, *scales = nullptr;
+    // B along its rows: its rows' sums over k into `sums`, by planes_sum_floats(N, K) of `sum_parts`
+    float *sums = nullptr, *sum_parts = nullptr;
+};
+
+bool planes_take(size_t M, size_t N, size_t K);
+size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b);
+size_t planes_sum_floats(size_t N, size_t K);
+int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s);
+// A and B codes along k
+int planes_packed_product(const LinearProduct &p, float *workspace, hipStream_t s);
 
 }  // namespace tship

@@ -1,102 +1,10 @@
 // A layer's forward and backward (ts_hip.h, ts_hip_linear and the entries after
-// it) and the kernels of its small products.
-//
-// Small products (linear_direct).  A wave computes 32 x 32 of C in blocks of
-// v_mfma_f32_16x16x4_f32, its operands straight from memory to registers: a
-// lane takes four k of a row (k 4 q + s of 16 in step s, the same for both
-// operands), so what lies along k comes in 16-byte loads.  Nothing is staged:
-// such a call is a launch and a few waits for memory, and a stage's barrier
-// would be one more.  The waves of a workgroup take equal parts of K and their
-// sums are added in order through LDS: few tiles have a long way each.
-#include "ts_hip_linear.h"
+// it) and the launches of its small products.
+#include "ts_hip_linear_direct.h"
 
 namespace tship {
 
 namespace {
-
-constexpr int kDirectTile = 32;
-constexpr int kDirectK = 16;
-
-// A small product and the layout of its grid.
-struct DirectProduct {
-    Operand A, B;
-    float *C;
-    LinearEpi epi;
-    int M, N, K, tiles_n, tiles;
-};
-
-template <Src SA, Src SB, int KG>
-__device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, float *lds) {
-    const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
-    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
-    f4v_t acc[2][2] = {};
-    int ra[2], rb[2];  // rows past an edge read the last one and are not stored
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        ra[x] = min(i0 + 16 * x + li, p.M - 1);
-        rb[x] = min(j0 + 16 * x + li, p.N - 1);
-    }
-    const int steps = (p.K + kDirectK - 1) / kDirectK, per = (steps + KG - 1) / KG;
-    const int from = group * per, to = min(from + per, steps);
-    constexpr int U = 4;  // steps whose loads are issued before the first is used
-    for (int s0 = from; s0 < to; s0 += U) {
-        float a[U][2][4], b[U][2][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = (s0 + u) * kDirectK + 4 * lq, K = s0 + u < to ? p.K : 0;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                operand4<SA>(p.A, ra[x], k, K, a[u][x]);
-                operand4<SB>(p.B, rb[x], k, K, b[u][x]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][x][s], b[u][c][s], acc[x][c], 0, 0, 0);
-    }
-    // lane (li, lq), register r of block (x, c): row 16 x + 4 lq + r, column 16 c + li
-    if constexpr (KG == 1) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int j = j0 + 16 * c + li;
-            if (j >= p.N) continue;
-            const float bias = p.epi.bias ? p.epi.bias[j] : 0.0f;
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = i0 + 16 * x + 4 * lq + r;
-                    if (i < p.M) epilogue_store(p.epi, p.C, static_cast<size_t>(i) * p.N + j, acc[x][c][r], bias);
-                }
-        }
-    } else {
-        // the groups' sums by LDS, [group][row][column]; the workgroup then adds
-        // and stores whole rows
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    lds[(group * kDirectTile + 16 * x + 4 * lq + r) * kDirectTile + 16 * c + li] = acc[x][c][r];
-        __syncthreads();
-        for (int n = threadIdx.x; n < kDirectTile * kDirectTile; n += 64 * KG) {
-            const int i = i0 + n / kDirectTile, j = j0 + n % kDirectTile;
-            float v = lds[n];
-#pragma unroll
-            for (int g = 1; g < KG; ++g) v += lds[g * kDirectTile * kDirectTile + n];
-            if (i < p.M && j < p.N)
-                epilogue_store(p.epi, p.C, static_cast<size_t>(i) * p.N + j, v, p.epi.bias ? p.epi.bias[j] : 0.0f);
-        }
-    }
-}
 
 // Work beside a product in its launch: the packing of x (forward)...
 struct PackJob {
@@ -181,11 +89,6 @@ __global__ __launch_bounds__(kBlock) void linear_dz(const float *__restrict__ z,
     }
 }
 
-DirectProduct direct_product(const LinearProduct &p) {
-    const int tm = (p.M + kDirectTile - 1) / kDirectTile, tn = (p.N + kDirectTile - 1) / kDirectTile;
-    return {p.A, p.B, p.C, p.epi, p.M, p.N, p.K, tn, tm * tn};
-}
-
 // Waves that share a tile's K: as many as bring the launch to four waves a
 // SIMD, while each has two rounds of loads of its own.
 int direct_groups(size_t tiles, size_t K) {
@@ -263,6 +166,30 @@ LinearProduct dw_product(const ts_hip_linear_shape &s, const float *x, const uin
     return p;
 }
 
+// The backward pass's workspace, in floats: dz, the parts of its column sums and
+// the planes of one product after another.
+struct BackLayout {
+    size_t parts, planes, total;
+};
+BackLayout back_layout(const ts_hip_linear_shape &s) {
+    BackLayout l{};
+    auto round = [](size_t n) { return (n + 63) / 64 * 64; };
+    l.parts = round(s.batch * s.fan_out);
+    l.planes = l.parts;
+    size_t most = 0;
+    auto product = [&](size_t M, size_t N, size_t K, Src a, Src b) {
+        if (!planes_take(M, N, K)) return;
+        const size_t n = planes_workspace_floats(M, N, K, a, b);
+        most = n > most ? n : most;
+    };
+    product(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR);
+    product(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK);
+    product(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR);
+    if (planes_take(s.fan_in, s.fan_out, s.batch)) l.planes += round(planes_sum_floats(s.fan_out, s.batch));
+    l.total = l.planes + most;
+    return l;
+}
+
 bool shape_ok(const ts_hip_linear_shape *s) {
     const size_t lim = size_t(1) << 24;  // row and column numbers stay far inside 32 bits
     if (!s || s->batch >= lim || s->fan_in >= lim || s->fan_out >= lim) return false;
@@ -280,8 +207,11 @@ using namespace tship;
 extern "C" {
 
 size_t ts_hip_linear_workspace_floats(const ts_hip_linear_shape *shape) {
-    (void)shape;
-    return 0;
+    if (!shape_ok(shape)) return 0;
+    const ts_hip_linear_shape &d = *shape;
+    return planes_take(d.batch, d.fan_out, d.fan_in)
+               ? planes_workspace_floats(d.batch, d.fan_out, d.fan_in, Src::kFloatK, Src::kFloatR)
+               : 0;
 }
 
 int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float *weight, const float *bias, int act,
@@ -296,7 +226,13 @@ int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float 
     if (!y || (d.fan_in && (!x || !weight))) return TS_HIP_EINVAL;
     const hipStream_t s = as_stream(stream);
     const LinearProduct p = forward_product(d, x, nullptr, nullptr, weight, y, {bias, residual, nullptr, z, act});
-    (void)workspace;
+    if (planes_take(d.batch, d.fan_out, d.fan_in)) {
+        if (!workspace) return TS_HIP_EINVAL;
+        PlanesExtra extra;
+        extra.codes = codes;
+        extra.scales = scales;
+        return planes_product(p, extra, workspace, s);
+    }
     const DirectProduct g = direct_product(p);
     with_groups(direct_groups(g.tiles, p.K), [&](auto kg) {
         const PackJob pack = pack_work(x, codes, scales, d.batch, d.fan_in, 64 * kg.value);
@@ -307,7 +243,7 @@ int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float 
 }
 
 size_t ts_hip_linear_backward_workspace_floats(const ts_hip_linear_shape *shape) {
-    return shape ? shape->batch * shape->fan_out + 64 : 0;
+    return shape_ok(shape) ? back_layout(*shape).total : 0;
 }
 
 int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, const uint8_t *codes,
@@ -330,6 +266,8 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
     }
     if (!dx && !dweight && !dbias) return TS_HIP_OK;
     if (!go || !workspace) return TS_HIP_EINVAL;
+    const BackLayout at = back_layout(d);
+    float *const planes = workspace + at.planes;
     const float *dz = go;
     if (act != TS_HIP_ACT_NONE) {
         if (z || d.fan_in == 0) {
@@ -340,21 +278,42 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
             if (!codes || !weight) return TS_HIP_EINVAL;
             const LinearProduct p =
                 forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
-            const DirectProduct g = direct_product(p);
-            with_groups(direct_groups(g.tiles, p.K), [&](auto kg) {
-                launch((linear_direct<Src::kCodesK, Src::kFloatR, kg.value>), dim3(g.tiles), dim3(64 * kg.value), 0, s, g,
-                       PackJob{});
-            });
+            if (planes_take(d.batch, d.fan_out, d.fan_in)) {
+                st = planes_product(p, {}, planes, s);
+                if (st) return st;
+            } else {
+                const DirectProduct g = direct_product(p);
+                with_groups(direct_groups(g.tiles, p.K), [&](auto kg) {
+                    launch((linear_direct<Src::kCodesK, Src::kFloatR, kg.value>), dim3(g.tiles), dim3(64 * kg.value), 0, s,
+                           g, PackJob{});
+                });
+            }
         }
         dz = workspace;
     }
     if ((dx && !weight) || (dweight && !codes && !x)) return TS_HIP_EINVAL;
     DirectProduct gx{}, gw{};
-    if (dx) gx = direct_product(dx_product(d, dz, weight, dx));
-    if (dweight) gw = direct_product(dw_product(d, x, codes, scales, dz, dweight));
+    if (dx) {
+        const LinearProduct p = dx_product(d, dz, weight, dx);
+        if (planes_take(p.M, p.N, p.K)) st = planes_product(p, {}, planes, s);
+        else gx = direct_product(p);
+    }
+    if (dweight && !st) {
+        const LinearProduct p = dw_product(d, x, codes, scales, dz, dweight);
+        if (planes_take(p.M, p.N, p.K)) {
+            PlanesExtra extra;
+            extra.sums = dbias;  // dz is passed over for its planes anyway
+            extra.sum_parts = workspace + at.parts;
+            st = planes_product(p, extra, planes, s);
+            dbias = nullptr;
+        } else {
+            gw = direct_product(p);
+        }
+    }
+    if (st || (!gx.tiles && !gw.tiles && !dbias)) return st ? st : launch_status();
     SumJob sum = {dz, dbias, static_cast<int>(d.batch), static_cast<int>(d.fan_out),
                   dbias ? static_cast<int>((d.fan_out + 15) / 16) : 0};
-    const size_t K = dweight ? d.batch : d.fan_out;
+    const size_t K = gw.tiles ? d.batch : d.fan_out;
     with_groups(direct_groups(static_cast<size_t>(gx.tiles) + gw.tiles, K), [&](auto kg) {
         const dim3 grid(gx.tiles + gw.tiles + sum.blocks), block(64 * kg.value);
         if (codes) launch((linear_direct_back<Src::kCodesR, kg.value>), grid, block, 0, s, gx, gw, sum);

@@ -20,8 +20,6 @@ namespace tship {
 
 namespace {
 
-typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
 
 struct PackedProduct {
@@ -31,19 +29,6 @@ struct PackedProduct {
     int M, N, groups, act;  // groups of 128 k
     int tiles_n;
 };
-
-// eight codes (two words) and their scale as bf16
-__device__ __forceinline__ bf8_t widen(unsigned lo, unsigned hi, float scale) {
-    union {
-        bf8_t v;
-        bf2_t p[4];
-    } u;
-    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
-    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
-    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-    return u.v;
-}
 
 // FN blocks of 16 columns, FM of 16 rows a wave; KG waves share K.
 template <int FN, int FM, int KG>
@@ -194,10 +179,9 @@ using namespace tship;
 extern "C" {
 
 size_t ts_hip_linear_packed_workspace_floats(size_t batch, size_t fan_in, size_t fan_out) {
-    (void)batch;
-    (void)fan_in;
-    (void)fan_out;
-    return 0;
+    return planes_take(batch, fan_out, fan_in)
+               ? planes_workspace_floats(batch, fan_out, fan_in, Src::kCodesK, Src::kCodesK)
+               : 0;
 }
 
 int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const uint8_t *w_codes,
@@ -210,7 +194,19 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
     if (batch == 0 || fan_out == 0) return TS_HIP_OK;
     if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;
     if (workspace_floats < ts_hip_linear_packed_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
-    (void)workspace;
+    if (planes_take(batch, fan_out, fan_in)) {
+        if (!workspace) return TS_HIP_EINVAL;
+        LinearProduct q{};
+        q.A = {nullptr, x_codes, x_scales, 0, static_cast<int>(batch), packed_pitch(fan_in), batch};
+        q.B = {nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), packed_pitch(fan_in), fan_out};
+        q.a = q.b = Src::kCodesK;
+        q.M = static_cast<int>(batch);
+        q.N = static_cast<int>(fan_out);
+        q.K = static_cast<int>(fan_in);
+        q.C = y;
+        q.epi = {bias, residual, nullptr, nullptr, act};
+        return planes_packed_product(q, workspace, as_stream(stream));
+    }
     const PackedProduct p = {x_codes, x_scales, w_codes, w_scales, bias, residual, y, static_cast<int>(batch),
                              static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0};
     if (batch <= 16) launch_packed<1, 1>(p, as_stream(stream));

@@ -1,0 +1,337 @@
+// The passes that write an operand's planes and the launches of the large
+// products (the kernel and the layout: ts_hip_linear_planes.h).
+#include "ts_hip_linear_direct.h"
+#include "ts_hip_linear_planes.h"
+#include "ts_hip_parts.h"
+
+namespace tship {
+
+namespace {
+
+typedef unsigned u4p_t __attribute__((ext_vector_type(4)));
+
+// eight values times scale as their three pieces, a lane's 16 bytes of each
+__device__ __forceinline__ void store_pieces(char *to, const float (&v)[8], float scale, int lane) {
+    u4p_t h, m, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const Pieces p = split2(v[2 * e], v[2 * e + 1], scale);
+        h[e] = p.h;
+        m[e] = p.m;
+        l[e] = p.l;
+    }
+    u4p_t *q = reinterpret_cast<u4p_t *>(to) + lane;
+    q[0] = h;
+    q[kFragBytes / 16] = m;
+    q[2 * kFragBytes / 16] = l;
+}
+
+// ---- floats along k ----------------------------------------------------------------
+// A wave takes a row block and eight k blocks (512 bytes of each row).  NEG: odd k
+// blocks negated.  PACK: the values in 8 bits too; a block of 32 k is two k blocks
+// of the lane and its partner in the other half.
+constexpr int kAlongBlocks = 8;
+
+template <bool NEG, bool PACK>
+__global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__ x, int ld, int rows, int K, int kb,
+                                                       char *__restrict__ out, uint8_t *__restrict__ codes,
+                                                       uint8_t *__restrict__ scales, size_t pitch, int chunks) {
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
+    const int rb = static_cast<int>(job / chunks), b0 = static_cast<int>(job % chunks) * kAlongBlocks;
+    if (rb * kPlaneRows >= rows) return;
+    const int row = rb * kPlaneRows + i;
+    const bool live = row < rows;
+    const float *p = x + static_cast<size_t>(live ? row : 0) * ld;
+    float v[kAlongBlocks][8];
+#pragma unroll
+    for (int b = 0; b < kAlongBlocks; ++b)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int k = (b0 + b) * kPlaneK + 8 * h + 4 * q;
+            float w[4] = {};
+            if (live && k + 4 <= K) {
+                const pk4u_t t = *reinterpret_cast<const pk4u_t *>(p + k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = t[e];
+            } else if (live) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? p[k + e] : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[b][4 * q + e] = w[e];
+        }
+#pragma unroll
+    for (int b = 0; b < kAlongBlocks; ++b) {
+        if (b0 + b >= kb) break;  // uniform
+        store_pieces(out + (static_cast<size_t>(rb) * kb + b0 + b) * 3 * kFragBytes, v[b],
+                     NEG && (b & 1) ? -kSplitScale : kSplitScale, lane);
+    }
+    if (PACK) {
+#pragma unroll
+        for (int b = 0; b < kAlongBlocks; b += 2) {
+            const size_t c = static_cast<size_t>(b0 + b) * kPlaneK;
+            if (c >= pitch) break;  // uniform
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(v[b][e]), fabsf(v[b + 1][e])));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            if (!live) continue;
+            const int k = pack_exponent(m);
+            const float inv = pow2f(-k);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float lo[4], hi[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    lo[e] = v[b + t][e];
+                    hi[e] = v[b + t][4 + e];
+                }
+                *reinterpret_cast<u2v_t *>(codes + row * pitch + c + t * kPlaneK + 8 * h) = u2v_t{pack4(lo, inv), pack4(hi, inv)};
+            }
+            if (h == 0)
+                scales[(c / kPackGroup * rows + row) * 4 + c / kPackBlock % 4] = static_cast<uint8_t>(k + kPackBias);
+        }
+    }
+}
+
+// ---- floats along the rows -----------------------------------------------------------
+// element (row, k) at x[k * ld + row].  A wave takes a row block and `run` k
+// blocks.  SUM: the rows' sums over them (f64) to part[chunk][rows].
+template <bool NEG, bool SUM>
+__global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict__ x, int ld, int rows, int K, int kb,
+                                                        char *__restrict__ out, float *__restrict__ part, int run,
+                                                        int row_blocks) {
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
+    const int rb = static_cast<int>(job % row_blocks), chunk = static_cast<int>(job / row_blocks);
+    const int from = chunk * run, to = min(from + run, kb);
+    if (from >= kb) return;
+    const int row = rb * kPlaneRows + i;
+    const bool live = row < rows;
+    const float *p = x + (live ? row : 0);
+    double sum = 0.0;
+#pragma unroll 2
+    for (int b = from; b < to; ++b) {
+        const int k = b * kPlaneK + 8 * h;
+        float v[8];
+        if ((b + 1) * kPlaneK <= K) {  // uniform
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = p[static_cast<size_t>(k + e) * ld];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? p[static_cast<size_t>(k + e) * ld] : 0.0f;
+        }
+        if (!live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        }
+        if (SUM) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += v[e];
+        }
+        store_pieces(out + (static_cast<size_t>(rb) * kb + b) * 3 * kFragBytes, v, NEG && (b & 1) ? -kSplitScale : kSplitScale,
+                     lane);
+    }
+    if (SUM) {
+        sum += __shfl_xor(sum, 32, 64);
+        if (h == 0 && live) part[static_cast<size_t>(chunk) * rows + row] = static_cast<float>(sum);
+    }
+}
+
+// ---- codes -----------------------------------------------------------------------------
+
+// Codes along k.  A wave takes a row block and a group of 128 k, the lane's scales in one word.
+__global__ __launch_bounds__(kBlock) void planes_codes_along(const uint8_t *__restrict__ codes,
+                                                             const uint8_t *__restrict__ scales, int rows, size_t pitch,
+                                                             int kb, char *__restrict__ out) {
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+    const int groups = static_cast<int>(pitch / kPackGroup);
+    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
+    const int rb = static_cast<int>(job / groups), g = static_cast<int>(job % groups);
+    if (rb * kPlaneRows >= rows) return;
+    const int row = rb * kPlaneRows + i;
+    const bool live = row < rows;
+    const size_t r = live ? row : 0;
+    const unsigned four = reinterpret_cast<const unsigned *>(scales)[static_cast<size_t>(g) * rows + r];
+    u2v_t c[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b)
+        c[b] = *reinterpret_cast<const u2v_t *>(codes + r * pitch + static_cast<size_t>(g) * kPackGroup + b * kPlaneK + 8 * h);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        if (g * 8 + b >= kb) break;  // uniform
+        bf8_t w = widen(c[b][0], c[b][1], pow2f(static_cast<int>(four >> (8 * (b / 2)) & 255u) - kPackBias));
+        if (!live) w = bf8_t{};
+        *(reinterpret_cast<bf8_t *>(out + (static_cast<size_t>(rb) * kb + g * 8 + b) * kFragBytes) + lane) = w;
+    }
+}
+
+// Codes along the rows: k is the code row, the product's rows its columns.  A wave
+// takes 32 columns (a row block, and a scale's block) of 64 code rows; a lane four
+// columns of eight.
+__global__ __launch_bounds__(kBlock) void planes_codes_across(const uint8_t *__restrict__ codes,
+                                                              const uint8_t *__restrict__ scales, int code_rows,
+                                                              size_t pitch, int kb, int row_blocks, char *__restrict__ out) {
+    const int lane = threadIdx.x & 63, i = lane & 7, o = lane >> 3;
+    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
+    const int rb = static_cast<int>(job % row_blocks), b0 = static_cast<int>(job / row_blocks) * 4;
+    if (b0 >= kb) return;
+    const int k0 = b0 * kPlaneK + 8 * o;
+    const size_t col = static_cast<size_t>(rb) * kPlaneRows;
+    const uint8_t *sp = scales + (col / kPackGroup * code_rows) * 4 + col / kPackBlock % 4;
+    unsigned c[8];
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // rows past the end: the last one's scale, codes of zero
+        const size_t k = min(k0 + e, code_rows - 1);
+        c[e] = *reinterpret_cast<const unsigned *>(codes + k * pitch + col + 4 * i);
+        if (k0 + e >= code_rows) c[e] = 0;
+        s[e] = pow2f(static_cast<int>(sp[4 * k]) - kPackBias);
+    }
+    const int b = b0 + (o >> 1), h = o & 1;
+    if (b >= kb) return;
+    bf2_t lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        lo[e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s[e], false);
+        hi[e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s[e], true);
+    }
+    bf8_t *to = reinterpret_cast<bf8_t *>(out + (static_cast<size_t>(rb) * kb + b) * kFragBytes) + 32 * h + 4 * i;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        bf8_t w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = n < 2 ? lo[e][n & 1] : hi[e][n & 1];
+        to[n] = w;
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------
+
+int row_blocks(size_t rows) { return static_cast<int>((rows + kPlaneRows - 1) / kPlaneRows); }
+int k_blocks(size_t K) { return static_cast<int>((K + 2 * kPlaneK - 1) / (2 * kPlaneK)) * 2; }
+bool coded(Src s) { return s == Src::kCodesK || s == Src::kCodesR; }
+size_t plane_bytes(size_t rows, size_t K, Src s) {
+    return static_cast<size_t>(row_blocks(rows)) * k_blocks(K) * (coded(s) ? 1 : 3) * kFragBytes;
+}
+
+unsigned wave_grid(size_t jobs) { return static_cast<unsigned>((jobs + kBlock / 64 - 1) / (kBlock / 64)); }
+
+// k blocks a wave of planes_across takes: as many as leave eight waves a SIMD
+int across_run(size_t rows, size_t K) {
+    const size_t waves = static_cast<size_t>(device_cu_count()) * 32, all = static_cast<size_t>(row_blocks(rows)) * k_blocks(K);
+    const size_t run = all / waves;
+    return static_cast<int>(run < 2 ? 2 : run > 16 ? 16 : run);
+}
+int across_chunks(size_t rows, size_t K) {
+    const int run = across_run(rows, K);
+    return (k_blocks(K) + run - 1) / run;
+}
+
+void write_planes(const Operand &o, Src src, int K, bool negate, char *out, const PlanesExtra &x, hipStream_t s) {
+    const int rows = o.rows, kb = k_blocks(K), rb = row_blocks(rows);
+    const dim3 block(kBlock);
+    if (src == Src::kFloatK) {
+        const size_t pitch = packed_pitch(K);
+        const int blocks = x.codes ? static_cast<int>(pitch / kPlaneK) : kb;
+        const int chunks = (blocks + kAlongBlocks - 1) / kAlongBlocks;
+        const dim3 grid(wave_grid(static_cast<size_t>(rb) * chunks));
+        if (x.codes) launch((planes_along<true, true>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
+        else if (negate) launch((planes_along<true, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
+        else launch((planes_along<false, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
+    } else if (src == Src::kFloatR) {
+        const int run = across_run(rows, K), chunks = across_chunks(rows, K);
+        const dim3 grid(wave_grid(static_cast<size_t>(rb) * chunks));
+        if (x.sums) {
+            launch((planes_across<false, true>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
+            launch(sum_parts, dim3((rows + 15) / 16), block, 0, s, static_cast<const float *>(x.sum_parts),
+                   static_cast<size_t>(chunks), static_cast<size_t>(rows), x.sums);
+        } else if (negate) {
+            launch((planes_across<true, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
+        } else {
+            launch((planes_across<false, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
+        }
+    } else if (src == Src::kCodesK) {
+        launch(planes_codes_along, dim3(wave_grid(static_cast<size_t>(rb) * (o.pitch / kPackGroup))), block, 0, s, o.codes,
+               o.scales, rows, o.pitch, kb, out);
+    } else {
+        launch(planes_codes_across, dim3(wave_grid(static_cast<size_t>(rb) * ((kb + 3) / 4))), block, 0, s, o.codes, o.scales,
+               static_cast<int>(o.code_rows), o.pitch, kb, rb, out);
+    }
+}
+
+// The tiles that were marked once more, in fp32.
+template <Src SA, Src SB>
+__global__ __launch_bounds__(64) void planes_again(DirectProduct p, const int *marks, int bm, int bn, int tiles_n) {
+    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+        const int i0 = t / p.tiles_n * kDirectTile, j0 = t % p.tiles_n * kDirectTile;
+        if (marks[i0 / bm * tiles_n + j0 / bn]) direct_tile<SA, SB, 1>(p, t, nullptr);  // uniform
+    }
+}
+
+__global__ __launch_bounds__(kBlock) void clear_marks(int *marks, int n) {
+    for (int i = blockIdx.x * kBlock + threadIdx.x; i < n; i += gridDim.x * kBlock) marks[i] = 0;
+}
+
+template <int BM, int BN, int WM, int WN, int PA, int PB, int SK, int NST>
+void launch_planes(PlanesArgs g, hipStream_t s) {
+    g.tiles_m = (g.M + BM - 1) / BM;
+    g.tiles_n = (g.N + BN - 1) / BN;
+    if (g.marks) launch(clear_marks, dim3(1), dim3(kBlock), 0, s, g.marks, g.tiles_m * g.tiles_n);
+    launch((linear_planes<BM, BN, WM, WN, PA, PB, SK, NST>), dim3(g.tiles_m * g.tiles_n), dim3(64 * WM * WN), 0, s, g);
+}
+
+size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+constexpr int kMarkTile = 128;  // the smallest tile
+
+}  // namespace
+
+bool planes_take(size_t M, size_t N, size_t K) { return 2.0 * M * N * K >= 1.5e9 && M >= 128 && N >= 128 && K >= 64; }
+
+size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b) {
+    const size_t marks = ((M + kMarkTile - 1) / kMarkTile) * ((N + kMarkTile - 1) / kMarkTile) * sizeof(int);
+    return (round_256(plane_bytes(M, K, a)) + round_256(plane_bytes(N, K, b)) + round_256(marks)) / sizeof(float);
+}
+
+size_t planes_sum_floats(size_t N, size_t K) { return static_cast<size_t>(across_chunks(N, K)) * N; }
+
+int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s) {
+    char *pa = reinterpret_cast<char *>(workspace);
+    char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
+    int *marks = reinterpret_cast<int *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
+    const bool pieces = !coded(p.a);
+    PlanesExtra of_a, of_b;
+    of_a.codes = extra.codes;
+    of_a.scales = extra.scales;
+    of_b.sums = extra.sums;
+    of_b.sum_parts = extra.sum_parts;
+    write_planes(p.A, p.a, p.K, pieces, pa, of_a, s);
+    write_planes(p.B, p.b, p.K, false, pb, of_b, s);
+    PlanesArgs g = {pa, pb, p.C, p.epi, p.M, p.N, k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, marks};
+    if (pieces) launch_planes<128, 128, 2, 2, 3, 3, 1, 3>(g, s);
+    else launch_planes<128, 128, 2, 2, 1, 3, 1, 4>(g, s);
+    const DirectProduct d = direct_product(p);
+    const int cap = device_cu_count() * 4;
+    const dim3 grid(d.tiles < cap ? d.tiles : cap);
+    const int tiles_n = (p.N + kMarkTile - 1) / kMarkTile;
+    const int *m = marks;
+    auto again = [&](auto a, auto b) {
+        launch((planes_again<a.value, b.value>), grid, dim3(64), 0, s, d, m, kMarkTile, kMarkTile, tiles_n);
+    };
+    with_sources(p.a, p.b, again);
+    return launch_status();
+}
+
+int planes_packed_product(const LinearProduct &p, float *workspace, hipStream_t s) {
+    char *pa = reinterpret_cast<char *>(workspace);
+    char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
+    write_planes(p.A, p.a, p.K, false, pa, {}, s);
+    write_planes(p.B, p.b, p.K, false, pb, {}, s);
+    PlanesArgs g = {pa, pb, p.C, p.epi, p.M, p.N, k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, nullptr};
+    launch_planes<128, 128, 2, 2, 1, 1, 2, 4>(g, s);
+    return launch_status();
+}
+
+}  // namespace tship

@@ -10,6 +10,7 @@
 // h^2's and g h's row sums only, and takes both in the same pass: nothing but h
 // is kept from the forward.
 #include "ts_hip_pack8.h"
+#include "ts_hip_parts.h"
 
 namespace tship {
 
@@ -261,26 +262,6 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
             for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw[i][e]);
             if (c < a.cols) store4(part, c, a.cols, o);
         }
-    }
-}
-
-// out[c] = the parts' sum over g, f64: 16 columns a workgroup, 16 groups of parts
-__global__ __launch_bounds__(kBlock) void sum_parts(const float *__restrict__ part, size_t parts, size_t cols,
-                                                    float *__restrict__ out) {
-    __shared__ double lds[16][17];
-    const int j = threadIdx.x & 15, q = threadIdx.x >> 4;
-    const size_t c = static_cast<size_t>(blockIdx.x) * 16 + j;
-    double s = 0.0;
-    if (c < cols) {
-#pragma unroll 8
-        for (size_t g = q; g < parts; g += 16) s += part[g * cols + c];
-    }
-    lds[q][j] = s;
-    __syncthreads();
-    if (q == 0 && c < cols) {
-#pragma unroll
-        for (int k = 1; k < 16; ++k) s += lds[k][j];
-        out[c] = static_cast<float>(s);
     }
 }
 

@@ -67,6 +67,22 @@ __device__ __forceinline__ void unpack4(unsigned code, uint8_t scale, float (&v)
     v[3] = hi[1] * k;
 }
 
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+
+// eight codes (two words) and their scale as bf16
+__device__ __forceinline__ bf8_t widen(unsigned lo, unsigned hi, float scale) {
+    union {
+        bf8_t v;
+        bf2_t p[4];
+    } u;
+    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return u.v;
+}
+
 // Packs four columns c .. c + 3 of a row (past cols: zeros in v); the eight
 // lanes of a block of 32 call together.  scales points at the row's entry of
 // group 0, groups scale_step bytes apart.
