@@ -147,7 +147,5 @@ bool planes_take(size_t M, size_t N, size_t K);
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b);
 size_t planes_sum_floats(size_t N, size_t K);
 int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s);
-// A and B codes along k
-int planes_packed_product(const LinearProduct &p, float *workspace, hipStream_t s);
 
 }  // namespace tship

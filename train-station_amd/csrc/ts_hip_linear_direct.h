@@ -26,10 +26,11 @@ struct DirectProduct {
     int M, N, K, tiles_n, tiles;
 };
 
+// KG waves share the tile (1: any wave by itself).
 template <Src SA, Src SB, int KG>
 __device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, float *lds) {
     const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
-    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
     f4v_t acc[2][2] = {};
     int ra[2], rb[2];  // rows past an edge read the last one and are not stored
@@ -112,6 +113,8 @@ void with_sources(Src a, Src b, F &&f) {
     if (a == Src::kFloatK && b == Src::kFloatR) f(K{}, R{});       // x W
     else if (a == Src::kFloatK) f(K{}, K{});                       // dz W^T
     else if (a == Src::kFloatR) f(R{}, R{});                       // x^T dz
+    else if (a == Src::kCodesK && b == Src::kCodesK)
+        f(std::integral_constant<Src, Src::kCodesK>{}, std::integral_constant<Src, Src::kCodesK>{});
     else if (a == Src::kCodesK) f(std::integral_constant<Src, Src::kCodesK>{}, R{});
     else f(std::integral_constant<Src, Src::kCodesR>{}, R{});
 }

@@ -195,7 +195,6 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
     if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;
     if (workspace_floats < ts_hip_linear_packed_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
     if (planes_take(batch, fan_out, fan_in)) {
-        if (!workspace) return TS_HIP_EINVAL;
         LinearProduct q{};
         q.A = {nullptr, x_codes, x_scales, 0, static_cast<int>(batch), packed_pitch(fan_in), batch};
         q.B = {nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), packed_pitch(fan_in), fan_out};
@@ -205,7 +204,7 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
         q.K = static_cast<int>(fan_in);
         q.C = y;
         q.epi = {bias, residual, nullptr, nullptr, act};
-        return planes_packed_product(q, workspace, as_stream(stream));
+        return planes_product(q, {}, workspace, as_stream(stream));
     }
     const PackedProduct p = {x_codes, x_scales, w_codes, w_scales, bias, residual, y, static_cast<int>(batch),
                              static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0};

@@ -2,17 +2,24 @@
 // lay its operands out and the launches: ts_hip_linear_planes.hip).
 //
 // Planes.  An operand is first rewritten into what the instruction reads: its
-// values as bf16 pieces (P = 3: the exact pieces h, m, l of ts_hip_gemm_split.h,
-// times 2^16; P = 1: values of 8 bits, which are bf16 numbers as they are), in
-// fragments of 32 rows and 16 k:
-//   planes [row blocks][k blocks][P] x 1024 bytes, a fragment 64 lanes x 16 bytes,
-//   lane 32 h + i holding k 8 h .. 8 h + 7 of row i,
+// values as the exact bf16 pieces h, m, l of ts_hip_gemm_split.h, times 2^16 (or,
+// where they are 8-bit values, as the one bf16 number they are), in fragments of
+// 32 rows and 16 k:
+//   planes [row blocks][k blocks][pieces] x 1024 bytes, a fragment 64 lanes x 16
+//   bytes, lane 32 h + i holding k 8 h .. 8 h + 7 of row i,
 // padded with zeros to whole row blocks and to an even number of k blocks.  The
 // product's loop is then nothing but 16-byte DMA from memory to LDS, fragment
 // reads in lane order (no bank conflict, no address but the lane's) and matrix
 // instructions: no edge, no transpose, no splitting, whatever the layout of the
-// operands was.  The rewriting costs a pass over each operand (10 % of a product
+// operands was.  The rewriting costs a pass over each operand (7 % of a product
 // of 8192 x 4096 x 4096).
+//
+// Codes along k on both sides need no pass: they go to LDS as they are, half the
+// bytes of bf16, and a fragment's eight are widened with their scale as they are
+// read, an instruction for two.  8192 x 4096 x 4096: 260 us, against 261 and 38 for
+// the passes from planes, whose LDS reads, 128 bytes a clock, are the bound.  Beside
+// three pieces on the other side codes are widened by a pass all the same: 598 and
+// 27 us, against 766 with the widening between the matrix instructions.
 //
 // Products.  With pieces on both sides the six of ts_hip_gemm_split.h, summed from
 // zero per 16 k and joined by the vector units, every second k block of A
@@ -20,36 +27,81 @@
 // summed in the accumulators.
 //
 // Finite.  A sum that is not finite comes from an operand that is not, a value past
-// 2^111 or a sum past 2^95; its tile is marked and computed again on the fp32
-// instructions by a launch that otherwise finds nothing to do.
+// 2^111 or a sum past 2^95; its tile is computed again from the operands
+// themselves on the fp32 instructions (direct_tile).
 #pragma once
 
 #include "ts_hip_gemm_split.h"
-#include "ts_hip_linear.h"
+#include "ts_hip_linear_direct.h"
 
 namespace tship {
+
+constexpr bool of_codes(Src s) { return s == Src::kCodesK || s == Src::kCodesR; }
+constexpr int pieces_of(Src s) { return of_codes(s) ? 1 : 3; }
+constexpr bool as_codes(Src a, Src b) { return a == Src::kCodesK && b == Src::kCodesK; }  // read as codes, not from planes
 
 constexpr int kPlaneRows = 32, kPlaneK = 16, kFragBytes = 1024;
 
 struct PlanesArgs {
     const char *A, *B;  // planes
-    float *C;
-    LinearEpi epi;
-    int M, N;
-    int kb;              // k blocks (even)
+    DirectProduct p;     // the product itself (its tiles: 32 x 32)
+    int kb;              // k blocks of the planes (even)
     int rows_a, rows_b;  // row blocks
+    int stages;
     int tiles_m, tiles_n;
-    int *marks;  // per tile: computed again; null: none is
 };
 
-// BM x BN by WM x WN waves; stages of SK k blocks, NST of them in LDS.
-template <int BM, int BN, int WM, int WN, int PA, int PB, int SK, int NST>
+// One side's part of a stage of SK k blocks: R rows.
+template <Src S, int R, int SK, bool CODES>
+struct PlaneSide {
+    static constexpr bool kCodes = CODES;
+    static constexpr int P = pieces_of(S), kBlocks = R / kPlaneRows;
+    static_assert(!kCodes || SK * kPlaneK == kPackGroup, "codes: a group of 128 a stage");
+    // DMA instructions of 1 KB: fragments, or 8 rows of 128 codes (a row's chunk c
+    // of 16 stands at c ^ row % 8, so that a fragment's reads, one chunk of 32 rows,
+    // take every bank alike)
+    static constexpr int kUnits = kCodes ? kBlocks * 4 : kBlocks * SK * P;
+    static constexpr int kBytes = kUnits * kFragBytes;
+    static constexpr int kScaleUnits = kCodes ? R / 64 : 0;  // of 64 words: a row's four scales each
+    static constexpr size_t kStep = kCodes ? kPackGroup : static_cast<size_t>(SK) * P * kFragBytes;  // bytes, a stage
+
+    // unit u of the tile of row block b0: where it starts, and the lane's offset from there
+    static __device__ __forceinline__ const char *start(const char *planes, const Operand &o, int b0, int u, int kb,
+                                                        int row_blocks) {
+        if constexpr (kCodes) {
+            return reinterpret_cast<const char *>(o.codes) + static_cast<size_t>(b0) * kPlaneRows * o.pitch;
+        } else {
+            const int row = min(b0 + u / (SK * P), row_blocks - 1);
+            return planes + (static_cast<size_t>(row) * kb * P + u % (SK * P)) * kFragBytes;
+        }
+    }
+    static __device__ __forceinline__ unsigned offset(const Operand &o, int b0, int u, int lane) {
+        if constexpr (kCodes) {
+            const int last = o.rows - 1 - b0 * kPlaneRows;  // rows past an edge: the last one's
+            return static_cast<unsigned>(min(u * 8 + (lane >> 3), last)) * static_cast<unsigned>(o.pitch) +
+                   16u * ((lane & 7) ^ (lane >> 3));
+        } else {
+            return 16u * lane;
+        }
+    }
+    // a code fragment's eight bytes: k block k of row block b
+    static __device__ __forceinline__ u2v_t codes8(const char *at, int b, int k, int lane) {
+        const int i = lane & 31, h = lane >> 5;
+        return *reinterpret_cast<const u2v_t *>(at + b * 4096 + i * 128 + 8 * h + (16 * k ^ 16 * (i & 7)));
+    }
+};
+
+// SA, SB: the operands' kinds.  BM x BN by WM x WN waves; stages of SK k blocks,
+// NST of them in LDS.
+template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
+    using A = PlaneSide<SA, BM, SK, as_codes(SA, SB)>;
+    using B = PlaneSide<SB, BN, SK, as_codes(SA, SB)>;
+    constexpr int PA = A::P, PB = B::P;
     constexpr int NW = WM * WN, FM = BM / WM / kPlaneRows, FN = BN / WN / kPlaneRows;
-    constexpr int NA = BM / kPlaneRows * SK * PA, NB = BN / kPlaneRows * SK * PB;  // fragments of a stage
-    constexpr int PER = (NA + NB) / NW;
-    static_assert((NA + NB) % NW == 0, "every wave moves as many fragments");
-    constexpr int kStage = (NA + NB) * kFragBytes;
+    constexpr int NU = A::kUnits + B::kUnits, PER = (NU + NW - 1) / NW;  // a wave's; the last may be moved twice
+    constexpr int NSC = A::kScaleUnits + B::kScaleUnits, SPER = (NSC + NW - 1) / NW;
+    constexpr int kScalesAt = A::kBytes + B::kBytes, kStage = kScalesAt + 256 * NSC;
     __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
 
     int tm, tn;
@@ -57,35 +109,58 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
+    const int ra = tm * A::kBlocks, rb = tn * B::kBlocks;  // first row blocks
 
-    // this wave's fragments of a stage: consecutive ones of A's, then of B's
+    // this wave's units of a stage: consecutive ones of A's, then of B's
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char *)lds));
     const char *src[PER];
-    unsigned dst[PER];
+    unsigned off[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int f = wave * PER + i;
-        const bool a = f < NA;
-        const int per_row = a ? SK * PA : SK * PB, n = a ? f : f - NA;
-        const int row = min((a ? tm * (BM / kPlaneRows) : tn * (BN / kPlaneRows)) + n / per_row, (a ? g.rows_a : g.rows_b) - 1);
-        src[i] = (a ? g.A : g.B) + (static_cast<size_t>(row) * g.kb * (a ? PA : PB) + n % per_row) * kFragBytes;
-        dst[i] = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char *)(lds + f * kFragBytes)));
+        const int f = min(wave * PER + i, NU - 1);
+        if (f < A::kUnits) {
+            src[i] = A::start(g.A, g.p.A, ra, f, g.kb, g.rows_a);
+            off[i] = A::offset(g.p.A, ra, f, lane);
+        } else {
+            src[i] = B::start(g.B, g.p.B, rb, f - A::kUnits, g.kb, g.rows_b);
+            off[i] = B::offset(g.p.B, rb, f - A::kUnits, lane);
+        }
     }
-    const unsigned voff = lane * 16;
-    const int stages = g.kb / SK;
     auto dma = [&](int stage, int slot) {
-        const size_t at = static_cast<size_t>(min(stage, stages - 1)) * SK * kFragBytes;  // past the end: the last again
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const char *p = src[i] + at * (wave * PER + i < NA ? PA : PB);
-            const unsigned to = dst[i] + slot * kStage;
+        const int at = min(stage, g.stages - 1);  // past the end: the last again
+        const unsigned base = lds0 + slot * kStage;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(p), "s"(to) : "memory", "m0");
-#pragma clang diagnostic pop
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int f = min(wave * PER + i, NU - 1);
+            const char *p = src[i] + at * (f < A::kUnits ? A::kStep : B::kStep);
+            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[i]), "s"(p), "s"(base + f * kFragBytes)
+                         : "memory", "m0");
         }
+        if constexpr (NSC > 0) {
+            const size_t group = at;
+#pragma unroll
+            for (int i = 0; i < SPER; ++i) {
+                const int f = (wave * SPER + i) % NSC;
+                const bool a = f < A::kScaleUnits;
+                const Operand &o = a ? g.p.A : g.p.B;
+                const int first = (a ? ra : rb) * kPlaneRows, row = first + (a ? f : f - A::kScaleUnits) * 64 + lane;
+                const char *p = reinterpret_cast<const char *>(o.scales) + group * o.code_rows * 4;
+                const unsigned to = 4u * static_cast<unsigned>(min(row, o.rows - 1));
+                asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(to), "s"(p),
+                             "s"(base + kScalesAt + f * 256)
+                             : "memory", "m0");
+            }
+        }
+#pragma clang diagnostic pop
     };
     auto frag = [&](const char *stage, int n) {
         return *reinterpret_cast<const b8v_t *>(stage + n * kFragBytes + lane * 16);
+    };
+    // a side's fragment of one piece from its codes: k block k of row block b, four: its row's scales
+    auto widened = [&](u2v_t c, unsigned four, int byte) {
+        return widen(c[0], c[1], __uint_as_float((four >> (8 * byte) & 255u) << 23));  // a scale byte is fp32's exponent
     };
 
     floatx16 acc[FM][FN];
@@ -97,24 +172,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) dma(s, s);
     int slot = 0;
-    for (int s = 0; s < stages; ++s) {
+    for (int s = 0; s < g.stages; ++s) {
         // this stage has landed, and every wave is done with the one before
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER *(NST - 2)) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((PER + SPER) * (NST - 2)) : "memory");
         dma(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
-        const char *at = lds + slot * kStage;
+        const char *at = lds + slot * kStage, *at_b = at + A::kBytes;
+        unsigned sa[FM], sb[FN];  // the rows' scales
+        auto row_scales = [&](int first, int row) {
+            return *reinterpret_cast<const unsigned *>(at + kScalesAt + first * 256 + (row * kPlaneRows + (lane & 31)) * 4);
+        };
+        if constexpr (A::kCodes) {
+#pragma unroll
+            for (int x = 0; x < FM; ++x) sa[x] = row_scales(0, wm * FM + x);
+        }
+        if constexpr (B::kCodes) {
+#pragma unroll
+            for (int c = 0; c < FN; ++c) sb[c] = row_scales(A::kScaleUnits, wn * FN + c);
+        }
 #pragma unroll
         for (int k = 0; k < SK; ++k) {
             b8v_t fb[FN][PB];
 #pragma unroll
-            for (int c = 0; c < FN; ++c)
+            for (int c = 0; c < FN; ++c) {
+                if constexpr (B::kCodes) {
+                    fb[c][0] = widened(B::codes8(at_b, wn * FN + c, k, lane), sb[c], k / 2);
+                } else {
 #pragma unroll
-                for (int p = 0; p < PB; ++p) fb[c][p] = frag(at, NA + ((wn * FN + c) * SK + k) * PB + p);
+                    for (int p = 0; p < PB; ++p) fb[c][p] = frag(at_b, ((wn * FN + c) * SK + k) * PB + p);
+                }
+            }
             const float sign = (s * SK + k) & 1 ? -1.0f : 1.0f;
 #pragma unroll
             for (int x = 0; x < FM; ++x) {
                 b8v_t fa[PA];
+                if constexpr (A::kCodes) {
+                    fa[0] = widened(A::codes8(at, wm * FM + x, k, lane), sa[x], k / 2);
+                } else {
 #pragma unroll
-                for (int p = 0; p < PA; ++p) fa[p] = frag(at, ((wm * FM + x) * SK + k) * PA + p);
+                    for (int p = 0; p < PA; ++p) fa[p] = frag(at, ((wm * FM + x) * SK + k) * PA + p);
+                }
 #pragma unroll
                 for (int c = 0; c < FN; ++c) {
                     auto mm = [&](floatx16 v, int pa, int pb) {
@@ -141,7 +237,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outstanding at exit
 
-    if (PB == 3 && g.marks) {
+    if constexpr (PB == 3) {  // (codes hold finite values, and their product's own range is fp32's)
         float worst = 0.0f;  // NaN * 0 and inf * 0 stay NaN
 #pragma unroll
         for (int x = 0; x < FM; ++x)
@@ -149,21 +245,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
             for (int c = 0; c < FN; ++c)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) worst = __builtin_fmaf(acc[x][c][r], 0.0f, worst);
-        if (worst != worst) g.marks[tm * g.tiles_n + tn] = 1;
+        if (__syncthreads_or(worst != worst)) {  // uniform
+            constexpr int TN = BN / kDirectTile;
+            for (int t = wave; t < BM / kDirectTile * TN; t += NW) {
+                const int ti = tm * (BM / kDirectTile) + t / TN, tj = tn * TN + t % TN;
+                if (ti * kDirectTile < g.p.M && tj < g.p.tiles_n) direct_tile<SA, SB, 1>(g.p, ti * g.p.tiles_n + tj, nullptr);
+            }
+            return;
+        }
     }
 
     // lane (i, h), register r of block (x, c): row 8 (r / 4) + 4 h + r % 4, column i
     const int li = lane & 31, lh = lane >> 5;
     const int i0 = tm * BM + wm * FM * kPlaneRows, j0 = tn * BN + wn * FN * kPlaneRows;
     constexpr int kScale = (PA == 3 ? 16 : 0) + (PB == 3 ? 16 : 0);
-    const float *extra = g.epi.go ? g.epi.go : g.epi.residual;
-    const bool inside = i0 + FM * kPlaneRows <= g.M && j0 + FN * kPlaneRows <= g.N;  // uniform
+    const float *extra = g.p.epi.go ? g.p.epi.go : g.p.epi.residual;
+    const bool inside = i0 + FM * kPlaneRows <= g.p.M && j0 + FN * kPlaneRows <= g.p.N;  // uniform
     auto store = [&](auto edge) {
 #pragma unroll
         for (int c = 0; c < FN; ++c) {
             const int j = j0 + c * kPlaneRows + li;
-            const int jc = edge ? min(j, g.N - 1) : j;
-            const float bias = g.epi.bias ? g.epi.bias[jc] : 0.0f;
+            const int jc = edge ? min(j, g.p.N - 1) : j;
+            const float bias = g.p.epi.bias ? g.p.epi.bias[jc] : 0.0f;
 #pragma unroll
             for (int x = 0; x < FM; ++x) {
                 float ev[16];
@@ -171,25 +274,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
                 if (extra) {  // all of a block's before the first is used
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int i = edge ? min(row_of(r), g.M - 1) : row_of(r);
-                        ev[r] = extra[static_cast<size_t>(i) * g.N + jc];
+                        const int i = edge ? min(row_of(r), g.p.M - 1) : row_of(r);
+                        ev[r] = extra[static_cast<size_t>(i) * g.p.N + jc];
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int i = row_of(r);
-                    if (edge && (i >= g.M || j >= g.N)) continue;
-                    const size_t to = static_cast<size_t>(i) * g.N + j;
+                    if (edge && (i >= g.p.M || j >= g.p.N)) continue;
+                    const size_t to = static_cast<size_t>(i) * g.p.N + j;
                     float v = kScale ? __builtin_ldexpf(acc[x][c][r], -kScale) : acc[x][c][r];
-                    if (g.epi.bias) v += bias;
-                    if (g.epi.z) g.epi.z[to] = v;
-                    if (g.epi.go) {
-                        v = ev[r] * act_slope(v, g.epi.act);
+                    if (g.p.epi.bias) v += bias;
+                    if (g.p.epi.z) g.p.epi.z[to] = v;
+                    if (g.p.epi.go) {
+                        v = ev[r] * act_slope(v, g.p.epi.act);
                     } else {
-                        v = activate(v, g.epi.act);
+                        v = activate(v, g.p.epi.act);
                         if (extra) v += ev[r];
                     }
-                    g.C[to] = v;
+                    g.p.C[to] = v;
                 }
             }
         }

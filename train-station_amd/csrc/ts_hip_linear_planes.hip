@@ -1,6 +1,5 @@
 // The passes that write an operand's planes and the launches of the large
 // products (the kernel and the layout: ts_hip_linear_planes.h).
-#include "ts_hip_linear_direct.h"
 #include "ts_hip_linear_planes.h"
 #include "ts_hip_parts.h"
 
@@ -211,9 +210,8 @@ __global__ __launch_bounds__(kBlock) void planes_codes_across(const uint8_t *__r
 
 int row_blocks(size_t rows) { return static_cast<int>((rows + kPlaneRows - 1) / kPlaneRows); }
 int k_blocks(size_t K) { return static_cast<int>((K + 2 * kPlaneK - 1) / (2 * kPlaneK)) * 2; }
-bool coded(Src s) { return s == Src::kCodesK || s == Src::kCodesR; }
 size_t plane_bytes(size_t rows, size_t K, Src s) {
-    return static_cast<size_t>(row_blocks(rows)) * k_blocks(K) * (coded(s) ? 1 : 3) * kFragBytes;
+    return static_cast<size_t>(row_blocks(rows)) * k_blocks(K) * (pieces_of(s)) * kFragBytes;
 }
 
 unsigned wave_grid(size_t jobs) { return static_cast<unsigned>((jobs + kBlock / 64 - 1) / (kBlock / 64)); }
@@ -261,38 +259,43 @@ void write_planes(const Operand &o, Src src, int K, bool negate, char *out, cons
     }
 }
 
-// The tiles that were marked once more, in fp32.
-template <Src SA, Src SB>
-__global__ __launch_bounds__(64) void planes_again(DirectProduct p, const int *marks, int bm, int bn, int tiles_n) {
-    for (int t = blockIdx.x; t < p.tiles; t += gridDim.x) {
-        const int i0 = t / p.tiles_n * kDirectTile, j0 = t % p.tiles_n * kDirectTile;
-        if (marks[i0 / bm * tiles_n + j0 / bn]) direct_tile<SA, SB, 1>(p, t, nullptr);  // uniform
-    }
-}
-
-__global__ __launch_bounds__(kBlock) void clear_marks(int *marks, int n) {
-    for (int i = blockIdx.x * kBlock + threadIdx.x; i < n; i += gridDim.x * kBlock) marks[i] = 0;
-}
-
-template <int BM, int BN, int WM, int WN, int PA, int PB, int SK, int NST>
+template <Src SA, Src SB, int BM, int BN, int SK, int NST>
 void launch_planes(PlanesArgs g, hipStream_t s) {
-    g.tiles_m = (g.M + BM - 1) / BM;
-    g.tiles_n = (g.N + BN - 1) / BN;
-    if (g.marks) launch(clear_marks, dim3(1), dim3(kBlock), 0, s, g.marks, g.tiles_m * g.tiles_n);
-    launch((linear_planes<BM, BN, WM, WN, PA, PB, SK, NST>), dim3(g.tiles_m * g.tiles_n), dim3(64 * WM * WN), 0, s, g);
+    g.tiles_m = (g.p.M + BM - 1) / BM;
+    g.tiles_n = (g.p.N + BN - 1) / BN;
+    g.stages = as_codes(SA, SB) ? static_cast<int>(g.p.A.pitch / kPackGroup) : g.kb / SK;
+    launch((linear_planes<SA, SB, BM, BN, 2, 2, SK, NST>), dim3(g.tiles_m * g.tiles_n), dim3(256), 0, s, g);
+}
+
+// The tile whose rounds over the chip cost least: rounds x its area, the smallest
+// tile 1.1 times as dear, and a larger one 1.3 times where a CU has but one
+// workgroup to fill its waits.  us in 128 x 128, 128 x 64, 64 x 64, pieces on both
+// sides: 8192 x 4096 x 4096 1284, 1295, 1381; 2048 x 4096 x 1024 93, 96, 99;
+// 1024 x 4096 x 2048 105, 90, 104; 2048 x 1024 x 4096 177, 122, 98; 1999 x 777 x
+// 1531 78, 53, 39.  One side's: 598, 662, 764; 52, 56, 59; 55, 54, 57; 87, 70, 57;
+// 46, 36, 28.  Codes: 260, 280, 324; 28.6, 30.4, 31.8; 32, 29, 31; 46, 35, 35; 26,
+// 22, 19.  (128 x 256 by eight waves: within 3 % of 128 x 128 at the largest, and
+// slower below; 256 x 256: slower.)
+enum class Tile { k128x128, k128x64, k64x64 };
+Tile choose_tile(size_t M, size_t N) {
+    const size_t cus = device_cu_count();
+    auto cost = [&](size_t bm, size_t bn, double each) {
+        const size_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn), rounds = (tiles + cus - 1) / cus;
+        return rounds * bm * bn * each * (rounds == 1 && bm > 64 ? 1.3 : 1.0);
+    };
+    const double a = cost(128, 128, 1.0), b = cost(128, 64, 1.0), c = cost(64, 64, 1.1);
+    return a <= b && a <= c ? Tile::k128x128 : b <= c ? Tile::k128x64 : Tile::k64x64;
 }
 
 size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
-
-constexpr int kMarkTile = 128;  // the smallest tile
 
 }  // namespace
 
 bool planes_take(size_t M, size_t N, size_t K) { return 2.0 * M * N * K >= 1.5e9 && M >= 128 && N >= 128 && K >= 64; }
 
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b) {
-    const size_t marks = ((M + kMarkTile - 1) / kMarkTile) * ((N + kMarkTile - 1) / kMarkTile) * sizeof(int);
-    return (round_256(plane_bytes(M, K, a)) + round_256(plane_bytes(N, K, b)) + round_256(marks)) / sizeof(float);
+    if (as_codes(a, b)) return 0;
+    return (round_256(plane_bytes(M, K, a)) + round_256(plane_bytes(N, K, b))) / sizeof(float);
 }
 
 size_t planes_sum_floats(size_t N, size_t K) { return static_cast<size_t>(across_chunks(N, K)) * N; }
@@ -300,37 +303,26 @@ size_t planes_sum_floats(size_t N, size_t K) { return static_cast<size_t>(across
 int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s) {
     char *pa = reinterpret_cast<char *>(workspace);
     char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
-    int *marks = reinterpret_cast<int *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
-    const bool pieces = !coded(p.a);
-    PlanesExtra of_a, of_b;
-    of_a.codes = extra.codes;
-    of_a.scales = extra.scales;
-    of_b.sums = extra.sums;
-    of_b.sum_parts = extra.sum_parts;
-    write_planes(p.A, p.a, p.K, pieces, pa, of_a, s);
-    write_planes(p.B, p.b, p.K, false, pb, of_b, s);
-    PlanesArgs g = {pa, pb, p.C, p.epi, p.M, p.N, k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, marks};
-    if (pieces) launch_planes<128, 128, 2, 2, 3, 3, 1, 3>(g, s);
-    else launch_planes<128, 128, 2, 2, 1, 3, 1, 4>(g, s);
-    const DirectProduct d = direct_product(p);
-    const int cap = device_cu_count() * 4;
-    const dim3 grid(d.tiles < cap ? d.tiles : cap);
-    const int tiles_n = (p.N + kMarkTile - 1) / kMarkTile;
-    const int *m = marks;
-    auto again = [&](auto a, auto b) {
-        launch((planes_again<a.value, b.value>), grid, dim3(64), 0, s, d, m, kMarkTile, kMarkTile, tiles_n);
-    };
-    with_sources(p.a, p.b, again);
-    return launch_status();
-}
-
-int planes_packed_product(const LinearProduct &p, float *workspace, hipStream_t s) {
-    char *pa = reinterpret_cast<char *>(workspace);
-    char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
-    write_planes(p.A, p.a, p.K, false, pa, {}, s);
-    write_planes(p.B, p.b, p.K, false, pb, {}, s);
-    PlanesArgs g = {pa, pb, p.C, p.epi, p.M, p.N, k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, nullptr};
-    launch_planes<128, 128, 2, 2, 1, 1, 2, 4>(g, s);
+    if (!as_codes(p.a, p.b)) {
+        PlanesExtra of_a, of_b;
+        of_a.codes = extra.codes;
+        of_a.scales = extra.scales;
+        of_b.sums = extra.sums;
+        of_b.sum_parts = extra.sum_parts;
+        write_planes(p.A, p.a, p.K, !of_codes(p.a), pa, of_a, s);
+        write_planes(p.B, p.b, p.K, false, pb, of_b, s);
+    }
+    const PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0};
+    const Tile tile = choose_tile(p.M, p.N);
+    with_sources(p.a, p.b, [&](auto a, auto b) {
+        constexpr Src A = a.value, B = b.value;
+        constexpr bool codes = as_codes(A, B), three = pieces_of(A) == 3;
+        // stages: of 128 codes; else of 16 k, three or four of them (two of 32 for one piece beside three:
+        // 8192 x 4096 x 4096 598 us, against 700 in four of 16)
+        if (tile == Tile::k128x128) launch_planes<A, B, 128, 128, codes ? 8 : three ? 1 : 2, codes || !three ? 2 : 3>(g, s);
+        else if (tile == Tile::k128x64) launch_planes<A, B, 128, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
+        else launch_planes<A, B, 64, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
+    });
     return launch_status();
 }
 
