@@ -19,6 +19,9 @@ import numpy as np
 from ._ffi import ACTIVATIONS, F, SZ, TsError, gradtrack as _G, last_error
 
 
+_Dims8 = SZ * 8
+
+
 def _dims(shape: Sequence[int]):
     shape = [int(d) for d in shape]
     arr = (SZ * max(len(shape), 1))(*shape)
@@ -167,10 +170,12 @@ class Tensor:
 
     @property
     def shape(self) -> tuple:
-        rank = _G.ts_tensor_rank(self._h)
-        out = (SZ * max(rank, 1))()
-        _G.ts_tensor_dims(self._h, out, rank)
-        return tuple(int(out[i]) for i in range(rank))
+        out = _Dims8()
+        rank = _G.ts_tensor_dims(self._h, out, 8)
+        if rank > 8:
+            out = (SZ * rank)()
+            _G.ts_tensor_dims(self._h, out, rank)
+        return tuple(out[:rank])
 
     def size(self) -> int:
         return int(_G.ts_tensor_size(self._h))
