@@ -106,7 +106,7 @@ ts_tensor *ts_tensor_add_rms_norm(const ts_tensor *x, const ts_tensor *residual,
 /* The layer act(x weight + bias) + residual as one op: x [..., fan_in], weight
  * [fan_in, fan_out], bias [fan_out] and residual [..., fan_out] may be NULL;
  * activation one of TS_HIP_ACT_* (ts_hip.h).  For the backward pass it keeps
- * its input, and with an activation the values before it (checkpoint 0), or the
+ * its input, and with an activation its slopes (checkpoint 0), or the
  * input's values in 8 bits alone (checkpoint 1): the backward pass then computes
  * the layer again from them where it needs the activation's slope, and the
  * weight's gradient from them. */

@@ -636,25 +636,25 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
                          void *stream);
 
 /* A layer's forward: z = x W + bias, y = act(z) + residual, x [batch, fan_in],
- * W [fan_in, fan_out]; bias and residual may be NULL.  z != NULL: z is stored
- * there as well (what the backward pass reads).  codes != NULL: x is also
+ * W [fan_in, fan_out]; bias and residual may be NULL.  slope != NULL: act'(z) is
+ * stored there, laid out as y (what the backward pass reads).  codes != NULL: x is also
  * packed into codes / scales (ts_hip_pack8). */
 typedef struct ts_hip_linear_shape {
     size_t batch, fan_in, fan_out;
 } ts_hip_linear_shape;
 size_t ts_hip_linear_workspace_floats(const ts_hip_linear_shape *shape);
 int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float *weight, const float *bias, int act,
-                  const float *residual, float *y, float *z, uint8_t *codes, uint8_t *scales, float *workspace,
+                  const float *residual, float *y, float *slope, uint8_t *codes, uint8_t *scales, float *workspace,
                   size_t workspace_floats, void *stream);
 /* The layer's gradients from go = dy:
  *   dz = go act'(z),  dx = dz W^T,  dweight = X^T dz,  dbias = dz's column sums
  * each of dx, dweight and dbias NULL where it is not wanted.  X is x, or what
- * codes / scales hold where codes != NULL (x is then not read); z is the
- * forward's (needed with x and an activation), or NULL: with codes it is
- * computed again from what they hold, z = X W + bias.  relu's slope at 0 is 0. */
+ * codes / scales hold where codes != NULL (x is then not read); slope is the
+ * forward's (needed with x and an activation), or NULL: with codes the slopes
+ * are computed again from what they hold, at z = X W + bias.  relu's slope at 0 is 0. */
 size_t ts_hip_linear_backward_workspace_floats(const ts_hip_linear_shape *shape);
 int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, const uint8_t *codes,
-                           const uint8_t *scales, const float *weight, const float *bias, int act, const float *z,
+                           const uint8_t *scales, const float *weight, const float *bias, int act, const float *slope,
                            const float *go, float *dx, float *dweight, float *dbias, float *workspace,
                            size_t workspace_floats, void *stream);
 

@@ -72,9 +72,9 @@ def linear(shape=(4, 8, 16), x=P, w=P, act=0, y=P, codes=None, scales=None, ws=N
     return hip.ts_hip_linear(ctypes.byref(s), x, w, None, act, None, y, None, codes, scales, ws, floats, None)
 
 
-def backward(shape=(4, 8, 16), x=P, codes=None, scales=None, w=P, act=0, z=None, go=P, dx=P, ws=P, floats=1 << 40):
+def backward(shape=(4, 8, 16), x=P, codes=None, scales=None, w=P, act=0, slope=None, go=P, dx=P, ws=P, floats=1 << 40):
     s = LinearShape(*shape)
-    return hip.ts_hip_linear_backward(ctypes.byref(s), x, codes, scales, w, None, act, z, go, dx, None, None, ws, floats,
+    return hip.ts_hip_linear_backward(ctypes.byref(s), x, codes, scales, w, None, act, slope, go, dx, None, None, ws, floats,
                                       None)
 
 
@@ -86,7 +86,7 @@ def test_layer_entries_refuse():
     assert linear(shape=(0, 8, 16)) == 0  # nothing to do
     assert hip.ts_hip_linear(None, P, P, None, 0, None, P, None, None, None, None, 0, None) == EINVAL
     assert backward(act=7) == EINVAL and backward(go=None) == EINVAL and backward(codes=P) == EINVAL
-    assert backward(act=2, z=None) == EINVAL  # neither z nor what to compute it from
+    assert backward(act=2, slope=None) == EINVAL  # neither the slopes nor what to compute them from
     assert backward(ws=None) == EINVAL and backward(floats=0) == EWORKSPACE
     assert backward(dx=None) == 0
 

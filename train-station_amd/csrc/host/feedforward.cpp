@@ -165,23 +165,23 @@ Tensor Tensor::linear(const Tensor &weight, const Tensor *bias, Activation act, 
     const ts_hip_linear_shape shape = {rows_of(*this), dims_.back(), od.back()};
     const bool req_b = bias && bias->requires_grad_, req_r = residual && residual->requires_grad_;
     const bool recorded = (requires_grad_ || weight.requires_grad_ || req_b || req_r) && is_grad_enabled();
-    // what the backward pass reads: X for the weight's gradient, z (or X, to
-    // compute it again) for every gradient but the residual's
-    const bool z_needed = recorded && act != Activation::None && (requires_grad_ || weight.requires_grad_ || req_b);
-    const bool x_needed = recorded && (weight.requires_grad_ || z_needed);
-    Tensor z;
+    // what the backward pass reads: X for the weight's gradient, the slopes (or X,
+    // to compute them again) for every gradient but the residual's
+    const bool slope_needed = recorded && act != Activation::None && (requires_grad_ || weight.requires_grad_ || req_b);
+    const bool x_needed = recorded && (weight.requires_grad_ || slope_needed);
+    Tensor slope;
     std::shared_ptr<Packed8> kept;
     if (x_needed && checkpoint == Checkpoint::EightBit && size_)
         kept = std::make_shared<Packed8>(Packed8::new_uninit(shape.batch, shape.fan_in));
-    if (z_needed && !kept) z = new_uninit(od);
+    if (slope_needed && !kept) slope = new_uninit(od);
     if (y.size_ || kept) {
         const size_t ws = ts_hip_linear_workspace_floats(&shape);
         const auto work = workspace(ws);
         const float *xp = dev(), *wp = weight.dev(), *bp = data_of(bias), *rp = data_of(residual);
-        float *yp = y.dev_mut(), *zp = z.size_ ? z.dev_mut() : nullptr;
+        float *yp = y.dev_mut(), *sp = slope.size_ ? slope.dev_mut() : nullptr;
         uint8_t *codes = kept ? kept->codes() : nullptr, *scales = kept ? kept->scales() : nullptr;
         launch(KernelClass::Gemm, 2.0 * shape.batch * shape.fan_in * shape.fan_out, "ts_hip_linear", [&] {
-            return ts_hip_linear(&shape, xp, wp, bp, static_cast<int>(act), rp, yp, zp, codes, scales,
+            return ts_hip_linear(&shape, xp, wp, bp, static_cast<int>(act), rp, yp, sp, codes, scales,
                                  work ? work->get() : nullptr, ws, S());
         });
     }
@@ -190,7 +190,7 @@ Tensor Tensor::linear(const Tensor &weight, const Tensor *bias, Activation act, 
         fn.activation = act;
         fn.input_shape = dims_;
         fn.saved = {x_needed && !kept ? saved() : SavedTensor{nullptr, dims_}, weight.saved(),
-                    bias ? bias->saved() : SavedTensor{}, z.saved()};
+                    bias ? bias->saved() : SavedTensor{}, slope.saved()};
         fn.checkpoint = std::move(kept);
         fn.req_left = requires_grad_;
         fn.req_right = weight.requires_grad_;
@@ -207,7 +207,7 @@ Tensor Tensor::linear(const Tensor &weight, const Tensor *bias, Activation act, 
 }
 
 std::vector<std::optional<Tensor>> linear_backward(const GradFn &fn, const Tensor &go) {
-    const SavedTensor &x = fn.saved[0], &w = fn.saved[1], &b = fn.saved[2], &z = fn.saved[3];
+    const SavedTensor &x = fn.saved[0], &w = fn.saved[1], &b = fn.saved[2], &slope = fn.saved[3];
     const ts_hip_linear_shape shape = {w.dims[0] ? [&] {
                                            size_t n = 1;
                                            for (size_t d : fn.input_shape) n *= d;
@@ -222,7 +222,7 @@ std::vector<std::optional<Tensor>> linear_backward(const GradFn &fn, const Tenso
     if (dx.size() || dw.size() || db.size()) {
         const size_t ws = ts_hip_linear_backward_workspace_floats(&shape);
         const auto work = workspace(ws);
-        const float *xp = x.ptr(), *wp = w.ptr(), *bp = b.ptr(), *zp = z.ptr(), *gp = go.dev();
+        const float *xp = x.ptr(), *wp = w.ptr(), *bp = b.ptr(), *sp = slope.ptr(), *gp = go.dev();
         const uint8_t *codes = fn.checkpoint ? fn.checkpoint->codes() : nullptr;
         const uint8_t *scales = fn.checkpoint ? fn.checkpoint->scales() : nullptr;
         float *dxp = dx.size() ? dx.dev_mut() : nullptr, *dwp = dw.size() ? dw.dev_mut() : nullptr,
@@ -230,7 +230,7 @@ std::vector<std::optional<Tensor>> linear_backward(const GradFn &fn, const Tenso
         const int again = fn.checkpoint && fn.activation != Activation::None ? 1 : 0;
         const double flops = 2.0 * shape.batch * shape.fan_in * shape.fan_out * ((dxp ? 1 : 0) + (dwp ? 1 : 0) + again);
         launch(KernelClass::Gemm, flops, "ts_hip_linear_backward", [&] {
-            return ts_hip_linear_backward(&shape, xp, codes, scales, wp, bp, static_cast<int>(fn.activation), zp, gp, dxp,
+            return ts_hip_linear_backward(&shape, xp, codes, scales, wp, bp, static_cast<int>(fn.activation), sp, gp, dxp,
                                           dwp, dbp, work ? work->get() : nullptr, ws, S());
         });
     }

@@ -414,7 +414,7 @@ class Packed8;
 // Activations of Tensor::linear (TS_HIP_ACT_*)
 enum class Activation : int { None = 0, Relu = 1, Silu = 2, GeluTanh = 3 };
 // What a layer keeps of its input for the backward pass: the tensor itself
-// (and, with an activation, the values before it), or its values in 8 bits,
+// (and, with an activation, its slopes), or its values in 8 bits,
 // from which the backward pass computes the layer again.
 enum class Checkpoint : int { Full = 0, EightBit = 1 };
 
@@ -445,7 +445,7 @@ struct GradFn {
     bool keepdim = false;
     size_t axis = 0;                   // softmax
     size_t dim0 = 0, dim1 = 0;         // transpose: the axes swapped
-    // a layer: saved = {x, weight, bias, z}, without a buffer where there is
+    // a layer: saved = {x, weight, bias, slopes}, without a buffer where there is
     // none; its input's values in 8 bits instead of x
     Activation activation = Activation::None;
     std::shared_ptr<Packed8> checkpoint;

@@ -21,62 +21,75 @@ __device__ __forceinline__ float exp_neg_abs(float v) {
 constexpr float kGelu1 = 1.59576912f;  // 2 sqrt(2 / pi)
 constexpr float kGelu2 = 0.044715f;
 
-// s(v) = 1 / (1 + e^-v) from q = e^-|v|, and s (1 - s): no cancellation at either end
-__device__ __forceinline__ float sigmoid_of(float v, float q) {
-    const float inv = 1.0f / (1.0f + q);
-    return v >= 0.0f ? inv : v < 0.0f ? q * inv : v;  // (a NaN stays)
-}
-
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == TS_HIP_ACT_NONE) return z;
-    if (act == TS_HIP_ACT_RELU) return z > 0.0f ? z : 0.0f;
-    const float v = act == TS_HIP_ACT_SILU ? z : kGelu1 * (z + kGelu2 * z * z * z);
-    return z * sigmoid_of(v, exp_neg_abs(v));
-}
-
-__device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == TS_HIP_ACT_NONE) return 1.0f;
-    if (act == TS_HIP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+// act(z) and, where SLOPE, act'(z)
+template <bool SLOPE>
+__device__ __forceinline__ float activate(float z, int act, float &slope) {
+    if (act == TS_HIP_ACT_NONE) {
+        slope = 1.0f;
+        return z;
+    }
+    if (act == TS_HIP_ACT_RELU) {
+        slope = z > 0.0f ? 1.0f : 0.0f;
+        return z > 0.0f ? z : 0.0f;
+    }
     const bool silu = act == TS_HIP_ACT_SILU;
     const float v = silu ? z : kGelu1 * (z + kGelu2 * z * z * z);
-    const float q = exp_neg_abs(v), s = sigmoid_of(v, q), inv = 1.0f / (1.0f + q);
-    if (q == 0.0f) return s;  // far out the second term is nothing, whatever its factors
-    return s + z * (q * inv * inv) * (silu ? 1.0f : kGelu1 * (1.0f + 3.0f * kGelu2 * z * z));
+    const float q = exp_neg_abs(v), inv = 1.0f / (1.0f + q);
+    const float s = v >= 0.0f ? inv : v < 0.0f ? q * inv : v;  // 1 / (1 + e^-v); a NaN stays
+    if (SLOPE) {
+        // s + z s (1 - s) v', s (1 - s) = q / (1 + q)^2: no cancellation at either end; far out the second
+        // term is nothing, whatever its factors
+        const float d = z * (q * inv * inv) * (silu ? 1.0f : kGelu1 * (1.0f + 3.0f * kGelu2 * z * z));
+        slope = q == 0.0f ? s : s + d;
+    }
+    return z * s;
 }
 
 // ---- epilogues -------------------------------------------------------------------
 
 // Of a product P [M, N] stored with ldc = N:
-//   v = P + bias[j];  z[i][j] = v where z is set
-//   go set:  c = go v's slope               (a layer's dz)
+//   v = P + bias[j];  slope[i][j] = act'(v) where slope is set
+//   go set:  c = go act'(v)                 (a layer's dz)
 //   else:    c = act(v) + residual
 struct LinearEpi {
     const float *bias, *residual, *go;
-    float *z;
+    float *slope;
     int act;
 };
 
-__device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, size_t at, float v, float bias) {
+// c from v = P and the value of go or residual at its place (extra)
+__device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, size_t at, float v, float bias, float extra) {
     if (e.bias) v += bias;
-    if (e.z) e.z[at] = v;
+    float slope;
     if (e.go) {
-        v = e.go[at] * act_slope(v, e.act);
-    } else {
-        v = activate(v, e.act);
-        if (e.residual) v += e.residual[at];
+        activate<true>(v, e.act, slope);
+        c[at] = extra * slope;
+        return;
     }
+    if (e.slope) {
+        v = activate<true>(v, e.act, slope);
+        e.slope[at] = slope;
+    } else {
+        v = activate<false>(v, e.act, slope);
+    }
+    if (e.residual) v += extra;
     c[at] = v;
+}
+__device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, size_t at, float v, float bias) {
+    const float *extra = e.go ? e.go : e.residual;
+    epilogue_store(e, c, at, v, bias, extra ? extra[at] : 0.0f);
 }
 
 // ---- operands --------------------------------------------------------------------
 
 // An operand's rows (its index in the product that is not k) and k: floats with
-// k or the row contiguous, or codes [rows][pitch] with k or the row along the
-// code rows.
+// k or the row contiguous (times, where set, what stands at the same place of
+// `times`: go and a layer's slopes), or codes [rows][pitch] with k or the row
+// along the code rows.
 enum class Src { kFloatK, kFloatR, kCodesK, kCodesR };
 
 struct Operand {
-    const float *p;
+    const float *p, *times;
     const uint8_t *codes, *scales;
     int ld;         // floats: the leading dimension
     int rows;       // the product's rows
@@ -86,39 +99,84 @@ struct Operand {
 
 template <Src S>
 __device__ __forceinline__ float operand_at(const Operand &o, int row, int k) {
-    if constexpr (S == Src::kFloatK) return o.p[static_cast<size_t>(row) * o.ld + k];
-    else if constexpr (S == Src::kFloatR) return o.p[static_cast<size_t>(k) * o.ld + row];
-    else {
+    if constexpr (S == Src::kFloatK || S == Src::kFloatR) {
+        const size_t at = S == Src::kFloatK ? static_cast<size_t>(row) * o.ld + k : static_cast<size_t>(k) * o.ld + row;
+        return o.times ? o.p[at] * o.times[at] : o.p[at];
+    } else {
         const size_t r = S == Src::kCodesK ? row : k, c = S == Src::kCodesK ? k : row;
         const int s = o.scales[(c / kPackGroup * o.code_rows + r) * 4 + c / kPackBlock % 4];
         return __builtin_amdgcn_cvt_f32_fp8(o.codes[r * o.pitch + c], 0) * pow2f(s - kPackBias);
     }
 }
 
-// k .. k + 3 of a row (k a multiple of 4), zeros from K on
+// k .. k + 3 (k a multiple of 4; zeros from K on) of rows row and row + 1 (row
+// even; past the last one: its values, or zeros)
 template <Src S>
-__device__ __forceinline__ void operand4(const Operand &o, int row, int k, int K, float (&v)[4]) {
+__device__ __forceinline__ void operand_pair(const Operand &o, int row, int k, int K, float (&v)[2][4]) {
+    typedef float pk2u_t __attribute__((ext_vector_type(2), aligned(4)));
     if constexpr (S == Src::kFloatK) {
-        const float *p = o.p + static_cast<size_t>(row) * o.ld;
-        if (k + 4 <= K) {
-            const pk4u_t q = *reinterpret_cast<const pk4u_t *>(p + k);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = q[c];
-        } else {
+        for (int x = 0; x < 2; ++x) {
+            const int r = min(row + x, o.rows - 1);
+            const size_t at = static_cast<size_t>(r) * o.ld + k;
+            if (k + 4 <= K) {
+                pk4u_t q = *reinterpret_cast<const pk4u_t *>(o.p + at);
+                if (o.times) q *= *reinterpret_cast<const pk4u_t *>(o.times + at);  // uniform
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = k + c < K ? p[k + c] : 0.0f;
+                for (int c = 0; c < 4; ++c) v[x][c] = q[c];
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[x][c] = k + c < K ? operand_at<S>(o, r, k + c) : 0.0f;
+            }
+        }
+    } else if constexpr (S == Src::kFloatR) {
+        const bool two = row + 1 < o.rows;
+        const int r = min(row, o.rows - 1);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            pk2u_t q = {0.0f, 0.0f};
+            if (k + c < K) {
+                const size_t at = static_cast<size_t>(k + c) * o.ld + r;
+                if (two) {
+                    q = *reinterpret_cast<const pk2u_t *>(o.p + at);
+                    if (o.times) q *= *reinterpret_cast<const pk2u_t *>(o.times + at);
+                } else {
+                    q[0] = operand_at<S>(o, r, k + c);
+                }
+            }
+            v[0][c] = q[0];
+            v[1][c] = q[1];
         }
     } else if constexpr (S == Src::kCodesK) {  // (the padding's codes are zeros)
-        if (k < K) {
-            const int s = o.scales[(static_cast<size_t>(k / kPackGroup) * o.code_rows + row) * 4 + k / kPackBlock % 4];
-            unpack4(*reinterpret_cast<const unsigned *>(o.codes + row * o.pitch + k), static_cast<uint8_t>(s), v);
-        } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = 0.0f;
+        for (int x = 0; x < 2; ++x) {
+            const size_t r = min(row + x, o.rows - 1);
+            unsigned code = 0;
+            uint8_t scale = 0;
+            if (k < K) {
+                code = *reinterpret_cast<const unsigned *>(o.codes + r * o.pitch + k);
+                scale = o.scales[(static_cast<size_t>(k / kPackGroup) * o.code_rows + r) * 4 + k / kPackBlock % 4];
+            }
+            unpack4(code, scale, v[x]);
         }
-    } else {
+    } else {  // two codes of a code row and its scale (a row's pitch holds the whole tile)
+        const size_t col = row, group = (col / kPackGroup * o.code_rows) * 4 + col / kPackBlock % 4;
+        unsigned code[4];
+        int scale[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = k + c < K ? operand_at<S>(o, row, k + c) : 0.0f;
+        for (int c = 0; c < 4; ++c) {
+            const size_t r = min(k + c, K - 1);
+            code[c] = *reinterpret_cast<const uint16_t *>(o.codes + r * o.pitch + col);
+            scale[c] = o.scales[group + 4 * r];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            const f2 q = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(code[c]), false);
+            const float by = k + c < K ? pow2f(scale[c] - kPackBias) : 0.0f;
+            v[0][c] = k + c < K ? q[0] * by : 0.0f;
+            v[1][c] = k + c < K ? q[1] * by : 0.0f;
+        }
     }
 }
 

@@ -13,17 +13,16 @@ struct PackJob {
     size_t rows, cols, pitch;
     int blocks;
 };
-// ... or dz's column sums (backward): f64, a workgroup per 16 columns
+// ... or dz's column sums (backward): f64, a workgroup per 16 columns and slice of rows
 struct SumJob {
-    const float *x;
-    float *out;
-    int rows, cols, blocks;
+    const float *x, *times;
+    float *out, *part;  // part: several slices, [slices][cols]
+    int rows, cols, slices, slice_rows, blocks;
 };
 
-template <int KG>
 __device__ __forceinline__ void pack_job(const PackJob &j, int block) {
-    const size_t quads = j.pitch / 4, total = j.rows * quads, stride = static_cast<size_t>(j.blocks) * 64 * KG;
-    for (size_t q = static_cast<size_t>(block) * 64 * KG + threadIdx.x; q < total; q += stride) {
+    const size_t quads = j.pitch / 4, total = j.rows * quads, stride = static_cast<size_t>(j.blocks) * kDirectThreads;
+    for (size_t q = static_cast<size_t>(block) * kDirectThreads + threadIdx.x; q < total; q += stride) {
         const size_t row = q / quads, c = 4 * (q % quads);
         float v[4];
 #pragma unroll
@@ -32,97 +31,150 @@ __device__ __forceinline__ void pack_job(const PackJob &j, int block) {
     }
 }
 
-template <int KG>
-__device__ __forceinline__ void sum_job(const SumJob &j, int block, float *lds) {
-    constexpr int Q = 4 * KG;  // rows side by side
-    double *part = reinterpret_cast<double *>(lds);
-    const int c = threadIdx.x & 15, q = threadIdx.x >> 4, col = block * 16 + c;
+constexpr int kSumLanes = kDirectThreads / 16;  // rows side by side
+
+__device__ __forceinline__ void sum_job(const SumJob &j, int block, double *lds) {
+    const int slice = block % j.slices, c = threadIdx.x & 15, q = threadIdx.x >> 4, col = block / j.slices * 16 + c;
+    const int from = slice * j.slice_rows, to = min(from + j.slice_rows, j.rows);
     double s = 0.0;
     if (col < j.cols) {
-#pragma unroll 4
-        for (int r = q; r < j.rows; r += Q) s += j.x[static_cast<size_t>(r) * j.cols + col];
+#pragma unroll 8
+        for (int r = from + q; r < to; r += kSumLanes) {
+            const size_t at = static_cast<size_t>(r) * j.cols + col;
+            s += j.times ? j.x[at] * j.times[at] : j.x[at];
+        }
     }
-    part[q * 16 + c] = s;
+    lds[q * 16 + c] = s;
     __syncthreads();
     if (q == 0 && col < j.cols) {
 #pragma unroll 4
-        for (int k = 1; k < Q; ++k) s += part[k * 16 + c];
-        j.out[col] = static_cast<float>(s);
+        for (int k = 1; k < kSumLanes; ++k) s += lds[k * 16 + c];
+        (j.slices > 1 ? j.part + static_cast<size_t>(slice) * j.cols : j.out)[col] = static_cast<float>(s);
     }
 }
 
-template <int KG>
-constexpr int kDirectLds = KG * kDirectTile * kDirectTile;
-
-template <Src SA, Src SB, int KG>
-__global__ __launch_bounds__(64 * KG) void linear_direct(DirectProduct p, PackJob pack) {
-    __shared__ float lds[kDirectLds<KG>];
+template <Src SA, Src SB>
+__global__ __launch_bounds__(kDirectThreads) void linear_direct(DirectProduct p, PackJob pack) {
+    __shared__ __attribute__((aligned(16))) float lds[kDirectWaves][kDirectTile * kDirectTile];
     const int b = blockIdx.x;
-    if (b < p.tiles) direct_tile<SA, SB, KG>(p, b, lds);  // uniform
-    else pack_job<KG>(pack, b - p.tiles);
+    if (b < p.blocks) direct_block<SA, SB>(p, b, lds);  // uniform
+    else pack_job(pack, b - p.blocks);
 }
 
 // dx = dz W^T, dweight = X^T dz and dz's column sums as one launch: none reads another's.
-template <Src SX, int KG>
-__global__ __launch_bounds__(64 * KG) void linear_direct_back(DirectProduct dx, DirectProduct dw, SumJob sum) {
-    __shared__ __attribute__((aligned(8))) float lds[kDirectLds<KG>];
+template <Src SX>
+__global__ __launch_bounds__(kDirectThreads) void linear_direct_back(DirectProduct dx, DirectProduct dw, SumJob sum) {
+    __shared__ __attribute__((aligned(16))) float lds[kDirectWaves][kDirectTile * kDirectTile];
     const int b = blockIdx.x;
-    if (b < dw.tiles) direct_tile<SX, Src::kFloatR, KG>(dw, b, lds);  // uniform
-    else if (b < dw.tiles + dx.tiles) direct_tile<Src::kFloatK, Src::kFloatK, KG>(dx, b - dw.tiles, lds);
-    else sum_job<KG>(sum, b - dw.tiles - dx.tiles, lds);
+    if (b < dw.blocks) direct_block<SX, Src::kFloatR>(dw, b, lds);  // uniform
+    else if (b < dw.blocks + dx.blocks) direct_block<Src::kFloatK, Src::kFloatK>(dx, b - dw.blocks, lds);
+    else sum_job(sum, b - dw.blocks - dx.blocks, reinterpret_cast<double *>(lds));
 }
 
-// dz = go act'(z)
-__global__ __launch_bounds__(kBlock) void linear_dz(const float *__restrict__ z, const float *__restrict__ go, int act,
-                                                    size_t n, float *__restrict__ dz) {
-    const size_t stride = static_cast<size_t>(gridDim.x) * kBlock * 4;
-    for (size_t i = (static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x) * 4; i < n; i += stride) {
-        if (i + 4 <= n) {
-            const pk4u_t zq = *reinterpret_cast<const pk4u_t *>(z + i), gq = *reinterpret_cast<const pk4u_t *>(go + i);
-            pk4u_t o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = gq[e] * act_slope(zq[e], act);
-            *reinterpret_cast<pk4u_t *>(dz + i) = o;
-        } else {
-            for (size_t k = i; k < n; ++k) dz[k] = go[k] * act_slope(z[k], act);
+// The slices' sums added in their order, with the products' epilogues.
+__global__ __launch_bounds__(kBlock) void linear_join(DirectProduct p, DirectProduct q, SumJob sum) {
+    const size_t np = p.slices > 1 ? static_cast<size_t>(p.M) * p.N : 0;
+    const size_t nq = q.slices > 1 ? static_cast<size_t>(q.M) * q.N : 0;
+    const size_t all = np + nq + (sum.slices > 1 ? sum.cols : 0), stride = static_cast<size_t>(gridDim.x) * kBlock;
+    for (size_t n = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; n < all; n += stride) {
+        auto total = [&](const float *part, size_t at, size_t size, int slices) {
+            float v = part[at];
+#pragma unroll 4
+            for (int s = 1; s < slices; ++s) v += part[s * size + at];
+            return v;
+        };
+        if (n < np) epilogue_store(p.epi, p.C, n, total(p.part, n, np, p.slices), p.epi.bias ? p.epi.bias[n % p.N] : 0.0f);
+        else if (n < np + nq)
+            epilogue_store(q.epi, q.C, n - np, total(q.part, n - np, nq, q.slices),
+                           q.epi.bias ? q.epi.bias[(n - np) % q.N] : 0.0f);
+        else sum.out[n - np - nq] = total(sum.part, n - np - nq, sum.cols, sum.slices);
+    }
+}
+
+// How a product's tiles share the chip: up to eight waves a tile while there are
+// fewer than four a SIMD and each has four steps of its own (one round of loads);
+// then slices of eight steps a wave, up to as many.
+struct DirectPlan {
+    int kg, slices, slice_steps;
+};
+DirectPlan direct_plan(size_t M, size_t N, size_t K) {
+    const size_t tiles = ((M + kDirectTile - 1) / kDirectTile) * ((N + kDirectTile - 1) / kDirectTile);
+    const size_t waves = static_cast<size_t>(device_cu_count()) * 16, steps = (K + kDirectK - 1) / kDirectK;
+    DirectPlan p = {1, 1, static_cast<int>(steps)};
+    while (p.kg < kDirectWaves && tiles * p.kg * 2 <= waves && steps >= static_cast<size_t>(p.kg) * 2 * 4) p.kg *= 2;
+    if (p.kg == kDirectWaves && steps > 16 * kDirectWaves) {
+        const size_t want = steps / (8 * kDirectWaves), room = waves / (tiles * kDirectWaves);
+        const size_t n = want < room ? want : room;
+        if (n > 1) {
+            p.slice_steps = static_cast<int>((steps + n - 1) / n);
+            p.slices = static_cast<int>((steps + p.slice_steps - 1) / p.slice_steps);
         }
     }
+    return p;
+}
+size_t round64(size_t n) { return (n + 63) / 64 * 64; }
+size_t direct_floats(size_t M, size_t N, size_t K) {
+    const int slices = direct_plan(M, N, K).slices;
+    return slices > 1 ? round64(slices * M * N) : 0;
 }
 
-// Waves that share a tile's K: as many as bring the launch to four waves a
-// SIMD, while each has two rounds of loads of its own.
-int direct_groups(size_t tiles, size_t K) {
-    const size_t waves = static_cast<size_t>(device_cu_count()) * 16;
-    int kg = 1;
-    while (kg < 8 && tiles * kg * 2 <= waves && K >= static_cast<size_t>(kg) * 2 * 64) kg *= 2;
-    return kg;
-}
-
-template <class F>
-void with_groups(int kg, F &&f) {
-    using std::integral_constant;
-    switch (kg) {
-        case 1: return f(integral_constant<int, 1>{});
-        case 2: return f(integral_constant<int, 2>{});
-        case 4: return f(integral_constant<int, 4>{});
-        default: return f(integral_constant<int, 8>{});
+// p with its plan; its parts from `part` on (moved past them)
+DirectProduct planned(const LinearProduct &p, float *&part) {
+    DirectProduct d = direct_product(p);
+    const DirectPlan plan = direct_plan(p.M, p.N, p.K);
+    d.kg = plan.kg;
+    d.slices = plan.slices;
+    d.slice_steps = plan.slice_steps;
+    const int per = kDirectWaves / d.kg;
+    d.blocks = (d.tiles * d.slices + per - 1) / per;
+    if (d.slices > 1) {
+        d.part = part;
+        part += direct_floats(p.M, p.N, p.K);
     }
+    return d;
 }
 
-PackJob pack_work(const float *x, uint8_t *codes, uint8_t *scales, size_t rows, size_t cols, int threads) {
+void join(const DirectProduct &p, const DirectProduct &q, const SumJob &sum, hipStream_t s) {
+    const size_t n = (p.slices > 1 ? static_cast<size_t>(p.M) * p.N : 0) + (q.slices > 1 ? static_cast<size_t>(q.M) * q.N : 0) +
+                     (sum.slices > 1 ? sum.cols : 0);
+    if (n) launch(linear_join, dim3(grid_for(n)), dim3(kBlock), 0, s, p, q, sum);
+}
+
+// One product by itself (with x packed beside it).
+template <Src SA>
+void run_direct(const LinearProduct &p, PackJob pack, float *part, hipStream_t s) {
+    const DirectProduct d = planned(p, part);
+    launch((linear_direct<SA, Src::kFloatR>), dim3(d.blocks + pack.blocks), dim3(kDirectThreads), 0, s, d, pack);
+    join(d, DirectProduct{}, SumJob{}, s);
+}
+
+PackJob pack_work(const float *x, uint8_t *codes, uint8_t *scales, size_t rows, size_t cols) {
     PackJob j = {x, codes, scales, rows, cols, packed_pitch(cols), 0};
     if (codes) {
-        const size_t need = (rows * j.pitch / 4 + threads - 1) / threads, cap = static_cast<size_t>(device_cu_count()) * 4;
+        const size_t need = (rows * j.pitch / 4 + kDirectThreads - 1) / kDirectThreads;
+        const size_t cap = static_cast<size_t>(device_cu_count()) * 4;
         j.blocks = static_cast<int>(need < cap ? need : cap);
     }
     return j;
 }
 
-Operand floats(const float *p, size_t ld, size_t rows) {
-    return {p, nullptr, nullptr, static_cast<int>(ld), static_cast<int>(rows), 0, 0};
+// dz's column sums: slices of 512 rows past 1024
+SumJob sum_work(const float *x, const float *times, float *out, size_t rows, size_t cols, float *part) {
+    SumJob j = {x, times, out, part, static_cast<int>(rows), static_cast<int>(cols), 1, static_cast<int>(rows), 0};
+    if (rows > 1024) {
+        j.slice_rows = 512;
+        j.slices = static_cast<int>((rows + 511) / 512);
+    }
+    j.blocks = static_cast<int>((cols + 15) / 16) * j.slices;
+    return j;
+}
+size_t sum_floats(size_t rows, size_t cols) { return rows > 1024 ? round64((rows + 511) / 512 * cols) : 0; }
+
+Operand floats(const float *p, size_t ld, size_t rows, const float *times = nullptr) {
+    return {p, times, nullptr, nullptr, static_cast<int>(ld), static_cast<int>(rows), 0, 0};
 }
 Operand packed(const uint8_t *codes, const uint8_t *scales, size_t code_rows, size_t cols, size_t rows) {
-    return {nullptr, codes, scales, 0, static_cast<int>(rows), packed_pitch(cols), code_rows};
+    return {nullptr, nullptr, codes, scales, 0, static_cast<int>(rows), packed_pitch(cols), code_rows};
 }
 
 // x W (of floats, or the codes of x)
@@ -140,9 +192,9 @@ LinearProduct forward_product(const ts_hip_linear_shape &s, const float *x, cons
     p.epi = e;
     return p;
 }
-LinearProduct dx_product(const ts_hip_linear_shape &s, const float *dz, const float *w, float *dx) {
+LinearProduct dx_product(const ts_hip_linear_shape &s, const float *dz, const float *slope, const float *w, float *dx) {
     LinearProduct p{};
-    p.A = floats(dz, s.fan_out, s.batch);
+    p.A = floats(dz, s.fan_out, s.batch, slope);
     p.a = Src::kFloatK;
     p.B = floats(w, s.fan_out, s.fan_in);
     p.b = Src::kFloatK;
@@ -153,11 +205,11 @@ LinearProduct dx_product(const ts_hip_linear_shape &s, const float *dz, const fl
     return p;
 }
 LinearProduct dw_product(const ts_hip_linear_shape &s, const float *x, const uint8_t *codes, const uint8_t *scales,
-                         const float *dz, float *dw) {
+                         const float *dz, const float *slope, float *dw) {
     LinearProduct p{};
     p.A = codes ? packed(codes, scales, s.batch, s.fan_in, s.fan_in) : floats(x, s.fan_in, s.fan_in);
     p.a = codes ? Src::kCodesR : Src::kFloatR;
-    p.B = floats(dz, s.fan_out, s.fan_out);
+    p.B = floats(dz, s.fan_out, s.fan_out, slope);
     p.b = Src::kFloatR;
     p.M = static_cast<int>(s.fan_in);
     p.N = static_cast<int>(s.fan_out);
@@ -166,27 +218,28 @@ LinearProduct dw_product(const ts_hip_linear_shape &s, const float *x, const uin
     return p;
 }
 
-// The backward pass's workspace, in floats: dz, the parts of its column sums and
-// the planes of one product after another.
+// The backward pass's workspace, in floats: dz, the parts of its column sums, and
+// the planes or slices of one product after another (dx's and dweight's slices
+// side by side).
 struct BackLayout {
-    size_t parts, planes, total;
+    size_t sums, work, total;
 };
 BackLayout back_layout(const ts_hip_linear_shape &s) {
     BackLayout l{};
-    auto round = [](size_t n) { return (n + 63) / 64 * 64; };
-    l.parts = round(s.batch * s.fan_out);
-    l.planes = l.parts;
-    size_t most = 0;
-    auto product = [&](size_t M, size_t N, size_t K, Src a, Src b) {
-        if (!planes_take(M, N, K)) return;
-        const size_t n = planes_workspace_floats(M, N, K, a, b);
+    l.sums = round64(s.batch * s.fan_out);
+    const bool dw_planes = planes_take(s.fan_in, s.fan_out, s.batch);
+    l.work = l.sums + (dw_planes ? round64(planes_sum_floats(s.fan_out, s.batch)) : sum_floats(s.batch, s.fan_out));
+    size_t most = 0, beside = 0;
+    auto product = [&](size_t M, size_t N, size_t K, Src a, Src b, bool pair) {
+        size_t n;
+        if (planes_take(M, N, K)) n = planes_workspace_floats(M, N, K, a, b);
+        else if (n = direct_floats(M, N, K); pair) n = beside += n;
         most = n > most ? n : most;
     };
-    product(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR);
-    product(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK);
-    product(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR);
-    if (planes_take(s.fan_in, s.fan_out, s.batch)) l.planes += round(planes_sum_floats(s.fan_out, s.batch));
-    l.total = l.planes + most;
+    product(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR, false);
+    product(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK, true);
+    product(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR, true);
+    l.total = l.work + most;
     return l;
 }
 
@@ -211,11 +264,11 @@ size_t ts_hip_linear_workspace_floats(const ts_hip_linear_shape *shape) {
     const ts_hip_linear_shape &d = *shape;
     return planes_take(d.batch, d.fan_out, d.fan_in)
                ? planes_workspace_floats(d.batch, d.fan_out, d.fan_in, Src::kFloatK, Src::kFloatR)
-               : 0;
+               : direct_floats(d.batch, d.fan_out, d.fan_in);
 }
 
 int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float *weight, const float *bias, int act,
-                  const float *residual, float *y, float *z, uint8_t *codes, uint8_t *scales, float *workspace,
+                  const float *residual, float *y, float *slope, uint8_t *codes, uint8_t *scales, float *workspace,
                   size_t workspace_floats, void *stream) {
     if (!shape_ok(shape) || !act_ok(act) || (codes != nullptr) != (scales != nullptr)) return TS_HIP_EINVAL;
     if (workspace_floats < ts_hip_linear_workspace_floats(shape)) return TS_HIP_EWORKSPACE;
@@ -225,20 +278,15 @@ int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float 
     if (d.fan_out == 0) return codes ? ts_hip_pack8(x, d.batch, d.fan_in, codes, scales, stream) : TS_HIP_OK;
     if (!y || (d.fan_in && (!x || !weight))) return TS_HIP_EINVAL;
     const hipStream_t s = as_stream(stream);
-    const LinearProduct p = forward_product(d, x, nullptr, nullptr, weight, y, {bias, residual, nullptr, z, act});
+    const LinearProduct p = forward_product(d, x, nullptr, nullptr, weight, y, {bias, residual, nullptr, slope, act});
+    if (!workspace && ts_hip_linear_workspace_floats(shape)) return TS_HIP_EINVAL;
     if (planes_take(d.batch, d.fan_out, d.fan_in)) {
-        if (!workspace) return TS_HIP_EINVAL;
         PlanesExtra extra;
         extra.codes = codes;
         extra.scales = scales;
         return planes_product(p, extra, workspace, s);
     }
-    const DirectProduct g = direct_product(p);
-    with_groups(direct_groups(g.tiles, p.K), [&](auto kg) {
-        const PackJob pack = pack_work(x, codes, scales, d.batch, d.fan_in, 64 * kg.value);
-        launch((linear_direct<Src::kFloatK, Src::kFloatR, kg.value>), dim3(g.tiles + pack.blocks), dim3(64 * kg.value), 0,
-               s, g, pack);
-    });
+    run_direct<Src::kFloatK>(p, pack_work(x, codes, scales, d.batch, d.fan_in), workspace, s);
     return launch_status();
 }
 
@@ -247,7 +295,7 @@ size_t ts_hip_linear_backward_workspace_floats(const ts_hip_linear_shape *shape)
 }
 
 int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, const uint8_t *codes,
-                           const uint8_t *scales, const float *weight, const float *bias, int act, const float *z,
+                           const uint8_t *scales, const float *weight, const float *bias, int act, const float *slope,
                            const float *go, float *dx, float *dweight, float *dbias, float *workspace,
                            size_t workspace_floats, void *stream) {
     if (!shape_ok(shape) || !act_ok(act) || (codes != nullptr) != (scales != nullptr)) return TS_HIP_EINVAL;
@@ -267,58 +315,54 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
     if (!dx && !dweight && !dbias) return TS_HIP_OK;
     if (!go || !workspace) return TS_HIP_EINVAL;
     const BackLayout at = back_layout(d);
-    float *const planes = workspace + at.planes;
+    float *const work = workspace + at.work;
+    // dz: go times the forward's slopes as the products read them, or go times the
+    // slopes of the layer computed again from its checkpoint, stored
     const float *dz = go;
-    if (act != TS_HIP_ACT_NONE) {
-        if (z || d.fan_in == 0) {
-            if (!z) return TS_HIP_EINVAL;
-            const size_t n = d.batch * d.fan_out;
-            launch(linear_dz, dim3(grid_for(n, 4)), dim3(kBlock), 0, s, z, go, act, n, workspace);
+    if (act == TS_HIP_ACT_NONE) {
+        slope = nullptr;
+    } else if (!slope) {
+        if (!codes || !weight) return TS_HIP_EINVAL;
+        const LinearProduct p =
+            forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
+        if (planes_take(d.batch, d.fan_out, d.fan_in)) {
+            st = planes_product(p, {}, work, s);
+            if (st) return st;
         } else {
-            if (!codes || !weight) return TS_HIP_EINVAL;
-            const LinearProduct p =
-                forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
-            if (planes_take(d.batch, d.fan_out, d.fan_in)) {
-                st = planes_product(p, {}, planes, s);
-                if (st) return st;
-            } else {
-                const DirectProduct g = direct_product(p);
-                with_groups(direct_groups(g.tiles, p.K), [&](auto kg) {
-                    launch((linear_direct<Src::kCodesK, Src::kFloatR, kg.value>), dim3(g.tiles), dim3(64 * kg.value), 0, s,
-                           g, PackJob{});
-                });
-            }
+            run_direct<Src::kCodesK>(p, PackJob{}, work, s);
         }
         dz = workspace;
     }
     if ((dx && !weight) || (dweight && !codes && !x)) return TS_HIP_EINVAL;
+    // products in planes first (each from the start of `work`), then the others as one launch
     DirectProduct gx{}, gw{};
+    LinearProduct px{}, pw{};
+    bool later_x = false, later_w = false;
     if (dx) {
-        const LinearProduct p = dx_product(d, dz, weight, dx);
-        if (planes_take(p.M, p.N, p.K)) st = planes_product(p, {}, planes, s);
-        else gx = direct_product(p);
+        px = dx_product(d, dz, slope, weight, dx);
+        later_x = !planes_take(px.M, px.N, px.K);
+        if (!later_x) st = planes_product(px, {}, work, s);
     }
     if (dweight && !st) {
-        const LinearProduct p = dw_product(d, x, codes, scales, dz, dweight);
-        if (planes_take(p.M, p.N, p.K)) {
+        pw = dw_product(d, x, codes, scales, dz, slope, dweight);
+        later_w = !planes_take(pw.M, pw.N, pw.K);
+        if (!later_w) {
             PlanesExtra extra;
             extra.sums = dbias;  // dz is passed over for its planes anyway
-            extra.sum_parts = workspace + at.parts;
-            st = planes_product(p, extra, planes, s);
+            extra.sum_parts = workspace + at.sums;
+            st = planes_product(pw, extra, work, s);
             dbias = nullptr;
-        } else {
-            gw = direct_product(p);
         }
     }
-    if (st || (!gx.tiles && !gw.tiles && !dbias)) return st ? st : launch_status();
-    SumJob sum = {dz, dbias, static_cast<int>(d.batch), static_cast<int>(d.fan_out),
-                  dbias ? static_cast<int>((d.fan_out + 15) / 16) : 0};
-    const size_t K = gw.tiles ? d.batch : d.fan_out;
-    with_groups(direct_groups(static_cast<size_t>(gx.tiles) + gw.tiles, K), [&](auto kg) {
-        const dim3 grid(gx.tiles + gw.tiles + sum.blocks), block(64 * kg.value);
-        if (codes) launch((linear_direct_back<Src::kCodesR, kg.value>), grid, block, 0, s, gx, gw, sum);
-        else launch((linear_direct_back<Src::kFloatR, kg.value>), grid, block, 0, s, gx, gw, sum);
-    });
+    if (st || (!later_x && !later_w && !dbias)) return st ? st : launch_status();
+    float *part = work;
+    if (later_x) gx = planned(px, part);
+    if (later_w) gw = planned(pw, part);
+    const SumJob sum = dbias ? sum_work(dz, slope, dbias, d.batch, d.fan_out, workspace + at.sums) : SumJob{};
+    const dim3 grid(gx.blocks + gw.blocks + sum.blocks), block(kDirectThreads);
+    if (codes) launch((linear_direct_back<Src::kCodesR>), grid, block, 0, s, gx, gw, sum);
+    else launch((linear_direct_back<Src::kFloatR>), grid, block, 0, s, gx, gw, sum);
+    join(gx, gw, sum, s);
     return launch_status();
 }
 

@@ -1,12 +1,16 @@
 // A layer's small products.
 //
-// A wave computes 32 x 32 of C in blocks of
-// v_mfma_f32_16x16x4_f32, its operands straight from memory to registers: a
-// lane takes four k of a row (k 4 q + s of 16 in step s, the same for both
-// operands), so what lies along k comes in 16-byte loads.  Nothing is staged:
-// such a call is a launch and a few waits for memory, and a stage's barrier
-// would be one more.  The waves of a workgroup take equal parts of K and their
-// sums are added in order through LDS: few tiles have a long way each.
+// A wave computes 32 x 32 of C in blocks of v_mfma_f32_16x16x4_f32, its operands
+// straight from memory to registers: a lane takes four k of two neighbouring rows
+// (k 4 q + s of 16 in step s, the same for both operands; row 2 i + x in block x),
+// so what lies along k comes in 16-byte loads and what lies along the rows in
+// 8-byte ones.  Nothing is staged: such a call is a launch and a few waits for
+// memory, and a stage's barrier would be one more.
+//
+// Few tiles have a long way each: kg waves of a workgroup take parts of a tile's
+// K, joined through LDS in their order, and past 2048 k several workgroups
+// (slices), whose sums a second launch adds in their order.  Layer 300 -> 200,
+// batch 8192: its weight's gradient, 70 tiles of 8192 k, 1050 us by a wave each.
 #pragma once
 
 #include <type_traits>
@@ -17,44 +21,44 @@ namespace tship {
 
 constexpr int kDirectTile = 32;
 constexpr int kDirectK = 16;
+constexpr int kDirectWaves = 8;  // of a workgroup
+constexpr int kDirectThreads = 64 * kDirectWaves;
 
-// A small product and the layout of its grid.
+// A small product and its share of a launch: blocks workgroups, of 8 / kg units
+// (a tile's slice) each.
 struct DirectProduct {
     Operand A, B;
     float *C;
     LinearEpi epi;
     int M, N, K, tiles_n, tiles;
+    int kg, slices, slice_steps, blocks;
+    float *part;  // several slices: [slices][M][N]
 };
 
-// KG waves share the tile (1: any wave by itself).
-template <Src SA, Src SB, int KG>
-__device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, float *lds) {
-    const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
-    const int group = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-    const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
-    f4v_t acc[2][2] = {};
-    int ra[2], rb[2];  // rows past an edge read the last one and are not stored
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        ra[x] = min(i0 + 16 * x + li, p.M - 1);
-        rb[x] = min(j0 + 16 * x + li, p.N - 1);
-    }
-    const int steps = (p.K + kDirectK - 1) / kDirectK, per = (steps + KG - 1) / KG;
-    const int from = group * per, to = min(from + per, steps);
-    constexpr int U = 4;  // steps whose loads are issued before the first is used
+inline DirectProduct direct_product(const LinearProduct &p) {
+    const int tm = (p.M + kDirectTile - 1) / kDirectTile, tn = (p.N + kDirectTile - 1) / kDirectTile;
+    const int steps = (p.K + kDirectK - 1) / kDirectK;
+    return {p.A, p.B, p.C, p.epi, p.M, p.N, p.K, tn, tm * tn, 1, 1, steps, 0, nullptr};
+}
+
+// Steps from .. to of a tile, added to acc; U steps' loads are issued before the first is used.
+template <Src SA, Src SB, int U>
+__device__ __forceinline__ void direct_steps(const DirectProduct &p, int i0, int j0, int from, int to, int lane,
+                                             f4v_t (&acc)[2][2]) {
+    const int li = lane & 15, lq = lane >> 4;
     for (int s0 = from; s0 < to; s0 += U) {
         float a[U][2][4], b[U][2][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = (s0 + u) * kDirectK + 4 * lq, K = s0 + u < to ? p.K : 0;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                operand4<SA>(p.A, ra[x], k, K, a[u][x]);
-                operand4<SB>(p.B, rb[x], k, K, b[u][x]);
+            if (s0 + u < to) {  // uniform
+                const int k = (s0 + u) * kDirectK + 4 * lq;
+                operand_pair<SA>(p.A, i0 + 2 * li, k, p.K, a[u]);
+                operand_pair<SB>(p.B, j0 + 2 * li, k, p.K, b[u]);
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u >= to) break;  // uniform
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -62,47 +66,71 @@ __device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, fl
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
                         acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][x][s], b[u][c][s], acc[x][c], 0, 0, 0);
-    }
-    // lane (li, lq), register r of block (x, c): row 16 x + 4 lq + r, column 16 c + li
-    if constexpr (KG == 1) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int j = j0 + 16 * c + li;
-            if (j >= p.N) continue;
-            const float bias = p.epi.bias ? p.epi.bias[j] : 0.0f;
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = i0 + 16 * x + 4 * lq + r;
-                    if (i < p.M) epilogue_store(p.epi, p.C, static_cast<size_t>(i) * p.N + j, acc[x][c][r], bias);
-                }
-        }
-    } else {
-        // the groups' sums by LDS, [group][row][column]; the workgroup then adds
-        // and stores whole rows
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    lds[(group * kDirectTile + 16 * x + 4 * lq + r) * kDirectTile + 16 * c + li] = acc[x][c][r];
-        __syncthreads();
-        for (int n = threadIdx.x; n < kDirectTile * kDirectTile; n += 64 * KG) {
-            const int i = i0 + n / kDirectTile, j = j0 + n % kDirectTile;
-            float v = lds[n];
-#pragma unroll
-            for (int g = 1; g < KG; ++g) v += lds[g * kDirectTile * kDirectTile + n];
-            if (i < p.M && j < p.N)
-                epilogue_store(p.epi, p.C, static_cast<size_t>(i) * p.N + j, v, p.epi.bias ? p.epi.bias[j] : 0.0f);
         }
     }
 }
+// lane (li, lq), register r of block (x, c): row 2 (4 lq + r) + x, column 2 li + c
+template <class F>
+__device__ __forceinline__ void direct_each(const f4v_t (&acc)[2][2], int lane, F &&f) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f(2 * (4 * (lane >> 4) + r) + x, 2 * (lane & 15), acc[x][0][r], acc[x][1][r]);
+}
 
-inline DirectProduct direct_product(const LinearProduct &p) {
-    const int tm = (p.M + kDirectTile - 1) / kDirectTile, tn = (p.N + kDirectTile - 1) / kDirectTile;
-    return {p.A, p.B, p.C, p.epi, p.M, p.N, p.K, tn, tm * tn};
+// A whole tile by one wave, with its epilogue (in few registers: what the large
+// products fall back to).
+template <Src SA, Src SB>
+__device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, int lane) {
+    const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
+    f4v_t acc[2][2] = {};
+    direct_steps<SA, SB, 1>(p, i0, j0, 0, (p.K + kDirectK - 1) / kDirectK, lane, acc);
+    direct_each(acc, lane, [&](int row, int col, float v0, float v1) {
+        const int i = i0 + row, j = j0 + col;
+        if (i >= p.M) return;
+        const size_t at = static_cast<size_t>(i) * p.N + j;
+        if (j < p.N) epilogue_store(p.epi, p.C, at, v0, p.epi.bias ? p.epi.bias[j] : 0.0f);
+        if (j + 1 < p.N) epilogue_store(p.epi, p.C, at + 1, v1, p.epi.bias ? p.epi.bias[j + 1] : 0.0f);
+    });
+}
+
+// Workgroup `block` of a product; lds: a tile per wave.
+template <Src SA, Src SB>
+__device__ __forceinline__ void direct_block(const DirectProduct &p, int block, float (*lds)[kDirectTile * kDirectTile]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = p.kg, group = wave % kg, unit = block * (kDirectWaves / kg) + wave / kg;
+    const bool live = unit < p.tiles * p.slices;  // uniform per wave; the others reach the barrier
+    const int tile = unit / p.slices, slice = unit % p.slices;
+    const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
+    if (live) {
+        const int steps = (p.K + kDirectK - 1) / kDirectK;
+        const int first = slice * p.slice_steps, last = min(first + p.slice_steps, steps);
+        const int per = (last - first + kg - 1) / kg, from = first + group * per;
+        f4v_t acc[2][2] = {};
+        direct_steps<SA, SB, 4>(p, i0, j0, from, min(from + per, last), lane, acc);
+        direct_each(acc, lane, [&](int row, int col, float v0, float v1) {
+            float *to = &lds[wave][row * kDirectTile + col];
+            to[0] = v0;
+            to[1] = v1;
+        });
+    }
+    __syncthreads();
+    if (!live) return;
+    // the unit's waves add and store four columns a lane
+    float *part = p.part + static_cast<size_t>(slice) * p.M * p.N;
+    for (int n = group * 64 + lane; n < kDirectTile * kDirectTile / 4; n += 64 * kg) {
+        const int i = i0 + n / (kDirectTile / 4), j = j0 + n % (kDirectTile / 4) * 4;
+        f4v_t v = *reinterpret_cast<const f4v_t *>(&lds[wave - group][4 * n]);
+        for (int g = 1; g < kg; ++g) v += *reinterpret_cast<const f4v_t *>(&lds[wave - group + g][4 * n]);
+        if (i >= p.M) continue;
+        const size_t at = static_cast<size_t>(i) * p.N + j;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (j + e >= p.N) continue;
+            if (p.slices > 1) part[at + e] = v[e];
+            else epilogue_store(p.epi, p.C, at + e, v[e], p.epi.bias ? p.epi.bias[j + e] : 0.0f);
+        }
+    }
 }
 
 // Calls f with a product's operand kinds as constants: the layouts that a layer's products have.

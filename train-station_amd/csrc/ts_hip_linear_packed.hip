@@ -136,7 +136,8 @@ __global__ __launch_bounds__(64 * KG) void packed_direct(PackedProduct p) {
             for (int r = 0; r < 4; ++r) {
                 float v = acc[a][b][r];
                 if (p.bias) v += bias[r];
-                v = activate(v, p.act);
+                float slope;
+                v = activate<false>(v, p.act, slope);
                 if (p.residual) v += res[r];
                 o[r] = v;
             }
@@ -196,8 +197,8 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
     if (workspace_floats < ts_hip_linear_packed_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
     if (planes_take(batch, fan_out, fan_in)) {
         LinearProduct q{};
-        q.A = {nullptr, x_codes, x_scales, 0, static_cast<int>(batch), packed_pitch(fan_in), batch};
-        q.B = {nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), packed_pitch(fan_in), fan_out};
+        q.A = {nullptr, nullptr, x_codes, x_scales, 0, static_cast<int>(batch), packed_pitch(fan_in), batch};
+        q.B = {nullptr, nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), packed_pitch(fan_in), fan_out};
         q.a = q.b = Src::kCodesK;
         q.M = static_cast<int>(batch);
         q.N = static_cast<int>(fan_out);

@@ -91,6 +91,39 @@ struct PlaneSide {
     }
 };
 
+// Four neighbouring sums (times 2^-scale) through the epilogue; cols of them are there.
+__device__ __forceinline__ void epilogue4(const LinearEpi &e, size_t at, const f4v_t &v, int scale, const float (&bias)[4],
+                                          const float (&extra)[4], int cols, float (&o)[4]) {
+    float slope[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        o[n] = scale ? __builtin_ldexpf(v[n], -scale) : v[n];
+        if (e.bias) o[n] += bias[n];
+    }
+    if (e.go) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            activate<true>(o[n], e.act, slope[n]);
+            o[n] = extra[n] * slope[n];
+        }
+        return;
+    }
+    if (e.slope) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            o[n] = activate<true>(o[n], e.act, slope[n]);
+            if (n < cols) e.slope[at + n] = slope[n];
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[n] = activate<false>(o[n], e.act, slope[n]);
+    }
+    if (e.residual) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[n] += extra[n];
+    }
+}
+
 // SA, SB: the operands' kinds.  BM x BN by WM x WN waves; stages of SK k blocks,
 // NST of them in LDS.
 template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST>
@@ -249,56 +282,84 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
             constexpr int TN = BN / kDirectTile;
             for (int t = wave; t < BM / kDirectTile * TN; t += NW) {
                 const int ti = tm * (BM / kDirectTile) + t / TN, tj = tn * TN + t % TN;
-                if (ti * kDirectTile < g.p.M && tj < g.p.tiles_n) direct_tile<SA, SB, 1>(g.p, ti * g.p.tiles_n + tj, nullptr);
+                if (ti * kDirectTile < g.p.M && tj < g.p.tiles_n) direct_tile<SA, SB>(g.p, ti * g.p.tiles_n + tj, lane);
             }
             return;
         }
     }
 
-    // lane (i, h), register r of block (x, c): row 8 (r / 4) + 4 h + r % 4, column i
-    const int li = lane & 31, lh = lane >> 5;
-    const int i0 = tm * BM + wm * FM * kPlaneRows, j0 = tn * BN + wn * FN * kPlaneRows;
+    // The tile by LDS (lane (i, h), register r of block (x, c): row 8 (r / 4) + 4 h +
+    // r % 4, column i, at column ^ 32 h: the halves in different banks), then by
+    // rows, four columns a lane, with the epilogue.
+    // A turn's go or residual is on its way while the one before is computed.
+    static_assert(NST * kStage >= BM * BN * 4 && BN >= 64, "room for the tile");
     constexpr int kScale = (PA == 3 ? 16 : 0) + (PB == 3 ? 16 : 0);
+    constexpr int kRowQuads = BN / 4, kRows = 4, kStep = 64 * NW / kRowQuads, kTurns = BM / kStep / kRows;
+    static_assert(kTurns * kStep * kRows == BM, "turns of kRows rows a lane");
+    float *const sums = reinterpret_cast<float *>(lds);
     const float *extra = g.p.epi.go ? g.p.epi.go : g.p.epi.residual;
-    const bool inside = i0 + FM * kPlaneRows <= g.p.M && j0 + FN * kPlaneRows <= g.p.N;  // uniform
-    auto store = [&](auto edge) {
+    const int jt = static_cast<int>(threadIdx.x) % kRowQuads * 4, j = tn * BN + jt;  // a lane keeps its columns
+    const int cols = min(4, g.p.N - j), row0 = static_cast<int>(threadIdx.x) / kRowQuads, last = g.p.M - 1 - tm * BM;
+    const size_t at0 = static_cast<size_t>(tm) * BM * g.p.N + j;
+    float ev[kRows][4];
+    auto fetch = [&](int turn) {
 #pragma unroll
-        for (int c = 0; c < FN; ++c) {
-            const int j = j0 + c * kPlaneRows + li;
-            const int jc = edge ? min(j, g.p.N - 1) : j;
-            const float bias = g.p.epi.bias ? g.p.epi.bias[jc] : 0.0f;
+        for (int t = 0; t < kRows; ++t) {  // (rows past the edge: the last one's)
+            const float *q = extra + at0 + static_cast<size_t>(min((turn * kRows + t) * kStep + row0, last)) * g.p.N;
+            if (cols == 4) {
+                *reinterpret_cast<f4v_t *>(ev[t]) = *reinterpret_cast<const f4u_t *>(q);
+            } else {
 #pragma unroll
-            for (int x = 0; x < FM; ++x) {
-                float ev[16];
-                auto row_of = [&](int r) { return i0 + x * kPlaneRows + 8 * (r >> 2) + 4 * lh + (r & 3); };
-                if (extra) {  // all of a block's before the first is used
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = edge ? min(row_of(r), g.p.M - 1) : row_of(r);
-                        ev[r] = extra[static_cast<size_t>(i) * g.p.N + jc];
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = row_of(r);
-                    if (edge && (i >= g.p.M || j >= g.p.N)) continue;
-                    const size_t to = static_cast<size_t>(i) * g.p.N + j;
-                    float v = kScale ? __builtin_ldexpf(acc[x][c][r], -kScale) : acc[x][c][r];
-                    if (g.p.epi.bias) v += bias;
-                    if (g.p.epi.z) g.p.epi.z[to] = v;
-                    if (g.p.epi.go) {
-                        v = ev[r] * act_slope(v, g.p.epi.act);
-                    } else {
-                        v = activate(v, g.p.epi.act);
-                        if (extra) v += ev[r];
-                    }
-                    g.p.C[to] = v;
-                }
+                for (int e = 0; e < 4; ++e) ev[t][e] = e < cols ? q[e] : 0.0f;
             }
         }
     };
-    if (inside) store(std::false_type{});
-    else store(std::true_type{});
+    float bias[4] = {};
+    if (cols > 0) {
+        if (extra) fetch(0);
+        if (g.p.epi.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[e] = g.p.epi.bias[min(j + e, g.p.N - 1)];
+        }
+    }
+    const int li = lane & 31, lh = lane >> 5;
+    __syncthreads();  // the last fragments
+#pragma unroll
+    for (int x = 0; x < FM; ++x)
+#pragma unroll
+        for (int c = 0; c < FN; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = (wm * FM + x) * kPlaneRows + 8 * (r >> 2) + 4 * lh + (r & 3);
+                sums[row * BN + (((wn * FN + c) * kPlaneRows + li) ^ 32 * lh)] = acc[x][c][r];
+            }
+    __syncthreads();
+    if (cols <= 0) return;  // (no barrier follows)
+#pragma unroll 1
+    for (int turn = 0; turn < kTurns; ++turn) {
+        float now[kRows][4];
+#pragma unroll
+        for (int t = 0; t < kRows; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) now[t][e] = ev[t][e];
+        if (extra && turn + 1 < kTurns) fetch(turn + 1);
+#pragma unroll
+        for (int t = 0; t < kRows; ++t) {
+            const int row = (turn * kRows + t) * kStep + row0;
+            if (row > last) continue;
+            const f4v_t v = *reinterpret_cast<const f4v_t *>(sums + row * BN + (jt ^ 32 * (row >> 2 & 1)));
+            const size_t at = at0 + static_cast<size_t>(row) * g.p.N;
+            float o[4];
+            epilogue4(g.p.epi, at, v, kScale, bias, now[t], cols, o);
+            if (cols == 4) {
+                *reinterpret_cast<f4u_t *>(g.p.C + at) = f4u_t{o[0], o[1], o[2], o[3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < cols) g.p.C[at + e] = o[e];
+            }
+        }
+    }
 }
 
 }  // namespace tship

@@ -31,8 +31,8 @@ __device__ __forceinline__ void store_pieces(char *to, const float (&v)[8], floa
 // of the lane and its partner in the other half.
 constexpr int kAlongBlocks = 8;
 
-template <bool NEG, bool PACK>
-__global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__ x, int ld, int rows, int K, int kb,
+template <bool NEG, bool PACK, bool TIMES>
+__global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__ x, const float *__restrict__ times, int ld, int rows, int K, int kb,
                                                        char *__restrict__ out, uint8_t *__restrict__ codes,
                                                        uint8_t *__restrict__ scales, size_t pitch, int chunks) {
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__
     if (rb * kPlaneRows >= rows) return;
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
-    const float *p = x + static_cast<size_t>(live ? row : 0) * ld;
+    const float *p = x + static_cast<size_t>(live ? row : 0) * ld, *tp = TIMES ? times + (p - x) : nullptr;
     float v[kAlongBlocks][8];
 #pragma unroll
     for (int b = 0; b < kAlongBlocks; ++b)
@@ -50,12 +50,13 @@ __global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__
             const int k = (b0 + b) * kPlaneK + 8 * h + 4 * q;
             float w[4] = {};
             if (live && k + 4 <= K) {
-                const pk4u_t t = *reinterpret_cast<const pk4u_t *>(p + k);
+                pk4u_t t = *reinterpret_cast<const pk4u_t *>(p + k);
+                if (TIMES) t *= *reinterpret_cast<const pk4u_t *>(tp + k);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = t[e];
             } else if (live) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? p[k + e] : 0.0f;
+                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? (TIMES ? p[k + e] * tp[k + e] : p[k + e]) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[b][4 * q + e] = w[e];
@@ -97,8 +98,8 @@ __global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__
 // ---- floats along the rows -----------------------------------------------------------
 // element (row, k) at x[k * ld + row].  A wave takes a row block and `run` k
 // blocks.  SUM: the rows' sums over them (f64) to part[chunk][rows].
-template <bool NEG, bool SUM>
-__global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict__ x, int ld, int rows, int K, int kb,
+template <bool NEG, bool SUM, bool TIMES>
+__global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict__ x, const float *__restrict__ times, int ld, int rows, int K, int kb,
                                                         char *__restrict__ out, float *__restrict__ part, int run,
                                                         int row_blocks) {
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict_
     if (from >= kb) return;
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
-    const float *p = x + (live ? row : 0);
+    const float *p = x + (live ? row : 0), *tp = TIMES ? times + (p - x) : nullptr;
     double sum = 0.0;
 #pragma unroll 2
     for (int b = from; b < to; ++b) {
@@ -117,9 +118,16 @@ __global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict_
         if ((b + 1) * kPlaneK <= K) {  // uniform
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = p[static_cast<size_t>(k + e) * ld];
+            if (TIMES) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= tp[static_cast<size_t>(k + e) * ld];
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? p[static_cast<size_t>(k + e) * ld] : 0.0f;
+            for (int e = 0; e < 8; ++e) {
+                const size_t at = static_cast<size_t>(k + e) * ld;
+                v[e] = k + e < K ? (TIMES ? p[at] * tp[at] : p[at]) : 0.0f;
+            }
         }
         if (!live) {
 #pragma unroll
@@ -235,21 +243,27 @@ void write_planes(const Operand &o, Src src, int K, bool negate, char *out, cons
         const int blocks = x.codes ? static_cast<int>(pitch / kPlaneK) : kb;
         const int chunks = (blocks + kAlongBlocks - 1) / kAlongBlocks;
         const dim3 grid(wave_grid(static_cast<size_t>(rb) * chunks));
-        if (x.codes) launch((planes_along<true, true>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
-        else if (negate) launch((planes_along<true, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
-        else launch((planes_along<false, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
+        auto along = [&](auto kernel) {
+            launch(kernel, grid, block, 0, s, o.p, o.times, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
+        };
+        if (x.codes) along(planes_along<true, true, false>);
+        else if (negate && o.times) along(planes_along<true, false, true>);
+        else if (negate) along(planes_along<true, false, false>);
+        else along(planes_along<false, false, false>);
     } else if (src == Src::kFloatR) {
         const int run = across_run(rows, K), chunks = across_chunks(rows, K);
         const dim3 grid(wave_grid(static_cast<size_t>(rb) * chunks));
-        if (x.sums) {
-            launch((planes_across<false, true>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
+        auto across = [&](auto kernel) {
+            launch(kernel, grid, block, 0, s, o.p, o.times, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
+        };
+        if (x.sums && o.times) across(planes_across<false, true, true>);
+        else if (x.sums) across(planes_across<false, true, false>);
+        else if (negate) across(planes_across<true, false, false>);
+        else if (o.times) across(planes_across<false, false, true>);
+        else across(planes_across<false, false, false>);
+        if (x.sums)
             launch(sum_parts, dim3((rows + 15) / 16), block, 0, s, static_cast<const float *>(x.sum_parts),
                    static_cast<size_t>(chunks), static_cast<size_t>(rows), x.sums);
-        } else if (negate) {
-            launch((planes_across<true, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
-        } else {
-            launch((planes_across<false, false>), grid, block, 0, s, o.p, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
-        }
     } else if (src == Src::kCodesK) {
         launch(planes_codes_along, dim3(wave_grid(static_cast<size_t>(rb) * (o.pitch / kPackGroup))), block, 0, s, o.codes,
                o.scales, rows, o.pitch, kb, out);

@@ -254,7 +254,7 @@ class Tensor:
         """The layer act(self weight + bias) + residual as one op; activation one
         of none, relu, silu and gelu_tanh.  checkpoint "8bit" keeps the input's
         values in 8 bits for the backward pass (and nothing else), "full" the
-        input itself and the values before the activation."""
+        input itself and the activation's slopes."""
         if checkpoint not in _CHECKPOINTS:
             raise TsError(f"unknown checkpoint {checkpoint!r}: one of {', '.join(_CHECKPOINTS)}")
         return _wrap(_G.ts_tensor_linear(self._h, weight._h, _optional(bias), _activation(activation),
