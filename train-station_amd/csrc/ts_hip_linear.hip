@@ -21,8 +21,8 @@ struct SumJob {
 };
 
 __device__ __forceinline__ void pack_job(const PackJob &j, int block) {
-    const size_t quads = j.pitch / 4, total = j.rows * quads, stride = static_cast<size_t>(j.blocks) * kDirectThreads;
-    for (size_t q = static_cast<size_t>(block) * kDirectThreads + threadIdx.x; q < total; q += stride) {
+    const size_t quads = j.pitch / 4, total = j.rows * quads, stride = static_cast<size_t>(j.blocks) * blockDim.x;
+    for (size_t q = static_cast<size_t>(block) * blockDim.x + threadIdx.x; q < total; q += stride) {
         const size_t row = q / quads, c = 4 * (q % quads);
         float v[4];
 #pragma unroll
@@ -31,15 +31,14 @@ __device__ __forceinline__ void pack_job(const PackJob &j, int block) {
     }
 }
 
-constexpr int kSumLanes = kDirectThreads / 16;  // rows side by side
-
 __device__ __forceinline__ void sum_job(const SumJob &j, int block, double *lds) {
+    const int lanes = blockDim.x / 16;  // rows side by side
     const int slice = block % j.slices, c = threadIdx.x & 15, q = threadIdx.x >> 4, col = block / j.slices * 16 + c;
     const int from = slice * j.slice_rows, to = min(from + j.slice_rows, j.rows);
     double s = 0.0;
     if (col < j.cols) {
 #pragma unroll 8
-        for (int r = from + q; r < to; r += kSumLanes) {
+        for (int r = from + q; r < to; r += lanes) {
             const size_t at = static_cast<size_t>(r) * j.cols + col;
             s += j.times ? j.x[at] * j.times[at] : j.x[at];
         }
@@ -48,27 +47,31 @@ __device__ __forceinline__ void sum_job(const SumJob &j, int block, double *lds)
     __syncthreads();
     if (q == 0 && col < j.cols) {
 #pragma unroll 4
-        for (int k = 1; k < kSumLanes; ++k) s += lds[k * 16 + c];
+        for (int k = 1; k < lanes; ++k) s += lds[k * 16 + c];
         (j.slices > 1 ? j.part + static_cast<size_t>(slice) * j.cols : j.out)[col] = static_cast<float>(s);
     }
 }
 
 template <Src SA, Src SB>
 __global__ __launch_bounds__(kDirectThreads) void linear_direct(DirectProduct p, PackJob pack) {
-    __shared__ __attribute__((aligned(16))) float lds[kDirectWaves][kDirectTile * kDirectTile];
+    extern __shared__ __attribute__((aligned(16))) float direct_lds[];
+    auto lds = reinterpret_cast<float(*)[kDirectTile * kDirectTile]>(direct_lds);
+    const int waves = blockDim.x / 64;
     const int b = blockIdx.x;
-    if (b < p.blocks) direct_block<SA, SB>(p, b, lds);  // uniform
+    if (b < p.blocks) direct_block<SA, SB>(p, b, waves, lds);  // uniform
     else pack_job(pack, b - p.blocks);
 }
 
 // dx = dz W^T, dweight = X^T dz and dz's column sums as one launch: none reads another's.
 template <Src SX>
 __global__ __launch_bounds__(kDirectThreads) void linear_direct_back(DirectProduct dx, DirectProduct dw, SumJob sum) {
-    __shared__ __attribute__((aligned(16))) float lds[kDirectWaves][kDirectTile * kDirectTile];
+    extern __shared__ __attribute__((aligned(16))) float direct_lds[];
+    auto lds = reinterpret_cast<float(*)[kDirectTile * kDirectTile]>(direct_lds);
+    const int waves = blockDim.x / 64;
     const int b = blockIdx.x;
-    if (b < dw.blocks) direct_block<SX, Src::kFloatR>(dw, b, lds);  // uniform
-    else if (b < dw.blocks + dx.blocks) direct_block<Src::kFloatK, Src::kFloatK>(dx, b - dw.blocks, lds);
-    else sum_job(sum, b - dw.blocks - dx.blocks, reinterpret_cast<double *>(lds));
+    if (b < dw.blocks) direct_block<SX, Src::kFloatR>(dw, b, waves, lds);  // uniform
+    else if (b < dw.blocks + dx.blocks) direct_block<Src::kFloatK, Src::kFloatK>(dx, b - dw.blocks, waves, lds);
+    else sum_job(sum, b - dw.blocks - dx.blocks, reinterpret_cast<double *>(direct_lds));
 }
 
 // The slices' sums added in their order, with the products' epilogues.
@@ -118,20 +121,23 @@ size_t direct_floats(size_t M, size_t N, size_t K) {
     return slices > 1 ? round64(slices * M * N) : 0;
 }
 
-// p with its plan; its parts from `part` on (moved past them)
+// p with its plan; its parts from `part` on (moved past them).  The launch's waves
+// a workgroup are set by direct_blocks.
 DirectProduct planned(const LinearProduct &p, float *&part) {
     DirectProduct d = direct_product(p);
     const DirectPlan plan = direct_plan(p.M, p.N, p.K);
     d.kg = plan.kg;
     d.slices = plan.slices;
     d.slice_steps = plan.slice_steps;
-    const int per = kDirectWaves / d.kg;
-    d.blocks = (d.tiles * d.slices + per - 1) / per;
     if (d.slices > 1) {
         d.part = part;
         part += direct_floats(p.M, p.N, p.K);
     }
     return d;
+}
+void direct_blocks(DirectProduct &d, int waves) {
+    const int per = waves / d.kg;
+    d.blocks = (d.tiles * d.slices + per - 1) / per;
 }
 
 void join(const DirectProduct &p, const DirectProduct &q, const SumJob &sum, hipStream_t s) {
@@ -143,15 +149,16 @@ void join(const DirectProduct &p, const DirectProduct &q, const SumJob &sum, hip
 // One product by itself (with x packed beside it).
 template <Src SA>
 void run_direct(const LinearProduct &p, PackJob pack, float *part, hipStream_t s) {
-    const DirectProduct d = planned(p, part);
-    launch((linear_direct<SA, Src::kFloatR>), dim3(d.blocks + pack.blocks), dim3(kDirectThreads), 0, s, d, pack);
+    DirectProduct d = planned(p, part);
+    direct_blocks(d, d.kg);
+    launch((linear_direct<SA, Src::kFloatR>), dim3(d.blocks + pack.blocks), dim3(64 * d.kg), d.kg * kDirectLds, s, d, pack);
     join(d, DirectProduct{}, SumJob{}, s);
 }
 
 PackJob pack_work(const float *x, uint8_t *codes, uint8_t *scales, size_t rows, size_t cols) {
     PackJob j = {x, codes, scales, rows, cols, packed_pitch(cols), 0};
     if (codes) {
-        const size_t need = (rows * j.pitch / 4 + kDirectThreads - 1) / kDirectThreads;
+        const size_t need = (rows * j.pitch / 4 + kBlock - 1) / kBlock;
         const size_t cap = static_cast<size_t>(device_cu_count()) * 4;
         j.blocks = static_cast<int>(need < cap ? need : cap);
     }
@@ -252,6 +259,8 @@ bool shape_ok(const ts_hip_linear_shape *s) {
 bool act_ok(int act) { return act >= TS_HIP_ACT_NONE && act <= TS_HIP_ACT_GELU_TANH; }
 
 }  // namespace
+
+void join_slices(const DirectProduct &p, hipStream_t s) { join(p, DirectProduct{}, SumJob{}, s); }
 
 }  // namespace tship
 
@@ -359,9 +368,15 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
     if (later_x) gx = planned(px, part);
     if (later_w) gw = planned(pw, part);
     const SumJob sum = dbias ? sum_work(dz, slope, dbias, d.batch, d.fan_out, workspace + at.sums) : SumJob{};
-    const dim3 grid(gx.blocks + gw.blocks + sum.blocks), block(kDirectThreads);
-    if (codes) launch((linear_direct_back<Src::kCodesR>), grid, block, 0, s, gx, gw, sum);
-    else launch((linear_direct_back<Src::kFloatR>), grid, block, 0, s, gx, gw, sum);
+    int waves = sum.blocks ? 4 : 1;  // (the sums: 16 rows side by side at least)
+    if (later_x) waves = gx.kg > waves ? gx.kg : waves;
+    if (later_w) waves = gw.kg > waves ? gw.kg : waves;
+    if (later_x) direct_blocks(gx, waves);
+    if (later_w) direct_blocks(gw, waves);
+    const dim3 grid(gx.blocks + gw.blocks + sum.blocks), block(64 * waves);
+    const unsigned lds = waves * kDirectLds;
+    if (codes) launch((linear_direct_back<Src::kCodesR>), grid, block, lds, s, gx, gw, sum);
+    else launch((linear_direct_back<Src::kFloatR>), grid, block, lds, s, gx, gw, sum);
     join(gx, gw, sum, s);
     return launch_status();
 }

@@ -21,11 +21,12 @@ namespace tship {
 
 constexpr int kDirectTile = 32;
 constexpr int kDirectK = 16;
-constexpr int kDirectWaves = 8;  // of a workgroup
+constexpr int kDirectWaves = 8;  // of a workgroup, at most: the largest kg of its launch
 constexpr int kDirectThreads = 64 * kDirectWaves;
+constexpr unsigned kDirectLds = kDirectTile * kDirectTile * sizeof(float);  // a wave's, in bytes
 
-// A small product and its share of a launch: blocks workgroups, of 8 / kg units
-// (a tile's slice) each.
+// A small product and its share of a launch: blocks workgroups, of waves / kg
+// units (a tile's slice) each.
 struct DirectProduct {
     Operand A, B;
     float *C;
@@ -41,21 +42,24 @@ inline DirectProduct direct_product(const LinearProduct &p) {
     return {p.A, p.B, p.C, p.epi, p.M, p.N, p.K, tn, tm * tn, 1, 1, steps, 0, nullptr};
 }
 
-// Steps from .. to of a tile, added to acc; U steps' loads are issued before the first is used.
-template <Src SA, Src SB, int U>
+// Steps from .. to of a tile, added to acc.  U steps' loads are issued at a time;
+// AHEAD: a round's before the products of the one before.
+template <Src SA, Src SB, int U, bool AHEAD>
 __device__ __forceinline__ void direct_steps(const DirectProduct &p, int i0, int j0, int from, int to, int lane,
                                              f4v_t (&acc)[2][2]) {
     const int li = lane & 15, lq = lane >> 4;
-    for (int s0 = from; s0 < to; s0 += U) {
-        float a[U][2][4], b[U][2][4];
+    constexpr int R = AHEAD ? 2 : 1;
+    float a[R][U][2][4], b[R][U][2][4];
+    auto load = [&](int r, int s0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (s0 + u < to) {  // uniform
-                const int k = (s0 + u) * kDirectK + 4 * lq;
-                operand_pair<SA>(p.A, i0 + 2 * li, k, p.K, a[u]);
-                operand_pair<SB>(p.B, j0 + 2 * li, k, p.K, b[u]);
-            }
+            if (s0 + u >= to) break;  // uniform
+            const int k = (s0 + u) * kDirectK + 4 * lq;
+            operand_pair<SA>(p.A, i0 + 2 * li, k, p.K, a[r][u]);
+            operand_pair<SB>(p.B, j0 + 2 * li, k, p.K, b[r][u]);
         }
+    };
+    auto multiply = [&](int r, int s0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s0 + u >= to) break;  // uniform
@@ -65,7 +69,22 @@ __device__ __forceinline__ void direct_steps(const DirectProduct &p, int i0, int
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
-                        acc[x][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][x][s], b[u][c][s], acc[x][c], 0, 0, 0);
+                        acc[x][c] =
+                            __builtin_amdgcn_mfma_f32_16x16x4f32(a[r][u][x][s], b[r][u][c][s], acc[x][c], 0, 0, 0);
+        }
+    };
+    if constexpr (AHEAD) {
+        load(0, from);
+        for (int s0 = from; s0 < to; s0 += 2 * U) {
+            load(1, s0 + U);
+            multiply(0, s0);
+            load(0, s0 + 2 * U);
+            multiply(1, s0 + U);
+        }
+    } else {
+        for (int s0 = from; s0 < to; s0 += U) {
+            load(0, s0);
+            multiply(0, s0);
         }
     }
 }
@@ -78,13 +97,13 @@ __device__ __forceinline__ void direct_each(const f4v_t (&acc)[2][2], int lane, 
         for (int r = 0; r < 4; ++r) f(2 * (4 * (lane >> 4) + r) + x, 2 * (lane & 15), acc[x][0][r], acc[x][1][r]);
 }
 
-// A whole tile by one wave, with its epilogue (in few registers: what the large
-// products fall back to).
+// Steps from .. to of a tile by one wave, with the epilogue (in few registers:
+// what the large products fall back to).
 template <Src SA, Src SB>
-__device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, int lane) {
+__device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, int from, int to, int lane) {
     const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
     f4v_t acc[2][2] = {};
-    direct_steps<SA, SB, 1>(p, i0, j0, 0, (p.K + kDirectK - 1) / kDirectK, lane, acc);
+    direct_steps<SA, SB, 1, false>(p, i0, j0, from, to, lane, acc);
     direct_each(acc, lane, [&](int row, int col, float v0, float v1) {
         const int i = i0 + row, j = j0 + col;
         if (i >= p.M) return;
@@ -94,11 +113,11 @@ __device__ __forceinline__ void direct_tile(const DirectProduct &p, int tile, in
     });
 }
 
-// Workgroup `block` of a product; lds: a tile per wave.
+// Workgroup `block` of a product, of `waves` waves; lds: a tile per wave.
 template <Src SA, Src SB>
-__device__ __forceinline__ void direct_block(const DirectProduct &p, int block, float (*lds)[kDirectTile * kDirectTile]) {
+__device__ __forceinline__ void direct_block(const DirectProduct &p, int block, int waves, float (*lds)[kDirectTile * kDirectTile]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kg = p.kg, group = wave % kg, unit = block * (kDirectWaves / kg) + wave / kg;
+    const int kg = p.kg, group = wave % kg, unit = block * (waves / kg) + wave / kg;
     const bool live = unit < p.tiles * p.slices;  // uniform per wave; the others reach the barrier
     const int tile = unit / p.slices, slice = unit % p.slices;
     const int i0 = tile / p.tiles_n * kDirectTile, j0 = tile % p.tiles_n * kDirectTile;
@@ -107,7 +126,7 @@ __device__ __forceinline__ void direct_block(const DirectProduct &p, int block, 
         const int first = slice * p.slice_steps, last = min(first + p.slice_steps, steps);
         const int per = (last - first + kg - 1) / kg, from = first + group * per;
         f4v_t acc[2][2] = {};
-        direct_steps<SA, SB, 4>(p, i0, j0, from, min(from + per, last), lane, acc);
+        direct_steps<SA, SB, 2, true>(p, i0, j0, from, min(from + per, last), lane, acc);
         direct_each(acc, lane, [&](int row, int col, float v0, float v1) {
             float *to = &lds[wave][row * kDirectTile + col];
             to[0] = v0;
@@ -132,6 +151,9 @@ __device__ __forceinline__ void direct_block(const DirectProduct &p, int block, 
         }
     }
 }
+
+// A product's slices added in their order, with its epilogue (ts_hip_linear.hip).
+void join_slices(const DirectProduct &p, hipStream_t s);
 
 // Calls f with a product's operand kinds as constants: the layouts that a layer's products have.
 template <class F>

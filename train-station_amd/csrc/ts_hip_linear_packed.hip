@@ -196,6 +196,7 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
     if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;
     if (workspace_floats < ts_hip_linear_packed_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
     if (planes_take(batch, fan_out, fan_in)) {
+        if (!workspace && ts_hip_linear_packed_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EINVAL;
         LinearProduct q{};
         q.A = {nullptr, nullptr, x_codes, x_scales, 0, static_cast<int>(batch), packed_pitch(fan_in), batch};
         q.B = {nullptr, nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), packed_pitch(fan_in), fan_out};

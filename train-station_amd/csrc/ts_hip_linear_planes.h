@@ -49,6 +49,7 @@ struct PlanesArgs {
     int rows_a, rows_b;  // row blocks
     int stages;
     int tiles_m, tiles_n;
+    int slice_stages;    // p.slices > 1: a workgroup's stages, its sums to p.part
 };
 
 // One side's part of a stage of SK k blocks: R rows.
@@ -138,7 +139,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
 
     int tm, tn;
-    tile_coords(g.tiles_m, g.tiles_n, blockIdx.x, tm, tn);
+    const int slice = static_cast<int>(blockIdx.x) % g.p.slices;
+    tile_coords(g.tiles_m, g.tiles_n, static_cast<int>(blockIdx.x) / g.p.slices, tm, tn);
+    if (g.p.slices > 1) {  // uniform
+        g.p.C = g.p.part + static_cast<size_t>(slice) * g.p.M * g.p.N;
+        g.p.epi = LinearEpi{};
+    }
+    const int first = slice * g.slice_stages, end = min(first + g.slice_stages, g.stages);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -160,7 +167,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
         }
     }
     auto dma = [&](int stage, int slot) {
-        const int at = min(stage, g.stages - 1);  // past the end: the last again
+        const int at = min(stage, end - 1);  // past the end: the last again
         const unsigned base = lds0 + slot * kStage;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -203,9 +210,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
         for (int c = 0; c < FN; ++c) acc[x][c] = floatx16{};
 
 #pragma unroll
-    for (int s = 0; s < NST - 1; ++s) dma(s, s);
+    for (int s = 0; s < NST - 1; ++s) dma(first + s, s);
     int slot = 0;
-    for (int s = 0; s < g.stages; ++s) {
+    for (int s = first; s < end; ++s) {
         // this stage has landed, and every wave is done with the one before
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((PER + SPER) * (NST - 2)) : "memory");
         dma(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
@@ -282,7 +289,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
             constexpr int TN = BN / kDirectTile;
             for (int t = wave; t < BM / kDirectTile * TN; t += NW) {
                 const int ti = tm * (BM / kDirectTile) + t / TN, tj = tn * TN + t % TN;
-                if (ti * kDirectTile < g.p.M && tj < g.p.tiles_n) direct_tile<SA, SB>(g.p, ti * g.p.tiles_n + tj, lane);
+                if (ti * kDirectTile < g.p.M && tj < g.p.tiles_n) direct_tile<SA, SB>(g.p, ti * g.p.tiles_n + tj, first * SK, end * SK, lane);
             }
             return;
         }

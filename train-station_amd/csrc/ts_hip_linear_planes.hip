@@ -278,27 +278,45 @@ void launch_planes(PlanesArgs g, hipStream_t s) {
     g.tiles_m = (g.p.M + BM - 1) / BM;
     g.tiles_n = (g.p.N + BN - 1) / BN;
     g.stages = as_codes(SA, SB) ? static_cast<int>(g.p.A.pitch / kPackGroup) : g.kb / SK;
-    launch((linear_planes<SA, SB, BM, BN, 2, 2, SK, NST>), dim3(g.tiles_m * g.tiles_n), dim3(256), 0, s, g);
+    g.slice_stages = (g.stages + g.p.slices - 1) / g.p.slices;
+    launch((linear_planes<SA, SB, BM, BN, 2, 2, SK, NST>), dim3(g.tiles_m * g.tiles_n * g.p.slices), dim3(256), 0, s, g);
 }
 
-// The tile whose rounds over the chip cost least: rounds x its area, the smallest
-// tile 1.1 times as dear, and a larger one 1.3 times where a CU has but one
-// workgroup to fill its waits.  us in 128 x 128, 128 x 64, 64 x 64, pieces on both
-// sides: 8192 x 4096 x 4096 1284, 1295, 1381; 2048 x 4096 x 1024 93, 96, 99;
-// 1024 x 4096 x 2048 105, 90, 104; 2048 x 1024 x 4096 177, 122, 98; 1999 x 777 x
-// 1531 78, 53, 39.  One side's: 598, 662, 764; 52, 56, 59; 55, 54, 57; 87, 70, 57;
-// 46, 36, 28.  Codes: 260, 280, 324; 28.6, 30.4, 31.8; 32, 29, 31; 46, 35, 35; 26,
-// 22, 19.  (128 x 256 by eight waves: within 3 % of 128 x 128 at the largest, and
-// slower below; 256 x 256: slower.)
-enum class Tile { k128x128, k128x64, k64x64 };
-Tile choose_tile(size_t M, size_t N) {
+// The tile, and the slices of K, that cost least: rounds over the chip x a tile's
+// share of K x its area, the smallest tile 1.1 times as dear, and a larger one 1.3
+// times where a CU has but one workgroup to fill its waits; slices cost a launch
+// and their sums' way to memory and back.  us in 128 x 128, 128 x 64, 64 x 64,
+// pieces on both sides: 8192 x 4096 x 4096 1284, 1295, 1381; 2048 x 4096 x 1024 93,
+// 96, 99; 1024 x 4096 x 2048 105, 90, 104; 2048 x 1024 x 4096 177, 122, 98; 1999 x
+// 777 x 1531 78, 53, 39.  One side's: 598, 662, 764; 52, 56, 59; 55, 54, 57; 87, 70,
+// 57; 46, 36, 28.  Codes: 260, 280, 324; 28.6, 30.4, 31.8; 32, 29, 31; 46, 35, 35;
+// 26, 22, 19.  (128 x 256 by eight waves: within 3 % of 128 x 128 at the largest,
+// and slower below; 256 x 256: slower.)
+struct PlanesPlan {
+    int bm, bn, slices;
+};
+PlanesPlan choose_plan(size_t M, size_t N, size_t K, Src a, Src b) {
     const size_t cus = device_cu_count();
-    auto cost = [&](size_t bm, size_t bn, double each) {
-        const size_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn), rounds = (tiles + cus - 1) / cus;
-        return rounds * bm * bn * each * (rounds == 1 && bm > 64 ? 1.3 : 1.0);
+    const double each = as_codes(a, b) ? 0.8e-6 : of_codes(a) ? 1.4e-6 : 2.6e-6;  // us per k of a column of a tile, one a CU
+    PlanesPlan best = {128, 128, 1};
+    double least = 1e30;
+    auto take = [&](size_t bm, size_t bn, double dear) {
+        const size_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
+        for (size_t n = 1; n <= 8 && (n == 1 || (K >= n * 512 && tiles * n <= 4 * cus)); n *= 2) {
+            const size_t rounds = (tiles * n + cus - 1) / cus;
+            double us = rounds * bm * bn * dear * each * K / n;
+            if (rounds == 1 && bm > 64) us *= 1.3;
+            if (n > 1) us += 6 + 2e-6 * M * N * n;
+            if (us < least) {
+                least = us;
+                best = {static_cast<int>(bm), static_cast<int>(bn), static_cast<int>(n)};
+            }
+        }
     };
-    const double a = cost(128, 128, 1.0), b = cost(128, 64, 1.0), c = cost(64, 64, 1.1);
-    return a <= b && a <= c ? Tile::k128x128 : b <= c ? Tile::k128x64 : Tile::k64x64;
+    take(128, 128, 1.0);
+    take(128, 64, 1.0);
+    take(64, 64, 1.1);
+    return best;
 }
 
 size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -308,8 +326,9 @@ size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 bool planes_take(size_t M, size_t N, size_t K) { return 2.0 * M * N * K >= 1.5e9 && M >= 128 && N >= 128 && K >= 64; }
 
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b) {
-    if (as_codes(a, b)) return 0;
-    return (round_256(plane_bytes(M, K, a)) + round_256(plane_bytes(N, K, b))) / sizeof(float);
+    const PlanesPlan plan = choose_plan(M, N, K, a, b);
+    const size_t planes = as_codes(a, b) ? 0 : (round_256(plane_bytes(M, K, a)) + round_256(plane_bytes(N, K, b))) / sizeof(float);
+    return planes + (plan.slices > 1 ? plan.slices * M * N : 0);
 }
 
 size_t planes_sum_floats(size_t N, size_t K) { return static_cast<size_t>(across_chunks(N, K)) * N; }
@@ -326,17 +345,21 @@ int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *work
         write_planes(p.A, p.a, p.K, !of_codes(p.a), pa, of_a, s);
         write_planes(p.B, p.b, p.K, false, pb, of_b, s);
     }
-    const PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0};
-    const Tile tile = choose_tile(p.M, p.N);
+    const PlanesPlan plan = choose_plan(p.M, p.N, p.K, p.a, p.b);
+    PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0, 0};
+    g.p.slices = plan.slices;
+    if (plan.slices > 1)
+        g.p.part = as_codes(p.a, p.b) ? workspace : reinterpret_cast<float *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
     with_sources(p.a, p.b, [&](auto a, auto b) {
         constexpr Src A = a.value, B = b.value;
         constexpr bool codes = as_codes(A, B), three = pieces_of(A) == 3;
         // stages: of 128 codes; else of 16 k, three or four of them (two of 32 for one piece beside three:
         // 8192 x 4096 x 4096 598 us, against 700 in four of 16)
-        if (tile == Tile::k128x128) launch_planes<A, B, 128, 128, codes ? 8 : three ? 1 : 2, codes || !three ? 2 : 3>(g, s);
-        else if (tile == Tile::k128x64) launch_planes<A, B, 128, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
-        else launch_planes<A, B, 64, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
+        if (plan.bm == 64) launch_planes<A, B, 64, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
+        else if (plan.bn == 64) launch_planes<A, B, 128, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
+        else launch_planes<A, B, 128, 128, codes ? 8 : three ? 1 : 2, codes || !three ? 2 : 3>(g, s);
     });
+    join_slices(g.p, s);
     return launch_status();
 }
 
