@@ -617,10 +617,13 @@ int ts_hip_rms_norm_packed(const float *x, const float *residual, const float *w
 /* The gradients of y = h r weight, r = 1 / sqrt(mean(h^2) + eps), from go = dy:
  *   dh = r (go weight) - h r^3 mean(go weight h),  dweight = sum over rows of go h r
  * Either may be NULL.  The workspace is needed for dweight.  A pass adds in a
- * fixed order, so equal calls give equal bits. */
+ * fixed order, so equal calls give equal bits.  ticket (may be NULL: one launch
+ * more) points to a device word that is zero, and is zero again when the call has
+ * run; calls that share it must run one after another (one stream). */
 size_t ts_hip_rms_norm_backward_workspace_floats(size_t rows, size_t cols);
 int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
-                             float *dh, float *dweight, float *workspace, size_t workspace_floats, void *stream);
+                             float *dh, float *dweight, float *workspace, size_t workspace_floats, unsigned *ticket,
+                             void *stream);
 
 /* Activations of a layer: none, max(z, 0), z s(z) with s(v) = 1 / (1 + e^-v), and
  * z s(2 sqrt(2 / pi) (z + 0.044715 z^3)) (the tanh form of gelu). */

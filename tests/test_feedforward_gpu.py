@@ -155,6 +155,23 @@ def test_rms_norm_packed(rows, cols, residual):
     assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 5), (128, 784), (700, 64), (3000, 1000)])
+def test_norm_backward_with_and_without_a_ticket(rows, cols):
+    """The same sums by one launch and by two, to the last place, and the ticket zero again."""
+    h, go = Dev.of(normal((rows, cols), 1)), Dev.of(normal((rows, cols), 2))
+    w, ticket = Dev.of(normal((cols,), 3)), Dev.of(np.zeros(1, np.float32))
+    floats = hip.ts_hip_rms_norm_backward_workspace_floats(rows, cols)
+    work, got = Dev(floats), []
+    for t in (None, ticket.ptr, ticket.ptr):
+        dh, dw = Dev(rows * cols), Dev(cols)
+        hip_check(hip.ts_hip_rms_norm_backward(h.ptr, w.ptr, go.ptr, rows, cols, 1e-6, dh.ptr, dw.ptr, work.ptr, floats, t,
+                                               None))
+        got.append((dh.get(), dw.get()))
+    assert not ticket.get().view(np.uint32).any()
+    for dh, dw in got[1:]:
+        assert np.array_equal(dh, got[0][0]) and np.allclose(dw, got[0][1], rtol=2e-7, atol=0)
+
+
 def test_norm_of_zero_and_tiny_and_huge_rows():
     x = np.zeros((4, 40), np.float32)
     x[1], x[2], x[3, 5] = 1e-30, 1e30, np.nan

@@ -109,9 +109,9 @@ def test_norm_entries_refuse():
     assert f(None, None, None, 0, 8, 1e-6, None, None, None) == 0
     assert hip.ts_hip_rms_norm_packed(P, None, P, 4, 8, 1e-6, None, P, None, None) == EINVAL
     b = hip.ts_hip_rms_norm_backward
-    assert b(P, P, None, 4, 8, 1e-6, P, None, None, 0, None) == EINVAL
-    assert b(P, P, P, 4, 8, 1e-6, None, P, None, 0, None) == EWORKSPACE
-    assert b(P, P, P, 4, 8, 1e-6, None, None, None, 0, None) == 0
+    assert b(P, P, None, 4, 8, 1e-6, P, None, None, 0, None, None) == EINVAL
+    assert b(P, P, P, 4, 8, 1e-6, None, P, None, 0, None, None) == EWORKSPACE
+    assert b(P, P, P, 4, 8, 1e-6, None, None, None, 0, None, None) == 0
     assert hip.ts_hip_pack8(None, 4, 8, P, P, None) == EINVAL and hip.ts_hip_pack8(P, 4, 8, P, None, None) == EINVAL
     assert hip.ts_hip_unpack8(P, P, 4, 8, None, None) == EINVAL
 

@@ -190,7 +190,7 @@ HIP_SIGNATURES = {
     "ts_hip_rms_norm": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP]),
     "ts_hip_rms_norm_packed": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, VP]),
     "ts_hip_rms_norm_backward_workspace_floats": (SZ, [SZ, SZ]),
-    "ts_hip_rms_norm_backward": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, SZ, VP]),
+    "ts_hip_rms_norm_backward": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, SZ, VP, VP]),
     "ts_hip_linear_packed_workspace_floats": (SZ, [SZ, SZ, SZ]),
     "ts_hip_linear_packed": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, SZ, VP, _c.c_int, VP, VP, VP, SZ, VP]),
     "ts_hip_linear_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),

@@ -143,7 +143,7 @@ std::vector<std::optional<Tensor>> rms_norm_backward(const GradFn &fn, const Ten
         float *dhp = fn.req_left ? dh.dev_mut() : nullptr, *dwp = fn.req_right ? dw.dev_mut() : nullptr;
         launch(KernelClass::Reduction, (fn.req_left ? 12.0 : 8.0) * go.size() + 8.0 * cols, "ts_hip_rms_norm_backward", [&] {
             return ts_hip_rms_norm_backward(hp, wp, gp, rows, cols, fn.scalar, dhp, dwp, work ? work->get() : nullptr, ws,
-                                            S());
+                                            Runtime::get().ticket(), S());
         });
     }
     std::vector<std::optional<Tensor>> r(2);

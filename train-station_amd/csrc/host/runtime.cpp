@@ -24,6 +24,10 @@ Runtime::Runtime() {
     check(ts_hip_malloc(&w, 2), "ts_hip_malloc(zero index)");
     zero_index_ = reinterpret_cast<unsigned long long *>(w);
     check(ts_hip_memcpy(w, reinterpret_cast<const float *>(&kNoZero), 2, 0), "ts_hip_memcpy");
+    const float zero = 0.0f;  // all bits 0
+    check(ts_hip_malloc(&w, 1), "ts_hip_malloc(ticket)");
+    check(ts_hip_memcpy(w, &zero, 1, 0), "ts_hip_memcpy");
+    ticket_ = reinterpret_cast<unsigned *>(w);
 }
 
 Runtime &Runtime::get() {

@@ -50,6 +50,8 @@ class Runtime {
     static Runtime &get();
     void *stream() const { return stream_; }
     unsigned long long *zero_index() const { return zero_index_; }
+    // a device word that is zero between the launches that count in it
+    unsigned *ticket() const { return ticket_; }
     // Waits for queued work; throws the reference's division-by-zero panic
     // message if a division kernel recorded a zero divisor.
     void sync();
@@ -58,6 +60,7 @@ class Runtime {
     Runtime();
     void *stream_ = nullptr;
     unsigned long long *zero_index_ = nullptr;
+    unsigned *ticket_ = nullptr;
 };
 
 // Size-bucketed caching allocator for device buffers.  All work runs on the

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kBlock) void linear_join(DirectProduct p, DirectPro
 }
 
 // How a product's tiles share the chip: up to eight waves a tile while there are
-// fewer than four a SIMD and each has four steps of its own (one round of loads);
+// fewer than four a SIMD and each has two steps of its own (one round of loads);
 // then slices of eight steps a wave, up to as many.
 struct DirectPlan {
     int kg, slices, slice_steps;
@@ -104,7 +104,7 @@ DirectPlan direct_plan(size_t M, size_t N, size_t K) {
     const size_t tiles = ((M + kDirectTile - 1) / kDirectTile) * ((N + kDirectTile - 1) / kDirectTile);
     const size_t waves = static_cast<size_t>(device_cu_count()) * 16, steps = (K + kDirectK - 1) / kDirectK;
     DirectPlan p = {1, 1, static_cast<int>(steps)};
-    while (p.kg < kDirectWaves && tiles * p.kg * 2 <= waves && steps >= static_cast<size_t>(p.kg) * 2 * 4) p.kg *= 2;
+    while (p.kg < kDirectWaves && tiles * p.kg * 2 <= waves && steps >= static_cast<size_t>(p.kg) * 2 * 2) p.kg *= 2;
     if (p.kg == kDirectWaves && steps > 16 * kDirectWaves) {
         const size_t want = steps / (8 * kDirectWaves), room = waves / (tiles * kDirectWaves);
         const size_t n = want < room ? want : room;

@@ -151,6 +151,8 @@ struct NormBackArgs {
     float *dh, *dw_part;  // dw_part: [gridDim.x][cols]
     size_t rows, cols;
     double eps;
+    float *dw;         // with a ticket: the last workgroup adds the parts up
+    unsigned *ticket;  // zero, and zero again when the launch has run; null: none
 };
 
 // Rows blockIdx.x * RPB + slot, and on by the grid's; a thread keeps dw's sums
@@ -246,22 +248,41 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
                     for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = dw[i][e];
             }
             __syncthreads();
-            if (slot > 0) return;
+            if (slot == 0) {
 #pragma unroll
-            for (int k = 0; k < RPB - 1; ++k)
+                for (int k = 0; k < RPB - 1; ++k)
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+                    for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dw[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
+                        for (int e = 0; e < 4; ++e) dw[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
+            }
         }
+        if (slot == 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t c = 4 * (t + 64 * W * i);
-            float o[4];
+            for (int i = 0; i < NV; ++i) {
+                const size_t c = 4 * (t + 64 * W * i);
+                float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw[i][e]);
-            if (c < a.cols) store4(part, c, a.cols, o);
+                for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw[i][e]);
+                if (c < a.cols) store4(part, c, a.cols, o);
+            }
         }
+    }
+    if (DW && a.ticket) {  // uniform: the last workgroup to get here adds the parts up
+        __shared__ bool last;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+        __syncthreads();
+        if (!last) return;
+        __threadfence();
+        for (size_t c = threadIdx.x; c < a.cols; c += kNormThreads<W>) {
+            double s = 0.0;
+#pragma unroll 16
+            for (size_t g = 0; g < gridDim.x; ++g) s += a.dw_part[g * a.cols + c];
+            a.dw[c] = static_cast<float>(s);
+        }
+        if (threadIdx.x == 0) *a.ticket = 0;
     }
 }
 
@@ -337,6 +358,10 @@ size_t back_blocks(size_t rows, size_t cols) {
 }
 
 constexpr size_t kMaxRows = size_t(1) << 31;
+// Parts that one workgroup adds up sooner than another launch has started: 128 x 784
+// (32 parts) forward and backward 26.8 us by two launches, 24.5 by one; 16384 x 64
+// (512 parts) 27.1 by two, 69 by one.
+constexpr size_t kTicketParts = 64, kTicketFloats = 32768;
 
 }  // namespace
 
@@ -391,19 +416,21 @@ int ts_hip_rms_norm_packed(const float *x, const float *residual, const float *w
 size_t ts_hip_rms_norm_backward_workspace_floats(size_t rows, size_t cols) { return back_blocks(rows, cols) * cols; }
 
 int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
-                             float *dh, float *dweight, float *workspace, size_t workspace_floats, void *stream) {
+                             float *dh, float *dweight, float *workspace, size_t workspace_floats, unsigned *ticket,
+                             void *stream) {
     if (cols == 0 || (!dh && !dweight)) return TS_HIP_OK;
     if (rows == 0) return dweight ? ts_hip_fill(dweight, 0.0f, cols, stream) : TS_HIP_OK;
     if (!h || !weight || !go || rows >= kMaxRows) return TS_HIP_EINVAL;
     if (dweight && (!workspace || workspace_floats < ts_hip_rms_norm_backward_workspace_floats(rows, cols)))
         return TS_HIP_EWORKSPACE;
     const unsigned grid = static_cast<unsigned>(back_blocks(rows, cols));
-    const NormBackArgs a = {h, weight, go, dh, dweight ? workspace : nullptr, rows, cols, eps};
+    if (!dweight || grid > kTicketParts || grid * cols > kTicketFloats) ticket = nullptr;
+    const NormBackArgs a = {h, weight, go, dh, dweight ? workspace : nullptr, rows, cols, eps, dweight, ticket};
     const hipStream_t s = as_stream(stream);
     for_cols(cols, [&](auto w, auto nv, auto long_rows) {
         launch_back<w.value, nv.value, long_rows.value>(a, grid, s);
     });
-    if (dweight)
+    if (dweight && !ticket)
         launch(sum_parts, dim3(static_cast<unsigned>((cols + 15) / 16)), dim3(kBlock), 0, s,
                static_cast<const float *>(workspace), static_cast<size_t>(grid), cols, dweight);
     return launch_status();
