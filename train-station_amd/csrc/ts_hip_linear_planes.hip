@@ -25,6 +25,18 @@ __device__ __forceinline__ void store_pieces(char *to, const float (&v)[8], floa
     q[2 * kFragBytes / 16] = l;
 }
 
+// One operand's part of a pass: its waves' jobs, in `blocks` workgroups.
+struct PlaneJob {
+    Operand o;
+    int K, kb;            // the product's k, in k blocks
+    char *out;
+    int chunks;           // floats along k: jobs of a row block
+    int run, row_blocks;  // along the rows: k blocks of a job
+    unsigned blocks;
+    uint8_t *codes, *scales;  // floats along k: the values in 8 bits too
+    float *sum_parts;         // floats along the rows: their sums, [chunk][rows]
+};
+
 // ---- floats along k ----------------------------------------------------------------
 // A wave takes a row block and eight k blocks (512 bytes of each row).  NEG: odd k
 // blocks negated.  PACK: the values in 8 bits too; a block of 32 k is two k blocks
@@ -32,16 +44,14 @@ __device__ __forceinline__ void store_pieces(char *to, const float (&v)[8], floa
 constexpr int kAlongBlocks = 8;
 
 template <bool NEG, bool PACK, bool TIMES>
-__global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__ x, const float *__restrict__ times, int ld, int rows, int K, int kb,
-                                                       char *__restrict__ out, uint8_t *__restrict__ codes,
-                                                       uint8_t *__restrict__ scales, size_t pitch, int chunks) {
-    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
-    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
-    const int rb = static_cast<int>(job / chunks), b0 = static_cast<int>(job % chunks) * kAlongBlocks;
+__device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, rows = j.o.rows, K = j.K, kb = j.kb;
+    const int rb = static_cast<int>(job / j.chunks), b0 = static_cast<int>(job % j.chunks) * kAlongBlocks;
     if (rb * kPlaneRows >= rows) return;
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
-    const float *p = x + static_cast<size_t>(live ? row : 0) * ld, *tp = TIMES ? times + (p - x) : nullptr;
+    const size_t at = static_cast<size_t>(live ? row : 0) * j.o.ld;
+    const float *p = j.o.p + at, *tp = TIMES ? j.o.times + at : nullptr;
     float v[kAlongBlocks][8];
 #pragma unroll
     for (int b = 0; b < kAlongBlocks; ++b)
@@ -64,10 +74,11 @@ __global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__
 #pragma unroll
     for (int b = 0; b < kAlongBlocks; ++b) {
         if (b0 + b >= kb) break;  // uniform
-        store_pieces(out + (static_cast<size_t>(rb) * kb + b0 + b) * 3 * kFragBytes, v[b],
+        store_pieces(j.out + (static_cast<size_t>(rb) * kb + b0 + b) * 3 * kFragBytes, v[b],
                      NEG && (b & 1) ? -kSplitScale : kSplitScale, lane);
     }
     if (PACK) {
+        const size_t pitch = packed_pitch(K);
 #pragma unroll
         for (int b = 0; b < kAlongBlocks; b += 2) {
             const size_t c = static_cast<size_t>(b0 + b) * kPlaneK;
@@ -87,10 +98,10 @@ __global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__
                     lo[e] = v[b + t][e];
                     hi[e] = v[b + t][4 + e];
                 }
-                *reinterpret_cast<u2v_t *>(codes + row * pitch + c + t * kPlaneK + 8 * h) = u2v_t{pack4(lo, inv), pack4(hi, inv)};
+                *reinterpret_cast<u2v_t *>(j.codes + row * pitch + c + t * kPlaneK + 8 * h) = u2v_t{pack4(lo, inv), pack4(hi, inv)};
             }
             if (h == 0)
-                scales[(c / kPackGroup * rows + row) * 4 + c / kPackBlock % 4] = static_cast<uint8_t>(k + kPackBias);
+                j.scales[(c / kPackGroup * rows + row) * 4 + c / kPackBlock % 4] = static_cast<uint8_t>(k + kPackBias);
         }
     }
 }
@@ -99,17 +110,14 @@ __global__ __launch_bounds__(kBlock) void planes_along(const float *__restrict__
 // element (row, k) at x[k * ld + row].  A wave takes a row block and `run` k
 // blocks.  SUM: the rows' sums over them (f64) to part[chunk][rows].
 template <bool NEG, bool SUM, bool TIMES>
-__global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict__ x, const float *__restrict__ times, int ld, int rows, int K, int kb,
-                                                        char *__restrict__ out, float *__restrict__ part, int run,
-                                                        int row_blocks) {
-    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
-    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
-    const int rb = static_cast<int>(job % row_blocks), chunk = static_cast<int>(job / row_blocks);
-    const int from = chunk * run, to = min(from + run, kb);
+__device__ __forceinline__ void planes_across(const PlaneJob &j, size_t job) {
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, ld = j.o.ld, rows = j.o.rows, K = j.K, kb = j.kb;
+    const int rb = static_cast<int>(job % j.row_blocks), chunk = static_cast<int>(job / j.row_blocks);
+    const int from = chunk * j.run, to = min(from + j.run, kb);
     if (from >= kb) return;
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
-    const float *p = x + (live ? row : 0), *tp = TIMES ? times + (p - x) : nullptr;
+    const float *p = j.o.p + (live ? row : 0), *tp = TIMES ? j.o.times + (live ? row : 0) : nullptr;
     double sum = 0.0;
 #pragma unroll 2
     for (int b = from; b < to; ++b) {
@@ -137,52 +145,49 @@ __global__ __launch_bounds__(kBlock) void planes_across(const float *__restrict_
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum += v[e];
         }
-        store_pieces(out + (static_cast<size_t>(rb) * kb + b) * 3 * kFragBytes, v, NEG && (b & 1) ? -kSplitScale : kSplitScale,
+        store_pieces(j.out + (static_cast<size_t>(rb) * kb + b) * 3 * kFragBytes, v, NEG && (b & 1) ? -kSplitScale : kSplitScale,
                      lane);
     }
     if (SUM) {
         sum += __shfl_xor(sum, 32, 64);
-        if (h == 0 && live) part[static_cast<size_t>(chunk) * rows + row] = static_cast<float>(sum);
+        if (h == 0 && live) j.sum_parts[static_cast<size_t>(chunk) * rows + row] = static_cast<float>(sum);
     }
 }
 
 // ---- codes -----------------------------------------------------------------------------
 
 // Codes along k.  A wave takes a row block and a group of 128 k, the lane's scales in one word.
-__global__ __launch_bounds__(kBlock) void planes_codes_along(const uint8_t *__restrict__ codes,
-                                                             const uint8_t *__restrict__ scales, int rows, size_t pitch,
-                                                             int kb, char *__restrict__ out) {
-    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+__device__ __forceinline__ void planes_codes_along(const PlaneJob &j, size_t job) {
+    const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, rows = j.o.rows, kb = j.kb;
+    const size_t pitch = j.o.pitch;
     const int groups = static_cast<int>(pitch / kPackGroup);
-    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
     const int rb = static_cast<int>(job / groups), g = static_cast<int>(job % groups);
     if (rb * kPlaneRows >= rows) return;
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
     const size_t r = live ? row : 0;
-    const unsigned four = reinterpret_cast<const unsigned *>(scales)[static_cast<size_t>(g) * rows + r];
+    const unsigned four = reinterpret_cast<const unsigned *>(j.o.scales)[static_cast<size_t>(g) * rows + r];
     u2v_t c[8];
 #pragma unroll
     for (int b = 0; b < 8; ++b)
-        c[b] = *reinterpret_cast<const u2v_t *>(codes + r * pitch + static_cast<size_t>(g) * kPackGroup + b * kPlaneK + 8 * h);
+        c[b] = *reinterpret_cast<const u2v_t *>(j.o.codes + r * pitch + static_cast<size_t>(g) * kPackGroup + b * kPlaneK + 8 * h);
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
         if (g * 8 + b >= kb) break;  // uniform
         bf8_t w = widen(c[b][0], c[b][1], pow2f(static_cast<int>(four >> (8 * (b / 2)) & 255u) - kPackBias));
         if (!live) w = bf8_t{};
-        *(reinterpret_cast<bf8_t *>(out + (static_cast<size_t>(rb) * kb + g * 8 + b) * kFragBytes) + lane) = w;
+        *(reinterpret_cast<bf8_t *>(j.out + (static_cast<size_t>(rb) * kb + g * 8 + b) * kFragBytes) + lane) = w;
     }
 }
 
 // Codes along the rows: k is the code row, the product's rows its columns.  A wave
 // takes 32 columns (a row block, and a scale's block) of 64 code rows; a lane four
 // columns of eight.
-__global__ __launch_bounds__(kBlock) void planes_codes_across(const uint8_t *__restrict__ codes,
-                                                              const uint8_t *__restrict__ scales, int code_rows,
-                                                              size_t pitch, int kb, int row_blocks, char *__restrict__ out) {
-    const int lane = threadIdx.x & 63, i = lane & 7, o = lane >> 3;
-    const size_t job = static_cast<size_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
-    const int rb = static_cast<int>(job % row_blocks), b0 = static_cast<int>(job / row_blocks) * 4;
+__device__ __forceinline__ void planes_codes_across(const PlaneJob &j, size_t job) {
+    const int lane = threadIdx.x & 63, i = lane & 7, o = lane >> 3, kb = j.kb, code_rows = static_cast<int>(j.o.code_rows);
+    const uint8_t *codes = j.o.codes, *scales = j.o.scales;
+    const size_t pitch = j.o.pitch;
+    const int rb = static_cast<int>(job % j.row_blocks), b0 = static_cast<int>(job / j.row_blocks) * 4;
     if (b0 >= kb) return;
     const int k0 = b0 * kPlaneK + 8 * o;
     const size_t col = static_cast<size_t>(rb) * kPlaneRows;
@@ -204,13 +209,31 @@ __global__ __launch_bounds__(kBlock) void planes_codes_across(const uint8_t *__r
         lo[e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s[e], false);
         hi[e] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[e], s[e], true);
     }
-    bf8_t *to = reinterpret_cast<bf8_t *>(out + (static_cast<size_t>(rb) * kb + b) * kFragBytes) + 32 * h + 4 * i;
+    bf8_t *to = reinterpret_cast<bf8_t *>(j.out + (static_cast<size_t>(rb) * kb + b) * kFragBytes) + 32 * h + 4 * i;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         bf8_t w;
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = n < 2 ? lo[e][n & 1] : hi[e][n & 1];
         to[n] = w;
+    }
+}
+
+// Both operands of a product, A's jobs first.  PACK and SUM: of A along k, of B
+// along its rows; TIMES: of the operand that is a layer's dz.
+template <Src SA, Src SB, bool PACK, bool SUM, bool TIMES>
+__global__ __launch_bounds__(kBlock) void write_planes(PlaneJob a, PlaneJob b) {
+    const bool first = blockIdx.x < a.blocks;  // uniform
+    const size_t job = static_cast<size_t>(first ? blockIdx.x : blockIdx.x - a.blocks) * (kBlock / 64) + (threadIdx.x >> 6);
+    if (first) {
+        if constexpr (SA == Src::kFloatK) planes_along<true, PACK, TIMES>(a, job);
+        else if constexpr (SA == Src::kFloatR) planes_across<true, false, false>(a, job);
+        else if constexpr (SA == Src::kCodesK) planes_codes_along(a, job);
+        else planes_codes_across(a, job);
+    } else if constexpr (SB == Src::kFloatK) {
+        planes_along<false, false, false>(b, job);
+    } else {
+        planes_across<false, SUM, TIMES && SA != Src::kFloatK>(b, job);
     }
 }
 
@@ -235,41 +258,44 @@ int across_chunks(size_t rows, size_t K) {
     return (k_blocks(K) + run - 1) / run;
 }
 
-void write_planes(const Operand &o, Src src, int K, bool negate, char *out, const PlanesExtra &x, hipStream_t s) {
-    const int rows = o.rows, kb = k_blocks(K), rb = row_blocks(rows);
-    const dim3 block(kBlock);
+PlaneJob plane_job(const Operand &o, Src src, int K, char *out, const PlanesExtra &x) {
+    PlaneJob j = {o, K, k_blocks(K), out, 0, 0, row_blocks(o.rows), 0, x.codes, x.scales, x.sum_parts};
+    const size_t rb = j.row_blocks;
     if (src == Src::kFloatK) {
-        const size_t pitch = packed_pitch(K);
-        const int blocks = x.codes ? static_cast<int>(pitch / kPlaneK) : kb;
-        const int chunks = (blocks + kAlongBlocks - 1) / kAlongBlocks;
-        const dim3 grid(wave_grid(static_cast<size_t>(rb) * chunks));
-        auto along = [&](auto kernel) {
-            launch(kernel, grid, block, 0, s, o.p, o.times, o.ld, rows, K, kb, out, x.codes, x.scales, pitch, chunks);
-        };
-        if (x.codes) along(planes_along<true, true, false>);
-        else if (negate && o.times) along(planes_along<true, false, true>);
-        else if (negate) along(planes_along<true, false, false>);
-        else along(planes_along<false, false, false>);
+        const size_t blocks = x.codes ? packed_pitch(K) / kPlaneK : j.kb;
+        j.chunks = static_cast<int>((blocks + kAlongBlocks - 1) / kAlongBlocks);
+        j.blocks = wave_grid(rb * j.chunks);
     } else if (src == Src::kFloatR) {
-        const int run = across_run(rows, K), chunks = across_chunks(rows, K);
-        const dim3 grid(wave_grid(static_cast<size_t>(rb) * chunks));
-        auto across = [&](auto kernel) {
-            launch(kernel, grid, block, 0, s, o.p, o.times, o.ld, rows, K, kb, out, x.sum_parts, run, rb);
-        };
-        if (x.sums && o.times) across(planes_across<false, true, true>);
-        else if (x.sums) across(planes_across<false, true, false>);
-        else if (negate) across(planes_across<true, false, false>);
-        else if (o.times) across(planes_across<false, false, true>);
-        else across(planes_across<false, false, false>);
-        if (x.sums)
-            launch(sum_parts, dim3((rows + 15) / 16), block, 0, s, static_cast<const float *>(x.sum_parts),
-                   static_cast<size_t>(chunks), static_cast<size_t>(rows), x.sums);
-    } else if (src == Src::kCodesK) {
-        launch(planes_codes_along, dim3(wave_grid(static_cast<size_t>(rb) * (o.pitch / kPackGroup))), block, 0, s, o.codes,
-               o.scales, rows, o.pitch, kb, out);
+        j.run = across_run(o.rows, K);
+        j.blocks = wave_grid(rb * across_chunks(o.rows, K));
     } else {
-        launch(planes_codes_across, dim3(wave_grid(static_cast<size_t>(rb) * ((kb + 3) / 4))), block, 0, s, o.codes, o.scales,
-               static_cast<int>(o.code_rows), o.pitch, kb, rb, out);
+        j.blocks = wave_grid(rb * (src == Src::kCodesK ? o.pitch / kPackGroup : (j.kb + 3) / 4));
+    }
+    return j;
+}
+
+// The planes of both operands by one launch, with what goes beside them.
+template <Src SA, Src SB>
+void launch_write(const LinearProduct &p, const PlanesExtra &x, char *pa, char *pb, hipStream_t s) {
+    const PlaneJob a = plane_job(p.A, SA, p.K, pa, x), b = plane_job(p.B, SB, p.K, pb, SB == Src::kFloatR ? x : PlanesExtra{});
+    const dim3 grid(a.blocks + b.blocks), block(kBlock);
+    if constexpr (SA == Src::kFloatK && SB == Src::kFloatR) {
+        if (x.codes) launch((write_planes<SA, SB, true, false, false>), grid, block, 0, s, a, b);
+        else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
+    } else if constexpr (SA == Src::kFloatK) {
+        if (p.A.times) launch((write_planes<SA, SB, false, false, true>), grid, block, 0, s, a, b);
+        else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
+    } else if constexpr (SA == Src::kCodesK) {
+        launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
+    } else if (x.sums) {
+        if (p.B.times) launch((write_planes<SA, SB, false, true, true>), grid, block, 0, s, a, b);
+        else launch((write_planes<SA, SB, false, true, false>), grid, block, 0, s, a, b);
+        const size_t rows = p.B.rows, chunks = across_chunks(rows, p.K);
+        launch(sum_parts, dim3(static_cast<unsigned>((rows + 15) / 16)), block, 0, s, static_cast<const float *>(x.sum_parts),
+               chunks, rows, x.sums);
+    } else {
+        if (p.B.times) launch((write_planes<SA, SB, false, false, true>), grid, block, 0, s, a, b);
+        else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
     }
 }
 
@@ -336,15 +362,6 @@ size_t planes_sum_floats(size_t N, size_t K) { return static_cast<size_t>(across
 int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s) {
     char *pa = reinterpret_cast<char *>(workspace);
     char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
-    if (!as_codes(p.a, p.b)) {
-        PlanesExtra of_a, of_b;
-        of_a.codes = extra.codes;
-        of_a.scales = extra.scales;
-        of_b.sums = extra.sums;
-        of_b.sum_parts = extra.sum_parts;
-        write_planes(p.A, p.a, p.K, !of_codes(p.a), pa, of_a, s);
-        write_planes(p.B, p.b, p.K, false, pb, of_b, s);
-    }
     const PlanesPlan plan = choose_plan(p.M, p.N, p.K, p.a, p.b);
     PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0, 0};
     g.p.slices = plan.slices;
@@ -353,6 +370,7 @@ int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *work
     with_sources(p.a, p.b, [&](auto a, auto b) {
         constexpr Src A = a.value, B = b.value;
         constexpr bool codes = as_codes(A, B), three = pieces_of(A) == 3;
+        if constexpr (!codes) launch_write<A, B>(p, extra, pa, pb, s);
         // stages: of 128 codes; else of 16 k, three or four of them (two of 32 for one piece beside three:
         // 8192 x 4096 x 4096 598 us, against 700 in four of 16)
         if (plan.bm == 64) launch_planes<A, B, 64, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
