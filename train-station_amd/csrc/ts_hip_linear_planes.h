@@ -33,6 +33,7 @@
 
 #include "ts_hip_gemm_split.h"
 #include "ts_hip_linear_direct.h"
+#include "ts_hip_parts.h"
 
 namespace tship {
 
@@ -50,6 +51,7 @@ struct PlanesArgs {
     int stages;
     int tiles_m, tiles_n;
     int slice_stages;    // p.slices > 1: a workgroup's stages, its sums to p.part
+    PartSums sums;       // a weight's gradient: dz's column sums, by workgroups past the tiles'
 };
 
 // One side's part of a stage of SK k blocks: R rows.
@@ -138,6 +140,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     constexpr int kScalesAt = A::kBytes + B::kBytes, kStage = kScalesAt + 256 * NSC;
     __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
 
+    if constexpr (SA == Src::kFloatR || SA == Src::kCodesR) {
+        const int past = static_cast<int>(blockIdx.x) - g.tiles_m * g.tiles_n * g.p.slices;
+        if (past >= 0) return part_sums_block(g.sums, past, reinterpret_cast<double *>(lds));  // uniform
+    }
     int tm, tn;
     const int slice = static_cast<int>(blockIdx.x) % g.p.slices;
     tile_coords(g.tiles_m, g.tiles_n, static_cast<int>(blockIdx.x) / g.p.slices, tm, tn);

@@ -1,7 +1,6 @@
 // The passes that write an operand's planes and the launches of the large
 // products (the kernel and the layout: ts_hip_linear_planes.h).
 #include "ts_hip_linear_planes.h"
-#include "ts_hip_parts.h"
 
 namespace tship {
 
@@ -290,9 +289,6 @@ void launch_write(const LinearProduct &p, const PlanesExtra &x, char *pa, char *
     } else if (x.sums) {
         if (p.B.times) launch((write_planes<SA, SB, false, true, true>), grid, block, 0, s, a, b);
         else launch((write_planes<SA, SB, false, true, false>), grid, block, 0, s, a, b);
-        const size_t rows = p.B.rows, chunks = across_chunks(rows, p.K);
-        launch(sum_parts, dim3(static_cast<unsigned>((rows + 15) / 16)), block, 0, s, static_cast<const float *>(x.sum_parts),
-               chunks, rows, x.sums);
     } else {
         if (p.B.times) launch((write_planes<SA, SB, false, false, true>), grid, block, 0, s, a, b);
         else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
@@ -305,7 +301,7 @@ void launch_planes(PlanesArgs g, hipStream_t s) {
     g.tiles_n = (g.p.N + BN - 1) / BN;
     g.stages = as_codes(SA, SB) ? static_cast<int>(g.p.A.pitch / kPackGroup) : g.kb / SK;
     g.slice_stages = (g.stages + g.p.slices - 1) / g.p.slices;
-    launch((linear_planes<SA, SB, BM, BN, 2, 2, SK, NST>), dim3(g.tiles_m * g.tiles_n * g.p.slices), dim3(256), 0, s, g);
+    launch((linear_planes<SA, SB, BM, BN, 2, 2, SK, NST>), dim3(g.tiles_m * g.tiles_n * g.p.slices + g.sums.blocks), dim3(kBlock), 0, s, g);
 }
 
 // The tile, and the slices of K, that cost least: rounds over the chip x a tile's
@@ -363,8 +359,9 @@ int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *work
     char *pa = reinterpret_cast<char *>(workspace);
     char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
     const PlanesPlan plan = choose_plan(p.M, p.N, p.K, p.a, p.b);
-    PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0, 0};
+    PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0, 0, {}};
     g.p.slices = plan.slices;
+    if (extra.sums) g.sums = part_sums(extra.sum_parts, across_chunks(p.N, p.K), p.N, extra.sums);
     if (plan.slices > 1)
         g.p.part = as_codes(p.a, p.b) ? workspace : reinterpret_cast<float *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
     with_sources(p.a, p.b, [&](auto a, auto b) {

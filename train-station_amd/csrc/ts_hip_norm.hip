@@ -286,6 +286,11 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
     }
 }
 
+__global__ __launch_bounds__(kBlock) void sum_parts(PartSums p) {
+    __shared__ double lds[kPartSumsLds];
+    part_sums_block(p, blockIdx.x, lds);
+}
+
 // Rows of plain values to 8 bits: a thread packs a quad, a grid stride over all quads.
 __global__ __launch_bounds__(kBlock) void pack_rows(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
                                                     uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
@@ -432,7 +437,7 @@ int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *g
     });
     if (dweight && !ticket)
         launch(sum_parts, dim3(static_cast<unsigned>((cols + 15) / 16)), dim3(kBlock), 0, s,
-               static_cast<const float *>(workspace), static_cast<size_t>(grid), cols, dweight);
+               part_sums(workspace, grid, cols, dweight));
     return launch_status();
 }
 

@@ -6,23 +6,34 @@
 
 namespace tship {
 
-// out[c] = the parts' sum over g, f64: 16 columns a workgroup, 16 groups of parts
-static __global__ __launch_bounds__(kBlock) void sum_parts(const float *__restrict__ part, size_t parts, size_t cols,
-                                                    float *__restrict__ out) {
-    __shared__ double lds[16][17];
+// out[c] = the sum over g of part[g][c], in f64; blocks workgroups of kBlock
+// threads, 16 columns each, 16 groups of parts side by side.
+struct PartSums {
+    const float *part;
+    size_t parts, cols;
+    float *out;
+    int blocks;
+};
+inline PartSums part_sums(const float *part, size_t parts, size_t cols, float *out) {
+    return {part, parts, cols, out, static_cast<int>((cols + 15) / 16)};
+}
+
+constexpr int kPartSumsLds = 16 * 17;  // doubles
+
+__device__ __forceinline__ void part_sums_block(const PartSums &p, int block, double *lds) {
     const int j = threadIdx.x & 15, q = threadIdx.x >> 4;
-    const size_t c = static_cast<size_t>(blockIdx.x) * 16 + j;
+    const size_t c = static_cast<size_t>(block) * 16 + j;
     double s = 0.0;
-    if (c < cols) {
+    if (c < p.cols) {
 #pragma unroll 8
-        for (size_t g = q; g < parts; g += 16) s += part[g * cols + c];
+        for (size_t g = q; g < p.parts; g += 16) s += p.part[g * p.cols + c];
     }
-    lds[q][j] = s;
+    lds[q * 17 + j] = s;
     __syncthreads();
-    if (q == 0 && c < cols) {
+    if (q == 0 && c < p.cols) {
 #pragma unroll
-        for (int k = 1; k < 16; ++k) s += lds[k][j];
-        out[c] = static_cast<float>(s);
+        for (int k = 1; k < 16; ++k) s += lds[k * 17 + j];
+        p.out[c] = static_cast<float>(s);
     }
 }
 
