@@ -565,3 +565,18 @@ def test_equal_calls_give_equal_bits():
     for first, second in (outs[:2], outs[2:]):
         for a, b in zip(first, second):
             assert np.array_equal(a, b)
+
+
+def test_example_trains_and_serves():
+    """The example block: its loss falls, and in 8 bits it is within what its three roundings of 2^-4 a value,
+    averaged over the sums, come to."""
+    import importlib.util
+
+    from conftest import ROOT
+
+    spec = importlib.util.spec_from_file_location("feedforward_block", ROOT / "examples" / "feedforward_block.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, off = example.main(width=96, hidden=160, batch=40, steps=12)
+    assert losses[-1] < 0.8 * losses[0] and np.all(np.isfinite(losses))
+    assert 0 < off < 2.0 ** -4
