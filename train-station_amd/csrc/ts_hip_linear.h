@@ -193,17 +193,25 @@ struct LinearProduct {
 
 // ---- the large products (ts_hip_linear_planes.hip) ---------------------------------
 
-// What the pass over an operand does beside its planes.
-struct PlanesExtra {
-    // A along k: its values in 8 bits as well
-    uint8_t *codes = nullptr, *scales = nullptr;
-    // B along its rows: its rows' sums over k into `sums`, by planes_sum_floats(N, K) of `sum_parts`
-    float *sums = nullptr, *sum_parts = nullptr;
-};
-
 bool planes_take(size_t M, size_t N, size_t K);
+// a product's planes (none where both operands are codes along k) and slices
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b);
 size_t planes_sum_floats(size_t N, size_t K);
-int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s);
+
+// One operand's way into planes, at planes_of_a / _b of its product's workspace,
+// and what the pass over it does beside.
+struct PlaneTask {
+    const LinearProduct *p;
+    bool b;  // B, else A
+    char *out;
+    uint8_t *codes, *scales;  // A of floats along k: its values in 8 bits as well
+    float *sum_parts;         // B of floats along its rows: parts of their sums over k
+};
+constexpr int kMaxPlaneTasks = 4;
+char *planes_of_a(const LinearProduct &p, float *workspace);
+char *planes_of_b(const LinearProduct &p, float *workspace);
+void planes_write(const PlaneTask *tasks, int count, hipStream_t s);
+// the product from its planes; sums: B's rows' sums from their parts
+void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_parts, float *sums, hipStream_t s);
 
 }  // namespace tship

@@ -121,18 +121,15 @@ size_t direct_floats(size_t M, size_t N, size_t K) {
     return slices > 1 ? round64(slices * M * N) : 0;
 }
 
-// p with its plan; its parts from `part` on (moved past them).  The launch's waves
-// a workgroup are set by direct_blocks.
-DirectProduct planned(const LinearProduct &p, float *&part) {
+// p with its plan, its parts at `part`.  Its workgroups follow from the launch's
+// waves (direct_blocks).
+DirectProduct planned(const LinearProduct &p, float *part) {
     DirectProduct d = direct_product(p);
     const DirectPlan plan = direct_plan(p.M, p.N, p.K);
     d.kg = plan.kg;
     d.slices = plan.slices;
     d.slice_steps = plan.slice_steps;
-    if (d.slices > 1) {
-        d.part = part;
-        part += direct_floats(p.M, p.N, p.K);
-    }
+    d.part = part;
     return d;
 }
 void direct_blocks(DirectProduct &d, int waves) {
@@ -225,30 +222,40 @@ LinearProduct dw_product(const ts_hip_linear_shape &s, const float *x, const uin
     return p;
 }
 
-// The backward pass's workspace, in floats: dz, the parts of its column sums, and
-// the planes or slices of one product after another (dx's and dweight's slices
-// side by side).
+// The backward pass's workspace, in floats: dz, the parts of its column sums, then
+// each product's planes or slices: the layer's computed again, dx's, dweight's.
 struct BackLayout {
-    size_t sums, work, total;
+    size_t sums, again, dx, dw, total;
 };
 BackLayout back_layout(const ts_hip_linear_shape &s) {
     BackLayout l{};
     l.sums = round64(s.batch * s.fan_out);
-    const bool dw_planes = planes_take(s.fan_in, s.fan_out, s.batch);
-    l.work = l.sums + (dw_planes ? round64(planes_sum_floats(s.fan_out, s.batch)) : sum_floats(s.batch, s.fan_out));
-    size_t most = 0, beside = 0;
-    auto product = [&](size_t M, size_t N, size_t K, Src a, Src b, bool pair) {
-        size_t n;
-        if (planes_take(M, N, K)) n = planes_workspace_floats(M, N, K, a, b);
-        else if (n = direct_floats(M, N, K); pair) n = beside += n;
-        most = n > most ? n : most;
+    l.again = l.sums + (planes_take(s.fan_in, s.fan_out, s.batch) ? round64(planes_sum_floats(s.fan_out, s.batch))
+                                                                  : sum_floats(s.batch, s.fan_out));
+    auto product = [](size_t M, size_t N, size_t K, Src a, Src b) {
+        return planes_take(M, N, K) ? round64(planes_workspace_floats(M, N, K, a, b)) : direct_floats(M, N, K);
     };
-    product(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR, false);
-    product(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK, true);
-    product(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR, true);
-    l.total = l.work + most;
+    l.dx = l.again + product(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR);
+    l.dw = l.dx + product(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK);
+    l.total = l.dw + product(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR);
     return l;
 }
+
+// Operands of products in planes, written by one launch.
+struct PlaneWrites {
+    PlaneTask tasks[kMaxPlaneTasks];
+    int count = 0;
+    void a(const LinearProduct &p, float *workspace, uint8_t *codes = nullptr, uint8_t *scales = nullptr) {
+        tasks[count++] = {&p, false, planes_of_a(p, workspace), codes, scales, nullptr};
+    }
+    void b(const LinearProduct &p, float *workspace, float *sum_parts = nullptr) {
+        tasks[count++] = {&p, true, planes_of_b(p, workspace), nullptr, nullptr, sum_parts};
+    }
+    void run(hipStream_t s) {
+        if (count) planes_write(tasks, count, s);
+        count = 0;
+    }
+};
 
 bool shape_ok(const ts_hip_linear_shape *s) {
     const size_t lim = size_t(1) << 24;  // row and column numbers stay far inside 32 bits
@@ -290,10 +297,12 @@ int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float 
     const LinearProduct p = forward_product(d, x, nullptr, nullptr, weight, y, {bias, residual, nullptr, slope, act});
     if (!workspace && ts_hip_linear_workspace_floats(shape)) return TS_HIP_EINVAL;
     if (planes_take(d.batch, d.fan_out, d.fan_in)) {
-        PlanesExtra extra;
-        extra.codes = codes;
-        extra.scales = scales;
-        return planes_product(p, extra, workspace, s);
+        PlaneWrites writes;
+        writes.a(p, workspace, codes, scales);
+        writes.b(p, workspace);
+        writes.run(s);
+        planes_multiply(p, workspace, nullptr, nullptr, s);
+        return launch_status();
     }
     run_direct<Src::kFloatK>(p, pack_work(x, codes, scales, d.batch, d.fan_in), workspace, s);
     return launch_status();
@@ -324,50 +333,45 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
     if (!dx && !dweight && !dbias) return TS_HIP_OK;
     if (!go || !workspace) return TS_HIP_EINVAL;
     const BackLayout at = back_layout(d);
-    float *const work = workspace + at.work;
+    float *const sums = workspace + at.sums, *const w_again = workspace + at.again, *const w_dx = workspace + at.dx,
+                *const w_dw = workspace + at.dw;
     // dz: go times the forward's slopes as the products read them, or go times the
     // slopes of the layer computed again from its checkpoint, stored
-    const float *dz = go;
-    if (act == TS_HIP_ACT_NONE) {
-        slope = nullptr;
-    } else if (!slope) {
-        if (!codes || !weight) return TS_HIP_EINVAL;
-        const LinearProduct p =
-            forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
-        if (planes_take(d.batch, d.fan_out, d.fan_in)) {
-            st = planes_product(p, {}, work, s);
-            if (st) return st;
+    const bool again = act != TS_HIP_ACT_NONE && !slope;
+    if (act == TS_HIP_ACT_NONE) slope = nullptr;
+    if ((again && (!codes || !weight)) || (dx && !weight) || (dweight && !codes && !x)) return TS_HIP_EINVAL;
+    const float *dz = again ? workspace : go;
+    const LinearProduct pz = forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
+    const LinearProduct px = dx_product(d, dz, slope, weight, dx), pw = dw_product(d, x, codes, scales, dz, slope, dweight);
+    const bool planes_x = dx && planes_take(px.M, px.N, px.K), planes_w = dweight && planes_take(pw.M, pw.N, pw.K);
+    // what does not wait for dz goes into planes first, with the layer's own operands
+    PlaneWrites writes;
+    if (planes_x) writes.b(px, w_dx);
+    if (planes_w) writes.a(pw, w_dw);
+    if (again) {
+        const bool planes_z = planes_take(pz.M, pz.N, pz.K);
+        if (planes_z) {
+            writes.a(pz, w_again);
+            writes.b(pz, w_again);
+            writes.run(s);
+            planes_multiply(pz, w_again, nullptr, nullptr, s);
         } else {
-            run_direct<Src::kCodesK>(p, PackJob{}, work, s);
+            run_direct<Src::kCodesK>(pz, PackJob{}, w_again, s);
         }
-        dz = workspace;
     }
-    if ((dx && !weight) || (dweight && !codes && !x)) return TS_HIP_EINVAL;
-    // products in planes first (each from the start of `work`), then the others as one launch
+    if (planes_x) writes.a(px, w_dx);
+    if (planes_w) writes.b(pw, w_dw, dbias ? sums : nullptr);  // dz is passed over for its planes anyway
+    writes.run(s);
+    if (planes_x) planes_multiply(px, w_dx, nullptr, nullptr, s);
+    if (planes_w) planes_multiply(pw, w_dw, sums, dbias, s);
+    if (planes_w) dbias = nullptr;
+    // the others as one launch
+    const bool later_x = dx && !planes_x, later_w = dweight && !planes_w;
+    if (!later_x && !later_w && !dbias) return launch_status();
     DirectProduct gx{}, gw{};
-    LinearProduct px{}, pw{};
-    bool later_x = false, later_w = false;
-    if (dx) {
-        px = dx_product(d, dz, slope, weight, dx);
-        later_x = !planes_take(px.M, px.N, px.K);
-        if (!later_x) st = planes_product(px, {}, work, s);
-    }
-    if (dweight && !st) {
-        pw = dw_product(d, x, codes, scales, dz, slope, dweight);
-        later_w = !planes_take(pw.M, pw.N, pw.K);
-        if (!later_w) {
-            PlanesExtra extra;
-            extra.sums = dbias;  // dz is passed over for its planes anyway
-            extra.sum_parts = workspace + at.sums;
-            st = planes_product(pw, extra, work, s);
-            dbias = nullptr;
-        }
-    }
-    if (st || (!later_x && !later_w && !dbias)) return st ? st : launch_status();
-    float *part = work;
-    if (later_x) gx = planned(px, part);
-    if (later_w) gw = planned(pw, part);
-    const SumJob sum = dbias ? sum_work(dz, slope, dbias, d.batch, d.fan_out, workspace + at.sums) : SumJob{};
+    if (later_x) gx = planned(px, w_dx);
+    if (later_w) gw = planned(pw, w_dw);
+    const SumJob sum = dbias ? sum_work(dz, slope, dbias, d.batch, d.fan_out, sums) : SumJob{};
     int waves = sum.blocks ? 4 : 1;  // (the sums: 16 rows side by side at least)
     if (later_x) waves = gx.kg > waves ? gx.kg : waves;
     if (later_w) waves = gw.kg > waves ? gw.kg : waves;

@@ -206,7 +206,8 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
         q.K = static_cast<int>(fan_in);
         q.C = y;
         q.epi = {bias, residual, nullptr, nullptr, act};
-        return planes_product(q, {}, workspace, as_stream(stream));
+        planes_multiply(q, workspace, nullptr, nullptr, as_stream(stream));
+        return launch_status();
     }
     const PackedProduct p = {x_codes, x_scales, w_codes, w_scales, bias, residual, y, static_cast<int>(batch),
                              static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0};

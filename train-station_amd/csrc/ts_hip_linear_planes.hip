@@ -27,6 +27,8 @@ __device__ __forceinline__ void store_pieces(char *to, const float (&v)[8], floa
 // One operand's part of a pass: its waves' jobs, in `blocks` workgroups.
 struct PlaneJob {
     Operand o;
+    Src src;
+    int negate;           // odd k blocks (A beside pieces)
     int K, kb;            // the product's k, in k blocks
     char *out;
     int chunks;           // floats along k: jobs of a row block
@@ -37,12 +39,11 @@ struct PlaneJob {
 };
 
 // ---- floats along k ----------------------------------------------------------------
-// A wave takes a row block and eight k blocks (512 bytes of each row).  NEG: odd k
-// blocks negated.  PACK: the values in 8 bits too; a block of 32 k is two k blocks
-// of the lane and its partner in the other half.
+// A wave takes a row block and eight k blocks (512 bytes of each row).  The values
+// in 8 bits: a block of 32 k is two k blocks of the lane and its partner in the
+// other half.
 constexpr int kAlongBlocks = 8;
 
-template <bool NEG, bool PACK, bool TIMES>
 __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, rows = j.o.rows, K = j.K, kb = j.kb;
     const int rb = static_cast<int>(job / j.chunks), b0 = static_cast<int>(job % j.chunks) * kAlongBlocks;
@@ -50,7 +51,7 @@ __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
     const size_t at = static_cast<size_t>(live ? row : 0) * j.o.ld;
-    const float *p = j.o.p + at, *tp = TIMES ? j.o.times + at : nullptr;
+    const float *p = j.o.p + at, *tp = j.o.times ? j.o.times + at : nullptr;
     float v[kAlongBlocks][8];
 #pragma unroll
     for (int b = 0; b < kAlongBlocks; ++b)
@@ -60,12 +61,12 @@ __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
             float w[4] = {};
             if (live && k + 4 <= K) {
                 pk4u_t t = *reinterpret_cast<const pk4u_t *>(p + k);
-                if (TIMES) t *= *reinterpret_cast<const pk4u_t *>(tp + k);
+                if (tp) t *= *reinterpret_cast<const pk4u_t *>(tp + k);  // uniform
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = t[e];
             } else if (live) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? (TIMES ? p[k + e] * tp[k + e] : p[k + e]) : 0.0f;
+                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? (tp ? p[k + e] * tp[k + e] : p[k + e]) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[b][4 * q + e] = w[e];
@@ -74,9 +75,9 @@ __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
     for (int b = 0; b < kAlongBlocks; ++b) {
         if (b0 + b >= kb) break;  // uniform
         store_pieces(j.out + (static_cast<size_t>(rb) * kb + b0 + b) * 3 * kFragBytes, v[b],
-                     NEG && (b & 1) ? -kSplitScale : kSplitScale, lane);
+                     j.negate && (b & 1) ? -kSplitScale : kSplitScale, lane);
     }
-    if (PACK) {
+    if (j.codes) {  // uniform
         const size_t pitch = packed_pitch(K);
 #pragma unroll
         for (int b = 0; b < kAlongBlocks; b += 2) {
@@ -106,9 +107,8 @@ __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
 }
 
 // ---- floats along the rows -----------------------------------------------------------
-// element (row, k) at x[k * ld + row].  A wave takes a row block and `run` k
-// blocks.  SUM: the rows' sums over them (f64) to part[chunk][rows].
-template <bool NEG, bool SUM, bool TIMES>
+// element (row, k) at p[k * ld + row].  A wave takes a row block and `run` k blocks;
+// with sum_parts the rows' sums over them (f64) too.
 __device__ __forceinline__ void planes_across(const PlaneJob &j, size_t job) {
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, ld = j.o.ld, rows = j.o.rows, K = j.K, kb = j.kb;
     const int rb = static_cast<int>(job % j.row_blocks), chunk = static_cast<int>(job / j.row_blocks);
@@ -116,7 +116,7 @@ __device__ __forceinline__ void planes_across(const PlaneJob &j, size_t job) {
     if (from >= kb) return;
     const int row = rb * kPlaneRows + i;
     const bool live = row < rows;
-    const float *p = j.o.p + (live ? row : 0), *tp = TIMES ? j.o.times + (live ? row : 0) : nullptr;
+    const float *p = j.o.p + (live ? row : 0), *tp = j.o.times ? j.o.times + (live ? row : 0) : nullptr;
     double sum = 0.0;
 #pragma unroll 2
     for (int b = from; b < to; ++b) {
@@ -125,7 +125,7 @@ __device__ __forceinline__ void planes_across(const PlaneJob &j, size_t job) {
         if ((b + 1) * kPlaneK <= K) {  // uniform
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = p[static_cast<size_t>(k + e) * ld];
-            if (TIMES) {
+            if (tp) {  // uniform
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= tp[static_cast<size_t>(k + e) * ld];
             }
@@ -133,21 +133,21 @@ __device__ __forceinline__ void planes_across(const PlaneJob &j, size_t job) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const size_t at = static_cast<size_t>(k + e) * ld;
-                v[e] = k + e < K ? (TIMES ? p[at] * tp[at] : p[at]) : 0.0f;
+                v[e] = k + e < K ? (tp ? p[at] * tp[at] : p[at]) : 0.0f;
             }
         }
         if (!live) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = 0.0f;
         }
-        if (SUM) {
+        if (j.sum_parts) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum += v[e];
         }
-        store_pieces(j.out + (static_cast<size_t>(rb) * kb + b) * 3 * kFragBytes, v, NEG && (b & 1) ? -kSplitScale : kSplitScale,
+        store_pieces(j.out + (static_cast<size_t>(rb) * kb + b) * 3 * kFragBytes, v, j.negate && (b & 1) ? -kSplitScale : kSplitScale,
                      lane);
     }
-    if (SUM) {
+    if (j.sum_parts) {
         sum += __shfl_xor(sum, 32, 64);
         if (h == 0 && live) j.sum_parts[static_cast<size_t>(chunk) * rows + row] = static_cast<float>(sum);
     }
@@ -218,21 +218,28 @@ __device__ __forceinline__ void planes_codes_across(const PlaneJob &j, size_t jo
     }
 }
 
-// Both operands of a product, A's jobs first.  PACK and SUM: of A along k, of B
-// along its rows; TIMES: of the operand that is a layer's dz.
-template <Src SA, Src SB, bool PACK, bool SUM, bool TIMES>
-__global__ __launch_bounds__(kBlock) void write_planes(PlaneJob a, PlaneJob b) {
-    const bool first = blockIdx.x < a.blocks;  // uniform
-    const size_t job = static_cast<size_t>(first ? blockIdx.x : blockIdx.x - a.blocks) * (kBlock / 64) + (threadIdx.x >> 6);
-    if (first) {
-        if constexpr (SA == Src::kFloatK) planes_along<true, PACK, TIMES>(a, job);
-        else if constexpr (SA == Src::kFloatR) planes_across<true, false, false>(a, job);
-        else if constexpr (SA == Src::kCodesK) planes_codes_along(a, job);
-        else planes_codes_across(a, job);
-    } else if constexpr (SB == Src::kFloatK) {
-        planes_along<false, false, false>(b, job);
-    } else {
-        planes_across<false, SUM, TIMES && SA != Src::kFloatK>(b, job);
+// Several operands' planes by one launch.
+struct PlaneJobs {
+    PlaneJob job[kMaxPlaneTasks];
+    int count;
+};
+
+__global__ __launch_bounds__(kBlock) void write_planes(PlaneJobs jobs) {
+    unsigned block = blockIdx.x;
+#pragma unroll
+    for (int n = 0; n < kMaxPlaneTasks; ++n) {
+        const PlaneJob &j = jobs.job[n];
+        if (n >= jobs.count) return;  // (uniform, as the rest)
+        if (block >= j.blocks) {
+            block -= j.blocks;
+            continue;
+        }
+        const size_t job = static_cast<size_t>(block) * (kBlock / 64) + (threadIdx.x >> 6);
+        if (j.src == Src::kFloatK) planes_along(j, job);
+        else if (j.src == Src::kFloatR) planes_across(j, job);
+        else if (j.src == Src::kCodesK) planes_codes_along(j, job);
+        else planes_codes_across(j, job);
+        return;
     }
 }
 
@@ -257,42 +264,23 @@ int across_chunks(size_t rows, size_t K) {
     return (k_blocks(K) + run - 1) / run;
 }
 
-PlaneJob plane_job(const Operand &o, Src src, int K, char *out, const PlanesExtra &x) {
-    PlaneJob j = {o, K, k_blocks(K), out, 0, 0, row_blocks(o.rows), 0, x.codes, x.scales, x.sum_parts};
+PlaneJob plane_job(const PlaneTask &t) {
+    const LinearProduct &p = *t.p;
+    const Operand &o = t.b ? p.B : p.A;
+    const Src src = t.b ? p.b : p.a;
+    PlaneJob j = {o, src, !t.b, p.K, k_blocks(p.K), t.out, 0, 0, row_blocks(o.rows), 0, t.codes, t.scales, t.sum_parts};
     const size_t rb = j.row_blocks;
     if (src == Src::kFloatK) {
-        const size_t blocks = x.codes ? packed_pitch(K) / kPlaneK : j.kb;
+        const size_t blocks = t.codes ? packed_pitch(p.K) / kPlaneK : j.kb;
         j.chunks = static_cast<int>((blocks + kAlongBlocks - 1) / kAlongBlocks);
         j.blocks = wave_grid(rb * j.chunks);
     } else if (src == Src::kFloatR) {
-        j.run = across_run(o.rows, K);
-        j.blocks = wave_grid(rb * across_chunks(o.rows, K));
+        j.run = across_run(o.rows, p.K);
+        j.blocks = wave_grid(rb * across_chunks(o.rows, p.K));
     } else {
         j.blocks = wave_grid(rb * (src == Src::kCodesK ? o.pitch / kPackGroup : (j.kb + 3) / 4));
     }
     return j;
-}
-
-// The planes of both operands by one launch, with what goes beside them.
-template <Src SA, Src SB>
-void launch_write(const LinearProduct &p, const PlanesExtra &x, char *pa, char *pb, hipStream_t s) {
-    const PlaneJob a = plane_job(p.A, SA, p.K, pa, x), b = plane_job(p.B, SB, p.K, pb, SB == Src::kFloatR ? x : PlanesExtra{});
-    const dim3 grid(a.blocks + b.blocks), block(kBlock);
-    if constexpr (SA == Src::kFloatK && SB == Src::kFloatR) {
-        if (x.codes) launch((write_planes<SA, SB, true, false, false>), grid, block, 0, s, a, b);
-        else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
-    } else if constexpr (SA == Src::kFloatK) {
-        if (p.A.times) launch((write_planes<SA, SB, false, false, true>), grid, block, 0, s, a, b);
-        else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
-    } else if constexpr (SA == Src::kCodesK) {
-        launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
-    } else if (x.sums) {
-        if (p.B.times) launch((write_planes<SA, SB, false, true, true>), grid, block, 0, s, a, b);
-        else launch((write_planes<SA, SB, false, true, false>), grid, block, 0, s, a, b);
-    } else {
-        if (p.B.times) launch((write_planes<SA, SB, false, false, true>), grid, block, 0, s, a, b);
-        else launch((write_planes<SA, SB, false, false, false>), grid, block, 0, s, a, b);
-    }
 }
 
 template <Src SA, Src SB, int BM, int BN, int SK, int NST>
@@ -350,24 +338,38 @@ bool planes_take(size_t M, size_t N, size_t K) { return 2.0 * M * N * K >= 1.5e9
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b) {
     const PlanesPlan plan = choose_plan(M, N, K, a, b);
     const size_t planes = as_codes(a, b) ? 0 : (round_256(plane_bytes(M, K, a)) + round_256(plane_bytes(N, K, b))) / sizeof(float);
-    return planes + (plan.slices > 1 ? plan.slices * M * N : 0);
+    return planes + (plan.slices > 1 ? round_256(plan.slices * M * N * sizeof(float)) / sizeof(float) : 0);
 }
 
 size_t planes_sum_floats(size_t N, size_t K) { return static_cast<size_t>(across_chunks(N, K)) * N; }
 
-int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *workspace, hipStream_t s) {
-    char *pa = reinterpret_cast<char *>(workspace);
-    char *pb = pa + round_256(plane_bytes(p.M, p.K, p.a));
+char *planes_of_a(const LinearProduct &, float *workspace) { return reinterpret_cast<char *>(workspace); }
+char *planes_of_b(const LinearProduct &p, float *workspace) {
+    return reinterpret_cast<char *>(workspace) + round_256(plane_bytes(p.M, p.K, p.a));
+}
+
+void planes_write(const PlaneTask *tasks, int count, hipStream_t s) {
+    PlaneJobs jobs = {};
+    jobs.count = count;
+    unsigned blocks = 0;
+    for (int n = 0; n < count; ++n) {
+        jobs.job[n] = plane_job(tasks[n]);
+        blocks += jobs.job[n].blocks;
+    }
+    if (blocks) launch(write_planes, dim3(blocks), dim3(kBlock), 0, s, jobs);
+}
+
+void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_parts, float *sums, hipStream_t s) {
+    char *pa = planes_of_a(p, workspace), *pb = planes_of_b(p, workspace);
     const PlanesPlan plan = choose_plan(p.M, p.N, p.K, p.a, p.b);
     PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0, 0, {}};
     g.p.slices = plan.slices;
-    if (extra.sums) g.sums = part_sums(extra.sum_parts, across_chunks(p.N, p.K), p.N, extra.sums);
+    if (sums) g.sums = part_sums(sum_parts, across_chunks(p.N, p.K), p.N, sums);
     if (plan.slices > 1)
         g.p.part = as_codes(p.a, p.b) ? workspace : reinterpret_cast<float *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
     with_sources(p.a, p.b, [&](auto a, auto b) {
         constexpr Src A = a.value, B = b.value;
         constexpr bool codes = as_codes(A, B), three = pieces_of(A) == 3;
-        if constexpr (!codes) launch_write<A, B>(p, extra, pa, pb, s);
         // stages: of 128 codes; else of 16 k, three or four of them (two of 32 for one piece beside three:
         // 8192 x 4096 x 4096 598 us, against 700 in four of 16)
         if (plan.bm == 64) launch_planes<A, B, 64, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
@@ -375,7 +377,6 @@ int planes_product(const LinearProduct &p, const PlanesExtra &extra, float *work
         else launch_planes<A, B, 128, 128, codes ? 8 : three ? 1 : 2, codes || !three ? 2 : 3>(g, s);
     });
     join_slices(g.p, s);
-    return launch_status();
 }
 
 }  // namespace tship
