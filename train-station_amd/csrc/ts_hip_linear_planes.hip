@@ -39,10 +39,10 @@ struct PlaneJob {
 };
 
 // ---- floats along k ----------------------------------------------------------------
-// A wave takes a row block and eight k blocks (512 bytes of each row).  The values
+// A wave takes a row block and four k blocks (256 bytes of each row).  The values
 // in 8 bits: a block of 32 k is two k blocks of the lane and its partner in the
 // other half.
-constexpr int kAlongBlocks = 8;
+constexpr int kAlongBlocks = 4;
 
 __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
     const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5, rows = j.o.rows, K = j.K, kb = j.kb;
