@@ -283,25 +283,26 @@ PlaneJob plane_job(const PlaneTask &t) {
     return j;
 }
 
-template <Src SA, Src SB, int BM, int BN, int SK, int NST>
+template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST>
 void launch_planes(PlanesArgs g, hipStream_t s) {
     g.tiles_m = (g.p.M + BM - 1) / BM;
     g.tiles_n = (g.p.N + BN - 1) / BN;
     g.stages = as_codes(SA, SB) ? static_cast<int>(g.p.A.pitch / kPackGroup) : g.kb / SK;
     g.slice_stages = (g.stages + g.p.slices - 1) / g.p.slices;
-    launch((linear_planes<SA, SB, BM, BN, 2, 2, SK, NST>), dim3(g.tiles_m * g.tiles_n * g.p.slices + g.sums.blocks), dim3(kBlock), 0, s, g);
+    launch((linear_planes<SA, SB, BM, BN, WM, WN, SK, NST>), dim3(g.tiles_m * g.tiles_n * g.p.slices + g.sums.blocks),
+           dim3(64 * WM * WN), 0, s, g);
 }
 
 // The tile, and the slices of K, that cost least: rounds over the chip x a tile's
-// share of K x its area, the smallest tile 1.1 times as dear, and a larger one 1.3
-// times where a CU has but one workgroup to fill its waits; slices cost a launch
-// and their sums' way to memory and back.  us in 128 x 128, 128 x 64, 64 x 64,
-// pieces on both sides: 8192 x 4096 x 4096 1284, 1295, 1381; 2048 x 4096 x 1024 93,
-// 96, 99; 1024 x 4096 x 2048 105, 90, 104; 2048 x 1024 x 4096 177, 122, 98; 1999 x
-// 777 x 1531 78, 53, 39.  One side's: 598, 662, 764; 52, 56, 59; 55, 54, 57; 87, 70,
-// 57; 46, 36, 28.  Codes: 260, 280, 324; 28.6, 30.4, 31.8; 32, 29, 31; 46, 35, 35;
-// 26, 22, 19.  (128 x 256 by eight waves: within 3 % of 128 x 128 at the largest,
-// and slower below; 256 x 256: slower.)
+// share of K x its area, the smaller tiles 1.03 and 1.1 times as dear, and a larger
+// one 1.15 or 1.3 times where a CU has but one workgroup to fill its waits; slices
+// cost a launch and their sums' way to memory and back.  us in 128 x 128, 128 x 64,
+// 64 x 64, pieces on both sides: 8192 x 4096 x 4096 1242, 1295, 1419; 2048 x 4096 x
+// 1024 89.6, 95, 98; 1024 x 4096 x 2048 98, 88, 106; 2048 x 1024 x 4096 163, -, 95;
+// 1024 x 1024 x 1024 45, -, 23.  One side's: 604, 631, 764; 48.5, 53, 59; 51, 50, 59;
+// 1003 x 2050 x 3000 66, 58, 53.  Codes: 256, 288, 324; 27.6, 31, 32; 31, 29, 31;
+// 2048 x 1024 x 4096 46, 35, 35; 1999 x 777 x 1531 26, 22, 19.  (128 x 256 and
+// 256 x 256 by eight waves: no faster at the largest, and slower below.)
 struct PlanesPlan {
     int bm, bn, slices;
 };
@@ -310,12 +311,11 @@ PlanesPlan choose_plan(size_t M, size_t N, size_t K, Src a, Src b) {
     const double each = as_codes(a, b) ? 0.8e-6 : of_codes(a) ? 1.4e-6 : 2.6e-6;  // us per k of a column of a tile, one a CU
     PlanesPlan best = {128, 128, 1};
     double least = 1e30;
-    auto take = [&](size_t bm, size_t bn, double dear) {
+    auto take = [&](size_t bm, size_t bn, double dear, double alone) {
         const size_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
         for (size_t n = 1; n <= 8 && (n == 1 || (K >= n * 512 && tiles * n <= 4 * cus)); n *= 2) {
             const size_t rounds = (tiles * n + cus - 1) / cus;
-            double us = rounds * bm * bn * dear * each * K / n;
-            if (rounds == 1 && bm > 64) us *= 1.3;
+            double us = rounds * bm * bn * (rounds == 1 ? alone : dear) * each * K / n;
             if (n > 1) us += 6 + 2e-6 * M * N * n;
             if (us < least) {
                 least = us;
@@ -323,9 +323,9 @@ PlanesPlan choose_plan(size_t M, size_t N, size_t K, Src a, Src b) {
             }
         }
     };
-    take(128, 128, 1.0);
-    take(128, 64, 1.0);
-    take(64, 64, 1.1);
+    take(128, 128, 1.0, 1.15);
+    take(128, 64, 1.03, 1.3);
+    take(64, 64, 1.1, 1.1);
     return best;
 }
 
@@ -369,12 +369,23 @@ void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_
         g.p.part = as_codes(p.a, p.b) ? workspace : reinterpret_cast<float *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
     with_sources(p.a, p.b, [&](auto a, auto b) {
         constexpr Src A = a.value, B = b.value;
-        constexpr bool codes = as_codes(A, B), three = pieces_of(A) == 3;
-        // stages: of 128 codes; else of 16 k, three or four of them (two of 32 for one piece beside three:
-        // 8192 x 4096 x 4096 598 us, against 700 in four of 16)
-        if (plan.bm == 64) launch_planes<A, B, 64, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
-        else if (plan.bn == 64) launch_planes<A, B, 128, 64, codes ? 8 : 1, codes ? 2 : 4>(g, s);
-        else launch_planes<A, B, 128, 128, codes ? 8 : three ? 1 : 2, codes || !three ? 2 : 3>(g, s);
+        // waves and stages: 128 codes a stage; else 32 k, two stages, but 16 k and three where
+        // 128 x 128 has three pieces on both sides (8192 x 4096 x 4096 1242 us by eight waves,
+        // 1302 by four), and four where the smallest tile has them on one (1024 x 4096 x 2048
+        // 59 us, 61 in three of 32)
+        if constexpr (as_codes(A, B)) {
+            if (plan.bm == 64) launch_planes<A, B, 64, 64, 2, 2, 8, 2>(g, s);
+            else if (plan.bn == 64) launch_planes<A, B, 128, 64, 2, 2, 8, 2>(g, s);
+            else launch_planes<A, B, 128, 128, 2, 2, 8, 2>(g, s);
+        } else if constexpr (pieces_of(A) == 3) {
+            if (plan.bm == 64) launch_planes<A, B, 64, 64, 2, 2, 2, 2>(g, s);
+            else if (plan.bn == 64) launch_planes<A, B, 128, 64, 2, 2, 2, 2>(g, s);
+            else launch_planes<A, B, 128, 128, 4, 2, 1, 3>(g, s);
+        } else {
+            if (plan.bm == 64) launch_planes<A, B, 64, 64, 2, 2, 1, 4>(g, s);
+            else if (plan.bn == 64) launch_planes<A, B, 128, 64, 2, 2, 2, 2>(g, s);
+            else launch_planes<A, B, 128, 128, 2, 4, 2, 2>(g, s);
+        }
     });
     join_slices(g.p, s);
 }

@@ -6,8 +6,8 @@
 
 namespace tship {
 
-// out[c] = the sum over g of part[g][c], in f64; blocks workgroups of kBlock
-// threads, 16 columns each, 16 groups of parts side by side.
+// out[c] = the sum over g of part[g][c], in f64; blocks workgroups of at
+// least kBlock threads, 16 columns each, 16 groups of parts side by side.
 struct PartSums {
     const float *part;
     size_t parts, cols;
@@ -24,11 +24,11 @@ __device__ __forceinline__ void part_sums_block(const PartSums &p, int block, do
     const int j = threadIdx.x & 15, q = threadIdx.x >> 4;
     const size_t c = static_cast<size_t>(block) * 16 + j;
     double s = 0.0;
-    if (c < p.cols) {
+    if (c < p.cols && q < 16) {  // (threads past kBlock only reach the barrier)
 #pragma unroll 8
         for (size_t g = q; g < p.parts; g += 16) s += p.part[g * p.cols + c];
     }
-    lds[q * 17 + j] = s;
+    if (q < 16) lds[q * 17 + j] = s;
     __syncthreads();
     if (q == 0 && c < p.cols) {
 #pragma unroll
