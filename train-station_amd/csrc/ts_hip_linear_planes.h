@@ -61,8 +61,8 @@ struct PlaneSide {
     static constexpr int P = pieces_of(S), kBlocks = R / kPlaneRows;
     static_assert(!kCodes || SK * kPlaneK == kPackGroup, "codes: a group of 128 a stage");
     // DMA instructions of 1 KB: fragments, or 8 rows of 128 codes (a row's chunk c
-    // of 16 stands at c ^ row % 8, so that a fragment's reads, one chunk of 32 rows,
-    // take every bank alike)
+    // of 16 stands at c ^ row / 2 % 8: two rows fill the banks once, so the reads of
+    // one chunk of 16 rows fall on all sixteen places)
     static constexpr int kUnits = kCodes ? kBlocks * 4 : kBlocks * SK * P;
     static constexpr int kBytes = kUnits * kFragBytes;
     static constexpr int kScaleUnits = kCodes ? R / 64 : 0;  // of 64 words: a row's four scales each
@@ -82,7 +82,7 @@ struct PlaneSide {
         if constexpr (kCodes) {
             const int last = o.rows - 1 - b0 * kPlaneRows;  // rows past an edge: the last one's
             return static_cast<unsigned>(min(u * 8 + (lane >> 3), last)) * static_cast<unsigned>(o.pitch) +
-                   16u * ((lane & 7) ^ (lane >> 3));
+                   16u * ((lane & 7) ^ (4 * u + (lane >> 4) & 7));
         } else {
             return 16u * lane;
         }
@@ -90,7 +90,7 @@ struct PlaneSide {
     // a code fragment's eight bytes: k block k of row block b
     static __device__ __forceinline__ u2v_t codes8(const char *at, int b, int k, int lane) {
         const int i = lane & 31, h = lane >> 5;
-        return *reinterpret_cast<const u2v_t *>(at + b * 4096 + i * 128 + 8 * h + (16 * k ^ 16 * (i & 7)));
+        return *reinterpret_cast<const u2v_t *>(at + b * 4096 + i * 128 + 8 * h + (16 * k ^ 16 * (i >> 1 & 7)));
     }
 };
 
