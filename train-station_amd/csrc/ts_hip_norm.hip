@@ -9,6 +9,12 @@
 // NV such quads, so memory is passed over once; sums are f64.  Backward needs
 // h^2's and g h's row sums only, and takes both in the same pass: nothing but h
 // is kept from the forward.
+//
+// Bound by memory from a few thousand rows on, by the launch below (us, 8192 x 4096
+// with the sum): forward 85 for 537 MB, packed 94 for 437 MB, backward 85 for 403 MB
+// (h partly from the last-level cache); 16384 x 2048 the same; 1 x 4096 packed 5.
+// The f64 sums and the packed form's f64 products are under that: a wave has four
+// loads of 16 bytes in flight per operand, and four waves a row leave two rows a SIMD.
 #include "ts_hip_pack8.h"
 #include "ts_hip_parts.h"
 
