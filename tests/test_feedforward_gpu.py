@@ -155,6 +155,24 @@ def test_rms_norm_packed(rows, cols, residual):
     assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
 
 
+def test_norm_of_more_rows_than_a_launch_has_workgroups():
+    rows, cols = (1 << 23) + 5, 3
+    x, w = normal((rows, cols), 1), normal((cols,), 2)
+    X = tensor(x)
+    y = X.rms_norm(tensor(w)).data()
+    want = R.rms_norm(x, w, 1e-6)
+    assert_within(y, want, 4 * R.U * np.abs(want) + 1e-40, "y")
+    del X
+
+
+def test_packed_norm_of_zero_rows_pads_with_zeros():
+    x = normal((3, 40), 1)
+    x[1] = 0.0
+    codes, scales = parts(tensor(x).rms_norm_packed(tensor(np.ones(40, np.float32)), 0.0))
+    assert np.all((codes[1, :40] & 127) == 127)  # 0 / 0
+    assert not codes[:, 40:].any()
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 5), (128, 784), (700, 64), (3000, 1000)])
 def test_norm_backward_with_and_without_a_ticket(rows, cols):
     """The same sums by one launch and by two, to the last place, and the ticket zero again."""

@@ -260,7 +260,7 @@ struct PlaneWrites {
 bool shape_ok(const ts_hip_linear_shape *s) {
     const size_t lim = size_t(1) << 24;  // row and column numbers stay far inside 32 bits
     if (!s || s->batch >= lim || s->fan_in >= lim || s->fan_out >= lim) return false;
-    const size_t most = size_t(1) << 40;  // elements of a matrix: tile numbers inside 32 bits
+    const size_t most = size_t(1) << 34;  // elements of a matrix: a launch has fewer than 2^32 threads
     return s->batch * s->fan_in < most && s->batch * s->fan_out < most && s->fan_in * s->fan_out < most;
 }
 bool act_ok(int act) { return act >= TS_HIP_ACT_NONE && act <= TS_HIP_ACT_GELU_TANH; }

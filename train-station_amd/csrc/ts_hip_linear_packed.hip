@@ -192,7 +192,7 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
                          int act, const float *residual, float *y, float *workspace, size_t workspace_floats,
                          void *stream) {
     const size_t lim = size_t(1) << 24;
-    if (batch >= lim || fan_in >= lim || fan_out >= lim || batch * fan_out >= size_t(1) << 38 || act < TS_HIP_ACT_NONE || act > TS_HIP_ACT_GELU_TANH)
+    if (batch >= lim || fan_in >= lim || fan_out >= lim || batch * fan_out >= size_t(1) << 34 || act < TS_HIP_ACT_NONE || act > TS_HIP_ACT_GELU_TANH)
         return TS_HIP_EINVAL;
     if (batch == 0 || fan_out == 0) return TS_HIP_OK;
     if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;

@@ -79,77 +79,76 @@ struct NormArgs {
     double eps;
 };
 
-// One row per W waves; LONG: more columns than the waves hold, passed over twice.
+// A row per W waves; LONG: more columns than the waves hold, passed over twice.
 template <int W, int NV, bool RES, bool PACK, bool LONG>
 __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_rows(NormArgs a) {
     constexpr int RPB = kNormRows<W>;
     __shared__ double lds[RPB * W];
     const int slot = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W);
-    const size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot;
-    const bool live = row < a.rows;  // uniform per wave; the others reach the barriers
-    const size_t base = live ? row * a.cols : 0;
-    const float *x = a.x + base, *res = RES ? a.residual + base : nullptr;
     const size_t span = static_cast<size_t>(256) * W * NV, end = PACK ? a.pitch : a.cols;
-
-    float v[NV][4];
-    auto fetch = [&](size_t c0) {  // h of the columns from c0 on (past the row: zeros)
-        float r[NV][4];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) load4(x, c0 + 4 * (t + 64 * W * i), live ? a.cols : 0, v[i]);
-        if (RES) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) load4(res, c0 + 4 * (t + 64 * W * i), live ? a.cols : 0, r[i]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
-        }
-    };
-    double s[1] = {0.0};
-    size_t c0 = 0;
-    do {
-        fetch(c0);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[0] += static_cast<double>(v[i][e]) * v[i][e];
-        c0 += span;
-    } while (LONG && c0 < a.cols);
-    // the weights are on their way while the row's sum is taken
     float w[NV][4];
     auto weights = [&](size_t from) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) load4(a.weight, from + 4 * (t + 64 * W * i), a.cols, w[i]);
     };
     if (!LONG) weights(0);
-    row_sum<W, 1>(s, lds + slot * W);
-    if (!live) return;  // (no barrier follows)
-    const double r = 1.0 / sqrt(s[0] / static_cast<double>(a.cols) + a.eps);
-    const float rf = static_cast<float>(r);
-    c0 = 0;
-    do {
-        if (LONG) {
-            fetch(c0);
-            weights(c0);
-        }
+    const size_t step = static_cast<size_t>(gridDim.x) * RPB;
+    for (size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot; row < a.rows; row += step) {  // (W > 1: uniform)
+        const size_t base = row * a.cols;
+        const float *x = a.x + base, *res = RES ? a.residual + base : nullptr;
+        float v[NV][4];
+        auto fetch = [&](size_t c0) {  // h of the columns from c0 on (past the row: zeros)
+            float r[NV][4];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const size_t c = c0 + 4 * (t + 64 * W * i);
-            if (c >= end) continue;
-            if (RES) store4(a.h + base, c, a.cols, v[i]);
-            float o[4];
-            if (PACK) {  // in f64: a code takes the side of its border that y itself is on
+            for (int i = 0; i < NV; ++i) load4(x, c0 + 4 * (t + 64 * W * i), a.cols, v[i]);
+            if (RES) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = round_odd(static_cast<double>(v[i][e]) * r * w[i][e]);
-                pack_store(o, c, a.codes + row * a.pitch, a.scales + 4 * row, 4 * a.rows);
-            } else {
+                for (int i = 0; i < NV; ++i) load4(res, c0 + 4 * (t + 64 * W * i), a.cols, r[i]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = v[i][e] * rf * w[i][e];
-                store4(a.y + base, c, a.cols, o);
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
             }
-        }
-        c0 += span;
-    } while (LONG && c0 < end);
+        };
+        double s[1] = {0.0};
+        size_t c0 = 0;
+        do {
+            fetch(c0);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[0] += static_cast<double>(v[i][e]) * v[i][e];
+            c0 += span;
+        } while (LONG && c0 < a.cols);
+        row_sum<W, 1>(s, lds + slot * W);
+        const double r = 1.0 / sqrt(s[0] / static_cast<double>(a.cols) + a.eps);
+        const float rf = static_cast<float>(r);
+        c0 = 0;
+        do {
+            if (LONG) {
+                fetch(c0);
+                weights(c0);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const size_t c = c0 + 4 * (t + 64 * W * i);
+                if (c >= end) continue;
+                if (RES) store4(a.h + base, c, a.cols, v[i]);
+                float o[4];
+                if (PACK) {  // in f64: a code takes the side of its border that y itself is on
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[e] = c + e < a.cols ? round_odd(static_cast<double>(v[i][e]) * r * w[i][e]) : 0.0f;
+                    pack_store(o, c, a.codes + row * a.pitch, a.scales + 4 * row, 4 * a.rows);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = v[i][e] * rf * w[i][e];
+                    store4(a.y + base, c, a.cols, o);
+                }
+            }
+            c0 += span;
+        } while (LONG && c0 < end);
+    }
 }
 
 struct NormBackArgs {
@@ -325,9 +324,12 @@ __global__ __launch_bounds__(kBlock) void unpack_rows(const uint8_t *__restrict_
     }
 }
 
+constexpr size_t kMaxBlocks = size_t(1) << 21;  // a launch has fewer than 2^32 threads; more rows take turns
+
 template <int W, int NV, bool LONG>
 void launch_norm(const NormArgs &a, bool pack, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.rows + kNormRows<W> - 1) / kNormRows<W>)), block(kNormThreads<W>);
+    const size_t need = (a.rows + kNormRows<W> - 1) / kNormRows<W>;
+    const dim3 grid(static_cast<unsigned>(need < kMaxBlocks ? need : kMaxBlocks)), block(kNormThreads<W>);
     if (a.residual && pack) launch((rms_norm_rows<W, NV, true, true, LONG>), grid, block, 0, s, a);
     else if (a.residual) launch((rms_norm_rows<W, NV, true, false, LONG>), grid, block, 0, s, a);
     else if (pack) launch((rms_norm_rows<W, NV, false, true, LONG>), grid, block, 0, s, a);
