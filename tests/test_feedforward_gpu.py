@@ -141,6 +141,12 @@ def test_rms_norm(rows, cols, residual):
     T.clear_gradients()
 
 
+@pytest.mark.parametrize("rows,cols", [(600, 8192), (600, 8200), (300, 16383), (1100, 4100), (1500, 1030)])
+def test_rms_norm_sums_many_rows(rows, cols):
+    """Weight gradients where each workgroup adds several rows, within the bounds of one."""
+    test_rms_norm(rows, cols, True)
+
+
 @pytest.mark.parametrize("rows,cols", NORMS)
 @pytest.mark.parametrize("residual", [False, True])
 def test_rms_norm_packed(rows, cols, residual):

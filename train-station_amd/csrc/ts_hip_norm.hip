@@ -11,7 +11,7 @@
 // is kept from the forward.
 //
 // Bound by memory from a few thousand rows on, by the launch below (us, 8192 x 4096
-// with the sum): forward 85 for 537 MB, packed 94 for 437 MB, backward 85 for 403 MB
+// with the sum): forward 85 for 537 MB, packed 87 for 437 MB, backward 85 for 403 MB
 // (h partly from the last-level cache); 16384 x 2048 the same; 1 x 4096 packed 5.
 // The f64 sums and the packed form's f64 products are under that: a wave has four
 // loads of 16 bytes in flight per operand, and four waves a row leave two rows a SIMD.
@@ -168,7 +168,20 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
     __shared__ double lds[RPB * 2 * W];
     const int slot = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W);
     const size_t span = static_cast<size_t>(256) * W * NV;
-    double dw[NV][4] = {};
+    // The sums stand in registers; where 16 waves of four quads leave none, in shared
+    // memory, each thread its own (2048 x 16384 forward and backward: registers, 60 of
+    // them spilled, 227 us, shared memory 195; 300 x 12000 47, 34).
+    constexpr bool SHARED = DW && !LONG && W * NV >= 64;
+    __shared__ double held[SHARED ? NV * 4 * 64 * W : 1];
+    double own[SHARED ? 1 : NV][4] = {};
+    auto dw = [&](int i, int e) -> double & {
+        if constexpr (SHARED) return held[(i * 4 + e) * 64 * W + t];
+        else return own[i][e];
+    };
+    if constexpr (SHARED) {
+#pragma unroll
+        for (int i = 0; i < 4 * NV; ++i) dw(i / 4, i % 4) = 0.0;
+    }
     float w[NV][4];
     auto weights = [&](size_t c0) {
 #pragma unroll
@@ -226,7 +239,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
                 }
                 if (DW && !LONG && live) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dw[i][e] += static_cast<double>(g[i][e]) * (h[i][e] * rf);
+                    for (int e = 0; e < 4; ++e) dw(i, e) += static_cast<double>(g[i][e]) * (h[i][e] * rf);
                 }
                 if (DW && LONG && c < n) {  // (one row at a time: the workgroup's own line)
                     float o[4];
@@ -250,7 +263,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = dw[i][e];
+                    for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = dw(i, e);
             }
             __syncthreads();
             if (slot == 0) {
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
 #pragma unroll
                     for (int i = 0; i < NV; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) dw[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
+                        for (int e = 0; e < 4; ++e) dw(i, e) += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
             }
         }
         if (slot == 0) {
@@ -268,7 +281,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
                 const size_t c = 4 * (t + 64 * W * i);
                 float o[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw[i][e]);
+                for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw(i, e));
                 if (c < a.cols) store4(part, c, a.cols, o);
             }
         }
@@ -344,20 +357,28 @@ void launch_back(const NormBackArgs &a, unsigned grid, hipStream_t s) {
     else launch((rms_norm_back<W, NV, false, true, LONG>), dim3(grid), block, 0, s, a);
 }
 
-// Calls f(W, NV, LONG as constants) for a row of n columns: the fewest waves
-// that hold it with at most four quads a lane.
+// Calls f(W, NV, LONG as constants) for a row of n columns: the fewest waves that
+// hold it with four quads a lane, but for rows of 4097 to 8192 packed, whose f64
+// products want the registers: two quads.  us, packed with the sum, four quads and
+// two: 8192 x 4096 87, 92; 4096 x 8192 120, 107.  Forward and backward: 4096 x 8192
+// 184, 187; 4096 x 6000 144, 157.  (Eight quads: 2048 x 16384 packed 129, four 109.)
 template <class F>
-void for_cols(size_t n, F &&f) {
+void for_cols(size_t n, bool packed, F &&f) {
     using std::integral_constant;
-    if (n <= 256) f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<bool, false>{});
-    else if (n <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 2>{}, integral_constant<bool, false>{});
-    else if (n <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
-    else if (n <= 2048) f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<bool, false>{});
-    else if (n <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
-    else if (n <= 8192) f(integral_constant<int, 16>{}, integral_constant<int, 2>{}, integral_constant<bool, false>{});
-    else if (n <= kMaxHeldCols)
-        f(integral_constant<int, 16>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
-    else f(integral_constant<int, 16>{}, integral_constant<int, 4>{}, integral_constant<bool, true>{});
+    const integral_constant<int, 1> one{};
+    const integral_constant<int, 2> two{};
+    const integral_constant<int, 4> four{};
+    const integral_constant<int, 8> eight{};
+    const integral_constant<int, 16> sixteen{};
+    const integral_constant<bool, false> held{};
+    if (n <= 256) f(one, one, held);
+    else if (n <= 512) f(one, two, held);
+    else if (n <= 1024) f(one, four, held);
+    else if (n <= 2048) f(four, two, held);
+    else if (n <= 4096) f(four, four, held);
+    else if (n <= 8192) packed ? f(sixteen, two, held) : f(eight, four, held);
+    else if (n <= kMaxHeldCols) f(sixteen, four, held);
+    else f(sixteen, four, integral_constant<bool, true>{});
 }
 
 size_t rows_per_block(size_t cols) { return cols <= 1024 ? 4 : 1; }
@@ -408,7 +429,7 @@ static int norm_forward(const float *x, const float *residual, const float *weig
     if (rows == 0 || cols == 0) return TS_HIP_OK;
     if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
     const NormArgs a = {x, residual, weight, h, y, codes, scales, rows, cols, packed_pitch(cols), eps};
-    for_cols(codes ? a.pitch : cols, [&](auto w, auto nv, auto long_rows) {
+    for_cols(codes ? a.pitch : cols, codes != nullptr, [&](auto w, auto nv, auto long_rows) {
         launch_norm<w.value, nv.value, long_rows.value>(a, codes != nullptr, as_stream(stream));
     });
     return launch_status();
@@ -440,7 +461,7 @@ int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *g
     if (!dweight || grid > kTicketParts || grid * cols > kTicketFloats) ticket = nullptr;
     const NormBackArgs a = {h, weight, go, dh, dweight ? workspace : nullptr, rows, cols, eps, dweight, ticket};
     const hipStream_t s = as_stream(stream);
-    for_cols(cols, [&](auto w, auto nv, auto long_rows) {
+    for_cols(cols, false, [&](auto w, auto nv, auto long_rows) {
         launch_back<w.value, nv.value, long_rows.value>(a, grid, s);
     });
     if (dweight && !ticket)
