@@ -54,6 +54,7 @@ typedef __bf16 b8v_t __attribute__((ext_vector_type(8)));
 typedef float f2v_t __attribute__((ext_vector_type(2)));
 typedef float f2u_t __attribute__((ext_vector_type(2), aligned(4)));
 typedef unsigned u2v_t __attribute__((ext_vector_type(2)));
+typedef unsigned u4v_t __attribute__((ext_vector_type(4)));
 // four floats at any 4-byte address (gfx950 loads them with one instruction)
 typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
 

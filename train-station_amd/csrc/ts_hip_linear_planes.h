@@ -88,10 +88,12 @@ struct PlaneSide {
             return 16u * lane;
         }
     }
-    // a code fragment's eight bytes: k block k of row block b
-    static __device__ __forceinline__ u2v_t codes8(const char *at, int b, int k, int lane) {
+    // the codes of k blocks 2 k and 2 k + 1 of row block b: lane 32 h + i has 16 h .. 16 h + 15
+    // of row i's 32, its first eight for the one fragment and the others for the next (the
+    // same order of k on both sides)
+    static __device__ __forceinline__ u4v_t codes16(const char *at, int b, int k, int lane) {
         const int i = lane & 31, h = lane >> 5;
-        return *reinterpret_cast<const u2v_t *>(at + b * 4096 + i * 128 + 8 * h + (16 * k ^ 16 * (i >> 1 & 7)));
+        return *reinterpret_cast<const u4v_t *>(at + b * 4096 + i * 128 + 16 * ((2 * k + h) ^ (i >> 1 & 7)));
     }
 };
 
@@ -205,9 +207,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     auto frag = [&](const char *stage, int n) {
         return *reinterpret_cast<const b8v_t *>(stage + n * kFragBytes + lane * 16);
     };
-    // a side's fragment of one piece from its codes: k block k of row block b, four: its row's scales
-    auto widened = [&](u2v_t c, unsigned four, int byte) {
-        return widen(c[0], c[1], __uint_as_float((four >> (8 * byte) & 255u) << 23));  // a scale byte is fp32's exponent
+    // a side's fragment from its codes, four: its row's scales
+    auto widened = [&](const u4v_t &c, int half, unsigned four, int byte) {  // a scale byte is fp32's exponent
+        return widen(c[2 * half], c[2 * half + 1], __uint_as_float((four >> (8 * byte) & 255u) << 23));
     };
 
     floatx16 acc[FM][FN];
@@ -236,13 +238,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
 #pragma unroll
             for (int c = 0; c < FN; ++c) sb[c] = row_scales(A::kScaleUnits, wn * FN + c);
         }
+        u4v_t ca[FM], cb[FN];  // two k blocks' codes
 #pragma unroll
         for (int k = 0; k < SK; ++k) {
+            if constexpr (A::kCodes) {
+                if (k % 2 == 0) {
+#pragma unroll
+                    for (int c = 0; c < FN; ++c) cb[c] = B::codes16(at_b, wn * FN + c, k / 2, lane);
+#pragma unroll
+                    for (int x = 0; x < FM; ++x) ca[x] = A::codes16(at, wm * FM + x, k / 2, lane);
+                }
+            }
             b8v_t fb[FN][PB];
 #pragma unroll
             for (int c = 0; c < FN; ++c) {
                 if constexpr (B::kCodes) {
-                    fb[c][0] = widened(B::codes8(at_b, wn * FN + c, k, lane), sb[c], k / 2);
+                    fb[c][0] = widened(cb[c], k % 2, sb[c], k / 2);
                 } else {
 #pragma unroll
                     for (int p = 0; p < PB; ++p) fb[c][p] = frag(at_b, ((wn * FN + c) * SK + k) * PB + p);
@@ -253,7 +264,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
             for (int x = 0; x < FM; ++x) {
                 b8v_t fa[PA];
                 if constexpr (A::kCodes) {
-                    fa[0] = widened(A::codes8(at, wm * FM + x, k, lane), sa[x], k / 2);
+                    fa[0] = widened(ca[x], k % 2, sa[x], k / 2);
                 } else {
 #pragma unroll
                     for (int p = 0; p < PA; ++p) fa[p] = frag(at, ((wm * FM + x) * SK + k) * PA + p);
