@@ -15,11 +15,11 @@ pytestmark = pytest.mark.gpu
 class DeviceArray:
     """A device buffer as other libraries expose theirs."""
 
-    def __init__(self, a):
+    def __init__(self, a, offset=0):
         self.host = np.ascontiguousarray(a)
         words = np.zeros(max((self.host.nbytes + 3) // 4, 1), np.float32)
         words.view(np.uint8)[: self.host.nbytes] = self.host.reshape(-1).view(np.uint8)
-        self.dev = Dev.of(words)
+        self.dev = Dev.of(words, offset)
         kind = "<f4" if self.host.dtype == np.float32 else "|u1"
         self.__cuda_array_interface__ = dict(shape=self.host.shape, typestr=kind, data=(self.dev.ptr, False), version=2)
 
@@ -301,6 +301,51 @@ def test_linear_large(m, k, n, name, bias, residual, checkpoint):
 @pytest.mark.parametrize("name,bias,residual,checkpoint", [("silu", True, True, "full"), ("gelu_tanh", True, False, "8bit")])
 def test_linear_long(m, k, n, name, bias, residual, checkpoint):
     check_layer(m, k, n, name, bias, residual, checkpoint)
+
+
+# few rows beside a large weight, which is read as it lies: one tile of rows and several, odd sizes of
+# everything but the weight's rows, k past a stage's end, k in one part and in eight
+STREAMS = [(17, 5003, 6404), (64, 4096, 2052), (65, 2501, 3244), (128, 2000, 2060), (129, 1531, 2604), (512, 1001, 1000),
+           (300, 130, 12900), (250, 16001, 132), (200, 2046, 2750)]
+
+
+@pytest.mark.parametrize("m,k,n", STREAMS)
+@pytest.mark.parametrize("name,bias,residual,checkpoint", [("silu", True, True, "full"), ("gelu_tanh", True, False, "8bit"),
+                                                           ("none", False, True, "8bit")])
+def test_linear_beside_a_large_weight(m, k, n, name, bias, residual, checkpoint):
+    check_layer(m, k, n, name, bias, residual, checkpoint)
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_linear_of_a_weight_at_any_address(offset):
+    m, k, n = 100, 2052, 2604
+    x, w, b, r, go = layer_case(m, k, n, True, True)
+    W = T.Tensor.from_device(DeviceArray(w, offset)).with_requires_grad()
+    X = tensor(x).with_requires_grad()
+    y = X.linear(W, bias=tensor(b), activation="silu", residual=tensor(r))
+    want, z = R.linear(x, w, b, "silu", r)
+    assert_within(y.data(), want, R.linear_bound(x, w, b, "silu", r, z), "y")
+    y.backward(tensor(go))
+    z = R.linear(x, w, b, "none", None)[0]
+    dx, dw, _ = R.linear_grads(x, w, z, "silu", go)
+    ex, ew, _ = R.linear_grads_bound(x, w, b, z, "silu", go)
+    assert_within(X.grad_by_value().data(), dx, ex, "dx")
+    assert_within(W.grad_by_value().data(), dw, ew, "dweight")
+    T.clear_gradients()
+
+
+def test_linear_beside_a_large_weight_that_is_not_finite():
+    m, k, n = 40, 4100, 4000
+    x, w = normal((m, k), 1), normal((k, n), 2)
+    w[4099, 7], w[0, 200], x[3, 5] = np.inf, np.nan, -np.inf
+    with np.errstate(invalid="ignore"):
+        want = x.astype(np.float64) @ w.astype(np.float64)
+    got = tensor(x).linear(tensor(w)).data()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    fine = np.isfinite(want)
+    bound = R.product_bound(*(np.where(np.isfinite(a), a, 0) for a in (x, w)))
+    assert fine.any() and np.all(np.abs(got[fine] - want[fine]) <= bound[fine])
 
 
 def test_linear_large_keeps_small_values_beside_large_ones():

@@ -189,11 +189,15 @@ struct LinearProduct {
     int M, N, K;
     float *C;
     LinearEpi epi;
+    bool streams = false;  // B is read as it lies (streams_take)
 };
 
 // ---- the large products (ts_hip_linear_planes.hip) ---------------------------------
 
 bool planes_take(size_t M, size_t N, size_t K);
+// whether floats B of rows of ld go to the product as they lie, if they begin at 16 bytes
+bool streams_take(size_t M, size_t N, size_t K, size_t ld);
+size_t streams_workspace_floats(size_t M, size_t N, size_t K, Src a);
 // a product's planes (none where both operands are codes along k) and slices
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b);
 size_t planes_sum_floats(size_t N, size_t K);

@@ -1,5 +1,7 @@
 // A layer's forward and backward (ts_hip.h, ts_hip_linear and the entries after
 // it) and the launches of its small products.
+#include <algorithm>
+
 #include "ts_hip_linear_direct.h"
 
 namespace tship {
@@ -222,6 +224,18 @@ LinearProduct dw_product(const ts_hip_linear_shape &s, const float *x, const uin
     return p;
 }
 
+// A product with a layer's weight goes by planes (true) or directly: floats that
+// stream by planes of the other side, where they begin at 16 bytes.
+bool weight_planes(LinearProduct &p) {
+    if (!streams_take(p.M, p.N, p.K, p.B.ld)) return planes_take(p.M, p.N, p.K);
+    p.streams = reinterpret_cast<uintptr_t>(p.B.p) % 16 == 0;
+    return p.streams;
+}
+size_t weight_floats(size_t M, size_t N, size_t K, Src a, Src b, size_t ld) {
+    if (streams_take(M, N, K, ld)) return std::max(streams_workspace_floats(M, N, K, a), direct_floats(M, N, K));
+    return planes_take(M, N, K) ? planes_workspace_floats(M, N, K, a, b) : direct_floats(M, N, K);
+}
+
 // The backward pass's workspace, in floats: dz, the parts of its column sums, then
 // each product's planes or slices: the layer's computed again, dx's, dweight's.
 struct BackLayout {
@@ -232,12 +246,11 @@ BackLayout back_layout(const ts_hip_linear_shape &s) {
     l.sums = round64(s.batch * s.fan_out);
     l.again = l.sums + (planes_take(s.fan_in, s.fan_out, s.batch) ? round64(planes_sum_floats(s.fan_out, s.batch))
                                                                   : sum_floats(s.batch, s.fan_out));
-    auto product = [](size_t M, size_t N, size_t K, Src a, Src b) {
-        return planes_take(M, N, K) ? round64(planes_workspace_floats(M, N, K, a, b)) : direct_floats(M, N, K);
-    };
-    l.dx = l.again + product(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR);
-    l.dw = l.dx + product(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK);
-    l.total = l.dw + product(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR);
+    l.dx = l.again + round64(weight_floats(s.batch, s.fan_out, s.fan_in, Src::kCodesK, Src::kFloatR, s.fan_out));
+    l.dw = l.dx + round64(weight_floats(s.batch, s.fan_in, s.fan_out, Src::kFloatK, Src::kFloatK, s.fan_out));
+    l.total = l.dw + (planes_take(s.fan_in, s.fan_out, s.batch)
+                          ? round64(planes_workspace_floats(s.fan_in, s.fan_out, s.batch, Src::kFloatR, Src::kFloatR))
+                          : direct_floats(s.fan_in, s.fan_out, s.batch));
     return l;
 }
 
@@ -278,9 +291,7 @@ extern "C" {
 size_t ts_hip_linear_workspace_floats(const ts_hip_linear_shape *shape) {
     if (!shape_ok(shape)) return 0;
     const ts_hip_linear_shape &d = *shape;
-    return planes_take(d.batch, d.fan_out, d.fan_in)
-               ? planes_workspace_floats(d.batch, d.fan_out, d.fan_in, Src::kFloatK, Src::kFloatR)
-               : direct_floats(d.batch, d.fan_out, d.fan_in);
+    return weight_floats(d.batch, d.fan_out, d.fan_in, Src::kFloatK, Src::kFloatR, d.fan_out);
 }
 
 int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float *weight, const float *bias, int act,
@@ -294,12 +305,12 @@ int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float 
     if (d.fan_out == 0) return codes ? ts_hip_pack8(x, d.batch, d.fan_in, codes, scales, stream) : TS_HIP_OK;
     if (!y || (d.fan_in && (!x || !weight))) return TS_HIP_EINVAL;
     const hipStream_t s = as_stream(stream);
-    const LinearProduct p = forward_product(d, x, nullptr, nullptr, weight, y, {bias, residual, nullptr, slope, act});
+    LinearProduct p = forward_product(d, x, nullptr, nullptr, weight, y, {bias, residual, nullptr, slope, act});
     if (!workspace && ts_hip_linear_workspace_floats(shape)) return TS_HIP_EINVAL;
-    if (planes_take(d.batch, d.fan_out, d.fan_in)) {
+    if (weight_planes(p)) {
         PlaneWrites writes;
         writes.a(p, workspace, codes, scales);
-        writes.b(p, workspace);
+        if (!p.streams) writes.b(p, workspace);
         writes.run(s);
         planes_multiply(p, workspace, nullptr, nullptr, s);
         return launch_status();
@@ -341,18 +352,18 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
     if (act == TS_HIP_ACT_NONE) slope = nullptr;
     if ((again && (!codes || !weight)) || (dx && !weight) || (dweight && !codes && !x)) return TS_HIP_EINVAL;
     const float *dz = again ? workspace : go;
-    const LinearProduct pz = forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
-    const LinearProduct px = dx_product(d, dz, slope, weight, dx), pw = dw_product(d, x, codes, scales, dz, slope, dweight);
-    const bool planes_x = dx && planes_take(px.M, px.N, px.K), planes_w = dweight && planes_take(pw.M, pw.N, pw.K);
+    LinearProduct pz = forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
+    LinearProduct px = dx_product(d, dz, slope, weight, dx);
+    const LinearProduct pw = dw_product(d, x, codes, scales, dz, slope, dweight);
+    const bool planes_x = dx && weight_planes(px), planes_w = dweight && planes_take(pw.M, pw.N, pw.K);
     // what does not wait for dz goes into planes first, with the layer's own operands
     PlaneWrites writes;
-    if (planes_x) writes.b(px, w_dx);
+    if (planes_x && !px.streams) writes.b(px, w_dx);
     if (planes_w) writes.a(pw, w_dw);
     if (again) {
-        const bool planes_z = planes_take(pz.M, pz.N, pz.K);
-        if (planes_z) {
+        if (weight_planes(pz)) {
             writes.a(pz, w_again);
-            writes.b(pz, w_again);
+            if (!pz.streams) writes.b(pz, w_again);
             writes.run(s);
             planes_multiply(pz, w_again, nullptr, nullptr, s);
         } else {

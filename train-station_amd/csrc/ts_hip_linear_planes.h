@@ -97,6 +97,67 @@ struct PlaneSide {
     }
 };
 
+// A side of floats as they lie in memory (16-byte rows: ld a multiple of 4 and the
+// base aligned), split as its fragments are read; R columns of C, stages of 32 k.
+//   along k: 8 rows of 32 k a unit, a row's chunk c of 16 bytes at c ^ row / 2 % 8
+//   along the rows: 2 k of 128 rows a unit, a k's row at row ^ 32 (k / 8 % 2)
+template <Src S, int R, int SK>
+struct StreamSide {
+    static constexpr bool kCodes = false;
+    static constexpr int P = 3, kBlocks = R / kPlaneRows, kUnits = R / 8;
+    static_assert(SK * kPlaneK == 32 && R == 128, "units");
+    static constexpr int kBytes = kUnits * kFragBytes, kScaleUnits = 0;
+
+    static __device__ __forceinline__ const char *start(const Operand &o, int b0) {
+        const size_t j0 = static_cast<size_t>(b0) * kPlaneRows;
+        return reinterpret_cast<const char *>(o.p + (S == Src::kFloatK ? j0 * o.ld : j0));
+    }
+    static __device__ __forceinline__ size_t step(const Operand &o) {
+        return S == Src::kFloatK ? 128 : static_cast<size_t>(128) * o.ld;
+    }
+    // unit u's lane: from a stage of `left` k (what lies past an edge: the last there
+    // is, beside zeros of the other side or sums that are not stored)
+    static __device__ __forceinline__ unsigned offset(const Operand &o, int b0, int u, int left, int lane) {
+        const int j0 = b0 * kPlaneRows;
+        if constexpr (S == Src::kFloatK) {
+            const int row = u * 8 + (lane >> 3), k = 4 * ((lane & 7) ^ (row >> 1 & 7));
+            return 4u * (static_cast<unsigned>(min(row, o.rows - 1 - j0)) * static_cast<unsigned>(o.ld) + min(k, left - 4));
+        } else {
+            const int k = u * 2 + (lane >> 5), row = 4 * (lane & 31) ^ 32 * (k >> 3 & 1);
+            return 4u * (static_cast<unsigned>(min(k, left - 1)) * static_cast<unsigned>(o.ld) + min(row, o.rows - 4 - j0));
+        }
+    }
+    // block b's fragment of k block k, its three pieces
+    static __device__ __forceinline__ void frags(const char *at, int b, int k, int lane, b8v_t (&f)[3]) {
+        const int i = lane & 31, h = lane >> 5;
+        float v[8];
+        if constexpr (S == Src::kFloatK) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const f4v_t four = *reinterpret_cast<const f4v_t *>(at + (b * kPlaneRows + i) * 128 +
+                                                                    16 * ((4 * k + 2 * h + q) ^ (i >> 1 & 7)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = four[e];
+            }
+        } else {
+            const float *from = reinterpret_cast<const float *>(at) + (16 * k + 8 * h) * R + ((b * kPlaneRows + i) ^ 32 * h);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = from[e * R];
+        }
+        u4v_t h4, m4, l4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const Pieces p = split2(v[2 * e], v[2 * e + 1], kSplitScale);
+            h4[e] = p.h;
+            m4[e] = p.m;
+            l4[e] = p.l;
+        }
+        f[0] = __builtin_bit_cast(b8v_t, h4);
+        f[1] = __builtin_bit_cast(b8v_t, m4);
+        f[2] = __builtin_bit_cast(b8v_t, l4);
+    }
+};
+
 // Four neighbouring sums (times 2^-scale) through the epilogue; cols of them are there.
 __device__ __forceinline__ void epilogue4(const LinearEpi &e, size_t at, const f4v_t &v, int scale, const float (&bias)[4],
                                           const float (&extra)[4], int cols, float (&o)[4]) {
@@ -131,13 +192,14 @@ __device__ __forceinline__ void epilogue4(const LinearEpi &e, size_t at, const f
 }
 
 // SA, SB: the operands' kinds.  BM x BN by WM x WN waves; stages of SK k blocks,
-// NST of them in LDS.
-template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST>
-__global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
+// NST of them in LDS.  STREAM: B is floats as they lie (StreamSide), and KG groups
+// of waves share a stage's k blocks.
+template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST, bool STREAM = false, int KG = 1>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs g) {
     using A = PlaneSide<SA, BM, SK, as_codes(SA, SB)>;
-    using B = PlaneSide<SB, BN, SK, as_codes(SA, SB)>;
+    using B = std::conditional_t<STREAM, StreamSide<SB, BN, 2>, PlaneSide<SB, BN, SK, as_codes(SA, SB)>>;
     constexpr int PA = A::P, PB = B::P;
-    constexpr int NW = WM * WN, FM = BM / WM / kPlaneRows, FN = BN / WN / kPlaneRows;
+    constexpr int NW = WM * WN * KG, FM = BM / WM / kPlaneRows, FN = BN / WN / kPlaneRows;
     constexpr int NU = A::kUnits + B::kUnits, PER = (NU + NW - 1) / NW;  // a wave's; the last may be moved twice
     constexpr int NSC = A::kScaleUnits + B::kScaleUnits, SPER = (NSC + NW - 1) / NW;
     constexpr int kScalesAt = A::kBytes + B::kBytes, kStage = kScalesAt + 256 * NSC;
@@ -157,7 +219,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     const int first = slice * g.slice_stages, end = min(first + g.slice_stages, g.stages);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
+    const int wm = wave / WN % WM, wn = wave % WN, kg = wave / (WM * WN);
     const int ra = tm * A::kBlocks, rb = tn * B::kBlocks;  // first row blocks
 
     // this wave's units of a stage: consecutive ones of A's, then of B's
@@ -170,6 +232,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
         if (f < A::kUnits) {
             src[i] = A::start(g.A, g.p.A, ra, f, g.kb, g.rows_a);
             off[i] = A::offset(g.p.A, ra, f, lane);
+        } else if constexpr (STREAM) {
+            src[i] = B::start(g.p.B, rb);
+            off[i] = B::offset(g.p.B, rb, f - A::kUnits, 32, lane);
         } else {
             src[i] = B::start(g.B, g.p.B, rb, f - A::kUnits, g.kb, g.rows_b);
             off[i] = B::offset(g.p.B, rb, f - A::kUnits, lane);
@@ -183,8 +248,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int f = min(wave * PER + i, NU - 1);
-            const char *p = src[i] + at * (f < A::kUnits ? A::kStep : B::kStep);
-            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[i]), "s"(p), "s"(base + f * kFragBytes)
+            unsigned from = off[i];
+            const char *p;
+            if constexpr (STREAM) {
+                const int left = g.p.K - at * SK * kPlaneK;  // 1 at least
+                p = src[i] + at * (f < A::kUnits ? A::kStep : B::step(g.p.B));
+                if (left < 32 && f >= A::kUnits) from = B::offset(g.p.B, rb, f - A::kUnits, left, lane);  // uniform
+            } else {
+                p = src[i] + at * (f < A::kUnits ? A::kStep : B::kStep);
+            }
+            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(from), "s"(p), "s"(base + f * kFragBytes)
                          : "memory", "m0");
         }
         if constexpr (NSC > 0) {
@@ -240,7 +313,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
         }
         u4v_t ca[FM], cb[FN];  // two k blocks' codes
 #pragma unroll
-        for (int k = 0; k < SK; ++k) {
+        for (int n = 0; n < SK / KG; ++n) {
+            const int k = KG == 1 ? n : n * KG + kg;
             if constexpr (A::kCodes) {
                 if (k % 2 == 0) {
 #pragma unroll
@@ -252,7 +326,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
             b8v_t fb[FN][PB];
 #pragma unroll
             for (int c = 0; c < FN; ++c) {
-                if constexpr (B::kCodes) {
+                if constexpr (STREAM) {
+                    B::frags(at_b, wn * FN + c, k, lane, fb[c]);
+                } else if constexpr (B::kCodes) {
                     fb[c][0] = widened(cb[c], k % 2, sb[c], k / 2);
                 } else {
 #pragma unroll
@@ -295,6 +371,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outstanding at exit
 
+    if constexpr (KG == 2) {  // the second group's sums onto the first's
+        static_assert(NST * kStage >= BM * BN * 4, "room for the second's");
+        f4v_t *const second = reinterpret_cast<f4v_t *>(lds) + wave % (WM * WN) * FM * FN * 256 + lane;
+        __syncthreads();  // the last fragments
+        if (kg == 1) {
+#pragma unroll
+            for (int n = 0; n < FM * FN * 4; ++n) {
+                const floatx16 &v = acc[n / 4 / FN][n / 4 % FN];
+                second[n * 64] = f4v_t{v[4 * (n % 4)], v[4 * (n % 4) + 1], v[4 * (n % 4) + 2], v[4 * (n % 4) + 3]};
+            }
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int n = 0; n < FM * FN * 4; ++n) {
+                const f4v_t v = second[n * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[n / 4 / FN][n / 4 % FN][4 * (n % 4) + e] += v[e];
+            }
+        }
+    }
     if constexpr (PB == 3) {  // (codes hold finite values, and their product's own range is fp32's)
         float worst = 0.0f;  // NaN * 0 and inf * 0 stay NaN
 #pragma unroll
@@ -319,7 +416,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     // A turn's go or residual is on its way while the one before is computed.
     static_assert(NST * kStage >= BM * BN * 4 && BN >= 64, "room for the tile");
     constexpr int kScale = (PA == 3 ? 16 : 0) + (PB == 3 ? 16 : 0);
-    constexpr int kRowQuads = BN / 4, kRows = 4, kStep = 64 * NW / kRowQuads, kTurns = BM / kStep / kRows;
+    constexpr int kRowQuads = BN / 4, kStep = 64 * NW / kRowQuads, kRows = BM / kStep < 4 ? BM / kStep : 4, kTurns = BM / kStep / kRows;
     static_assert(kTurns * kStep * kRows == BM, "turns of kRows rows a lane");
     float *const sums = reinterpret_cast<float *>(lds);
     const float *extra = g.p.epi.go ? g.p.epi.go : g.p.epi.residual;
@@ -349,8 +446,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
     }
     const int li = lane & 31, lh = lane >> 5;
     __syncthreads();  // the last fragments
+    if (kg == 0) {  // uniform
 #pragma unroll
-    for (int x = 0; x < FM; ++x)
+        for (int x = 0; x < FM; ++x)
 #pragma unroll
         for (int c = 0; c < FN; ++c)
 #pragma unroll
@@ -358,6 +456,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_planes(PlanesArgs g) {
                 const int row = (wm * FM + x) * kPlaneRows + 8 * (r >> 2) + 4 * lh + (r & 3);
                 sums[row * BN + (((wn * FN + c) * kPlaneRows + li) ^ 32 * lh)] = acc[x][c][r];
             }
+    }
     __syncthreads();
     if (cols <= 0) return;  // (no barrier follows)
 #pragma unroll 1

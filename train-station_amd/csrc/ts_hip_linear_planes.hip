@@ -283,14 +283,14 @@ PlaneJob plane_job(const PlaneTask &t) {
     return j;
 }
 
-template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST>
+template <Src SA, Src SB, int BM, int BN, int WM, int WN, int SK, int NST, bool STREAM = false, int KG = 1>
 void launch_planes(PlanesArgs g, hipStream_t s) {
     g.tiles_m = (g.p.M + BM - 1) / BM;
     g.tiles_n = (g.p.N + BN - 1) / BN;
     g.stages = as_codes(SA, SB) ? static_cast<int>(g.p.A.pitch / kPackGroup) : g.kb / SK;
     g.slice_stages = (g.stages + g.p.slices - 1) / g.p.slices;
-    launch((linear_planes<SA, SB, BM, BN, WM, WN, SK, NST>), dim3(g.tiles_m * g.tiles_n * g.p.slices + g.sums.blocks),
-           dim3(64 * WM * WN), 0, s, g);
+    launch((linear_planes<SA, SB, BM, BN, WM, WN, SK, NST, STREAM, KG>),
+           dim3(g.tiles_m * g.tiles_n * g.p.slices + g.sums.blocks), dim3(64 * WM * WN * KG), 0, s, g);
 }
 
 // The tile, and the slices of K, that cost least: rounds over the chip x a tile's
@@ -329,11 +329,29 @@ PlanesPlan choose_plan(size_t M, size_t N, size_t K, Src a, Src b) {
     return best;
 }
 
+// Tiles of a product whose B streams: 128 columns, all rows up to 128, and the
+// slices of K that fill the chip, of 256 k at least.
+PlanesPlan stream_plan(size_t M, size_t N, size_t K) {
+    PlanesPlan p = {M <= 64 ? 64 : 128, 128, 1};
+    const size_t tiles = (M + p.bm - 1) / p.bm * ((N + 127) / 128), cus = device_cu_count();
+    while (tiles * p.slices * 2 <= cus && K >= static_cast<size_t>(p.slices) * 2 * 256) p.slices *= 2;
+    return p;
+}
+
 size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace
 
 bool planes_take(size_t M, size_t N, size_t K) { return 2.0 * M * N * K >= 1.5e9 && M >= 128 && N >= 128 && K >= 64; }
+
+bool streams_take(size_t M, size_t N, size_t K, size_t ld) {
+    return M > 16 && M <= 512 && N >= 128 && K >= 64 && 2.0 * M * N * K >= 1e9 && ld % 4 == 0 && ld <= size_t(1) << 20;
+}
+
+size_t streams_workspace_floats(size_t M, size_t N, size_t K, Src a) {
+    const PlanesPlan plan = stream_plan(M, N, K);
+    return (round_256(plane_bytes(M, K, a)) + (plan.slices > 1 ? round_256(plan.slices * M * N * sizeof(float)) : 0)) / sizeof(float);
+}
 
 size_t planes_workspace_floats(size_t M, size_t N, size_t K, Src a, Src b) {
     const PlanesPlan plan = choose_plan(M, N, K, a, b);
@@ -361,11 +379,12 @@ void planes_write(const PlaneTask *tasks, int count, hipStream_t s) {
 
 void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_parts, float *sums, hipStream_t s) {
     char *pa = planes_of_a(p, workspace), *pb = planes_of_b(p, workspace);
-    const PlanesPlan plan = choose_plan(p.M, p.N, p.K, p.a, p.b);
+    const PlanesPlan plan = p.streams ? stream_plan(p.M, p.N, p.K) : choose_plan(p.M, p.N, p.K, p.a, p.b);
     PlanesArgs g = {pa, pb, direct_product(p), k_blocks(p.K), row_blocks(p.M), row_blocks(p.N), 0, 0, 0, 0, {}};
     g.p.slices = plan.slices;
     if (sums) g.sums = part_sums(sum_parts, across_chunks(p.N, p.K), p.N, sums);
-    if (plan.slices > 1)
+    if (p.streams && plan.slices > 1) g.p.part = reinterpret_cast<float *>(pb);
+    else if (plan.slices > 1)
         g.p.part = as_codes(p.a, p.b) ? workspace : reinterpret_cast<float *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
     with_sources(p.a, p.b, [&](auto a, auto b) {
         constexpr Src A = a.value, B = b.value;
@@ -373,6 +392,13 @@ void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_
         // 128 x 128 has three pieces on both sides (8192 x 4096 x 4096 1242 us by eight waves,
         // 1302 by four), and four where the smallest tile has them on one (1024 x 4096 x 2048
         // 59 us, 61 in three of 32)
+        if constexpr (A != Src::kFloatR && A != Src::kCodesR && !as_codes(A, B)) {
+            if (p.streams) {
+                if (plan.bm == 64) launch_planes<A, B, 64, 128, 1, 4, 2, 3, true, 2>(g, s);
+                else launch_planes<A, B, 128, 128, 1, 4, 2, 3, true, 2>(g, s);
+                return;
+            }
+        }
         if constexpr (as_codes(A, B)) {
             if (plan.bm == 64) launch_planes<A, B, 64, 64, 2, 2, 8, 2>(g, s);
             else if (plan.bn == 64) launch_planes<A, B, 128, 64, 2, 2, 8, 2>(g, s);
