@@ -127,10 +127,9 @@ struct StreamSide {
             return 4u * (static_cast<unsigned>(min(k, left - 1)) * static_cast<unsigned>(o.ld) + min(row, o.rows - 4 - j0));
         }
     }
-    // block b's fragment of k block k, its three pieces
-    static __device__ __forceinline__ void frags(const char *at, int b, int k, int lane, b8v_t (&f)[3]) {
+    // a lane's eight values of block b's fragment of k block k
+    static __device__ __forceinline__ void values(const char *at, int b, int k, int lane, float (&v)[8]) {
         const int i = lane & 31, h = lane >> 5;
-        float v[8];
         if constexpr (S == Src::kFloatK) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -144,6 +143,9 @@ struct StreamSide {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = from[e * R];
         }
+    }
+    // ... and its three pieces
+    static __device__ __forceinline__ void split(const float (&v)[8], b8v_t (&f)[3]) {
         u4v_t h4, m4, l4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -291,9 +293,62 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs
 #pragma unroll
         for (int c = 0; c < FN; ++c) acc[x][c] = floatx16{};
 
+    // a k block's products of a block, added to acc
+    auto multiply = [](floatx16 &acc, const b8v_t (&a)[PA], const b8v_t (&b)[PB], float sign) {
+        auto mm = [&](floatx16 v, int pa, int pb) {
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa], b[pb], v, 0, 0, 0);
+        };
+        if constexpr (PA == 3) {
+            floatx16 v = {};
+            v = mm(v, 0, 2);
+            v = mm(v, 1, 1);
+            v = mm(v, 2, 0);
+            v = mm(v, 0, 1);
+            v = mm(v, 1, 0);
+            v = mm(v, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = __builtin_fmaf(v[r], sign, acc[r]);
+        } else {
+#pragma unroll
+            for (int p = PB - 1; p >= 0; --p) acc = mm(acc, 0, p);
+        }
+    };
+    int slot = 0;
+    if constexpr (STREAM) {
+        // A group's wave has one k block a stage.  B's values of the next are read and
+        // split beside the last block's products of this one, whose A is read by then.
+        static_assert(SK == KG && FN == 1 && FM > 1, "a k block a wave");
+        auto read_a = [&](int slot, int x, b8v_t (&fa)[PA]) {
+#pragma unroll
+            for (int p = 0; p < PA; ++p) fa[p] = frag(lds + slot * kStage, ((wm * FM + x) * SK + kg) * PA + p);
+        };
+        float v[8];
+        b8v_t fb[3];
+#pragma unroll
+        for (int s = 0; s < NST; ++s) dma(first + s, s);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PER * (NST - 1)) : "memory");
+        B::values(lds + A::kBytes, wn, kg, lane, v);
+        B::split(v, fb);
+        const float sign = kg ? -1.0f : 1.0f;
+        for (int s = first; s < end; ++s) {
+            b8v_t fa[PA];
+#pragma unroll
+            for (int x = 0; x + 1 < FM; ++x) {
+                read_a(slot, x, fa);
+                multiply(acc[x][0], fa, fb, sign);
+            }
+            read_a(slot, FM - 1, fa);
+            // the next stage has landed, and every wave has read this one
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER * (NST - 2)) : "memory");
+            dma(s + NST, slot);
+            slot = slot + 1 == NST ? 0 : slot + 1;
+            B::values(lds + slot * kStage + A::kBytes, wn, kg, lane, v);  // (past the end: not used)
+            multiply(acc[FM - 1][0], fa, fb, sign);
+            B::split(v, fb);
+        }
+    } else {
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) dma(first + s, s);
-    int slot = 0;
     for (int s = first; s < end; ++s) {
         // this stage has landed, and every wave is done with the one before
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((PER + SPER) * (NST - 2)) : "memory");
@@ -313,8 +368,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs
         }
         u4v_t ca[FM], cb[FN];  // two k blocks' codes
 #pragma unroll
-        for (int n = 0; n < SK / KG; ++n) {
-            const int k = KG == 1 ? n : n * KG + kg;
+        for (int k = 0; k < SK; ++k) {
             if constexpr (A::kCodes) {
                 if (k % 2 == 0) {
 #pragma unroll
@@ -326,9 +380,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs
             b8v_t fb[FN][PB];
 #pragma unroll
             for (int c = 0; c < FN; ++c) {
-                if constexpr (STREAM) {
-                    B::frags(at_b, wn * FN + c, k, lane, fb[c]);
-                } else if constexpr (B::kCodes) {
+                if constexpr (B::kCodes) {
                     fb[c][0] = widened(cb[c], k % 2, sb[c], k / 2);
                 } else {
 #pragma unroll
@@ -346,28 +398,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs
                     for (int p = 0; p < PA; ++p) fa[p] = frag(at, ((wm * FM + x) * SK + k) * PA + p);
                 }
 #pragma unroll
-                for (int c = 0; c < FN; ++c) {
-                    auto mm = [&](floatx16 v, int pa, int pb) {
-                        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[pa], fb[c][pb], v, 0, 0, 0);
-                    };
-                    if constexpr (PA == 3) {
-                        floatx16 v = {};
-                        v = mm(v, 0, 2);
-                        v = mm(v, 1, 1);
-                        v = mm(v, 2, 0);
-                        v = mm(v, 0, 1);
-                        v = mm(v, 1, 0);
-                        v = mm(v, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[x][c][r] = __builtin_fmaf(v[r], sign, acc[x][c][r]);
-                    } else {
-#pragma unroll
-                        for (int p = PB - 1; p >= 0; --p) acc[x][c] = mm(acc[x][c], 0, p);
-                    }
-                }
+                for (int c = 0; c < FN; ++c) multiply(acc[x][c], fa, fb[c], sign);
             }
         }
         slot = slot + 1 == NST ? 0 : slot + 1;
+    }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outstanding at exit
 

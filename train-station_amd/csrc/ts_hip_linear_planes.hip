@@ -1,5 +1,7 @@
 // The passes that write an operand's planes and the launches of the large
 // products (the kernel and the layout: ts_hip_linear_planes.h).
+#include <algorithm>
+
 #include "ts_hip_linear_planes.h"
 
 namespace tship {
@@ -334,7 +336,8 @@ PlanesPlan choose_plan(size_t M, size_t N, size_t K, Src a, Src b) {
 PlanesPlan stream_plan(size_t M, size_t N, size_t K) {
     PlanesPlan p = {M <= 64 ? 64 : 128, 128, 1};
     const size_t tiles = (M + p.bm - 1) / p.bm * ((N + 127) / 128), cus = device_cu_count();
-    while (tiles * p.slices * 2 <= cus && K >= static_cast<size_t>(p.slices) * 2 * 256) p.slices *= 2;
+    const size_t n = std::min(cus / tiles, K / 128);
+    if (n > 1) p.slices = static_cast<int>(n);
     return p;
 }
 
@@ -342,10 +345,12 @@ size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace
 
-bool planes_take(size_t M, size_t N, size_t K) { return 2.0 * M * N * K >= 1.5e9 && M >= 128 && N >= 128 && K >= 64; }
+bool planes_take(size_t M, size_t N, size_t K) {
+    return M >= 128 && N >= 128 && K >= 16 && (2.0 * M * N * K >= 1.5e9 || 1.0 * M * N >= 6e6);
+}
 
 bool streams_take(size_t M, size_t N, size_t K, size_t ld) {
-    return M > 16 && M <= 512 && N >= 128 && K >= 64 && 2.0 * M * N * K >= 1e9 && ld % 4 == 0 && ld <= size_t(1) << 20;
+    return M > 16 && M <= 512 && N >= 128 && K >= 64 && 2.0 * M * N * K >= 1.5e9 && ld % 4 == 0 && ld <= size_t(1) << 20;
 }
 
 size_t streams_workspace_floats(size_t M, size_t N, size_t K, Src a) {
