@@ -316,6 +316,19 @@ def test_linear_beside_a_large_weight(m, k, n, name, bias, residual, checkpoint)
     check_layer(m, k, n, name, bias, residual, checkpoint)
 
 
+# weights read as they lie by a row or a few, and large results of few k
+@pytest.mark.parametrize("m,k,n", [(1, 4100, 3000), (2, 3001, 4004), (9, 4097, 3004), (31, 2048, 6004), (33, 2500, 2504),
+                                   (4000, 1, 3100), (3501, 17, 2003)])
+@pytest.mark.parametrize("name,bias,residual,checkpoint", [("silu", True, True, "full"), ("gelu_tanh", True, False, "8bit")])
+def test_linear_of_few_rows_or_inputs(m, k, n, name, bias, residual, checkpoint):
+    check_layer(m, k, n, name, bias, residual, checkpoint)
+
+
+def test_linear_of_no_inputs_and_many_rows():
+    b, w = normal((3100,), 1), T.Tensor.zeros((0, 3100))
+    assert np.array_equal(T.Tensor.zeros((4000, 0)).linear(w, bias=tensor(b)).data(), np.tile(b, (4000, 1)))
+
+
 @pytest.mark.parametrize("offset", [0, 1, 2, 3])
 def test_linear_of_a_weight_at_any_address(offset):
     m, k, n = 100, 2052, 2604

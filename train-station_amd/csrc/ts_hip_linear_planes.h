@@ -22,6 +22,14 @@
 // three pieces on the other side codes are widened by a pass all the same: 598 and
 // 27 us, against 766 with the widening between the matrix instructions.
 //
+// Streams.  Few rows beside a large weight read each of its values once or a few
+// times, and planes of it would cost more than the product.  Its floats then go to LDS
+// as they lie, a wave has 32 columns of all the tile's rows, and splits its fragments as
+// it reads them (a fifth of the time of their products of 128 rows); the waves are in
+// two groups that share a stage's k.  128 x 4096 x 4096: 36 us, against 43 to 53 and 32
+// for the weight's planes; 64 x 4096 x 4096: 22, 45 directly (67 MB at 4.8 TB/s: 14).
+// Bound by the two in turn: without the products 128 rows take 22 us.
+//
 // Products.  With pieces on both sides the six of ts_hip_gemm_split.h, summed from
 // zero per 16 k and joined by the vector units, every second k block of A
 // negated; with pieces on one side their three products and with none the one,
@@ -348,61 +356,61 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs
         }
     } else {
 #pragma unroll
-    for (int s = 0; s < NST - 1; ++s) dma(first + s, s);
-    for (int s = first; s < end; ++s) {
-        // this stage has landed, and every wave is done with the one before
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((PER + SPER) * (NST - 2)) : "memory");
-        dma(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
-        const char *at = lds + slot * kStage, *at_b = at + A::kBytes;
-        unsigned sa[FM], sb[FN];  // the rows' scales
-        auto row_scales = [&](int first, int row) {
-            return *reinterpret_cast<const unsigned *>(at + kScalesAt + first * 256 + (row * kPlaneRows + (lane & 31)) * 4);
-        };
-        if constexpr (A::kCodes) {
-#pragma unroll
-            for (int x = 0; x < FM; ++x) sa[x] = row_scales(0, wm * FM + x);
-        }
-        if constexpr (B::kCodes) {
-#pragma unroll
-            for (int c = 0; c < FN; ++c) sb[c] = row_scales(A::kScaleUnits, wn * FN + c);
-        }
-        u4v_t ca[FM], cb[FN];  // two k blocks' codes
-#pragma unroll
-        for (int k = 0; k < SK; ++k) {
+        for (int s = 0; s < NST - 1; ++s) dma(first + s, s);
+        for (int s = first; s < end; ++s) {
+            // this stage has landed, and every wave is done with the one before
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((PER + SPER) * (NST - 2)) : "memory");
+            dma(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+            const char *at = lds + slot * kStage, *at_b = at + A::kBytes;
+            unsigned sa[FM], sb[FN];  // the rows' scales
+            auto row_scales = [&](int first, int row) {
+                return *reinterpret_cast<const unsigned *>(at + kScalesAt + first * 256 + (row * kPlaneRows + (lane & 31)) * 4);
+            };
             if constexpr (A::kCodes) {
-                if (k % 2 == 0) {
 #pragma unroll
-                    for (int c = 0; c < FN; ++c) cb[c] = B::codes16(at_b, wn * FN + c, k / 2, lane);
-#pragma unroll
-                    for (int x = 0; x < FM; ++x) ca[x] = A::codes16(at, wm * FM + x, k / 2, lane);
-                }
+                for (int x = 0; x < FM; ++x) sa[x] = row_scales(0, wm * FM + x);
             }
-            b8v_t fb[FN][PB];
+            if constexpr (B::kCodes) {
 #pragma unroll
-            for (int c = 0; c < FN; ++c) {
-                if constexpr (B::kCodes) {
-                    fb[c][0] = widened(cb[c], k % 2, sb[c], k / 2);
-                } else {
-#pragma unroll
-                    for (int p = 0; p < PB; ++p) fb[c][p] = frag(at_b, ((wn * FN + c) * SK + k) * PB + p);
-                }
+                for (int c = 0; c < FN; ++c) sb[c] = row_scales(A::kScaleUnits, wn * FN + c);
             }
-            const float sign = (s * SK + k) & 1 ? -1.0f : 1.0f;
+            u4v_t ca[FM], cb[FN];  // two k blocks' codes
 #pragma unroll
-            for (int x = 0; x < FM; ++x) {
-                b8v_t fa[PA];
+            for (int k = 0; k < SK; ++k) {
                 if constexpr (A::kCodes) {
-                    fa[0] = widened(ca[x], k % 2, sa[x], k / 2);
-                } else {
+                    if (k % 2 == 0) {
 #pragma unroll
-                    for (int p = 0; p < PA; ++p) fa[p] = frag(at, ((wm * FM + x) * SK + k) * PA + p);
+                        for (int c = 0; c < FN; ++c) cb[c] = B::codes16(at_b, wn * FN + c, k / 2, lane);
+#pragma unroll
+                        for (int x = 0; x < FM; ++x) ca[x] = A::codes16(at, wm * FM + x, k / 2, lane);
+                    }
                 }
+                b8v_t fb[FN][PB];
 #pragma unroll
-                for (int c = 0; c < FN; ++c) multiply(acc[x][c], fa, fb[c], sign);
+                for (int c = 0; c < FN; ++c) {
+                    if constexpr (B::kCodes) {
+                        fb[c][0] = widened(cb[c], k % 2, sb[c], k / 2);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < PB; ++p) fb[c][p] = frag(at_b, ((wn * FN + c) * SK + k) * PB + p);
+                    }
+                }
+                const float sign = (s * SK + k) & 1 ? -1.0f : 1.0f;
+#pragma unroll
+                for (int x = 0; x < FM; ++x) {
+                    b8v_t fa[PA];
+                    if constexpr (A::kCodes) {
+                        fa[0] = widened(ca[x], k % 2, sa[x], k / 2);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < PA; ++p) fa[p] = frag(at, ((wm * FM + x) * SK + k) * PA + p);
+                    }
+#pragma unroll
+                    for (int c = 0; c < FN; ++c) multiply(acc[x][c], fa, fb[c], sign);
+                }
             }
+            slot = slot + 1 == NST ? 0 : slot + 1;
         }
-        slot = slot + 1 == NST ? 0 : slot + 1;
-    }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outstanding at exit
 
@@ -485,12 +493,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_planes(PlanesArgs
 #pragma unroll
         for (int x = 0; x < FM; ++x)
 #pragma unroll
-        for (int c = 0; c < FN; ++c)
+            for (int c = 0; c < FN; ++c)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = (wm * FM + x) * kPlaneRows + 8 * (r >> 2) + 4 * lh + (r & 3);
-                sums[row * BN + (((wn * FN + c) * kPlaneRows + li) ^ 32 * lh)] = acc[x][c][r];
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const int row = (wm * FM + x) * kPlaneRows + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    sums[row * BN + (((wn * FN + c) * kPlaneRows + li) ^ 32 * lh)] = acc[x][c][r];
+                }
     }
     __syncthreads();
     if (cols <= 0) return;  // (no barrier follows)

@@ -331,8 +331,10 @@ PlanesPlan choose_plan(size_t M, size_t N, size_t K, Src a, Src b) {
     return best;
 }
 
-// Tiles of a product whose B streams: 128 columns, all rows up to 128, and the
-// slices of K that fill the chip, of 256 k at least.
+// Tiles of a product whose B streams: 128 columns, all rows up to 128 (half the
+// rows everywhere, and four stages: 128 x 4096 x 4096 133 us, 138 here; 256 x 4096 x
+// 4096 216, 208; 300 x 8000 x 1000 155, 145), and the slices of K that fill the chip
+// (doublings: 300 x 8000 x 1000 162, 155), of 128 k at least.
 PlanesPlan stream_plan(size_t M, size_t N, size_t K) {
     PlanesPlan p = {M <= 64 ? 64 : 128, 128, 1};
     const size_t tiles = (M + p.bm - 1) / p.bm * ((N + 127) / 128), cus = device_cu_count();
@@ -345,12 +347,24 @@ size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace
 
+// Large by its operations, or a large C of few k, whose stores bound it: 1 x 4096 x
+// 4096 forward and backward 74 us, 87 directly, 32 x 4096 x 4096 89, 108; 32 x 2048 x
+// 2048 (4e6) 68, 63; 1 x 1024 x 8192 (8e6) 57, 47.
 bool planes_take(size_t M, size_t N, size_t K) {
-    return M >= 128 && N >= 128 && K >= 16 && (2.0 * M * N * K >= 1.5e9 || 1.0 * M * N >= 6e6);
+    const double c = 1.0 * M * N;
+    return M >= 128 && N >= 128 && K > 0 && (2 * c * K >= 1.5e9 || c >= (K < 16 ? 12e6 : 6e6));
 }
 
+// Few rows beside a large weight: its planes would be written for a few readings.
+// Forward and backward, us, streamed, from planes, directly: 512 x 4096 x 4096 346,
+// 405; 256 x 2500 x 2500 125, 158; 128 x 4096 x 4096 138, 257; 64 x 4096 x 4096 93, -,
+// 145; 60 x 3000 x 3000 81, -, 113; 8 x 8192 x 8192 233, -, 310.  And where it is not
+// taken: 700 x 3000 x 3000 383, 349; 512 x 1024 x 1024 98, -, 80; 64 x 2048 x 2048 with
+// an 8-bit checkpoint 87, -, 82; 1 x 1024 x 8192 57, -, 47.
 bool streams_take(size_t M, size_t N, size_t K, size_t ld) {
-    return M > 16 && M <= 512 && N >= 128 && K >= 64 && 2.0 * M * N * K >= 1.5e9 && ld % 4 == 0 && ld <= size_t(1) << 20;
+    const double weight = 1.0 * N * K;
+    return M <= 512 && N >= 128 && K >= 64 && (2 * M * weight >= 1.5e9 || weight >= (M < 32 ? 12e6 : 6e6)) && ld % 4 == 0 &&
+           ld <= size_t(1) << 20;  // (a tile's offsets in 32 bits)
 }
 
 size_t streams_workspace_floats(size_t M, size_t N, size_t K, Src a) {
