@@ -17,7 +17,7 @@
 //
 // Codes along k on both sides need no pass: they go to LDS as they are, half the
 // bytes of bf16, and a fragment's eight are widened with their scale as they are
-// read, an instruction for two.  8192 x 4096 x 4096: 260 us, against 261 and 38 for
+// read, an instruction for two.  8192 x 4096 x 4096: 253 us, against 261 and 38 for
 // the passes from planes, whose LDS reads, 128 bytes a clock, are the bound.  Beside
 // three pieces on the other side codes are widened by a pass all the same: 598 and
 // 27 us, against 766 with the widening between the matrix instructions.

@@ -302,8 +302,8 @@ void launch_planes(PlanesArgs g, hipStream_t s) {
 // 64 x 64, pieces on both sides: 8192 x 4096 x 4096 1242, 1295, 1419; 2048 x 4096 x
 // 1024 89.6, 95, 98; 1024 x 4096 x 2048 98, 88, 106; 2048 x 1024 x 4096 163, -, 95;
 // 1024 x 1024 x 1024 45, -, 23.  One side's: 604, 631, 764; 48.5, 53, 59; 51, 50, 59;
-// 1003 x 2050 x 3000 66, 58, 53.  Codes: 256, 288, 324; 27.6, 31, 32; 31, 29, 31;
-// 2048 x 1024 x 4096 46, 35, 35; 1999 x 777 x 1531 26, 22, 19.  (128 x 256 and
+// 1003 x 2050 x 3000 66, 58, 53.  Codes: 253, 268, 298; 28, 28, 29; 29, 26, 26;
+// 2048 x 1024 x 4096 40, 29, 27; 1999 x 777 x 1531 22, 16, 14.  (128 x 256 and
 // 256 x 256 by eight waves: no faster at the largest, and slower below.)
 struct PlanesPlan {
     int bm, bn, slices;
