@@ -347,12 +347,14 @@ size_t round_256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace
 
-// Large by its operations, or a large C of few k, whose stores bound it: 1 x 4096 x
-// 4096 forward and backward 74 us, 87 directly, 32 x 4096 x 4096 89, 108; 32 x 2048 x
-// 2048 (4e6) 68, 63; 1 x 1024 x 8192 (8e6) 57, 47.
+// Large by its operations (forward and backward, us, by planes and directly: 8192 x 300 x
+// 200 (0.98e9) 82, 115; 4118 x 448 x 225 (0.83e9) 68, 87; 750 x 600 x 700 (0.63e9) 67, 64;
+// 1024 x 512 x 512 (0.54e9) 65, 50; codes, 2048 x 512 x 512 (1.07e9) 8.6, 9.6, 1024 x 512 x
+// 512 8.2, 7.5), or a large C of few k, whose stores bound it: 1 x 4096 x 4096 74, 87; 32 x
+// 4096 x 4096 89, 108; 32 x 2048 x 2048 (4e6) 68, 63; 1 x 1024 x 8192 (8e6) 57, 47.
 bool planes_take(size_t M, size_t N, size_t K) {
     const double c = 1.0 * M * N;
-    return M >= 128 && N >= 128 && K > 0 && (2 * c * K >= 1.5e9 || c >= (K < 16 ? 12e6 : 6e6));
+    return M >= 128 && N >= 128 && K > 0 && (2 * c * K >= 0.8e9 || c >= (K < 16 ? 12e6 : 6e6));
 }
 
 // Few rows beside a large weight: its planes would be written for a few readings.
@@ -407,10 +409,6 @@ void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_
         g.p.part = as_codes(p.a, p.b) ? workspace : reinterpret_cast<float *>(pb + round_256(plane_bytes(p.N, p.K, p.b)));
     with_sources(p.a, p.b, [&](auto a, auto b) {
         constexpr Src A = a.value, B = b.value;
-        // waves and stages: 128 codes a stage; else 32 k, two stages, but 16 k and three where
-        // 128 x 128 has three pieces on both sides (8192 x 4096 x 4096 1242 us by eight waves,
-        // 1302 by four), and four where the smallest tile has them on one (1024 x 4096 x 2048
-        // 59 us, 61 in three of 32)
         if constexpr (A != Src::kFloatR && A != Src::kCodesR && !as_codes(A, B)) {
             if (p.streams) {
                 if (plan.bm == 64) launch_planes<A, B, 64, 128, 1, 4, 2, 3, true, 2>(g, s);
@@ -418,6 +416,10 @@ void planes_multiply(const LinearProduct &p, float *workspace, const float *sum_
                 return;
             }
         }
+        // waves and stages: 128 codes a stage; else 32 k, two stages, but 16 k and three where
+        // 128 x 128 has three pieces on both sides (8192 x 4096 x 4096 1242 us by eight waves,
+        // 1302 by four), and four where the smallest tile has them on one (1024 x 4096 x 2048
+        // 59 us, 61 in three of 32)
         if constexpr (as_codes(A, B)) {
             if (plan.bm == 64) launch_planes<A, B, 64, 64, 2, 2, 8, 2>(g, s);
             else if (plan.bn == 64) launch_planes<A, B, 128, 64, 2, 2, 8, 2>(g, s);
