@@ -456,6 +456,24 @@ def test_linear_of_nothing(shape, checkpoint):
     T.clear_gradients()
 
 
+# sizes past which sums are shared by workgroups and weights are read as they lie, beside a zero
+@pytest.mark.parametrize("shape", [(0, 4096, 16), (0, 4096, 4096), (4, 0, 4096), (4, 4096, 0), (2100, 0, 300)])
+@pytest.mark.parametrize("checkpoint", ["full", "8bit"])
+def test_linear_of_nothing_beside_a_long_side(shape, checkpoint):
+    m, k, n = shape
+    x, w, b, go = np.zeros((m, k), np.float32), np.zeros((k, n), np.float32), normal((n,), 1), np.ones((m, n), np.float32)
+    X, W, B = (tensor(a).with_requires_grad() for a in (x, w, b))
+    y = X.linear(W, bias=B, activation="silu", checkpoint=checkpoint)
+    want, z = R.linear(x, w, b, "silu", None)
+    assert_within(y.data(), want, R.linear_bound(x, w, b, "silu", None, z), "y")
+    y.backward(tensor(go))
+    dx, dw, db = R.linear_grads(x, w, z, "silu", go)
+    eb = R.linear_grads_bound(x, w, b, z, "silu", go)[2]
+    assert np.array_equal(X.grad_by_value().data(), dx) and np.array_equal(W.grad_by_value().data(), dw)
+    assert_within(B.grad_by_value().data(), db, eb, "dbias")
+    T.clear_gradients()
+
+
 def test_linear_of_more_axes():
     x, w = normal((2, 3, 5), 1), normal((5, 4), 2)
     X = tensor(x).with_requires_grad()

@@ -91,6 +91,20 @@ def test_layer_entries_refuse():
     assert backward(dx=None) == 0
 
 
+@pytest.mark.parametrize("shape", [(0, 4096, 16), (4, 4096, 0), (0, 4096, 4096), (4, 0, 4096), (4096, 0, 16), (4, 16, 0),
+                                   (0, 16, 4096), (0, 0, 0), (4096, 4096, 0), (0, 1 << 20, 1 << 10)])
+def test_workspaces_of_empty_layers(shape):
+    """No product, so nothing for one: dz (batch x fan_out) at most."""
+    s = LinearShape(*shape)
+    assert hip.ts_hip_linear_workspace_floats(ctypes.byref(s)) == 0
+    dz = -(-shape[0] * shape[2] // 64) * 64
+    parts = -(-shape[0] // 512) * shape[2] if shape[0] > 1024 else 0
+    assert hip.ts_hip_linear_backward_workspace_floats(ctypes.byref(s)) == dz + -(-parts // 64) * 64
+    if shape[0] == 0:
+        assert linear(shape=shape, floats=0) == 0 and backward(shape=shape, dx=None, floats=0) == 0
+    assert linear(shape=(shape[0], shape[1], 0), floats=0) == 0
+
+
 def test_packed_layer_refuses():
     def call(batch=4, k=8, n=16, act=0, y=P, xc=P, ws=P):
         return hip.ts_hip_linear_packed(xc, P, ws, P, batch, k, n, None, act, None, y, None, 1 << 40, None)

@@ -106,6 +106,7 @@ DirectPlan direct_plan(size_t M, size_t N, size_t K) {
     const size_t tiles = ((M + kDirectTile - 1) / kDirectTile) * ((N + kDirectTile - 1) / kDirectTile);
     const size_t waves = static_cast<size_t>(device_cu_count()) * 16, steps = (K + kDirectK - 1) / kDirectK;
     DirectPlan p = {1, 1, static_cast<int>(steps)};
+    if (tiles == 0) return p;  // (no rows or no columns: asked for its workspace all the same)
     while (p.kg < kDirectWaves && tiles * p.kg * 2 <= waves && steps >= static_cast<size_t>(p.kg) * 2 * 2) p.kg *= 2;
     if (p.kg == kDirectWaves && steps > 16 * kDirectWaves) {
         const size_t want = steps / (8 * kDirectWaves), room = waves / (tiles * kDirectWaves);

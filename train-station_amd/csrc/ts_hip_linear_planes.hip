@@ -365,7 +365,7 @@ bool planes_take(size_t M, size_t N, size_t K) {
 // an 8-bit checkpoint 87, -, 82; 1 x 1024 x 8192 57, -, 47.
 bool streams_take(size_t M, size_t N, size_t K, size_t ld) {
     const double weight = 1.0 * N * K;
-    return M <= 512 && N >= 128 && K >= 64 && (2 * M * weight >= 1.5e9 || weight >= (M < 32 ? 12e6 : 6e6)) && ld % 4 == 0 &&
+    return M > 0 && M <= 512 && N >= 128 && K >= 64 && (2 * M * weight >= 1.5e9 || weight >= (M < 32 ? 12e6 : 6e6)) && ld % 4 == 0 &&
            ld <= size_t(1) << 20;  // (a tile's offsets in 32 bits)
 }
 
