@@ -207,6 +207,36 @@ def test_norm_of_zero_and_tiny_and_huge_rows():
     assert np.isnan(z).all()
 
 
+# rows whose r, r^3 or sums leave fp32's range while their norm and its gradients stay inside
+FAR_ROWS = [1e-42, 1e-38, 1e-30, 1e-20, 1e-12, 1.0, 1e12, 1e18, 1e20, 1e22, 1e30, 3e37]
+FAR_COLS = [1, 40, 300, 1000, 1500, 4000, 8000, 16384, 20000]
+
+
+def far_case(cols):
+    """A row of each size and a constant one beside it, small rows' gradients small enough for theirs."""
+    size = np.repeat(np.asarray(FAR_ROWS), 2)[:, None]
+    h = normal((size.size, cols), 1).astype(np.float64)
+    h[1::2] = 1.0
+    go = normal((size.size, cols), 2) * np.sqrt(np.minimum(size, 1.0))
+    w = (1 + 0.2 * normal((cols,), 3)).astype(np.float32)
+    return (np.clip(h, -6, 6) * size).astype(np.float32), w, go.astype(np.float32)
+
+
+@pytest.mark.parametrize("cols", FAR_COLS)
+def test_norm_gradients_of_tiny_and_huge_rows(cols):
+    h, w, go = far_case(cols)
+    X, W = tensor(h).with_requires_grad(), tensor(w).with_requires_grad()
+    X.rms_norm(W, 0.0).backward(tensor(go))
+    dh, dw = R.rms_norm_grads(h, w, go, 0.0)
+    s = 1 / np.sqrt((h.astype(np.float64) ** 2).mean(1, keepdims=True))
+    g = np.abs(go.astype(np.float64) * w)
+    back = np.abs(h) * s ** 3 * np.abs((go.astype(np.float64) * w * h).mean(1, keepdims=True))
+    assert_within(X.grad_by_value().data(), dh, 4 * R.U * (s * g + back) + 1e-40, "dx")
+    steps = 5 + (len(h) if cols > 16384 else 0)
+    assert_within(W.grad_by_value().data(), dw, steps * R.U * np.abs(go * h * s).sum(0) + 1e-40, "dweight")
+    T.clear_gradients()
+
+
 def test_norm_gradients_accumulate_and_pass_through_the_sum():
     x, r, w, h = norm_case(6, 96, True)
     X, Rs, W = (tensor(a).with_requires_grad() for a in (x, r, w))

@@ -8,7 +8,10 @@
 // A row is held in registers by W waves, four neighbouring columns a lane and
 // NV such quads, so memory is passed over once; sums are f64.  Backward needs
 // h^2's and g h's row sums only, and takes both in the same pass: nothing but h
-// is kept from the forward.
+// is kept from the forward.  r is held as a power of two and a factor near one
+// (row_scale): with u the power and f the factor, dh = u (f g - (u h) b) and
+// b = f^2 r mean(g h), whose parts are of g's size however long a row is, where
+// r and r^3 mean(g h) themselves leave fp32 long before dh does.
 //
 // Bound by memory from a few thousand rows on, by the launch below (us, 8192 x 4096
 // with the sum): forward 85 for 537 MB, packed 87 for 437 MB, backward 85 for 403 MB
@@ -64,6 +67,18 @@ __device__ __forceinline__ void row_sum(double (&s)[N], double *lds) {
 #pragma unroll
         for (int w = 0; w < W; ++w) s[n] += lds[n * W + w];
     }
+}
+
+// r = up * f with up a power of two (as fp32 has them) and f in [1, 2) where r is
+// one of fp32's range, within a few binades of it for what rows can give beyond.
+struct RowScale {
+    float up;
+    double f;
+};
+__device__ __forceinline__ RowScale row_scale(double r) {
+    const int e = min(max(static_cast<int>(__double_as_longlong(r) >> 52 & 0x7ff) - 1023, -126), 127);  // (inf, NaN: 127)
+    const double down = __longlong_as_double(static_cast<long long>(1023 - e) << 52);
+    return {__uint_as_float(static_cast<unsigned>(e + 127) << 23), r * down};
 }
 
 template <int W>
@@ -221,7 +236,9 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
         row_sum<W, 2>(s, lds + slot * 2 * W);
         const double cols = static_cast<double>(a.cols);
         const double r = 1.0 / sqrt(s[0] / cols + a.eps);
-        const float rf = static_cast<float>(r), back = static_cast<float>(r * r * r * (s[1] / cols));
+        const RowScale scale = row_scale(r);
+        const float up = scale.up, rf = static_cast<float>(scale.f);
+        const float back = static_cast<float>(scale.f * scale.f * (r * (s[1] / cols)));
         c0 = 0;
         do {
             if (LONG) {
@@ -234,12 +251,12 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
                 if (DH && c < n) {
                     float o[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = rf * (g[i][e] * w[i][e]) - h[i][e] * back;
+                    for (int e = 0; e < 4; ++e) o[e] = up * (rf * (g[i][e] * w[i][e]) - up * h[i][e] * back);
                     store4(a.dh + base, c, a.cols, o);
                 }
                 if (DW && !LONG && live) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dw(i, e) += static_cast<double>(g[i][e]) * (h[i][e] * rf);
+                    for (int e = 0; e < 4; ++e) dw(i, e) += static_cast<double>(g[i][e]) * (up * h[i][e] * rf);
                 }
                 if (DW && LONG && c < n) {  // (one row at a time: the workgroup's own line)
                     float o[4];
@@ -247,7 +264,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
                     for (int e = 0; e < 4; ++e) o[e] = 0.0f;
                     if (!first) load4(part, c, a.cols, o);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] += g[i][e] * (h[i][e] * rf);
+                    for (int e = 0; e < 4; ++e) o[e] += g[i][e] * (up * h[i][e] * rf);
                     store4(part, c, a.cols, o);
                 }
             }
