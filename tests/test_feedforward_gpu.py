@@ -223,6 +223,17 @@ def far_case(cols):
 
 
 @pytest.mark.parametrize("cols", FAR_COLS)
+def test_norm_of_tiny_and_huge_rows_without_eps(cols):
+    h, w, _ = far_case(cols)
+    h = np.r_[h, np.full((1, cols), 3.3e38, np.float32), np.full((1, cols), 1e-45, np.float32)]
+    want = R.rms_norm(h, w, 0.0)
+    assert_within(tensor(h).rms_norm(tensor(w), 0.0).data(), want, 4 * R.U * np.abs(want) + 1e-40, "y")
+    codes, scales = parts(tensor(h).rms_norm_packed(tensor(w), 0.0))
+    packed_want = R.pack8(want)
+    assert np.array_equal(scales, packed_want[1]) and np.array_equal(codes, packed_want[0])
+
+
+@pytest.mark.parametrize("cols", FAR_COLS)
 def test_norm_gradients_of_tiny_and_huge_rows(cols):
     h, w, go = far_case(cols)
     X, W = tensor(h).with_requires_grad(), tensor(w).with_requires_grad()

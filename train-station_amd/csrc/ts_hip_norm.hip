@@ -137,7 +137,8 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_rows(NormArgs a) {
         } while (LONG && c0 < a.cols);
         row_sum<W, 1>(s, lds + slot * W);
         const double r = 1.0 / sqrt(s[0] / static_cast<double>(a.cols) + a.eps);
-        const float rf = static_cast<float>(r);
+        const RowScale scale = row_scale(r);
+        const float up = scale.up, rf = static_cast<float>(scale.f);
         c0 = 0;
         do {
             if (LONG) {
@@ -157,7 +158,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_rows(NormArgs a) {
                     pack_store(o, c, a.codes + row * a.pitch, a.scales + 4 * row, 4 * a.rows);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = v[i][e] * rf * w[i][e];
+                    for (int e = 0; e < 4; ++e) o[e] = up * v[i][e] * rf * w[i][e];
                     store4(a.y + base, c, a.cols, o);
                 }
             }
