@@ -9,7 +9,7 @@ import pytest
 
 import feedforward_ref as R
 import train_station_amd as T
-from train_station_amd._ffi import LinearShape, hip
+from train_station_amd._ffi import LinearShape, gradtrack, hip, last_error
 
 EINVAL, EWORKSPACE = 100001, 100003
 
@@ -145,6 +145,30 @@ def test_device_arrays_are_checked():
                        (Array(typestr="|u1", shape=(128,)), scales, 100), (Array(), scales, 100)):
         with pytest.raises(T.TsError):
             T.Packed8.from_device(c, s, cols)
+
+
+@pytest.mark.parametrize("shape", [(1 << 62,), (1 << 32, 1 << 32), (1 << 31, 1 << 31, 4), (3, (1 << 62) + 1), (1 << 64,), (-1,),
+                                   (1 << 40, 1 << 40, 1 << 40)])
+def test_shapes_whose_size_wraps_are_refused(shape):
+    with pytest.raises(T.TsError, match="larger than any memory|no shape"):
+        T.Tensor.from_device(Array(shape=shape))
+    dims = (ctypes.c_size_t * len(shape))(*shape)
+    if all(0 <= d < 1 << 64 for d in shape):
+        released = []
+        release = ctypes.CFUNCTYPE(None, ctypes.c_void_p)(released.append)
+        assert not gradtrack.ts_tensor_from_device(P, dims, len(shape), release, 7) and released == [7]
+
+
+def test_empty_shapes_of_long_sides_are_empty():
+    t = T.Tensor.from_device(Array(shape=(1 << 62, 0, 1 << 62), data=(0, False)))
+    assert t.size() == 0
+
+
+@pytest.mark.parametrize("rows,cols", [(1 << 57, 128), (1 << 56, 256), (1, (1 << 64) - 1), (1, (1 << 64) - 127), (3, 1 << 63),
+                                       ((1 << 57) + 1, 128)])
+def test_packed_sizes_that_wrap_are_refused(rows, cols):
+    assert not gradtrack.ts_packed8_from_device(P, P, rows, cols, None, None)
+    assert "larger than any memory" in last_error()
 
 
 def test_names_are_checked():

@@ -265,8 +265,11 @@ Packed8 Packed8::from_device(uint8_t *codes, uint8_t *scales, size_t rows, size_
         if (release) release();
         return p;
     }
+    const size_t pitch = p.pitch();
+    if (pitch < cols || rows > SIZE_MAX / pitch)
+        throw Error("Packed8: [" + std::to_string(rows) + ", " + std::to_string(cols) + "] is larger than any memory");
     Runtime::get();
-    const size_t nc = rows * p.pitch(), ns = nc / 32;
+    const size_t nc = rows * pitch, ns = nc / 32;
     if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 4)
         throw Error("Packed8: codes must be 16-byte aligned and scales 4-byte aligned");
     if (!codes || !scales || ts_hip_check_device_range(codes, nc) != TS_HIP_OK ||

@@ -47,6 +47,19 @@ size_t product(const std::vector<size_t> &d) {
     return n;
 }
 
+// the number of values, refused where their bytes have no size_t
+size_t checked_product(const std::vector<size_t> &d, const char *what) {
+    size_t n = 1;
+    bool fits = true;
+    for (size_t x : d) {
+        if (x == 0) return 0;
+        fits = fits && n <= SIZE_MAX / sizeof(float) / x;
+        n *= x;
+    }
+    if (!fits) throw Error(std::string(what) + ": " + dims_str(d) + " is larger than any memory");
+    return n;
+}
+
 // Reference AVX2 body/tail split: 8-wide for negate and Adam
 // (core/utils.rs:856-865, adam/mod.rs:727-773), 32-wide unrolled body for the
 // division zero check (ops/div.rs:356-417).
@@ -1143,7 +1156,7 @@ Tensor Tensor::from_slice(const float *data, size_t len, std::vector<size_t> dim
 
 Tensor Tensor::from_device(float *data, std::vector<size_t> dims, std::function<void()> release) {
     Tensor t;
-    t.size_ = product(dims);
+    t.size_ = checked_product(dims, "from_device");
     t.dims_ = std::move(dims);
     t.id_ = next_tensor_id();
     if (t.size_ == 0) {

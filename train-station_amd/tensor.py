@@ -80,6 +80,8 @@ def _device_array(obj, typestr: str):
     except (AttributeError, TypeError) as e:
         raise TsError(f"from_device: {type(obj).__name__} exposes no device memory") from e
     shape = tuple(int(d) for d in a["shape"])
+    if any(d < 0 or d >= 1 << 63 for d in shape):
+        raise TsError(f"from_device: {list(shape)} is no shape")
     if a["typestr"] != typestr:
         raise TsError(f"from_device: values of type {a['typestr']}, not {typestr}")
     strides, step = a.get("strides"), int(typestr[2:])
