@@ -159,6 +159,16 @@ def test_shapes_whose_size_wraps_are_refused(shape):
         assert not gradtrack.ts_tensor_from_device(P, dims, len(shape), release, 7) and released == [7]
 
 
+def test_arrays_that_may_not_be_written_are_refused():
+    with pytest.raises(T.TsError, match="read-only"):
+        T.Tensor.from_device(Array(shape=(0, 3), data=(P, True)))
+    with pytest.raises(T.TsError, match="masked"):
+        T.Tensor.from_device(Array(shape=(0, 3), mask=object()))
+    # codes and scales are read only
+    codes, scales = Array(typestr="|u1", shape=(0, 128), data=(P, True)), Array(typestr="|u1", shape=(1, 0, 4), data=(P, True))
+    assert T.Packed8.from_device(codes, scales, 100).shape == (0, 100)
+
+
 def test_empty_shapes_of_long_sides_are_empty():
     t = T.Tensor.from_device(Array(shape=(1 << 62, 0, 1 << 62), data=(0, False)))
     assert t.size() == 0

@@ -73,8 +73,9 @@ def _lend(owners) -> int:
     return token
 
 
-def _device_array(obj, typestr: str):
-    """(address, shape) of an object that exposes contiguous device memory."""
+def _device_array(obj, typestr: str, written: bool):
+    """(address, shape) of an object that exposes contiguous device memory
+    (written: that the library may write to)."""
     try:
         a = obj.__cuda_array_interface__
     except (AttributeError, TypeError) as e:
@@ -84,6 +85,10 @@ def _device_array(obj, typestr: str):
         raise TsError(f"from_device: {list(shape)} is no shape")
     if a["typestr"] != typestr:
         raise TsError(f"from_device: values of type {a['typestr']}, not {typestr}")
+    if a.get("mask") is not None:
+        raise TsError("from_device: the array is masked")
+    if written and a["data"][1]:
+        raise TsError("from_device: the array is read-only")
     strides, step = a.get("strides"), int(typestr[2:])
     if strides is not None and 0 not in shape:
         for d, s in zip(reversed(shape), reversed(strides)):
@@ -144,12 +149,12 @@ class Tensor:
 
     @staticmethod
     def from_device(array) -> "Tensor":
-        """A tensor over the memory of a contiguous float32 device array (any
+        """A tensor over the memory of a contiguous, writable float32 device array (any
         object with ``__cuda_array_interface__``), not copied; the array is held
         until the library's last use of it.  What wrote it must have finished,
         and others may read what the library writes to it only after
         ``synchronize()`` (or an event on ``stream()``)."""
-        ptr, shape = _device_array(array, "<f4")
+        ptr, shape = _device_array(array, "<f4", True)
         d, r = _dims(shape)
         return _wrap(_G.ts_tensor_from_device(ptr, d, r, _give_back, _lend(array)))
 
@@ -432,7 +437,7 @@ class Packed8:
     def from_device(codes, scales, cols: int) -> "Packed8":
         """Over a caller's uint8 device arrays, codes [rows, pitch] and scales
         [pitch / 128, rows, 4], as Tensor.from_device."""
-        (cp, cshape), (sp, sshape) = _device_array(codes, "|u1"), _device_array(scales, "|u1")
+        (cp, cshape), (sp, sshape) = _device_array(codes, "|u1", False), _device_array(scales, "|u1", False)
         pitch = -(-int(cols) // 128) * 128
         if cols < 0 or len(cshape) != 2 or cshape[1] != pitch or sshape != (pitch // 128, cshape[0], 4):
             raise TsError(f"Packed8: codes {list(cshape)} and scales {list(sshape)} for {cols} columns")
