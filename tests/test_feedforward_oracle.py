@@ -159,6 +159,16 @@ def test_shapes_whose_size_wraps_are_refused(shape):
         assert not gradtrack.ts_tensor_from_device(P, dims, len(shape), release, 7) and released == [7]
 
 
+def test_an_array_that_will_not_be_shared_is_an_error_of_the_library():
+    class Kept:  # as torch's tensors that require grad
+        @property
+        def __cuda_array_interface__(self):
+            raise RuntimeError("use detach()")
+
+    with pytest.raises(T.TsError, match=r"exposes no device memory: use detach\(\)"):
+        T.Tensor.from_device(Kept())
+
+
 def test_arrays_that_may_not_be_written_are_refused():
     with pytest.raises(T.TsError, match="read-only"):
         T.Tensor.from_device(Array(shape=(0, 3), data=(P, True)))

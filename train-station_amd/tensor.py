@@ -78,8 +78,8 @@ def _device_array(obj, typestr: str, written: bool):
     (written: that the library may write to)."""
     try:
         a = obj.__cuda_array_interface__
-    except (AttributeError, TypeError) as e:
-        raise TsError(f"from_device: {type(obj).__name__} exposes no device memory") from e
+    except (AttributeError, TypeError, RuntimeError) as e:  # (RuntimeError: torch's, of a tensor that requires grad)
+        raise TsError(f"from_device: {type(obj).__name__} exposes no device memory: {e}") from e
     shape = tuple(int(d) for d in a["shape"])
     if any(d < 0 or d >= 1 << 63 for d in shape):
         raise TsError(f"from_device: {list(shape)} is no shape")
