@@ -40,8 +40,8 @@ ts_tensor *ts_tensor_from_slice(const float *data, size_t len, const size_t *dim
  * then has run; also at once when this call fails or the tensor is empty.
  * Work on other streams that writes the memory must have finished before the
  * library reads it, and the library's work before others read what it wrote
- * (ts_synchronize, or an event on ts_stream).  Memory that is not device
- * memory of one allocation is refused. */
+ * (ts_synchronize, or an event on ts_stream).  Memory that is not one
+ * allocation's on the current device is refused. */
 ts_tensor *ts_tensor_from_device(float *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx);
 /* The process is ending: from here on no release call is made. */
 void ts_external_detach(void);

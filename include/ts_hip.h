@@ -112,7 +112,7 @@ int ts_hip_graph_launch(void *graph_exec, void *stream);
 int ts_hip_graph_destroy(void *graph_exec);
 /* message for a status returned by any ts_hip_* call */
 const char *ts_hip_error_string(int status);
-/* TS_HIP_OK when [ptr, ptr + bytes) is device memory of one allocation, else TS_HIP_EINVAL */
+/* TS_HIP_OK when [ptr, ptr + bytes) is memory of one allocation on the current device, else TS_HIP_EINVAL */
 int ts_hip_check_device_range(const void *ptr, size_t bytes);
 /* free / total device memory in bytes */
 int ts_hip_mem_info(size_t *free_bytes, size_t *total_bytes);

@@ -659,6 +659,24 @@ def test_device_memory_is_used_in_place_and_given_back():
     assert len(module._lent) == held - 1
 
 
+def test_memory_of_another_device_is_refused():
+    import ctypes
+
+    count = ctypes.c_int()
+    hip_check(hip.ts_hip_get_device_count(ctypes.byref(count)), "ts_hip_get_device_count")
+    a = DeviceArray(normal((8, 16), 1))
+    assert hip.ts_hip_check_device_range(a.dev.ptr, a.host.nbytes) == 0
+    if count.value < 2:
+        pytest.skip("one device")
+    hip_check(hip.ts_hip_set_device(1), "ts_hip_set_device")
+    try:
+        assert hip.ts_hip_check_device_range(a.dev.ptr, a.host.nbytes) != 0
+        with pytest.raises(T.TsError, match="device memory"):
+            T.Tensor.from_device(a)
+    finally:
+        hip_check(hip.ts_hip_set_device(0), "ts_hip_set_device")
+
+
 def block_parameters(d=48, f=80, seed=0):
     return [tensor(a).with_requires_grad() for a in (np.ones(d, np.float32), normal((d, f), seed + 1, d ** -0.5),
                                                      np.zeros(f, np.float32), normal((f, d), seed + 2, f ** -0.5),

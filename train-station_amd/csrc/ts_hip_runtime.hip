@@ -308,6 +308,11 @@ int ts_hip_check_device_range(const void *ptr, size_t bytes) {
         (void)hipGetLastError();  // a host pointer is not an error of a later call
         return TS_HIP_EINVAL;
     }
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess || at.device != device) {
+        (void)hipGetLastError();
+        return TS_HIP_EINVAL;
+    }
     hipDeviceptr_t base = nullptr;
     size_t size = 0;
     if (hipMemGetAddressRange(&base, &size, const_cast<void *>(ptr)) != hipSuccess) {
