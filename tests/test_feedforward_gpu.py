@@ -458,6 +458,18 @@ def test_linear_gradient_is_the_difference(checkpoint):
     T.clear_gradients()
 
 
+@pytest.mark.parametrize("batch,fan_in,fan_out", [(1 << 21, 1, 3), (1000003, 2, 17)])
+def test_bias_gradients_of_many_rows_are_summed_in_64_bits(batch, fan_in, fan_out):
+    go = np.abs(normal((batch, fan_out), 1))
+    B = tensor(np.zeros(fan_out, np.float32)).with_requires_grad()
+    X, W = T.Tensor.zeros((batch, fan_in)), T.Tensor.zeros((fan_in, fan_out))
+    X.linear(W, bias=B).backward(tensor(go))
+    want = go.astype(np.float64).sum(0)
+    # a rounding of each part, and one of their sum
+    assert_within(B.grad_by_value().data(), want, 2.01 * R.U * want, "dbias")
+    T.clear_gradients()
+
+
 def test_linear_grads_for_some_inputs_only():
     x, w, b, r, go = layer_case(12, 20, 9, True, True)
     for need in range(16):

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kDirectThreads) void linear_direct_back(DirectProdu
     else sum_job(sum, b - dw.blocks - dx.blocks, reinterpret_cast<double *>(direct_lds));
 }
 
-// The slices' sums added in their order, with the products' epilogues.
+// The slices' sums added in their order, with the products' epilogues; dz's column sums in f64, as each slice took its own.
 __global__ __launch_bounds__(kBlock) void linear_join(DirectProduct p, DirectProduct q, SumJob sum) {
     const size_t np = p.slices > 1 ? static_cast<size_t>(p.M) * p.N : 0;
     const size_t nq = q.slices > 1 ? static_cast<size_t>(q.M) * q.N : 0;
@@ -92,7 +92,13 @@ __global__ __launch_bounds__(kBlock) void linear_join(DirectProduct p, DirectPro
         else if (n < np + nq)
             epilogue_store(q.epi, q.C, n - np, total(q.part, n - np, nq, q.slices),
                            q.epi.bias ? q.epi.bias[(n - np) % q.N] : 0.0f);
-        else sum.out[n - np - nq] = total(sum.part, n - np - nq, sum.cols, sum.slices);
+        else {
+            const size_t at = n - np - nq;
+            double v = 0.0;
+#pragma unroll 4
+            for (int s = 0; s < sum.slices; ++s) v += sum.part[s * static_cast<size_t>(sum.cols) + at];
+            sum.out[at] = static_cast<float>(v);
+        }
     }
 }
 
