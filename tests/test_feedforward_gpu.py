@@ -147,6 +147,38 @@ def test_rms_norm_sums_many_rows(rows, cols):
     test_rms_norm(rows, cols, True)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 16385), (3, 40001), (300, 16390), (700, 20003)])
+@pytest.mark.parametrize("need", ["both", "weight", "x"])
+def test_long_rows_weight_gradients_are_summed_in_64_bits(rows, cols, need):
+    x, _, w, h = norm_case(rows, cols, False)
+    go = np.abs(normal((rows, cols), 4)) * np.sign(x)  # every term of a sum of one sign
+    X, W = tensor(x), tensor(w)
+    for t in (X, W) if need == "both" else (W,) if need == "weight" else (X,):
+        t.with_requires_grad()
+    X.rms_norm(W, 1e-6).backward(tensor(go))
+    dh, dw = R.rms_norm_grads(h, w, go, 1e-6)
+    s = 1 / np.sqrt((h.astype(np.float64) ** 2).mean(1, keepdims=True) + 1e-6)
+    if need != "x":
+        assert_within(W.grad_by_value().data(), dw, 5 * R.U * np.abs(go * h * s).sum(0) + 1e-40, "dweight")
+    if need != "weight":
+        g = np.abs(go.astype(np.float64) * w)
+        back = np.abs(h) * s ** 3 * np.abs((go.astype(np.float64) * w * h).mean(1, keepdims=True))
+        assert_within(X.grad_by_value().data(), dh, 4 * R.U * (s * g + back) + 1e-40, "dx")
+    T.clear_gradients()
+
+
+def test_long_rows_weight_gradients_keep_what_fp32_sums_lose():
+    rows, cols = 40 * 256 + 1, 16388
+    go = np.zeros((rows, cols), np.float32)
+    go[::256] = 0.9 * 2.0 ** -25  # of rows that one workgroup of 256 takes in turn; beside 1, nothing in fp32
+    go[0] = 1.0
+    W = tensor(np.ones(cols, np.float32)).with_requires_grad()
+    T.Tensor.ones((rows, cols)).rms_norm(W, 0.0).backward(tensor(go))
+    want = go[::256].astype(np.float64).sum(0)
+    assert_within(W.grad_by_value().data(), want, 5 * R.U * want, "dweight")
+    T.clear_gradients()
+
+
 @pytest.mark.parametrize("rows,cols", NORMS)
 @pytest.mark.parametrize("residual", [False, True])
 def test_rms_norm_packed(rows, cols, residual):

@@ -170,6 +170,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_rows(NormArgs a) {
 struct NormBackArgs {
     const float *h, *weight, *go;
     float *dh, *dw_part;  // dw_part: [gridDim.x][cols]
+    float *scales;        // LONG with dw_part: each row's up, f and back
     size_t rows, cols;
     double eps;
     float *dw;         // with a ticket: the last workgroup adds the parts up
@@ -177,7 +178,8 @@ struct NormBackArgs {
 };
 
 // Rows blockIdx.x * RPB + slot, and on by the grid's; a thread keeps dw's sums
-// of its columns (f64), the workgroup's go to dw_part.
+// of its columns (f64), the workgroup's go to dw_part.  LONG with dw: no thread has
+// columns of its own; the rows' scales are left for long_columns.
 template <int W, int NV, bool DH, bool DW, bool LONG>
 __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a) {
     constexpr int RPB = kNormRows<W>;
@@ -205,7 +207,6 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
     };
     if (!LONG) weights(0);
     float *part = DW ? a.dw_part + static_cast<size_t>(blockIdx.x) * a.cols : nullptr;
-    bool first = true;
     const size_t step = static_cast<size_t>(gridDim.x) * RPB;
     // every wave of the workgroup takes every round (the barriers)
     for (size_t r0 = static_cast<size_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += step) {
@@ -240,6 +241,14 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
         const RowScale scale = row_scale(r);
         const float up = scale.up, rf = static_cast<float>(scale.f);
         const float back = static_cast<float>(scale.f * scale.f * (r * (s[1] / cols)));
+        if (DW && LONG) {
+            if (t == 0) {
+                a.scales[3 * row] = up;
+                a.scales[3 * row + 1] = rf;
+                a.scales[3 * row + 2] = back;
+            }
+            continue;
+        }
         c0 = 0;
         do {
             if (LONG) {
@@ -259,19 +268,9 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dw(i, e) += static_cast<double>(g[i][e]) * (up * h[i][e] * rf);
                 }
-                if (DW && LONG && c < n) {  // (one row at a time: the workgroup's own line)
-                    float o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = 0.0f;
-                    if (!first) load4(part, c, a.cols, o);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] += g[i][e] * (up * h[i][e] * rf);
-                    store4(part, c, a.cols, o);
-                }
             }
             c0 += span;
         } while (LONG && c0 < a.cols);
-        first = false;
     }
     if (DW && !LONG) {
         if constexpr (RPB > 1) {  // the workgroup's rows together, in their order
@@ -320,6 +319,41 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_back(NormBackArgs a)
         }
         if (threadIdx.x == 0) *a.ticket = 0;
     }
+}
+
+// dw, and dh, of rows longer than a workgroup holds, by columns: a thread has four of
+// them, of `run` rows (dw: f64).  Rows are read twice either way: the first pass by rows
+// takes their sums alone.  Forward and backward, us: 2048 x 20000 277, 512 x 65536 197
+// (dh by rows, and dw row by row on a line of each workgroup's in fp32: 293, 242).
+constexpr size_t kLongCols = 4 * kBlock;  // of a workgroup
+template <bool DH>
+__global__ __launch_bounds__(kBlock) void long_columns(NormBackArgs a, size_t run) {
+    const size_t c = blockIdx.x * kLongCols + 4 * threadIdx.x, first = blockIdx.y * run;
+    if (c >= a.cols) return;
+    const size_t last = first + run < a.rows ? first + run : a.rows;
+    float w[4];
+    if (DH) load4(a.weight, c, a.cols, w);
+    double s[4] = {};
+#pragma unroll 4
+    for (size_t row = first; row < last; ++row) {
+        const float up = a.scales[3 * row], rf = a.scales[3 * row + 1], back = a.scales[3 * row + 2];
+        const size_t base = row * a.cols;
+        float h[4], g[4];
+        load4(a.h + base, c, a.cols, h);
+        load4(a.go + base, c, a.cols, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += static_cast<double>(g[e]) * (up * h[e] * rf);
+        if (DH) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = up * (rf * (g[e] * w[e]) - up * h[e] * back);
+            store4(a.dh + base, c, a.cols, o);
+        }
+    }
+    float o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(s[e]);
+    store4(a.dw_part + blockIdx.y * a.cols, c, a.cols, o);
 }
 
 __global__ __launch_bounds__(kBlock) void sum_parts(PartSums p) {
@@ -409,6 +443,14 @@ size_t back_blocks(size_t rows, size_t cols) {
     return need < cap ? need : cap;
 }
 
+// Rows of a part of long_columns: as many as leave eight workgroups a CU, in no more parts than back_blocks
+size_t long_run(size_t rows, size_t cols) {
+    const size_t wide = (cols + kLongCols - 1) / kLongCols, most = back_blocks(rows, cols);
+    const size_t want = (static_cast<size_t>(device_cu_count()) * 8 + wide - 1) / wide;
+    const size_t parts = want < most ? want : most;
+    return (rows + parts - 1) / parts;
+}
+
 constexpr size_t kMaxRows = size_t(1) << 31;
 // Parts that one workgroup adds up sooner than another launch has started: 128 x 784
 // (32 parts) forward and backward 26.8 us by two launches, 24.5 by one; 16384 x 64
@@ -465,7 +507,9 @@ int ts_hip_rms_norm_packed(const float *x, const float *residual, const float *w
     return norm_forward(x, residual, weight, rows, cols, eps, h, nullptr, codes, scales, stream);
 }
 
-size_t ts_hip_rms_norm_backward_workspace_floats(size_t rows, size_t cols) { return back_blocks(rows, cols) * cols; }
+size_t ts_hip_rms_norm_backward_workspace_floats(size_t rows, size_t cols) {
+    return back_blocks(rows, cols) * cols + (cols > kMaxHeldCols ? 3 * rows : 0);
+}
 
 int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
                              float *dh, float *dweight, float *workspace, size_t workspace_floats, unsigned *ticket,
@@ -476,15 +520,23 @@ int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *g
     if (dweight && (!workspace || workspace_floats < ts_hip_rms_norm_backward_workspace_floats(rows, cols)))
         return TS_HIP_EWORKSPACE;
     const unsigned grid = static_cast<unsigned>(back_blocks(rows, cols));
-    if (!dweight || grid > kTicketParts || grid * cols > kTicketFloats) ticket = nullptr;
-    const NormBackArgs a = {h, weight, go, dh, dweight ? workspace : nullptr, rows, cols, eps, dweight, ticket};
+    const bool long_rows = cols > kMaxHeldCols;
+    if (!dweight || long_rows || grid > kTicketParts || grid * cols > kTicketFloats) ticket = nullptr;
+    float *const parts = dweight ? workspace : nullptr, *const scales = parts ? parts + grid * cols : nullptr;
+    const NormBackArgs a = {h, weight, go, dh, parts, scales, rows, cols, eps, dweight, ticket};
     const hipStream_t s = as_stream(stream);
-    for_cols(cols, false, [&](auto w, auto nv, auto long_rows) {
-        launch_back<w.value, nv.value, long_rows.value>(a, grid, s);
-    });
+    for_cols(cols, false, [&](auto w, auto nv, auto lng) { launch_back<w.value, nv.value, lng.value>(a, grid, s); });
+    size_t count = grid;
+    if (dweight && long_rows) {
+        const size_t run = long_run(rows, cols);
+        count = (rows + run - 1) / run;
+        const dim3 columns(static_cast<unsigned>((cols + kLongCols - 1) / kLongCols), static_cast<unsigned>(count));
+        if (dh) launch(long_columns<true>, columns, dim3(kBlock), 0, s, a, run);
+        else launch(long_columns<false>, columns, dim3(kBlock), 0, s, a, run);
+    }
     if (dweight && !ticket)
         launch(sum_parts, dim3(static_cast<unsigned>((cols + 15) / 16)), dim3(kBlock), 0, s,
-               part_sums(workspace, grid, cols, dweight));
+               part_sums(parts, count, cols, dweight));
     return launch_status();
 }
 
