@@ -502,6 +502,29 @@ def test_bias_gradients_of_many_rows_are_summed_in_64_bits(batch, fan_in, fan_ou
     T.clear_gradients()
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 8, 8), (33, 65, 31), (9000, 20, 30), (1000, 777, 1531), (64, 4096, 2052), (3, 5003, 40)])
+@pytest.mark.parametrize("checkpoint", ["full", "8bit"])
+def test_relu_passes_nothing_on_where_it_is_zero(m, k, n, checkpoint):
+    """Infinities and NaN of the output's gradient at places that relu holds back, as for Tensor.relu."""
+    x, w, b, _, go = layer_case(m, k, n, True, False)
+    kept = x if checkpoint == "full" else R.unpack8(*R.pack8(x), k)
+    z = R.linear(kept, w, b, "none", None)[0]
+    safe = R.relu_safe(x, w, b, kept)
+    go = np.where(safe, go, 0).astype(np.float32)
+    off = safe & (z < 0)
+    sent = go.copy()
+    sent[off] = np.resize(np.float32([np.inf, -np.inf, np.nan, 1.0]), off.sum())
+    assert not np.isfinite(sent).all()
+    X, W, B = (tensor(a).with_requires_grad() for a in (x, w, b))
+    X.linear(W, bias=B, activation="relu", checkpoint=checkpoint).backward(tensor(sent))
+    dx, dw, db = R.linear_grads(kept, w, z, "relu", go)
+    ex, ew, eb = R.linear_grads_bound(kept, w, b, z, "relu", np.where(off, 0, go))
+    assert_within(X.grad_by_value().data(), dx, ex, "dx")
+    assert_within(W.grad_by_value().data(), dw, ew, "dweight")
+    assert_within(B.grad_by_value().data(), db, eb, "dbias")
+    T.clear_gradients()
+
+
 def test_linear_grads_for_some_inputs_only():
     x, w, b, r, go = layer_case(12, 20, 9, True, True)
     for need in range(16):

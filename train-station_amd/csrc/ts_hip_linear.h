@@ -45,6 +45,12 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
     return z * s;
 }
 
+// dz = go act'(z); relu's gradient is go's where it passes it on and zero elsewhere, whatever go is there
+__device__ __forceinline__ float through_slope(float go, float slope, bool relu) {
+    const float v = go * slope;
+    return relu && slope == 0.0f ? 0.0f : v;
+}
+
 // ---- epilogues -------------------------------------------------------------------
 
 // Of a product P [M, N] stored with ldc = N:
@@ -63,7 +69,7 @@ __device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, siz
     float slope;
     if (e.go) {
         activate<true>(v, e.act, slope);
-        c[at] = extra * slope;
+        c[at] = through_slope(extra, slope, e.act == TS_HIP_ACT_RELU);
         return;
     }
     if (e.slope) {
@@ -83,8 +89,8 @@ __device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, siz
 // ---- operands --------------------------------------------------------------------
 
 // An operand's rows (its index in the product that is not k) and k: floats with
-// k or the row contiguous (times, where set, what stands at the same place of
-// `times`: go and a layer's slopes), or codes [rows][pitch] with k or the row
+// k or the row contiguous (through what stands at the same place of `times`,
+// where set: go and a layer's slopes, relu's or others), or codes [rows][pitch] with k or the row
 // along the code rows.
 enum class Src { kFloatK, kFloatR, kCodesK, kCodesR };
 
@@ -93,15 +99,16 @@ struct Operand {
     const uint8_t *codes, *scales;
     int ld;         // floats: the leading dimension
     int rows;       // the product's rows
-    size_t pitch;   // codes
-    size_t code_rows;
+    unsigned pitch;  // codes
+    bool relu;       // times: relu's slopes
+    size_t code_rows;  // codes
 };
 
 template <Src S>
 __device__ __forceinline__ float operand_at(const Operand &o, int row, int k) {
     if constexpr (S == Src::kFloatK || S == Src::kFloatR) {
         const size_t at = S == Src::kFloatK ? static_cast<size_t>(row) * o.ld + k : static_cast<size_t>(k) * o.ld + row;
-        return o.times ? o.p[at] * o.times[at] : o.p[at];
+        return o.times ? through_slope(o.p[at], o.times[at], o.relu) : o.p[at];
     } else {
         const size_t r = S == Src::kCodesK ? row : k, c = S == Src::kCodesK ? k : row;
         const int s = o.scales[(c / kPackGroup * o.code_rows + r) * 4 + c / kPackBlock % 4];
@@ -120,10 +127,14 @@ __device__ __forceinline__ void operand_pair(const Operand &o, int row, int k, i
             const int r = min(row + x, o.rows - 1);
             const size_t at = static_cast<size_t>(r) * o.ld + k;
             if (k + 4 <= K) {
-                pk4u_t q = *reinterpret_cast<const pk4u_t *>(o.p + at);
-                if (o.times) q *= *reinterpret_cast<const pk4u_t *>(o.times + at);  // uniform
+                const pk4u_t q = *reinterpret_cast<const pk4u_t *>(o.p + at);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) v[x][c] = q[c];
+                if (o.times) {  // uniform
+                    const pk4u_t t = *reinterpret_cast<const pk4u_t *>(o.times + at);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[x][c] = through_slope(q[c], t[c], o.relu);
+                }
             } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) v[x][c] = k + c < K ? operand_at<S>(o, r, k + c) : 0.0f;
@@ -139,7 +150,10 @@ __device__ __forceinline__ void operand_pair(const Operand &o, int row, int k, i
                 const size_t at = static_cast<size_t>(k + c) * o.ld + r;
                 if (two) {
                     q = *reinterpret_cast<const pk2u_t *>(o.p + at);
-                    if (o.times) q *= *reinterpret_cast<const pk2u_t *>(o.times + at);
+                    if (o.times) {
+                        const pk2u_t t = *reinterpret_cast<const pk2u_t *>(o.times + at);
+                        q = pk2u_t{through_slope(q[0], t[0], o.relu), through_slope(q[1], t[1], o.relu)};
+                    }
                 } else {
                     q[0] = operand_at<S>(o, r, k + c);
                 }
