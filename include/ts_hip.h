@@ -640,7 +640,7 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
 
 /* A layer's forward: z = x W + bias, y = act(z) + residual, x [batch, fan_in],
  * W [fan_in, fan_out]; bias and residual may be NULL.  slope != NULL: act'(z) is
- * stored there, laid out as y (what the backward pass reads).  codes != NULL: x is also
+ * stored there, laid out as y (what the backward pass reads; relu's 0 as -0).  codes != NULL: x is also
  * packed into codes / scales (ts_hip_pack8). */
 typedef struct ts_hip_linear_shape {
     size_t batch, fan_in, fan_out;
@@ -654,8 +654,8 @@ int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float 
  * each of dx, dweight and dbias NULL where it is not wanted.  X is x, or what
  * codes / scales hold where codes != NULL (x is then not read); slope is the
  * forward's (needed with x and an activation), or NULL: with codes the slopes
- * are computed again from what they hold, at z = X W + bias.  relu's slope at 0 is 0,
- * and where it is 0 dz is, whatever go (as ts_hip_relu_backward). */
+ * are computed again from what they hold, at z = X W + bias.  relu's slope at 0 is 0.
+ * Where a slope is -0 dz is 0, whatever go (as ts_hip_relu_backward). */
 size_t ts_hip_linear_backward_workspace_floats(const ts_hip_linear_shape *shape);
 int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, const uint8_t *codes,
                            const uint8_t *scales, const float *weight, const float *bias, int act, const float *slope,

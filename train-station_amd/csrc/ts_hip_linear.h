@@ -21,7 +21,7 @@ __device__ __forceinline__ float exp_neg_abs(float v) {
 constexpr float kGelu1 = 1.59576912f;  // 2 sqrt(2 / pi)
 constexpr float kGelu2 = 0.044715f;
 
-// act(z) and, where SLOPE, act'(z)
+// act(z) and, where SLOPE, act'(z); relu's zero is -0, which the other two do not give (s + d, s >= 0)
 template <bool SLOPE>
 __device__ __forceinline__ float activate(float z, int act, float &slope) {
     if (act == TS_HIP_ACT_NONE) {
@@ -29,7 +29,7 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
         return z;
     }
     if (act == TS_HIP_ACT_RELU) {
-        slope = z > 0.0f ? 1.0f : 0.0f;
+        slope = z > 0.0f ? 1.0f : -0.0f;
         return z > 0.0f ? z : 0.0f;
     }
     const bool silu = act == TS_HIP_ACT_SILU;
@@ -45,10 +45,9 @@ __device__ __forceinline__ float activate(float z, int act, float &slope) {
     return z * s;
 }
 
-// dz = go act'(z); relu's gradient is go's where it passes it on and zero elsewhere, whatever go is there
-__device__ __forceinline__ float through_slope(float go, float slope, bool relu) {
-    const float v = go * slope;
-    return relu && slope == 0.0f ? 0.0f : v;
+// dz = go act'(z), but nothing where relu holds go back (a slope of -0), whatever go is
+__device__ __forceinline__ float through_slope(float go, float slope) {
+    return __float_as_uint(slope) == 0x80000000u ? 0.0f : go * slope;
 }
 
 // ---- epilogues -------------------------------------------------------------------
@@ -69,7 +68,7 @@ __device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, siz
     float slope;
     if (e.go) {
         activate<true>(v, e.act, slope);
-        c[at] = through_slope(extra, slope, e.act == TS_HIP_ACT_RELU);
+        c[at] = through_slope(extra, slope);
         return;
     }
     if (e.slope) {
@@ -90,7 +89,7 @@ __device__ __forceinline__ void epilogue_store(const LinearEpi &e, float *c, siz
 
 // An operand's rows (its index in the product that is not k) and k: floats with
 // k or the row contiguous (through what stands at the same place of `times`,
-// where set: go and a layer's slopes, relu's or others), or codes [rows][pitch] with k or the row
+// where set: go and a layer's slopes), or codes [rows][pitch] with k or the row
 // along the code rows.
 enum class Src { kFloatK, kFloatR, kCodesK, kCodesR };
 
@@ -99,16 +98,15 @@ struct Operand {
     const uint8_t *codes, *scales;
     int ld;         // floats: the leading dimension
     int rows;       // the product's rows
-    unsigned pitch;  // codes
-    bool relu;       // times: relu's slopes
-    size_t code_rows;  // codes
+    size_t pitch;   // codes
+    size_t code_rows;
 };
 
 template <Src S>
 __device__ __forceinline__ float operand_at(const Operand &o, int row, int k) {
     if constexpr (S == Src::kFloatK || S == Src::kFloatR) {
         const size_t at = S == Src::kFloatK ? static_cast<size_t>(row) * o.ld + k : static_cast<size_t>(k) * o.ld + row;
-        return o.times ? through_slope(o.p[at], o.times[at], o.relu) : o.p[at];
+        return o.times ? through_slope(o.p[at], o.times[at]) : o.p[at];
     } else {
         const size_t r = S == Src::kCodesK ? row : k, c = S == Src::kCodesK ? k : row;
         const int s = o.scales[(c / kPackGroup * o.code_rows + r) * 4 + c / kPackBlock % 4];
@@ -133,7 +131,7 @@ __device__ __forceinline__ void operand_pair(const Operand &o, int row, int k, i
                 if (o.times) {  // uniform
                     const pk4u_t t = *reinterpret_cast<const pk4u_t *>(o.times + at);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) v[x][c] = through_slope(q[c], t[c], o.relu);
+                    for (int c = 0; c < 4; ++c) v[x][c] = through_slope(q[c], t[c]);
                 }
             } else {
 #pragma unroll
@@ -152,7 +150,7 @@ __device__ __forceinline__ void operand_pair(const Operand &o, int row, int k, i
                     q = *reinterpret_cast<const pk2u_t *>(o.p + at);
                     if (o.times) {
                         const pk2u_t t = *reinterpret_cast<const pk2u_t *>(o.times + at);
-                        q = pk2u_t{through_slope(q[0], t[0], o.relu), through_slope(q[1], t[1], o.relu)};
+                        q = pk2u_t{through_slope(q[0], t[0]), through_slope(q[1], t[1])};
                     }
                 } else {
                     q[0] = operand_at<S>(o, r, k + c);

@@ -20,7 +20,6 @@ struct SumJob {
     const float *x, *times;
     float *out, *part;  // part: several slices, [slices][cols]
     int rows, cols, slices, slice_rows, blocks;
-    bool relu;
 };
 
 __device__ __forceinline__ void pack_job(const PackJob &j, int block) {
@@ -43,7 +42,7 @@ __device__ __forceinline__ void sum_job(const SumJob &j, int block, double *lds)
 #pragma unroll 8
         for (int r = from + q; r < to; r += lanes) {
             const size_t at = static_cast<size_t>(r) * j.cols + col;
-            s += j.times ? through_slope(j.x[at], j.times[at], j.relu) : j.x[at];
+            s += j.times ? through_slope(j.x[at], j.times[at]) : j.x[at];
         }
     }
     lds[q * 16 + c] = s;
@@ -173,8 +172,8 @@ PackJob pack_work(const float *x, uint8_t *codes, uint8_t *scales, size_t rows, 
 }
 
 // dz's column sums: slices of 512 rows past 1024
-SumJob sum_work(const float *x, const float *times, bool relu, float *out, size_t rows, size_t cols, float *part) {
-    SumJob j = {x, times, out, part, static_cast<int>(rows), static_cast<int>(cols), 1, static_cast<int>(rows), 0, relu};
+SumJob sum_work(const float *x, const float *times, float *out, size_t rows, size_t cols, float *part) {
+    SumJob j = {x, times, out, part, static_cast<int>(rows), static_cast<int>(cols), 1, static_cast<int>(rows), 0};
     if (rows > 1024) {
         j.slice_rows = 512;
         j.slices = static_cast<int>((rows + 511) / 512);
@@ -184,12 +183,11 @@ SumJob sum_work(const float *x, const float *times, bool relu, float *out, size_
 }
 size_t sum_floats(size_t rows, size_t cols) { return rows > 1024 ? round64((rows + 511) / 512 * cols) : 0; }
 
-Operand floats(const float *p, size_t ld, size_t rows, const float *times = nullptr, bool relu = false) {
-    return {p, times, nullptr, nullptr, static_cast<int>(ld), static_cast<int>(rows), 0, relu, 0};
+Operand floats(const float *p, size_t ld, size_t rows, const float *times = nullptr) {
+    return {p, times, nullptr, nullptr, static_cast<int>(ld), static_cast<int>(rows), 0, 0};
 }
 Operand packed(const uint8_t *codes, const uint8_t *scales, size_t code_rows, size_t cols, size_t rows) {
-    return {nullptr, nullptr, codes, scales, 0, static_cast<int>(rows), static_cast<unsigned>(packed_pitch(cols)), false,
-            code_rows};
+    return {nullptr, nullptr, codes, scales, 0, static_cast<int>(rows), packed_pitch(cols), code_rows};
 }
 
 // x W (of floats, or the codes of x)
@@ -207,10 +205,9 @@ LinearProduct forward_product(const ts_hip_linear_shape &s, const float *x, cons
     p.epi = e;
     return p;
 }
-LinearProduct dx_product(const ts_hip_linear_shape &s, const float *dz, const float *slope, bool relu, const float *w,
-                         float *dx) {
+LinearProduct dx_product(const ts_hip_linear_shape &s, const float *dz, const float *slope, const float *w, float *dx) {
     LinearProduct p{};
-    p.A = floats(dz, s.fan_out, s.batch, slope, relu);
+    p.A = floats(dz, s.fan_out, s.batch, slope);
     p.a = Src::kFloatK;
     p.B = floats(w, s.fan_out, s.fan_in);
     p.b = Src::kFloatK;
@@ -221,11 +218,11 @@ LinearProduct dx_product(const ts_hip_linear_shape &s, const float *dz, const fl
     return p;
 }
 LinearProduct dw_product(const ts_hip_linear_shape &s, const float *x, const uint8_t *codes, const uint8_t *scales,
-                         const float *dz, const float *slope, bool relu, float *dw) {
+                         const float *dz, const float *slope, float *dw) {
     LinearProduct p{};
     p.A = codes ? packed(codes, scales, s.batch, s.fan_in, s.fan_in) : floats(x, s.fan_in, s.fan_in);
     p.a = codes ? Src::kCodesR : Src::kFloatR;
-    p.B = floats(dz, s.fan_out, s.fan_out, slope, relu);
+    p.B = floats(dz, s.fan_out, s.fan_out, slope);
     p.b = Src::kFloatR;
     p.M = static_cast<int>(s.fan_in);
     p.N = static_cast<int>(s.fan_out);
@@ -358,13 +355,13 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
                 *const w_dw = workspace + at.dw;
     // dz: go times the forward's slopes as the products read them, or go times the
     // slopes of the layer computed again from its checkpoint, stored
-    const bool again = act != TS_HIP_ACT_NONE && !slope, relu = act == TS_HIP_ACT_RELU;
+    const bool again = act != TS_HIP_ACT_NONE && !slope;
     if (act == TS_HIP_ACT_NONE) slope = nullptr;
     if ((again && (!codes || !weight)) || (dx && !weight) || (dweight && !codes && !x)) return TS_HIP_EINVAL;
     const float *dz = again ? workspace : go;
     LinearProduct pz = forward_product(d, nullptr, codes, scales, weight, workspace, {bias, nullptr, go, nullptr, act});
-    LinearProduct px = dx_product(d, dz, slope, relu, weight, dx);
-    const LinearProduct pw = dw_product(d, x, codes, scales, dz, slope, relu, dweight);
+    LinearProduct px = dx_product(d, dz, slope, weight, dx);
+    const LinearProduct pw = dw_product(d, x, codes, scales, dz, slope, dweight);
     const bool planes_x = dx && weight_planes(px), planes_w = dweight && planes_take(pw.M, pw.N, pw.K);
     // what does not wait for dz goes into planes first, with the layer's own operands
     PlaneWrites writes;
@@ -392,7 +389,7 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
     DirectProduct gx{}, gw{};
     if (later_x) gx = planned(px, w_dx);
     if (later_w) gw = planned(pw, w_dw);
-    const SumJob sum = dbias ? sum_work(dz, slope, relu, dbias, d.batch, d.fan_out, sums) : SumJob{};
+    const SumJob sum = dbias ? sum_work(dz, slope, dbias, d.batch, d.fan_out, sums) : SumJob{};
     int waves = sum.blocks ? 4 : 1;  // (the sums: 16 rows side by side at least)
     if (later_x) waves = gx.kg > waves ? gx.kg : waves;
     if (later_w) waves = gw.kg > waves ? gw.kg : waves;

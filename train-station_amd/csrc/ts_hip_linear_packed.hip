@@ -200,9 +200,8 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
     if (planes_take(batch, fan_out, fan_in)) {
         if (!workspace && ts_hip_linear_packed_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EINVAL;
         LinearProduct q{};
-        const unsigned pitch = static_cast<unsigned>(packed_pitch(fan_in));
-        q.A = {nullptr, nullptr, x_codes, x_scales, 0, static_cast<int>(batch), pitch, false, batch};
-        q.B = {nullptr, nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), pitch, false, fan_out};
+        q.A = {nullptr, nullptr, x_codes, x_scales, 0, static_cast<int>(batch), packed_pitch(fan_in), batch};
+        q.B = {nullptr, nullptr, w_codes, w_scales, 0, static_cast<int>(fan_out), packed_pitch(fan_in), fan_out};
         q.a = q.b = Src::kCodesK;
         q.M = static_cast<int>(batch);
         q.N = static_cast<int>(fan_out);

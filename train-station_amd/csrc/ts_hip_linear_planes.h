@@ -90,7 +90,7 @@ struct PlaneSide {
     static __device__ __forceinline__ unsigned offset(const Operand &o, int b0, int u, int lane) {
         if constexpr (kCodes) {
             const int last = o.rows - 1 - b0 * kPlaneRows;  // rows past an edge: the last one's
-            return static_cast<unsigned>(min(u * 8 + (lane >> 3), last)) * o.pitch +
+            return static_cast<unsigned>(min(u * 8 + (lane >> 3), last)) * static_cast<unsigned>(o.pitch) +
                    16u * ((lane & 7) ^ (4 * u + (lane >> 4) & 7));
         } else {
             return 16u * lane;
@@ -181,7 +181,7 @@ __device__ __forceinline__ void epilogue4(const LinearEpi &e, size_t at, const f
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             activate<true>(o[n], e.act, slope[n]);
-            o[n] = through_slope(extra[n], slope[n], e.act == TS_HIP_ACT_RELU);
+            o[n] = through_slope(extra[n], slope[n]);
         }
         return;
     }

@@ -68,11 +68,11 @@ __device__ __forceinline__ void planes_along(const PlaneJob &j, size_t job) {
                 if (tp) {  // uniform
                     const pk4u_t s = *reinterpret_cast<const pk4u_t *>(tp + k);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = through_slope(t[e], s[e], j.o.relu);
+                    for (int e = 0; e < 4; ++e) w[e] = through_slope(t[e], s[e]);
                 }
             } else if (live) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? (tp ? through_slope(p[k + e], tp[k + e], j.o.relu) : p[k + e]) : 0.0f;
+                for (int e = 0; e < 4; ++e) w[e] = k + e < K ? (tp ? through_slope(p[k + e], tp[k + e]) : p[k + e]) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[b][4 * q + e] = w[e];
@@ -133,13 +133,13 @@ __device__ __forceinline__ void planes_across(const PlaneJob &j, size_t job) {
             for (int e = 0; e < 8; ++e) v[e] = p[static_cast<size_t>(k + e) * ld];
             if (tp) {  // uniform
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = through_slope(v[e], tp[static_cast<size_t>(k + e) * ld], j.o.relu);
+                for (int e = 0; e < 8; ++e) v[e] = through_slope(v[e], tp[static_cast<size_t>(k + e) * ld]);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const size_t at = static_cast<size_t>(k + e) * ld;
-                v[e] = k + e < K ? (tp ? through_slope(p[at], tp[at], j.o.relu) : p[at]) : 0.0f;
+                v[e] = k + e < K ? (tp ? through_slope(p[at], tp[at]) : p[at]) : 0.0f;
             }
         }
         if (!live) {
