@@ -3,11 +3,13 @@ the entry points refuse before they touch a device.  CPU only."""
 from __future__ import annotations
 
 import ctypes
+import subprocess
 
 import numpy as np
 import pytest
 
 import feedforward_ref as R
+from conftest import ROOT
 import train_station_amd as T
 from train_station_amd._ffi import LinearShape, gradtrack, hip, last_error
 
@@ -177,6 +179,14 @@ def test_arrays_that_may_not_be_written_are_refused():
     # codes and scales are read only
     codes, scales = Array(typestr="|u1", shape=(0, 128), data=(P, True)), Array(typestr="|u1", shape=(1, 0, 4), data=(P, True))
     assert T.Packed8.from_device(codes, scales, 100).shape == (0, 100)
+
+
+def test_memory_is_given_back_once_whatever_allocation_fails(tmp_path):
+    lib, here = ROOT / "train-station_amd", ROOT / "tests" / "release_calls.cpp"
+    subprocess.run(["g++", "-O1", "-std=c++17", f"-I{ROOT / 'include'}", "-o", tmp_path / "p", here, f"-L{lib}", "-lts_gradtrack",
+                    "-lts_hip", f"-Wl,-rpath,{lib}", "-Wl,-rpath,/opt/rocm/lib"], check=True)
+    got = subprocess.run([tmp_path / "p"], capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout + got.stderr
 
 
 def test_empty_shapes_of_long_sides_are_empty():

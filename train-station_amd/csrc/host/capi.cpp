@@ -1,4 +1,5 @@
 // C handle API (include/ts_gradtrack.h) over the C++ host classes.
+#include <atomic>
 #include <cstdlib>
 #include <cstring>
 #include <exception>
@@ -78,14 +79,32 @@ ts::Activation activation_of(int act) {
     return static_cast<ts::Activation>(act);
 }
 
-// A caller's release call, for the memory's last user (when the tensor is not
-// made, the entry itself makes it).
-std::function<void()> release_call(void (*release)(void *), void *ctx) {
-    if (!release) return {};
-    return [release, ctx] {
-        if (!ts::external_detached()) release(ctx);
-    };
+// A caller's release call: for the memory's last user, or, where the call that
+// takes the memory fails, for its entry; whichever comes first makes it.
+struct ReleaseCall {
+    void (*release)(void *);
+    void *ctx;
+    std::atomic<bool> made{false};
+    ReleaseCall(void (*r)(void *), void *c) : release(r), ctx(c) {}
+    void operator()() {
+        if (release && !made.exchange(true) && !ts::external_detached()) release(ctx);
+    }
+};
+
+// take(release) as a handle; without one the caller's memory is given back.
+template <class F>
+auto guard_taking(void (*release)(void *), void *ctx, F &&take) -> decltype(take(std::function<void()>())) {
+    std::shared_ptr<ReleaseCall> call;
+    auto *h = guard_ptr([&] {
+        call = std::make_shared<ReleaseCall>(release, ctx);
+        return take(std::function<void()>([call] { (*call)(); }));
+    });
+    if (h) return h;
+    if (call) (*call)();
+    else ReleaseCall(release, ctx)();
+    return nullptr;
 }
+
 std::vector<ts::Tensor *> param_list(ts_tensor *const *params, size_t count) {
     if (count && !params) throw ts::Error("parameter list is NULL");
     std::vector<ts::Tensor *> v;
@@ -128,10 +147,9 @@ int ts_tensor_fill_randn(ts_tensor *t, uint64_t seed, int has_seed) {
     });
 }
 ts_tensor *ts_tensor_from_device(float *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx) {
-    ts_tensor *t =
-        guard_ptr([&] { return wrap(ts::Tensor::from_device(data, dims_of(dims, rank), release_call(release, ctx))); });
-    if (!t && release) release(ctx);
-    return t;
+    return guard_taking(release, ctx, [&](std::function<void()> give_back) {
+        return wrap(ts::Tensor::from_device(data, dims_of(dims, rank), std::move(give_back)));
+    });
 }
 void ts_external_detach(void) { ts::detach_external(); }
 
@@ -172,11 +190,9 @@ ts_packed8 *ts_tensor_rms_norm_packed(const ts_tensor *x, const ts_tensor *resid
 }
 ts_packed8 *ts_packed8_from_device(uint8_t *codes, uint8_t *scales, size_t rows, size_t cols, void (*release)(void *),
                                    void *ctx) {
-    ts_packed8 *p = guard_ptr([&] {
-        return new ts_packed8{ts::Packed8::from_device(codes, scales, rows, cols, release_call(release, ctx))};
+    return guard_taking(release, ctx, [&](std::function<void()> give_back) {
+        return new ts_packed8{ts::Packed8::from_device(codes, scales, rows, cols, std::move(give_back))};
     });
-    if (!p && release) release(ctx);
-    return p;
 }
 void ts_packed8_free(ts_packed8 *p) { delete p; }
 size_t ts_packed8_rows(const ts_packed8 *p) { return p ? p->p.rows() : 0; }
