@@ -194,6 +194,10 @@ def prepare(case, seed):
 
 
 # ---- one pass with the framework's operators ----------------------------------------
+# A pass is queued on the library's own stream, as a program's next call follows
+# it there.  The tensors returned are views of the library's buffers: read them
+# after torch.cuda.synchronize() (or on the library's stream), and before they are
+# let go, since the next pass may then write their memory.
 
 
 def _run_own(s):
