@@ -37,7 +37,8 @@ ts_tensor *ts_tensor_from_slice(const float *data, size_t len, const size_t *dim
  * counterpart in the reference).  `release` (may be NULL) is called with ctx,
  * from whichever thread lets the last user go, once every handle, saved
  * operand and step graph that uses the memory is gone and the work queued by
- * then has run; also at once when this call fails or the tensor is empty.
+ * then has run (the thread that lets the last user go waits for it); also at
+ * once when this call fails or the tensor is empty.
  * Work on other streams that writes the memory must have finished before the
  * library reads it, and the library's work before others read what it wrote
  * (ts_synchronize, or an event on ts_stream).  Memory that is not one

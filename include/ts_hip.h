@@ -643,7 +643,7 @@ int ts_hip_linear_packed(const uint8_t *x_codes, const uint8_t *x_scales, const 
  * stored there, laid out as y (what the backward pass reads; relu's 0 as -0).  codes != NULL: x is also
  * packed into codes / scales (ts_hip_pack8). */
 typedef struct ts_hip_linear_shape {
-    size_t batch, fan_in, fan_out;
+    size_t batch, fan_in, fan_out;  /* each below 2^24, a matrix below 2^34 values: TS_HIP_EINVAL past that */
 } ts_hip_linear_shape;
 size_t ts_hip_linear_workspace_floats(const ts_hip_linear_shape *shape);
 int ts_hip_linear(const ts_hip_linear_shape *shape, const float *x, const float *weight, const float *bias, int act,

@@ -788,6 +788,46 @@ def test_block_trains_and_replays_as_it_runs(batch, d, f):
     g.free()
 
 
+def test_a_stack_of_blocks_by_leaves_has_the_stacks_gradients():
+    """Each block's input a leaf of its own, its gradient passed on to the block below: every node runs once."""
+    depth, batch, d, f = 4, 24, 48, 80
+    stack = [block_parameters(d, f, 10 * i) for i in range(depth)]
+    x, go = normal((batch, d), 5), normal((batch, d), 6)
+
+    def block(ps, h):
+        norm, w1, b1, w2, b2 = ps
+        y = h.rms_norm(norm).linear(w1, bias=b1, activation="silu")
+        return y.linear(w2, bias=b2, residual=h)
+
+    def grads(first):
+        g = [first.grad_by_value().data()] + [p.grad_by_value().data() for ps in stack for p in ps]
+        for ps in stack:
+            for p in ps:
+                p.zero_grad()
+        T.clear_gradients()
+        return g
+
+    X = tensor(x).with_requires_grad()
+    h = X
+    for ps in stack:
+        h = block(ps, h)
+    h.backward(tensor(go))
+    whole = grads(X)
+
+    leaves, outs = [tensor(x).with_requires_grad()], []
+    for ps in stack:
+        outs.append(block(ps, leaves[-1]))
+        with T.NoGradTrack():
+            leaves.append(outs[-1].clone())
+        leaves[-1].with_requires_grad()
+    g = tensor(go)
+    for leaf, y in zip(reversed(leaves[:-1]), reversed(outs)):
+        y.backward(g)
+        g = leaf.grad_by_value()
+    for a, b in zip(grads(leaves[0]), whole):
+        assert np.linalg.norm(a - b) <= 1e-5 * np.linalg.norm(b)
+
+
 def test_a_recorded_step_keeps_the_device_memory_it_reads():
     import gc
 

@@ -13,9 +13,10 @@
 // b = f^2 r mean(g h), whose parts are of g's size however long a row is, where
 // r and r^3 mean(g h) themselves leave fp32 long before dh does.
 //
-// Bound by memory from a few thousand rows on, by the launch below (us, 8192 x 4096
-// with the sum): forward 85 for 537 MB, packed 87 for 437 MB, backward 85 for 403 MB
-// (h partly from the last-level cache); 16384 x 2048 the same; 1 x 4096 packed 5.
+// Bound by memory from a few thousand rows on, below by the launch and by what a
+// row's waves wait for in turn: loads, sums, stores (3000 x 1003 packed 8.6 us for 15 MB).
+// us, 8192 x 4096 with the sum: forward 85 for 537 MB, packed 87 for 437 MB, backward 85
+// for 403 MB (h partly from the last-level cache); 16384 x 2048 the same; 1 x 4096 packed 5.
 // The f64 sums and the packed form's f64 products are under that: a wave has four
 // loads of 16 bytes in flight per operand, and four waves a row leave two rows a SIMD.
 #include "ts_hip_pack8.h"
