@@ -726,6 +726,58 @@ def test_device_memory_is_used_in_place_and_given_back():
     assert len(module._lent) == held - 1
 
 
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("rows,cols", [(3, 5), (64, 8), (40, 300), (700, 64)])
+def test_every_operation_takes_memory_at_any_address(rows, cols, offset):
+    """The framework's operations over a caller's memory, as over its own: only the order of a sum may differ."""
+    x, y, w = np.abs(normal((rows, cols), 1)) + 0.1, normal((rows, cols), 2), normal((cols, 24), 3)
+    v, go = normal((cols,), 4), normal((rows, 24), 5)
+
+    def run(place):
+        X, Y, W, V, G = (place(a) for a in (x, y, w, v, go))
+        out = [X.add_tensor(Y), X.sub_tensor(Y), Y.mul_tensor(X), Y.div_tensor(X), X.add_tensor(V), X.exp(), X.log(), X.sqrt(),
+               Y.tanh(), Y.sigmoid(), Y.relu(), Y.leaky_relu(0.1), X.pow_scalar(1.5), X.add_scalar(2.0), Y.softmax(1), Y.softmax(0),
+               X.sum(), X.mean(), X.sum_dims([0]), X.sum_dims([1]), X.mean_dims([0, 1]), Y.t().contiguous(), Y.clone(),
+               Y.matmul(W), Y.t().matmul(G), G.t().matmul(Y), Y.matmul(X.t()), Y.rms_norm(V), Y.pack8().unpack(),
+               Y.linear(W, activation="silu", residual=G), T.Tensor.from_binary(Y.to_binary()), T.Tensor.from_json(Y.to_json())]
+        got = [t.data() for t in out]
+        # a layer's step: gradients, the optimizer on the caller's parameters
+        B = place(np.zeros(24, np.float32))
+        for p in (W, B):
+            p.with_requires_grad()
+        opt = T.Adam.with_learning_rate(1e-2)
+        opt.add_parameters([W, B])
+        loss = G.mul_tensor(G).mean()  # of the gradient that the products read
+        Y.matmul(W).add_tensor(B).backward(G)
+        got += [W.grad_by_value().data(), B.grad_by_value().data(), loss.data()]
+        opt.step([W, B])
+        opt.zero_grad([W, B])
+        T.clear_gradients()
+        X.fill(3.0)
+        return got + [W.data(), B.data(), X.data()]
+
+    own = run(tensor)
+    lent = run(lambda a: T.Tensor.from_device(DeviceArray(np.ascontiguousarray(a, np.float32), offset)))
+    for n, (a, b) in enumerate(zip(own, lent)):
+        assert a.shape == b.shape and np.allclose(a, b, rtol=2e-6, atol=2e-5), n
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+@pytest.mark.parametrize("m,k,n", [(64, 8, 8), (32, 784, 128), (64, 40, 64)])
+def test_a_sum_beside_a_weights_gradient_takes_memory_at_any_address(m, k, n, offset):
+    """A gradient over a caller's memory whose sum waits: the weight gradient's launch forms it where it can."""
+    x, w, go = normal((m, k), 1), normal((k, n), 2), normal((m, n), 3)
+    W, B = tensor(w).with_requires_grad(), tensor(np.zeros(n, np.float32)).with_requires_grad()
+    g = T.Tensor.from_device(DeviceArray(go, offset))
+    total = g.mul_scalar(2.0).sum()
+    tensor(x).matmul(W).add_tensor(B).backward(g)
+    g64 = go.astype(np.float64)
+    assert abs(total.value() - 2 * g64.sum()) <= m * n * R.U * 2 * np.abs(g64).sum()
+    assert_within(W.grad_by_value().data(), x.T.astype(np.float64) @ g64, R.product_bound(x.T, go), "dweight")
+    assert_within(B.grad_by_value().data(), g64.sum(0), m * R.U * np.abs(g64).sum(0), "dbias")
+    T.clear_gradients()
+
+
 def test_memory_of_another_device_is_refused():
     import ctypes
 

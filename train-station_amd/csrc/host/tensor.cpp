@@ -2154,11 +2154,13 @@ std::vector<std::optional<Tensor>> GradFn::apply(const Tensor &go) const {
                                     operand_xf(go.allocation(), leaf, xb);
                     // a deferred sum of the buffer read as B, or of a chain over
                     // it (the README step's loss over relu's output; an MSE's
-                    // mean of d * d), comes out of this launch too
+                    // mean of d * d), comes out of this launch too, unless the
+                    // buffer is a caller's whose address its loads do not take
                     ts_hip_operand_xf xs{};
+                    const std::shared_ptr<Allocation> &summed = fx ? leaf : go.allocation();
                     const std::shared_ptr<Allocation> bsum =
-                        db && ts_hip_gemm_takes_bsum(ta, Kd, N, M)
-                            ? pending_sum_of(fx ? leaf : go.allocation(), M * N, xs)
+                        db && ts_hip_gemm_takes_bsum(ta, Kd, N, M) && reinterpret_cast<uintptr_t>(summed->raw()) % 16 == 0
+                            ? pending_sum_of(summed, M * N, xs)
                             : nullptr;
                     const bool mean = bsum && bsum->reduce->mean;
                     if (db) db->colsum.reset();
