@@ -41,7 +41,10 @@ ts_tensor *ts_tensor_from_slice(const float *data, size_t len, const size_t *dim
  * once when this call fails or the tensor is empty.
  * Work on other streams that writes the memory must have finished before the
  * library reads it, and the library's work before others read what it wrote
- * (ts_synchronize, or an event on ts_stream).  Memory that is not one
+ * or write what it reads (ts_synchronize, or an event recorded on ts_stream
+ * when that call has returned: either first runs what the calling thread has
+ * deferred of such reads; a backward pass still to come reads its saved
+ * operands then).  Memory that is not one
  * allocation's on the current device is refused. */
 ts_tensor *ts_tensor_from_device(float *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx);
 /* The process is ending: from here on no release call is made. */
@@ -240,7 +243,8 @@ int ts_adam_config_from_binary(const uint8_t *data, size_t len, float *values5, 
 int ts_adam_config_to_json(const float *values5, int amsgrad, char **json, size_t *len);
 int ts_adam_config_from_json(const char *json, size_t len, float *values5, int *amsgrad);
 
-/* runtime: wait for queued work (reports a recorded division by zero) */
+/* runtime: wait for queued work and deferred reads of callers' memory
+ * (reports a recorded division by zero) */
 int ts_synchronize(void);
 
 /* Fusion of recorded ops into the producing product (no counterpart in the
@@ -289,7 +293,8 @@ void ts_step_graph_abort(void);
 int ts_step_graph_recording(void);
 int ts_step_graph_replay(ts_step_graph *g, size_t times);
 void ts_step_graph_free(ts_step_graph *g);
-/* library stream (for timing events on the stream the kernels run on) */
+/* library stream (for timing events on the stream the kernels run on, and for
+ * ordering others' work behind it: deferred reads of callers' memory are queued first) */
 void *ts_stream(void);
 /* device pool statistics and cache release */
 size_t ts_pool_live_bytes(void);

@@ -762,6 +762,35 @@ def test_every_operation_takes_memory_at_any_address(rows, cols, offset):
         assert a.shape == b.shape and np.allclose(a, b, rtol=2e-6, atol=2e-5), n
 
 
+@pytest.mark.parametrize("order", ["synchronize", "stream"])
+def test_lent_memory_may_be_written_again_once_the_library_is_waited_for(order):
+    """What was computed from it has the values it held then, read or not by the time it is written."""
+    x, w = normal((48, 32), 1), normal((32, 24), 2)
+    go = np.abs(normal((48, 24), 3))
+
+    def values(t, g, W):
+        y = t.matmul(W)
+        m = t.mul_scalar(2.0).add_scalar(1.0)
+        W.with_requires_grad()
+        s = g.mul_scalar(3.0).sum()
+        out = [y, y.relu(), t.matmul(W).add_tensor(y).sum(), m, m.mul_tensor(m).mean(), t.sum(), t.t().contiguous(), t.exp(),
+               t.softmax(1), t.sum_dims([0]), t.linear(W), t.clone(), s]
+        return out
+
+    want = [v.data() for v in values(tensor(x), tensor(go), tensor(w))]
+    a, b, c = DeviceArray(x), DeviceArray(go), DeviceArray(w)
+    got = values(*(T.Tensor.from_device(v) for v in (a, b, c)))
+    if order == "synchronize":
+        T.synchronize()
+    else:  # as an event recorded there would
+        hip_check(hip.ts_hip_stream_synchronize(T.stream()), "ts_hip_stream_synchronize")
+    for v in (a, b, c):
+        v.dev.put(np.full(v.host.size, 7.0, np.float32))
+    for n, (g, v) in enumerate(zip(got, want)):
+        assert np.array_equal(g.data(), v), n
+    T.clear_gradients()
+
+
 @pytest.mark.parametrize("offset", [0, 1, 2, 3])
 @pytest.mark.parametrize("m,k,n", [(64, 8, 8), (32, 784, 128), (64, 40, 64)])
 def test_a_sum_beside_a_weights_gradient_takes_memory_at_any_address(m, k, n, offset):

@@ -613,11 +613,17 @@ int ts_step_graph_replay(ts_step_graph *g, size_t times) {
 void ts_step_graph_free(ts_step_graph *g) { delete g; }
 
 int ts_synchronize(void) {
-    return guard_int([&] { ts::Runtime::get().sync(); });
+    return guard_int([&] {
+        ts::Runtime &rt = ts::Runtime::get();
+        if (!ts::StepRecorder::get().open()) ts::run_external_reads();
+        rt.sync();
+    });
 }
 void *ts_stream(void) {
     try {
-        return ts::Runtime::get().stream();
+        ts::Runtime &rt = ts::Runtime::get();
+        if (!ts::StepRecorder::get().open()) ts::run_external_reads();
+        return rt.stream();
     } catch (...) {
         return nullptr;
     }

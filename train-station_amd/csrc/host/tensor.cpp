@@ -258,8 +258,28 @@ void axis_view(const std::vector<size_t> &dims, size_t dim, size_t &outer, size_
 namespace {
 bool g_fusion = true;
 
+// Callers' memory that deferred work of this thread reads.
+std::vector<std::weak_ptr<Allocation>> &external_reads() {
+    thread_local std::vector<std::weak_ptr<Allocation>> v;
+    return v;
+}
+
+void note_external_read(const std::shared_ptr<Allocation> &input) {
+    auto &v = external_reads();
+    size_t live = 0;  // drop memory let go meanwhile
+    bool known = false;
+    for (auto &w : v) {
+        const auto a = w.lock();
+        known = known || a == input;
+        if (a) v[live++] = w;
+    }
+    v.resize(live);
+    if (!known) v.push_back(input);
+}
+
 void add_reader(const std::shared_ptr<Allocation> &input, const std::shared_ptr<Allocation> &reader) {
     if (!input) return;
+    if (input->external()) note_external_read(input);
     auto &rs = input->readers;
     size_t live = 0;  // drop readers that are gone or already produced
     for (auto &w : rs) {
@@ -270,6 +290,13 @@ void add_reader(const std::shared_ptr<Allocation> &input, const std::shared_ptr<
     rs.push_back(reader);
 }
 }  // namespace
+
+void run_external_reads() {
+    std::vector<std::weak_ptr<Allocation>> v;
+    v.swap(external_reads());
+    for (auto &w : v)
+        if (const auto a = w.lock()) a->before_write();
+}
 
 void set_fusion(bool on) { g_fusion = on; }
 bool fusion_enabled() { return g_fusion; }

@@ -255,6 +255,7 @@ struct Allocation : std::enable_shared_from_this<Allocation> {
     // Before this buffer is written in place: runs every still-pending
     // producer that reads it, so they see the old contents.
     void before_write();
+    bool external() const { return static_cast<bool>(release_); }  // a caller's memory
     std::shared_ptr<PendingGemm> pending;
     std::shared_ptr<PendingMap> map;                 // deferred elementwise value
     std::shared_ptr<PendingColsum> colsum;           // deferred column sum
@@ -277,6 +278,10 @@ struct Allocation : std::enable_shared_from_this<Allocation> {
 // The process is ending: callers' memory is let go without their release calls.
 void detach_external();
 bool external_detached();
+
+// Runs what this thread deferred of reads of callers' memory: they may write it
+// once they have waited for the library (tensor.cpp).
+void run_external_reads();
 
 // Runs a's pending producer (tensor.cpp).
 void materialize(Allocation &a);

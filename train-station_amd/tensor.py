@@ -152,8 +152,9 @@ class Tensor:
         """A tensor over the memory of a contiguous, writable float32 device array (any
         object with ``__cuda_array_interface__``), not copied; the array is held
         until the library's last use of it.  What wrote it must have finished,
-        and others may read what the library writes to it only after
-        ``synchronize()`` (or an event on ``stream()``)."""
+        and others may read what the library writes to it, or write to it
+        again, only after ``synchronize()`` (or an event recorded on what
+        ``stream()`` returns then) and the backward passes that read it."""
         ptr, shape = _device_array(array, "<f4", True)
         d, r = _dims(shape)
         return _wrap(_G.ts_tensor_from_device(ptr, d, r, _give_back, _lend(array)))
