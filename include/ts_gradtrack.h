@@ -43,8 +43,10 @@ ts_tensor *ts_tensor_from_slice(const float *data, size_t len, const size_t *dim
  * library reads it, and the library's work before others read what it wrote
  * or write what it reads (ts_synchronize, or an event recorded on ts_stream
  * when that call has returned: either first runs what the calling thread has
- * deferred of such reads; a backward pass still to come reads its saved
- * operands then).  Memory that is not one
+ * deferred of such reads, and copies gradients that stand in such memory, as a
+ * residual's does where the output's gradient is the caller's; a handle of
+ * ts_tensor_grad_view or ts_tensor_grad taken before stays on it, and a
+ * backward pass still to come reads its saved operands then).  Memory that is not one
  * allocation's on the current device is refused. */
 ts_tensor *ts_tensor_from_device(float *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx);
 /* The process is ending: from here on no release call is made. */

@@ -791,6 +791,28 @@ def test_lent_memory_may_be_written_again_once_the_library_is_waited_for(order):
     T.clear_gradients()
 
 
+def test_gradients_outlive_the_lent_memory_of_the_one_they_came_from():
+    """A residual's gradient is the output's own; it stays when the caller writes that memory again, and adds up."""
+    x, w, r = normal((20, 16), 1), normal((16, 12), 2), normal((20, 12), 3)
+    X, Rs, W = tensor(x), tensor(r).with_requires_grad(), tensor(w)
+    A = tensor(r).with_requires_grad()
+    first, second = normal((20, 12), 4), normal((20, 12), 5)
+    lent = DeviceArray(first)
+    g = T.Tensor.from_device(lent)
+    y = X.linear(W, residual=Rs).add_tensor(A)
+    y.backward(g)
+    T.synchronize()
+    lent.dev.put(second)
+    for t in (Rs, A, y):
+        assert np.array_equal(t.grad_by_value().data(), first)
+    X.linear(W, residual=Rs).add_tensor(A).backward(g)
+    T.synchronize()
+    lent.dev.put(np.zeros_like(second))
+    for t in (Rs, A):
+        assert np.array_equal(t.grad_by_value().data(), first + second)
+    T.clear_gradients()
+
+
 @pytest.mark.parametrize("offset", [0, 1, 2, 3])
 @pytest.mark.parametrize("m,k,n", [(64, 8, 8), (32, 784, 128), (64, 40, 64)])
 def test_a_sum_beside_a_weights_gradient_takes_memory_at_any_address(m, k, n, offset):

@@ -70,6 +70,31 @@ const Tensor *accumulated_gradient(size_t id) {
 }
 
 namespace {
+// Gradients stored on tensors (the roots') that stand in a caller's memory.
+std::vector<std::weak_ptr<Tensor>> &lent_gradients() {
+    thread_local std::vector<std::weak_ptr<Tensor>> v;
+    return v;
+}
+bool lent(const Tensor &t) { return t.allocation() && t.allocation()->external(); }
+}  // namespace
+
+void note_lent_gradient(const std::shared_ptr<Tensor> &g) {
+    if (!lent(*g)) return;
+    auto &v = lent_gradients();
+    v.erase(std::remove_if(v.begin(), v.end(), [](const auto &w) { return w.expired(); }), v.end());
+    v.push_back(g);
+}
+
+void own_gradients() {
+    for (auto &kv : graph().gradients)
+        if (lent(kv.second)) kv.second = kv.second.clone();
+    for (auto &w : lent_gradients())
+        if (const auto g = w.lock())
+            if (lent(*g)) *g = g->clone();
+    lent_gradients().clear();
+}
+
+namespace {
 thread_local int g_backward_depth = 0;  // backward calls running on this thread
 struct BackwardScope {
     BackwardScope() { ++g_backward_depth; }

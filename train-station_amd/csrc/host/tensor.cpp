@@ -296,6 +296,7 @@ void run_external_reads() {
     v.swap(external_reads());
     for (auto &w : v)
         if (const auto a = w.lock()) a->before_write();
+    own_gradients();
 }
 
 void set_fusion(bool on) { g_fusion = on; }
@@ -1393,6 +1394,7 @@ void Tensor::accumulate_grad(Tensor g) {
         grad_ = std::make_shared<Tensor>(std::move(acc));
     } else {
         grad_ = std::make_shared<Tensor>(std::move(g));
+        note_lent_gradient(grad_);
     }
 }
 

@@ -279,9 +279,11 @@ struct Allocation : std::enable_shared_from_this<Allocation> {
 void detach_external();
 bool external_detached();
 
-// Runs what this thread deferred of reads of callers' memory: they may write it
-// once they have waited for the library (tensor.cpp).
+// Runs what this thread deferred of reads of callers' memory, which they may write
+// once they have waited for the library, and copies gradients that stand in it (a
+// residual's is the output's own) (tensor.cpp; engine.cpp).
 void run_external_reads();
+void own_gradients();
 
 // Runs a's pending producer (tensor.cpp).
 void materialize(Allocation &a);
@@ -625,6 +627,9 @@ class Packed8 {
     std::shared_ptr<Allocation> codes_, scales_;
     size_t rows_ = 0, cols_ = 0;
 };
+
+// A gradient just stored on a tensor: noted where it stands in a caller's memory (engine.cpp).
+void note_lent_gradient(const std::shared_ptr<Tensor> &g);
 
 // The gradients of Kind::RmsNorm and Kind::Linear (feedforward.cpp).
 std::vector<std::optional<Tensor>> rms_norm_backward(const GradFn &fn, const Tensor &go);
