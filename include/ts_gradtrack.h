@@ -139,6 +139,51 @@ ts_tensor *ts_packed8_unpack(const ts_packed8 *p);
 ts_tensor *ts_packed8_linear(const ts_packed8 *x, const ts_packed8 *weight, const ts_tensor *bias, int activation,
                              const ts_tensor *residual);
 
+/* ---- a student's operators (no counterpart in the reference) -------------------
+ * Layer norm over the last axis, (h - mean(h)) / sqrt(var(h) + eps) * weight + bias
+ * (bias may be NULL): of x, or of h = x + residual (same shape), which *h_out receives
+ * (recorded as add_tensor's sum).  Gradients go to x, residual, weight and bias. */
+ts_tensor *ts_tensor_layer_norm(const ts_tensor *x, const ts_tensor *weight, const ts_tensor *bias, float eps);
+ts_tensor *ts_tensor_add_layer_norm(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight,
+                                    const ts_tensor *bias, float eps, ts_tensor **h_out);
+/* Matrices in 8 bits with a 32-bit scale per 128 columns of a row or, tiles != 0, of 128
+ * rows (layout and rounding: ts_hip_block8).  No gradient passes through them.  residual
+ * of the norm: NULL, or h goes to *h_out. */
+typedef struct ts_block8 ts_block8;
+ts_block8 *ts_tensor_block8(const ts_tensor *x, int tiles);
+ts_block8 *ts_tensor_layer_norm_block8(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight,
+                                       const ts_tensor *bias, float eps, ts_tensor **h_out);
+/* the caller's codes [rows, pitch] (16-byte aligned) and scales [pitch / 128, rows], or
+ * as tiles [pitch / 128, rows / 128 rounded up], on the device, as ts_tensor_from_device */
+ts_block8 *ts_block8_from_device(uint8_t *codes, float *scales, size_t rows, size_t cols, int tiles, void (*release)(void *),
+                                 void *ctx);
+void ts_block8_free(ts_block8 *p);
+size_t ts_block8_rows(const ts_block8 *p);
+size_t ts_block8_cols(const ts_block8 *p);
+int ts_block8_tiles(const ts_block8 *p);
+size_t ts_block8_pitch(const ts_block8 *p);
+const uint8_t *ts_block8_codes_ptr(const ts_block8 *p);
+const float *ts_block8_scales_ptr(const ts_block8 *p);
+ts_tensor *ts_block8_unpack(const ts_block8 *p);
+/* act(x weight^T + bias) + residual, x [batch, fan_in] not in tiles and weight [fan_out, fan_in] in tiles */
+ts_tensor *ts_block8_linear(const ts_block8 *x, const ts_block8 *weight, const ts_tensor *bias, int activation,
+                            const ts_tensor *residual);
+/* Whole numbers on the device, 32 bits each (copied, or a caller's memory as ts_tensor_from_device) */
+typedef struct ts_indices ts_indices;
+ts_indices *ts_indices_from_slice(const int32_t *data, size_t len, const size_t *dims, size_t rank);
+ts_indices *ts_indices_from_device(int32_t *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx);
+void ts_indices_free(ts_indices *i);
+size_t ts_indices_dims(const ts_indices *i, size_t *out, size_t cap);
+const int32_t *ts_indices_device_ptr(const ts_indices *i);
+/* The loss, one value, of a student's logits [rows, vocab] against a teacher's top logits
+ * (indices and teacher [rows, kept]) at a temperature, and, with weight hard from 0 to 1,
+ * the labels [rows] (NULL where hard is 0); weights [rows] of the rows, NULL: 1 / rows
+ * each (formulas and what is left out: ts_hip_distillation).  The gradient goes to the
+ * logits alone, and is computed with the loss.  An index outside the vocabulary is
+ * reported by the next synchronisation. */
+ts_tensor *ts_tensor_distillation(const ts_tensor *logits, const ts_indices *indices, const ts_tensor *teacher,
+                                  float temperature, const ts_indices *labels, float hard, const ts_tensor *weights);
+
 /* transpose(dim0, dim1) / t() (transform/transpose.rs:156-208, :283-291): a
  * transposed view, recorded (Transpose GradFn, grad_fn/mod.rs:243-249, :575)
  * whenever the input requires grad.  The view's values are copied only when
@@ -246,7 +291,7 @@ int ts_adam_config_to_json(const float *values5, int amsgrad, char **json, size_
 int ts_adam_config_from_json(const char *json, size_t len, float *values5, int *amsgrad);
 
 /* runtime: wait for queued work and deferred reads of callers' memory
- * (reports a recorded division by zero) */
+ * (reports a recorded division by zero, or an index outside a vocabulary) */
 int ts_synchronize(void);
 
 /* Fusion of recorded ops into the producing product (no counterpart in the

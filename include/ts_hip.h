@@ -662,6 +662,69 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
                            const float *go, float *dx, float *dweight, float *dbias, float *workspace,
                            size_t workspace_floats, void *stream);
 
+/* ---- a student's operators (no counterpart in the reference) -----------------------
+ *
+ * Values in 8 bits with a 32-bit scale for each block of 128 columns.  Codes are
+ * e4m3, rows padded with zeros to pitch = ts_hip_packed_pitch(cols) columns:
+ *   codes  [rows][pitch] bytes, 16-byte aligned
+ *   scales [pitch / 128][ts_hip_block8_scale_rows(rows, tiles)] floats: of a row's 128
+ *          columns (tiles 0: an input), or of 128 rows' (tiles 1: a weight)
+ * A block's scale is its largest magnitude, held to 2^-100 .. 448 2^119, over 448; its
+ * codes are its values times 1 / scale, rounded to the nearest (ties to even, past 448:
+ * 448).  A NaN gets a NaN code (of either sign) and is left out of its block's largest. */
+size_t ts_hip_block8_scale_rows(size_t rows, int tiles);
+int ts_hip_block8(const float *x, size_t rows, size_t cols, int tiles, uint8_t *codes, float *scales, void *stream);
+/* out [rows, cols]: the values that the codes stand for, rounded to fp32 */
+int ts_hip_unblock8(const uint8_t *codes, const float *scales, size_t rows, size_t cols, int tiles, float *out, void *stream);
+/* y [batch, fan_out] = act(x W^T + bias) + residual with x [batch, fan_in] (a scale per
+ * row) and W [fan_out, fan_in] (a scale per 128 rows); bias (fan_out) and residual (laid
+ * out as y) may be NULL.  Sizes as ts_hip_linear_packed's.  The products of the codes
+ * are exact, summed in fp32 over 128 columns and these sums in fp32 with their scales'
+ * product (which a row and a tile with scales below 2^-63 may take below fp32's range). */
+size_t ts_hip_linear_block8_workspace_floats(size_t batch, size_t fan_in, size_t fan_out);
+int ts_hip_linear_block8(const uint8_t *x_codes, const float *x_scales, const uint8_t *w_codes, const float *w_scales,
+                         size_t batch, size_t fan_in, size_t fan_out, const float *bias, int act, const float *residual,
+                         float *y, float *workspace, size_t workspace_floats, void *stream);
+
+/* Layer norm over the rows of [rows, cols], with the residual's addition: h = x +
+ * residual (fp32; residual NULL: h = x and the argument h is NULL too),
+ *   y = (h - mean(h)) / sqrt(mean((h - mean(h))^2) + eps) * weight + bias
+ * bias may be NULL.  Mean and variance are taken in f64.  h may be x or residual. */
+int ts_hip_layer_norm(const float *x, const float *residual, const float *weight, const float *bias, size_t rows, size_t cols,
+                      float eps, float *h, float *y, void *stream);
+/* The same with y in 8 bits, a scale per row and 128 columns: ts_hip_block8 of y. */
+int ts_hip_layer_norm_block8(const float *x, const float *residual, const float *weight, const float *bias, size_t rows,
+                             size_t cols, float eps, float *h, uint8_t *codes, float *scales, void *stream);
+/* The gradients from go = dy, with u = (h - mean(h)) r, r = 1 / sqrt(var + eps) and g = go weight:
+ *   dh = r (g - mean(g) - u mean(g u)),  dweight = sum over rows of go u,  dbias = of go
+ * Each may be NULL.  The workspace (8-byte aligned) is needed for dweight and dbias.  A
+ * pass adds in a fixed order.  ticket: as ts_hip_rms_norm_backward's. */
+size_t ts_hip_layer_norm_backward_workspace_floats(size_t rows, size_t cols);
+int ts_hip_layer_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
+                               float *dh, float *dweight, float *dbias, float *workspace, size_t workspace_floats,
+                               unsigned *ticket, void *stream);
+
+/* A student's loss against a teacher's top logits and the true labels.  Of each row z of
+ * logits [rows, vocab], with q the softmax of the teacher's kept logits over the
+ * temperature T, p the softmax of z / T (over all columns), s that of z and a = hard:
+ *   loss[0] = sum over rows of w ((1 - a) T^2 sum over k of q_k (log q_k - log p[i_k])
+ *                                 - a log s[label])
+ *   dlogits = go w ((1 - a) T (p - q) + a (s - 1 at the label))   (NULL: not wanted)
+ * indices and teacher [rows, kept]: the columns i_k and their logits; an index below 0
+ * is no entry, nor is a logit of -inf, and an index given twice counts twice.  labels
+ * [rows]: below 0 is none.  A row without entries has no first term, one without a
+ * label no second; a row of weight 0 (or with neither term) is not looked at and its
+ * gradients are 0.  weights [rows] NULL: 1 / rows each.  go: a device float, NULL: 1.
+ * kept is at most 1024, vocab 2^30, T from 1e-18 to 1e19, hard from 0 to 1 (0: labels may be NULL).
+ * An index past the vocabulary is no entry, and the smallest (row * kept + k, or 2^63 +
+ * row for a label) is left in *bad, a device word (atomic minimum).  The workspace is
+ * 16-byte aligned.  A pass adds in a fixed order. */
+size_t ts_hip_distillation_workspace_floats(size_t rows, size_t vocab);
+int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const int32_t *indices, const float *teacher, size_t kept,
+                        float temperature, const int32_t *labels, float hard, const float *weights, const float *go,
+                        float *loss, float *dlogits, unsigned long long *bad, float *workspace, size_t workspace_floats,
+                        void *stream);
+
 /* ---- optimizer ------------------------------------------------------------------ */
 
 /* optimizers/adam/mod.rs:485-1007, one parameter, fused into one pass that

@@ -193,6 +193,17 @@ HIP_SIGNATURES = {
     "ts_hip_rms_norm_backward": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, SZ, VP, VP]),
     "ts_hip_linear_packed_workspace_floats": (SZ, [SZ, SZ, SZ]),
     "ts_hip_linear_packed": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, SZ, VP, _c.c_int, VP, VP, VP, SZ, VP]),
+    "ts_hip_block8_scale_rows": (SZ, [SZ, _c.c_int]),
+    "ts_hip_block8": (_c.c_int, [VP, SZ, SZ, _c.c_int, VP, VP, VP]),
+    "ts_hip_unblock8": (_c.c_int, [VP, VP, SZ, SZ, _c.c_int, VP, VP]),
+    "ts_hip_linear_block8_workspace_floats": (SZ, [SZ, SZ, SZ]),
+    "ts_hip_linear_block8": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, SZ, VP, _c.c_int, VP, VP, VP, SZ, VP]),
+    "ts_hip_layer_norm": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP]),
+    "ts_hip_layer_norm_block8": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, VP]),
+    "ts_hip_layer_norm_backward_workspace_floats": (SZ, [SZ, SZ]),
+    "ts_hip_layer_norm_backward": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, VP, SZ, VP, VP]),
+    "ts_hip_distillation_workspace_floats": (SZ, [SZ, SZ]),
+    "ts_hip_distillation": (_c.c_int, [VP, SZ, SZ, VP, VP, SZ, _c.c_float, VP, _c.c_float, VP, VP, VP, VP, VP, VP, SZ, VP]),
     "ts_hip_linear_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),
     "ts_hip_linear": (_c.c_int, [_c.POINTER(LinearShape), VP, VP, VP, _c.c_int, VP, VP, VP, VP, VP, VP, SZ, VP]),
     "ts_hip_linear_backward_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),
@@ -264,6 +275,26 @@ GRADTRACK_SIGNATURES = {
     "ts_packed8_scales_ptr": (VP, [TP]),
     "ts_packed8_unpack": (TP, [TP]),
     "ts_packed8_linear": (TP, [TP, TP, TP, _c.c_int, TP]),
+    "ts_tensor_layer_norm": (TP, [TP, TP, TP, _c.c_float]),
+    "ts_tensor_add_layer_norm": (TP, [TP, TP, TP, TP, _c.c_float, _c.POINTER(TP)]),
+    "ts_tensor_block8": (TP, [TP, _c.c_int]),
+    "ts_tensor_layer_norm_block8": (TP, [TP, TP, TP, TP, _c.c_float, _c.POINTER(TP)]),
+    "ts_block8_from_device": (TP, [VP, VP, SZ, SZ, _c.c_int, VP, VP]),
+    "ts_block8_free": (None, [TP]),
+    "ts_block8_rows": (SZ, [TP]),
+    "ts_block8_cols": (SZ, [TP]),
+    "ts_block8_tiles": (_c.c_int, [TP]),
+    "ts_block8_pitch": (SZ, [TP]),
+    "ts_block8_codes_ptr": (VP, [TP]),
+    "ts_block8_scales_ptr": (VP, [TP]),
+    "ts_block8_unpack": (TP, [TP]),
+    "ts_block8_linear": (TP, [TP, TP, TP, _c.c_int, TP]),
+    "ts_indices_from_slice": (TP, [VP, SZ, _c.POINTER(SZ), SZ]),
+    "ts_indices_from_device": (TP, [VP, _c.POINTER(SZ), SZ, VP, VP]),
+    "ts_indices_free": (None, [TP]),
+    "ts_indices_dims": (SZ, [TP, _c.POINTER(SZ), SZ]),
+    "ts_indices_device_ptr": (VP, [TP]),
+    "ts_tensor_distillation": (TP, [TP, TP, TP, _c.c_float, TP, _c.c_float, TP]),
     "ts_tensor_add_tensor": (TP, [TP, TP]),
     "ts_tensor_sub_tensor": (TP, [TP, TP]),
     "ts_tensor_mul_tensor": (TP, [TP, TP]),

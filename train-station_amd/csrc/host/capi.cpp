@@ -20,6 +20,14 @@ struct ts_packed8 {
     ts::Packed8 p;
 };
 
+struct ts_block8 {
+    ts::Block8 p;
+};
+
+struct ts_indices {
+    ts::Indices i;
+};
+
 struct ts_step_graph {
     std::unique_ptr<ts::StepGraph> g;
 };
@@ -70,6 +78,16 @@ const ts::Tensor &T(const ts_tensor *h) {
 const ts::Packed8 &P(const ts_packed8 *h) {
     if (!h) throw ts::Error("packed handle is NULL");
     return h->p;
+}
+
+const ts::Block8 &B(const ts_block8 *h) {
+    if (!h) throw ts::Error("block8 handle is NULL");
+    return h->p;
+}
+
+const ts::Indices &I(const ts_indices *h) {
+    if (!h) throw ts::Error("indices handle is NULL");
+    return h->i;
 }
 
 const ts::Tensor *optional_tensor(const ts_tensor *h) { return h ? &h->t : nullptr; }
@@ -211,6 +229,88 @@ ts_tensor *ts_packed8_linear(const ts_packed8 *x, const ts_packed8 *weight, cons
                              const ts_tensor *residual) {
     return guard_ptr([&] {
         return wrap(P(x).linear(P(weight), optional_tensor(bias), activation_of(activation), optional_tensor(residual)));
+    });
+}
+
+ts_tensor *ts_tensor_layer_norm(const ts_tensor *x, const ts_tensor *weight, const ts_tensor *bias, float eps) {
+    return guard_ptr([&] { return wrap(T(x).layer_norm(T(weight), optional_tensor(bias), eps)); });
+}
+ts_tensor *ts_tensor_add_layer_norm(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight,
+                                    const ts_tensor *bias, float eps, ts_tensor **h_out) {
+    return guard_ptr([&] {
+        if (!h_out) throw ts::Error("h_out is NULL");
+        auto r = T(x).add_layer_norm(T(residual), T(weight), optional_tensor(bias), eps);
+        std::unique_ptr<ts_tensor> y(wrap(std::move(r.first)));
+        *h_out = wrap(std::move(r.second));
+        return y.release();
+    });
+}
+ts_block8 *ts_tensor_block8(const ts_tensor *x, int tiles) {
+    return guard_ptr([&] { return new ts_block8{T(x).block8(tiles != 0)}; });
+}
+ts_block8 *ts_tensor_layer_norm_block8(const ts_tensor *x, const ts_tensor *residual, const ts_tensor *weight,
+                                       const ts_tensor *bias, float eps, ts_tensor **h_out) {
+    return guard_ptr([&] {
+        if (!residual) return new ts_block8{T(x).layer_norm_block8(T(weight), optional_tensor(bias), eps)};
+        if (!h_out) throw ts::Error("h_out is NULL");
+        auto r = T(x).add_layer_norm_block8(T(residual), T(weight), optional_tensor(bias), eps);
+        std::unique_ptr<ts_block8> p(new ts_block8{std::move(r.first)});
+        *h_out = wrap(std::move(r.second));
+        return p.release();
+    });
+}
+ts_block8 *ts_block8_from_device(uint8_t *codes, float *scales, size_t rows, size_t cols, int tiles, void (*release)(void *),
+                                 void *ctx) {
+    return guard_taking(release, ctx, [&](std::function<void()> give_back) {
+        return new ts_block8{ts::Block8::from_device(codes, scales, rows, cols, tiles != 0, std::move(give_back))};
+    });
+}
+void ts_block8_free(ts_block8 *p) { delete p; }
+size_t ts_block8_rows(const ts_block8 *p) { return p ? p->p.rows() : 0; }
+size_t ts_block8_cols(const ts_block8 *p) { return p ? p->p.cols() : 0; }
+int ts_block8_tiles(const ts_block8 *p) { return p && p->p.tiles() ? 1 : 0; }
+size_t ts_block8_pitch(const ts_block8 *p) { return p ? p->p.pitch() : 0; }
+const uint8_t *ts_block8_codes_ptr(const ts_block8 *p) {
+    return guard_ptr([&] { return static_cast<const uint8_t *>(B(p).codes()); });
+}
+const float *ts_block8_scales_ptr(const ts_block8 *p) {
+    return guard_ptr([&] { return static_cast<const float *>(B(p).scales()); });
+}
+ts_tensor *ts_block8_unpack(const ts_block8 *p) {
+    return guard_ptr([&] { return wrap(B(p).unpack()); });
+}
+ts_tensor *ts_block8_linear(const ts_block8 *x, const ts_block8 *weight, const ts_tensor *bias, int activation,
+                            const ts_tensor *residual) {
+    return guard_ptr([&] {
+        return wrap(B(x).linear(B(weight), optional_tensor(bias), activation_of(activation), optional_tensor(residual)));
+    });
+}
+ts_indices *ts_indices_from_slice(const int32_t *data, size_t len, const size_t *dims, size_t rank) {
+    return guard_ptr([&] {
+        if (len && !data) throw ts::Error("data pointer is NULL");
+        return new ts_indices{ts::Indices::from_slice(data, len, dims_of(dims, rank))};
+    });
+}
+ts_indices *ts_indices_from_device(int32_t *data, const size_t *dims, size_t rank, void (*release)(void *), void *ctx) {
+    return guard_taking(release, ctx, [&](std::function<void()> give_back) {
+        return new ts_indices{ts::Indices::from_device(data, dims_of(dims, rank), std::move(give_back))};
+    });
+}
+void ts_indices_free(ts_indices *i) { delete i; }
+size_t ts_indices_dims(const ts_indices *i, size_t *out, size_t cap) {
+    if (!i) return 0;
+    const auto &d = i->i.dims();
+    for (size_t k = 0; k < d.size() && k < cap; ++k) out[k] = d[k];
+    return d.size();
+}
+const int32_t *ts_indices_device_ptr(const ts_indices *i) {
+    return guard_ptr([&] { return I(i).ptr(); });
+}
+ts_tensor *ts_tensor_distillation(const ts_tensor *logits, const ts_indices *indices, const ts_tensor *teacher,
+                                  float temperature, const ts_indices *labels, float hard, const ts_tensor *weights) {
+    return guard_ptr([&] {
+        return wrap(T(logits).distillation(I(indices), T(teacher), temperature, labels ? &I(labels) : nullptr, hard,
+                                           optional_tensor(weights)));
     });
 }
 

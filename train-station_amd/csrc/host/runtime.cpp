@@ -21,9 +21,10 @@ Runtime::Runtime() {
     check(ts_hip_initialize(), "ts_hip_initialize");
     check(ts_hip_stream_create(&stream_), "ts_hip_stream_create");
     float *w = nullptr;
-    check(ts_hip_malloc(&w, 2), "ts_hip_malloc(zero index)");
+    check(ts_hip_malloc(&w, 4), "ts_hip_malloc(zero index, bad entry)");
     zero_index_ = reinterpret_cast<unsigned long long *>(w);
-    check(ts_hip_memcpy(w, reinterpret_cast<const float *>(&kNoZero), 2, 0), "ts_hip_memcpy");
+    const unsigned long long none[2] = {kNoZero, kNoZero};
+    check(ts_hip_memcpy(w, reinterpret_cast<const float *>(none), 4, 0), "ts_hip_memcpy");
     const float zero = 0.0f;  // all bits 0
     check(ts_hip_malloc(&w, 1), "ts_hip_malloc(ticket)");
     check(ts_hip_memcpy(w, &zero, 1, 0), "ts_hip_memcpy");
@@ -41,16 +42,18 @@ void Runtime::sync() {
         throw Error("a step being recorded cannot wait for or read device results: end the recording first");
     run_division_checks();  // quotients never read still check their divisors
     check(ts_hip_stream_synchronize(stream_), "ts_hip_stream_synchronize");
-    unsigned long long idx = kNoZero;
-    check(ts_hip_memcpy(reinterpret_cast<float *>(&idx),
-                        reinterpret_cast<const float *>(zero_index_), 2, 1),
-          "ts_hip_memcpy");
-    if (idx != kNoZero) {
-        check(ts_hip_memcpy(reinterpret_cast<float *>(zero_index_),
-                            reinterpret_cast<const float *>(&kNoZero), 2, 0),
+    unsigned long long found[2] = {kNoZero, kNoZero};  // zero index, bad entry
+    check(ts_hip_memcpy(reinterpret_cast<float *>(found), reinterpret_cast<const float *>(zero_index_), 4, 1), "ts_hip_memcpy");
+    for (int k = 0; k < 2; ++k) {
+        const unsigned long long at = found[k];
+        if (at == kNoZero) continue;
+        check(ts_hip_memcpy(reinterpret_cast<float *>(zero_index_ + k), reinterpret_cast<const float *>(&kNoZero), 2, 0),
               "ts_hip_memcpy");
         // ops/div.rs:383-416
-        throw Error("Division by zero detected at index " + std::to_string(idx));
+        if (k == 0) throw Error("Division by zero detected at index " + std::to_string(at));
+        const bool label = at >> 63;
+        throw Error("distillation: " + std::string(label ? "the label of row " : "entry ") +
+                    std::to_string(at & ~(1ull << 63)) + " is outside the vocabulary");
     }
 }
 

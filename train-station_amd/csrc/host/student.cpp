@@ -1,0 +1,354 @@
+// A student's operators: layer norm with the residual's addition, values in 8 bits with
+// a 32-bit scale per block of 128 and the layer over them, and the loss against a
+// teacher's top logits (no counterpart in the reference).  Each forward and each
+// backward is one call of ts_hip.h.
+#include <cmath>
+
+#include "ts_hip.h"
+#include "ts_host.h"
+
+namespace ts {
+
+namespace {
+
+void *S() { return Runtime::get().stream(); }
+
+const float *data_of(const Tensor *t) { return t ? t->dev() : nullptr; }
+
+size_t checked_norm(const Tensor &x, const Tensor &weight, const Tensor *bias, const Tensor *residual, float eps) {
+    if (x.dims().empty()) throw Error("layer_norm requires at least 1 dimension, got 0");
+    const size_t cols = x.dims().back();
+    for (const Tensor *t : {&weight, bias})
+        if (t && (t->dims().size() != 1 || t->dims()[0] != cols))
+            throw Error(std::string("layer_norm: ") + (t == bias ? "bias " : "weight ") + dims_str(t->dims()) + " for rows of " +
+                        std::to_string(cols));
+    if (residual && residual->dims() != x.dims())
+        throw Error("layer_norm: residual " + dims_str(residual->dims()) + " added to " + dims_str(x.dims()));
+    if (!(eps >= 0.0f)) throw Error("layer_norm: eps must not be negative");
+    return cols;
+}
+
+void need_matrix(const Tensor &t, const char *what) {
+    if (t.dims().size() != 2) throw Error(std::string(what) + " requires a matrix, got " + dims_str(t.dims()));
+}
+
+std::unique_ptr<Allocation> workspace(size_t floats) {
+    return floats ? std::make_unique<Allocation>(floats) : nullptr;
+}
+
+// y = norm(h), h = x (+ residual): y in full or in 8 bits
+void run_norm(const Tensor &x, const Tensor *residual, const Tensor &weight, const Tensor *bias, float eps, Tensor *h, Tensor *y,
+              Block8 *p) {
+    if (!x.size()) return;
+    const size_t cols = x.dims().back(), rows = x.size() / cols;
+    const float *xp = x.dev(), *rp = data_of(residual), *wp = weight.dev(), *bp = data_of(bias);
+    float *hp = h ? h->dev_mut() : nullptr, *yp = y ? y->dev_mut() : nullptr, *scales = p ? p->scales() : nullptr;
+    uint8_t *codes = p ? p->codes() : nullptr;
+    const double bytes = 4.0 * x.size() * (residual ? 3 : 1) + (p ? 33.0 / 32 : 4.0) * x.size() + 8.0 * cols;
+    launch(KernelClass::Reduction, bytes, "ts_hip_layer_norm", [&] {
+        return p ? ts_hip_layer_norm_block8(xp, rp, wp, bp, rows, cols, eps, hp, codes, scales, S())
+                 : ts_hip_layer_norm(xp, rp, wp, bp, rows, cols, eps, hp, yp, S());
+    });
+}
+
+// the norm's record: of h (its id, its values), weight and bias
+GradFn norm_record(const Tensor &h, const Tensor &weight, const Tensor *bias, float eps) {
+    GradFn fn{GradFn::Kind::LayerNorm};
+    fn.scalar = eps;
+    fn.saved = {h.saved(), weight.saved()};
+    fn.req_left = h.requires_grad();
+    fn.req_right = weight.requires_grad();
+    fn.has_bias = bias != nullptr;
+    fn.req_bias = bias && bias->requires_grad();
+    return fn;
+}
+
+std::vector<size_t> norm_inputs(const Tensor &h, const Tensor &weight, const Tensor *bias) {
+    std::vector<size_t> ids = {h.id(), weight.id()};
+    if (bias) ids.push_back(bias->id());
+    return ids;
+}
+
+std::vector<size_t> sum_inputs(const Tensor &x, const Tensor &residual) {
+    std::vector<size_t> ids;
+    if (x.requires_grad()) ids.push_back(x.id());
+    if (residual.requires_grad()) ids.push_back(residual.id());
+    return ids;
+}
+
+}  // namespace
+
+// ---- layer norm -------------------------------------------------------------------
+
+Tensor Tensor::layer_norm(const Tensor &weight, const Tensor *bias, float eps) const {
+    checked_norm(*this, weight, bias, nullptr, eps);
+    Tensor y = new_uninit(dims_);
+    run_norm(*this, nullptr, weight, bias, eps, nullptr, &y, nullptr);
+    if ((requires_grad_ || weight.requires_grad_ || (bias && bias->requires_grad_)) && is_grad_enabled())
+        record(y, norm_inputs(*this, weight, bias), norm_record(*this, weight, bias, eps));
+    return y;
+}
+
+std::pair<Tensor, Tensor> Tensor::add_layer_norm(const Tensor &residual, const Tensor &weight, const Tensor *bias,
+                                                 float eps) const {
+    checked_norm(*this, weight, bias, &residual, eps);
+    Tensor y = new_uninit(dims_), h = new_uninit(dims_);
+    run_norm(*this, &residual, weight, bias, eps, &h, &y, nullptr);
+    if (is_grad_enabled()) {
+        // the sum, as add_tensor records it
+        if (requires_grad_ || residual.requires_grad_) record(h, sum_inputs(*this, residual), GradFn{GradFn::Kind::Add});
+        if (h.requires_grad_ || weight.requires_grad_ || (bias && bias->requires_grad_))
+            record(y, norm_inputs(h, weight, bias), norm_record(h, weight, bias, eps));
+    }
+    return {std::move(y), std::move(h)};
+}
+
+Block8 Tensor::layer_norm_block8(const Tensor &weight, const Tensor *bias, float eps) const {
+    need_matrix(*this, "layer_norm_block8");
+    checked_norm(*this, weight, bias, nullptr, eps);
+    Block8 p = Block8::new_uninit(dims_[0], dims_[1], false);
+    run_norm(*this, nullptr, weight, bias, eps, nullptr, nullptr, &p);
+    return p;
+}
+
+std::pair<Block8, Tensor> Tensor::add_layer_norm_block8(const Tensor &residual, const Tensor &weight, const Tensor *bias,
+                                                        float eps) const {
+    need_matrix(*this, "add_layer_norm_block8");
+    checked_norm(*this, weight, bias, &residual, eps);
+    Block8 p = Block8::new_uninit(dims_[0], dims_[1], false);
+    Tensor h = new_uninit(dims_);
+    run_norm(*this, &residual, weight, bias, eps, &h, nullptr, &p);
+    if ((requires_grad_ || residual.requires_grad_) && is_grad_enabled())
+        record(h, sum_inputs(*this, residual), GradFn{GradFn::Kind::Add});
+    return {std::move(p), std::move(h)};
+}
+
+std::vector<std::optional<Tensor>> layer_norm_backward(const GradFn &fn, const Tensor &go) {
+    const SavedTensor &h = fn.saved[0], &w = fn.saved[1];
+    const size_t cols = h.dims.back(), rows = cols ? go.size() / cols : 0;
+    Tensor dh, dw, db;
+    if (fn.req_left) dh = Tensor::new_uninit(h.dims);
+    if (fn.req_right) dw = rows ? Tensor::new_uninit(w.dims) : Tensor::zeros(w.dims);
+    if (fn.req_bias) db = rows ? Tensor::new_uninit(w.dims) : Tensor::zeros(w.dims);
+    if (go.size()) {
+        const size_t ws = fn.req_right || fn.req_bias ? ts_hip_layer_norm_backward_workspace_floats(rows, cols) : 0;
+        const auto work = workspace(ws);
+        const float *hp = h.ptr(), *wp = w.ptr(), *gp = go.dev();
+        float *dhp = fn.req_left ? dh.dev_mut() : nullptr, *dwp = fn.req_right ? dw.dev_mut() : nullptr,
+              *dbp = fn.req_bias ? db.dev_mut() : nullptr;
+        launch(KernelClass::Reduction, (fn.req_left ? 12.0 : 8.0) * go.size() + 12.0 * cols, "ts_hip_layer_norm_backward", [&] {
+            return ts_hip_layer_norm_backward(hp, wp, gp, rows, cols, fn.scalar, dhp, dwp, dbp, work ? work->get() : nullptr, ws,
+                                              Runtime::get().ticket(), S());
+        });
+    }
+    std::vector<std::optional<Tensor>> r(2);
+    if (fn.req_left) r[0] = std::move(dh);
+    if (fn.req_right) r[1] = std::move(dw);
+    if (fn.has_bias) r.push_back(fn.req_bias ? std::optional<Tensor>(std::move(db)) : std::nullopt);
+    return r;
+}
+
+// ---- values in 8 bits ---------------------------------------------------------------
+
+size_t Block8::pitch() const { return ts_hip_packed_pitch(cols_); }
+
+Block8 Block8::new_uninit(size_t rows, size_t cols, bool tiles) {
+    Block8 p;
+    p.rows_ = rows;
+    p.cols_ = cols;
+    p.tiles_ = tiles;
+    if (rows && cols) {
+        p.codes_ = std::make_shared<Allocation>(rows * (p.pitch() / 4));
+        p.scales_ = std::make_shared<Allocation>(p.pitch() / 128 * ts_hip_block8_scale_rows(rows, tiles));
+    }
+    return p;
+}
+
+Block8 Block8::from_device(uint8_t *codes, float *scales, size_t rows, size_t cols, bool tiles, std::function<void()> release) {
+    Block8 p;
+    p.rows_ = rows;
+    p.cols_ = cols;
+    p.tiles_ = tiles;
+    if (!rows || !cols) {
+        if (release) release();
+        return p;
+    }
+    const size_t pitch = p.pitch();
+    if (pitch < cols || rows > SIZE_MAX / pitch)
+        throw Error("Block8: [" + std::to_string(rows) + ", " + std::to_string(cols) + "] is larger than any memory");
+    Runtime::get();
+    const size_t nc = rows * pitch, ns = pitch / 128 * ts_hip_block8_scale_rows(rows, tiles);
+    if (reinterpret_cast<uintptr_t>(codes) % 16 || reinterpret_cast<uintptr_t>(scales) % 4)
+        throw Error("Block8: codes must be 16-byte aligned and scales 4-byte aligned");
+    if (!codes || !scales || ts_hip_check_device_range(codes, nc) != TS_HIP_OK ||
+        ts_hip_check_device_range(scales, ns * sizeof(float)) != TS_HIP_OK)
+        throw Error("Block8: the codes and scales of [" + std::to_string(rows) + ", " + std::to_string(cols) +
+                    "] are not each in one allocation of device memory");
+    // one release call for the two buffers
+    std::shared_ptr<void> both(nullptr, [release](void *) {
+        if (release) release();
+    });
+    p.codes_ = std::make_shared<Allocation>(reinterpret_cast<float *>(codes), nc / 4, [both]() mutable { both.reset(); });
+    p.scales_ = std::make_shared<Allocation>(scales, ns, [both]() mutable { both.reset(); });
+    return p;
+}
+
+Block8 Tensor::block8(bool tiles) const {
+    need_matrix(*this, "block8");
+    Block8 p = Block8::new_uninit(dims_[0], dims_[1], tiles);
+    if (size_) {
+        const float *x = dev();
+        launch(KernelClass::Elementwise, 4.0 * size_ + 33.0 / 32 * size_, "ts_hip_block8",
+               [&] { return ts_hip_block8(x, dims_[0], dims_[1], tiles, p.codes(), p.scales(), S()); });
+    }
+    return p;
+}
+
+Tensor Block8::unpack() const {
+    Tensor t = Tensor::new_uninit({rows_, cols_});
+    if (t.size())
+        launch(KernelClass::Elementwise, 4.0 * t.size() + 33.0 / 32 * t.size(), "ts_hip_unblock8",
+               [&] { return ts_hip_unblock8(codes(), scales(), rows_, cols_, tiles_, t.dev_mut(), S()); });
+    return t;
+}
+
+Tensor Block8::linear(const Block8 &weight, const Tensor *bias, Activation act, const Tensor *residual) const {
+    if (tiles_ || !weight.tiles_)
+        throw Error("linear: the input has a scale per row (block8()) and the weight one per 128 rows (block8(tiles))");
+    const std::vector<size_t> od = {rows_, weight.rows_};
+    if (weight.cols_ != cols_)
+        throw Error("Inner dimensions must match: " + std::to_string(cols_) + " vs " + std::to_string(weight.cols_));
+    if (bias && (bias->dims().size() != 1 || bias->dims()[0] != weight.rows_))
+        throw Error("linear: bias " + dims_str(bias->dims()) + " for " + std::to_string(weight.rows_) + " outputs");
+    if (residual && residual->dims() != od)
+        throw Error("linear: residual " + dims_str(residual->dims()) + " added to " + dims_str(od));
+    Tensor y = Tensor::new_uninit(od);
+    if (y.size()) {
+        const size_t ws = ts_hip_linear_block8_workspace_floats(rows_, cols_, weight.rows_);
+        const auto work = workspace(ws);
+        const float *bp = data_of(bias), *rp = data_of(residual);
+        launch(KernelClass::Gemm, 2.0 * rows_ * cols_ * weight.rows_, "ts_hip_linear_block8", [&] {
+            return ts_hip_linear_block8(codes(), scales(), weight.codes(), weight.scales(), rows_, cols_, weight.rows_, bp,
+                                        static_cast<int>(act), rp, y.dev_mut(), work ? work->get() : nullptr, ws, S());
+        });
+    }
+    return y;
+}
+
+// ---- indices ------------------------------------------------------------------------
+
+namespace {
+size_t elements(const std::vector<size_t> &dims) {
+    size_t n = 1;
+    bool some = true;
+    for (size_t d : dims) some = some && d;
+    for (size_t d : dims) {
+        if (some && d > SIZE_MAX / sizeof(int32_t) / n) throw Error("Indices: " + dims_str(dims) + " is larger than any memory");
+        n = some ? n * d : 0;
+    }
+    return n;
+}
+}  // namespace
+
+Indices Indices::from_slice(const int32_t *data, size_t len, std::vector<size_t> dims) {
+    Indices i;
+    i.size_ = elements(dims);
+    if (len != i.size_)
+        throw Error("Data length " + std::to_string(len) + " doesn't match shape " + dims_str(dims) + " (size " +
+                    std::to_string(i.size_) + ")");
+    refuse_while_recording("Indices");
+    i.dims_ = std::move(dims);
+    if (len) {
+        i.alloc_ = std::make_shared<Allocation>(len);
+        check(ts_hip_memcpy_async(i.alloc_->get(), reinterpret_cast<const float *>(data), len, 0, S()), "ts_hip_memcpy_async");
+        check(ts_hip_stream_synchronize(S()), "ts_hip_stream_synchronize");
+    }
+    return i;
+}
+
+Indices Indices::from_device(int32_t *data, std::vector<size_t> dims, std::function<void()> release) {
+    Indices i;
+    i.size_ = elements(dims);
+    i.dims_ = std::move(dims);
+    if (!i.size_) {
+        if (release) release();
+        return i;
+    }
+    Runtime::get();  // a stream to wait for when it is let go
+    if (!data || reinterpret_cast<uintptr_t>(data) % sizeof(int32_t) ||
+        ts_hip_check_device_range(data, i.size_ * sizeof(int32_t)) != TS_HIP_OK)
+        throw Error("Indices: " + dims_str(i.dims_) + " numbers are not in one allocation of device memory");
+    i.alloc_ = std::make_shared<Allocation>(reinterpret_cast<float *>(data), i.size_, std::move(release));
+    return i;
+}
+
+// ---- distillation -----------------------------------------------------------------------
+
+void Distillation::run(const float *go, float *loss, float *dlogits) const {
+    const size_t rows = logits.dims[0], vocab = logits.dims[1], kept = indices.dims()[1];
+    const size_t ws = ts_hip_distillation_workspace_floats(rows, vocab);
+    const auto work = workspace(ws);
+    const float *z = logits.ptr(), *t = teacher.ptr(), *w = weights.ptr();
+    launch(KernelClass::Reduction, (dlogits ? 8.0 : 4.0) * rows * vocab + 8.0 * rows * kept, "ts_hip_distillation", [&] {
+        return ts_hip_distillation(z, rows, vocab, indices.ptr(), t, kept, temperature, labels.ptr(), hard, w, go, loss, dlogits,
+                                   Runtime::get().bad_entry(), work ? work->get() : nullptr, ws, S());
+    });
+}
+
+Tensor Tensor::distillation(const Indices &indices, const Tensor &teacher, float temperature, const Indices *labels, float hard,
+                            const Tensor *weights) const {
+    need_matrix(*this, "distillation");
+    const std::vector<size_t> per_row = {dims_[0]};
+    if (dims_[0] && !dims_[1]) throw Error("distillation: logits " + dims_str(dims_) + " have no columns");
+    if (indices.dims().size() != 2 || indices.dims()[0] != dims_[0])
+        throw Error("distillation: indices " + dims_str(indices.dims()) + " for logits " + dims_str(dims_));
+    if (teacher.dims() != indices.dims())
+        throw Error("distillation: teacher " + dims_str(teacher.dims()) + " for indices " + dims_str(indices.dims()));
+    if (indices.dims()[1] > 1024) throw Error("distillation: at most 1024 of the teacher's logits a row, got " + dims_str(indices.dims()));
+    if (!(temperature >= 1e-18f && temperature <= 1e19f)) throw Error("distillation: the temperature must be positive");
+    if (!(hard >= 0.0f && hard <= 1.0f)) throw Error("distillation: the labels' share must be from 0 to 1");
+    if (hard > 0.0f && !labels) throw Error("distillation: no labels for their share of " + std::to_string(hard));
+    if (labels && labels->dims() != per_row)
+        throw Error("distillation: labels " + dims_str(labels->dims()) + " for logits " + dims_str(dims_));
+    if (weights && weights->dims() != per_row)
+        throw Error("distillation: weights " + dims_str(weights->dims()) + " for logits " + dims_str(dims_));
+    auto d = std::make_shared<Distillation>();
+    d->logits = saved();
+    d->teacher = teacher.saved();
+    if (weights) d->weights = weights->saved();
+    d->indices = indices;
+    if (labels) d->labels = *labels;
+    d->temperature = temperature;
+    d->hard = hard;
+    const bool recorded = requires_grad_ && is_grad_enabled();
+    Tensor loss = new_uninit({1});
+    if (recorded && size_) d->gradient = std::make_shared<Allocation>(size_);
+    d->run(nullptr, loss.dev_mut(), d->gradient ? d->gradient->get() : nullptr);
+    if (recorded) {
+        GradFn fn{GradFn::Kind::Distillation};
+        fn.distillation = std::move(d);
+        record(loss, {id_}, std::move(fn));
+    }
+    return loss;
+}
+
+std::vector<std::optional<Tensor>> distillation_backward(const GradFn &fn, const Tensor &go) {
+    Distillation &d = *fn.distillation;
+    std::vector<std::optional<Tensor>> r(1);
+    const float *one = go.allocation()->map ? go.allocation()->map->constant() : nullptr;
+    if (one && *one == 1.0f && d.gradient) {
+        r[0] = Tensor::from_saved({std::move(d.gradient), d.logits.dims});
+        d.gradient.reset();
+        return r;
+    }
+    d.gradient.reset();
+    Tensor dz = Tensor::new_uninit(d.logits.dims);
+    if (dz.size()) {
+        const Allocation loss(1);  // (computed again beside it)
+        d.run(go.dev(), loss.raw(), dz.dev_mut());
+    }
+    r[0] = std::move(dz);
+    return r;
+}
+
+}  // namespace ts

@@ -2262,6 +2262,10 @@ std::vector<std::optional<Tensor>> GradFn::apply(const Tensor &go) const {
             return rms_norm_backward(*this, go);
         case K::Linear:
             return linear_backward(*this, go);
+        case K::LayerNorm:
+            return layer_norm_backward(*this, go);
+        case K::Distillation:
+            return distillation_backward(*this, go);
         case K::Transpose:  // grad_fn/transforms/transpose.rs: the same two axes swapped back
             r.emplace_back(transposed_value(go, dim0, dim1, false));
             break;

@@ -50,10 +50,13 @@ class Runtime {
     static Runtime &get();
     void *stream() const { return stream_; }
     unsigned long long *zero_index() const { return zero_index_; }
+    // the same for entries outside a vocabulary (ts_hip_distillation)
+    unsigned long long *bad_entry() const { return zero_index_ + 1; }
     // a device word that is zero between the launches that count in it
     unsigned *ticket() const { return ticket_; }
     // Waits for queued work; throws the reference's division-by-zero panic
-    // message if a division kernel recorded a zero divisor.
+    // message if a division kernel recorded a zero divisor, or that an index
+    // was outside the vocabulary.
     void sync();
 
   private:
@@ -420,6 +423,9 @@ void launch(KernelClass k, double work, const char *what, F &&f) {
 
 class Tensor;
 class Packed8;
+class Block8;
+class Indices;
+struct Distillation;
 
 // Activations of Tensor::linear (TS_HIP_ACT_*)
 enum class Activation : int { None = 0, Relu = 1, Silu = 2, GeluTanh = 3 };
@@ -440,7 +446,7 @@ struct GradFn {
         Add, Sub, Mul, Div, AddScalar, SubScalar, MulScalar, DivScalar,
         Relu, PowScalar, MatMul, ReduceSum, ReduceMean,
         Exp, Log, Sqrt, Tanh, Sigmoid, LeakyRelu, Softmax, ReduceSumDims, ReduceMeanDims,
-        Transpose, Contiguous, RmsNorm, Linear
+        Transpose, Contiguous, RmsNorm, Linear, LayerNorm, Distillation
     };
     explicit GradFn(Kind k) : kind(k) {}
     Kind kind;
@@ -460,6 +466,7 @@ struct GradFn {
     Activation activation = Activation::None;
     std::shared_ptr<Packed8> checkpoint;
     bool has_bias = false, has_residual = false, req_bias = false, req_residual = false;
+    std::shared_ptr<Distillation> distillation;
 
     // GradFn::apply (grad_fn/mod.rs:490-789): gradients by operand position.
     std::vector<std::optional<Tensor>> apply(const Tensor &grad_output) const;
@@ -570,6 +577,19 @@ class Tensor {
     Tensor linear(const Tensor &weight, const Tensor *bias, Activation act, const Tensor *residual,
                   Checkpoint checkpoint) const;
     Packed8 pack8() const;
+    // A student's operators (student.cpp; no counterpart in the reference): layer norm
+    // over the last axis, (h - mean) / sqrt(var + eps) * weight + bias; its values in 8
+    // bits; and the loss of logits, this tensor, against a teacher's and the labels.
+    Tensor layer_norm(const Tensor &weight, const Tensor *bias, float eps) const;
+    std::pair<Tensor, Tensor> add_layer_norm(const Tensor &residual, const Tensor &weight, const Tensor *bias,
+                                             float eps) const;  // y, h
+    // y in 8 bits (no gradient passes through it)
+    Block8 layer_norm_block8(const Tensor &weight, const Tensor *bias, float eps) const;
+    std::pair<Block8, Tensor> add_layer_norm_block8(const Tensor &residual, const Tensor &weight, const Tensor *bias,
+                                                    float eps) const;
+    Block8 block8(bool tiles) const;
+    Tensor distillation(const Indices &indices, const Tensor &teacher, float temperature, const Indices *labels, float hard,
+                        const Tensor *weights) const;
     // transform/transpose.rs:156-291, contiguous.rs:123-157: a transposed
     // view (deferred copy, see PendingTranspose), t() = the last two axes;
     // contiguous() of a view is its copy, of anything else a clone; both
@@ -628,12 +648,68 @@ class Packed8 {
     size_t rows_ = 0, cols_ = 0;
 };
 
+// A matrix in 8 bits with a 32-bit scale per 128 columns of a row or, as tiles, of 128
+// rows (the layout: ts_hip.h, ts_hip_block8).
+class Block8 {
+  public:
+    static Block8 new_uninit(size_t rows, size_t cols, bool tiles);
+    // a caller's codes [rows, pitch] and scales [pitch / 128, scale rows] on the device
+    static Block8 from_device(uint8_t *codes, float *scales, size_t rows, size_t cols, bool tiles,
+                              std::function<void()> release);
+    size_t rows() const { return rows_; }
+    size_t cols() const { return cols_; }
+    bool tiles() const { return tiles_; }
+    size_t pitch() const;
+    uint8_t *codes() const { return codes_ ? reinterpret_cast<uint8_t *>(codes_->get()) : nullptr; }
+    float *scales() const { return scales_ ? scales_->get() : nullptr; }
+    // the values that the codes stand for
+    Tensor unpack() const;
+    // act(self weight^T + bias) + residual, weight [fan_out, fan_in] in tiles
+    Tensor linear(const Block8 &weight, const Tensor *bias, Activation act, const Tensor *residual) const;
+
+  private:
+    std::shared_ptr<Allocation> codes_, scales_;
+    size_t rows_ = 0, cols_ = 0;
+    bool tiles_ = false;
+};
+
+// Whole numbers on the device, 32 bits each: columns of a vocabulary.
+class Indices {
+  public:
+    static Indices from_slice(const int32_t *data, size_t len, std::vector<size_t> dims);
+    // over a caller's device memory (row-major, not copied)
+    static Indices from_device(int32_t *data, std::vector<size_t> dims, std::function<void()> release);
+    const std::vector<size_t> &dims() const { return dims_; }
+    size_t size() const { return size_; }
+    const int32_t *ptr() const { return alloc_ ? reinterpret_cast<const int32_t *>(alloc_->get()) : nullptr; }
+
+  private:
+    std::shared_ptr<Allocation> alloc_;
+    std::vector<size_t> dims_;
+    size_t size_ = 0;
+};
+
+// What a loss against a teacher keeps: its inputs, and the logits' gradient of a
+// loss whose own is one, computed with the loss and given to the first backward
+// pass that asks for just that.  Any other computes it again.
+struct Distillation {
+    SavedTensor logits, teacher, weights;
+    Indices indices, labels;
+    float temperature = 1.0f, hard = 0.0f;
+    std::shared_ptr<Allocation> gradient;
+    // the loss into `loss` and, unless null, its gradient (times *go, unless null) into dlogits
+    void run(const float *go, float *loss, float *dlogits) const;
+};
+
 // A gradient just stored on a tensor: noted where it stands in a caller's memory (engine.cpp).
 void note_lent_gradient(const std::shared_ptr<Tensor> &g);
 
 // The gradients of Kind::RmsNorm and Kind::Linear (feedforward.cpp).
 std::vector<std::optional<Tensor>> rms_norm_backward(const GradFn &fn, const Tensor &go);
 std::vector<std::optional<Tensor>> linear_backward(const GradFn &fn, const Tensor &go);
+// The gradients of Kind::LayerNorm and Kind::Distillation (student.cpp).
+std::vector<std::optional<Tensor>> layer_norm_backward(const GradFn &fn, const Tensor &go);
+std::vector<std::optional<Tensor>> distillation_backward(const GradFn &fn, const Tensor &go);
 
 // x with axes d0 != d1 swapped, deferred (no recording): a deferred bare
 // matrix product becomes the product of its swapped operands; a pending view

@@ -1,0 +1,501 @@
+// A student's loss against a teacher's top logits and the true labels, with the gradient
+// of every logit (ts_hip.h, ts_hip_distillation).
+//
+// Of a row z, with c = log2(e) / T:
+//   M = max(z),  S = sum of 2^(c (z - M)),  p = 2^(c (z - M)) / S   (and the same at T = 1: s)
+//   teacher: b = max(t),  e_k = 2^(c (t_k - b)),  A = sum e_k,  q_k = e_k / A
+//   KL = sum q_k ((t_k - b) - (z_k - M)) / T + ln S - ln A
+//   loss = w ((1 - a) T^2 KL + a (ln S1 + M - z_label))
+//   dz_j = w ((1 - a) T (p_j - q_j) + a (s_j - [j = label]))
+//
+// A row is held in registers by W waves, four neighbouring columns a lane and NV such
+// quads, so that it is read once for the loss and its gradients; each lane sums against
+// its own largest, and one exchange joins lanes and waves.  Longer rows are passed over
+// with a running largest, the last columns stay, and the others are read again, from the
+// caches as long as the rows on their way fit there.  Rows too few to fill the chip are
+// shared out by segments of columns, by two launches.  The teacher's entries and the
+// label have a thread each: it adds their term to its part of the loss, and stores the
+// gradient there after the others are stored (an index given twice: the first entry's,
+// with both).  Sums past a lane are f64.
+#include <type_traits>
+
+#include "ts_hip_internal.h"
+
+namespace tship {
+
+namespace {
+
+typedef float df4_t __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr float kLog2e = 1.44269504f;
+constexpr float kNone = -__builtin_inff();
+
+struct DistillArgs {
+    const float *logits, *teacher, *weights, *go;
+    const int *indices, *labels;  // labels null: none (hard is 0 then)
+    float *dlogits;               // null: the loss alone
+    double *row_loss;             // each workgroup's part of the loss
+    unsigned long long *bad;      // the smallest number of an entry outside the vocabulary
+    size_t rows, vocab;
+    int kept;
+    float temperature, c;  // c = log2(e) / temperature
+    float soft, hard;      // 1 - a, a
+    // segments
+    float4 *parts;  // [rows][segments]: a segment's largest and its sums
+    int segments;
+};
+
+__device__ __forceinline__ float pow2_of(float v, float from, float c) { return __builtin_amdgcn_exp2f((v - from) * c); }
+__device__ __forceinline__ float wave_max(float m) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    return m;
+}
+// where to count from: anything, where there is nothing but -inf
+__device__ __forceinline__ float origin(float largest) { return largest == kNone ? 0.0f : largest; }
+// a sum against `from` in terms of `to`
+__device__ __forceinline__ double rebased(double s, float from, float to, float c) {
+    return from == kNone ? 0.0 : s * pow2_of(from, to, c);
+}
+
+// What is known of a row: the softmax's M and S (and S1), the teacher's b and A.
+struct RowSums {
+    float m, b;
+    double s, s1, a;
+};
+
+// Sums of lanes joined to a wave's (in every lane).
+template <bool TWO>
+__device__ __forceinline__ void join_lanes(RowSums &r, float c) {
+    const float m = wave_max(r.m);
+    r.s = wave_sum(rebased(r.s, r.m, m, c));
+    if (TWO) r.s1 = wave_sum(rebased(r.s1, r.m, m, kLog2e));
+    r.m = m;
+}
+__device__ __forceinline__ void join_teacher(RowSums &r, float c) {
+    const float b = wave_max(r.b);
+    r.a = wave_sum(rebased(r.a, r.b, b, c));
+    r.b = b;
+}
+// ... and waves' to the row's.
+template <bool TWO, int W>
+__device__ __forceinline__ void join_waves(RowSums &r, RowSums *lds, float c) {
+    if (W == 1) return;
+    __syncthreads();  // the last row's reads
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = r;
+    __syncthreads();
+    RowSums all = {kNone, kNone, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        all.m = fmaxf(all.m, lds[w].m);
+        all.b = fmaxf(all.b, lds[w].b);
+    }
+#pragma unroll 4
+    for (int w = 0; w < W; ++w) {
+        const RowSums one = lds[w];
+        all.s += rebased(one.s, one.m, all.m, c);
+        if (TWO) all.s1 += rebased(one.s1, one.m, all.m, kLog2e);
+        all.a += rebased(one.a, one.b, all.b, c);
+    }
+    r = all;
+}
+
+// A row's share of the loss and its gradients' coefficients: zero where it has none.
+struct RowShare {
+    float weight, soft, hard;  // weight; (1 - a) T, a
+    int label;
+};
+
+// The entries of a row: the teacher's kept ones, then the label.  -1: none.
+__device__ __forceinline__ int entry_at(const DistillArgs &g, const int *indices, const RowShare &share, int k) {
+    const int j = k < g.kept ? indices[k] : share.label;
+    return j >= 0 && static_cast<size_t>(j) < g.vocab ? j : -1;
+}
+
+// The teacher's entries first + 0, + step, ... of a row, as a lane's sums (f64).
+__device__ __forceinline__ void teacher_sums(const DistillArgs &g, size_t row, int first, int step, RowSums &r) {
+    const size_t at = row * g.kept;
+    for (int k = first; k < g.kept; k += step) {
+        const int j = g.indices[at + k];
+        if (j < 0) continue;
+        if (static_cast<size_t>(j) >= g.vocab) {
+            atomicMin(g.bad, static_cast<unsigned long long>(at + k));
+            continue;
+        }
+        const float t = g.teacher[at + k];
+        if (t == kNone) continue;
+        const float b = fmaxf(r.b, t);
+        r.a = rebased(r.a, r.b, b, g.c) + pow2_of(t, b, g.c);  // (a NaN stays)
+        r.b = b;
+    }
+}
+
+__device__ __forceinline__ RowShare row_share(const DistillArgs &g, size_t row) {
+    RowShare s = {g.weights ? g.weights[row] : static_cast<float>(1.0 / static_cast<double>(g.rows)), g.soft * g.temperature,
+                  0.0f, -1};
+    if (g.labels) {
+        s.label = g.labels[row];
+        if (s.label >= 0 && static_cast<size_t>(s.label) >= g.vocab) {
+            if ((threadIdx.x & 63) == 0) atomicMin(g.bad, (1ull << 63) | row);
+            s.label = -1;
+        }
+        if (s.label >= 0) s.hard = g.hard;
+    }
+    return s;
+}
+
+// dz of a logit but for what its entries take: by_p 2^(c (z - M)) + by_s 2^(log2(e) (z - M))
+struct Gradient {
+    float m, by_p, by_s;
+    bool none;  // nothing is asked of the row: zeros, whatever it holds
+    template <bool TWO>
+    __device__ __forceinline__ float at(float z, float c) const {
+        const float p = by_p * pow2_of(z, m, c);
+        return TWO ? p + by_s * pow2_of(z, m, kLog2e) : p;
+    }
+};
+template <bool TWO>
+__device__ __forceinline__ Gradient gradient(const RowShare &share, const RowSums &r, float weight) {
+    const double soft = r.a != 0.0 ? static_cast<double>(weight) * share.soft : 0.0, hard = static_cast<double>(weight) * share.hard;
+    const bool none = soft == 0.0 && hard == 0.0;
+    if (TWO)
+        return {r.m, soft == 0.0 ? 0.0f : static_cast<float>(soft / r.s), hard == 0.0 ? 0.0f : static_cast<float>(hard / r.s1), none};
+    return {r.m, static_cast<float>((soft + hard) / r.s), 0.0f, none};
+}
+
+// The entries of a row in columns from .. to, by threads first + 0, + step, ...: their
+// terms of the loss (the result; first 0 adds what is the row's own, where `own`), and
+// the gradients there.
+template <bool TWO>
+__device__ __forceinline__ double entries(const DistillArgs &g, size_t row, const RowShare &share, const RowSums &r,
+                                          const Gradient &by, float weight, int first, int step, size_t from, size_t to, bool own) {
+    const size_t at = row * g.kept;
+    const float *z = g.logits + row * g.vocab;
+    const bool asked = share.soft != 0.0f && r.a != 0.0;
+    const double per_e = asked ? static_cast<double>(share.soft) / r.a : 0.0;
+    double loss = 0.0;
+    if (first == 0 && own && asked) loss = static_cast<double>(share.soft) * g.temperature * (log(r.s) - log(r.a));
+    auto takes = [&](int k) {  // of the gradient there, without its weight
+        if (k == g.kept) return static_cast<double>(share.hard);
+        return asked ? per_e * pow2_of(g.teacher[at + k], r.b, g.c) : 0.0;
+    };
+    for (int k = first; k <= g.kept; k += step) {
+        const int j = entry_at(g, g.indices + at, share, k);
+        if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
+        double sum = takes(k);
+        const float zj = z[j];
+        if (k == g.kept) loss += sum * (log(TWO ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
+        else if (sum != 0.0)
+            loss += sum * ((static_cast<double>(g.teacher[at + k]) - r.b) - (static_cast<double>(zj) - r.m));
+        if (!g.dlogits) continue;
+        bool mine = true;  // the first entry of an index stores, with the later ones' shares
+        for (int other = 0; other <= g.kept; ++other) {  // (uniform: scalar loads)
+            if (other == k || entry_at(g, g.indices + at, share, other) != j) continue;
+            if (other < k) mine = false;
+            else sum += takes(other);
+        }
+        if (mine) g.dlogits[row * g.vocab + j] = by.at<TWO>(zj, g.c) - static_cast<float>(weight * sum);
+    }
+    return loss * share.weight;
+}
+
+// The sum of a workgroup's losses, in a fixed order, to its place.
+template <int T>
+__device__ __forceinline__ void store_loss(double loss, double *to) {
+    __shared__ double waves[T / 64];
+    loss = wave_sum(loss);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = loss;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = 0.0;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) all += waves[w];
+        *to = all;
+    }
+}
+
+__device__ __forceinline__ void load_quad(const float *p, size_t c, size_t n, float (&v)[4], float past) {
+    if (c + 4 <= n) {
+        const df4_t q = *reinterpret_cast<const df4_t *>(p + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < n ? p[c + e] : past;
+    }
+}
+__device__ __forceinline__ void store_quad(float *p, size_t c, size_t n, const float (&v)[4]) {
+    if (c + 4 <= n) {
+        *reinterpret_cast<df4_t *>(p + c) = df4_t{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < n) p[c + e] = v[e];
+    }
+}
+
+template <int W>
+constexpr int kThreads = W < 4 ? 256 : 64 * W;
+template <int W>
+constexpr int kRows = kThreads<W> / (64 * W);  // rows of a workgroup
+
+// NV quads' sums added to a lane's.
+template <bool TWO, int NV>
+__device__ __forceinline__ void add_quads(const float (&v)[NV][4], float c, RowSums &r) {
+    float m = r.m;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, v[i][e]);
+    const float from = origin(m);
+    float s = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s += pow2_of(v[i][e], from, c);
+            if (TWO) s1 += pow2_of(v[i][e], from, kLog2e);
+        }
+    r.s = rebased(r.s, r.m, m, c) + s;
+    if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + s1;
+    r.m = m;
+}
+
+// A row per W waves, rows in turn over the grid.  LONG: more columns than the waves hold.
+template <int W, int NV, bool TWO, bool LONG>
+__global__ __launch_bounds__(kThreads<W>) void distill_rows(DistillArgs g) {
+    constexpr int RPB = kRows<W>;
+    __shared__ RowSums lds[W > 1 ? W : 1];
+    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W, t = threadIdx.x % (64 * W);
+    const size_t span = static_cast<size_t>(256) * W * NV, step = static_cast<size_t>(gridDim.x) * RPB;
+    const float go = g.go ? *g.go : 1.0f;
+    double loss = 0.0;
+    for (size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot; row < g.rows; row += step) {  // (W > 1: uniform)
+        const RowShare share = row_share(g, row);
+        const float *z = g.logits + row * g.vocab;
+        float *dz = g.dlogits ? g.dlogits + row * g.vocab : nullptr;
+        RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
+        float v[NV][4];
+        auto fetch = [&](size_t c0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load_quad(z, c0 + 4 * (t + 64 * W * i), g.vocab, v[i], kNone);
+        };
+        const size_t last = LONG ? (g.vocab - 1) / span * span : 0;  // the first of the columns held
+        if (share.weight != 0.0f) {
+            fetch(0);
+            if (share.soft != 0.0f) teacher_sums(g, row, t, 64 * W, r);
+            add_quads<TWO, NV>(v, g.c, r);
+            if (LONG) {
+                for (size_t c0 = span; c0 < g.vocab; c0 += span) {
+                    fetch(c0);
+                    add_quads<TWO, NV>(v, g.c, r);
+                }
+            }
+            join_lanes<TWO>(r, g.c);
+            join_teacher(r, g.c);
+            join_waves<TWO, W>(r, lds, g.c);
+        }
+        const float weight = share.weight * go;
+        Gradient by = {0.0f, 0.0f, 0.0f, true};
+        if (share.weight != 0.0f) by = gradient<TWO>(share, r, weight);
+        for (size_t c0 = last; dz;) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const size_t c = c0 + 4 * (t + 64 * W * i);
+                if (c >= g.vocab) continue;
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = by.none ? 0.0f : by.at<TWO>(v[i][e], g.c);
+                store_quad(dz, c, g.vocab, o);
+            }
+            if (!LONG || c0 == 0) break;
+            c0 -= span;
+            if (!by.none) fetch(c0);
+        }
+        if (by.none) continue;  // (uniform over the row's waves)
+        if (W > 1 && dz) __syncthreads();  // the entries' gradients are stored after the others
+        loss += entries<TWO>(g, row, share, r, by, weight, t, 64 * W, 0, g.vocab, true);
+    }
+    store_loss<kThreads<W>>(loss, g.row_loss + blockIdx.x);
+}
+
+// ---- rows by segments ------------------------------------------------------------------
+
+constexpr int kSegWaves = 4, kSegQuads = 4, kSegment = 256 * kSegWaves * kSegQuads;  // columns
+
+template <bool TWO>
+__global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillArgs g) {
+    __shared__ RowSums lds[kSegWaves];
+    const size_t row = blockIdx.x / g.segments, c0 = blockIdx.x % g.segments * static_cast<size_t>(kSegment);
+    RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
+    float v[kSegQuads][4];
+#pragma unroll
+    for (int i = 0; i < kSegQuads; ++i)
+        load_quad(g.logits + row * g.vocab, c0 + 4 * (threadIdx.x + 64 * kSegWaves * i), g.vocab, v[i], kNone);
+    add_quads<TWO, kSegQuads>(v, g.c, r);
+    join_lanes<TWO>(r, g.c);
+    join_waves<TWO, kSegWaves>(r, lds, g.c);
+    if (threadIdx.x == 0) g.parts[blockIdx.x] = make_float4(r.m, static_cast<float>(r.s), static_cast<float>(r.s1), 0.0f);
+}
+
+template <bool TWO>
+__global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g) {
+    __shared__ RowSums lds[kSegWaves];
+    constexpr int T = 64 * kSegWaves;
+    const size_t row = blockIdx.x / g.segments, segment = blockIdx.x % g.segments, c0 = segment * kSegment;
+    const int t = threadIdx.x;
+    const RowShare share = row_share(g, row);
+    const float *z = g.logits + row * g.vocab;
+    const bool asked = share.weight != 0.0f;
+    float v[kSegQuads][4];
+    RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
+    if (asked) {
+        if (g.dlogits) {
+#pragma unroll
+            for (int i = 0; i < kSegQuads; ++i) load_quad(z, c0 + 4 * (t + T * i), g.vocab, v[i], kNone);
+        }
+        for (int k = t; k < g.segments; k += T) {
+            const float4 one = g.parts[row * g.segments + k];
+            const float m = fmaxf(r.m, one.x);
+            r.s = rebased(r.s, r.m, m, g.c) + rebased(one.y, one.x, m, g.c);
+            if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + rebased(one.z, one.x, m, kLog2e);
+            r.m = m;
+        }
+        if (share.soft != 0.0f) teacher_sums(g, row, t, T, r);
+        join_lanes<TWO>(r, g.c);
+        join_teacher(r, g.c);
+        join_waves<TWO, kSegWaves>(r, lds, g.c);
+    }
+    const float weight = share.weight * (g.go ? *g.go : 1.0f);
+    Gradient by = {0.0f, 0.0f, 0.0f, true};
+    if (asked) by = gradient<TWO>(share, r, weight);
+#pragma unroll
+    for (int i = 0; i < kSegQuads; ++i) {
+        const size_t c = c0 + 4 * (t + T * i);
+        if (!g.dlogits || c >= g.vocab) continue;
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = by.none ? 0.0f : by.at<TWO>(v[i][e], g.c);
+        store_quad(g.dlogits + row * g.vocab, c, g.vocab, o);
+    }
+    double loss = 0.0;
+    if (!by.none) {  // (uniform)
+        __syncthreads();  // the entries' gradients are stored after the others
+        loss = entries<TWO>(g, row, share, r, by, weight, t, T, c0, c0 + kSegment, segment == 0);
+    }
+    store_loss<T>(loss, g.row_loss + blockIdx.x);
+}
+
+__global__ __launch_bounds__(kBlock) void sum_losses(const double *parts, size_t n, float *loss) {
+    double s = 0.0;
+    for (size_t i = threadIdx.x; i < n; i += kBlock) s += parts[i];
+    s = block_sum(s);
+    if (threadIdx.x == 0) *loss = static_cast<float>(s);
+}
+
+// ---- launches ------------------------------------------------------------------------------
+
+// Calls f(W, NV, LONG as constants) for rows of n columns: the waves that hold them.
+template <class F>
+void for_vocab(size_t n, F &&f) {
+    using std::integral_constant;
+    const integral_constant<bool, false> held{};
+    if (n <= 256) f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, held);
+    else if (n <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 2>{}, held);
+    else if (n <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 4>{}, held);
+    else if (n <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 4>{}, held);
+    else if (n <= 8192) f(integral_constant<int, 4>{}, integral_constant<int, 8>{}, held);
+    else if (n <= 16384) f(integral_constant<int, 8>{}, integral_constant<int, 8>{}, held);
+    else if (n <= 32768) f(integral_constant<int, 16>{}, integral_constant<int, 8>{}, held);
+    else if (n <= 65536) f(integral_constant<int, 16>{}, integral_constant<int, 16>{}, held);
+    else f(integral_constant<int, 16>{}, integral_constant<int, 16>{}, integral_constant<bool, true>{});
+}
+
+size_t waves_for(size_t vocab) { return vocab <= 1024 ? 1 : vocab <= 8192 ? 4 : vocab <= 16384 ? 8 : 16; }
+
+bool by_segments(size_t rows, size_t vocab) { return vocab > 4096 && rows * 2 <= static_cast<size_t>(device_cu_count()); }
+
+// Workgroups of distill_rows: twice what runs at once
+size_t row_blocks(size_t rows, size_t vocab) {
+    const size_t w = waves_for(vocab), per = w < 4 ? 4 / w : 1, need = (rows + per - 1) / per;
+    const size_t cap = static_cast<size_t>(device_cu_count()) * 2 * (32 / (w < 4 ? 4 : w));
+    return need < cap ? need : cap;
+}
+
+size_t segments_of(size_t vocab) { return (vocab + kSegment - 1) / kSegment; }
+
+constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 30, kMaxRows = size_t(1) << 31;
+
+}  // namespace
+
+}  // namespace tship
+
+using namespace tship;
+
+extern "C" {
+
+size_t ts_hip_distillation_workspace_floats(size_t rows, size_t vocab) {
+    if (!rows || !vocab) return 0;
+    if (by_segments(rows, vocab)) return 6 * rows * segments_of(vocab);  // sums, losses
+    return 2 * row_blocks(rows, vocab);
+}
+
+int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const int32_t *indices, const float *teacher, size_t kept,
+                        float temperature, const int32_t *labels, float hard, const float *weights, const float *go, float *loss,
+                        float *dlogits, unsigned long long *bad, float *workspace, size_t workspace_floats, void *stream) {
+    const double t = temperature;
+    if (!(t > 0.0) || !(t * t <= 3e38) || !(t * t >= 1e-36) || !(hard >= 0.0f && hard <= 1.0f) || kept > kMaxKept || vocab > kMaxVocab ||
+        rows >= kMaxRows || (hard > 0.0f && !labels && rows))
+        return TS_HIP_EINVAL;
+    if (!loss) return TS_HIP_EINVAL;
+    if (!rows || !vocab) return ts_hip_fill(loss, 0.0f, 1, stream);
+    if (!logits || !bad || (kept && (!indices || !teacher))) return TS_HIP_EINVAL;
+    if (!workspace || workspace_floats < ts_hip_distillation_workspace_floats(rows, vocab)) return TS_HIP_EWORKSPACE;
+    // with nothing asked of the teacher there is one softmax, at 1
+    if (hard == 1.0f) temperature = 1.0f;
+    const bool two = hard > 0.0f && temperature != 1.0f;
+    DistillArgs g = {};
+    g.logits = logits;
+    g.teacher = teacher;
+    g.weights = weights;
+    g.go = go;
+    g.indices = indices;
+    g.labels = hard > 0.0f ? labels : nullptr;
+    g.dlogits = dlogits;
+    g.bad = bad;
+    g.rows = rows;
+    g.vocab = vocab;
+    g.kept = static_cast<int>(kept);
+    g.temperature = temperature;
+    g.c = static_cast<float>(1.4426950408889634 / static_cast<double>(temperature));
+    g.soft = 1.0f - hard;
+    g.hard = hard;
+    const hipStream_t s = as_stream(stream);
+    size_t parts;
+    if (by_segments(rows, vocab)) {
+        g.segments = static_cast<int>(segments_of(vocab));
+        g.parts = reinterpret_cast<float4 *>(workspace);
+        g.row_loss = reinterpret_cast<double *>(workspace + 4 * rows * g.segments);
+        const dim3 grid(static_cast<unsigned>(rows * g.segments)), block(64 * kSegWaves);
+        if (two) {
+            launch(distill_segment_sums<true>, grid, block, 0, s, g);
+            launch(distill_segments<true>, grid, block, 0, s, g);
+        } else {
+            launch(distill_segment_sums<false>, grid, block, 0, s, g);
+            launch(distill_segments<false>, grid, block, 0, s, g);
+        }
+        parts = rows * g.segments;
+    } else {
+        g.row_loss = reinterpret_cast<double *>(workspace);
+        parts = row_blocks(rows, vocab);
+        for_vocab(vocab, [&](auto w, auto nv, auto lng) {
+            const dim3 grid(static_cast<unsigned>(parts)), block(kThreads<w.value>);
+            if (two) launch((distill_rows<w.value, nv.value, true, lng.value>), grid, block, 0, s, g);
+            else launch((distill_rows<w.value, nv.value, false, lng.value>), grid, block, 0, s, g);
+        });
+    }
+    launch(sum_losses, dim3(1), dim3(kBlock), 0, s, static_cast<const double *>(g.row_loss), parts, loss);
+    return launch_status();
+}
+
+}  // extern "C"

@@ -1,0 +1,303 @@
+// Values in 8 bits with a 32-bit scale per block of 128 columns: packing, unpacking and
+// a layer over them (ts_hip.h, ts_hip_block8 and the entries after it).
+//
+//   y[i][j] = act(sum over blocks g of sx[g][i] sw[g][j / 128] P[g] + bias[j]) + residual[i][j]
+//   P[g] = the sum over g's 128 columns k of x[i][k] W[j][k], of the codes' values
+//
+// P is summed from zero by the bf16 instructions, whose operands hold a code's value and
+// whose sums are fp32 (the 8-bit instructions drop what is 2^-13 below the largest of
+// eight products: ts_hip_linear_packed.hip), and joined to y by one fused multiply-add
+// with the two scales' product.
+#include "ts_hip_block8.h"
+#include "ts_hip_linear.h"
+
+namespace tship {
+
+namespace {
+
+typedef unsigned u4_t __attribute__((ext_vector_type(4)));
+
+// ---- packing -----------------------------------------------------------------------
+
+__device__ __forceinline__ void read4(const float *row, size_t c, size_t cols, float (&v)[4]) {
+    if (c + 4 <= cols) {
+        const pk4u_t q = *reinterpret_cast<const pk4u_t *>(row + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? row[c + e] : 0.0f;
+    }
+}
+
+// A scale per row: a thread packs a quad, a grid stride over all quads (32 lanes a block).
+__global__ __launch_bounds__(kBlock) void block8_rows(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
+                                                      uint8_t *__restrict__ codes, float *__restrict__ scales) {
+    const size_t quads = pitch / 4, total = rows * quads;  // a multiple of 32
+    const size_t stride = static_cast<size_t>(gridDim.x) * kBlock;
+    for (size_t q = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; q < total; q += stride) {
+        const size_t row = q / quads, c = 4 * (q % quads);
+        float v[4];
+        read4(x + row * cols, c, cols, v);
+        block8_store(v, c, codes + row * pitch, scales + row, rows);
+    }
+}
+
+// A scale per 128 rows: a workgroup a block, a thread every eighth row's quad.
+__global__ __launch_bounds__(kBlock) void block8_tiles(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
+                                                       uint8_t *__restrict__ codes, float *__restrict__ scales) {
+    __shared__ float lds[kBlock / 64];
+    const size_t groups = pitch / kPackGroup, tiles = (rows + kPackGroup - 1) / kPackGroup;
+    for (size_t b = blockIdx.x; b < groups * tiles; b += gridDim.x) {
+        const size_t row0 = b / groups * kPackGroup + threadIdx.x / 32, c = b % groups * kPackGroup + threadIdx.x % 32 * 4;
+        float v[16][4], m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const size_t row = row0 + 8 * i;
+            if (row < rows) {
+                read4(x + row * cols, c, cols, v[i]);
+                m = fmaxf(m, largest4(v[i]));
+            }
+        }
+        m = half_wave_max(m);
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+        __syncthreads();
+        const Block8Scale s = block8_scale(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])));
+        __syncthreads();  // (the next block's)
+        if (threadIdx.x == 0) scales[b % groups * tiles + b / groups] = s.scale;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const size_t row = row0 + 8 * i;
+            if (row < rows) *reinterpret_cast<unsigned *>(codes + row * pitch + c) = pack4(v[i], s.inv);
+        }
+    }
+}
+
+__global__ __launch_bounds__(kBlock) void block8_values(const uint8_t *__restrict__ codes, const float *__restrict__ scales,
+                                                        size_t rows, size_t cols, size_t pitch, size_t high,
+                                                        float *__restrict__ out) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const size_t quads = (cols + 3) / 4, total = rows * quads, scale_rows = (rows + high - 1) / high;
+    const size_t stride = static_cast<size_t>(gridDim.x) * kBlock;
+    for (size_t q = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; q < total; q += stride) {
+        const size_t row = q / quads, c = 4 * (q % quads);
+        const int code = *reinterpret_cast<const int *>(codes + row * pitch + c);
+        const float s = scales[c / kPackGroup * scale_rows + row / high];
+        const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(code, true);
+        const float v[4] = {lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+        if (c + 4 <= cols) {
+            *reinterpret_cast<pk4u_t *>(out + row * cols + c) = pk4u_t{v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < cols) out[row * cols + c + e] = v[e];
+        }
+    }
+}
+
+// ---- few rows ------------------------------------------------------------------------
+
+struct Block8Product {
+    const uint8_t *xc, *wc;
+    const float *xs, *ws;
+    const float *bias, *residual;
+    float *y;
+    int M, N, groups, act;  // groups of 128 k
+    int tiles_n;
+};
+
+// A wave has FN blocks of 16 columns and FM of 16 rows, W's rows as the instruction's A
+// operand, so that a lane ends with four neighbouring columns of one row; KG waves share K.
+template <int FN, int FM, int KG>
+__global__ __launch_bounds__(64 * KG) void block8_direct(Block8Product p) {
+    const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int j0 = static_cast<int>(blockIdx.x) % p.tiles_n * 16 * FN, i0 = static_cast<int>(blockIdx.x) / p.tiles_n * 16 * FM;
+    const size_t pitch = static_cast<size_t>(p.groups) * kPackGroup;
+    const int w_tiles = (p.N + kPackGroup - 1) / kPackGroup;
+    f4v_t acc[FN][FM] = {};
+    const uint8_t *wp[FN], *xp[FM];
+    const float *wsp[FN], *xsp[FM];
+#pragma unroll
+    for (int a = 0; a < FN; ++a) {  // rows past an edge: the last one's, not stored
+        wp[a] = p.wc + min(j0 + 16 * a + li, p.N - 1) * pitch + 32 * lq;
+        wsp[a] = p.ws + min(j0 + 16 * a, p.N - 1) / kPackGroup;
+    }
+#pragma unroll
+    for (int b = 0; b < FM; ++b) {
+        const int i = min(i0 + 16 * b + li, p.M - 1);
+        xp[b] = p.xc + i * pitch + 32 * lq;
+        xsp[b] = p.xs + i;
+    }
+    constexpr int U = FN * FM == 1 ? 4 : 2;  // groups whose loads are issued before the first is used
+    for (int g0 = group; g0 < p.groups; g0 += KG * U) {
+        u4_t w[U][FN][2], x[U][FM][2];
+        float wk[U][FN], xk[U][FM];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int g = min(g0 + u * KG, p.groups - 1);  // (past the last: read again, not used)
+            const size_t at = static_cast<size_t>(g) * kPackGroup;
+#pragma unroll
+            for (int a = 0; a < FN; ++a) {
+                const u4_t *q = reinterpret_cast<const u4_t *>(wp[a] + at);
+                w[u][a][0] = q[0];
+                w[u][a][1] = q[1];
+                wk[u][a] = wsp[a][static_cast<size_t>(g) * w_tiles];
+            }
+#pragma unroll
+            for (int b = 0; b < FM; ++b) {
+                const u4_t *q = reinterpret_cast<const u4_t *>(xp[b] + at);
+                x[u][b][0] = q[0];
+                x[u][b][1] = q[1];
+                xk[u][b] = xsp[b][static_cast<size_t>(g) * p.M];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (g0 + u * KG >= p.groups) break;  // uniform
+            f4v_t part[FN][FM] = {};
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {  // eight of the lane's 32 k at a time
+                bf8_t fw[FN], fx[FM];
+#pragma unroll
+                for (int a = 0; a < FN; ++a) fw[a] = widen(w[u][a][h >> 1][2 * (h & 1)], w[u][a][h >> 1][2 * (h & 1) + 1], 1.0f);
+#pragma unroll
+                for (int b = 0; b < FM; ++b) fx[b] = widen(x[u][b][h >> 1][2 * (h & 1)], x[u][b][h >> 1][2 * (h & 1) + 1], 1.0f);
+#pragma unroll
+                for (int a = 0; a < FN; ++a)
+#pragma unroll
+                    for (int b = 0; b < FM; ++b)
+                        part[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[a], fx[b], part[a][b], 0, 0, 0);
+            }
+#pragma unroll
+            for (int a = 0; a < FN; ++a)
+#pragma unroll
+                for (int b = 0; b < FM; ++b) {
+                    const float s = wk[u][a] * xk[u][b];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[a][b][r] = __builtin_fmaf(part[a][b][r], s, acc[a][b][r]);
+                }
+        }
+    }
+    // lane (li, lq), register r of block (a, b): column 16 a + 4 lq + r of row 16 b + li
+    if constexpr (KG > 1) {
+        __shared__ f4v_t sums[KG - 1][FN * FM][64];
+        if (group > 0) {
+#pragma unroll
+            for (int n = 0; n < FN * FM; ++n) sums[group - 1][n][lane] = acc[n / FM][n % FM];
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+            for (int n = 0; n < FN * FM; ++n) acc[n / FM][n % FM] += sums[g][n][lane];
+    }
+#pragma unroll
+    for (int a = 0; a < FN; ++a) {
+        const int j = j0 + 16 * a + 4 * lq, cols = min(4, p.N - j);
+        if (cols <= 0) continue;
+        float bias[4] = {};
+        if (p.bias) read4(p.bias, j, p.N, bias);
+#pragma unroll
+        for (int b = 0; b < FM; ++b) {
+            const int i = i0 + 16 * b + li;
+            if (i >= p.M) continue;
+            const size_t at = static_cast<size_t>(i) * p.N;
+            float extra[4] = {}, o[4];
+            if (p.residual) read4(p.residual + at, j, p.N, extra);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = acc[a][b][r], slope;
+                if (p.bias) v += bias[r];
+                v = activate<false>(v, p.act, slope);
+                if (p.residual) v += extra[r];
+                o[r] = v;
+            }
+            if (cols == 4) {
+                *reinterpret_cast<pk4u_t *>(p.y + at + j) = pk4u_t{o[0], o[1], o[2], o[3]};
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r < cols) p.y[at + j + r] = o[r];
+            }
+        }
+    }
+}
+
+template <int FN, int FM, int KG>
+void launch_direct(Block8Product p, hipStream_t s) {
+    p.tiles_n = (p.N + 16 * FN - 1) / (16 * FN);
+    const size_t tiles = static_cast<size_t>(p.tiles_n) * ((p.M + 16 * FM - 1) / (16 * FM));
+    launch((block8_direct<FN, FM, KG>), dim3(static_cast<unsigned>(tiles)), dim3(64 * KG), 0, s, p);
+}
+
+template <int FN, int FM>
+void launch_direct(const Block8Product &p, hipStream_t s) {
+    const size_t tiles = static_cast<size_t>((p.N + 16 * FN - 1) / (16 * FN)) * ((p.M + 16 * FM - 1) / (16 * FM));
+    const size_t waves = static_cast<size_t>(device_cu_count()) * 16;
+    int kg = 1;
+    while (kg < 8 && tiles * kg * 2 <= waves && kg * 2 <= p.groups) kg *= 2;
+    if (kg == 8) launch_direct<FN, FM, 8>(p, s);
+    else if (kg == 4) launch_direct<FN, FM, 4>(p, s);
+    else if (kg == 2) launch_direct<FN, FM, 2>(p, s);
+    else launch_direct<FN, FM, 1>(p, s);
+}
+
+constexpr size_t kMaxTileBlocks = size_t(1) << 20;  // more blocks take turns
+
+}  // namespace
+
+}  // namespace tship
+
+using namespace tship;
+
+extern "C" {
+
+size_t ts_hip_block8_scale_rows(size_t rows, int tiles) { return tiles ? (rows + kPackGroup - 1) / kPackGroup : rows; }
+
+int ts_hip_block8(const float *x, size_t rows, size_t cols, int tiles, uint8_t *codes, float *scales, void *stream) {
+    if (rows == 0 || cols == 0) return TS_HIP_OK;
+    if (!x || !codes || !scales) return TS_HIP_EINVAL;
+    const size_t pitch = packed_pitch(cols);
+    if (tiles) {
+        const size_t blocks = pitch / kPackGroup * ts_hip_block8_scale_rows(rows, 1);
+        launch(block8_tiles, dim3(static_cast<unsigned>(blocks < kMaxTileBlocks ? blocks : kMaxTileBlocks)), dim3(kBlock), 0,
+               as_stream(stream), x, rows, cols, pitch, codes, scales);
+    } else {
+        launch(block8_rows, dim3(grid_for(rows * pitch / 4)), dim3(kBlock), 0, as_stream(stream), x, rows, cols, pitch, codes,
+               scales);
+    }
+    return launch_status();
+}
+
+int ts_hip_unblock8(const uint8_t *codes, const float *scales, size_t rows, size_t cols, int tiles, float *out, void *stream) {
+    if (rows == 0 || cols == 0) return TS_HIP_OK;
+    if (!codes || !scales || !out) return TS_HIP_EINVAL;
+    launch(block8_values, dim3(grid_for(rows * ((cols + 3) / 4))), dim3(kBlock), 0, as_stream(stream), codes, scales, rows, cols,
+           packed_pitch(cols), tiles ? static_cast<size_t>(kPackGroup) : static_cast<size_t>(1), out);
+    return launch_status();
+}
+
+size_t ts_hip_linear_block8_workspace_floats(size_t, size_t, size_t) { return 0; }
+
+int ts_hip_linear_block8(const uint8_t *x_codes, const float *x_scales, const uint8_t *w_codes, const float *w_scales,
+                         size_t batch, size_t fan_in, size_t fan_out, const float *bias, int act, const float *residual,
+                         float *y, float *workspace, size_t workspace_floats, void *stream) {
+    const size_t lim = size_t(1) << 24;
+    if (batch >= lim || fan_in >= lim || fan_out >= lim || batch * fan_out >= size_t(1) << 34 || act < TS_HIP_ACT_NONE ||
+        act > TS_HIP_ACT_GELU_TANH)
+        return TS_HIP_EINVAL;
+    if (batch == 0 || fan_out == 0) return TS_HIP_OK;
+    if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;
+    if (workspace_floats < ts_hip_linear_block8_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
+    const Block8Product p = {x_codes, w_codes, x_scales, w_scales, bias, residual, y, static_cast<int>(batch),
+                             static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0};
+    (void)workspace;
+    if (batch <= 16) launch_direct<1, 1>(p, as_stream(stream));
+    else launch_direct<2, 2>(p, as_stream(stream));
+    return launch_status();
+}
+
+}  // extern "C"

@@ -272,6 +272,50 @@ class Tensor:
         """The matrix in 8 bits."""
         return _wrap_packed(_G.ts_tensor_pack8(self._h))
 
+    # -- a student's operators (include/ts_gradtrack.h) -----------------------------
+    def layer_norm(self, weight: "Tensor", bias: Optional["Tensor"] = None, eps: float = 1e-5) -> "Tensor":
+        """(self - mean) / sqrt(var + eps) * weight + bias over the last axis."""
+        return _wrap(_G.ts_tensor_layer_norm(self._h, weight._h, _optional(bias), eps))
+
+    def add_layer_norm(self, residual: "Tensor", weight: "Tensor", bias: Optional["Tensor"] = None, eps: float = 1e-5):
+        """(layer_norm(h), h) of h = self + residual, in one pass."""
+        h = ctypes.c_void_p()
+        y = _wrap(_G.ts_tensor_add_layer_norm(self._h, residual._h, weight._h, _optional(bias), eps, ctypes.byref(h)))
+        return y, Tensor(h.value)
+
+    def layer_norm_block8(self, weight: "Tensor", bias: Optional["Tensor"] = None, eps: float = 1e-5) -> "Block8":
+        """layer_norm of a matrix, in 8 bits: what layer_norm(...).block8() gives."""
+        return _wrap_block8(_G.ts_tensor_layer_norm_block8(self._h, None, weight._h, _optional(bias), eps, None))
+
+    def add_layer_norm_block8(self, residual: "Tensor", weight: "Tensor", bias: Optional["Tensor"] = None,
+                              eps: float = 1e-5):
+        """(layer_norm(h) in 8 bits, h) of the matrix h = self + residual, in one pass."""
+        h = ctypes.c_void_p()
+        p = _wrap_block8(_G.ts_tensor_layer_norm_block8(self._h, residual._h, weight._h, _optional(bias), eps,
+                                                        ctypes.byref(h)))
+        return p, Tensor(h.value)
+
+    def block8(self, tiles: bool = False) -> "Block8":
+        """The matrix in 8 bits with a scale for each 128 columns of a row (an input),
+        or, as tiles, of 128 rows (a weight)."""
+        return _wrap_block8(_G.ts_tensor_block8(self._h, int(bool(tiles))))
+
+    def distillation(self, indices: "Indices", teacher: "Tensor", temperature: float = 1.0,
+                     labels: Optional["Indices"] = None, hard: float = 0.0, weights: Optional["Tensor"] = None) -> "Tensor":
+        """The loss of these logits [rows, vocab] against a teacher's top logits, at
+        ``indices`` [rows, kept] (at most 1024; below 0: no entry):
+
+            sum over rows of w ((1 - hard) T^2 KL(q, p) - hard log s[label])
+
+        with q the softmax of the row's teacher / T over its entries, p that of the
+        logits / T over all columns and s that of the logits.  labels [rows]: below 0 is
+        none; weights [rows]: 1 / rows each without.  A row of weight 0, or without
+        entries and label, adds nothing and gets a gradient of 0, whatever it holds.
+        The gradient goes to these logits alone and is computed with the loss.  An index
+        or a label outside the vocabulary raises at the next synchronisation."""
+        return _wrap(_G.ts_tensor_distillation(self._h, indices._h, teacher._h, temperature, _optional(labels), hard,
+                                               _optional(weights)))
+
     # -- tensor/ops/{exp,log,sqrt,tanh,sigmoid,leaky_relu,softmax}.rs -------------
     def exp(self) -> "Tensor":
         return _wrap(_G.ts_tensor_exp(self._h))
@@ -470,6 +514,122 @@ class Packed8:
 
     def __repr__(self) -> str:
         return f"Packed8(shape={list(self.shape)})"
+
+
+def _wrap_block8(handle) -> "Block8":
+    if not handle:
+        raise TsError(last_error() or "native call returned no block8 matrix")
+    return Block8(handle)
+
+
+class Block8:
+    """Handle on a matrix in 8 bits with a 32-bit scale for each block of 128 columns:
+    e4m3 codes [rows, pitch] and scales [pitch / 128, rows], or, as tiles, [pitch / 128,
+    rows / 128 rounded up] (include/ts_hip.h, ts_hip_block8)."""
+
+    __slots__ = ("_h",)
+
+    def __init__(self, handle):
+        self._h = ctypes.c_void_p(handle)
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            _G.ts_block8_free(h)
+            self._h = None
+
+    @staticmethod
+    def from_device(codes, scales, cols: int, tiles: bool = False) -> "Block8":
+        """Over a caller's device arrays, codes uint8 [rows, pitch] and scales float32
+        as the class says, as Tensor.from_device."""
+        (cp, cshape), (sp, sshape) = _device_array(codes, "|u1", False), _device_array(scales, "<f4", False)
+        pitch = -(-int(cols) // 128) * 128
+        rows = -(-cshape[0] // 128) if tiles and cshape else (cshape[0] if cshape else 0)
+        if cols < 0 or len(cshape) != 2 or cshape[1] != pitch or sshape != (pitch // 128, rows):
+            raise TsError(f"Block8: codes {list(cshape)} and scales {list(sshape)} for {cols} columns")
+        return _wrap_block8(_G.ts_block8_from_device(cp, sp, cshape[0], int(cols), int(bool(tiles)), _give_back,
+                                                     _lend((codes, scales))))
+
+    @property
+    def shape(self) -> tuple:
+        return int(_G.ts_block8_rows(self._h)), int(_G.ts_block8_cols(self._h))
+
+    @property
+    def tiles(self) -> bool:
+        return bool(_G.ts_block8_tiles(self._h))
+
+    @property
+    def pitch(self) -> int:
+        return int(_G.ts_block8_pitch(self._h))
+
+    def codes_ptr(self) -> int:
+        return int(_G.ts_block8_codes_ptr(self._h) or 0)
+
+    def scales_ptr(self) -> int:
+        return int(_G.ts_block8_scales_ptr(self._h) or 0)
+
+    def unpack(self) -> Tensor:
+        """The values that the codes stand for."""
+        return _wrap(_G.ts_block8_unpack(self._h))
+
+    def linear(self, weight: "Block8", bias: Optional[Tensor] = None, activation: str = "none",
+               residual: Optional[Tensor] = None) -> Tensor:
+        """act(self weight^T + bias) + residual, weight [fan_out, fan_in] in tiles."""
+        return _wrap(_G.ts_block8_linear(self._h, weight._h, _optional(bias), _activation(activation),
+                                         _optional(residual)))
+
+    def __repr__(self) -> str:
+        return f"Block8(shape={list(self.shape)}, tiles={self.tiles})"
+
+
+class Indices:
+    """Handle on whole numbers on the device, 32 bits each."""
+
+    __slots__ = ("_h",)
+
+    def __init__(self, handle):
+        if not handle:
+            raise TsError(last_error() or "native call returned no indices")
+        self._h = ctypes.c_void_p(handle)
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            _G.ts_indices_free(h)
+            self._h = None
+
+    @staticmethod
+    def from_slice(data, shape: Sequence[int]) -> "Indices":
+        a = np.asarray(data).reshape(-1)
+        if a.size and a.dtype.kind not in "iu":
+            raise TsError(f"Indices: values of type {a.dtype}, not whole numbers")
+        if a.size and (a.min() < -(1 << 31) or a.max() >= 1 << 31):
+            raise TsError("Indices: a value does not fit 32 bits")
+        a = np.ascontiguousarray(a, dtype=np.int32)
+        d, r = _dims(shape)
+        return Indices(_G.ts_indices_from_slice(a.ctypes.data, a.size, d, r))
+
+    @staticmethod
+    def from_device(array) -> "Indices":
+        """Over the memory of a contiguous int32 device array, as Tensor.from_device."""
+        ptr, shape = _device_array(array, "<i4", False)
+        d, r = _dims(shape)
+        return Indices(_G.ts_indices_from_device(ptr, d, r, _give_back, _lend(array)))
+
+    @property
+    def shape(self) -> tuple:
+        out = _Dims8()
+        rank = _G.ts_indices_dims(self._h, out, 8)
+        if rank > 8:
+            out = (SZ * rank)()
+            _G.ts_indices_dims(self._h, out, rank)
+        return tuple(out[:rank])
+
+    def device_ptr(self) -> int:
+        return int(_G.ts_indices_device_ptr(self._h) or 0)
+
+    def __repr__(self) -> str:
+        return f"Indices(shape={list(self.shape)})"
 
 
 def _handles(params: Iterable[Tensor]):
