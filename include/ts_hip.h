@@ -669,9 +669,10 @@ int ts_hip_linear_backward(const ts_hip_linear_shape *shape, const float *x, con
  *   codes  [rows][pitch] bytes, 16-byte aligned
  *   scales [pitch / 128][ts_hip_block8_scale_rows(rows, tiles)] floats: of a row's 128
  *          columns (tiles 0: an input), or of 128 rows' (tiles 1: a weight)
- * A block's scale is its largest magnitude, held to 2^-100 .. 448 2^119, over 448; its
- * codes are its values times 1 / scale, rounded to the nearest (ties to even, past 448:
- * 448).  A NaN gets a NaN code (of either sign) and is left out of its block's largest. */
+ * A block's scale is its largest magnitude, held to 2^-100 .. 448 2^119, over 448, rounded
+ * to fp32; its codes are its values times 448 / largest (in f64), rounded to the nearest
+ * (ties to even, past 448: 448).  A NaN gets a NaN code (of either sign) and is left out
+ * of its block's largest. */
 size_t ts_hip_block8_scale_rows(size_t rows, int tiles);
 int ts_hip_block8(const float *x, size_t rows, size_t cols, int tiles, uint8_t *codes, float *scales, void *stream);
 /* out [rows, cols]: the values that the codes stand for, rounded to fp32 */
@@ -692,7 +693,8 @@ int ts_hip_linear_block8(const uint8_t *x_codes, const float *x_scales, const ui
  * bias may be NULL.  Mean and variance are taken in f64.  h may be x or residual. */
 int ts_hip_layer_norm(const float *x, const float *residual, const float *weight, const float *bias, size_t rows, size_t cols,
                       float eps, float *h, float *y, void *stream);
-/* The same with y in 8 bits, a scale per row and 128 columns: ts_hip_block8 of y. */
+/* The same with y in 8 bits, a scale per row and 128 columns (as ts_hip_block8 of y, y
+ * taken in f64 before its rounding to fp32). */
 int ts_hip_layer_norm_block8(const float *x, const float *residual, const float *weight, const float *bias, size_t rows,
                              size_t cols, float eps, float *h, uint8_t *codes, float *scales, void *stream);
 /* The gradients from go = dy, with u = (h - mean(h)) r, r = 1 / sqrt(var + eps) and g = go weight:

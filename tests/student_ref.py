@@ -1,13 +1,12 @@
-"""A student's operators in plain numpy: what their tests compare with, in 64 bits
-but for packing, which is fp32's own.  Values in 8 bits follow include/ts_hip.h
-(ts_hip_block8)."""
+"""A student's operators in plain numpy, 64 bits: what their tests compare with.
+Values in 8 bits follow include/ts_hip.h (ts_hip_block8)."""
 from __future__ import annotations
 
 import numpy as np
 
 from feedforward_ref import U, act, e4m3_values, pitch_of
 
-LEAST, MOST = np.float32(2.0 ** -100), np.float32(448 * 2.0 ** 119)
+LEAST, MOST = 2.0 ** -100, 448 * 2.0 ** 119
 
 
 def scale_rows(rows, tiles):
@@ -15,18 +14,16 @@ def scale_rows(rows, tiles):
 
 
 def block8(x, tiles=False):
-    """(codes [rows, pitch], scales [pitch / 128, scale rows]) of fp32 values."""
-    x = np.asarray(x, np.float32)
+    """(codes [rows, pitch], scales [pitch / 128, scale rows]) of x, taken as 64 bits."""
+    x = np.asarray(x, np.float64)
     rows, cols = x.shape
     high = 128 if tiles else 1
-    pad = np.zeros((scale_rows(rows, tiles) * high, pitch_of(cols)), np.float32)
+    pad = np.zeros((scale_rows(rows, tiles) * high, pitch_of(cols)))
     pad[:rows, :cols] = x
     b = pad.reshape(pad.shape[0] // high, high, -1, 128)
-    top = np.max(np.where(np.isnan(b), np.float32(0), np.abs(b)), axis=(1, 3))
-    scale = np.clip(top, LEAST, MOST) / np.float32(448)
-    inv = np.float32(1) / scale
-    with np.errstate(over="ignore"):
-        q = np.clip(b * inv[:, None, :, None], np.float32(-448), np.float32(448)).astype(np.float64)  # (NaN stays)
+    top = np.clip(np.max(np.where(np.isnan(b), 0.0, np.abs(b)), axis=(1, 3)), LEAST, MOST)
+    scale = (top / 448).astype(np.float32)
+    q = np.clip(b * (448 / top)[:, None, :, None], -448, 448)  # (NaN stays)
     a = np.where(np.isnan(q), 1.0, np.abs(q))
     step = 2.0 ** (np.floor(np.log2(np.maximum(a, 2.0 ** -6))) - 3)
     codes = np.searchsorted(e4m3_values()[:127], np.minimum(np.rint(a / step) * step, 448.0))

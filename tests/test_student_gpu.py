@@ -300,18 +300,18 @@ def test_layer_norm_backward_with_and_without_a_ticket(rows, cols):
 
 @pytest.mark.parametrize("rows,cols", NORMS)
 @pytest.mark.parametrize("residual,bias", [(False, False), (True, True)])
-def test_layer_norm_block8_is_block8_of_layer_norm(rows, cols, residual, bias):
+def test_layer_norm_block8(rows, cols, residual, bias):
     x, r, w, b, h = norm_case(rows, cols, residual, bias)
     X, W, B = tensor(x), tensor(w), tensor(b) if bias else None
     if residual:
         p, stream = X.add_layer_norm_block8(tensor(r), W, B)
         assert np.array_equal(stream.data(), h)
-        y = X.add_layer_norm(tensor(r), W, B)[0]
     else:
-        p, y = X.layer_norm_block8(W, B), X.layer_norm(W, B)
+        p = X.layer_norm_block8(W, B)
     codes, scales = parts(p)
-    want = R.block8(y.data())
-    assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
+    want = R.block8(R.layer_norm(h, w, b, EPS))
+    # (a row of one column and no bias is 0 / sqrt(eps): the mean's last bit is of no size)
+    assert np.allclose(scales, want[1], rtol=2 * R.U, atol=0) and np.array_equal(codes, want[0])
 
 
 def test_layer_norm_block8_pads_rows_of_nan_with_zeros():

@@ -115,7 +115,8 @@ __global__ __launch_bounds__(kNormThreads<W>) void layer_norm_rows(LayerNormArgs
         } while (LONG && c0 < a.cols);
         row_sum<W, 2>(s, lds + slot * 2 * W);
         const double cols = static_cast<double>(a.cols), mean_d = s[0] / cols;
-        const RowNorm n = row_norm(shift, mean_d, row_r(mean_d, s[1] / cols, a.eps));
+        const double r = row_r(mean_d, s[1] / cols, a.eps), mean = shift + mean_d;
+        const RowNorm n = row_norm(shift, mean_d, r);
         c0 = 0;
         do {
             if (LONG) {
@@ -127,15 +128,16 @@ __global__ __launch_bounds__(kNormThreads<W>) void layer_norm_rows(LayerNormArgs
                 const size_t c = c0 + 4 * (t + 64 * W * i);
                 if (c >= end) continue;
                 if (RES) store4(a.h + base, c, a.cols, v[i]);
-                float o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(n.unit(v[i][e]), w[i][e], b[i][e]);
-                if (PACK) {
+                if constexpr (PACK) {  // in f64: a code takes the side of its border that y itself is on
+                    double o[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (c + e >= a.cols) o[e] = 0.0f;
+                        o[e] = c + e < a.cols ? __builtin_fma((v[i][e] - mean) * r, static_cast<double>(w[i][e]), static_cast<double>(b[i][e])) : 0.0;
                     block8_store(o, c, a.codes + row * a.pitch, a.scales + row, a.rows);
                 } else {
+                    float o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(n.unit(v[i][e]), w[i][e], b[i][e]);
                     store4(a.y + base, c, a.cols, o);
                 }
             }

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kBlock) void block8_tiles(const float *__restrict__
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const size_t row = row0 + 8 * i;
-            if (row < rows) *reinterpret_cast<unsigned *>(codes + row * pitch + c) = pack4(v[i], s.inv);
+            if (row < rows) *reinterpret_cast<unsigned *>(codes + row * pitch + c) = block8_codes(v[i], s.inv);
         }
     }
 }

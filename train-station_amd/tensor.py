@@ -284,7 +284,7 @@ class Tensor:
         return y, Tensor(h.value)
 
     def layer_norm_block8(self, weight: "Tensor", bias: Optional["Tensor"] = None, eps: float = 1e-5) -> "Block8":
-        """layer_norm of a matrix, in 8 bits: what layer_norm(...).block8() gives."""
+        """layer_norm of a matrix, in 8 bits."""
         return _wrap_block8(_G.ts_tensor_layer_norm_block8(self._h, None, weight._h, _optional(bias), eps, None))
 
     def add_layer_norm_block8(self, residual: "Tensor", weight: "Tensor", bias: Optional["Tensor"] = None,
