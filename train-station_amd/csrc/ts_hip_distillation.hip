@@ -106,28 +106,40 @@ struct RowShare {
     int label;
 };
 
-// The entries of a row: the teacher's kept ones, then the label.  -1: none.
-__device__ __forceinline__ int entry_at(const DistillArgs &g, const int *indices, const RowShare &share, int k) {
-    const int j = k < g.kept ? indices[k] : share.label;
-    return j >= 0 && static_cast<size_t>(j) < g.vocab ? j : -1;
-}
+// The entries of a row are the teacher's, then the label; -1: none.  A thread's first is
+// kept from the sums to its gradient, and the columns of all are in LDS from then on.
+struct Entry {
+    int j;
+    float t;
+};
+constexpr int kEntries = 1028;  // a row's, and what fills four
 
 // The teacher's entries first + 0, + step, ... of a row, as a lane's sums (f64).
-__device__ __forceinline__ void teacher_sums(const DistillArgs &g, size_t row, int first, int step, RowSums &r) {
+__device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, const RowShare &share, int first, int step,
+                                              RowSums &r, int *columns) {
     const size_t at = row * g.kept;
-    for (int k = first; k < g.kept; k += step) {
-        const int j = g.indices[at + k];
-        if (j < 0) continue;
-        if (static_cast<size_t>(j) >= g.vocab) {
-            atomicMin(g.bad, static_cast<unsigned long long>(at + k));
-            continue;
+    Entry mine = {-1, kNone};
+    for (int k = first; k < (g.kept + 4) / 4 * 4; k += step) {
+        Entry e = {-1, kNone};
+        if (k < g.kept && share.soft != 0.0f) {
+            e = {g.indices[at + k], g.teacher[at + k]};
+            if (e.j >= 0 && static_cast<size_t>(e.j) >= g.vocab) {
+                atomicMin(g.bad, static_cast<unsigned long long>(at + k));
+                e.j = -1;
+            }
+            if (e.j < 0) e = {-1, kNone};
+            if (e.t != kNone) {
+                const float b = fmaxf(r.b, e.t);
+                r.a = rebased(r.a, r.b, b, g.c) + pow2_of(e.t, b, g.c);  // (a NaN stays)
+                r.b = b;
+            }
+        } else if (k == g.kept) {
+            e.j = share.label;
         }
-        const float t = g.teacher[at + k];
-        if (t == kNone) continue;
-        const float b = fmaxf(r.b, t);
-        r.a = rebased(r.a, r.b, b, g.c) + pow2_of(t, b, g.c);  // (a NaN stays)
-        r.b = b;
+        columns[k] = e.j;
+        if (k == first) mine = e;
     }
+    return mine;
 }
 
 __device__ __forceinline__ RowShare row_share(const DistillArgs &g, size_t row) {
@@ -163,36 +175,56 @@ __device__ __forceinline__ Gradient gradient(const RowShare &share, const RowSum
     return {r.m, static_cast<float>((soft + hard) / r.s), 0.0f, none};
 }
 
+// ln x of a sum: its power of two in f64, and the rest, from 3/4 to 3/2, by the fp32
+// instruction, within 2^-24 or so
+__device__ __forceinline__ double ln(double x) {
+    int e;
+    double f = frexp(x, &e);  // [1/2, 1)
+    if (f < 0.75) {
+        f *= 2.0;
+        --e;
+    }
+    return 0.6931471805599453 * (e + static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(f))));
+}
+
 // The entries of a row in columns from .. to, by threads first + 0, + step, ...: their
 // terms of the loss (the result; first 0 adds what is the row's own, where `own`), and
 // the gradients there.
 template <bool TWO>
 __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, const RowShare &share, const RowSums &r,
-                                          const Gradient &by, float weight, int first, int step, size_t from, size_t to, bool own) {
+                                          const Gradient &by, float weight, const Entry &kept, const int *columns, int first,
+                                          int step, size_t from, size_t to, bool own) {
     const size_t at = row * g.kept;
     const float *z = g.logits + row * g.vocab;
     const bool asked = share.soft != 0.0f && r.a != 0.0;
     const double per_e = asked ? static_cast<double>(share.soft) / r.a : 0.0;
     double loss = 0.0;
-    if (first == 0 && own && asked) loss = static_cast<double>(share.soft) * g.temperature * (log(r.s) - log(r.a));
-    auto takes = [&](int k) {  // of the gradient there, without its weight
+    if (first == 0 && own && asked) loss = static_cast<double>(share.soft) * g.temperature * (ln(r.s) - ln(r.a));
+    auto takes = [&](int k, float t) {  // of the gradient there, without its weight
         if (k == g.kept) return static_cast<double>(share.hard);
-        return asked ? per_e * pow2_of(g.teacher[at + k], r.b, g.c) : 0.0;
+        return asked ? per_e * pow2_of(t, r.b, g.c) : 0.0;
     };
     for (int k = first; k <= g.kept; k += step) {
-        const int j = entry_at(g, g.indices + at, share, k);
+        const int j = k == first ? kept.j : columns[k];
         if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
-        double sum = takes(k);
-        const float zj = z[j];
-        if (k == g.kept) loss += sum * (log(TWO ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
-        else if (sum != 0.0)
-            loss += sum * ((static_cast<double>(g.teacher[at + k]) - r.b) - (static_cast<double>(zj) - r.m));
+        const float t = k == g.kept ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = z[j];
+        double sum = takes(k, t);
+        if (k == g.kept) loss += sum * (ln(TWO ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
+        else if (sum != 0.0) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
         if (!g.dlogits) continue;
-        bool mine = true;  // the first entry of an index stores, with the later ones' shares
-        for (int other = 0; other <= g.kept; ++other) {  // (uniform: scalar loads)
-            if (other == k || entry_at(g, g.indices + at, share, other) != j) continue;
-            if (other < k) mine = false;
-            else sum += takes(other);
+        int same = 0;  // entries of this column
+#pragma unroll 2
+        for (int other = 0; other <= g.kept; other += 4) {
+            const int4 four = *reinterpret_cast<const int4 *>(columns + other);
+            same += (four.x == j) + (four.y == j) + (four.z == j) + (four.w == j);
+        }
+        bool mine = true;  // the first of them stores, with the later ones' shares
+        if (same > 1) {
+            for (int other = 0; other <= g.kept; ++other) {
+                if (other == k || columns[other] != j) continue;
+                if (other < k) mine = false;
+                else sum += takes(other, other == g.kept ? 0.0f : g.teacher[at + other]);
+            }
         }
         if (mine) g.dlogits[row * g.vocab + j] = by.at<TWO>(zj, g.c) - static_cast<float>(weight * sum);
     }
@@ -214,24 +246,37 @@ __device__ __forceinline__ void store_loss(double loss, double *to) {
     }
 }
 
-__device__ __forceinline__ void load_quad(const float *p, size_t c, size_t n, float (&v)[4], float past) {
-    if (c + 4 <= n) {
-        const df4_t q = *reinterpret_cast<const df4_t *>(p + c);
+// The quads c0 + 4 (t + T i) of a row of n columns (a uniform pointer and a lane's 32-bit
+// offset in bytes), -inf where there are none.  The one to three columns past the last
+// quad are lanes 0 .. 2's: tail_column.
+template <int T, int NV>
+__device__ __forceinline__ void load_quads(const float *row, unsigned n, unsigned c0, unsigned t, float (&v)[NV][4]) {
+    const char *p = reinterpret_cast<const char *>(row);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = q[e];
-    } else {
+    for (int i = 0; i < NV; ++i) {
+        const unsigned c = c0 + 4 * T * i + 4 * t;
+        df4_t q = {kNone, kNone, kNone, kNone};
+        if (c0 + 4 * T * (i + 1) <= n) q = *reinterpret_cast<const df4_t *>(p + 4 * c);  // uniform
+        else if (c + 4 <= n) q = *reinterpret_cast<const df4_t *>(p + 4 * c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c + e < n ? p[c + e] : past;
+        for (int e = 0; e < 4; ++e) v[i][e] = q[e];
     }
 }
-__device__ __forceinline__ void store_quad(float *p, size_t c, size_t n, const float (&v)[4]) {
-    if (c + 4 <= n) {
-        *reinterpret_cast<df4_t *>(p + c) = df4_t{v[0], v[1], v[2], v[3]};
-    } else {
+template <int T, int NV, class F>
+__device__ __forceinline__ void store_quads(float *row, unsigned n, unsigned c0, unsigned t, F &&value) {
+    char *p = reinterpret_cast<char *>(row);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < n) p[c + e] = v[e];
+    for (int i = 0; i < NV; ++i) {
+        const unsigned c = c0 + 4 * T * i + 4 * t;
+        if (c0 + 4 * T * i >= n) break;  // uniform
+        const df4_t o = {value(i, 0), value(i, 1), value(i, 2), value(i, 3)};
+        if (c + 4 <= n) *reinterpret_cast<df4_t *>(p + 4 * c) = o;
     }
+}
+// the lane's column past the last quad of n, or n
+__device__ __forceinline__ unsigned tail_column(unsigned n, unsigned t) {
+    const unsigned c = n / 4 * 4 + t;
+    return t < 3 && c < n ? c : n;
 }
 
 template <int W>
@@ -240,6 +285,15 @@ template <int W>
 constexpr int kRows = kThreads<W> / (64 * W);  // rows of a workgroup
 
 // NV quads' sums added to a lane's.
+// A value's added to a lane's sums.
+template <bool TWO>
+__device__ __forceinline__ void add_value(float v, float c, RowSums &r) {
+    if (v == kNone) return;
+    const float m = fmaxf(r.m, v), from = origin(m);
+    r.s = rebased(r.s, r.m, m, c) + pow2_of(v, from, c);
+    if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + pow2_of(v, from, kLog2e);
+    r.m = m;
+}
 template <bool TWO, int NV>
 __device__ __forceinline__ void add_quads(const float (&v)[NV][4], float c, RowSums &r) {
     float m = r.m;
@@ -263,34 +317,42 @@ __device__ __forceinline__ void add_quads(const float (&v)[NV][4], float c, RowS
 
 // A row per W waves, rows in turn over the grid.  LONG: more columns than the waves hold.
 template <int W, int NV, bool TWO, bool LONG>
-__global__ __launch_bounds__(kThreads<W>) void distill_rows(DistillArgs g) {
+__global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(DistillArgs g) {
     constexpr int RPB = kRows<W>;
     __shared__ RowSums lds[W > 1 ? W : 1];
+    // the rows' columns; in turn where waves share a row: some still read the last one's
+    __shared__ __attribute__((aligned(16))) int columns[W > 1 ? 2 : RPB][kEntries];
     const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W, t = threadIdx.x % (64 * W);
-    const size_t span = static_cast<size_t>(256) * W * NV, step = static_cast<size_t>(gridDim.x) * RPB;
+    constexpr unsigned span = 256 * W * NV;
+    const unsigned n = static_cast<unsigned>(g.vocab);
+    const size_t step = static_cast<size_t>(gridDim.x) * RPB;
     const float go = g.go ? *g.go : 1.0f;
     double loss = 0.0;
+    int turn = 0;
     for (size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot; row < g.rows; row += step) {  // (W > 1: uniform)
         const RowShare share = row_share(g, row);
+        int *const cols = columns[W > 1 ? turn : slot];
+        turn ^= 1;
+        Entry kept = {-1, kNone};
         const float *z = g.logits + row * g.vocab;
         float *dz = g.dlogits ? g.dlogits + row * g.vocab : nullptr;
         RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
-        float v[NV][4];
-        auto fetch = [&](size_t c0) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) load_quad(z, c0 + 4 * (t + 64 * W * i), g.vocab, v[i], kNone);
-        };
-        const size_t last = LONG ? (g.vocab - 1) / span * span : 0;  // the first of the columns held
+        float v[NV][4], past = kNone;  // past: the lane's column past the last quad
+        auto fetch = [&](unsigned c0) { load_quads<64 * W, NV>(z, n, c0, t, v); };
+        const unsigned last = LONG ? (n - 1) / span * span : 0;  // the first of the columns held
         if (share.weight != 0.0f) {
             fetch(0);
-            if (share.soft != 0.0f) teacher_sums(g, row, t, 64 * W, r);
+            const unsigned tail = tail_column(n, t);
+            if (tail < n) past = z[tail];
+            kept = teacher_sums(g, row, share, t, 64 * W, r, cols);
             add_quads<TWO, NV>(v, g.c, r);
             if (LONG) {
-                for (size_t c0 = span; c0 < g.vocab; c0 += span) {
+                for (unsigned c0 = span; c0 < n; c0 += span) {
                     fetch(c0);
                     add_quads<TWO, NV>(v, g.c, r);
                 }
             }
+            add_value<TWO>(past, g.c, r);
             join_lanes<TWO>(r, g.c);
             join_teacher(r, g.c);
             join_waves<TWO, W>(r, lds, g.c);
@@ -298,15 +360,12 @@ __global__ __launch_bounds__(kThreads<W>) void distill_rows(DistillArgs g) {
         const float weight = share.weight * go;
         Gradient by = {0.0f, 0.0f, 0.0f, true};
         if (share.weight != 0.0f) by = gradient<TWO>(share, r, weight);
-        for (size_t c0 = last; dz;) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const size_t c = c0 + 4 * (t + 64 * W * i);
-                if (c >= g.vocab) continue;
-                float o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = by.none ? 0.0f : by.at<TWO>(v[i][e], g.c);
-                store_quad(dz, c, g.vocab, o);
+        for (unsigned c0 = last; dz;) {
+            if (by.none) store_quads<64 * W, NV>(dz, n, c0, t, [](int, int) { return 0.0f; });
+            else store_quads<64 * W, NV>(dz, n, c0, t, [&](int i, int e) { return by.template at<TWO>(v[i][e], g.c); });
+            if (c0 == last) {
+                const unsigned tail = tail_column(n, t);
+                if (tail < n) dz[tail] = by.none ? 0.0f : by.template at<TWO>(past, g.c);
             }
             if (!LONG || c0 == 0) break;
             c0 -= span;
@@ -314,7 +373,8 @@ __global__ __launch_bounds__(kThreads<W>) void distill_rows(DistillArgs g) {
         }
         if (by.none) continue;  // (uniform over the row's waves)
         if (W > 1 && dz) __syncthreads();  // the entries' gradients are stored after the others
-        loss += entries<TWO>(g, row, share, r, by, weight, t, 64 * W, 0, g.vocab, true);
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        loss += entries<TWO>(g, row, share, r, by, weight, kept, cols, t, 64 * W, 0, g.vocab, true);
     }
     store_loss<kThreads<W>>(loss, g.row_loss + blockIdx.x);
 }
@@ -329,10 +389,11 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillAr
     const size_t row = blockIdx.x / g.segments, c0 = blockIdx.x % g.segments * static_cast<size_t>(kSegment);
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
     float v[kSegQuads][4];
-#pragma unroll
-    for (int i = 0; i < kSegQuads; ++i)
-        load_quad(g.logits + row * g.vocab, c0 + 4 * (threadIdx.x + 64 * kSegWaves * i), g.vocab, v[i], kNone);
+    load_quads<64 * kSegWaves, kSegQuads>(g.logits + row * g.vocab, static_cast<unsigned>(g.vocab), static_cast<unsigned>(c0),
+                                          threadIdx.x, v);
     add_quads<TWO, kSegQuads>(v, g.c, r);
+    const unsigned n = static_cast<unsigned>(g.vocab), tail = tail_column(n, threadIdx.x);
+    if (tail < n && c0 + kSegment >= n) add_value<TWO>(g.logits[row * g.vocab + tail], g.c, r);
     join_lanes<TWO>(r, g.c);
     join_waves<TWO, kSegWaves>(r, lds, g.c);
     if (threadIdx.x == 0) g.parts[blockIdx.x] = make_float4(r.m, static_cast<float>(r.s), static_cast<float>(r.s1), 0.0f);
@@ -341,19 +402,19 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillAr
 template <bool TWO>
 __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g) {
     __shared__ RowSums lds[kSegWaves];
+    __shared__ __attribute__((aligned(16))) int columns[kEntries];
     constexpr int T = 64 * kSegWaves;
     const size_t row = blockIdx.x / g.segments, segment = blockIdx.x % g.segments, c0 = segment * kSegment;
     const int t = threadIdx.x;
+    const unsigned n = static_cast<unsigned>(g.vocab);
     const RowShare share = row_share(g, row);
     const float *z = g.logits + row * g.vocab;
     const bool asked = share.weight != 0.0f;
+    Entry kept = {-1, kNone};
     float v[kSegQuads][4];
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
     if (asked) {
-        if (g.dlogits) {
-#pragma unroll
-            for (int i = 0; i < kSegQuads; ++i) load_quad(z, c0 + 4 * (t + T * i), g.vocab, v[i], kNone);
-        }
+        if (g.dlogits) load_quads<T, kSegQuads>(z, n, static_cast<unsigned>(c0), t, v);
         for (int k = t; k < g.segments; k += T) {
             const float4 one = g.parts[row * g.segments + k];
             const float m = fmaxf(r.m, one.x);
@@ -361,7 +422,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
             if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + rebased(one.z, one.x, m, kLog2e);
             r.m = m;
         }
-        if (share.soft != 0.0f) teacher_sums(g, row, t, T, r);
+        kept = teacher_sums(g, row, share, t, T, r, columns);
         join_lanes<TWO>(r, g.c);
         join_teacher(r, g.c);
         join_waves<TWO, kSegWaves>(r, lds, g.c);
@@ -369,19 +430,17 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     const float weight = share.weight * (g.go ? *g.go : 1.0f);
     Gradient by = {0.0f, 0.0f, 0.0f, true};
     if (asked) by = gradient<TWO>(share, r, weight);
-#pragma unroll
-    for (int i = 0; i < kSegQuads; ++i) {
-        const size_t c = c0 + 4 * (t + T * i);
-        if (!g.dlogits || c >= g.vocab) continue;
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = by.none ? 0.0f : by.at<TWO>(v[i][e], g.c);
-        store_quad(g.dlogits + row * g.vocab, c, g.vocab, o);
+    if (g.dlogits) {
+        float *dz = g.dlogits + row * g.vocab;
+        if (by.none) store_quads<T, kSegQuads>(dz, n, static_cast<unsigned>(c0), t, [](int, int) { return 0.0f; });
+        else store_quads<T, kSegQuads>(dz, n, static_cast<unsigned>(c0), t, [&](int i, int e) { return by.at<TWO>(v[i][e], g.c); });
+        const unsigned tail = tail_column(n, t);
+        if (tail < n && c0 + kSegment >= n) dz[tail] = by.none ? 0.0f : by.at<TWO>(z[tail], g.c);
     }
     double loss = 0.0;
     if (!by.none) {  // (uniform)
         __syncthreads();  // the entries' gradients are stored after the others
-        loss = entries<TWO>(g, row, share, r, by, weight, t, T, c0, c0 + kSegment, segment == 0);
+        loss = entries<TWO>(g, row, share, r, by, weight, kept, columns, t, T, c0, c0 + kSegment, segment == 0);
     }
     store_loss<T>(loss, g.row_loss + blockIdx.x);
 }
@@ -406,12 +465,12 @@ void for_vocab(size_t n, F &&f) {
     else if (n <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 4>{}, held);
     else if (n <= 8192) f(integral_constant<int, 4>{}, integral_constant<int, 8>{}, held);
     else if (n <= 16384) f(integral_constant<int, 8>{}, integral_constant<int, 8>{}, held);
-    else if (n <= 32768) f(integral_constant<int, 16>{}, integral_constant<int, 8>{}, held);
-    else if (n <= 65536) f(integral_constant<int, 16>{}, integral_constant<int, 16>{}, held);
-    else f(integral_constant<int, 16>{}, integral_constant<int, 16>{}, integral_constant<bool, true>{});
+    else if (n <= 32768) f(integral_constant<int, 8>{}, integral_constant<int, 16>{}, held);
+    else if (n <= 65536) f(integral_constant<int, 8>{}, integral_constant<int, 32>{}, held);
+    else f(integral_constant<int, 8>{}, integral_constant<int, 32>{}, integral_constant<bool, true>{});
 }
 
-size_t waves_for(size_t vocab) { return vocab <= 1024 ? 1 : vocab <= 8192 ? 4 : vocab <= 16384 ? 8 : 16; }
+size_t waves_for(size_t vocab) { return vocab <= 1024 ? 1 : vocab <= 8192 ? 4 : 8; }
 
 bool by_segments(size_t rows, size_t vocab) { return vocab > 4096 && rows * 2 <= static_cast<size_t>(device_cu_count()); }
 
