@@ -427,8 +427,9 @@ def test_distillation(rows, vocab, kept, t, hard, weighted):
     check_distillation(rows, vocab, kept, t, hard, weighted)
 
 
-@pytest.mark.parametrize("rows,vocab,kept", [(27, 300, 6), (20, 9000, 12), (140, 9001, 12)])
-@pytest.mark.parametrize("t,hard,weighted", [(1.0, 0.5, True), (0.5, 0.5, False), (3.0, 1.0, True), (1.0, 1.0, False), (10.0, 0.0, True)])
+@pytest.mark.parametrize("rows,vocab,kept", [(27, 300, 6), (20, 9000, 12), (140, 9001, 12), (260, 33001, 12), (130, 70001, 5)])
+@pytest.mark.parametrize("t,hard,weighted", [(1.0, 0.5, True), (0.5, 0.5, False), (3.0, 1.0, True), (1.0, 1.0, False), (10.0, 0.0, True),
+                                             (2.0, 0.5, True), (4.0, 0.3, False), (1.5, 0.2, True)])
 def test_distillation_s_shares_and_temperatures(rows, vocab, kept, t, hard, weighted):
     check_distillation(rows, vocab, kept, t, hard, weighted)
 
@@ -469,6 +470,24 @@ def test_distillation_where_the_student_gives_no_chance(rows, vocab):
     g = Z.grad_by_value().data()
     assert np.isnan(g[2]).all() and np.isfinite(np.delete(g, 2, 0)).all()
     T.clear_gradients()
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 3), (6, 1001), (6, 6001), (132, 6001), (131, 33001), (130, 70001)])
+@pytest.mark.parametrize("t,hard", [(1.0, 0.0), (2.0, 0.5), (1.5, 0.5)])
+def test_distillation_of_logits_that_are_no_numbers(rows, vocab, t, hard):
+    """A NaN anywhere in a row, or an infinity, makes the loss NaN and that row's gradient, no other's."""
+    z = normal((rows, vocab), 1)
+    idx, teacher, labels = np.zeros((rows, 1), np.int32), np.zeros((rows, 1), np.float32), np.zeros(rows, np.int32)
+    for at, what in ((0, np.nan), (vocab - 1, np.nan), (vocab // 2, np.nan), (slice(None), np.nan), (vocab - 1, np.inf)):
+        bad = z.copy()
+        bad[1, at] = what
+        Z = tensor(bad).with_requires_grad()
+        loss = Z.distillation(indices(idx), tensor(teacher), t, indices(labels), hard)
+        assert np.isnan(loss.value())
+        loss.backward()
+        g = Z.grad_by_value().data()
+        assert np.isnan(g[1]).all() and np.isfinite(np.delete(g, 1, 0)).all()
+        T.clear_gradients()
 
 
 @pytest.mark.parametrize("rows,vocab", [(5, 90), (5, 6000), (133, 6000)])

@@ -136,7 +136,7 @@ def test_distillation_entry_refuses():
 
     for bad in (dict(t=0.0), dict(t=-1.0), dict(t=np.nan), dict(t=INF), dict(t=1e-30), dict(hard=-0.1), dict(hard=1.1),
                 dict(hard=np.nan), dict(kept=1025), dict(labels=None), dict(z=None), dict(idx=None), dict(teacher=None),
-                dict(loss=None), dict(bad=None), dict(vocab=(1 << 30) + 1), dict(rows=1 << 31)):
+                dict(loss=None), dict(bad=None), dict(vocab=(1 << 29) + 1), dict(rows=1 << 31)):
         assert call(**bad) == EINVAL, bad
     assert call(work=None) == EWORKSPACE and call(floats=1) == EWORKSPACE
 

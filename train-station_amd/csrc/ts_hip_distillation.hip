@@ -27,6 +27,11 @@ namespace {
 
 typedef float df4_t __attribute__((ext_vector_type(4), aligned(4)));
 
+// The softmaxes of a call: one (at T, or at 1); that at T and that at 1; the same at T = 2
+// or 4, where the terms of that at 1 are the squares, or their squares, of the other's.
+// us, 999 x 50001 at T = 2, squares and without: SQ_US.
+enum class Two { kNo, kYes, kSquares };
+
 constexpr float kLog2e = 1.44269504f;
 constexpr float kNone = -__builtin_inff();
 
@@ -53,9 +58,9 @@ __device__ __forceinline__ float wave_max(float m) {
 }
 // where to count from: anything, where there is nothing but -inf
 __device__ __forceinline__ float origin(float largest) { return largest == kNone ? 0.0f : largest; }
-// a sum against `from` in terms of `to`
+// a sum against `from` in terms of `to` (of nothing, or of NaN alone: itself)
 __device__ __forceinline__ double rebased(double s, float from, float to, float c) {
-    return from == kNone ? 0.0 : s * pow2_of(from, to, c);
+    return from == kNone ? s : s * pow2_of(from, to, c);
 }
 
 // What is known of a row: the softmax's M and S (and S1), the teacher's b and A.
@@ -65,11 +70,11 @@ struct RowSums {
 };
 
 // Sums of lanes joined to a wave's (in every lane).
-template <bool TWO>
+template <Two TWO>
 __device__ __forceinline__ void join_lanes(RowSums &r, float c) {
     const float m = wave_max(r.m);
     r.s = wave_sum(rebased(r.s, r.m, m, c));
-    if (TWO) r.s1 = wave_sum(rebased(r.s1, r.m, m, kLog2e));
+    if (TWO != Two::kNo) r.s1 = wave_sum(rebased(r.s1, r.m, m, kLog2e));
     r.m = m;
 }
 __device__ __forceinline__ void join_teacher(RowSums &r, float c) {
@@ -78,7 +83,7 @@ __device__ __forceinline__ void join_teacher(RowSums &r, float c) {
     r.b = b;
 }
 // ... and waves' to the row's.
-template <bool TWO, int W>
+template <Two TWO, int W>
 __device__ __forceinline__ void join_waves(RowSums &r, RowSums *lds, float c) {
     if (W == 1) return;
     __syncthreads();  // the last row's reads
@@ -94,7 +99,7 @@ __device__ __forceinline__ void join_waves(RowSums &r, RowSums *lds, float c) {
     for (int w = 0; w < W; ++w) {
         const RowSums one = lds[w];
         all.s += rebased(one.s, one.m, all.m, c);
-        if (TWO) all.s1 += rebased(one.s1, one.m, all.m, kLog2e);
+        if (TWO != Two::kNo) all.s1 += rebased(one.s1, one.m, all.m, kLog2e);
         all.a += rebased(one.a, one.b, all.b, c);
     }
     r = all;
@@ -160,17 +165,17 @@ __device__ __forceinline__ RowShare row_share(const DistillArgs &g, size_t row) 
 struct Gradient {
     float m, by_p, by_s;
     bool none;  // nothing is asked of the row: zeros, whatever it holds
-    template <bool TWO>
+    template <Two TWO>
     __device__ __forceinline__ float at(float z, float c) const {
         const float p = by_p * pow2_of(z, m, c);
-        return TWO ? p + by_s * pow2_of(z, m, kLog2e) : p;
+        return TWO != Two::kNo ? p + by_s * pow2_of(z, m, kLog2e) : p;
     }
 };
-template <bool TWO>
+template <Two TWO>
 __device__ __forceinline__ Gradient gradient(const RowShare &share, const RowSums &r, float weight) {
     const double soft = r.a != 0.0 ? static_cast<double>(weight) * share.soft : 0.0, hard = static_cast<double>(weight) * share.hard;
     const bool none = soft == 0.0 && hard == 0.0;
-    if (TWO)
+    if (TWO != Two::kNo)
         return {r.m, soft == 0.0 ? 0.0f : static_cast<float>(soft / r.s), hard == 0.0 ? 0.0f : static_cast<float>(hard / r.s1), none};
     return {r.m, static_cast<float>((soft + hard) / r.s), 0.0f, none};
 }
@@ -190,7 +195,7 @@ __device__ __forceinline__ double ln(double x) {
 // The entries of a row in columns from .. to, by threads first + 0, + step, ...: their
 // terms of the loss (the result; first 0 adds what is the row's own, where `own`), and
 // the gradients there.
-template <bool TWO>
+template <Two TWO>
 __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, const RowShare &share, const RowSums &r,
                                           const Gradient &by, float weight, const Entry &kept, const int *columns, int first,
                                           int step, size_t from, size_t to, bool own) {
@@ -209,7 +214,7 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
         if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
         const float t = k == g.kept ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = z[j];
         double sum = takes(k, t);
-        if (k == g.kept) loss += sum * (ln(TWO ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
+        if (k == g.kept) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
         else if (sum != 0.0) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
         if (!g.dlogits) continue;
         int same = 0;  // entries of this column
@@ -246,31 +251,43 @@ __device__ __forceinline__ void store_loss(double loss, double *to) {
     }
 }
 
-// The quads c0 + 4 (t + T i) of a row of n columns (a uniform pointer and a lane's 32-bit
-// offset in bytes), -inf where there are none.  The one to three columns past the last
-// quad are lanes 0 .. 2's: tail_column.
-template <int T, int NV>
-__device__ __forceinline__ void load_quads(const float *row, unsigned n, unsigned c0, unsigned t, float (&v)[NV][4]) {
-    const char *p = reinterpret_cast<const char *>(row);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const unsigned c = c0 + 4 * T * i + 4 * t;
-        df4_t q = {kNone, kNone, kNone, kNone};
-        if (c0 + 4 * T * (i + 1) <= n) q = *reinterpret_cast<const df4_t *>(p + 4 * c);  // uniform
-        else if (c + 4 <= n) q = *reinterpret_cast<const df4_t *>(p + 4 * c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = q[e];
+// A row as the buffer instructions take it: what a lane asks for past the last whole quad
+// is not read (0 comes back) and not written; the check is of the vector offset alone, so
+// that holds all of it.  The one to three columns past it are lanes 0 .. 2's: tail_column.
+struct RowBuffer {
+    __amdgpu_buffer_rsrc_t row;
+    // four columns, at `lane` bytes past the uniform column c
+    __device__ __forceinline__ df4_t load(unsigned lane, unsigned c) const {
+        return __builtin_bit_cast(df4_t, __builtin_amdgcn_raw_buffer_load_b128(row, lane + 4 * c, 0, 0));
     }
+    __device__ __forceinline__ void store(unsigned lane, unsigned c, df4_t v) const {
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), row, lane + 4 * c, 0, 0);
+    }
+};
+// a lane's offset, as if new: or the compiler keeps its sum with every quad's column in a register
+__device__ __forceinline__ unsigned lane_bytes(unsigned t) {
+    unsigned b = 16 * t;
+    asm volatile("" : "+v"(b));
+    return b;
 }
-template <int T, int NV, class F>
-__device__ __forceinline__ void store_quads(float *row, unsigned n, unsigned c0, unsigned t, F &&value) {
-    char *p = reinterpret_cast<char *>(row);
+// n: the row's columns, 0 where there is no row
+__device__ __forceinline__ RowBuffer row_buffer(const float *row, unsigned n) {
+    return {__builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(row), 0, static_cast<int>(n / 4 * 16), 0x00020000)};
+}
+template <int T, int NV>
+__device__ __forceinline__ void load_quads(const RowBuffer &row, unsigned c0, unsigned t, df4_t (&v)[NV]) {
+    const unsigned lane = lane_bytes(t);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = row.load(lane, c0 + 4 * T * i);
+}
+// -inf in what lies past a row of n columns
+template <int T, int NV>
+__device__ __forceinline__ void fill_past(unsigned n, unsigned c0, unsigned t, df4_t (&v)[NV]) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const unsigned c = c0 + 4 * T * i + 4 * t;
-        if (c0 + 4 * T * i >= n) break;  // uniform
-        const df4_t o = {value(i, 0), value(i, 1), value(i, 2), value(i, 3)};
-        if (c + 4 <= n) *reinterpret_cast<df4_t *>(p + 4 * c) = o;
+        const unsigned c = c0 + 4 * T * i;
+        if (c + 4 * T > n && c + 4 * t + 4 > n) v[i] = df4_t{kNone, kNone, kNone, kNone};  // (the first part uniform)
     }
 }
 // the lane's column past the last quad of n, or n
@@ -284,39 +301,69 @@ constexpr int kThreads = W < 4 ? 256 : 64 * W;
 template <int W>
 constexpr int kRows = kThreads<W> / (64 * W);  // rows of a workgroup
 
-// NV quads' sums added to a lane's.
+// terms of the softmax at T = 2, or 4 where `fourth`, as those at 1
+__device__ __forceinline__ df4_t at_one(df4_t x, bool fourth) {
+    df4_t q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = x[e] * x[e];
+    if (fourth) {  // uniform
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = q[e] * q[e];
+    }
+    return q;
+}
+
 // A value's added to a lane's sums.
-template <bool TWO>
+template <Two TWO>
 __device__ __forceinline__ void add_value(float v, float c, RowSums &r) {
     if (v == kNone) return;
     const float m = fmaxf(r.m, v), from = origin(m);
     r.s = rebased(r.s, r.m, m, c) + pow2_of(v, from, c);
-    if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + pow2_of(v, from, kLog2e);
+    if (TWO != Two::kNo) r.s1 = rebased(r.s1, r.m, m, kLog2e) + pow2_of(v, from, kLog2e);
     r.m = m;
 }
-template <bool TWO, int NV>
-__device__ __forceinline__ void add_quads(const float (&v)[NV][4], float c, RowSums &r) {
-    float m = r.m;
+// NV quads', eight at a time against their own largest, so that the first are added while
+// the last are still on their way; HOLD: the exponentials stay in their place, and
+// held[k] says against what.
+constexpr int kChunk = 8;
+template <int NV>
+constexpr int kChunks = (NV + kChunk - 1) / kChunk;
+template <Two TWO, bool HOLD, int NV>
+__device__ __forceinline__ void add_quads(df4_t (&v)[NV], float c, bool fourth, RowSums &r, float (&held)[kChunks<NV>]) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int k = 0; k < kChunks<NV>; ++k) {
+        float m = kNone, s = 0.0f, s1 = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, v[i][e]);
-    const float from = origin(m);
-    float s = 0.0f, s1 = 0.0f;
+        for (int i = k * kChunk; i < (k + 1) * kChunk && i < NV; ++i)
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, v[i][e]);
+        held[k] = m;
+        const float from = origin(m);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            s += pow2_of(v[i][e], from, c);
-            if (TWO) s1 += pow2_of(v[i][e], from, kLog2e);
+        for (int i = k * kChunk; i < (k + 1) * kChunk && i < NV; ++i) {
+            df4_t x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = pow2_of(v[i][e], from, c);
+                s += x[e];
+                if (TWO == Two::kYes) s1 += pow2_of(v[i][e], from, kLog2e);
+            }
+            if (TWO == Two::kSquares) {
+                const df4_t q = at_one(x, fourth);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s1 += q[e];
+            }
+            if (HOLD) v[i] = x;
         }
-    r.s = rebased(r.s, r.m, m, c) + s;
-    if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + s1;
-    r.m = m;
+        const float all = fmaxf(r.m, m);
+        r.s = rebased(r.s, r.m, all, c) + rebased(s, m, all, c);
+        if (TWO != Two::kNo) r.s1 = rebased(r.s1, r.m, all, kLog2e) + rebased(s1, m, all, kLog2e);
+        r.m = all;
+    }
 }
 
 // A row per W waves, rows in turn over the grid.  LONG: more columns than the waves hold.
-template <int W, int NV, bool TWO, bool LONG>
+template <int W, int NV, Two TWO, bool LONG>
 __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(DistillArgs g) {
     constexpr int RPB = kRows<W>;
     __shared__ RowSums lds[W > 1 ? W : 1];
@@ -327,29 +374,39 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
     const unsigned n = static_cast<unsigned>(g.vocab);
     const size_t step = static_cast<size_t>(gridDim.x) * RPB;
     const float go = g.go ? *g.go : 1.0f;
+    constexpr bool HOLD = TWO != Two::kYes && !LONG;
+    const bool fourth = g.temperature == 4.0f;
+    const unsigned last = LONG ? (n - 1) / span * span : 0;  // the first of the columns held at a row's end
+    const unsigned tail = tail_column(n, t);
     double loss = 0.0;
     int turn = 0;
-    for (size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot; row < g.rows; row += step) {  // (W > 1: uniform)
+    size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot;
+    df4_t v[NV];
+    float past = kNone;  // the lane's column past the last quad
+    if (row < g.rows) {
+        load_quads<64 * W, NV>(row_buffer(g.logits + row * g.vocab, n), 0, t, v);
+        if (tail < n) past = g.logits[row * g.vocab + tail];
+    }
+    for (; row < g.rows; row += step) {  // (W > 1: uniform)
         const RowShare share = row_share(g, row);
         int *const cols = columns[W > 1 ? turn : slot];
-        turn ^= 1;
         Entry kept = {-1, kNone};
-        const float *z = g.logits + row * g.vocab;
+        const bool more = row + step < g.rows;
+        const float *z = g.logits + row * g.vocab, *const next = z + (more ? step * g.vocab : 0);
         float *dz = g.dlogits ? g.dlogits + row * g.vocab : nullptr;
         RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
-        float v[NV][4], past = kNone;  // past: the lane's column past the last quad
-        auto fetch = [&](unsigned c0) { load_quads<64 * W, NV>(z, n, c0, t, v); };
-        const unsigned last = LONG ? (n - 1) / span * span : 0;  // the first of the columns held
+        float largest[kChunks<NV>];  // HOLD: what the columns held are against
         if (share.weight != 0.0f) {
-            fetch(0);
-            const unsigned tail = tail_column(n, t);
-            if (tail < n) past = z[tail];
+            turn ^= 1;
             kept = teacher_sums(g, row, share, t, 64 * W, r, cols);
-            add_quads<TWO, NV>(v, g.c, r);
+            fill_past<64 * W, NV>(n, 0, t, v);
+            add_quads<TWO, HOLD, NV>(v, g.c, fourth, r, largest);
             if (LONG) {
+                const RowBuffer from = row_buffer(z, n);
                 for (unsigned c0 = span; c0 < n; c0 += span) {
-                    fetch(c0);
-                    add_quads<TWO, NV>(v, g.c, r);
+                    load_quads<64 * W, NV>(from, c0, t, v);
+                    fill_past<64 * W, NV>(n, c0, t, v);
+                    add_quads<TWO, HOLD, NV>(v, g.c, fourth, r, largest);
                 }
             }
             add_value<TWO>(past, g.c, r);
@@ -360,16 +417,45 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         const float weight = share.weight * go;
         Gradient by = {0.0f, 0.0f, 0.0f, true};
         if (share.weight != 0.0f) by = gradient<TWO>(share, r, weight);
-        for (unsigned c0 = last; dz;) {
-            if (by.none) store_quads<64 * W, NV>(dz, n, c0, t, [](int, int) { return 0.0f; });
-            else store_quads<64 * W, NV>(dz, n, c0, t, [&](int i, int e) { return by.template at<TWO>(v[i][e], g.c); });
-            if (c0 == last) {
-                const unsigned tail = tail_column(n, t);
-                if (tail < n) dz[tail] = by.none ? 0.0f : by.template at<TWO>(past, g.c);
+        // the gradients, the columns held first; then the next row's values are on their way
+        const RowBuffer to = row_buffer(dz, dz ? n : 0), then = row_buffer(next, more ? n : 0);
+        float held[kChunks<NV>], held_s[kChunks<NV>];
+        if (HOLD && !by.none) {
+#pragma unroll
+            for (int k = 0; k < kChunks<NV>; ++k) {
+                held[k] = by.by_p * (largest[k] == kNone ? 0.0f : pow2_of(largest[k], r.m, g.c));
+                held_s[k] = by.by_s * (largest[k] == kNone ? 0.0f : pow2_of(largest[k], r.m, kLog2e));
             }
-            if (!LONG || c0 == 0) break;
-            c0 -= span;
-            if (!by.none) fetch(c0);
+        }
+        auto value = [&](int i) {
+            df4_t o = {};
+            if (by.none) return o;  // uniform
+            if (TWO == Two::kSquares && HOLD) o = at_one(v[i], fourth);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!HOLD) o[e] = by.template at<TWO>(v[i][e], g.c);
+                else if (TWO == Two::kSquares) o[e] = __builtin_fmaf(held_s[i / kChunk], o[e], held[i / kChunk] * v[i][e]);
+                else o[e] = held[i / kChunk] * v[i][e];
+            }
+            return o;
+        };
+        if (dz && tail < n) dz[tail] = by.none ? 0.0f : by.template at<TWO>(past, g.c);
+        if (more && tail < n) past = next[tail];
+        const unsigned lane = lane_bytes(t);
+        if (LONG && dz) {
+            const RowBuffer from = row_buffer(z, n);
+            for (unsigned c0 = last; c0 > 0; c0 -= span) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    to.store(lane, c0 + 256 * W * i, value(i));
+                    v[i] = from.load(lane, c0 - span + 256 * W * i);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            to.store(lane, 256 * W * i, value(i));
+            v[i] = then.load(lane, 256 * W * i);
         }
         if (by.none) continue;  // (uniform over the row's waves)
         if (W > 1 && dz) __syncthreads();  // the entries' gradients are stored after the others
@@ -383,43 +469,46 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
 
 constexpr int kSegWaves = 4, kSegQuads = 4, kSegment = 256 * kSegWaves * kSegQuads;  // columns
 
-template <bool TWO>
+template <Two TWO>
 __global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillArgs g) {
     __shared__ RowSums lds[kSegWaves];
-    const size_t row = blockIdx.x / g.segments, c0 = blockIdx.x % g.segments * static_cast<size_t>(kSegment);
+    const size_t row = blockIdx.x / g.segments;
+    const unsigned c0 = blockIdx.x % g.segments * kSegment;
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
-    float v[kSegQuads][4];
-    load_quads<64 * kSegWaves, kSegQuads>(g.logits + row * g.vocab, static_cast<unsigned>(g.vocab), static_cast<unsigned>(c0),
-                                          threadIdx.x, v);
-    add_quads<TWO, kSegQuads>(v, g.c, r);
     const unsigned n = static_cast<unsigned>(g.vocab), tail = tail_column(n, threadIdx.x);
+    df4_t v[kSegQuads];
+    load_quads<64 * kSegWaves, kSegQuads>(row_buffer(g.logits + row * g.vocab, n), c0, threadIdx.x, v);
+    fill_past<64 * kSegWaves, kSegQuads>(n, c0, threadIdx.x, v);
+    float unused[kChunks<kSegQuads>];
+    add_quads<TWO, false, kSegQuads>(v, g.c, g.temperature == 4.0f, r, unused);
     if (tail < n && c0 + kSegment >= n) add_value<TWO>(g.logits[row * g.vocab + tail], g.c, r);
     join_lanes<TWO>(r, g.c);
     join_waves<TWO, kSegWaves>(r, lds, g.c);
     if (threadIdx.x == 0) g.parts[blockIdx.x] = make_float4(r.m, static_cast<float>(r.s), static_cast<float>(r.s1), 0.0f);
 }
 
-template <bool TWO>
+template <Two TWO>
 __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g) {
     __shared__ RowSums lds[kSegWaves];
     __shared__ __attribute__((aligned(16))) int columns[kEntries];
     constexpr int T = 64 * kSegWaves;
-    const size_t row = blockIdx.x / g.segments, segment = blockIdx.x % g.segments, c0 = segment * kSegment;
+    const size_t row = blockIdx.x / g.segments;  // (offsets of a row in 32 bits: kMaxVocab)
+    const unsigned segment = blockIdx.x % g.segments, c0 = segment * kSegment;
     const int t = threadIdx.x;
-    const unsigned n = static_cast<unsigned>(g.vocab);
+    const unsigned n = static_cast<unsigned>(g.vocab), tail = tail_column(n, t);
     const RowShare share = row_share(g, row);
     const float *z = g.logits + row * g.vocab;
     const bool asked = share.weight != 0.0f;
     Entry kept = {-1, kNone};
-    float v[kSegQuads][4];
+    df4_t v[kSegQuads];
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
     if (asked) {
-        if (g.dlogits) load_quads<T, kSegQuads>(z, n, static_cast<unsigned>(c0), t, v);
+        if (g.dlogits) load_quads<T, kSegQuads>(row_buffer(z, n), c0, t, v);
         for (int k = t; k < g.segments; k += T) {
             const float4 one = g.parts[row * g.segments + k];
             const float m = fmaxf(r.m, one.x);
             r.s = rebased(r.s, r.m, m, g.c) + rebased(one.y, one.x, m, g.c);
-            if (TWO) r.s1 = rebased(r.s1, r.m, m, kLog2e) + rebased(one.z, one.x, m, kLog2e);
+            if (TWO != Two::kNo) r.s1 = rebased(r.s1, r.m, m, kLog2e) + rebased(one.z, one.x, m, kLog2e);
             r.m = m;
         }
         kept = teacher_sums(g, row, share, t, T, r, columns);
@@ -432,9 +521,16 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     if (asked) by = gradient<TWO>(share, r, weight);
     if (g.dlogits) {
         float *dz = g.dlogits + row * g.vocab;
-        if (by.none) store_quads<T, kSegQuads>(dz, n, static_cast<unsigned>(c0), t, [](int, int) { return 0.0f; });
-        else store_quads<T, kSegQuads>(dz, n, static_cast<unsigned>(c0), t, [&](int i, int e) { return by.at<TWO>(v[i][e], g.c); });
-        const unsigned tail = tail_column(n, t);
+        const RowBuffer to = row_buffer(dz, n);
+#pragma unroll
+        for (int i = 0; i < kSegQuads; ++i) {
+            df4_t o = {};
+            if (!by.none) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = by.at<TWO>(v[i][e], g.c);
+            }
+            to.store(16 * t, c0 + 4 * T * i, o);
+        }
         if (tail < n && c0 + kSegment >= n) dz[tail] = by.none ? 0.0f : by.at<TWO>(z[tail], g.c);
     }
     double loss = 0.0;
@@ -454,6 +550,14 @@ __global__ __launch_bounds__(kBlock) void sum_losses(const double *parts, size_t
 
 // ---- launches ------------------------------------------------------------------------------
 
+template <class F>
+void with_two(float hard, float temperature, F &&f) {
+    using std::integral_constant;
+    if (hard == 0.0f || temperature == 1.0f) f(integral_constant<Two, Two::kNo>{});
+    else if (temperature == 2.0f || temperature == 4.0f) f(integral_constant<Two, Two::kSquares>{});
+    else f(integral_constant<Two, Two::kYes>{});
+}
+
 // Calls f(W, NV, LONG as constants) for rows of n columns: the waves that hold them.
 template <class F>
 void for_vocab(size_t n, F &&f) {
@@ -470,20 +574,20 @@ void for_vocab(size_t n, F &&f) {
     else f(integral_constant<int, 8>{}, integral_constant<int, 32>{}, integral_constant<bool, true>{});
 }
 
-size_t waves_for(size_t vocab) { return vocab <= 1024 ? 1 : vocab <= 8192 ? 4 : 8; }
-
 bool by_segments(size_t rows, size_t vocab) { return vocab > 4096 && rows * 2 <= static_cast<size_t>(device_cu_count()); }
 
-// Workgroups of distill_rows: twice what runs at once
+// Workgroups of distill_rows: as many as run at once, each with rows in turn (the next
+// one's values come in while the last one's gradients go out).
 size_t row_blocks(size_t rows, size_t vocab) {
-    const size_t w = waves_for(vocab), per = w < 4 ? 4 / w : 1, need = (rows + per - 1) / per;
-    const size_t cap = static_cast<size_t>(device_cu_count()) * 2 * (32 / (w < 4 ? 4 : w));
+    const size_t per = vocab <= 1024 ? 4 : 1, need = (rows + per - 1) / per;
+    const size_t a_cu = vocab <= 1024 ? 6 : vocab <= 4096 ? 5 : vocab <= 8192 ? 4 : vocab <= 32768 ? 2 : 1;
+    const size_t cap = static_cast<size_t>(device_cu_count()) * a_cu;
     return need < cap ? need : cap;
 }
 
 size_t segments_of(size_t vocab) { return (vocab + kSegment - 1) / kSegment; }
 
-constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 30, kMaxRows = size_t(1) << 31;
+constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 29, kMaxRows = size_t(1) << 31;
 
 }  // namespace
 
@@ -512,7 +616,6 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
     if (!workspace || workspace_floats < ts_hip_distillation_workspace_floats(rows, vocab)) return TS_HIP_EWORKSPACE;
     // with nothing asked of the teacher there is one softmax, at 1
     if (hard == 1.0f) temperature = 1.0f;
-    const bool two = hard > 0.0f && temperature != 1.0f;
     DistillArgs g = {};
     g.logits = logits;
     g.teacher = teacher;
@@ -536,21 +639,19 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
         g.parts = reinterpret_cast<float4 *>(workspace);
         g.row_loss = reinterpret_cast<double *>(workspace + 4 * rows * g.segments);
         const dim3 grid(static_cast<unsigned>(rows * g.segments)), block(64 * kSegWaves);
-        if (two) {
-            launch(distill_segment_sums<true>, grid, block, 0, s, g);
-            launch(distill_segments<true>, grid, block, 0, s, g);
-        } else {
-            launch(distill_segment_sums<false>, grid, block, 0, s, g);
-            launch(distill_segments<false>, grid, block, 0, s, g);
-        }
+        with_two(hard, temperature, [&](auto two) {
+            launch(distill_segment_sums<two.value>, grid, block, 0, s, g);
+            launch(distill_segments<two.value>, grid, block, 0, s, g);
+        });
         parts = rows * g.segments;
     } else {
         g.row_loss = reinterpret_cast<double *>(workspace);
         parts = row_blocks(rows, vocab);
         for_vocab(vocab, [&](auto w, auto nv, auto lng) {
             const dim3 grid(static_cast<unsigned>(parts)), block(kThreads<w.value>);
-            if (two) launch((distill_rows<w.value, nv.value, true, lng.value>), grid, block, 0, s, g);
-            else launch((distill_rows<w.value, nv.value, false, lng.value>), grid, block, 0, s, g);
+            with_two(hard, temperature, [&](auto two) {
+                launch((distill_rows<w.value, nv.value, two.value, lng.value>), grid, block, 0, s, g);
+            });
         });
     }
     launch(sum_losses, dim3(1), dim3(kBlock), 0, s, static_cast<const double *>(g.row_loss), parts, loss);
