@@ -115,24 +115,53 @@ struct RowShare {
 // kept from the sums to its gradient, and the columns of all are in LDS from then on.
 struct Entry {
     int j;
-    float t;
+    float t, z;  // the teacher's logit, the student's
 };
 constexpr int kEntries = 1028;  // a row's, and what fills four
 
+// What a row's own arrays hold for a lane whose first entry is `first`: on its way before
+// the row's turn comes.
+struct RowInput {
+    float weight;
+    int label, j;
+    float t;
+};
+__device__ __forceinline__ RowInput row_input(const DistillArgs &g, size_t row, int first) {
+    RowInput in = {static_cast<float>(1.0 / static_cast<double>(g.rows)), -1, -1, kNone};
+    if (g.weights) in.weight = g.weights[row];
+    if (g.labels) in.label = g.labels[row];
+    if (first < g.kept) {
+        in.j = g.indices[row * g.kept + first];
+        in.t = g.teacher[row * g.kept + first];
+    }
+    return in;
+}
+
+__device__ __forceinline__ RowShare row_share(const DistillArgs &g, size_t row, const RowInput &in) {
+    RowShare s = {in.weight, g.soft * g.temperature, 0.0f, in.label};
+    if (s.label >= 0 && static_cast<size_t>(s.label) >= g.vocab) {
+        if ((threadIdx.x & 63) == 0) atomicMin(g.bad, (1ull << 63) | row);
+        s.label = -1;
+    }
+    if (s.label >= 0) s.hard = g.hard;
+    return s;
+}
+
 // The teacher's entries first + 0, + step, ... of a row, as a lane's sums (f64).
-__device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, const RowShare &share, int first, int step,
-                                              RowSums &r, int *columns) {
+__device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, const RowShare &share, const RowInput &in, int first,
+                                              int step, RowSums &r, int *columns) {
     const size_t at = row * g.kept;
-    Entry mine = {-1, kNone};
+    Entry mine = {-1, kNone, 0.0f};
     for (int k = first; k < (g.kept + 4) / 4 * 4; k += step) {
-        Entry e = {-1, kNone};
+        Entry e = {-1, kNone, 0.0f};
         if (k < g.kept && share.soft != 0.0f) {
-            e = {g.indices[at + k], g.teacher[at + k]};
+            e.j = k == first ? in.j : g.indices[at + k];
+            e.t = k == first ? in.t : g.teacher[at + k];
             if (e.j >= 0 && static_cast<size_t>(e.j) >= g.vocab) {
                 atomicMin(g.bad, static_cast<unsigned long long>(at + k));
                 e.j = -1;
             }
-            if (e.j < 0) e = {-1, kNone};
+            if (e.j < 0) e.t = kNone;
             if (e.t != kNone) {
                 const float b = fmaxf(r.b, e.t);
                 r.a = rebased(r.a, r.b, b, g.c) + pow2_of(e.t, b, g.c);  // (a NaN stays)
@@ -144,21 +173,8 @@ __device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, 
         columns[k] = e.j;
         if (k == first) mine = e;
     }
+    if (mine.j >= 0) mine.z = g.logits[row * g.vocab + mine.j];
     return mine;
-}
-
-__device__ __forceinline__ RowShare row_share(const DistillArgs &g, size_t row) {
-    RowShare s = {g.weights ? g.weights[row] : static_cast<float>(1.0 / static_cast<double>(g.rows)), g.soft * g.temperature,
-                  0.0f, -1};
-    if (g.labels) {
-        s.label = g.labels[row];
-        if (s.label >= 0 && static_cast<size_t>(s.label) >= g.vocab) {
-            if ((threadIdx.x & 63) == 0) atomicMin(g.bad, (1ull << 63) | row);
-            s.label = -1;
-        }
-        if (s.label >= 0) s.hard = g.hard;
-    }
-    return s;
 }
 
 // dz of a logit but for what its entries take: by_p 2^(c (z - M)) + by_s 2^(log2(e) (z - M))
@@ -212,7 +228,7 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
     for (int k = first; k <= g.kept; k += step) {
         const int j = k == first ? kept.j : columns[k];
         if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
-        const float t = k == g.kept ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = z[j];
+        const float t = k == g.kept ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = k == first ? kept.z : z[j];
         double sum = takes(k, t);
         if (k == g.kept) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
         else if (sum != 0.0) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
@@ -387,10 +403,12 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         load_quads<64 * W, NV>(row_buffer(g.logits + row * g.vocab, n), 0, t, v);
         if (tail < n) past = g.logits[row * g.vocab + tail];
     }
+    RowInput in = {};
+    if (row < g.rows) in = row_input(g, row, t);
     for (; row < g.rows; row += step) {  // (W > 1: uniform)
-        const RowShare share = row_share(g, row);
+        const RowShare share = row_share(g, row, in);
         int *const cols = columns[W > 1 ? turn : slot];
-        Entry kept = {-1, kNone};
+        Entry kept = {-1, kNone, 0.0f};
         const bool more = row + step < g.rows;
         const float *z = g.logits + row * g.vocab, *const next = z + (more ? step * g.vocab : 0);
         float *dz = g.dlogits ? g.dlogits + row * g.vocab : nullptr;
@@ -398,7 +416,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         float largest[kChunks<NV>];  // HOLD: what the columns held are against
         if (share.weight != 0.0f) {
             turn ^= 1;
-            kept = teacher_sums(g, row, share, t, 64 * W, r, cols);
+            kept = teacher_sums(g, row, share, in, t, 64 * W, r, cols);
             fill_past<64 * W, NV>(n, 0, t, v);
             add_quads<TWO, HOLD, NV>(v, g.c, fourth, r, largest);
             if (LONG) {
@@ -441,6 +459,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         };
         if (dz && tail < n) dz[tail] = by.none ? 0.0f : by.template at<TWO>(past, g.c);
         if (more && tail < n) past = next[tail];
+        if (more) in = row_input(g, row + step, t);
         const unsigned lane = lane_bytes(t);
         if (LONG && dz) {
             const RowBuffer from = row_buffer(z, n);
@@ -496,10 +515,11 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     const unsigned segment = blockIdx.x % g.segments, c0 = segment * kSegment;
     const int t = threadIdx.x;
     const unsigned n = static_cast<unsigned>(g.vocab), tail = tail_column(n, t);
-    const RowShare share = row_share(g, row);
+    const RowInput in = row_input(g, row, t);
+    const RowShare share = row_share(g, row, in);
     const float *z = g.logits + row * g.vocab;
     const bool asked = share.weight != 0.0f;
-    Entry kept = {-1, kNone};
+    Entry kept = {-1, kNone, 0.0f};
     df4_t v[kSegQuads];
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
     if (asked) {
@@ -511,7 +531,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
             if (TWO != Two::kNo) r.s1 = rebased(r.s1, r.m, m, kLog2e) + rebased(one.z, one.x, m, kLog2e);
             r.m = m;
         }
-        kept = teacher_sums(g, row, share, t, T, r, columns);
+        kept = teacher_sums(g, row, share, in, t, T, r, columns);
         join_lanes<TWO>(r, g.c);
         join_teacher(r, g.c);
         join_waves<TWO, kSegWaves>(r, lds, g.c);
