@@ -548,9 +548,16 @@ def test_distillation_reports_entries_outside_the_vocabulary(rows, vocab):
 
 
 def test_distillation_over_a_caller_s_memory_at_any_address():
-    z, idx, teacher, labels, w = distill_case(12, 4999, 9)
+    for rows, vocab in ((12, 4999), (140, 4999), (30, 1), (30, 2), (31, 3), (30, 5), (25, 31), (25, 33), (33, 993), (9, 1000), (9, 4065),
+                        (10, 8161), (140, 16353), (140, 32737), (140, 32736), (131, 65505)):
+        for offset in (1, 2, 3, 5, 30):
+            check_at_an_address(rows, vocab, offset)
+
+
+def check_at_an_address(rows, vocab, offset):
+    z, idx, teacher, labels, w = distill_case(rows, vocab, 9)
     z[7::9, 0] = 0.0
-    Z = T.Tensor.from_device(DeviceArray(z, 1)).with_requires_grad()
+    Z = T.Tensor.from_device(DeviceArray(z, offset)).with_requires_grad()
     loss = Z.distillation(T.Indices.from_device(IndexArray(idx, 1)), T.Tensor.from_device(DeviceArray(teacher, 3)), 1.5,
                           T.Indices.from_device(IndexArray(labels, 2)), 0.5, T.Tensor.from_device(DeviceArray(w, 1)))
     want, dz, bound, bz = R.distillation(z, idx, teacher, 1.5, labels, 0.5, w)
@@ -558,8 +565,11 @@ def test_distillation_over_a_caller_s_memory_at_any_address():
     loss.backward()
     assert_within(Z.grad_by_value().data(), dz, bz, "dz")
     T.clear_gradients()
+
+
+def test_indices_are_in_one_allocation():
     with pytest.raises(T.TsError, match="one allocation"):
-        far = IndexArray(idx)
+        far = IndexArray(np.zeros((3, 4), np.int32))
         far.__cuda_array_interface__["shape"] = (1 << 30,)
         T.Indices.from_device(far)
 
@@ -583,7 +593,8 @@ def test_distillation_of_far_logits():
 
 
 def test_distillation_entry_by_itself():
-    """The C entry with a device gradient of the loss, and equal bits from equal calls."""
+    """The C entry with a device gradient of the loss, by one launch and by two, and equal bits from equal calls."""
+    ticket = Dev.of(np.zeros(1, np.float32))
     for rows, vocab in ((33, 500), (20, 9000), (140, 9000)):
         z, idx, teacher, labels, w = distill_case(rows, vocab, 11)
         z[7::9, 0] = 0.0
@@ -591,17 +602,19 @@ def test_distillation_entry_by_itself():
                Dev.of(np.array([3.0], np.float32))]
         floats, bad, got = hip.ts_hip_distillation_workspace_floats(rows, vocab), ZeroIndex(), []
         work = Dev(floats)
-        for _ in range(3):
+        for one in (None, ticket.ptr, ticket.ptr, None):
             loss, out = Dev(1), Dev(rows * vocab + 2)
             out.put(np.full(rows * vocab + 2, 7.0, np.float32))
             hip_check(hip.ts_hip_distillation(dev[0].ptr, rows, vocab, dev[1].ptr, dev[2].ptr, 11, 2.0, dev[3].ptr, 0.5, dev[4].ptr,
-                                              dev[5].ptr, loss.ptr, out.ptr, bad.ptr, work.ptr, floats, None))
+                                              dev[5].ptr, loss.ptr, out.ptr, bad.ptr, work.ptr, floats, one, None))
             got.append((loss.get(), out.get()))
         want, dz, bound, bz = R.distillation(z, idx, teacher, 2.0, labels, 0.5, w)
         assert_within(got[0][0], np.array([want]), bound, "loss")
         assert_within(got[0][1][:-2].reshape(rows, vocab), 3 * dz, 3 * bz + 2 * R.U * np.abs(3 * dz), "dz")
         assert np.all(got[0][1][-2:] == 7.0) and bad.value() is None
-        assert all(np.array_equal(a, b) for g in got[1:] for a, b in zip(g, got[0]))
+        assert not ticket.get().view(np.uint32).any()
+        assert all(np.array_equal(g[1], got[0][1]) for g in got) and got[1][0] == got[2][0] and got[3][0] == got[0][0]
+        assert abs(got[1][0] - got[0][0]) <= 2 * R.U * abs(want)  # (the parts in another order of f64 sums)
 
 
 # ---- together ---------------------------------------------------------------------------

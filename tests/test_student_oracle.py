@@ -132,11 +132,11 @@ def test_block8_entries_refuse():
 def test_distillation_entry_refuses():
     def call(rows=4, vocab=8, kept=2, t=1.0, hard=0.5, z=P, idx=P, teacher=P, labels=P, loss=P, bad=P, work=P, floats=1 << 40):
         return hip.ts_hip_distillation(z, rows, vocab, idx, teacher, kept, t, labels, hard, None, None, loss, P, bad, work, floats,
-                                       None)
+                                       None, None)
 
     for bad in (dict(t=0.0), dict(t=-1.0), dict(t=np.nan), dict(t=INF), dict(t=1e-30), dict(hard=-0.1), dict(hard=1.1),
                 dict(hard=np.nan), dict(kept=1025), dict(labels=None), dict(z=None), dict(idx=None), dict(teacher=None),
-                dict(loss=None), dict(bad=None), dict(vocab=(1 << 29) + 1), dict(rows=1 << 31)):
+                dict(loss=None), dict(bad=None), dict(vocab=(1 << 28) + 1), dict(rows=1 << 31)):
         assert call(**bad) == EINVAL, bad
     assert call(work=None) == EWORKSPACE and call(floats=1) == EWORKSPACE
 

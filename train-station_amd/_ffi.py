@@ -203,7 +203,7 @@ HIP_SIGNATURES = {
     "ts_hip_layer_norm_backward_workspace_floats": (SZ, [SZ, SZ]),
     "ts_hip_layer_norm_backward": (_c.c_int, [VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, VP, SZ, VP, VP]),
     "ts_hip_distillation_workspace_floats": (SZ, [SZ, SZ]),
-    "ts_hip_distillation": (_c.c_int, [VP, SZ, SZ, VP, VP, SZ, _c.c_float, VP, _c.c_float, VP, VP, VP, VP, VP, VP, SZ, VP]),
+    "ts_hip_distillation": (_c.c_int, [VP, SZ, SZ, VP, VP, SZ, _c.c_float, VP, _c.c_float, VP, VP, VP, VP, VP, VP, SZ, VP, VP]),
     "ts_hip_linear_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),
     "ts_hip_linear": (_c.c_int, [_c.POINTER(LinearShape), VP, VP, VP, _c.c_int, VP, VP, VP, VP, VP, VP, SZ, VP]),
     "ts_hip_linear_backward_workspace_floats": (SZ, [_c.POINTER(LinearShape)]),

@@ -291,7 +291,8 @@ void Distillation::run(const float *go, float *loss, float *dlogits) const {
     const float *z = logits.ptr(), *t = teacher.ptr(), *w = weights.ptr();
     launch(KernelClass::Reduction, (dlogits ? 8.0 : 4.0) * rows * vocab + 8.0 * rows * kept, "ts_hip_distillation", [&] {
         return ts_hip_distillation(z, rows, vocab, indices.ptr(), t, kept, temperature, labels.ptr(), hard, w, go, loss, dlogits,
-                                   Runtime::get().bad_entry(), work ? work->get() : nullptr, ws, S());
+                                   Runtime::get().bad_entry(), work ? work->get() : nullptr, ws,
+                                   Runtime::get().ticket(), S());
     });
 }
 

@@ -17,6 +17,7 @@
 // label have a thread each: it adds their term to its part of the loss, and stores the
 // gradient there after the others are stored (an index given twice: the first entry's,
 // with both).  Sums past a lane are f64.
+#include <algorithm>
 #include <type_traits>
 
 #include "ts_hip_internal.h"
@@ -27,9 +28,8 @@ namespace {
 
 typedef float df4_t __attribute__((ext_vector_type(4), aligned(4)));
 
-// The softmaxes of a call: one (at T, or at 1); that at T and that at 1; the same at T = 2
-// or 4, where the terms of that at 1 are the squares, or their squares, of the other's.
-// us, 999 x 50001 at T = 2, squares and without: SQ_US.
+// The softmaxes of a call: one (at T, or at 1); that at T and that at 1; the same at T = 2,
+// where the terms of that at 1 are the squares of the other's.  SQ_US
 enum class Two { kNo, kYes, kSquares };
 
 constexpr float kLog2e = 1.44269504f;
@@ -40,6 +40,8 @@ struct DistillArgs {
     const int *indices, *labels;  // labels null: none (hard is 0 then)
     float *dlogits;               // null: the loss alone
     double *row_loss;             // each workgroup's part of the loss
+    float *loss;
+    unsigned *ticket;             // zero, and zero again when the launch has run; null: the parts are added by another
     unsigned long long *bad;      // the smallest number of an entry outside the vocabulary
     size_t rows, vocab;
     int kept;
@@ -112,12 +114,13 @@ struct RowShare {
 };
 
 // The entries of a row are the teacher's, then the label; -1: none.  A thread's first is
-// kept from the sums to its gradient, and the columns of all are in LDS from then on.
+// kept from the sums to its gradient, and the columns of the teacher's are in LDS from
+// then on.
 struct Entry {
     int j;
     float t, z;  // the teacher's logit, the student's
 };
-constexpr int kEntries = 1028;  // a row's, and what fills four
+constexpr int kEntries = 1024;  // the teacher's of a row, at most
 
 // What a row's own arrays hold for a lane whose first entry is `first`: on its way before
 // the row's turn comes.
@@ -152,7 +155,7 @@ __device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, 
                                               int step, RowSums &r, int *columns) {
     const size_t at = row * g.kept;
     Entry mine = {-1, kNone, 0.0f};
-    for (int k = first; k < (g.kept + 4) / 4 * 4; k += step) {
+    for (int k = first; k < g.kept + 4; k += step) {  // (to whole fours)
         Entry e = {-1, kNone, 0.0f};
         if (k < g.kept && share.soft != 0.0f) {
             e.j = k == first ? in.j : g.indices[at + k];
@@ -170,7 +173,7 @@ __device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, 
         } else if (k == g.kept) {
             e.j = share.label;
         }
-        columns[k] = e.j;
+        if (k < (g.kept + 3) / 4 * 4) columns[k] = k < g.kept ? e.j : -1;
         if (k == first) mine = e;
     }
     if (mine.j >= 0) mine.z = g.logits[row * g.vocab + mine.j];
@@ -221,113 +224,151 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
     const double per_e = asked ? static_cast<double>(share.soft) / r.a : 0.0;
     double loss = 0.0;
     if (first == 0 && own && asked) loss = static_cast<double>(share.soft) * g.temperature * (ln(r.s) - ln(r.a));
-    auto takes = [&](int k, float t) {  // of the gradient there, without its weight
-        if (k == g.kept) return static_cast<double>(share.hard);
-        return asked ? per_e * pow2_of(t, r.b, g.c) : 0.0;
-    };
+    auto takes = [&](float t) { return asked ? per_e * pow2_of(t, r.b, g.c) : 0.0; };  // of the gradient, without its weight
     for (int k = first; k <= g.kept; k += step) {
-        const int j = k == first ? kept.j : columns[k];
+        const bool label = k == g.kept;
+        const int j = k == first ? kept.j : label ? share.label : columns[k];
         if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
-        const float t = k == g.kept ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = k == first ? kept.z : z[j];
-        double sum = takes(k, t);
-        if (k == g.kept) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
+        const float t = label ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = k == first ? kept.z : z[j];
+        double sum = label ? static_cast<double>(share.hard) : takes(t);
+        if (label) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
         else if (sum != 0.0) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
         if (!g.dlogits) continue;
-        int same = 0;  // entries of this column
+        int same = 0;  // the teacher's entries of this column
 #pragma unroll 2
-        for (int other = 0; other <= g.kept; other += 4) {
+        for (int other = 0; other < g.kept; other += 4) {
             const int4 four = *reinterpret_cast<const int4 *>(columns + other);
             same += (four.x == j) + (four.y == j) + (four.z == j) + (four.w == j);
         }
-        bool mine = true;  // the first of them stores, with the later ones' shares
-        if (same > 1) {
-            for (int other = 0; other <= g.kept; ++other) {
-                if (other == k || columns[other] != j) continue;
-                if (other < k) mine = false;
-                else sum += takes(other, other == g.kept ? 0.0f : g.teacher[at + other]);
+        bool mine = label ? same == 0 : true;  // the first of them stores, with the later ones' shares and the label's
+        if (!label) {
+            if (same > 1) {
+                for (int other = 0; other < g.kept; ++other) {
+                    if (other == k || columns[other] != j) continue;
+                    if (other < k) mine = false;
+                    else sum += takes(g.teacher[at + other]);
+                }
             }
+            if (j == share.label) sum += share.hard;
         }
         if (mine) g.dlogits[row * g.vocab + j] = by.at<TWO>(zj, g.c) - static_cast<float>(weight * sum);
     }
     return loss * share.weight;
 }
 
-// The sum of a workgroup's losses, in a fixed order, to its place.
+// The sum over a workgroup's threads, in a fixed order, in thread 0.
 template <int T>
-__device__ __forceinline__ void store_loss(double loss, double *to) {
+__device__ __forceinline__ double threads_sum(double v) {
     __shared__ double waves[T / 64];
-    loss = wave_sum(loss);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = loss;
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
     __syncthreads();
+    double all = 0.0;
     if (threadIdx.x == 0) {
-        double all = 0.0;
 #pragma unroll
         for (int w = 0; w < T / 64; ++w) all += waves[w];
-        *to = all;
+    }
+    return all;
+}
+
+// A workgroup's losses to its place; with a ticket the last workgroup to get here adds
+// them all up.  (The parts go past the caches of the chip's dies, and are there before
+// the ticket counts them: a fence would write back all that the die holds.)
+template <int T>
+__device__ __forceinline__ void store_loss(const DistillArgs &g, double loss) {
+    loss = threads_sum<T>(loss);
+    if (!g.ticket) {
+        if (threadIdx.x == 0) g.row_loss[blockIdx.x] = loss;
+        return;
+    }
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(g.row_loss + blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last = __hip_atomic_fetch_add(g.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;  // (uniform)
+    double s = 0.0;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += T)
+        s += __hip_atomic_load(g.row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();  // (threads_sum's memory)
+    s = threads_sum<T>(s);
+    if (threadIdx.x == 0) {
+        *g.loss = static_cast<float>(s);
+        __hip_atomic_store(g.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
-// A row as the buffer instructions take it: what a lane asks for past the last whole quad
-// is not read (0 comes back) and not written; the check is of the vector offset alone, so
-// that holds all of it.  The one to three columns past it are lanes 0 .. 2's: tail_column.
-struct RowBuffer {
-    __amdgpu_buffer_rsrc_t row;
-    // four columns, at `lane` bytes past the uniform column c
-    __device__ __forceinline__ df4_t load(unsigned lane, unsigned c) const {
-        return __builtin_bit_cast(df4_t, __builtin_amdgcn_raw_buffer_load_b128(row, lane + 4 * c, 0, 0));
-    }
-    __device__ __forceinline__ void store(unsigned lane, unsigned c, df4_t v) const {
-        typedef unsigned u4 __attribute__((ext_vector_type(4)));
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), row, lane + 4 * c, 0, 0);
+// Where a row's columns stand: column c at place c + s, counted from the line of 128 bytes
+// that its first value is in, so that a wave's quads of places are whole lines (rows of
+// 50001: ALIGN_US).  The quads that lie within the row are read and written by the buffer
+// instructions; the columns before the first and after the last, three each at most, are
+// the edge, lanes 0 .. 5's.
+struct Places {
+    unsigned s, n;
+    __device__ __forceinline__ Places(const float *row, unsigned n, bool lines = true)
+        : s(lines ? static_cast<unsigned>(reinterpret_cast<uintptr_t>(row)) / 4 & 31 : 0), n(n) {}
+    __device__ __forceinline__ unsigned end() const { return s + n; }
+    __device__ __forceinline__ bool holds(unsigned place) const { return place >= s && place + 4 <= end(); }
+    // lane t's edge column, or n
+    __device__ __forceinline__ unsigned edge(unsigned t) const {
+        const unsigned head = min((4 - s % 4) % 4, n);
+        if (t < 3) return t < head ? t : n;
+        const int tail = static_cast<int>(end() / 4 * 4) - static_cast<int>(s);
+        const unsigned c = static_cast<unsigned>(max(tail, static_cast<int>(head))) + t - 3;
+        return t < 6 && c < n ? c : n;
     }
 };
-// a lane's offset, as if new: or the compiler keeps its sum with every quad's column in a register
+// A row for the buffer instructions: what lies past its last whole quad is not read (0
+// comes back) and not written.  The check is of the vector offset alone, which therefore
+// holds all of a place's.
+struct RowBuffer {
+    __amdgpu_buffer_rsrc_t row;
+    unsigned skip;  // bytes before the row
+    // (there: whether there is a row)
+    __device__ __forceinline__ RowBuffer(const float *p, const Places &at, bool there)
+        : row(__builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p - at.s), 0, there ? static_cast<int>(at.end() / 4 * 16) : 0,
+                                                0x00020000)),
+          skip(4 * at.s) {}
+    // the quad at `lane` bytes past the uniform place p (p 0: it may be before the row)
+    __device__ __forceinline__ unsigned offset(unsigned lane, unsigned p) const {
+        return p == 0 && lane < skip ? 0x80000000u : lane + 4 * p;  // (past any row: kMaxVocab)
+    }
+    __device__ __forceinline__ df4_t load(unsigned lane, unsigned p) const {
+        return __builtin_bit_cast(df4_t, __builtin_amdgcn_raw_buffer_load_b128(row, offset(lane, p), 0, 0));
+    }
+    __device__ __forceinline__ void store(unsigned lane, unsigned p, df4_t v) const {
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), row, offset(lane, p), 0, 0);
+    }
+};
+// a lane's offset, as if new: or the compiler keeps its sum with every quad's place in a register
 __device__ __forceinline__ unsigned lane_bytes(unsigned t) {
     unsigned b = 16 * t;
     asm volatile("" : "+v"(b));
     return b;
 }
-// n: the row's columns, 0 where there is no row
-__device__ __forceinline__ RowBuffer row_buffer(const float *row, unsigned n) {
-    return {__builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(row), 0, static_cast<int>(n / 4 * 16), 0x00020000)};
-}
 template <int T, int NV>
-__device__ __forceinline__ void load_quads(const RowBuffer &row, unsigned c0, unsigned t, df4_t (&v)[NV]) {
+__device__ __forceinline__ void load_quads(const RowBuffer &row, unsigned p0, unsigned t, df4_t (&v)[NV]) {
     const unsigned lane = lane_bytes(t);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = row.load(lane, c0 + 4 * T * i);
+    for (int i = 0; i < NV; ++i) v[i] = row.load(lane, p0 + 4 * T * i);
 }
-// -inf in what lies past a row of n columns
+// -inf in the quads that do not lie within the row
 template <int T, int NV>
-__device__ __forceinline__ void fill_past(unsigned n, unsigned c0, unsigned t, df4_t (&v)[NV]) {
+__device__ __forceinline__ void fill_outside(const Places &at, unsigned p0, unsigned t, df4_t (&v)[NV]) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const unsigned c = c0 + 4 * T * i;
-        if (c + 4 * T > n && c + 4 * t + 4 > n) v[i] = df4_t{kNone, kNone, kNone, kNone};  // (the first part uniform)
+        const unsigned p = p0 + 4 * T * i;
+        if ((p == 0 || p + 4 * T > at.end()) && !at.holds(p + 4 * t)) v[i] = df4_t{kNone, kNone, kNone, kNone};  // (the first part uniform)
     }
-}
-// the lane's column past the last quad of n, or n
-__device__ __forceinline__ unsigned tail_column(unsigned n, unsigned t) {
-    const unsigned c = n / 4 * 4 + t;
-    return t < 3 && c < n ? c : n;
 }
 
 template <int W>
 constexpr int kThreads = W < 4 ? 256 : 64 * W;
 template <int W>
 constexpr int kRows = kThreads<W> / (64 * W);  // rows of a workgroup
-
-// terms of the softmax at T = 2, or 4 where `fourth`, as those at 1
-__device__ __forceinline__ df4_t at_one(df4_t x, bool fourth) {
-    df4_t q;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = x[e] * x[e];
-    if (fourth) {  // uniform
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = q[e] * q[e];
-    }
-    return q;
-}
 
 // A value's added to a lane's sums.
 template <Two TWO>
@@ -345,7 +386,7 @@ constexpr int kChunk = 8;
 template <int NV>
 constexpr int kChunks = (NV + kChunk - 1) / kChunk;
 template <Two TWO, bool HOLD, int NV>
-__device__ __forceinline__ void add_quads(df4_t (&v)[NV], float c, bool fourth, RowSums &r, float (&held)[kChunks<NV>]) {
+__device__ __forceinline__ void add_quads(df4_t (&v)[NV], float c, RowSums &r, float (&held)[kChunks<NV>]) {
 #pragma unroll
     for (int k = 0; k < kChunks<NV>; ++k) {
         float m = kNone, s = 0.0f, s1 = 0.0f;
@@ -362,12 +403,8 @@ __device__ __forceinline__ void add_quads(df4_t (&v)[NV], float c, bool fourth, 
             for (int e = 0; e < 4; ++e) {
                 x[e] = pow2_of(v[i][e], from, c);
                 s += x[e];
+                if (TWO == Two::kSquares) s1 = __builtin_fmaf(x[e], x[e], s1);
                 if (TWO == Two::kYes) s1 += pow2_of(v[i][e], from, kLog2e);
-            }
-            if (TWO == Two::kSquares) {
-                const df4_t q = at_one(x, fourth);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s1 += q[e];
             }
             if (HOLD) v[i] = x;
         }
@@ -391,17 +428,16 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
     const size_t step = static_cast<size_t>(gridDim.x) * RPB;
     const float go = g.go ? *g.go : 1.0f;
     constexpr bool HOLD = TWO != Two::kYes && !LONG;
-    const bool fourth = g.temperature == 4.0f;
-    const unsigned last = LONG ? (n - 1) / span * span : 0;  // the first of the columns held at a row's end
-    const unsigned tail = tail_column(n, t);
     double loss = 0.0;
     int turn = 0;
     size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot;
     df4_t v[NV];
-    float past = kNone;  // the lane's column past the last quad
+    float edge = kNone;  // the lane's edge column
     if (row < g.rows) {
-        load_quads<64 * W, NV>(row_buffer(g.logits + row * g.vocab, n), 0, t, v);
-        if (tail < n) past = g.logits[row * g.vocab + tail];
+        const float *z = g.logits + row * g.vocab;
+        const Places at(z, n, W > 1);
+        load_quads<64 * W, NV>(RowBuffer(z, at, true), 0, t, v);
+        if (at.edge(t) < n) edge = z[at.edge(t)];
     }
     RowInput in = {};
     if (row < g.rows) in = row_input(g, row, t);
@@ -412,22 +448,24 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         const bool more = row + step < g.rows;
         const float *z = g.logits + row * g.vocab, *const next = z + (more ? step * g.vocab : 0);
         float *dz = g.dlogits ? g.dlogits + row * g.vocab : nullptr;
+        const Places at(z, n, W > 1), after(next, n, W > 1);
+        const unsigned last = LONG ? (at.end() - 1) / span * span : 0;  // the first of the places held at the row's end
         RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
         float largest[kChunks<NV>];  // HOLD: what the columns held are against
         if (share.weight != 0.0f) {
             turn ^= 1;
             kept = teacher_sums(g, row, share, in, t, 64 * W, r, cols);
-            fill_past<64 * W, NV>(n, 0, t, v);
-            add_quads<TWO, HOLD, NV>(v, g.c, fourth, r, largest);
+            fill_outside<64 * W, NV>(at, 0, t, v);
+            add_quads<TWO, HOLD, NV>(v, g.c, r, largest);
             if (LONG) {
-                const RowBuffer from = row_buffer(z, n);
-                for (unsigned c0 = span; c0 < n; c0 += span) {
-                    load_quads<64 * W, NV>(from, c0, t, v);
-                    fill_past<64 * W, NV>(n, c0, t, v);
-                    add_quads<TWO, HOLD, NV>(v, g.c, fourth, r, largest);
+                const RowBuffer from(z, at, true);
+                for (unsigned p0 = span; p0 < at.end(); p0 += span) {
+                    load_quads<64 * W, NV>(from, p0, t, v);
+                    fill_outside<64 * W, NV>(at, p0, t, v);
+                    add_quads<TWO, HOLD, NV>(v, g.c, r, largest);
                 }
             }
-            add_value<TWO>(past, g.c, r);
+            add_value<TWO>(edge, g.c, r);
             join_lanes<TWO>(r, g.c);
             join_teacher(r, g.c);
             join_waves<TWO, W>(r, lds, g.c);
@@ -436,7 +474,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         Gradient by = {0.0f, 0.0f, 0.0f, true};
         if (share.weight != 0.0f) by = gradient<TWO>(share, r, weight);
         // the gradients, the columns held first; then the next row's values are on their way
-        const RowBuffer to = row_buffer(dz, dz ? n : 0), then = row_buffer(next, more ? n : 0);
+        const RowBuffer to(dz, at, dz), then(next, after, more);
         float held[kChunks<NV>], held_s[kChunks<NV>];
         if (HOLD && !by.none) {
 #pragma unroll
@@ -448,26 +486,25 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         auto value = [&](int i) {
             df4_t o = {};
             if (by.none) return o;  // uniform
-            if (TWO == Two::kSquares && HOLD) o = at_one(v[i], fourth);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (!HOLD) o[e] = by.template at<TWO>(v[i][e], g.c);
-                else if (TWO == Two::kSquares) o[e] = __builtin_fmaf(held_s[i / kChunk], o[e], held[i / kChunk] * v[i][e]);
+                else if (TWO == Two::kSquares) o[e] = v[i][e] * __builtin_fmaf(held_s[i / kChunk], v[i][e], held[i / kChunk]);
                 else o[e] = held[i / kChunk] * v[i][e];
             }
             return o;
         };
-        if (dz && tail < n) dz[tail] = by.none ? 0.0f : by.template at<TWO>(past, g.c);
-        if (more && tail < n) past = next[tail];
+        if (dz && at.edge(t) < n) dz[at.edge(t)] = by.none ? 0.0f : by.template at<TWO>(edge, g.c);
+        edge = more && after.edge(t) < n ? next[after.edge(t)] : kNone;
         if (more) in = row_input(g, row + step, t);
         const unsigned lane = lane_bytes(t);
         if (LONG && dz) {
-            const RowBuffer from = row_buffer(z, n);
-            for (unsigned c0 = last; c0 > 0; c0 -= span) {
+            const RowBuffer from(z, at, true);
+            for (unsigned p0 = last; p0 > 0; p0 -= span) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    to.store(lane, c0 + 256 * W * i, value(i));
-                    v[i] = from.load(lane, c0 - span + 256 * W * i);
+                    to.store(lane, p0 + 256 * W * i, value(i));
+                    v[i] = from.load(lane, p0 - span + 256 * W * i);
                 }
             }
         }
@@ -481,26 +518,34 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         loss += entries<TWO>(g, row, share, r, by, weight, kept, cols, t, 64 * W, 0, g.vocab, true);
     }
-    store_loss<kThreads<W>>(loss, g.row_loss + blockIdx.x);
+    store_loss<kThreads<W>>(g, loss);
 }
 
 // ---- rows by segments ------------------------------------------------------------------
 
-constexpr int kSegWaves = 4, kSegQuads = 4, kSegment = 256 * kSegWaves * kSegQuads;  // columns
+constexpr int kSegWaves = 4, kSegQuads = 4, kSegment = 256 * kSegWaves * kSegQuads;  // places
+
+// lane t's edge column where its place is one of the segment's from p0 on, else n
+__device__ __forceinline__ unsigned segment_edge(const Places &at, unsigned p0, unsigned t) {
+    const unsigned c = at.edge(t);
+    return c < at.n && (c + at.s) / kSegment == p0 / kSegment ? c : at.n;
+}
 
 template <Two TWO>
 __global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillArgs g) {
     __shared__ RowSums lds[kSegWaves];
     const size_t row = blockIdx.x / g.segments;
-    const unsigned c0 = blockIdx.x % g.segments * kSegment;
+    const unsigned p0 = blockIdx.x % g.segments * kSegment;
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
-    const unsigned n = static_cast<unsigned>(g.vocab), tail = tail_column(n, threadIdx.x);
+    const float *z = g.logits + row * g.vocab;
+    const Places at(z, static_cast<unsigned>(g.vocab));
     df4_t v[kSegQuads];
-    load_quads<64 * kSegWaves, kSegQuads>(row_buffer(g.logits + row * g.vocab, n), c0, threadIdx.x, v);
-    fill_past<64 * kSegWaves, kSegQuads>(n, c0, threadIdx.x, v);
+    load_quads<64 * kSegWaves, kSegQuads>(RowBuffer(z, at, true), p0, threadIdx.x, v);
+    fill_outside<64 * kSegWaves, kSegQuads>(at, p0, threadIdx.x, v);
     float unused[kChunks<kSegQuads>];
-    add_quads<TWO, false, kSegQuads>(v, g.c, g.temperature == 4.0f, r, unused);
-    if (tail < n && c0 + kSegment >= n) add_value<TWO>(g.logits[row * g.vocab + tail], g.c, r);
+    add_quads<TWO, false, kSegQuads>(v, g.c, r, unused);
+    const unsigned edge = segment_edge(at, p0, threadIdx.x);
+    if (edge < at.n) add_value<TWO>(z[edge], g.c, r);
     join_lanes<TWO>(r, g.c);
     join_waves<TWO, kSegWaves>(r, lds, g.c);
     if (threadIdx.x == 0) g.parts[blockIdx.x] = make_float4(r.m, static_cast<float>(r.s), static_cast<float>(r.s1), 0.0f);
@@ -512,18 +557,18 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     __shared__ __attribute__((aligned(16))) int columns[kEntries];
     constexpr int T = 64 * kSegWaves;
     const size_t row = blockIdx.x / g.segments;  // (offsets of a row in 32 bits: kMaxVocab)
-    const unsigned segment = blockIdx.x % g.segments, c0 = segment * kSegment;
+    const unsigned segment = blockIdx.x % g.segments, p0 = segment * kSegment;
     const int t = threadIdx.x;
-    const unsigned n = static_cast<unsigned>(g.vocab), tail = tail_column(n, t);
     const RowInput in = row_input(g, row, t);
     const RowShare share = row_share(g, row, in);
     const float *z = g.logits + row * g.vocab;
+    const Places at(z, static_cast<unsigned>(g.vocab));
     const bool asked = share.weight != 0.0f;
     Entry kept = {-1, kNone, 0.0f};
     df4_t v[kSegQuads];
     RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
     if (asked) {
-        if (g.dlogits) load_quads<T, kSegQuads>(row_buffer(z, n), c0, t, v);
+        if (g.dlogits) load_quads<T, kSegQuads>(RowBuffer(z, at, true), p0, t, v);
         for (int k = t; k < g.segments; k += T) {
             const float4 one = g.parts[row * g.segments + k];
             const float m = fmaxf(r.m, one.x);
@@ -541,7 +586,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     if (asked) by = gradient<TWO>(share, r, weight);
     if (g.dlogits) {
         float *dz = g.dlogits + row * g.vocab;
-        const RowBuffer to = row_buffer(dz, n);
+        const RowBuffer to(dz, at, true);
 #pragma unroll
         for (int i = 0; i < kSegQuads; ++i) {
             df4_t o = {};
@@ -549,16 +594,18 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = by.at<TWO>(v[i][e], g.c);
             }
-            to.store(16 * t, c0 + 4 * T * i, o);
+            to.store(16 * t, p0 + 4 * T * i, o);
         }
-        if (tail < n && c0 + kSegment >= n) dz[tail] = by.none ? 0.0f : by.at<TWO>(z[tail], g.c);
+        const unsigned edge = segment_edge(at, p0, t);
+        if (edge < at.n) dz[edge] = by.none ? 0.0f : by.at<TWO>(z[edge], g.c);
     }
     double loss = 0.0;
     if (!by.none) {  // (uniform)
         __syncthreads();  // the entries' gradients are stored after the others
-        loss = entries<TWO>(g, row, share, r, by, weight, kept, columns, t, T, c0, c0 + kSegment, segment == 0);
+        loss = entries<TWO>(g, row, share, r, by, weight, kept, columns, t, T,
+                            p0 > at.s ? p0 - at.s : 0, p0 + kSegment - at.s, segment == 0);
     }
-    store_loss<T>(loss, g.row_loss + blockIdx.x);
+    store_loss<T>(g, loss);
 }
 
 __global__ __launch_bounds__(kBlock) void sum_losses(const double *parts, size_t n, float *loss) {
@@ -574,11 +621,11 @@ template <class F>
 void with_two(float hard, float temperature, F &&f) {
     using std::integral_constant;
     if (hard == 0.0f || temperature == 1.0f) f(integral_constant<Two, Two::kNo>{});
-    else if (temperature == 2.0f || temperature == 4.0f) f(integral_constant<Two, Two::kSquares>{});
+    else if (temperature == 2.0f) f(integral_constant<Two, Two::kSquares>{});
     else f(integral_constant<Two, Two::kYes>{});
 }
 
-// Calls f(W, NV, LONG as constants) for rows of n columns: the waves that hold them.
+// Calls f(W, NV, LONG as constants) for rows of n places: the waves that hold them.
 template <class F>
 void for_vocab(size_t n, F &&f) {
     using std::integral_constant;
@@ -598,16 +645,18 @@ bool by_segments(size_t rows, size_t vocab) { return vocab > 4096 && rows * 2 <=
 
 // Workgroups of distill_rows: as many as run at once, each with rows in turn (the next
 // one's values come in while the last one's gradients go out).
-size_t row_blocks(size_t rows, size_t vocab) {
-    const size_t per = vocab <= 1024 ? 4 : 1, need = (rows + per - 1) / per;
-    const size_t a_cu = vocab <= 1024 ? 6 : vocab <= 4096 ? 5 : vocab <= 8192 ? 4 : vocab <= 32768 ? 2 : 1;
+size_t row_blocks(size_t rows, size_t places) {
+    const size_t per = places <= 1024 ? 4 : 1, need = (rows + per - 1) / per;
+    const size_t a_cu = places <= 1024 ? 6 : places <= 4096 ? 5 : places <= 8192 ? 4 : places <= 32768 ? 2 : 1;
     const size_t cap = static_cast<size_t>(device_cu_count()) * a_cu;
     return need < cap ? need : cap;
 }
 
-size_t segments_of(size_t vocab) { return (vocab + kSegment - 1) / kSegment; }
+constexpr size_t kWaveVocab = 1024;  // a wave's row, at most
 
-constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 29, kMaxRows = size_t(1) << 31;
+size_t segments_of(size_t vocab) { return (vocab + 31 + kSegment - 1) / kSegment; }
+
+constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 28, kMaxRows = size_t(1) << 31;
 
 }  // namespace
 
@@ -620,12 +669,13 @@ extern "C" {
 size_t ts_hip_distillation_workspace_floats(size_t rows, size_t vocab) {
     if (!rows || !vocab) return 0;
     if (by_segments(rows, vocab)) return 6 * rows * segments_of(vocab);  // sums, losses
-    return 2 * row_blocks(rows, vocab);
+    return 2 * std::max(row_blocks(rows, vocab), row_blocks(rows, vocab + 31));
 }
 
 int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const int32_t *indices, const float *teacher, size_t kept,
                         float temperature, const int32_t *labels, float hard, const float *weights, const float *go, float *loss,
-                        float *dlogits, unsigned long long *bad, float *workspace, size_t workspace_floats, void *stream) {
+                        float *dlogits, unsigned long long *bad, float *workspace, size_t workspace_floats, unsigned *ticket,
+                        void *stream) {
     const double t = temperature;
     if (!(t > 0.0) || !(t * t <= 3e38) || !(t * t >= 1e-36) || !(hard >= 0.0f && hard <= 1.0f) || kept > kMaxKept || vocab > kMaxVocab ||
         rows >= kMaxRows || (hard > 0.0f && !labels && rows))
@@ -645,6 +695,8 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
     g.labels = hard > 0.0f ? labels : nullptr;
     g.dlogits = dlogits;
     g.bad = bad;
+    g.loss = loss;
+    g.ticket = ticket;
     g.rows = rows;
     g.vocab = vocab;
     g.kept = static_cast<int>(kept);
@@ -666,15 +718,18 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
         parts = rows * g.segments;
     } else {
         g.row_loss = reinterpret_cast<double *>(workspace);
-        parts = row_blocks(rows, vocab);
-        for_vocab(vocab, [&](auto w, auto nv, auto lng) {
+        // a row's places: its columns, and where waves share it those before it in its first line
+        const size_t before = vocab % 32 ? 31 : reinterpret_cast<uintptr_t>(logits) / 4 % 32;
+        const size_t places = vocab <= kWaveVocab ? vocab : vocab + before;
+        parts = row_blocks(rows, places);
+        for_vocab(places, [&](auto w, auto nv, auto lng) {
             const dim3 grid(static_cast<unsigned>(parts)), block(kThreads<w.value>);
             with_two(hard, temperature, [&](auto two) {
                 launch((distill_rows<w.value, nv.value, two.value, lng.value>), grid, block, 0, s, g);
             });
         });
     }
-    launch(sum_losses, dim3(1), dim3(kBlock), 0, s, static_cast<const double *>(g.row_loss), parts, loss);
+    if (!ticket) launch(sum_losses, dim3(1), dim3(kBlock), 0, s, static_cast<const double *>(g.row_loss), parts, loss);
     return launch_status();
 }
 
