@@ -16,7 +16,8 @@
 // shared out by segments of columns, by two launches.  The teacher's entries and the
 // label have a thread each: it adds their term to its part of the loss, and stores the
 // gradient there after the others are stored (an index given twice: the first entry's,
-// with both).  Sums past a lane are f64.
+// with both).  A softmax's terms are added in fp32, by lanes, waves and segments; the
+// loss in f64.
 #include <algorithm>
 #include <type_traits>
 
@@ -29,7 +30,8 @@ namespace {
 typedef float df4_t __attribute__((ext_vector_type(4), aligned(4)));
 
 // The softmaxes of a call: one (at T, or at 1); that at T and that at 1; the same at T = 2,
-// where the terms of that at 1 are the squares of the other's.  SQ_US
+// where the terms of that at 1 are the squares of the other's.  8192 x 32768: 450 us,
+// 478 by exponentials.
 enum class Two { kNo, kYes, kSquares };
 
 constexpr float kLog2e = 1.44269504f;
@@ -53,58 +55,75 @@ struct DistillArgs {
 };
 
 __device__ __forceinline__ float pow2_of(float v, float from, float c) { return __builtin_amdgcn_exp2f((v - from) * c); }
-__device__ __forceinline__ float wave_max(float m) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    return m;
+// A wave's maximum and sum, in a fixed order, in every lane.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143;
+__device__ __forceinline__ float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp<kShr1>(v, v));
+    v = fmaxf(v, dpp<kShr2>(v, v));
+    v = fmaxf(v, dpp<kShr4>(v, v));
+    v = fmaxf(v, dpp<kShr8>(v, v));
+    v = fmaxf(v, dpp<kBcast15, 0xa>(v, v));
+    v = fmaxf(v, dpp<kBcast31, 0xc>(v, v));
+    return last_lane(v);
+}
+__device__ __forceinline__ float wave_add(float v) {
+    v += dpp<kShr1>(0.0f, v);
+    v += dpp<kShr2>(0.0f, v);
+    v += dpp<kShr4>(0.0f, v);
+    v += dpp<kShr8>(0.0f, v);
+    v += dpp<kBcast15, 0xa>(0.0f, v);
+    v += dpp<kBcast31, 0xc>(0.0f, v);
+    return last_lane(v);
 }
 // where to count from: anything, where there is nothing but -inf
 __device__ __forceinline__ float origin(float largest) { return largest == kNone ? 0.0f : largest; }
 // a sum against `from` in terms of `to` (of nothing, or of NaN alone: itself)
-__device__ __forceinline__ double rebased(double s, float from, float to, float c) {
+__device__ __forceinline__ float rebased(float s, float from, float to, float c) {
     return from == kNone ? s : s * pow2_of(from, to, c);
 }
 
 // What is known of a row: the softmax's M and S (and S1), the teacher's b and A.
 struct RowSums {
-    float m, b;
-    double s, s1, a;
+    float m, b, s, s1, a;
 };
+constexpr RowSums kNothing = {kNone, kNone, 0.0f, 0.0f, 0.0f};
 
 // Sums of lanes joined to a wave's (in every lane).
 template <Two TWO>
 __device__ __forceinline__ void join_lanes(RowSums &r, float c) {
-    const float m = wave_max(r.m);
-    r.s = wave_sum(rebased(r.s, r.m, m, c));
-    if (TWO != Two::kNo) r.s1 = wave_sum(rebased(r.s1, r.m, m, kLog2e));
+    const float m = wave_max(r.m), b = wave_max(r.b);
+    r.s = wave_add(rebased(r.s, r.m, m, c));
+    if (TWO != Two::kNo) r.s1 = wave_add(rebased(r.s1, r.m, m, kLog2e));
+    r.a = wave_add(rebased(r.a, r.b, b, c));
     r.m = m;
-}
-__device__ __forceinline__ void join_teacher(RowSums &r, float c) {
-    const float b = wave_max(r.b);
-    r.a = wave_sum(rebased(r.a, r.b, b, c));
     r.b = b;
 }
-// ... and waves' to the row's.
+// ... and waves' to the row's: eight lanes, or four, have a wave's each.
 template <Two TWO, int W>
 __device__ __forceinline__ void join_waves(RowSums &r, RowSums *lds, float c) {
+    static_assert(W == 1 || W == 4 || W == 8, "neighbouring lanes");
     if (W == 1) return;
     __syncthreads();  // the last row's reads
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = r;
     __syncthreads();
-    RowSums all = {kNone, kNone, 0.0, 0.0, 0.0};
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        all.m = fmaxf(all.m, lds[w].m);
-        all.b = fmaxf(all.b, lds[w].b);
-    }
-#pragma unroll 4
-    for (int w = 0; w < W; ++w) {
-        const RowSums one = lds[w];
-        all.s += rebased(one.s, one.m, all.m, c);
-        if (TWO != Two::kNo) all.s1 += rebased(one.s1, one.m, all.m, kLog2e);
-        all.a += rebased(one.a, one.b, all.b, c);
-    }
-    r = all;
+    const RowSums one = lds[threadIdx.x % W];
+    auto join = [](float v, auto &&f) {
+        v = f(v, dpp<0xB1>(v, v));  // lanes 1 0 3 2
+        v = f(v, dpp<0x4E>(v, v));  // lanes 2 3 0 1
+        return W == 8 ? f(v, dpp<0x141>(v, v)) : v;  // eight lanes mirrored
+    };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto sum = [](float x, float y) { return x + y; };
+    r.m = join(one.m, larger);
+    r.b = join(one.b, larger);
+    r.s = join(rebased(one.s, one.m, r.m, c), sum);
+    if (TWO != Two::kNo) r.s1 = join(rebased(one.s1, one.m, r.m, kLog2e), sum);
+    r.a = join(rebased(one.a, one.b, r.b, c), sum);
 }
 
 // A row's share of the loss and its gradients' coefficients: zero where it has none.
@@ -150,7 +169,7 @@ __device__ __forceinline__ RowShare row_share(const DistillArgs &g, size_t row, 
     return s;
 }
 
-// The teacher's entries first + 0, + step, ... of a row, as a lane's sums (f64).
+// The teacher's entries first + 0, + step, ... of a row, as a lane's sums.
 __device__ __forceinline__ Entry teacher_sums(const DistillArgs &g, size_t row, const RowShare &share, const RowInput &in, int first,
                                               int step, RowSums &r, int *columns) {
     const size_t at = row * g.kept;
@@ -192,23 +211,22 @@ struct Gradient {
 };
 template <Two TWO>
 __device__ __forceinline__ Gradient gradient(const RowShare &share, const RowSums &r, float weight) {
-    const double soft = r.a != 0.0 ? static_cast<double>(weight) * share.soft : 0.0, hard = static_cast<double>(weight) * share.hard;
-    const bool none = soft == 0.0 && hard == 0.0;
-    if (TWO != Two::kNo)
-        return {r.m, soft == 0.0 ? 0.0f : static_cast<float>(soft / r.s), hard == 0.0 ? 0.0f : static_cast<float>(hard / r.s1), none};
-    return {r.m, static_cast<float>((soft + hard) / r.s), 0.0f, none};
+    const float soft = r.a != 0.0f ? weight * share.soft : 0.0f, hard = weight * share.hard;
+    const bool none = soft == 0.0f && hard == 0.0f;
+    if (TWO != Two::kNo) return {r.m, soft == 0.0f ? 0.0f : soft / r.s, hard == 0.0f ? 0.0f : hard / r.s1, none};
+    return {r.m, (soft + hard) / r.s, 0.0f, none};
 }
 
 // ln x of a sum: its power of two in f64, and the rest, from 3/4 to 3/2, by the fp32
 // instruction, within 2^-24 or so
-__device__ __forceinline__ double ln(double x) {
-    int e;
-    double f = frexp(x, &e);  // [1/2, 1)
-    if (f < 0.75) {
-        f *= 2.0;
+__device__ __forceinline__ double ln(float x) {
+    int e = __builtin_amdgcn_frexp_expf(x);
+    float f = __builtin_amdgcn_frexp_mantf(x);  // [1/2, 1)
+    if (f < 0.75f) {
+        f *= 2.0f;
         --e;
     }
-    return 0.6931471805599453 * (e + static_cast<double>(__builtin_amdgcn_logf(static_cast<float>(f))));
+    return 0.6931471805599453 * (e + static_cast<double>(__builtin_amdgcn_logf(f)));
 }
 
 // The entries of a row in columns from .. to, by threads first + 0, + step, ...: their
@@ -220,19 +238,19 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
                                           int step, size_t from, size_t to, bool own) {
     const size_t at = row * g.kept;
     const float *z = g.logits + row * g.vocab;
-    const bool asked = share.soft != 0.0f && r.a != 0.0;
-    const double per_e = asked ? static_cast<double>(share.soft) / r.a : 0.0;
+    const bool asked = share.soft != 0.0f && r.a != 0.0f;
+    const float per_e = asked ? share.soft / r.a : 0.0f;
     double loss = 0.0;
     if (first == 0 && own && asked) loss = static_cast<double>(share.soft) * g.temperature * (ln(r.s) - ln(r.a));
-    auto takes = [&](float t) { return asked ? per_e * pow2_of(t, r.b, g.c) : 0.0; };  // of the gradient, without its weight
+    auto takes = [&](float t) { return asked ? per_e * pow2_of(t, r.b, g.c) : 0.0f; };  // of the gradient, without its weight
     for (int k = first; k <= g.kept; k += step) {
         const bool label = k == g.kept;
         const int j = k == first ? kept.j : label ? share.label : columns[k];
         if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
         const float t = label ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = k == first ? kept.z : z[j];
-        double sum = label ? static_cast<double>(share.hard) : takes(t);
+        float sum = label ? share.hard : takes(t);
         if (label) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
-        else if (sum != 0.0) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
+        else if (sum != 0.0f) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
         if (!g.dlogits) continue;
         int same = 0;  // the teacher's entries of this column
 #pragma unroll 2
@@ -251,7 +269,7 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
             }
             if (j == share.label) sum += share.hard;
         }
-        if (mine) g.dlogits[row * g.vocab + j] = by.at<TWO>(zj, g.c) - static_cast<float>(weight * sum);
+        if (mine) g.dlogits[row * g.vocab + j] = by.at<TWO>(zj, g.c) - weight * sum;
     }
     return loss * share.weight;
 }
@@ -302,7 +320,7 @@ __device__ __forceinline__ void store_loss(const DistillArgs &g, double loss) {
 
 // Where a row's columns stand: column c at place c + s, counted from the line of 128 bytes
 // that its first value is in, so that a wave's quads of places are whole lines (rows of
-// 50001: ALIGN_US).  The quads that lie within the row are read and written by the buffer
+// 50001: 999 of them 108 us as they lie, 103 so).  The quads that lie within the row are read and written by the buffer
 // instructions; the columns before the first and after the last, three each at most, are
 // the edge, lanes 0 .. 5's.
 struct Places {
@@ -450,7 +468,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         float *dz = g.dlogits ? g.dlogits + row * g.vocab : nullptr;
         const Places at(z, n, W > 1), after(next, n, W > 1);
         const unsigned last = LONG ? (at.end() - 1) / span * span : 0;  // the first of the places held at the row's end
-        RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
+        RowSums r = kNothing;
         float largest[kChunks<NV>];  // HOLD: what the columns held are against
         if (share.weight != 0.0f) {
             turn ^= 1;
@@ -467,7 +485,6 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
             }
             add_value<TWO>(edge, g.c, r);
             join_lanes<TWO>(r, g.c);
-            join_teacher(r, g.c);
             join_waves<TWO, W>(r, lds, g.c);
         }
         const float weight = share.weight * go;
@@ -536,7 +553,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillAr
     __shared__ RowSums lds[kSegWaves];
     const size_t row = blockIdx.x / g.segments;
     const unsigned p0 = blockIdx.x % g.segments * kSegment;
-    RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
+    RowSums r = kNothing;
     const float *z = g.logits + row * g.vocab;
     const Places at(z, static_cast<unsigned>(g.vocab));
     df4_t v[kSegQuads];
@@ -548,7 +565,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segment_sums(DistillAr
     if (edge < at.n) add_value<TWO>(z[edge], g.c, r);
     join_lanes<TWO>(r, g.c);
     join_waves<TWO, kSegWaves>(r, lds, g.c);
-    if (threadIdx.x == 0) g.parts[blockIdx.x] = make_float4(r.m, static_cast<float>(r.s), static_cast<float>(r.s1), 0.0f);
+    if (threadIdx.x == 0) g.parts[blockIdx.x] = make_float4(r.m, r.s, r.s1, 0.0f);
 }
 
 template <Two TWO>
@@ -566,7 +583,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     const bool asked = share.weight != 0.0f;
     Entry kept = {-1, kNone, 0.0f};
     df4_t v[kSegQuads];
-    RowSums r = {kNone, kNone, 0.0, 0.0, 0.0};
+    RowSums r = kNothing;
     if (asked) {
         if (g.dlogits) load_quads<T, kSegQuads>(RowBuffer(z, at, true), p0, t, v);
         for (int k = t; k < g.segments; k += T) {
@@ -578,7 +595,6 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
         }
         kept = teacher_sums(g, row, share, in, t, T, r, columns);
         join_lanes<TWO>(r, g.c);
-        join_teacher(r, g.c);
         join_waves<TWO, kSegWaves>(r, lds, g.c);
     }
     const float weight = share.weight * (g.go ? *g.go : 1.0f);
@@ -633,6 +649,7 @@ void for_vocab(size_t n, F &&f) {
     if (n <= 256) f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, held);
     else if (n <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 2>{}, held);
     else if (n <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 4>{}, held);
+    else if (n <= 2048) f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, held);
     else if (n <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 4>{}, held);
     else if (n <= 8192) f(integral_constant<int, 4>{}, integral_constant<int, 8>{}, held);
     else if (n <= 16384) f(integral_constant<int, 8>{}, integral_constant<int, 8>{}, held);
@@ -641,7 +658,14 @@ void for_vocab(size_t n, F &&f) {
     else f(integral_constant<int, 8>{}, integral_constant<int, 32>{}, integral_constant<bool, true>{});
 }
 
-bool by_segments(size_t rows, size_t vocab) { return vocab > 4096 && rows * 2 <= static_cast<size_t>(device_cu_count()); }
+// By segments where that is less, in us, as measured by rows and by segments: 16 x 50000
+// 15.2, 12.1; 32 x 50000 15.8, 15.4; 16 x 131072 24, 13.6; 64 x 131072 27, 27; and not
+// 16 x 32000 11.2, 11.1; 64 x 16000 9.4, 12.7; 128 x 50000 19, 23; 96 x 131072 29, 35.
+bool by_segments(size_t rows, size_t vocab) {
+    const size_t cus = device_cu_count(), rounds = (rows + cus - 1) / cus;
+    const double n = static_cast<double>(vocab);
+    return vocab > 4096 && 11 + 2e-6 * n * static_cast<double>(rows) < 6 + 1.7e-4 * n * static_cast<double>(rounds);
+}
 
 // Workgroups of distill_rows: as many as run at once, each with rows in turn (the next
 // one's values come in while the last one's gradients go out).
@@ -655,6 +679,11 @@ size_t row_blocks(size_t rows, size_t places) {
 constexpr size_t kWaveVocab = 1024;  // a wave's row, at most
 
 size_t segments_of(size_t vocab) { return (vocab + 31 + kSegment - 1) / kSegment; }
+
+// Workgroups whose tickets take less than another launch: 8192 x 1001 (1536 of them) 30 us
+// with it, 20 by two launches; 8 x
+// 131072 (264) 13.3 and 14.9.
+constexpr size_t kTicketParts = 512;
 
 constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 28, kMaxRows = size_t(1) << 31;
 
@@ -696,7 +725,6 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
     g.dlogits = dlogits;
     g.bad = bad;
     g.loss = loss;
-    g.ticket = ticket;
     g.rows = rows;
     g.vocab = vocab;
     g.kept = static_cast<int>(kept);
@@ -706,22 +734,25 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
     g.hard = hard;
     const hipStream_t s = as_stream(stream);
     size_t parts;
+    auto with_ticket = [&] { g.ticket = parts <= kTicketParts ? ticket : nullptr; };
     if (by_segments(rows, vocab)) {
         g.segments = static_cast<int>(segments_of(vocab));
         g.parts = reinterpret_cast<float4 *>(workspace);
         g.row_loss = reinterpret_cast<double *>(workspace + 4 * rows * g.segments);
-        const dim3 grid(static_cast<unsigned>(rows * g.segments)), block(64 * kSegWaves);
+        parts = rows * g.segments;
+        with_ticket();
+        const dim3 grid(static_cast<unsigned>(parts)), block(64 * kSegWaves);
         with_two(hard, temperature, [&](auto two) {
             launch(distill_segment_sums<two.value>, grid, block, 0, s, g);
             launch(distill_segments<two.value>, grid, block, 0, s, g);
         });
-        parts = rows * g.segments;
     } else {
         g.row_loss = reinterpret_cast<double *>(workspace);
         // a row's places: its columns, and where waves share it those before it in its first line
         const size_t before = vocab % 32 ? 31 : reinterpret_cast<uintptr_t>(logits) / 4 % 32;
         const size_t places = vocab <= kWaveVocab ? vocab : vocab + before;
         parts = row_blocks(rows, places);
+        with_ticket();
         for_vocab(places, [&](auto w, auto nv, auto lng) {
             const dim3 grid(static_cast<unsigned>(parts)), block(kThreads<w.value>);
             with_two(hard, temperature, [&](auto two) {
@@ -729,7 +760,7 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
             });
         });
     }
-    if (!ticket) launch(sum_losses, dim3(1), dim3(kBlock), 0, s, static_cast<const double *>(g.row_loss), parts, loss);
+    if (!g.ticket) launch(sum_losses, dim3(1), dim3(kBlock), 0, s, static_cast<const double *>(g.row_loss), parts, loss);
     return launch_status();
 }
 
