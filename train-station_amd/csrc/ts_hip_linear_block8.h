@@ -1,0 +1,55 @@
+// What the layers over blocks of 128 in 8 bits share (ts_hip_linear_block8.hip: the
+// entries and few rows; ts_hip_linear_block8_tiles.hip: the large ones).
+#pragma once
+
+#include "ts_hip_block8.h"
+#include "ts_hip_linear.h"
+
+namespace tship {
+
+struct Block8Product {
+    const uint8_t *xc, *wc;
+    const float *xs, *ws;
+    const float *bias, *residual;
+    float *y;
+    int M, N, groups, act;  // groups of 128 k
+    int tiles_m, tiles_n;
+};
+
+// y's four neighbouring columns of one row from their sums; cols of them are there
+__device__ __forceinline__ void block8_output(const Block8Product &p, float *to, const f4v_t &sum, const float (&bias)[4],
+                                              const float (&extra)[4], int cols) {
+    float o[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        float v = sum[r], slope;
+        if (p.bias) v += bias[r];
+        v = activate<false>(v, p.act, slope);
+        if (p.residual) v += extra[r];
+        o[r] = v;
+    }
+    if (cols >= 4) {
+        *reinterpret_cast<pk4u_t *>(to) = pk4u_t{o[0], o[1], o[2], o[3]};
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < cols) to[r] = o[r];
+    }
+}
+
+// four floats at c of a row of n (past it: zeros)
+__device__ __forceinline__ void read4(const float *row, size_t c, size_t n, float (&v)[4]) {
+    if (c + 4 <= n) {
+        const pk4u_t q = *reinterpret_cast<const pk4u_t *>(row + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < n ? row[c + e] : 0.0f;
+    }
+}
+
+bool block8_tiles_take(size_t M, size_t N, size_t K);
+void block8_tiles(const Block8Product &p, hipStream_t s);
+
+}  // namespace tship

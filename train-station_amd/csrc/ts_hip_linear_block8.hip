@@ -8,8 +8,7 @@
 // whose sums are fp32 (the 8-bit instructions drop what is 2^-13 below the largest of
 // eight products: ts_hip_linear_packed.hip), and joined to y by one fused multiply-add
 // with the two scales' product.
-#include "ts_hip_block8.h"
-#include "ts_hip_linear.h"
+#include "ts_hip_linear_block8.h"
 
 namespace tship {
 
@@ -18,17 +17,6 @@ namespace {
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
 
 // ---- packing -----------------------------------------------------------------------
-
-__device__ __forceinline__ void read4(const float *row, size_t c, size_t cols, float (&v)[4]) {
-    if (c + 4 <= cols) {
-        const pk4u_t q = *reinterpret_cast<const pk4u_t *>(row + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = q[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? row[c + e] : 0.0f;
-    }
-}
 
 // A scale per row: a thread packs a quad, a grid stride over all quads (32 lanes a block).
 __global__ __launch_bounds__(kBlock) void block8_rows(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
@@ -44,7 +32,7 @@ __global__ __launch_bounds__(kBlock) void block8_rows(const float *__restrict__ 
 }
 
 // A scale per 128 rows: a workgroup a block, a thread every eighth row's quad.
-__global__ __launch_bounds__(kBlock) void block8_tiles(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
+__global__ __launch_bounds__(kBlock) void block8_by_tiles(const float *__restrict__ x, size_t rows, size_t cols, size_t pitch,
                                                        uint8_t *__restrict__ codes, float *__restrict__ scales) {
     __shared__ float lds[kBlock / 64];
     const size_t groups = pitch / kPackGroup, tiles = (rows + kPackGroup - 1) / kPackGroup;
@@ -97,15 +85,6 @@ __global__ __launch_bounds__(kBlock) void block8_values(const uint8_t *__restric
 }
 
 // ---- few rows ------------------------------------------------------------------------
-
-struct Block8Product {
-    const uint8_t *xc, *wc;
-    const float *xs, *ws;
-    const float *bias, *residual;
-    float *y;
-    int M, N, groups, act;  // groups of 128 k
-    int tiles_n;
-};
 
 // A wave has FN blocks of 16 columns and FM of 16 rows, W's rows as the instruction's A
 // operand, so that a lane ends with four neighbouring columns of one row; KG waves share K.
@@ -205,23 +184,9 @@ __global__ __launch_bounds__(64 * KG) void block8_direct(Block8Product p) {
             const int i = i0 + 16 * b + li;
             if (i >= p.M) continue;
             const size_t at = static_cast<size_t>(i) * p.N;
-            float extra[4] = {}, o[4];
+            float extra[4] = {};
             if (p.residual) read4(p.residual + at, j, p.N, extra);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v = acc[a][b][r], slope;
-                if (p.bias) v += bias[r];
-                v = activate<false>(v, p.act, slope);
-                if (p.residual) v += extra[r];
-                o[r] = v;
-            }
-            if (cols == 4) {
-                *reinterpret_cast<pk4u_t *>(p.y + at + j) = pk4u_t{o[0], o[1], o[2], o[3]};
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (r < cols) p.y[at + j + r] = o[r];
-            }
+            block8_output(p, p.y + at + j, acc[a][b], bias, extra, cols);
         }
     }
 }
@@ -263,7 +228,7 @@ int ts_hip_block8(const float *x, size_t rows, size_t cols, int tiles, uint8_t *
     const size_t pitch = packed_pitch(cols);
     if (tiles) {
         const size_t blocks = pitch / kPackGroup * ts_hip_block8_scale_rows(rows, 1);
-        launch(block8_tiles, dim3(static_cast<unsigned>(blocks < kMaxTileBlocks ? blocks : kMaxTileBlocks)), dim3(kBlock), 0,
+        launch(block8_by_tiles, dim3(static_cast<unsigned>(blocks < kMaxTileBlocks ? blocks : kMaxTileBlocks)), dim3(kBlock), 0,
                as_stream(stream), x, rows, cols, pitch, codes, scales);
     } else {
         launch(block8_rows, dim3(grid_for(rows * pitch / 4)), dim3(kBlock), 0, as_stream(stream), x, rows, cols, pitch, codes,
@@ -293,9 +258,10 @@ int ts_hip_linear_block8(const uint8_t *x_codes, const float *x_scales, const ui
     if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;
     if (workspace_floats < ts_hip_linear_block8_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
     const Block8Product p = {x_codes, w_codes, x_scales, w_scales, bias, residual, y, static_cast<int>(batch),
-                             static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0};
+                             static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0, 0};
     (void)workspace;
-    if (batch <= 16) launch_direct<1, 1>(p, as_stream(stream));
+    if (block8_tiles_take(batch, fan_out, fan_in)) block8_tiles(p, as_stream(stream));
+    else if (batch <= 16) launch_direct<1, 1>(p, as_stream(stream));
     else launch_direct<2, 2>(p, as_stream(stream));
     return launch_status();
 }

@@ -1,0 +1,197 @@
+// A layer over values in 8 bits with a scale per block of 128, large ones: tiles of BM x
+// BN by WM x WN waves (the formula: ts_hip_linear_block8.hip).
+//
+// A stage is one block of 128 columns k of the tile's rows of x and W: codes as they lie,
+// by DMA of 16 bytes a lane into LDS, NST stages on their way.  A row's chunk c of 16
+// codes stands at c ^ row / 2 % 8, so that the reads of one chunk of 32 rows fall on all
+// banks.  A wave reads sixteen codes at a time and widens them to bf16 between its
+// matrix instructions; a stage's products of 32 x 32 sums are added from zero and
+// joined to the tile's by one multiply-add a sum with the row's scale times the tile's.
+// W's rows are the instruction's A operand: a lane has one row of x, whose scale is one
+// value, and W's is the same for all of the tile, which lies within 128 of its rows.
+#include "ts_hip_linear_block8.h"
+#include "ts_hip_gemm_split.h"
+
+namespace tship {
+
+namespace {
+
+constexpr int kRowsA = 32;  // of an instruction's operand
+
+template <int BM, int BN, int WM, int WN, int NST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void block8_tile(Block8Product g) {
+    constexpr int NW = WM * WN, FM = BM / WM / kRowsA, FN = BN / WN / kRowsA;  // blocks of a wave: of x's rows, of W's
+    constexpr int kXUnits = BM / 8, kUnits = kXUnits + BN / 8, kPer = kUnits / NW;  // DMA instructions: 8 rows of 128 codes
+    constexpr int kScaleUnits = BM / 64 + 1;  // 64 rows' scales each, and the tile's
+    constexpr int kScalesAt = kUnits * 1024, kStage = kScalesAt + kScaleUnits * 256;
+    static_assert(kUnits % NW == 0 && kScaleUnits <= NW, "units of a wave");
+    static_assert(NST * kStage >= BM * BN * 4 && kPackGroup % BN == 0, "room for the tile, within one of W's");
+    __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
+
+    int tm, tn;
+    tile_coords(g.tiles_m, g.tiles_n, static_cast<int>(blockIdx.x), tm, tn);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN, li = lane & 31, lh = lane >> 5;
+    const int i0 = tm * BM, j0 = tn * BN;
+    const size_t pitch = static_cast<size_t>(g.groups) * kPackGroup;
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char *)lds));
+
+    // this wave's units of a stage: a lane's row (past an edge: the last one's) and chunk
+    const uint8_t *src[kPer];
+    unsigned off[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+        const int f = wave * kPer + u;
+        const bool x = f < kXUnits;  // uniform
+        const int first = x ? i0 : j0, last = (x ? g.M : g.N) - 1 - first, row = (x ? f : f - kXUnits) * 8 + (lane >> 3);
+        src[u] = (x ? g.xc : g.wc) + static_cast<size_t>(first) * pitch;
+        off[u] = static_cast<unsigned>(min(row, last)) * static_cast<unsigned>(pitch) + 16u * ((lane & 7) ^ (row >> 1 & 7));
+    }
+    const int scale_unit = min(wave, kScaleUnits - 1);  // (the waves past the units: the last one's again)
+    const bool of_x = scale_unit < kScaleUnits - 1;     // uniform
+    const float *const scale_src = of_x ? g.xs + i0 : g.ws + j0 / kPackGroup;
+    const size_t scale_step = of_x ? g.M : (g.N + kPackGroup - 1) / kPackGroup;
+    const unsigned scale_off = of_x ? 4u * static_cast<unsigned>(min(scale_unit * 64 + lane, g.M - 1 - i0)) : 0u;
+    auto dma = [&](int stage, int slot) {
+        const int at = min(stage, g.groups - 1);  // past the end: the last again
+        const unsigned base = lds0 + slot * kStage;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+#pragma unroll
+        for (int u = 0; u < kPer; ++u)
+            asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[u]),
+                         "s"(src[u] + static_cast<size_t>(at) * kPackGroup), "s"(base + (wave * kPer + u) * 1024)
+                         : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(scale_off), "s"(scale_src + at * scale_step),
+                     "s"(base + kScalesAt + scale_unit * 256)
+                     : "memory", "m0");
+#pragma clang diagnostic pop
+    };
+    // codes 32 k + 16 lh .. of row li of block b of 32 rows
+    auto codes16 = [&](const char *at, int b, int k) {
+        return *reinterpret_cast<const u4v_t *>(at + b * 4096 + li * 128 + 16 * ((2 * k + lh) ^ (li >> 1 & 7)));
+    };
+
+    floatx16 acc[FN][FM];
+#pragma unroll
+    for (int a = 0; a < FN; ++a)
+#pragma unroll
+        for (int b = 0; b < FM; ++b) acc[a][b] = floatx16{};
+    int slot = 0;
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s) dma(s, s);
+    for (int s = 0; s < g.groups; ++s) {
+        // this stage has landed, and every wave is done with the one before
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kPer + 1) * (NST - 2)) : "memory");
+        dma(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+        const char *xa = lds + slot * kStage, *wa = xa + kXUnits * 1024;
+        const float *scales = reinterpret_cast<const float *>(xa + kScalesAt);
+        float by[FM];
+#pragma unroll
+        for (int b = 0; b < FM; ++b) by[b] = scales[(wm * FM + b) * kRowsA + li] * scales[(kScaleUnits - 1) * 64];
+        floatx16 part[FN][FM];
+#pragma unroll
+        for (int a = 0; a < FN; ++a)
+#pragma unroll
+            for (int b = 0; b < FM; ++b) part[a][b] = floatx16{};
+#pragma unroll
+        for (int k = 0; k < kPackGroup / 32; ++k) {
+            u4v_t cw[FN], cx[FM];
+#pragma unroll
+            for (int a = 0; a < FN; ++a) cw[a] = codes16(wa, wn * FN + a, k);
+#pragma unroll
+            for (int b = 0; b < FM; ++b) cx[b] = codes16(xa, wm * FM + b, k);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // (the same order of k on both sides)
+                bf8_t fw[FN], fx[FM];
+#pragma unroll
+                for (int a = 0; a < FN; ++a) fw[a] = widen(cw[a][2 * h], cw[a][2 * h + 1], 1.0f);
+#pragma unroll
+                for (int b = 0; b < FM; ++b) fx[b] = widen(cx[b][2 * h], cx[b][2 * h + 1], 1.0f);
+#pragma unroll
+                for (int a = 0; a < FN; ++a)
+#pragma unroll
+                    for (int b = 0; b < FM; ++b)
+                        part[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[a], fx[b], part[a][b], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < FN; ++a)
+#pragma unroll
+            for (int b = 0; b < FM; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[a][b][r] = __builtin_fmaf(part[a][b][r], by[b], acc[a][b][r]);
+        slot = slot + 1 == NST ? 0 : slot + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outstanding at exit
+
+    // The tile by LDS (lane (li, lh), registers 4 q .. of block (a, b): row li, columns 8 q +
+    // 4 lh ..; a row's quad c at c ^ row, so that a column's are in different banks), then by
+    // rows, four columns a lane.  A turn's residual is on its way while the one before is computed.
+    constexpr int kQuads = BN / 4, kStep = 64 * NW / kQuads, kRows = BM / kStep < 4 ? BM / kStep : 4, kTurns = BM / kStep / kRows;
+    static_assert(kTurns * kStep * kRows == BM, "turns of kRows rows a lane");
+    f4v_t *const sums = reinterpret_cast<f4v_t *>(lds);
+    const int q = static_cast<int>(threadIdx.x) % kQuads, j = j0 + 4 * q, row0 = static_cast<int>(threadIdx.x) / kQuads;
+    const int cols = min(4, g.N - j), last = g.M - 1 - i0;
+    float ev[kRows][4];
+    auto fetch = [&](int turn) {
+#pragma unroll
+        for (int t = 0; t < kRows; ++t)  // (rows past the edge: the last one's)
+            read4(g.residual + static_cast<size_t>(i0 + min((turn * kRows + t) * kStep + row0, last)) * g.N, j, g.N, ev[t]);
+    };
+    float bias[4] = {};
+    if (cols > 0) {
+        if (g.residual) fetch(0);
+        if (g.bias) read4(g.bias, j, g.N, bias);
+    }
+    __syncthreads();  // the last codes
+#pragma unroll
+    for (int a = 0; a < FN; ++a)
+#pragma unroll
+        for (int b = 0; b < FM; ++b)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int row = (wm * FM + b) * kRowsA + li, quad = (wn * FN + a) * 8 + 2 * c + lh;
+                sums[row * kQuads + (quad ^ (row & kQuads - 1))] =
+                    f4v_t{acc[a][b][4 * c], acc[a][b][4 * c + 1], acc[a][b][4 * c + 2], acc[a][b][4 * c + 3]};
+            }
+    __syncthreads();
+    if (cols <= 0) return;  // (no barrier follows)
+#pragma unroll 1
+    for (int turn = 0; turn < kTurns; ++turn) {
+        float now[kRows][4];
+#pragma unroll
+        for (int t = 0; t < kRows; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) now[t][e] = ev[t][e];
+        if (g.residual && turn + 1 < kTurns) fetch(turn + 1);
+#pragma unroll
+        for (int t = 0; t < kRows; ++t) {
+            const int row = (turn * kRows + t) * kStep + row0;
+            if (row > last) continue;
+            block8_output(g, g.y + static_cast<size_t>(i0 + row) * g.N + j, sums[row * kQuads + (q ^ (row & kQuads - 1))], bias, now[t],
+                          cols);
+        }
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int NST>
+void launch_tile(Block8Product p, hipStream_t s) {
+    p.tiles_m = (p.M + BM - 1) / BM;
+    p.tiles_n = (p.N + BN - 1) / BN;
+    launch((block8_tile<BM, BN, WM, WN, NST>), dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN), 0, s, p);
+}
+
+}  // namespace
+
+bool block8_tiles_take(size_t M, size_t N, size_t K) { return M >= 64 && N >= 64 && 2.0 * M * N * K >= 0.8e9; }
+
+void block8_tiles(const Block8Product &p, hipStream_t s) {
+    const size_t cus = device_cu_count();
+    auto tiles = [&](size_t bm, size_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };
+    if (tiles(128, 128) >= 2 * cus) launch_tile<128, 128, 2, 2, 2>(p, s);
+    else if (tiles(128, 64) >= 2 * cus) launch_tile<128, 64, 2, 2, 2>(p, s);
+    else launch_tile<64, 64, 2, 2, 2>(p, s);
+}
+
+}  // namespace tship
