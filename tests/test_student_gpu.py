@@ -118,6 +118,17 @@ def test_block8_linear(m, k, n, act, bias, residual):
     assert_within(y.data(), want, bound, "y")
 
 
+@pytest.mark.parametrize("m,k,n", [(64, 200, 8200), (8255, 100, 65), (1003, 1, 900), (2000, 150, 2101), (2011, 1153, 2080),
+                                   (2975, 130, 2801), (3001, 700, 2820)])
+def test_block8_linear_by_tiles(m, k, n):
+    """Each size of tile, with edges within it, one and several blocks of columns."""
+    x, xv = blocks(normal((m, k), 1))
+    w, wv = blocks(normal((n, k), 2, k ** -0.5), True)
+    b, r = normal((n,), 3, 0.1), normal((m, n), 4)
+    want, bound = R.linear(xv, wv, b, "silu", r)
+    assert_within(x.linear(w, tensor(b), "silu", tensor(r)).data(), want, bound, "y")
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 300, 140), (150, 300, 300), (1500, 900, 800)])
 def test_block8_linear_of_far_scales_and_odd_codes(m, k, n):
     """Rows and tiles of sizes far apart, and every row its own: a wrong row's or block's scale shows."""
@@ -135,6 +146,8 @@ def test_block8_linear_of_nothing_and_of_nan(m, n):
     X, W = T.Tensor.zeros((m, 0)).block8(), T.Tensor.zeros((n, 0)).block8(True)
     assert np.array_equal(X.linear(W, tensor(b), "relu", tensor(r)).data(), np.maximum(b, 0) + r)
     assert T.Tensor.zeros((0, 5)).block8().linear(T.Tensor.ones((4, 5)).block8(True)).shape == (0, 4)
+    large = T.Tensor.zeros((1100, 0)).block8().linear(T.Tensor.zeros((1030, 0)).block8(True)).data()
+    assert large.shape == (1100, 1030) and not large.any()
     x, w = normal((m, 1200), 1), normal((n, 1200), 2)
     x[1, 700] = np.nan
     y = tensor(x).block8().linear(tensor(w).block8(True)).data()

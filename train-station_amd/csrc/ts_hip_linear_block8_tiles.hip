@@ -9,6 +9,13 @@
 // joined to the tile's by one multiply-add a sum with the row's scale times the tile's.
 // W's rows are the instruction's A operand: a lane has one row of x, whose scale is one
 // value, and W's is the same for all of the tile, which lies within 128 of its rows.
+//
+// What bounds it: 8192 x 4096 x 4096 takes 306 us (325 with the residual), 0.90 PFLOP/s;
+// with codes of zero, the same instructions, 229: the chip's power, as the bf16 library
+// product of 8192^3 too has 1.65 PFLOP/s of zeros and 1.23 of values.  Small tiles are bound
+// by a stage's own chain (barrier, DMA, reads, widening, instructions: 0.45 us alone):
+// four stages on their way in place of two gain nothing, two groups of waves that
+// share a stage's k 3 to 8% (1999 x 1531 x 777 14.6 -> 13.8 us).
 #include "ts_hip_linear_block8.h"
 #include "ts_hip_gemm_split.h"
 
@@ -18,20 +25,21 @@ namespace {
 
 constexpr int kRowsA = 32;  // of an instruction's operand
 
-template <int BM, int BN, int WM, int WN, int NST>
-__global__ __launch_bounds__(64 * WM * WN, 2) void block8_tile(Block8Product g) {
-    constexpr int NW = WM * WN, FM = BM / WM / kRowsA, FN = BN / WN / kRowsA;  // blocks of a wave: of x's rows, of W's
+template <int BM, int BN, int WM, int WN, int NST, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void block8_tile(Block8Product g) {
+    constexpr int NW = WM * WN * KG, FM = BM / WM / kRowsA, FN = BN / WN / kRowsA;  // blocks of a wave: of x's rows, of W's
     constexpr int kXUnits = BM / 8, kUnits = kXUnits + BN / 8, kPer = kUnits / NW;  // DMA instructions: 8 rows of 128 codes
+    constexpr int kSteps = kPackGroup / 32 / KG;  // of a wave: the KG groups share a stage's k
     constexpr int kScaleUnits = BM / 64 + 1;  // 64 rows' scales each, and the tile's
     constexpr int kScalesAt = kUnits * 1024, kStage = kScalesAt + kScaleUnits * 256;
     static_assert(kUnits % NW == 0 && kScaleUnits <= NW, "units of a wave");
-    static_assert(NST * kStage >= BM * BN * 4 && kPackGroup % BN == 0, "room for the tile, within one of W's");
+    static_assert(NST * kStage >= KG * BM * BN * 4 && kPackGroup % BN == 0, "room for the tile, within one of W's");
     __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
 
     int tm, tn;
     tile_coords(g.tiles_m, g.tiles_n, static_cast<int>(blockIdx.x), tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN, li = lane & 31, lh = lane >> 5;
+    const int wm = wave / WN % WM, wn = wave % WN, kg = wave / (WM * WN), li = lane & 31, lh = lane >> 5;
     const int i0 = tm * BM, j0 = tn * BN;
     const size_t pitch = static_cast<size_t>(g.groups) * kPackGroup;
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) char *)lds));
@@ -95,7 +103,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void block8_tile(Block8Product g) 
 #pragma unroll
             for (int b = 0; b < FM; ++b) part[a][b] = floatx16{};
 #pragma unroll
-        for (int k = 0; k < kPackGroup / 32; ++k) {
+        for (int n = 0; n < kSteps; ++n) {
+            const int k = kg * kSteps + n;
             u4v_t cw[FN], cx[FM];
 #pragma unroll
             for (int a = 0; a < FN; ++a) cw[a] = codes16(wa, wn * FN + a, k);
@@ -152,7 +161,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void block8_tile(Block8Product g) 
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int row = (wm * FM + b) * kRowsA + li, quad = (wn * FN + a) * 8 + 2 * c + lh;
-                sums[row * kQuads + (quad ^ (row & kQuads - 1))] =
+                sums[(kg * BM + row) * kQuads + (quad ^ (row & kQuads - 1))] =
                     f4v_t{acc[a][b][4 * c], acc[a][b][4 * c + 1], acc[a][b][4 * c + 2], acc[a][b][4 * c + 3]};
             }
     __syncthreads();
@@ -169,29 +178,44 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void block8_tile(Block8Product g) 
         for (int t = 0; t < kRows; ++t) {
             const int row = (turn * kRows + t) * kStep + row0;
             if (row > last) continue;
-            block8_output(g, g.y + static_cast<size_t>(i0 + row) * g.N + j, sums[row * kQuads + (q ^ (row & kQuads - 1))], bias, now[t],
-                          cols);
+            f4v_t v = sums[row * kQuads + (q ^ (row & kQuads - 1))];
+#pragma unroll
+            for (int k = 1; k < KG; ++k) v += sums[(k * BM + row) * kQuads + (q ^ (row & kQuads - 1))];
+            block8_output(g, g.y + static_cast<size_t>(i0 + row) * g.N + j, v, bias, now[t], cols);
         }
     }
 }
 
-template <int BM, int BN, int WM, int WN, int NST>
+template <int BM, int BN, int WM, int WN, int NST, int KG = 1>
 void launch_tile(Block8Product p, hipStream_t s) {
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
-    launch((block8_tile<BM, BN, WM, WN, NST>), dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN), 0, s, p);
+    launch((block8_tile<BM, BN, WM, WN, NST, KG>), dim3(p.tiles_m * p.tiles_n), dim3(64 * WM * WN * KG), 0, s, p);
 }
+
+size_t tiles_of(size_t M, size_t N, size_t bm, size_t bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); }
 
 }  // namespace
 
-bool block8_tiles_take(size_t M, size_t N, size_t K) { return M >= 64 && N >= 64 && 2.0 * M * N * K >= 0.8e9; }
+// Where half of the CUs get a tile.  us, few rows' kernel and tiles of 64 x 64 (M x K x N):
+// 1999 x 1531 x 777 23.9, 13.8; 1024^3 11.8, 8.7; 4096 x 512 x 512 12.3, 8.5; 64 x 4096 x
+// 16384 35.9, 20.8; 128 x 8192 x 8192 68.8, 35.4; 128 x 784 x 4096 8.1, 8.2; 1024 x 512 x
+// 512 6.0, 5.9; 65 x 4096 x 4096 16.6, 17.7.  Below: 512 x 4096 x 512 11.4, 17.5; 256 x 1024
+// x 1024 6.2, 7.1; 512^3 5.3, 5.8; 64 x 4096 x 4096 12.5, 18.
+bool block8_tiles_take(size_t M, size_t N, size_t K) {
+    return K > 0 && M >= 64 && N >= 64 && tiles_of(M, N, 64, 64) >= static_cast<size_t>(device_cu_count()) / 2;
+}
 
+// The largest tile of which every CU gets two.  us, 128 x 128, 128 x 64 and 64 x 64:
+// 8192 x 4096 x 4096 306, 350, 386; 8192 x 1024 x 4096 104, 105, 110; 16384 x 4096 x 512 72,
+// 76, 88; below two a CU: 4096 x 8192 x 1024 81, 75, 87; 4096 x 4096 x 1024 46.8, 41.8, 47.2;
+// then 512 x 4096 x 4096 42.4, 28.9, 27.4; 2048 x 4096 x 1024 43, 31, 27.7; 8192 x 256 x 256
+// 12.1, 8.7, 8.1.
 void block8_tiles(const Block8Product &p, hipStream_t s) {
-    const size_t cus = device_cu_count();
-    auto tiles = [&](size_t bm, size_t bn) { return (p.M + bm - 1) / bm * ((p.N + bn - 1) / bn); };
-    if (tiles(128, 128) >= 2 * cus) launch_tile<128, 128, 2, 2, 2>(p, s);
-    else if (tiles(128, 64) >= 2 * cus) launch_tile<128, 64, 2, 2, 2>(p, s);
-    else launch_tile<64, 64, 2, 2, 2>(p, s);
+    const size_t fill = 2 * static_cast<size_t>(device_cu_count());
+    if (tiles_of(p.M, p.N, 128, 128) >= fill) launch_tile<128, 128, 2, 2, 2>(p, s);
+    else if (tiles_of(p.M, p.N, 128, 64) >= fill) launch_tile<128, 64, 2, 2, 2>(p, s);
+    else launch_tile<64, 64, 2, 2, 2, 2>(p, s);
 }
 
 }  // namespace tship
