@@ -46,6 +46,106 @@ __device__ __forceinline__ void fill_past(float (&v)[4], size_t c, size_t cols, 
         if (c + e >= cols) v[e] = first;
 }
 
+// The sum over the W waves of a row, in every lane, joined within a wave by DPP.  lds: N * W
+// doubles of this row, others than the last row's (a barrier stands between the two).
+constexpr int kBcast15 = 0x142, kBcast31 = 0x143;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_0(double v) {  // 0 in the other rows of 16
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false));
+}
+template <int W, int N>
+__device__ __forceinline__ void row_sums(double (&s)[N], double *lds) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        double v = s[n];
+        v += dpp<0xB1>(v);   // lanes 1 0 3 2
+        v += dpp<0x4E>(v);   // lanes 2 3 0 1
+        v += dpp<0x141>(v);  // eight lanes mirrored
+        v += dpp<0x140>(v);  // sixteen lanes mirrored
+        v += dpp_or_0<kBcast15, 0xa>(v);
+        v += dpp_or_0<kBcast31, 0xc>(v);  // lane 63: all
+        s[n] = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+    }
+    if (W == 1) return;
+    const int wave = (threadIdx.x >> 6) % W;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) lds[n * W + wave] = s[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[n] = 0.0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s[n] += lds[n * W + w];
+    }
+}
+
+// A lane's quads c = 4 (t + 64 W i) of rows of `cols` columns, by the buffer instructions,
+// for which a lane past the row is one past the buffer: 0 comes back, nothing is written.
+// The quad that a row ends in is read from the row's last four columns and moved into place.
+template <int W, int NV>
+struct RowQuads {
+    unsigned t, cols;
+    __device__ __forceinline__ RowQuads(unsigned t, size_t cols) : t(t), cols(static_cast<unsigned>(cols)) {}
+    __device__ __forceinline__ unsigned col(int i) const { return 4 * (t + 64 * W * i); }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t row(const float *p, bool there) const {  // p, there: uniform
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, there ? static_cast<int>(4 * cols) : 0, 0x00020000);
+    }
+    __device__ __forceinline__ void load(const float *p, bool there, float (&v)[NV][4]) const {
+        const __amdgpu_buffer_rsrc_t r = row(p, there);
+        if (W * NV == 1 && cols < 4) {  // uniform
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[i][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * (col(i) + e), 0, 0));
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const unsigned off = col(i) < cols ? 4 * min(col(i), cols - 4) : kPast;
+            const f4v_t q = __builtin_bit_cast(f4v_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = q[e];
+        }
+    }
+    // what was loaded into place, and `past` in the columns past the row
+    __device__ __forceinline__ void fill(float (&v)[NV][4], float past) const {
+        if (cols == 256 * W * NV) return;  // uniform
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const unsigned c = col(i);
+            const bool ends = c < cols && c + 4 > cols && cols >= 4;
+            if (cols & 1) {  // uniform: by 4 - cols % 4
+#pragma unroll
+                for (int e = 0; e < 3; ++e) v[i][e] = ends ? v[i][e + 1] : v[i][e];
+            }
+            if ((cols & 3) == 1 || (cols & 3) == 2) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) v[i][e] = ends ? v[i][e + 2] : v[i][e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = c + e < cols ? v[i][e] : past;
+        }
+    }
+    // quad i of the row at p
+    __device__ __forceinline__ void store(float *p, int i, const float (&v)[4]) const {
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        const unsigned c = col(i), off = c + 4 <= cols ? 4 * c : kPast;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f4v_t{v[0], v[1], v[2], v[3]}), row(p, true), off, 0, 0);
+        if (cols & 3) {  // uniform
+            if (c < cols && c + 4 > cols) {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (c + e < cols) p[c + e] = v[e];
+            }
+        }
+    }
+    static constexpr unsigned kPast = 0x80000000u;
+};
+
 struct LayerNormArgs {
     const float *x, *residual, *weight, *bias;
     float *h, *y;  // h: with a residual
@@ -149,7 +249,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void layer_norm_rows(LayerNormArgs
 struct LayerNormBackArgs {
     const float *h, *weight, *go;
     float *dh, *dw_part, *db_part;  // parts: [gridDim.x][cols]; db_part may be null beside dw_part
-    RowNorm *norms;                 // LONG with parts: each row's
+    RowNorm *norms;                 // long rows with parts: each row's
     float2 *means;                  // and its mean(g) and mean(g u)
     size_t rows, cols;
     double eps;
@@ -157,18 +257,49 @@ struct LayerNormBackArgs {
     unsigned *ticket;  // zero, and zero again when the launch has run; null: none
 };
 
-// Rows blockIdx.x * RPB + slot, and on by the grid's; a thread keeps the sums of its
-// columns for dw and db (f64), the workgroup's go to the parts.  LONG with DP: no thread
-// has columns of its own; what a row's values need is left for long_layer_columns.
-template <int W, int NV, bool DH, bool DP, bool LONG>
-__global__ __launch_bounds__(kNormThreads<W>) void layer_norm_back(LayerNormBackArgs a) {
+// s += a quad's part of sum d, sum d^2, sum g and sum g d, with g = go w
+__device__ __forceinline__ void back_sums(const float (&h)[4], const float (&go)[4], const float (&w)[4], double shift,
+                                          double (&s)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const double d = h[e] - shift, g = static_cast<double>(go[e]) * w[e];
+        s[0] += d;
+        s[1] += d * d;
+        s[2] += g;
+        s[3] += g * d;
+    }
+}
+
+// What a row's sums say of its gradients
+struct RowBack {
+    RowNorm norm;
+    float mean_g, mean_gu;
+    __device__ __forceinline__ float dh(float go, float w, float u) const {
+        return norm.post * (norm.pre * (norm.rf * (go * w - mean_g - u * mean_gu)));
+    }
+};
+__device__ __forceinline__ RowBack row_back(const double (&s)[4], double cols, double shift, double eps) {
+    const double mean_d = s[0] / cols, r = row_r(mean_d, s[1] / cols, eps);
+    return {row_norm(shift, mean_d, r), static_cast<float>(s[2] / cols), static_cast<float>(r * ((s[3] - mean_d * s[2]) / cols))};
+}
+
+// A lane's quads of a row of h and of go, and its first value
+template <int NV>
+struct BackRow {
+    float h[NV][4], g[NV][4], first;
+};
+
+// Rows blockIdx.x * RPB + slot, and on by the grid's, the next one's values on their way
+// while one is computed; a thread keeps the sums of its columns for dw and db (f64), the
+// workgroup's go to the parts.
+template <int W, int NV, bool DH, bool DP>
+__global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_back(LayerNormBackArgs a) {
     constexpr int RPB = kNormRows<W>;
-    __shared__ double lds[RPB * 4 * W];
-    const int slot = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W);
-    const size_t span = static_cast<size_t>(256) * W * NV;
+    __shared__ double lds[RPB * 2 * 4 * W];
+    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / W, t = threadIdx.x % (64 * W);
     // dw's sums stand in registers; where 16 waves of four quads leave none, in shared
     // memory, each thread its own, and db's alone in registers
-    constexpr bool SHARED = DP && !LONG && W * NV >= 64;
+    constexpr bool SHARED = DP && W * NV >= 64;
     __shared__ double held[SHARED ? NV * 4 * 64 * W : 1];
     double own[SHARED ? 1 : NV][4] = {}, db[NV][4] = {};
     auto dw = [&](int i, int e) -> double & {
@@ -179,146 +310,196 @@ __global__ __launch_bounds__(kNormThreads<W>) void layer_norm_back(LayerNormBack
 #pragma unroll
         for (int i = 0; i < 4 * NV; ++i) dw(i / 4, i % 4) = 0.0;
     }
+    const RowQuads<W, NV> at(t, a.cols);
+    constexpr bool AHEAD = W * NV < 64;  // (there no registers are left for the next row)
     float w[NV][4];
-    auto weights = [&](size_t c0) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) load4(a.weight, c0 + 4 * (t + 64 * W * i), a.cols, w[i]);
-    };
-    if (!LONG) weights(0);
+    at.load(a.weight, true, w);
+    at.fill(w, 0.0f);
     const size_t step = static_cast<size_t>(gridDim.x) * RPB;
+    auto fetch = [&](size_t row, BackRow<NV> &v) {  // a row past the last: zeros
+        const bool live = row < a.rows;
+        const size_t base = live ? row * a.cols : 0;
+        v.first = a.h[base];
+        at.load(a.h + base, live, v.h);
+        at.load(a.go + base, live, v.g);
+    };
+    BackRow<NV> v, next;
+    if (AHEAD) fetch(static_cast<size_t>(blockIdx.x) * RPB + slot, next);
+    int turn = 0;
     // every wave of the workgroup takes every round (the barriers)
     for (size_t r0 = static_cast<size_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += step) {
         const size_t row = r0 + slot;
-        const bool live = row < a.rows;
-        const size_t base = live ? row * a.cols : 0, n = live ? a.cols : 0;
-        float h[NV][4], g[NV][4];
-        const float first = a.h[base];
-        const double shift = first;
-        auto fetch = [&](size_t c0) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) load4(a.h + base, c0 + 4 * (t + 64 * W * i), n, h[i]);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) load4(a.go + base, c0 + 4 * (t + 64 * W * i), n, g[i]);
-        };
-        double s[4] = {0.0, 0.0, 0.0, 0.0};
-        size_t c0 = 0;
-        do {
-            fetch(c0);
-            if (LONG) weights(c0);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                fill_past(h[i], c0 + 4 * (t + 64 * W * i), n, first);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const double d = h[i][e] - shift, gw = static_cast<double>(g[i][e]) * w[i][e];
-                    s[0] += d;
-                    s[1] += d * d;
-                    s[2] += gw;
-                    s[3] += gw * d;
-                }
-            }
-            c0 += span;
-        } while (LONG && c0 < a.cols);
-        row_sum<W, 4>(s, lds + slot * 4 * W);
-        const double cols = static_cast<double>(a.cols), mean_d = s[0] / cols;
-        const double r = row_r(mean_d, s[1] / cols, a.eps);
-        const RowNorm norm = row_norm(shift, mean_d, r);
-        const float mean_g = static_cast<float>(s[2] / cols), mean_gu = static_cast<float>(r * ((s[3] - mean_d * s[2]) / cols));
-        if (DP && LONG) {
-            if (t == 0) {
-                a.norms[row] = norm;
-                a.means[row] = make_float2(mean_g, mean_gu);
-            }
-            continue;
+        if constexpr (AHEAD) {
+            v = next;
+            if (r0 + step < a.rows) fetch(row + step, next);
+        } else {
+            fetch(row, v);
         }
-        c0 = 0;
-        do {
-            if (LONG) {
-                fetch(c0);
-                weights(c0);
+        at.fill(v.h, v.first);
+        at.fill(v.g, 0.0f);
+        const double shift = v.first;
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (!AHEAD) {  // (or the weights' f64 stand in registers through the loop)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(w[i][e]));
             }
+            back_sums(v.h[i], v.g[i], w[i], shift, s);
+        }
+        row_sums<W, 4>(s, lds + (slot * 2 + turn) * 4 * W);
+        turn ^= 1;
+        if (row >= a.rows) continue;  // (uniform in a wave, past the round's barrier)
+        const RowBack back = row_back(s, static_cast<double>(a.cols), shift, a.eps);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const size_t c = c0 + 4 * (t + 64 * W * i);
-                float u[4];
+        for (int i = 0; i < NV; ++i) {
+            float o[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] = norm.unit(h[i][e]);
-                if (DH && c < n) {
-                    float o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        o[e] = norm.post * (norm.pre * (norm.rf * (g[i][e] * w[i][e] - mean_g - u[e] * mean_gu)));
-                    store4(a.dh + base, c, a.cols, o);
-                }
-                if (DP && !LONG && live) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        dw(i, e) += static_cast<double>(g[i][e]) * u[e];
-                        db[i][e] += g[i][e];
-                    }
+            for (int e = 0; e < 4; ++e) {
+                float go = v.g[i][e];
+                asm volatile("" : "+v"(go));  // (or the first pass's f64 of it stands in a register until here)
+                const float u = back.norm.unit(v.h[i][e]);
+                if (DH) o[e] = back.dh(go, w[i][e], u);
+                if (DP) {
+                    dw(i, e) += static_cast<double>(go) * u;
+                    db[i][e] += go;
                 }
             }
-            c0 += span;
-        } while (LONG && c0 < a.cols);
+            if (DH) at.store(a.dh + row * a.cols, i, o);
+            if (SHARED) asm volatile("" ::: "memory");  // (or every quad's sums of dw are read first)
+        }
     }
-    if (DP && !LONG) {
-        if constexpr (RPB > 1) {  // the workgroup's rows together, in their order
-            __shared__ double sum[(RPB - 1) * 64 * W * NV * 4];
-            auto join = [&](double (&v)[NV][4]) {
-                __syncthreads();
-                if (slot > 0) {
+    if constexpr (!DP) return;
+    if constexpr (RPB > 1) {  // the workgroup's rows together, in their order
+        __shared__ double sum[(RPB - 1) * 64 * W * NV * 4];
+        auto join = [&](double (&v)[NV][4]) {
+            __syncthreads();
+            if (slot > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = v[i][e];
+            }
+            __syncthreads();
+            if (slot == 0) {
+#pragma unroll
+                for (int k = 0; k < RPB - 1; ++k)
 #pragma unroll
                     for (int i = 0; i < NV; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = v[i][e];
-                }
-                __syncthreads();
-                if (slot == 0) {
-#pragma unroll
-                    for (int k = 0; k < RPB - 1; ++k)
-#pragma unroll
-                        for (int i = 0; i < NV; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
-                }
-            };
-            join(own);
-            join(db);
-        }
-        if (slot == 0) {
+                        for (int e = 0; e < 4; ++e) v[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
+            }
+        };
+        join(own);
+        join(db);
+    }
+    // The parts.  With a ticket they go past the caches of the chip's dies, and are there
+    // before the ticket counts them (a fence would write back all that the die holds).
+    if (slot == 0) {
+        auto put = [&](float *part, auto &&value) {
+            if (!part) return;  // uniform
+            part += static_cast<size_t>(blockIdx.x) * a.cols;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const size_t c = 4 * (t + 64 * W * i), at = static_cast<size_t>(blockIdx.x) * a.cols;
-                float o[4];
-                if (c >= a.cols) continue;
+                const size_t c = 4 * (t + 64 * W * i);
+                if (a.ticket) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(dw(i, e));
-                if (a.dw_part) store4(a.dw_part + at, c, a.cols, o);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(db[i][e]);
-                if (a.db_part) store4(a.db_part + at, c, a.cols, o);
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < a.cols)
+                            __hip_atomic_store(part + c + e, value(i, e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                } else {
+                    const float o[4] = {value(i, 0), value(i, 1), value(i, 2), value(i, 3)};
+                    if (c < a.cols) store4(part, c, a.cols, o);
+                }
             }
-        }
+        };
+        put(a.dw_part, [&](int i, int e) { return static_cast<float>(dw(i, e)); });
+        put(a.db_part, [&](int i, int e) { return static_cast<float>(db[i][e]); });
     }
-    if (DP && a.ticket) {  // uniform: the last workgroup to get here adds the parts up
+    if (a.ticket) {  // uniform: the last workgroup to get here adds the parts up
         __shared__ bool last;
-        __threadfence();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+        if (threadIdx.x == 0)
+            last = __hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
         __syncthreads();
         if (!last) return;
-        __threadfence();
-        for (size_t c = threadIdx.x; c < 2 * a.cols; c += kNormThreads<W>) {
-            const bool second = c >= a.cols;
-            const size_t at = second ? c - a.cols : c;
-            const float *part = second ? a.db_part : a.dw_part;
-            if (!part) continue;
-            double s = 0.0;
-#pragma unroll 16
-            for (size_t g = 0; g < gridDim.x; ++g) s += part[g * a.cols + at];
-            (second ? a.db : a.dw)[at] = static_cast<float>(s);
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        // a thread a quad (a row's last one: its last four columns), or a column where there are fewer
+        auto add_up = [&](auto value, size_t count, auto &&column) {
+            using Value = decltype(value);
+            for (size_t q = threadIdx.x; q < 2 * count; q += kNormThreads<W>) {
+                const bool second = q >= count;
+                const size_t c = column(second ? q - count : q);
+                const float *part = (second ? a.db_part : a.dw_part);
+                if (!part) continue;
+                constexpr int n = sizeof(Value) / 4, batch = W == 16 ? 8 : 32;
+                double s[n] = {};
+                for (unsigned g0 = 0; g0 < gridDim.x; g0 += batch) {
+                    float v[batch][n];
+#pragma unroll
+                    for (int u = 0; u < batch; ++u)  // (past the last: it again, not added)
+                        __builtin_memcpy(v[u], part + static_cast<size_t>(min(g0 + u, gridDim.x - 1)) * a.cols + c, sizeof(Value));
+#pragma unroll
+                    for (int u = 0; u < batch; ++u)
+#pragma unroll
+                        for (int e = 0; e < n; ++e) s[e] += g0 + u < gridDim.x ? v[u][e] : 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < n; ++e) (second ? a.db : a.dw)[c + e] = static_cast<float>(s[e]);
+            }
+        };
+        if (a.cols < 4) add_up(0.0f, a.cols, [](size_t q) { return q; });
+        else add_up(pk4u_t{}, (a.cols + 3) / 4, [&](size_t q) { return q * 4 + 4 <= a.cols ? q * 4 : a.cols - 4; });
+        if (threadIdx.x == 0) __hip_atomic_store(a.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
+// A row longer than a workgroup holds, passed over twice; with parts (DP) once, what its
+// values need left for long_layer_columns.
+template <bool DP>
+__global__ __launch_bounds__(1024) void long_layer_rows(LayerNormBackArgs a) {
+    constexpr int W = 16, NV = 4;
+    __shared__ double lds[2 * 4 * W];
+    const size_t cols = a.cols, span = static_cast<size_t>(256) * W * NV;
+    int turn = 0;
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {  // uniform
+        const size_t base = row * cols;
+        const float first = a.h[base];
+        auto pass = [&](auto &&f) {
+            for (size_t c0 = 4 * threadIdx.x; c0 < cols; c0 += span) {
+                float h[NV][4], g[NV][4], w[NV][4];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) load4(a.h + base, c0 + 256 * W * i, cols, h[i]);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) load4(a.go + base, c0 + 256 * W * i, cols, g[i]);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) load4(a.weight, c0 + 256 * W * i, cols, w[i]);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) f(c0 + 256 * W * i, h[i], g[i], w[i]);
+            }
+        };
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+        pass([&](size_t c, float (&h)[4], const float (&g)[4], const float (&w)[4]) {
+            fill_past(h, c, cols, first);
+            back_sums(h, g, w, first, s);
+        });
+        row_sums<W, 4>(s, lds + turn * 4 * W);
+        turn ^= 1;
+        const RowBack back = row_back(s, static_cast<double>(cols), first, a.eps);
+        if constexpr (DP) {
+            if (threadIdx.x == 0) {
+                a.norms[row] = back.norm;
+                a.means[row] = make_float2(back.mean_g, back.mean_gu);
+            }
+        } else {
+            pass([&](size_t c, const float (&h)[4], const float (&g)[4], const float (&w)[4]) {
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = back.dh(g[e], w[e], back.norm.unit(h[e]));
+                if (c < cols) store4(a.dh + base, c, cols, o);
+            });
         }
-        if (threadIdx.x == 0) *a.ticket = 0;
     }
 }
 
@@ -334,22 +515,22 @@ __global__ __launch_bounds__(kBlock) void long_layer_columns(LayerNormBackArgs a
     double s[4] = {}, sb[4] = {};
 #pragma unroll 4
     for (size_t row = first; row < last; ++row) {
-        const RowNorm norm = a.norms[row];
         const float2 mean = a.means[row];
+        const RowBack back = {a.norms[row], mean.x, mean.y};
         const size_t base = row * a.cols;
         float h[4], g[4], u[4];
         load4(a.h + base, c, a.cols, h);
         load4(a.go + base, c, a.cols, g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            u[e] = norm.unit(h[e]);
+            u[e] = back.norm.unit(h[e]);
             s[e] += static_cast<double>(g[e]) * u[e];
             sb[e] += g[e];
         }
         if (DH) {
             float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = norm.post * (norm.pre * (norm.rf * (g[e] * w[e] - mean.x - u[e] * mean.y)));
+            for (int e = 0; e < 4; ++e) o[e] = back.dh(g[e], w[e], u[e]);
             store4(a.dh + base, c, a.cols, o);
         }
     }
@@ -384,9 +565,14 @@ template <int W, int NV, bool LONG>
 void launch_layer_back(const LayerNormBackArgs &a, unsigned grid, hipStream_t s) {
     const dim3 block(kNormThreads<W>);
     const bool parts = a.dw_part || a.db_part;
-    if (a.dh && parts) launch((layer_norm_back<W, NV, true, true, LONG>), dim3(grid), block, 0, s, a);
-    else if (a.dh) launch((layer_norm_back<W, NV, true, false, LONG>), dim3(grid), block, 0, s, a);
-    else launch((layer_norm_back<W, NV, false, true, LONG>), dim3(grid), block, 0, s, a);
+    if constexpr (LONG) {
+        if (parts) launch(long_layer_rows<true>, dim3(grid), block, 0, s, a);
+        else launch(long_layer_rows<false>, dim3(grid), block, 0, s, a);
+    } else {
+        if (a.dh && parts) launch((layer_norm_back<W, NV, true, true>), dim3(grid), block, 0, s, a);
+        else if (a.dh) launch((layer_norm_back<W, NV, true, false>), dim3(grid), block, 0, s, a);
+        else launch((layer_norm_back<W, NV, false, true>), dim3(grid), block, 0, s, a);
+    }
 }
 
 int layer_norm_forward(const float *x, const float *residual, const float *weight, const float *bias, size_t rows, size_t cols,
@@ -394,7 +580,7 @@ int layer_norm_forward(const float *x, const float *residual, const float *weigh
     if (rows == 0 || cols == 0) return TS_HIP_OK;
     if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
     const LayerNormArgs a = {x, residual, weight, bias, h, y, codes, scales, rows, cols, packed_pitch(cols), eps};
-    for_cols(codes ? a.pitch : cols, false, [&](auto w, auto nv, auto long_rows) {
+    for_cols<true>(codes ? a.pitch : cols, codes != nullptr, [&](auto w, auto nv, auto long_rows) {
         launch_layer_norm<w.value, nv.value, long_rows.value>(a, codes != nullptr, as_stream(stream));
     });
     return launch_status();
@@ -449,7 +635,7 @@ int ts_hip_layer_norm_backward(const float *h, const float *weight, const float 
     const LayerNormBackArgs a = {h, weight, go, dh, dweight ? sums : nullptr, dbias ? sums + grid * cols : nullptr,
                                  norms, means, rows, cols, eps, dweight, dbias, ticket};
     const hipStream_t s = as_stream(stream);
-    for_cols(cols, false, [&](auto w, auto nv, auto lng) { launch_layer_back<w.value, nv.value, lng.value>(a, grid, s); });
+    for_cols<false>(cols, false, [&](auto w, auto nv, auto lng) { launch_layer_back<w.value, nv.value, lng.value>(a, grid, s); });
     size_t count = grid;
     if (parts && long_rows) {
         const size_t run = long_run(rows, cols);

@@ -79,7 +79,8 @@ constexpr size_t kMaxBlocks = size_t(1) << 21;  // a launch has fewer than 2^32 
 // products want the registers: two quads.  us, packed with the sum, four quads and
 // two: 8192 x 4096 87, 92; 4096 x 8192 120, 107.  Forward and backward: 4096 x 8192
 // 184, 187; 4096 x 6000 144, 157.  (Eight quads: 2048 x 16384 packed 129, four 109.)
-template <class F>
+// MAY_PACK: whether the caller's kernels pack at all.
+template <bool MAY_PACK, class F>
 void for_cols(size_t n, bool packed, F &&f) {
     using std::integral_constant;
     const integral_constant<int, 1> one{};
@@ -93,7 +94,12 @@ void for_cols(size_t n, bool packed, F &&f) {
     else if (n <= 1024) f(one, four, held);
     else if (n <= 2048) f(four, two, held);
     else if (n <= 4096) f(four, four, held);
-    else if (n <= 8192) packed ? f(sixteen, two, held) : f(eight, four, held);
+    else if (n <= 8192) {
+        if constexpr (MAY_PACK) {
+            if (packed) return f(sixteen, two, held);
+        }
+        f(eight, four, held);
+    }
     else if (n <= kMaxHeldCols) f(sixteen, four, held);
     else f(sixteen, four, integral_constant<bool, true>{});
 }

@@ -377,7 +377,7 @@ static int norm_forward(const float *x, const float *residual, const float *weig
     if (rows == 0 || cols == 0) return TS_HIP_OK;
     if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
     const NormArgs a = {x, residual, weight, h, y, codes, scales, rows, cols, packed_pitch(cols), eps};
-    for_cols(codes ? a.pitch : cols, codes != nullptr, [&](auto w, auto nv, auto long_rows) {
+    for_cols<true>(codes ? a.pitch : cols, codes != nullptr, [&](auto w, auto nv, auto long_rows) {
         launch_norm<w.value, nv.value, long_rows.value>(a, codes != nullptr, as_stream(stream));
     });
     return launch_status();
@@ -413,7 +413,7 @@ int ts_hip_rms_norm_backward(const float *h, const float *weight, const float *g
     float *const parts = dweight ? workspace : nullptr, *const scales = parts ? parts + grid * cols : nullptr;
     const NormBackArgs a = {h, weight, go, dh, parts, scales, rows, cols, eps, dweight, ticket};
     const hipStream_t s = as_stream(stream);
-    for_cols(cols, false, [&](auto w, auto nv, auto lng) { launch_back<w.value, nv.value, lng.value>(a, grid, s); });
+    for_cols<false>(cols, false, [&](auto w, auto nv, auto lng) { launch_back<w.value, nv.value, lng.value>(a, grid, s); });
     size_t count = grid;
     if (dweight && long_rows) {
         const size_t run = long_run(rows, cols);
