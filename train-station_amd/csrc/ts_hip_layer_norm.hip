@@ -11,6 +11,11 @@
 // K being one of the n values, (m - K)^2 <= n var, and var = mean(d^2) - mean(d)^2 loses
 // no more than a factor n of f64's 2^-53 however far the row is from zero.
 // m is kept as two fp32, and h - m taken in fp32, exactly where h is near m.
+//
+// What bounds it is memory.  8192 x 4096 with the residual: forward 90 us (537 MB, 6.0 TB/s),
+// packed 82 (437 MB, 5.3), backward 86 (403 MB, 4.7) and 6.5 for the parts' sums; a copy of
+// 2 GB reaches 4.9, one that the last cache holds 8.7.  3000 x 1003 without it: 7.2,
+// 12.4 and 4.0.  128 x 784: 4.6 and 12; 1 x 4096 packed 4.8 (a launch alone is 2 to 3).
 #include "ts_hip_block8.h"
 #include "ts_hip_norm.h"
 
@@ -155,94 +160,147 @@ struct LayerNormArgs {
     double eps;
 };
 
-// A row per W waves; LONG: more columns than the waves hold, passed over twice.
-template <int W, int NV, bool RES, bool PACK, bool LONG>
-__global__ __launch_bounds__(kNormThreads<W>) void layer_norm_rows(LayerNormArgs a) {
+// s += a quad's part of sum d and sum d^2
+__device__ __forceinline__ void norm_sums(const float (&h)[4], double shift, double (&s)[2]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const double d = h[e] - shift;
+        s[0] += d;
+        s[1] += d * d;
+    }
+}
+
+// What a row's sums say of its output; packed in f64: a code takes the side of its border
+// that y itself is on
+struct RowOut {
+    RowNorm norm;
+    double mean, r;
+    __device__ __forceinline__ RowOut(const double (&s)[2], double cols, double shift, double eps) {
+        const double mean_d = s[0] / cols;
+        r = row_r(mean_d, s[1] / cols, eps);
+        mean = shift + mean_d;
+        norm = row_norm(shift, mean_d, r);
+    }
+    __device__ __forceinline__ float y(float h, float w, float b) const { return __builtin_fmaf(norm.unit(h), w, b); }
+    __device__ __forceinline__ double wide_y(float h, float w, float b) const {
+        return __builtin_fma((h - mean) * r, static_cast<double>(w), static_cast<double>(b));
+    }
+};
+
+// A row per W waves, and on by the grid's where there are more rows than workgroups.
+template <int W, int NV, bool RES, bool PACK>
+__global__ __launch_bounds__(kNormThreads<W>, 4) void layer_norm_rows(LayerNormArgs a) {
     constexpr int RPB = kNormRows<W>;
-    __shared__ double lds[RPB * 2 * W];
-    const int slot = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W);
-    const size_t span = static_cast<size_t>(256) * W * NV, end = PACK ? a.pitch : a.cols;
+    __shared__ double lds[RPB * 2 * 2 * W];
+    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / W, t = threadIdx.x % (64 * W);
+    const RowQuads<W, NV> at(t, a.cols);
     float w[NV][4], b[NV][4];
-    auto weights = [&](size_t from) {
+    at.load(a.weight, true, w);
+    at.load(a.bias, a.bias != nullptr, b);
+    at.fill(w, 0.0f);
+    at.fill(b, 0.0f);
+    const size_t step = static_cast<size_t>(gridDim.x) * RPB;
+    int turn = 0;
+    // every wave of the workgroup takes every round (the barriers)
+    for (size_t r0 = static_cast<size_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += step) {
+        const size_t row = r0 + slot;
+        const bool live = row < a.rows;
+        const size_t base = live ? row * a.cols : 0;
+        float v[NV][4], first = a.x[base];
+        at.load(a.x + base, live, v);
+        if constexpr (RES) {
+            float r[NV][4];
+            at.load(a.residual + base, live, r);
+            first += a.residual[base];
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
+        }
+        at.fill(v, first);
+        double s[2] = {0.0, 0.0};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) norm_sums(v[i], first, s);
+        row_sums<W, 2>(s, lds + (slot * 2 + turn) * 2 * W);
+        turn ^= 1;
+        if (!live) continue;  // (uniform in a wave, past the round's barrier)
+        const RowOut out(s, static_cast<double>(a.cols), first, a.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const size_t c = from + 4 * (t + 64 * W * i);
-            load4(a.weight, c, a.cols, w[i]);
-            if (a.bias) {  // uniform
-                load4(a.bias, c, a.cols, b[i]);
-            } else {
+            if (RES) at.store(a.h + base, i, v[i]);
+            if constexpr (PACK) {
+                const size_t c = at.col(i);
+                if (c >= a.pitch) continue;  // (whole blocks)
+                // a quad after the other, and nothing in f64 kept for it: registers
 #pragma unroll
-                for (int e = 0; e < 4; ++e) b[i][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(v[i][e]), "+v"(w[i][e]), "+v"(b[i][e])::"memory");
+                double o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = c + e < a.cols ? out.wide_y(v[i][e], w[i][e], b[i][e]) : 0.0;
+                block8_store(o, c, a.codes + row * a.pitch, a.scales + row, a.rows);
+            } else {
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = out.y(v[i][e], w[i][e], b[i][e]);
+                at.store(a.y + base, i, o);
             }
         }
-    };
-    if (!LONG) weights(0);
-    const size_t step = static_cast<size_t>(gridDim.x) * RPB;
-    for (size_t row = static_cast<size_t>(blockIdx.x) * RPB + slot; row < a.rows; row += step) {  // (W > 1: uniform)
-        const size_t base = row * a.cols;
-        const float *x = a.x + base, *res = RES ? a.residual + base : nullptr;
-        const float first = RES ? x[0] + res[0] : x[0];
-        const double shift = first;
-        float v[NV][4];
-        auto fetch = [&](size_t c0) {  // h of the columns from c0 on
-            float r[NV][4];
+    }
+}
+
+// A row longer than a workgroup holds, passed over twice.
+template <bool RES, bool PACK>
+__global__ __launch_bounds__(1024) void long_layer_norm(LayerNormArgs a) {
+    constexpr int W = 16, NV = 4;
+    __shared__ double lds[2 * 2 * W];
+    const size_t cols = a.cols, span = static_cast<size_t>(256) * W * NV, end = PACK ? a.pitch : cols;
+    int turn = 0;
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {  // uniform
+        const size_t base = row * cols;
+        const float first = RES ? a.x[base] + a.residual[base] : a.x[base];
+        auto pass = [&](size_t end, auto &&f) {
+            for (size_t c0 = 4 * threadIdx.x; c0 < end; c0 += span) {
+                float v[NV][4], r[NV][4];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) load4(x, c0 + 4 * (t + 64 * W * i), a.cols, v[i]);
-            if (RES) {
+                for (int i = 0; i < NV; ++i) load4(a.x + base, c0 + 256 * W * i, cols, v[i]);
+                if (RES) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) load4(res, c0 + 4 * (t + 64 * W * i), a.cols, r[i]);
+                    for (int i = 0; i < NV; ++i) load4(a.residual + base, c0 + 256 * W * i, cols, r[i]);
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+                    for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
+                        for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
+                }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) f(c0 + 256 * W * i, v[i]);
             }
         };
         double s[2] = {0.0, 0.0};
-        size_t c0 = 0;
-        do {
-            fetch(c0);
+        pass(cols, [&](size_t c, float (&v)[4]) {
+            fill_past(v, c, cols, first);
+            norm_sums(v, first, s);
+        });
+        row_sums<W, 2>(s, lds + turn * 2 * W);
+        turn ^= 1;
+        const RowOut out(s, static_cast<double>(cols), first, a.eps);
+        pass(end, [&](size_t c, const float (&v)[4]) {
+            if (c >= end) return;  // (packed: whole blocks)
+            float w[4], b[4] = {};
+            load4(a.weight, c, cols, w);
+            if (a.bias) load4(a.bias, c, cols, b);
+            if (RES && c < cols) store4(a.h + base, c, cols, v);
+            if constexpr (PACK) {
+                double o[4];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                fill_past(v[i], c0 + 4 * (t + 64 * W * i), a.cols, first);
+                for (int e = 0; e < 4; ++e) o[e] = c + e < cols ? out.wide_y(v[e], w[e], b[e]) : 0.0;
+                block8_store(o, c, a.codes + row * a.pitch, a.scales + row, a.rows);
+            } else {
+                float o[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const double d = v[i][e] - shift;
-                    s[0] += d;
-                    s[1] += d * d;
-                }
+                for (int e = 0; e < 4; ++e) o[e] = out.y(v[e], w[e], b[e]);
+                store4(a.y + base, c, cols, o);
             }
-            c0 += span;
-        } while (LONG && c0 < a.cols);
-        row_sum<W, 2>(s, lds + slot * 2 * W);
-        const double cols = static_cast<double>(a.cols), mean_d = s[0] / cols;
-        const double r = row_r(mean_d, s[1] / cols, a.eps), mean = shift + mean_d;
-        const RowNorm n = row_norm(shift, mean_d, r);
-        c0 = 0;
-        do {
-            if (LONG) {
-                fetch(c0);
-                weights(c0);
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const size_t c = c0 + 4 * (t + 64 * W * i);
-                if (c >= end) continue;
-                if (RES) store4(a.h + base, c, a.cols, v[i]);
-                if constexpr (PACK) {  // in f64: a code takes the side of its border that y itself is on
-                    double o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        o[e] = c + e < a.cols ? __builtin_fma((v[i][e] - mean) * r, static_cast<double>(w[i][e]), static_cast<double>(b[i][e])) : 0.0;
-                    block8_store(o, c, a.codes + row * a.pitch, a.scales + row, a.rows);
-                } else {
-                    float o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(n.unit(v[i][e]), w[i][e], b[i][e]);
-                    store4(a.y + base, c, a.cols, o);
-                }
-            }
-            c0 += span;
-        } while (LONG && c0 < end);
+        });
     }
 }
 
@@ -551,14 +609,22 @@ __global__ __launch_bounds__(kBlock) void sum_two_parts(PartSums first, PartSums
     else part_sums_block(second, block - first.blocks, lds);
 }
 
+template <bool LONG, int W, int NV, bool RES, bool PACK>
+void launch_layer_norm(const LayerNormArgs &a, hipStream_t s) {
+    // a row each; of 16 waves as many workgroups as run at once, which keep the weights.  us, a
+    // row each and as many as run at once: 8192 x 4096 89, 96, packed 82, 86; 4096 x 8192 98,
+    // 97; 2048 x 16384 113, 100
+    const size_t need = (a.rows + kNormRows<W> - 1) / kNormRows<W>, cap = W == 16 ? device_cu_count() : kMaxBlocks;
+    const dim3 grid(static_cast<unsigned>(need < cap ? need : cap)), block(kNormThreads<W>);
+    if constexpr (LONG) launch((long_layer_norm<RES, PACK>), grid, block, 0, s, a);
+    else launch((layer_norm_rows<W, NV, RES, PACK>), grid, block, 0, s, a);
+}
 template <int W, int NV, bool LONG>
-void launch_layer_norm(const LayerNormArgs &a, bool pack, hipStream_t s) {
-    const size_t need = (a.rows + kNormRows<W> - 1) / kNormRows<W>;
-    const dim3 grid(static_cast<unsigned>(need < kMaxBlocks ? need : kMaxBlocks)), block(kNormThreads<W>);
-    if (a.residual && pack) launch((layer_norm_rows<W, NV, true, true, LONG>), grid, block, 0, s, a);
-    else if (a.residual) launch((layer_norm_rows<W, NV, true, false, LONG>), grid, block, 0, s, a);
-    else if (pack) launch((layer_norm_rows<W, NV, false, true, LONG>), grid, block, 0, s, a);
-    else launch((layer_norm_rows<W, NV, false, false, LONG>), grid, block, 0, s, a);
+void launch_layer_norm(const LayerNormArgs &a, hipStream_t s) {
+    if (a.residual && a.codes) launch_layer_norm<LONG, W, NV, true, true>(a, s);
+    else if (a.residual) launch_layer_norm<LONG, W, NV, true, false>(a, s);
+    else if (a.codes) launch_layer_norm<LONG, W, NV, false, true>(a, s);
+    else launch_layer_norm<LONG, W, NV, false, false>(a, s);
 }
 
 template <int W, int NV, bool LONG>
@@ -580,8 +646,8 @@ int layer_norm_forward(const float *x, const float *residual, const float *weigh
     if (rows == 0 || cols == 0) return TS_HIP_OK;
     if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
     const LayerNormArgs a = {x, residual, weight, bias, h, y, codes, scales, rows, cols, packed_pitch(cols), eps};
-    for_cols<true>(codes ? a.pitch : cols, codes != nullptr, [&](auto w, auto nv, auto long_rows) {
-        launch_layer_norm<w.value, nv.value, long_rows.value>(a, codes != nullptr, as_stream(stream));
+    for_cols<false>(codes ? a.pitch : cols, false, [&](auto w, auto nv, auto long_rows) {
+        launch_layer_norm<w.value, nv.value, long_rows.value>(a, as_stream(stream));
     });
     return launch_status();
 }

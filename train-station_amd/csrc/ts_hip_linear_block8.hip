@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kBlock) void block8_by_tiles(const float *__restric
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const size_t row = row0 + 8 * i;
-            if (row < rows) *reinterpret_cast<unsigned *>(codes + row * pitch + c) = block8_codes(v[i], s.inv);
+            if (row < rows) *reinterpret_cast<unsigned *>(codes + row * pitch + c) = block8_codes(v[i], s);
         }
     }
 }
