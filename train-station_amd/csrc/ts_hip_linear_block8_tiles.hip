@@ -4,18 +4,21 @@
 // A stage is one block of 128 columns k of the tile's rows of x and W: codes as they lie,
 // by DMA of 16 bytes a lane into LDS, NST stages on their way.  A row's chunk c of 16
 // codes stands at c ^ row / 2 % 8, so that the reads of one chunk of 32 rows fall on all
-// banks.  A wave reads sixteen codes at a time and widens them to bf16 between its
-// matrix instructions; a stage's products of 32 x 32 sums are added from zero and
-// joined to the tile's by one multiply-add a sum with the row's scale times the tile's.
+// banks.  A wave reads a stage's codes while it multiplies the one before, and widens
+// eight at a time to bf16 between its matrix instructions; a stage's products of 32 x 32
+// sums are added from zero and joined to the tile's by one multiply-add a sum with the
+// row's scale times the tile's.
 // W's rows are the instruction's A operand: a lane has one row of x, whose scale is one
 // value, and W's is the same for all of the tile, which lies within 128 of its rows.
 //
-// What bounds it: 8192 x 4096 x 4096 takes 306 us (325 with the residual), 0.90 PFLOP/s;
-// with codes of zero, the same instructions, 229: the chip's power, as the bf16 library
-// product of 8192^3 too has 1.65 PFLOP/s of zeros and 1.23 of values.  Small tiles are bound
-// by a stage's own chain (barrier, DMA, reads, widening, instructions: 0.45 us alone):
-// four stages on their way in place of two gain nothing, two groups of waves that
-// share a stage's k 3 to 8% (1999 x 1531 x 777 14.6 -> 13.8 us).
+// What bounds it: 8192 x 4096 x 4096 (rows x k x columns) takes 260 us, 1.06 PFLOP/s (317
+// with the residual), and with codes of zero, the same instructions, a quarter less: the
+// chip's power, as the bf16 library product of 8192^3 too has 1.65 PFLOP/s of zeros and
+// 1.23 of values.  (306 with a stage read and multiplied in turn.)  Small tiles are bound
+// by a stage's own chain of barrier, DMA, reads and instructions, 0.35 us alone: more
+// stages on their way gain nothing there (64 x 4096 x 64 14.7 us with three, 14.9 with
+// six), two groups of waves that share a stage's k do (17.4 without, and 1999 x 1531 x 777
+// 13.1 in place of 14.2).
 #include "ts_hip_linear_block8.h"
 #include "ts_hip_gemm_split.h"
 
@@ -85,52 +88,69 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void block8_tile(Block8Produc
     for (int a = 0; a < FN; ++a)
 #pragma unroll
         for (int b = 0; b < FM; ++b) acc[a][b] = floatx16{};
-    int slot = 0;
-#pragma unroll
-    for (int s = 0; s < NST - 1; ++s) dma(s, s);
-    for (int s = 0; s < g.groups; ++s) {
-        // this stage has landed, and every wave is done with the one before
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kPer + 1) * (NST - 2)) : "memory");
-        dma(s + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+    // what a wave reads of a stage
+    struct Codes {
+        u4v_t w[kSteps][FN], x[kSteps][FM];
+        float xs[FM], ws;
+    };
+    auto read = [&](int slot, Codes &c) {
         const char *xa = lds + slot * kStage, *wa = xa + kXUnits * 1024;
         const float *scales = reinterpret_cast<const float *>(xa + kScalesAt);
-        float by[FM];
 #pragma unroll
-        for (int b = 0; b < FM; ++b) by[b] = scales[(wm * FM + b) * kRowsA + li] * scales[(kScaleUnits - 1) * 64];
+        for (int n = 0; n < kSteps; ++n) {
+#pragma unroll
+            for (int a = 0; a < FN; ++a) c.w[n][a] = codes16(wa, wn * FN + a, kg * kSteps + n);
+#pragma unroll
+            for (int b = 0; b < FM; ++b) c.x[n][b] = codes16(xa, wm * FM + b, kg * kSteps + n);
+        }
+        c.ws = scales[(kScaleUnits - 1) * 64];
+#pragma unroll
+        for (int b = 0; b < FM; ++b) c.xs[b] = scales[(wm * FM + b) * kRowsA + li];
+    };
+    auto multiply = [&](const Codes &c) {
         floatx16 part[FN][FM];
 #pragma unroll
         for (int a = 0; a < FN; ++a)
 #pragma unroll
             for (int b = 0; b < FM; ++b) part[a][b] = floatx16{};
 #pragma unroll
-        for (int n = 0; n < kSteps; ++n) {
-            const int k = kg * kSteps + n;
-            u4v_t cw[FN], cx[FM];
-#pragma unroll
-            for (int a = 0; a < FN; ++a) cw[a] = codes16(wa, wn * FN + a, k);
-#pragma unroll
-            for (int b = 0; b < FM; ++b) cx[b] = codes16(xa, wm * FM + b, k);
+        for (int n = 0; n < kSteps; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // (the same order of k on both sides)
                 bf8_t fw[FN], fx[FM];
 #pragma unroll
-                for (int a = 0; a < FN; ++a) fw[a] = widen(cw[a][2 * h], cw[a][2 * h + 1], 1.0f);
+                for (int a = 0; a < FN; ++a) fw[a] = widen(c.w[n][a][2 * h], c.w[n][a][2 * h + 1], 1.0f);
 #pragma unroll
-                for (int b = 0; b < FM; ++b) fx[b] = widen(cx[b][2 * h], cx[b][2 * h + 1], 1.0f);
+                for (int b = 0; b < FM; ++b) fx[b] = widen(c.x[n][b][2 * h], c.x[n][b][2 * h + 1], 1.0f);
 #pragma unroll
                 for (int a = 0; a < FN; ++a)
 #pragma unroll
                     for (int b = 0; b < FM; ++b)
                         part[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[a], fx[b], part[a][b], 0, 0, 0);
             }
-        }
 #pragma unroll
         for (int a = 0; a < FN; ++a)
 #pragma unroll
-            for (int b = 0; b < FM; ++b)
+            for (int b = 0; b < FM; ++b) {
+                const float by = c.xs[b] * c.ws;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[a][b][r] = __builtin_fmaf(part[a][b][r], by[b], acc[a][b][r]);
+                for (int r = 0; r < 16; ++r) acc[a][b][r] = __builtin_fmaf(part[a][b][r], by, acc[a][b][r]);
+            }
+    };
+#pragma unroll
+    for (int s = 0; s < NST; ++s) dma(s, s);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((kPer + 1) * (NST - 1)) : "memory");
+    Codes now, next;
+    read(0, now);
+    int slot = 0;
+    for (int s = 0; s < g.groups; ++s) {
+        // the next stage has landed, and every wave has read this one
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kPer + 1) * (NST - 2)) : "memory");
+        dma(s + NST, slot);
         slot = slot + 1 == NST ? 0 : slot + 1;
+        read(slot, next);
+        multiply(now);
+        now = next;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outstanding at exit
 
@@ -197,25 +217,33 @@ size_t tiles_of(size_t M, size_t N, size_t bm, size_t bn) { return (M + bm - 1) 
 
 }  // namespace
 
-// Where half of the CUs get a tile.  us, few rows' kernel and tiles of 64 x 64 (M x K x N):
-// 1999 x 1531 x 777 23.9, 13.8; 1024^3 11.8, 8.7; 4096 x 512 x 512 12.3, 8.5; 64 x 4096 x
-// 16384 35.9, 20.8; 128 x 8192 x 8192 68.8, 35.4; 128 x 784 x 4096 8.1, 8.2; 1024 x 512 x
-// 512 6.0, 5.9; 65 x 4096 x 4096 16.6, 17.7.  Below: 512 x 4096 x 512 11.4, 17.5; 256 x 1024
-// x 1024 6.2, 7.1; 512^3 5.3, 5.8; 64 x 4096 x 4096 12.5, 18.
+// Where half of the CUs get a tile.  us, few rows' kernel and tiles of 64 x 64 (rows x k x
+// columns): 1999 x 1531 x 777 23.7, 13.1; 1024^3 12.2, 8.6; 4096 x 512 x 512 12.6, 8.2; 64 x
+// 4096 x 16384 35, 17; 128 x 8192 x 8192 61, 31; 128 x 784 x 4096 7.9, 7.4; 1024 x 512 x 512
+// 6.2, 5.0; 65 x 4096 x 4096 15.8, 15.5.  Below: 512 x 4096 x 512 11.5, 14.9; 256 x 1024 x
+// 1024 6.2, 6.8; 512^3 5.2, 5.4.
 bool block8_tiles_take(size_t M, size_t N, size_t K) {
     return K > 0 && M >= 64 && N >= 64 && tiles_of(M, N, 64, 64) >= static_cast<size_t>(device_cu_count()) / 2;
 }
 
-// The largest tile of which every CU gets two.  us, 128 x 128, 128 x 64 and 64 x 64:
-// 8192 x 4096 x 4096 306, 350, 386; 8192 x 1024 x 4096 104, 105, 110; 16384 x 4096 x 512 72,
-// 76, 88; below two a CU: 4096 x 8192 x 1024 81, 75, 87; 4096 x 4096 x 1024 46.8, 41.8, 47.2;
-// then 512 x 4096 x 4096 42.4, 28.9, 27.4; 2048 x 4096 x 1024 43, 31, 27.7; 8192 x 256 x 256
-// 12.1, 8.7, 8.1.
+// The largest tile of which every CU gets one, or three in four of the CUs one of 128 x 64.
+// us, 128 x 128, 128 x 64 and 64 x 64: 8192 x 1024 x 4096 90, 111, 118; 4096 x 8192 x 1024 76,
+// 80, 92; below one a CU 2048 x 4096 x 1024 35, 25.7, 27.8; 2048 x 8192 x 1000 63, 46, 50;
+// 1999 x 1531 x 777 17.4, 12.6, 13.1; and fewer: 256 x 4096 x 4096 32, 22.6, 17.9; 1000 x
+// 5000 x 1000 40, 26.7, 21.1.
+// 128 x 128 by four waves of 64 x 64 or eight of 32 x 64: 8192 x 4096 x 4096 260, 279; 8192 x
+// 2048 x 4096 151, 145; 8192 x 1024 x 4096 103, 90; 8192 x 512 x 4096 73, 64.
 void block8_tiles(const Block8Product &p, hipStream_t s) {
-    const size_t fill = 2 * static_cast<size_t>(device_cu_count());
-    if (tiles_of(p.M, p.N, 128, 128) >= fill) launch_tile<128, 128, 2, 2, 2>(p, s);
-    else if (tiles_of(p.M, p.N, 128, 64) >= fill) launch_tile<128, 64, 2, 2, 2>(p, s);
-    else launch_tile<64, 64, 2, 2, 2, 2>(p, s);
+    constexpr int kLong = 16;  // blocks of k: the larger blocks of four waves are worth their fewer waves
+    const size_t cus = device_cu_count();
+    if (tiles_of(p.M, p.N, 128, 128) >= cus) {
+        if (p.groups > kLong) launch_tile<128, 128, 2, 2, 2>(p, s);
+        else launch_tile<128, 128, 4, 2, 2>(p, s);
+    } else if (4 * tiles_of(p.M, p.N, 128, 64) >= 3 * cus) {
+        launch_tile<128, 64, 2, 2, 3, 2>(p, s);
+    } else {
+        launch_tile<64, 64, 2, 2, 3, 2>(p, s);
+    }
 }
 
 }  // namespace tship
