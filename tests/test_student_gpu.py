@@ -631,6 +631,22 @@ def test_distillation_entry_by_itself():
         assert abs(got[1][0] - got[0][0]) <= 2 * R.U * abs(want)  # (the parts in another order of f64 sums)
 
 
+@pytest.mark.parametrize("rows,vocab", [(33, 500), (40, 9000), (9, 60000)])
+def test_distillation_entry_has_its_loss_where_its_gradient_is_held_back(rows, vocab):
+    z, idx, teacher, labels, w = distill_case(rows, vocab, 11)
+    z[7::9, 0] = 0.0
+    dev = [Dev.of(z), Dev.of(idx.view(np.float32)), Dev.of(teacher), Dev.of(labels.view(np.float32)), Dev.of(w),
+           Dev.of(np.zeros(1, np.float32))]
+    floats, bad = hip.ts_hip_distillation_workspace_floats(rows, vocab), ZeroIndex()
+    work, loss, out = Dev(floats), Dev(1), Dev(rows * vocab)
+    out.put(np.full(rows * vocab, 7.0, np.float32))
+    hip_check(hip.ts_hip_distillation(dev[0].ptr, rows, vocab, dev[1].ptr, dev[2].ptr, 11, 2.0, dev[3].ptr, 0.5, dev[4].ptr,
+                                      dev[5].ptr, loss.ptr, out.ptr, bad.ptr, work.ptr, floats, None, None))
+    want, _, bound, _ = R.distillation(z, idx, teacher, 2.0, labels, 0.5, w)
+    assert_within(loss.get(), np.array([want]), bound, "loss")
+    assert not out.get().any()
+
+
 # ---- together ---------------------------------------------------------------------------
 
 

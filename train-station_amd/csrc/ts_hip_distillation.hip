@@ -18,6 +18,11 @@
 // gradient there after the others are stored (an index given twice: the first entry's,
 // with both).  A softmax's terms are added in fp32, by lanes, waves and segments; the
 // loss in f64.
+//
+// What bounds it is memory, a row read and its gradients written: 8192 x 32768 with both
+// terms 450 us (2.1 GB, 4.8 TB/s; a copy of as much 4.9), 999 x 50001 99 (4.0; few rows a
+// workgroup, no lines in common), 8 x 131072 3.5 and 9.7 by two launches, 128 x 1000 7.6
+// (a launch and three waits for memory, one after another).
 #include <algorithm>
 #include <type_traits>
 
@@ -211,8 +216,8 @@ struct Gradient {
 };
 template <Two TWO>
 __device__ __forceinline__ Gradient gradient(const RowShare &share, const RowSums &r, float weight) {
+    const bool none = (r.a == 0.0f || share.soft == 0.0f) && share.hard == 0.0f;  // (not by the weight: go may be 0, and the loss is asked for)
     const float soft = r.a != 0.0f ? weight * share.soft : 0.0f, hard = weight * share.hard;
-    const bool none = soft == 0.0f && hard == 0.0f;
     if (TWO != Two::kNo) return {r.m, soft == 0.0f ? 0.0f : soft / r.s, hard == 0.0f ? 0.0f : hard / r.s1, none};
     return {r.m, (soft + hard) / r.s, 0.0f, none};
 }
@@ -319,10 +324,10 @@ __device__ __forceinline__ void store_loss(const DistillArgs &g, double loss) {
 }
 
 // Where a row's columns stand: column c at place c + s, counted from the line of 128 bytes
-// that its first value is in, so that a wave's quads of places are whole lines (rows of
-// 50001: 999 of them 108 us as they lie, 103 so).  The quads that lie within the row are read and written by the buffer
-// instructions; the columns before the first and after the last, three each at most, are
-// the edge, lanes 0 .. 5's.
+// that its first value is in, so that a wave's quads of places are whole lines (999 rows of
+// 50001: 108 us as they lie, 103 so).  The quads that lie within the row are read and
+// written by the buffer instructions; the columns before the first and after the last,
+// three each at most, are the edge, lanes 0 .. 5's.
 struct Places {
     unsigned s, n;
     __device__ __forceinline__ Places(const float *row, unsigned n, bool lines = true)
@@ -681,8 +686,7 @@ constexpr size_t kWaveVocab = 1024;  // a wave's row, at most
 size_t segments_of(size_t vocab) { return (vocab + 31 + kSegment - 1) / kSegment; }
 
 // Workgroups whose tickets take less than another launch: 8192 x 1001 (1536 of them) 30 us
-// with it, 20 by two launches; 8 x
-// 131072 (264) 13.3 and 14.9.
+// with it, 20 by two launches; 8 x 131072 (264) 13.3 and 14.9.
 constexpr size_t kTicketParts = 512;
 
 constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 28, kMaxRows = size_t(1) << 31;
