@@ -90,6 +90,24 @@ def test_block8_borders_and_what_no_code_holds(tiles):
     assert codes[0, 0] == 0x7e and codes[0, 1] == 0xfe and np.all(np.isfinite(scales))
 
 
+@pytest.mark.parametrize("tiles", [False, True])
+def test_block8_of_values_within_a_rounding_of_a_border(tiles):
+    """Their fp32 rounding is the border itself, at every border and for scales of many bits: the code is the value's own."""
+    v = R.e4m3_values()[:127]
+    border = (v[1:] + v[:-1]) / 2
+    x = np.zeros((40, 3 * 128), np.float32)
+    for row, top in zip(x, np.random.default_rng(3).uniform(1, 2, len(x)).astype(np.float32)):
+        near = (border * (np.float64(top) / 448)).astype(np.float32)
+        near = np.r_[near, np.nextafter(near, np.float32(np.inf)), np.nextafter(near, np.float32(-np.inf))]
+        row.reshape(3, 128)[:, 0] = top
+        row.reshape(3, 128)[:, 1:] = np.resize(near, (3, 127)) * np.resize([1, -1], 127)
+    if tiles:
+        x = np.concatenate([x, np.zeros((127 * len(x), x.shape[1]), np.float32)]).reshape(128, len(x), -1).swapaxes(0, 1).reshape(-1, x.shape[1])
+    codes, scales = parts(tensor(x).block8(tiles))
+    want = R.block8(x, tiles)
+    assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
+
+
 def test_block8_of_nothing_and_of_a_view():
     assert T.Tensor.zeros((0, 5)).block8().shape == (0, 5) and T.Tensor.zeros((5, 0)).block8(True).unpack().shape == (5, 0)
     x = normal((40, 300), 1)
@@ -214,7 +232,8 @@ def test_layer_norm(rows, cols, residual, bias):
     check_layer_norm(rows, cols, residual, bias)
 
 
-@pytest.mark.parametrize("rows,cols", [(600, 8192), (600, 8200), (300, 16383), (1100, 4100), (1500, 1030), (300, 16390), (70, 40001)])
+@pytest.mark.parametrize("rows,cols", [(600, 8192), (600, 8200), (300, 16383), (1100, 4100), (1500, 1030), (300, 16390), (70, 40001),
+                                       (2100, 255), (2101, 510), (2102, 1021), (1025, 2047)])
 def test_layer_norm_sums_many_rows(rows, cols):
     check_layer_norm(rows, cols, True, True)
 
@@ -326,6 +345,48 @@ def test_layer_norm_block8(rows, cols, residual, bias):
     want = R.block8(R.layer_norm(h, w, b, EPS))
     # (a row of one column and no bias is 0 / sqrt(eps): the mean's last bit is of no size)
     assert np.allclose(scales, want[1], rtol=2 * R.U, atol=0) and np.array_equal(codes, want[0])
+
+
+def test_layer_norm_block8_of_many_values():
+    """A code each on y's own side of its border, of three million."""
+    x, r, w, b, h = norm_case(700, 4096, True, True)
+    codes, scales = parts(tensor(x).add_layer_norm_block8(tensor(r), tensor(w), tensor(b))[0])
+    want = R.block8(R.layer_norm(h, w, b, EPS))
+    assert np.allclose(scales, want[1], rtol=2 * R.U, atol=0) and np.array_equal(codes, want[0])
+
+
+@pytest.mark.parametrize("cols", [1, 2, 3, 4, 5, 6, 255, 257, 258, 509, 1021, 1022, 1026, 2047, 4094, 4099, 8189, 8194, 12289, 16381, 16386])
+def test_layer_norm_entries_at_any_address(cols):
+    """Rows that end within a quad, 4 bytes from any boundary, the sum in place of either input; nothing past the last row."""
+    rows = 5
+    x, r, w, b, h = norm_case(rows, cols, True, True)
+    go = normal((rows, cols), 4)
+    y_want, y_bound = R.layer_norm(h, w, b, EPS), R.layer_norm_bound(h, w, b, EPS)
+    W, B, G = Dev.of(w, 1), Dev.of(b, 2), Dev.of(go, 3)
+    past = np.full(3, 7.0, np.float32)
+
+    def room(a, offset):
+        return Dev.of(np.r_[np.asarray(a, np.float32).ravel(), past], offset)
+
+    def of(d):
+        a = d.get()
+        assert np.array_equal(a[-3:], past)
+        return a[:-3]
+
+    for place in ("x", "residual", "apart"):
+        X, Rs, Y = room(x, 1), room(r, 3), room(np.full(rows * cols, 7.0), 2)
+        H = dict(x=X, residual=Rs, apart=room(np.zeros(rows * cols), 2))[place]
+        hip_check(hip.ts_hip_layer_norm(X.ptr, Rs.ptr, W.ptr, B.ptr, rows, cols, EPS, H.ptr, Y.ptr, None))
+        assert np.array_equal(of(H).reshape(rows, cols), h)
+        assert_within(of(Y).reshape(rows, cols), y_want, y_bound, "y")
+        of(X), of(Rs)
+    floats = hip.ts_hip_layer_norm_backward_workspace_floats(rows, cols)
+    work, ticket = Dev(floats), Dev.of(np.zeros(1, np.float32))
+    dh, dw, db = room(np.full(rows * cols, 7.0), 1), room(np.full(cols, 7.0), 2), room(np.full(cols, 7.0), 3)
+    hip_check(hip.ts_hip_layer_norm_backward(H.ptr, W.ptr, G.ptr, rows, cols, EPS, dh.ptr, dw.ptr, db.ptr, work.ptr, floats, ticket.ptr, None))
+    want, bound = R.layer_norm_grads(h, w, go, EPS), R.layer_norm_grads_bound(h, w, go, EPS)
+    for got, shape, a, e, what in zip((dh, dw, db), ((rows, cols), (cols,), (cols,)), want, bound, ("dh", "dweight", "dbias")):
+        assert_within(of(got).reshape(shape), a, e, what)
 
 
 def test_layer_norm_block8_pads_rows_of_nan_with_zeros():
