@@ -21,7 +21,7 @@
 //
 // What bounds it is memory, a row read and its gradients written: 8192 x 32768 with both
 // terms 450 us (2.1 GB, 4.8 TB/s; a copy of as much 4.9), 999 x 50001 99 (4.0; few rows a
-// workgroup, no lines in common), 8 x 131072 3.5 and 9.7 by two launches, 128 x 1000 7.6
+// workgroup, no lines in common), 8 x 131072 3.5 and 7.4 by two launches, 128 x 1000 7.4
 // (a launch and three waits for memory, one after another).
 #include <algorithm>
 #include <type_traits>
@@ -234,9 +234,9 @@ __device__ __forceinline__ double ln(float x) {
     return 0.6931471805599453 * (e + static_cast<double>(__builtin_amdgcn_logf(f)));
 }
 
-// The entries of a row in columns from .. to, by threads first + 0, + step, ...: their
-// terms of the loss (the result; first 0 adds what is the row's own, where `own`), and
-// the gradients there.
+// The entries of a row, by threads first + 0, + step, ...: their terms of the loss (the
+// result, where `own`; first 0 adds the row's), and the gradients of those in columns
+// from .. to.
 template <Two TWO>
 __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, const RowShare &share, const RowSums &r,
                                           const Gradient &by, float weight, const Entry &kept, const int *columns, int first,
@@ -251,12 +251,15 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
     for (int k = first; k <= g.kept; k += step) {
         const bool label = k == g.kept;
         const int j = k == first ? kept.j : label ? share.label : columns[k];
-        if (j < 0 || static_cast<size_t>(j) < from || static_cast<size_t>(j) >= to) continue;
+        const bool here = static_cast<size_t>(j) >= from && static_cast<size_t>(j) < to;
+        if (j < 0 || !(here || own)) continue;
         const float t = label ? 0.0f : k == first ? kept.t : g.teacher[at + k], zj = k == first ? kept.z : z[j];
         float sum = label ? share.hard : takes(t);
-        if (label) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
-        else if (sum != 0.0f) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
-        if (!g.dlogits) continue;
+        if (own) {
+            if (label) loss += sum * (ln(TWO != Two::kNo ? r.s1 : r.s) + (static_cast<double>(r.m) - zj));
+            else if (sum != 0.0f) loss += sum * ((static_cast<double>(t) - r.b) - (static_cast<double>(zj) - r.m));
+        }
+        if (!g.dlogits || !here) continue;
         int same = 0;  // the teacher's entries of this column
 #pragma unroll 2
         for (int other = 0; other < g.kept; other += 4) {
@@ -294,26 +297,26 @@ __device__ __forceinline__ double threads_sum(double v) {
     return all;
 }
 
-// A workgroup's losses to its place; with a ticket the last workgroup to get here adds
-// them all up.  (The parts go past the caches of the chip's dies, and are there before
+// Part `part` of the loss to its place; with a ticket the last workgroup of `parts` to get
+// here adds them all up.  (The parts go past the caches of the chip's dies, and are there before
 // the ticket counts them: a fence would write back all that the die holds.)
 template <int T>
-__device__ __forceinline__ void store_loss(const DistillArgs &g, double loss) {
+__device__ __forceinline__ void store_loss(const DistillArgs &g, double loss, unsigned part, unsigned parts) {
     loss = threads_sum<T>(loss);
     if (!g.ticket) {
-        if (threadIdx.x == 0) g.row_loss[blockIdx.x] = loss;
+        if (threadIdx.x == 0) g.row_loss[part] = loss;
         return;
     }
     __shared__ bool last;
     if (threadIdx.x == 0) {
-        __hip_atomic_store(g.row_loss + blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(g.row_loss + part, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        last = __hip_atomic_fetch_add(g.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        last = __hip_atomic_fetch_add(g.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
     }
     __syncthreads();
     if (!last) return;  // (uniform)
     double s = 0.0;
-    for (unsigned i = threadIdx.x; i < gridDim.x; i += T)
+    for (unsigned i = threadIdx.x; i < parts; i += T)
         s += __hip_atomic_load(g.row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();  // (threads_sum's memory)
     s = threads_sum<T>(s);
@@ -540,7 +543,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         loss += entries<TWO>(g, row, share, r, by, weight, kept, cols, t, 64 * W, 0, g.vocab, true);
     }
-    store_loss<kThreads<W>>(g, loss);
+    store_loss<kThreads<W>>(g, loss, blockIdx.x, gridDim.x);
 }
 
 // ---- rows by segments ------------------------------------------------------------------
@@ -626,7 +629,7 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
         loss = entries<TWO>(g, row, share, r, by, weight, kept, columns, t, T,
                             p0 > at.s ? p0 - at.s : 0, p0 + kSegment - at.s, segment == 0);
     }
-    store_loss<T>(g, loss);
+    if (segment == 0) store_loss<T>(g, loss, static_cast<unsigned>(row), static_cast<unsigned>(g.rows));  // (uniform: the row's, whole)
 }
 
 __global__ __launch_bounds__(kBlock) void sum_losses(const double *parts, size_t n, float *loss) {
@@ -663,13 +666,13 @@ void for_vocab(size_t n, F &&f) {
     else f(integral_constant<int, 8>{}, integral_constant<int, 32>{}, integral_constant<bool, true>{});
 }
 
-// By segments where that is less, in us, as measured by rows and by segments: 16 x 50000
-// 15.2, 12.1; 32 x 50000 15.8, 15.4; 16 x 131072 24, 13.6; 64 x 131072 27, 27; and not
-// 16 x 32000 11.2, 11.1; 64 x 16000 9.4, 12.7; 128 x 50000 19, 23; 96 x 131072 29, 35.
+// By segments where that is less, in us, as measured by rows and by segments: 1 x 32000 10.2,
+// 8.8; 16 x 32000 11.5, 9.2; 64 x 50000 16.7, 14.2; 64 x 131072 26.9, 22.3; and not 16 x
+// 16000 9.1, 9.6; 64 x 16000 9.4, 10.8; 96 x 131072 28.8, 29.7; 200 x 131072 61, 62.
 bool by_segments(size_t rows, size_t vocab) {
     const size_t cus = device_cu_count(), rounds = (rows + cus - 1) / cus;
     const double n = static_cast<double>(vocab);
-    return vocab > 4096 && 11 + 2e-6 * n * static_cast<double>(rows) < 6 + 1.7e-4 * n * static_cast<double>(rounds);
+    return vocab > 4096 && 9.5 + 1.6e-6 * n * static_cast<double>(rows) < 7 + 1.65e-4 * n * static_cast<double>(rounds);
 }
 
 // Workgroups of distill_rows: as many as run at once, each with rows in turn (the next
@@ -686,7 +689,8 @@ constexpr size_t kWaveVocab = 1024;  // a wave's row, at most
 size_t segments_of(size_t vocab) { return (vocab + 31 + kSegment - 1) / kSegment; }
 
 // Workgroups whose tickets take less than another launch: 8192 x 1001 (1536 of them) 30 us
-// with it, 20 by two launches; 8 x 131072 (264) 13.3 and 14.9.
+// with it, 20 by two launches; 8 x 131072, of which each segment had a part (264) 13.3 and
+// 14.9, and by a part a row 11.1.
 constexpr size_t kTicketParts = 512;
 
 constexpr size_t kMaxKept = 1024, kMaxVocab = size_t(1) << 28, kMaxRows = size_t(1) << 31;
@@ -701,7 +705,7 @@ extern "C" {
 
 size_t ts_hip_distillation_workspace_floats(size_t rows, size_t vocab) {
     if (!rows || !vocab) return 0;
-    if (by_segments(rows, vocab)) return 6 * rows * segments_of(vocab);  // sums, losses
+    if (by_segments(rows, vocab)) return 4 * rows * segments_of(vocab) + 2 * rows;  // sums, losses
     return 2 * std::max(row_blocks(rows, vocab), row_blocks(rows, vocab + 31));
 }
 
@@ -743,9 +747,9 @@ int ts_hip_distillation(const float *logits, size_t rows, size_t vocab, const in
         g.segments = static_cast<int>(segments_of(vocab));
         g.parts = reinterpret_cast<float4 *>(workspace);
         g.row_loss = reinterpret_cast<double *>(workspace + 4 * rows * g.segments);
-        parts = rows * g.segments;
+        parts = rows;
         with_ticket();
-        const dim3 grid(static_cast<unsigned>(parts)), block(64 * kSegWaves);
+        const dim3 grid(static_cast<unsigned>(rows * g.segments)), block(64 * kSegWaves);
         with_two(hard, temperature, [&](auto two) {
             launch(distill_segment_sums<two.value>, grid, block, 0, s, g);
             launch(distill_segments<two.value>, grid, block, 0, s, g);
