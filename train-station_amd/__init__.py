@@ -7,8 +7,9 @@ Layers, bottom up:
   contractions), bit-exact elementwise and ReLU-mask kernels, deterministic
   wave/LDS reductions, one fused Adam kernel, device randn, checkpoint
   record encoding, a feed-forward block's operators (root-mean-square norm,
-  layers with their activation and residual, values in 8 bits), a student's (layer
-  norm, 8-bit blocks of 128, distillation from a teacher's top logits), plus malloc / async copy / stream / event wrappers.
+  layers with their activation and residual, values in 8 bits), a student's
+  (layer norm, 8-bit blocks of 128, distillation from a teacher's top logits),
+  plus malloc / async copy / stream / event wrappers.
 * ``libts_gradtrack.so`` -- the reference's Tensor / gradtrack engine / Adam
   restated in C++ over that C-ABI (``include/ts_gradtrack.h``).
 * this package -- a ctypes face of the same API for Python callers.
