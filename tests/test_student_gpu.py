@@ -138,7 +138,8 @@ def test_block8_linear(m, k, n, act, bias, residual):
 
 @pytest.mark.parametrize("m,k,n", [(64, 200, 8200), (8255, 100, 65), (1003, 1, 900), (2000, 150, 2101), (2011, 1153, 2080),
                                    (2975, 130, 2801), (3001, 700, 2820),
-                                   (2050, 2200, 2050), (1100, 2300, 1100), (70, 2190, 8200)])
+                                   (2050, 2200, 2050), (1100, 2300, 1100), (70, 2190, 8200),
+                                   (33, 300, 8300), (64, 140, 33000), (8200, 300, 33), (33000, 140, 64)])
 def test_block8_linear_by_tiles(m, k, n):
     """Each size of tile, with edges within it, one and several blocks of columns."""
     x, xv = blocks(normal((m, k), 1))

@@ -217,29 +217,33 @@ size_t tiles_of(size_t M, size_t N, size_t bm, size_t bn) { return (M + bm - 1) 
 
 }  // namespace
 
-// Where half of the CUs get a tile.  us, few rows' kernel and tiles of 64 x 64 (rows x k x
-// columns): 1999 x 1531 x 777 23.7, 13.1; 1024^3 12.2, 8.6; 4096 x 512 x 512 12.6, 8.2; 64 x
-// 4096 x 16384 35, 17; 128 x 8192 x 8192 61, 31; 128 x 784 x 4096 7.9, 7.4; 1024 x 512 x 512
-// 6.2, 5.0; 65 x 4096 x 4096 15.8, 15.5.  Below: 512 x 4096 x 512 11.5, 14.9; 256 x 1024 x
-// 1024 6.2, 6.8; 512^3 5.2, 5.4.
+// Where half of the CUs get a tile, of more than the 32 rows and columns of the few rows'
+// kernel's.  us, that one and tiles of 64 x 64 (rows x k x columns): 1999 x 1531 x 777 23.7,
+// 13.1; 1024^3 12.2, 8.6; 4096 x 512 x 512 12.6, 8.2; 64 x 4096 x 16384 35, 17; 48 x 4096 x 8192
+// 18.7, 16.3; 128 x 8192 x 8192 61, 31; 128 x 784 x 4096 7.9, 7.4; 1024 x 512 x 512 6.2, 5.0;
+// 65 x 4096 x 4096 15.8, 15.5; 8192 x 512 x 33 6.4, 4.8.  Below: 512 x 4096 x 512 11.5, 14.9; 256 x
+// 1024 x 1024 6.2, 6.8; 512^3 5.2, 5.4; 64 x 4096 x 4096 12.1, 16; 32 x 4096 x 8192 12.7, 15.7;
+// 65536 x 512 x 32 12.1, 14.1.
 bool block8_tiles_take(size_t M, size_t N, size_t K) {
-    return K > 0 && M >= 64 && N >= 64 && tiles_of(M, N, 64, 64) >= static_cast<size_t>(device_cu_count()) / 2;
+    return K > 0 && M > 32 && N > 32 && tiles_of(M, N, 64, 64) >= static_cast<size_t>(device_cu_count()) / 2;
 }
 
-// The largest tile of which every CU gets one, or three in four of the CUs one of 128 x 64.
+// The largest tile that rows and columns fill and of which every CU gets one, or three in
+// four of the CUs one of 128 x 64.
 // us, 128 x 128, 128 x 64 and 64 x 64: 8192 x 1024 x 4096 90, 111, 118; 4096 x 8192 x 1024 76,
 // 80, 92; below one a CU 2048 x 4096 x 1024 35, 25.7, 27.8; 2048 x 8192 x 1000 63, 46, 50;
 // 1999 x 1531 x 777 17.4, 12.6, 13.1; and fewer: 256 x 4096 x 4096 32, 22.6, 17.9; 1000 x
-// 5000 x 1000 40, 26.7, 21.1.
+// 5000 x 1000 40, 26.7, 21.1.  No more than 64 rows, or columns: 64 x 4096 x 65536 78, 90, 65; 64 x
+// 1024 x 65536 23, 28, 19; 65536 x 1024 x 64 25, 20, 19.
 // 128 x 128 by four waves of 64 x 64 or eight of 32 x 64: 8192 x 4096 x 4096 260, 279; 8192 x
 // 2048 x 4096 151, 145; 8192 x 1024 x 4096 103, 90; 8192 x 512 x 4096 73, 64.
 void block8_tiles(const Block8Product &p, hipStream_t s) {
     constexpr int kLong = 16;  // blocks of k: the larger blocks of four waves are worth their fewer waves
     const size_t cus = device_cu_count();
-    if (tiles_of(p.M, p.N, 128, 128) >= cus) {
+    if (p.M > 64 && p.N > 64 && tiles_of(p.M, p.N, 128, 128) >= cus) {
         if (p.groups > kLong) launch_tile<128, 128, 2, 2, 2>(p, s);
         else launch_tile<128, 128, 4, 2, 2>(p, s);
-    } else if (4 * tiles_of(p.M, p.N, 128, 64) >= 3 * cus) {
+    } else if (p.M > 64 && 4 * tiles_of(p.M, p.N, 128, 64) >= 3 * cus) {
         launch_tile<128, 64, 2, 2, 3, 2>(p, s);
     } else {
         launch_tile<64, 64, 2, 2, 3, 2>(p, s);
