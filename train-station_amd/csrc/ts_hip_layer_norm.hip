@@ -40,7 +40,10 @@ __device__ __forceinline__ RowNorm row_norm(double shift, double mean_d, double 
 }
 __device__ __forceinline__ double row_r(double mean_d, double mean_dd, double eps) {
     const double var = mean_dd - mean_d * mean_d;
-    return 1.0 / sqrt((var < 0.0 ? 0.0 : var) + eps);  // (a NaN stays)
+    const double v = (var < 0.0 ? 0.0 : var) + eps;  // (a NaN stays)
+    // 1 / sqrt(v): the instruction's 24 bits and one step of third order; 0, infinity and NaN: the instruction's
+    const double r = __builtin_amdgcn_rsq(v), e = __builtin_fma(-v * r, r, 1.0);
+    return v > 0.0 && v < __builtin_inf() ? __builtin_fma(r * e, __builtin_fma(0.375, e, 0.5), r) : r;
 }
 
 // columns past the row: its first value, so that d is 0
@@ -93,8 +96,13 @@ __device__ __forceinline__ void row_sums(double (&s)[N], double *lds) {
 template <int W, int NV>
 struct RowQuads {
     unsigned t, cols;
-    __device__ __forceinline__ RowQuads(unsigned t, size_t cols) : t(t), cols(static_cast<unsigned>(cols)) {}
+    int wave, parts;  // the wave's place in the row, the row's parts of 256 columns
+    __device__ __forceinline__ RowQuads(unsigned t, size_t cols)
+        : t(t), cols(static_cast<unsigned>(cols)), wave(__builtin_amdgcn_readfirstlane(t / 64)), parts(static_cast<int>((cols + 255) / 256)) {}
     __device__ __forceinline__ unsigned col(int i) const { return 4 * (t + 64 * W * i); }
+    // whether any lane of the wave has columns of quad i (uniform): what is past the row is not
+    // computed (backward, us: 3400 x 4100 46, 51 with it computed; 1700 x 8200 53, 67)
+    __device__ __forceinline__ bool some(int i) const { return i == 0 || W * i + wave < parts; }
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t row(const float *p, bool there) const {  // p, there: uniform
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, there ? static_cast<int>(4 * cols) : 0, 0x00020000);
     }
@@ -157,7 +165,7 @@ struct LayerNormArgs {
     uint8_t *codes;
     float *scales;  // packed
     size_t rows, cols, pitch;
-    double eps;
+    double eps, per_col;  // 1 / cols
 };
 
 // s += a quad's part of sum d and sum d^2
@@ -175,9 +183,9 @@ __device__ __forceinline__ void norm_sums(const float (&h)[4], double shift, dou
 struct RowOut {
     RowNorm norm;
     double mean, r;
-    __device__ __forceinline__ RowOut(const double (&s)[2], double cols, double shift, double eps) {
-        const double mean_d = s[0] / cols;
-        r = row_r(mean_d, s[1] / cols, eps);
+    __device__ __forceinline__ RowOut(const double (&s)[2], double per_col, double shift, double eps) {
+        const double mean_d = s[0] * per_col;
+        r = row_r(mean_d, s[1] * per_col, eps);
         mean = shift + mean_d;
         norm = row_norm(shift, mean_d, r);
     }
@@ -224,7 +232,7 @@ __global__ __launch_bounds__(kNormThreads<W>, 4) void layer_norm_rows(LayerNormA
         row_sums<W, 2>(s, lds + (slot * 2 + turn) * 2 * W);
         turn ^= 1;
         if (!live) continue;  // (uniform in a wave, past the round's barrier)
-        const RowOut out(s, static_cast<double>(a.cols), first, a.eps);
+        const RowOut out(s, a.per_col, first, a.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (RES) at.store(a.h + base, i, v[i]);
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(1024) void long_layer_norm(LayerNormArgs a) {
         });
         row_sums<W, 2>(s, lds + turn * 2 * W);
         turn ^= 1;
-        const RowOut out(s, static_cast<double>(cols), first, a.eps);
+        const RowOut out(s, a.per_col, first, a.eps);
         pass(end, [&](size_t c, const float (&v)[4]) {
             if (c >= end) return;  // (packed: whole blocks)
             float w[4], b[4] = {};
@@ -310,7 +318,7 @@ struct LayerNormBackArgs {
     RowNorm *norms;                 // long rows with parts: each row's
     float2 *means;                  // and its mean(g) and mean(g u)
     size_t rows, cols;
-    double eps;
+    double eps, per_col;  // 1 / cols
     float *dw, *db;    // with a ticket: the last workgroup adds the parts up
     unsigned *ticket;  // zero, and zero again when the launch has run; null: none
 };
@@ -336,9 +344,10 @@ struct RowBack {
         return norm.post * (norm.pre * (norm.rf * (go * w - mean_g - u * mean_gu)));
     }
 };
-__device__ __forceinline__ RowBack row_back(const double (&s)[4], double cols, double shift, double eps) {
-    const double mean_d = s[0] / cols, r = row_r(mean_d, s[1] / cols, eps);
-    return {row_norm(shift, mean_d, r), static_cast<float>(s[2] / cols), static_cast<float>(r * ((s[3] - mean_d * s[2]) / cols))};
+__device__ __forceinline__ RowBack row_back(const double (&s)[4], double per_col, double shift, double eps) {
+    const double mean_d = s[0] * per_col, r = row_r(mean_d, s[1] * per_col, eps);
+    return {row_norm(shift, mean_d, r), static_cast<float>(s[2] * per_col),
+            static_cast<float>(r * ((s[3] - mean_d * s[2]) * per_col))};
 }
 
 // A lane's quads of a row of h and of go, and its first value
@@ -399,6 +408,7 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
         double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!at.some(i)) continue;
             if (!AHEAD) {  // (or the weights' f64 stand in registers through the loop)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(w[i][e]));
@@ -408,9 +418,10 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
         row_sums<W, 4>(s, lds + (slot * 2 + turn) * 4 * W);
         turn ^= 1;
         if (row >= a.rows) continue;  // (uniform in a wave, past the round's barrier)
-        const RowBack back = row_back(s, static_cast<double>(a.cols), shift, a.eps);
+        const RowBack back = row_back(s, a.per_col, shift, a.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!at.some(i)) continue;
             float o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -544,7 +555,7 @@ __global__ __launch_bounds__(1024) void long_layer_rows(LayerNormBackArgs a) {
         });
         row_sums<W, 4>(s, lds + turn * 4 * W);
         turn ^= 1;
-        const RowBack back = row_back(s, static_cast<double>(cols), first, a.eps);
+        const RowBack back = row_back(s, a.per_col, first, a.eps);
         if constexpr (DP) {
             if (threadIdx.x == 0) {
                 a.norms[row] = back.norm;
@@ -641,11 +652,26 @@ void launch_layer_back(const LayerNormBackArgs &a, unsigned grid, hipStream_t s)
     }
 }
 
+// The backward pass's for_cols: for rows of 1025 to 2048 two waves of four quads in place of
+// four of two, since what a wave does for its row beside its quads is as much as a quad
+// and a half.  us: 13000 x 1100 41, 58; 7000 x 2048 32, 33.
+template <class F>
+void for_back_cols(size_t n, F &&f) {
+    using std::integral_constant;
+    if (n > 1024 && n <= 2048) f(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
+    else for_cols<false>(n, false, [&](auto w, auto nv, auto lng) {
+        if constexpr (!(w.value == 4 && nv.value == 2)) f(w, nv, lng);
+    });
+}
+size_t layer_back_blocks(size_t rows, size_t cols) {
+    return cols > 1024 && cols <= 2048 ? back_blocks((rows + 1) / 2, cols) : back_blocks(rows, cols);  // (two rows a workgroup)
+}
+
 int layer_norm_forward(const float *x, const float *residual, const float *weight, const float *bias, size_t rows, size_t cols,
                        float eps, float *h, float *y, uint8_t *codes, float *scales, void *stream) {
     if (rows == 0 || cols == 0) return TS_HIP_OK;
     if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
-    const LayerNormArgs a = {x, residual, weight, bias, h, y, codes, scales, rows, cols, packed_pitch(cols), eps};
+    const LayerNormArgs a = {x, residual, weight, bias, h, y, codes, scales, rows, cols, packed_pitch(cols), eps, 1.0 / static_cast<double>(cols)};
     for_cols<false>(codes ? a.pitch : cols, false, [&](auto w, auto nv, auto long_rows) {
         launch_layer_norm<w.value, nv.value, long_rows.value>(a, as_stream(stream));
     });
@@ -675,7 +701,7 @@ int ts_hip_layer_norm_block8(const float *x, const float *residual, const float 
 }
 
 size_t ts_hip_layer_norm_backward_workspace_floats(size_t rows, size_t cols) {
-    return 2 * back_blocks(rows, cols) * cols + (cols > kMaxHeldCols ? kRowFloats * rows : 0);
+    return 2 * layer_back_blocks(rows, cols) * cols + (cols > kMaxHeldCols ? kRowFloats * rows : 0);
 }
 
 int ts_hip_layer_norm_backward(const float *h, const float *weight, const float *go, size_t rows, size_t cols, float eps,
@@ -691,7 +717,7 @@ int ts_hip_layer_norm_backward(const float *h, const float *weight, const float 
     if (!h || !weight || !go || rows >= kMaxRows) return TS_HIP_EINVAL;
     if (parts && (!workspace || workspace_floats < ts_hip_layer_norm_backward_workspace_floats(rows, cols)))
         return TS_HIP_EWORKSPACE;
-    const unsigned grid = static_cast<unsigned>(back_blocks(rows, cols));
+    const unsigned grid = static_cast<unsigned>(layer_back_blocks(rows, cols));
     const bool long_rows = cols > kMaxHeldCols;
     if (!parts || long_rows || grid > kTicketParts || grid * cols > kTicketFloats) ticket = nullptr;
     // workspace: a long row's means and norms, then the parts
@@ -699,9 +725,9 @@ int ts_hip_layer_norm_backward(const float *h, const float *weight, const float 
     RowNorm *const norms = reinterpret_cast<RowNorm *>(workspace + 2 * rows);
     float *const sums = parts ? workspace + (long_rows ? kRowFloats * rows : 0) : nullptr;
     const LayerNormBackArgs a = {h, weight, go, dh, dweight ? sums : nullptr, dbias ? sums + grid * cols : nullptr,
-                                 norms, means, rows, cols, eps, dweight, dbias, ticket};
+                                 norms, means, rows, cols, eps, 1.0 / static_cast<double>(cols), dweight, dbias, ticket};
     const hipStream_t s = as_stream(stream);
-    for_cols<false>(cols, false, [&](auto w, auto nv, auto lng) { launch_layer_back<w.value, nv.value, lng.value>(a, grid, s); });
+    for_back_cols(cols, [&](auto w, auto nv, auto lng) { launch_layer_back<w.value, nv.value, lng.value>(a, grid, s); });
     size_t count = grid;
     if (parts && long_rows) {
         const size_t run = long_run(rows, cols);
