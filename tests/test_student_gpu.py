@@ -493,7 +493,7 @@ def check_distillation(rows, vocab, kept, t, hard, weighted, seed=0, case=None):
 
 # by rows (a wave, waves, long rows) and by segments (few rows of many columns)
 DISTILL = [(1, 1, 1), (3, 7, 2), (19, 10, 3), (9, 255, 10), (10, 257, 5), (37, 1000, 64), (9, 1025, 300), (11, 4095, 20), (9, 4096, 8),
-           (130, 1003, 17), (5000, 33, 4), (9, 1500, 7), (9, 2049, 64), (27, 5001, 10), (3, 50001, 20), (2, 66000, 9), (30, 131071, 12), (10, 50001, 100), (2, 131072, 1024), (1, 300001, 5),
+           (130, 1003, 17), (5000, 33, 4), (6000, 1029, 9), (70, 2047, 200), (41, 2048, 40), (9, 1500, 7), (9, 2049, 64), (27, 5001, 10), (3, 50001, 20), (2, 66000, 9), (30, 131071, 12), (10, 50001, 100), (2, 131072, 1024), (1, 300001, 5),
            (140, 4101, 30), (150, 8193, 9), (135, 16385, 33), (129, 32768, 70), (131, 40003, 11), (129, 65537, 20), (129, 131100, 40)]
 
 

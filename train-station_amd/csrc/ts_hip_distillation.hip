@@ -649,7 +649,10 @@ void with_two(float hard, float temperature, F &&f) {
     else f(integral_constant<Two, Two::kYes>{});
 }
 
-// Calls f(W, NV, LONG as constants) for rows of n places: the waves that hold them.
+// Calls f(W, NV, LONG as constants) for rows of n places: the waves that hold them, one to
+// 2048 (what a wave does for its row beside its quads is as much as they are).  us at T 1 and
+// T 1.5 with labels, 8192 rows by one wave and by four: 1100 columns 20.5, 25 and 34, 46;
+// 2000 31, 33 and 38, 48; 3000 50, 52 and 50, 61; 4096 67, 69 and 58, 64.
 template <class F>
 void for_vocab(size_t n, F &&f) {
     using std::integral_constant;
@@ -657,7 +660,7 @@ void for_vocab(size_t n, F &&f) {
     if (n <= 256) f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, held);
     else if (n <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 2>{}, held);
     else if (n <= 1024) f(integral_constant<int, 1>{}, integral_constant<int, 4>{}, held);
-    else if (n <= 2048) f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, held);
+    else if (n <= 2048) f(integral_constant<int, 1>{}, integral_constant<int, 8>{}, held);
     else if (n <= 4096) f(integral_constant<int, 4>{}, integral_constant<int, 4>{}, held);
     else if (n <= 8192) f(integral_constant<int, 4>{}, integral_constant<int, 8>{}, held);
     else if (n <= 16384) f(integral_constant<int, 8>{}, integral_constant<int, 8>{}, held);
@@ -675,16 +678,16 @@ bool by_segments(size_t rows, size_t vocab) {
     return vocab > 4096 && 9.5 + 1.6e-6 * n * static_cast<double>(rows) < 7 + 1.65e-4 * n * static_cast<double>(rounds);
 }
 
+constexpr size_t kWaveVocab = 2048;  // a wave's row, at most
+
 // Workgroups of distill_rows: as many as run at once, each with rows in turn (the next
 // one's values come in while the last one's gradients go out).
 size_t row_blocks(size_t rows, size_t places) {
-    const size_t per = places <= 1024 ? 4 : 1, need = (rows + per - 1) / per;
+    const size_t per = places <= kWaveVocab ? 4 : 1, need = (rows + per - 1) / per;
     const size_t a_cu = places <= 1024 ? 6 : places <= 4096 ? 5 : places <= 8192 ? 4 : places <= 32768 ? 2 : 1;
     const size_t cap = static_cast<size_t>(device_cu_count()) * a_cu;
     return need < cap ? need : cap;
 }
-
-constexpr size_t kWaveVocab = 1024;  // a wave's row, at most
 
 size_t segments_of(size_t vocab) { return (vocab + 31 + kSegment - 1) / kSegment; }
 
