@@ -237,12 +237,30 @@ __device__ __forceinline__ double ln(float x) {
 // The entries of a row, by threads first + 0, + step, ...: their terms of the loss (the
 // result, where `own`; first 0 adds the row's), and the gradients of those in columns
 // from .. to.
-template <Two TWO>
+//
+// TABLE: one wave, and a place in LDS for each of the row's columns, for whether an index
+// is given twice: every entry leaves its number at its column, one that finds another's
+// leaves kTwice.  (By a search of all entries for each, as other rows do it, 8192 x 1000 with
+// 256 of them takes 60 us, so 38; with 32 17.6, 16.4.)
+constexpr unsigned short kTwice = 0xffff;
+template <Two TWO, bool TABLE>
 __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, const RowShare &share, const RowSums &r,
                                           const Gradient &by, float weight, const Entry &kept, const int *columns, int first,
-                                          int step, size_t from, size_t to, bool own) {
+                                          int step, size_t from, size_t to, bool own, unsigned short *at_column) {
     const size_t at = row * g.kept;
     const float *z = g.logits + row * g.vocab;
+    if (TABLE && g.dlogits) {
+        for (int k = first; k < g.kept; k += step) {
+            const int j = k == first ? kept.j : columns[k];
+            if (j >= 0) at_column[j] = static_cast<unsigned short>(k);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int k = first; k < g.kept; k += step) {
+            const int j = k == first ? kept.j : columns[k];
+            if (j >= 0 && at_column[j] != k) at_column[j] = kTwice;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
     const bool asked = share.soft != 0.0f && r.a != 0.0f;
     const float per_e = asked ? share.soft / r.a : 0.0f;
     double loss = 0.0;
@@ -261,10 +279,15 @@ __device__ __forceinline__ double entries(const DistillArgs &g, size_t row, cons
         }
         if (!g.dlogits || !here) continue;
         int same = 0;  // the teacher's entries of this column
+        const int there = TABLE ? at_column[j] : kTwice;
+        if (there != kTwice) {  // (the label's column may hold another row's entry)
+            same = label ? there < g.kept && columns[there] == j : 1;
+        } else {
 #pragma unroll 2
-        for (int other = 0; other < g.kept; other += 4) {
-            const int4 four = *reinterpret_cast<const int4 *>(columns + other);
-            same += (four.x == j) + (four.y == j) + (four.z == j) + (four.w == j);
+            for (int other = 0; other < g.kept; other += 4) {
+                const int4 four = *reinterpret_cast<const int4 *>(columns + other);
+                same += (four.x == j) + (four.y == j) + (four.z == j) + (four.w == j);
+            }
         }
         bool mine = label ? same == 0 : true;  // the first of them stores, with the later ones' shares and the label's
         if (!label) {
@@ -448,6 +471,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
     __shared__ RowSums lds[W > 1 ? W : 1];
     // the rows' columns; in turn where waves share a row: some still read the last one's
     __shared__ __attribute__((aligned(16))) int columns[W > 1 ? 2 : RPB][kEntries];
+    __shared__ unsigned short at_column[W > 1 ? 1 : RPB][W > 1 ? 1 : 256 * NV];
     const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W, t = threadIdx.x % (64 * W);
     constexpr unsigned span = 256 * W * NV;
     const unsigned n = static_cast<unsigned>(g.vocab);
@@ -541,7 +565,7 @@ __global__ __launch_bounds__(kThreads<W>, NV > 16 ? 2 : 4) void distill_rows(Dis
         if (by.none) continue;  // (uniform over the row's waves)
         if (W > 1 && dz) __syncthreads();  // the entries' gradients are stored after the others
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        loss += entries<TWO>(g, row, share, r, by, weight, kept, cols, t, 64 * W, 0, g.vocab, true);
+        loss += entries<TWO, W == 1>(g, row, share, r, by, weight, kept, cols, t, 64 * W, 0, g.vocab, true, at_column[W == 1 ? slot : 0]);
     }
     store_loss<kThreads<W>>(g, loss, blockIdx.x, gridDim.x);
 }
@@ -626,8 +650,8 @@ __global__ __launch_bounds__(64 * kSegWaves) void distill_segments(DistillArgs g
     double loss = 0.0;
     if (!by.none) {  // (uniform)
         __syncthreads();  // the entries' gradients are stored after the others
-        loss = entries<TWO>(g, row, share, r, by, weight, kept, columns, t, T,
-                            p0 > at.s ? p0 - at.s : 0, p0 + kSegment - at.s, segment == 0);
+        loss = entries<TWO, false>(g, row, share, r, by, weight, kept, columns, t, T,
+                            p0 > at.s ? p0 - at.s : 0, p0 + kSegment - at.s, segment == 0, nullptr);
     }
     if (segment == 0) store_loss<T>(g, loss, static_cast<unsigned>(row), static_cast<unsigned>(g.rows));  // (uniform: the row's, whole)
 }
@@ -684,7 +708,7 @@ constexpr size_t kWaveVocab = 2048;  // a wave's row, at most
 // one's values come in while the last one's gradients go out).
 size_t row_blocks(size_t rows, size_t places) {
     const size_t per = places <= kWaveVocab ? 4 : 1, need = (rows + per - 1) / per;
-    const size_t a_cu = places <= 1024 ? 6 : places <= 4096 ? 5 : places <= 8192 ? 4 : places <= 32768 ? 2 : 1;
+    const size_t a_cu = places <= 1024 ? 6 : places <= kWaveVocab ? 4 : places <= 4096 ? 5 : places <= 8192 ? 4 : places <= 32768 ? 2 : 1;
     const size_t cap = static_cast<size_t>(device_cu_count()) * a_cu;
     return need < cap ? need : cap;
 }
