@@ -120,7 +120,7 @@ def test_block8_of_nothing_and_of_a_view():
 
 LAYERS = [(1, 1, 1), (1, 128, 128), (3, 5, 7), (16, 130, 128), (17, 65, 31), (33, 784, 10), (128, 129, 130), (2, 1000, 3),
           (257, 40, 300), (1, 513, 129), (300, 17, 33), (128, 128, 128), (129, 1000, 257), (200, 2000, 260), (1, 4096, 1000),
-          (500, 300, 700), (1000, 1003, 1029)]
+          (500, 300, 700), (1000, 1003, 1029), (20, 2000, 2100), (20, 1200, 8200), (500, 1100, 700), (29, 130, 17000)]
 
 
 @pytest.mark.parametrize("m,k,n", LAYERS)

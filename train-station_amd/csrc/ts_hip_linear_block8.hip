@@ -210,6 +210,20 @@ void launch_direct(const Block8Product &p, hipStream_t s) {
     else launch_direct<FN, FM, 1>(p, s);
 }
 
+// The blocks of a wave: one where all of them are no more than the CUs, and of 16 rows at
+// most; else two of rows, and two of columns where K is long and every CU still gets such
+// a tile.  us, 1 x 1, 1 x 2 and 2 x 2 (rows x k x columns): 64 x 4096 x 1024 6.4, 8.6, 11.3; 1000 x
+// 784 x 10 3.0, 4.3, 4.4; 17 x 4096 x 4096 8.6, 7.4, 10.5; 32 x 4096 x 4096 9.8, 8.5, 11.3; 256 x
+// 1024 x 1024 5.8, 5.2, 5.5; 64 x 1024 x 4096 6.5, 5.5, 6.6; 64 x 4096 x 4096 17, 14.2, 12.1; 512 x
+// 4096 x 512 16.8, 13.6, 11.4; 32 x 8192 x 8192 31, 25, 20.
+void launch_direct(const Block8Product &p, hipStream_t s) {
+    const size_t cus = device_cu_count();
+    auto blocks = [&](size_t n) { return (p.M + n - 1) / n * ((p.N + n - 1) / n); };
+    if (p.M <= 16 || blocks(16) <= cus) launch_direct<1, 1>(p, s);
+    else if (p.groups > 8 && blocks(32) >= cus) launch_direct<2, 2>(p, s);
+    else launch_direct<1, 2>(p, s);
+}
+
 constexpr size_t kMaxTileBlocks = size_t(1) << 20;  // more blocks take turns
 
 }  // namespace
@@ -261,8 +275,7 @@ int ts_hip_linear_block8(const uint8_t *x_codes, const float *x_scales, const ui
                              static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0, 0};
     (void)workspace;
     if (block8_tiles_take(batch, fan_out, fan_in)) block8_tiles(p, as_stream(stream));
-    else if (batch <= 16) launch_direct<1, 1>(p, as_stream(stream));
-    else launch_direct<2, 2>(p, as_stream(stream));
+    else launch_direct(p, as_stream(stream));
     return launch_status();
 }
 

@@ -217,15 +217,17 @@ size_t tiles_of(size_t M, size_t N, size_t bm, size_t bn) { return (M + bm - 1) 
 
 }  // namespace
 
-// Where half of the CUs get a tile, of more than the 32 rows and columns of the few rows'
-// kernel's.  us, that one and tiles of 64 x 64 (rows x k x columns): 1999 x 1531 x 777 23.7,
-// 13.1; 1024^3 12.2, 8.6; 4096 x 512 x 512 12.6, 8.2; 64 x 4096 x 16384 35, 17; 48 x 4096 x 8192
-// 18.7, 16.3; 128 x 8192 x 8192 61, 31; 128 x 784 x 4096 7.9, 7.4; 1024 x 512 x 512 6.2, 5.0;
-// 65 x 4096 x 4096 15.8, 15.5; 8192 x 512 x 33 6.4, 4.8.  Below: 512 x 4096 x 512 11.5, 14.9; 256 x
-// 1024 x 1024 6.2, 6.8; 512^3 5.2, 5.4; 64 x 4096 x 4096 12.1, 16; 32 x 4096 x 8192 12.7, 15.7;
-// 65536 x 512 x 32 12.1, 14.1.
+// Where half of the CUs get a tile, and all of them for 17 to 32 rows, which the few rows'
+// kernel reads W once for.  us, that one and tiles of 64 x 64 (rows x k x columns): 1999 x 1531
+// x 777 23.7, 13.1; 1024^3 12.2, 8.6; 4096 x 512 x 512 12.6, 8.2; 64 x 4096 x 16384 35, 17; 48 x
+// 8192 x 8192 34, 27; 40 x 4096 x 8192 18.0, 16.0; 128 x 8192 x 8192 61, 31; 128 x 784 x 4096 7.9,
+// 7.4; 1024 x 512 x 512 6.2, 5.0; 65 x 4096 x 4096 15.8, 15.5; 8192 x 512 x 33 6.4, 4.8; 32 x 4096 x
+// 16384 21, 16; 17 x 4096 x 16384 18.2, 16.7.  Below: 512 x 4096 x 512 11.4, 15.2; 256 x 1024 x 1024
+// 5.2, 6.9; 512^3 4.6, 4.8; 64 x 4096 x 4096 12.1, 15.3; 32 x 8192 x 8192 20, 26; 65536 x 512 x 32
+// 12.1, 14.1.
 bool block8_tiles_take(size_t M, size_t N, size_t K) {
-    return K > 0 && M > 32 && N > 32 && tiles_of(M, N, 64, 64) >= static_cast<size_t>(device_cu_count()) / 2;
+    const size_t cus = device_cu_count();
+    return K > 0 && M > 16 && N > 32 && tiles_of(M, N, 64, 64) >= (M > 32 ? cus / 2 : cus);
 }
 
 // The largest tile that rows and columns fill and of which every CU gets one, or three in
