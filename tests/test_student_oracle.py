@@ -122,7 +122,7 @@ def test_block8_entries_refuse():
     assert hip.ts_hip_block8_scale_rows(129, 0) == 129
 
     def call(batch=4, k=8, n=16, act=0, y=P, xc=P, xs=P, wc=P, ws=P):
-        return hip.ts_hip_linear_block8(xc, xs, wc, ws, batch, k, n, None, act, None, y, None, 1 << 40, None)
+        return hip.ts_hip_linear_block8(xc, xs, wc, ws, batch, k, n, None, act, None, y, None)
 
     assert call(act=9) == EINVAL and call(y=None) == EINVAL and call(xc=None) == EINVAL and call(ws=None) == EINVAL
     assert call(xs=None) == EINVAL and call(wc=None) == EINVAL

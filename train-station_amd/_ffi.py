@@ -196,8 +196,7 @@ HIP_SIGNATURES = {
     "ts_hip_block8_scale_rows": (SZ, [SZ, _c.c_int]),
     "ts_hip_block8": (_c.c_int, [VP, SZ, SZ, _c.c_int, VP, VP, VP]),
     "ts_hip_unblock8": (_c.c_int, [VP, VP, SZ, SZ, _c.c_int, VP, VP]),
-    "ts_hip_linear_block8_workspace_floats": (SZ, [SZ, SZ, SZ]),
-    "ts_hip_linear_block8": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, SZ, VP, _c.c_int, VP, VP, VP, SZ, VP]),
+    "ts_hip_linear_block8": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, SZ, VP, _c.c_int, VP, VP, VP]),
     "ts_hip_layer_norm": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP]),
     "ts_hip_layer_norm_block8": (_c.c_int, [VP, VP, VP, VP, SZ, SZ, _c.c_float, VP, VP, VP, VP]),
     "ts_hip_layer_norm_backward_workspace_floats": (SZ, [SZ, SZ]),

@@ -224,12 +224,10 @@ Tensor Block8::linear(const Block8 &weight, const Tensor *bias, Activation act, 
         throw Error("linear: residual " + dims_str(residual->dims()) + " added to " + dims_str(od));
     Tensor y = Tensor::new_uninit(od);
     if (y.size()) {
-        const size_t ws = ts_hip_linear_block8_workspace_floats(rows_, cols_, weight.rows_);
-        const auto work = workspace(ws);
         const float *bp = data_of(bias), *rp = data_of(residual);
         launch(KernelClass::Gemm, 2.0 * rows_ * cols_ * weight.rows_, "ts_hip_linear_block8", [&] {
             return ts_hip_linear_block8(codes(), scales(), weight.codes(), weight.scales(), rows_, cols_, weight.rows_, bp,
-                                        static_cast<int>(act), rp, y.dev_mut(), work ? work->get() : nullptr, ws, S());
+                                        static_cast<int>(act), rp, y.dev_mut(), S());
         });
     }
     return y;

@@ -259,21 +259,17 @@ int ts_hip_unblock8(const uint8_t *codes, const float *scales, size_t rows, size
     return launch_status();
 }
 
-size_t ts_hip_linear_block8_workspace_floats(size_t, size_t, size_t) { return 0; }
-
 int ts_hip_linear_block8(const uint8_t *x_codes, const float *x_scales, const uint8_t *w_codes, const float *w_scales,
                          size_t batch, size_t fan_in, size_t fan_out, const float *bias, int act, const float *residual,
-                         float *y, float *workspace, size_t workspace_floats, void *stream) {
+                         float *y, void *stream) {
     const size_t lim = size_t(1) << 24;
     if (batch >= lim || fan_in >= lim || fan_out >= lim || batch * fan_out >= size_t(1) << 34 || act < TS_HIP_ACT_NONE ||
         act > TS_HIP_ACT_GELU_TANH)
         return TS_HIP_EINVAL;
     if (batch == 0 || fan_out == 0) return TS_HIP_OK;
     if (!y || (fan_in && (!x_codes || !x_scales || !w_codes || !w_scales))) return TS_HIP_EINVAL;
-    if (workspace_floats < ts_hip_linear_block8_workspace_floats(batch, fan_in, fan_out)) return TS_HIP_EWORKSPACE;
     const Block8Product p = {x_codes, w_codes, x_scales, w_scales, bias, residual, y, static_cast<int>(batch),
                              static_cast<int>(fan_out), static_cast<int>(packed_pitch(fan_in) / kPackGroup), act, 0, 0};
-    (void)workspace;
     if (block8_tiles_take(batch, fan_out, fan_in)) block8_tiles(p, as_stream(stream));
     else launch_direct(p, as_stream(stream));
     return launch_status();
