@@ -234,7 +234,8 @@ def test_layer_norm(rows, cols, residual, bias):
 
 
 @pytest.mark.parametrize("rows,cols", [(600, 8192), (600, 8200), (300, 16383), (1100, 4100), (1500, 1030), (300, 16390), (70, 40001),
-                                       (2100, 255), (2101, 510), (2102, 1021), (1025, 2047)])
+                                       (2100, 255), (2101, 510), (2102, 1021), (1025, 2047),
+                                       (9000, 128), (5001, 60), (4099, 127), (3001, 5), (2, 3)])
 def test_layer_norm_sums_many_rows(rows, cols):
     check_layer_norm(rows, cols, True, True)
 

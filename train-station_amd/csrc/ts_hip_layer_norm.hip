@@ -54,8 +54,17 @@ __device__ __forceinline__ void fill_past(float (&v)[4], size_t c, size_t cols, 
         if (c + e >= cols) v[e] = first;
 }
 
-// The sum over the W waves of a row, in every lane, joined within a wave by DPP.  lds: N * W
-// doubles of this row, others than the last row's (a barrier stands between the two).
+// A row has W waves, or half a wave (W 0): its lanes, the rows of a wave and of a workgroup.
+// us, 16384 x 64 by half waves and by waves: forward 8.6, 13; backward 10.5, 15.
+template <int W>
+constexpr int kRowLanes = W ? 64 * W : 32;
+template <int W>
+constexpr int kWaveRows = W ? 1 : 2;
+template <int W>
+constexpr int kLayerRows = kNormThreads<W> / kRowLanes<W>;
+
+// The sum over a row's lanes, in every one, joined within a wave by DPP.  lds: N * W doubles
+// of this row, others than the last row's (a barrier stands between the two).
 constexpr int kBcast15 = 0x142, kBcast31 = 0x143;
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_or_0(double v) {  // 0 in the other rows of 16
@@ -71,54 +80,80 @@ __device__ __forceinline__ void row_sums(double (&s)[N], double *lds) {
         v += dpp<0x4E>(v);   // lanes 2 3 0 1
         v += dpp<0x141>(v);  // eight lanes mirrored
         v += dpp<0x140>(v);  // sixteen lanes mirrored
+        if (W == 0) {  // the neighbouring row of 16: one copy ends with the even rows, the other with the odd
+            const auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+            const auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+            s[n] = __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+            continue;
+        }
         v += dpp_or_0<kBcast15, 0xa>(v);
         v += dpp_or_0<kBcast31, 0xc>(v);  // lane 63: all
         s[n] = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
     }
-    if (W == 1) return;
-    const int wave = (threadIdx.x >> 6) % W;
-    if ((threadIdx.x & 63) == 0) {
+    if constexpr (W > 1) {
+        const int wave = (threadIdx.x >> 6) % W;
+        if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) lds[n * W + wave] = s[n];
-    }
-    __syncthreads();
+            for (int n = 0; n < N; ++n) lds[n * W + wave] = s[n];
+        }
+        __syncthreads();
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        s[n] = 0.0;
+        for (int n = 0; n < N; ++n) {
+            s[n] = 0.0;
 #pragma unroll
-        for (int w = 0; w < W; ++w) s[n] += lds[n * W + w];
+            for (int w = 0; w < W; ++w) s[n] += lds[n * W + w];
+        }
     }
 }
 
-// A lane's quads c = 4 (t + 64 W i) of rows of `cols` columns, by the buffer instructions,
+// The rows that a wave has of a round's from r0 on: the first of them and how many there are
+// (uniform), the lane's own.
+template <int W>
+struct WaveRows {
+    size_t first, row;
+    unsigned there;
+    bool live;
+    __device__ __forceinline__ WaveRows(size_t r0, int wave_row, int slot, size_t rows) : first(r0 + wave_row), row(r0 + slot) {
+        there = first < rows ? static_cast<unsigned>(min(rows - first, static_cast<size_t>(kWaveRows<W>))) : 0;
+        live = row < rows;
+        if (!there) first = 0;
+    }
+    __device__ __forceinline__ size_t at(size_t cols) const { return W || !live ? first * cols : row * cols; }  // (a row that exists)
+};
+
+// A lane's quads c = 4 (t + lanes i) of rows of `cols` columns, by the buffer instructions,
 // for which a lane past the row is one past the buffer: 0 comes back, nothing is written.
 // The quad that a row ends in is read from the row's last four columns and moved into place.
 template <int W, int NV>
 struct RowQuads {
     unsigned t, cols;
     int wave, parts;  // the wave's place in the row, the row's parts of 256 columns
+    unsigned skip;    // bytes from the wave's first row to the lane's
+    static constexpr int L = kRowLanes<W>;
     __device__ __forceinline__ RowQuads(unsigned t, size_t cols)
-        : t(t), cols(static_cast<unsigned>(cols)), wave(__builtin_amdgcn_readfirstlane(t / 64)), parts(static_cast<int>((cols + 255) / 256)) {}
-    __device__ __forceinline__ unsigned col(int i) const { return 4 * (t + 64 * W * i); }
+        : t(t), cols(static_cast<unsigned>(cols)), wave(__builtin_amdgcn_readfirstlane(t / 64)), parts(static_cast<int>((cols + 255) / 256)),
+          skip(W ? 0 : threadIdx.x % 64 / L * 4 * static_cast<unsigned>(cols)) {}
+    __device__ __forceinline__ unsigned col(int i) const { return 4 * (t + L * i); }
     // whether any lane of the wave has columns of quad i (uniform): what is past the row is not
     // computed (backward, us: 3400 x 4100 46, 51 with it computed; 1700 x 8200 53, 67)
     __device__ __forceinline__ bool some(int i) const { return i == 0 || W * i + wave < parts; }
-    __device__ __forceinline__ __amdgpu_buffer_rsrc_t row(const float *p, bool there) const {  // p, there: uniform
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, there ? static_cast<int>(4 * cols) : 0, 0x00020000);
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const float *p, unsigned rows) const {  // p, rows: uniform
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, static_cast<int>(4 * cols * rows), 0x00020000);
     }
-    __device__ __forceinline__ void load(const float *p, bool there, float (&v)[NV][4]) const {
-        const __amdgpu_buffer_rsrc_t r = row(p, there);
-        if (W * NV == 1 && cols < 4) {  // uniform
+    // the lane's quads of the row at p, or of its own of the rows there (by: its skip)
+    __device__ __forceinline__ void load(const float *p, unsigned rows, float (&v)[NV][4], unsigned by = 0) const {
+        const __amdgpu_buffer_rsrc_t r = buffer(p, rows);
+        if (W == 0 && cols < 4) {  // uniform
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    v[i][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * (col(i) + e), 0, 0));
+                    v[i][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, col(i) + e < cols ? by + 4 * (col(i) + e) : kPast, 0, 0));
             return;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const unsigned off = col(i) < cols ? 4 * min(col(i), cols - 4) : kPast;
+            const unsigned off = col(i) < cols ? by + 4 * min(col(i), cols - 4) : kPast;
             const f4v_t q = __builtin_bit_cast(f4v_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i][e] = q[e];
@@ -126,7 +161,7 @@ struct RowQuads {
     }
     // what was loaded into place, and `past` in the columns past the row
     __device__ __forceinline__ void fill(float (&v)[NV][4], float past) const {
-        if (cols == 256 * W * NV) return;  // uniform
+        if (cols == 4 * L * NV) return;  // uniform
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const unsigned c = col(i);
@@ -143,16 +178,16 @@ struct RowQuads {
             for (int e = 0; e < 4; ++e) v[i][e] = c + e < cols ? v[i][e] : past;
         }
     }
-    // quad i of the row at p
-    __device__ __forceinline__ void store(float *p, int i, const float (&v)[4]) const {
+    // quad i of the lane's row, of the rows at p (a lane whose row is not there does not call)
+    __device__ __forceinline__ void store(float *p, unsigned rows, int i, const float (&v)[4]) const {
         typedef unsigned u4 __attribute__((ext_vector_type(4)));
-        const unsigned c = col(i), off = c + 4 <= cols ? 4 * c : kPast;
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f4v_t{v[0], v[1], v[2], v[3]}), row(p, true), off, 0, 0);
+        const unsigned c = col(i), off = c + 4 <= cols ? skip + 4 * c : kPast;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f4v_t{v[0], v[1], v[2], v[3]}), buffer(p, rows), off, 0, 0);
         if (cols & 3) {  // uniform
             if (c < cols && c + 4 > cols) {
 #pragma unroll
                 for (int e = 0; e < 3; ++e)
-                    if (c + e < cols) p[c + e] = v[e];
+                    if (c + e < cols) p[skip / 4 + c + e] = v[e];
             }
         }
     }
@@ -195,31 +230,31 @@ struct RowOut {
     }
 };
 
-// A row per W waves, and on by the grid's where there are more rows than workgroups.
+// A row per W waves (or half a wave), and on by the grid's where there are more rows than workgroups.
 template <int W, int NV, bool RES, bool PACK>
 __global__ __launch_bounds__(kNormThreads<W>, 4) void layer_norm_rows(LayerNormArgs a) {
-    constexpr int RPB = kNormRows<W>;
-    __shared__ double lds[RPB * 2 * 2 * W];
-    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / W, t = threadIdx.x % (64 * W);
+    constexpr int RPB = kLayerRows<W>, L = kRowLanes<W>;
+    __shared__ double lds[W > 1 ? RPB * 2 * 2 * W : 1];
+    const int wave_row = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64 / L, t = threadIdx.x % L;
+    const int slot = W ? wave_row : threadIdx.x / L;
     const RowQuads<W, NV> at(t, a.cols);
     float w[NV][4], b[NV][4];
-    at.load(a.weight, true, w);
-    at.load(a.bias, a.bias != nullptr, b);
+    at.load(a.weight, 1, w);
+    at.load(a.bias, a.bias ? 1 : 0, b);
     at.fill(w, 0.0f);
     at.fill(b, 0.0f);
     const size_t step = static_cast<size_t>(gridDim.x) * RPB;
     int turn = 0;
     // every wave of the workgroup takes every round (the barriers)
     for (size_t r0 = static_cast<size_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += step) {
-        const size_t row = r0 + slot;
-        const bool live = row < a.rows;
-        const size_t base = live ? row * a.cols : 0;
-        float v[NV][4], first = a.x[base];
-        at.load(a.x + base, live, v);
+        const WaveRows<W> rows(r0, wave_row, slot, a.rows);
+        const size_t base = rows.first * a.cols, own = rows.at(a.cols);
+        float v[NV][4], first = a.x[own];
+        at.load(a.x + base, rows.there, v, at.skip);
         if constexpr (RES) {
             float r[NV][4];
-            at.load(a.residual + base, live, r);
-            first += a.residual[base];
+            at.load(a.residual + base, rows.there, r, at.skip);
+            first += a.residual[own];
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -229,13 +264,13 @@ __global__ __launch_bounds__(kNormThreads<W>, 4) void layer_norm_rows(LayerNormA
         double s[2] = {0.0, 0.0};
 #pragma unroll
         for (int i = 0; i < NV; ++i) norm_sums(v[i], first, s);
-        row_sums<W, 2>(s, lds + (slot * 2 + turn) * 2 * W);
+        row_sums<W, 2>(s, W > 1 ? lds + (slot * 2 + turn) * 2 * W : lds);
         turn ^= 1;
-        if (!live) continue;  // (uniform in a wave, past the round's barrier)
+        if (!rows.live) continue;  // (uniform in a wave, past the round's barrier)
         const RowOut out(s, a.per_col, first, a.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (RES) at.store(a.h + base, i, v[i]);
+            if (RES) at.store(a.h + base, rows.there, i, v[i]);
             if constexpr (PACK) {
                 const size_t c = at.col(i);
                 if (c >= a.pitch) continue;  // (whole blocks)
@@ -245,12 +280,12 @@ __global__ __launch_bounds__(kNormThreads<W>, 4) void layer_norm_rows(LayerNormA
                 double o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = c + e < a.cols ? out.wide_y(v[i][e], w[i][e], b[i][e]) : 0.0;
-                block8_store(o, c, a.codes + row * a.pitch, a.scales + row, a.rows);
+                block8_store(o, c, a.codes + rows.row * a.pitch, a.scales + rows.row, a.rows);
             } else {
                 float o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = out.y(v[i][e], w[i][e], b[i][e]);
-                at.store(a.y + base, i, o);
+                at.store(a.y + base, rows.there, i, o);
             }
         }
     }
@@ -361,16 +396,17 @@ struct BackRow {
 // workgroup's go to the parts.
 template <int W, int NV, bool DH, bool DP>
 __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_back(LayerNormBackArgs a) {
-    constexpr int RPB = kNormRows<W>;
-    __shared__ double lds[RPB * 2 * 4 * W];
-    const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) / W, t = threadIdx.x % (64 * W);
+    constexpr int RPB = kLayerRows<W>, L = kRowLanes<W>;
+    __shared__ double lds[W > 1 ? RPB * 2 * 4 * W : 1];
+    const int wave_row = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64 / L, t = threadIdx.x % L;
+    const int slot = W ? wave_row : threadIdx.x / L;
     // dw's sums stand in registers; where 16 waves of four quads leave none, in shared
     // memory, each thread its own, and db's alone in registers
     constexpr bool SHARED = DP && W * NV >= 64;
-    __shared__ double held[SHARED ? NV * 4 * 64 * W : 1];
+    __shared__ double held[SHARED ? NV * 4 * L : 1];
     double own[SHARED ? 1 : NV][4] = {}, db[NV][4] = {};
     auto dw = [&](int i, int e) -> double & {
-        if constexpr (SHARED) return held[(i * 4 + e) * 64 * W + t];
+        if constexpr (SHARED) return held[(i * 4 + e) * L + t];
         else return own[i][e];
     };
     if constexpr (SHARED) {
@@ -380,27 +416,27 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
     const RowQuads<W, NV> at(t, a.cols);
     constexpr bool AHEAD = W * NV < 64;  // (there no registers are left for the next row)
     float w[NV][4];
-    at.load(a.weight, true, w);
+    at.load(a.weight, 1, w);
     at.fill(w, 0.0f);
     const size_t step = static_cast<size_t>(gridDim.x) * RPB;
-    auto fetch = [&](size_t row, BackRow<NV> &v) {  // a row past the last: zeros
-        const bool live = row < a.rows;
-        const size_t base = live ? row * a.cols : 0;
-        v.first = a.h[base];
-        at.load(a.h + base, live, v.h);
-        at.load(a.go + base, live, v.g);
+    auto fetch = [&](size_t r0, BackRow<NV> &v) {  // a row past the last: zeros
+        const WaveRows<W> rows(r0, wave_row, slot, a.rows);
+        const size_t base = rows.first * a.cols;
+        v.first = a.h[rows.at(a.cols)];
+        at.load(a.h + base, rows.there, v.h, at.skip);
+        at.load(a.go + base, rows.there, v.g, at.skip);
     };
     BackRow<NV> v, next;
-    if (AHEAD) fetch(static_cast<size_t>(blockIdx.x) * RPB + slot, next);
+    if (AHEAD) fetch(static_cast<size_t>(blockIdx.x) * RPB, next);
     int turn = 0;
     // every wave of the workgroup takes every round (the barriers)
     for (size_t r0 = static_cast<size_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += step) {
-        const size_t row = r0 + slot;
+        const WaveRows<W> rows(r0, wave_row, slot, a.rows);
         if constexpr (AHEAD) {
             v = next;
-            if (r0 + step < a.rows) fetch(row + step, next);
+            if (r0 + step < a.rows) fetch(r0 + step, next);
         } else {
-            fetch(row, v);
+            fetch(r0, v);
         }
         at.fill(v.h, v.first);
         at.fill(v.g, 0.0f);
@@ -415,9 +451,9 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
             }
             back_sums(v.h[i], v.g[i], w[i], shift, s);
         }
-        row_sums<W, 4>(s, lds + (slot * 2 + turn) * 4 * W);
+        row_sums<W, 4>(s, W > 1 ? lds + (slot * 2 + turn) * 4 * W : lds);
         turn ^= 1;
-        if (row >= a.rows) continue;  // (uniform in a wave, past the round's barrier)
+        if (!rows.live) continue;  // (uniform in a wave, past the round's barrier)
         const RowBack back = row_back(s, a.per_col, shift, a.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -434,20 +470,20 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
                     db[i][e] += go;
                 }
             }
-            if (DH) at.store(a.dh + row * a.cols, i, o);
+            if (DH) at.store(a.dh + rows.first * a.cols, rows.there, i, o);
             if (SHARED) asm volatile("" ::: "memory");  // (or every quad's sums of dw are read first)
         }
     }
     if constexpr (!DP) return;
     if constexpr (RPB > 1) {  // the workgroup's rows together, in their order
-        __shared__ double sum[(RPB - 1) * 64 * W * NV * 4];
+        __shared__ double sum[(RPB - 1) * L * NV * 4];
         auto join = [&](double (&v)[NV][4]) {
             __syncthreads();
             if (slot > 0) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * 64 * W + t] = v[i][e];
+                    for (int e = 0; e < 4; ++e) sum[((slot - 1) * NV * 4 + i * 4 + e) * L + t] = v[i][e];
             }
             __syncthreads();
             if (slot == 0) {
@@ -456,7 +492,7 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
 #pragma unroll
                     for (int i = 0; i < NV; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[i][e] += sum[(k * NV * 4 + i * 4 + e) * 64 * W + t];
+                        for (int e = 0; e < 4; ++e) v[i][e] += sum[(k * NV * 4 + i * 4 + e) * L + t];
             }
         };
         join(own);
@@ -470,7 +506,7 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
             part += static_cast<size_t>(blockIdx.x) * a.cols;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const size_t c = 4 * (t + 64 * W * i);
+                const size_t c = at.col(i);
                 if (a.ticket) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -625,7 +661,7 @@ void launch_layer_norm(const LayerNormArgs &a, hipStream_t s) {
     // a row each; of 16 waves as many workgroups as run at once, which keep the weights.  us, a
     // row each and as many as run at once: 8192 x 4096 89, 96, packed 82, 86; 4096 x 8192 98,
     // 97; 2048 x 16384 113, 100
-    const size_t need = (a.rows + kNormRows<W> - 1) / kNormRows<W>, cap = W == 16 ? device_cu_count() : kMaxBlocks;
+    const size_t need = (a.rows + kLayerRows<W> - 1) / kLayerRows<W>, cap = W == 16 ? device_cu_count() : kMaxBlocks;
     const dim3 grid(static_cast<unsigned>(need < cap ? need : cap)), block(kNormThreads<W>);
     if constexpr (LONG) launch((long_layer_norm<RES, PACK>), grid, block, 0, s, a);
     else launch((layer_norm_rows<W, NV, RES, PACK>), grid, block, 0, s, a);
@@ -652,19 +688,26 @@ void launch_layer_back(const LayerNormBackArgs &a, unsigned grid, hipStream_t s)
     }
 }
 
-// The backward pass's for_cols: for rows of 1025 to 2048 two waves of four quads in place of
-// four of two, since what a wave does for its row beside its quads is as much as a quad
-// and a half.  us: 13000 x 1100 41, 58; 7000 x 2048 32, 33.
+// for_cols, with half a wave for rows of 128 at most
+template <class F>
+void for_layer_cols(size_t n, F &&f) {
+    using std::integral_constant;
+    if (n <= 128) f(integral_constant<int, 0>{}, integral_constant<int, 1>{}, integral_constant<bool, false>{});
+    else for_cols<false>(n, false, f);
+}
+// The backward pass's: for rows of 1025 to 2048 two waves of four quads in place of four of
+// two, since what a wave does for its row beside its quads is as much as a quad and a
+// half.  us: 13000 x 1100 41, 58; 7000 x 2048 32, 33.
 template <class F>
 void for_back_cols(size_t n, F &&f) {
     using std::integral_constant;
     if (n > 1024 && n <= 2048) f(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
-    else for_cols<false>(n, false, [&](auto w, auto nv, auto lng) {
+    else for_layer_cols(n, [&](auto w, auto nv, auto lng) {
         if constexpr (!(w.value == 4 && nv.value == 2)) f(w, nv, lng);
     });
 }
-size_t layer_back_blocks(size_t rows, size_t cols) {
-    return cols > 1024 && cols <= 2048 ? back_blocks((rows + 1) / 2, cols) : back_blocks(rows, cols);  // (two rows a workgroup)
+size_t layer_back_blocks(size_t rows, size_t cols) {  // (twice back_blocks's rows a workgroup there)
+    return cols <= 128 || (cols > 1024 && cols <= 2048) ? back_blocks((rows + 1) / 2, cols) : back_blocks(rows, cols);
 }
 
 int layer_norm_forward(const float *x, const float *residual, const float *weight, const float *bias, size_t rows, size_t cols,
@@ -672,7 +715,7 @@ int layer_norm_forward(const float *x, const float *residual, const float *weigh
     if (rows == 0 || cols == 0) return TS_HIP_OK;
     if (!x || !weight || (residual != nullptr) != (h != nullptr) || rows >= kMaxRows) return TS_HIP_EINVAL;
     const LayerNormArgs a = {x, residual, weight, bias, h, y, codes, scales, rows, cols, packed_pitch(cols), eps, 1.0 / static_cast<double>(cols)};
-    for_cols<false>(codes ? a.pitch : cols, false, [&](auto w, auto nv, auto long_rows) {
+    for_layer_cols(codes ? a.pitch : cols, [&](auto w, auto nv, auto long_rows) {
         launch_layer_norm<w.value, nv.value, long_rows.value>(a, as_stream(stream));
     });
     return launch_status();
