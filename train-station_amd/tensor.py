@@ -284,7 +284,7 @@ class Tensor:
         return y, Tensor(h.value)
 
     def layer_norm_block8(self, weight: "Tensor", bias: Optional["Tensor"] = None, eps: float = 1e-5) -> "Block8":
-        """layer_norm of a matrix, in 8 bits."""
+        """layer_norm of a matrix, in 8 bits; no gradient passes through them."""
         return _wrap_block8(_G.ts_tensor_layer_norm_block8(self._h, None, weight._h, _optional(bias), eps, None))
 
     def add_layer_norm_block8(self, residual: "Tensor", weight: "Tensor", bias: Optional["Tensor"] = None,
@@ -574,7 +574,8 @@ class Block8:
 
     def linear(self, weight: "Block8", bias: Optional[Tensor] = None, activation: str = "none",
                residual: Optional[Tensor] = None) -> Tensor:
-        """act(self weight^T + bias) + residual, weight [fan_out, fan_in] in tiles."""
+        """act(self weight^T + bias) + residual, weight [fan_out, fan_in] in tiles; no
+        gradient passes through it."""
         return _wrap(_G.ts_block8_linear(self._h, weight._h, _optional(bias), _activation(activation),
                                          _optional(residual)))
 
