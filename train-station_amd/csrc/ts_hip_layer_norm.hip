@@ -395,14 +395,14 @@ struct BackRow {
 // while one is computed; a thread keeps the sums of its columns for dw and db (f64), the
 // workgroup's go to the parts.
 template <int W, int NV, bool DH, bool DP>
-__global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_back(LayerNormBackArgs a) {
+__global__ __launch_bounds__(kNormThreads<W>, 2) void layer_norm_back(LayerNormBackArgs a) {
     constexpr int RPB = kLayerRows<W>, L = kRowLanes<W>;
     __shared__ double lds[W > 1 ? RPB * 2 * 4 * W : 1];
     const int wave_row = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 64 / L, t = threadIdx.x % L;
     const int slot = W ? wave_row : threadIdx.x / L;
-    // dw's sums stand in registers; where 16 waves of four quads leave none, in shared
-    // memory, each thread its own, and db's alone in registers
-    constexpr bool SHARED = DP && W * NV >= 64;
+    // dw's sums stand in registers; where eight quads a lane leave none, in shared memory,
+    // each thread its own, and db's alone in registers
+    constexpr bool SHARED = DP && NV == 8;
     __shared__ double held[SHARED ? NV * 4 * L : 1];
     double own[SHARED ? 1 : NV][4] = {}, db[NV][4] = {};
     auto dw = [&](int i, int e) -> double & {
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
         for (int i = 0; i < 4 * NV; ++i) dw(i / 4, i % 4) = 0.0;
     }
     const RowQuads<W, NV> at(t, a.cols);
-    constexpr bool AHEAD = W * NV < 64;  // (there no registers are left for the next row)
+    constexpr bool AHEAD = NV < 8;  // (there no registers are left for the next row)
     float w[NV][4];
     at.load(a.weight, 1, w);
     at.fill(w, 0.0f);
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(kNormThreads<W>, W == 16 ? 4 : 2) void layer_norm_b
                 const size_t c = column(second ? q - count : q);
                 const float *part = (second ? a.db_part : a.dw_part);
                 if (!part) continue;
-                constexpr int n = sizeof(Value) / 4, batch = W == 16 ? 8 : 32;
+                constexpr int n = sizeof(Value) / 4, batch = 32;
                 double s[n] = {};
                 for (unsigned g0 = 0; g0 < gridDim.x; g0 += batch) {
                     float v[batch][n];
@@ -697,13 +697,16 @@ void for_layer_cols(size_t n, F &&f) {
 }
 // The backward pass's: for rows of 1025 to 2048 two waves of four quads in place of four of
 // two, since what a wave does for its row beside its quads is as much as a quad and a
-// half.  us: 13000 x 1100 41, 58; 7000 x 2048 32, 33.
+// half.  us: 13000 x 1100 41, 58; 7000 x 2048 32, 33.  For longer ones than 8192 eight waves
+// of eight quads in place of 16 of four, with twice the registers: 2048 x 16384 105, 124; 1200
+// x 12000 51, 56; 1700 x 8200 53, 53.
 template <class F>
 void for_back_cols(size_t n, F &&f) {
     using std::integral_constant;
     if (n > 1024 && n <= 2048) f(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<bool, false>{});
+    else if (n > 8192 && n <= kMaxHeldCols) f(integral_constant<int, 8>{}, integral_constant<int, 8>{}, integral_constant<bool, false>{});
     else for_layer_cols(n, [&](auto w, auto nv, auto lng) {
-        if constexpr (!(w.value == 4 && nv.value == 2)) f(w, nv, lng);
+        if constexpr (!(w.value == 4 && nv.value == 2) && !(w.value == 16 && nv.value == 4 && !lng.value)) f(w, nv, lng);
     });
 }
 size_t layer_back_blocks(size_t rows, size_t cols) {  // (twice back_blocks's rows a workgroup there)
